@@ -577,6 +577,61 @@ int nq_e8_stream_codes(const float* quantized, const float* scales, int64_t n_gr
 int nq_e8_stream_values(const int8_t* codes, const uint16_t* scales_f16, int64_t n_groups, int64_t n_scales,
                         float* out, void* stream);
 
+/*
+ * A pool of equally sized compressed pages: per layer and page the codes and
+ * scales of a page (nq_page_desc layout), and one position a token for all
+ * layers.  Codes and scales 16-byte aligned.  The host keeps which pages are
+ * in use (nexusquant_amd/page_pool.py).
+ */
+typedef struct nq_pool {
+    int32_t layers, pages, heads, tokens, head_dim; /* head_dim 64, 128 or 256 */
+    int32_t reserved;
+    int8_t* key_codes;    /* [layers, pages, heads, tokens, head_dim] */
+    int8_t* value_codes;
+    void* key_scales;     /* fp16 [layers, pages, heads, tokens] */
+    void* value_scales;
+    int32_t* positions;   /* [pages, tokens] */
+} nq_pool;
+
+/*
+ * Pages dst[i] become copies of pages src[i] in every layer, positions too.
+ * src and dst are HOST arrays of n page numbers, read during the call.  A
+ * page may be read any number of times, is written at most once, and is not
+ * both read and written (NQ_EINVAL).
+ */
+int nq_pool_copy_pages(const nq_pool* pool, const int32_t* src, const int32_t* dst, int32_t n, void* stream);
+
+/*
+ * Kept tokens of sequences into fewer pages, in every layer: token j of
+ * sequence b's new pages is token kept[b * kept_stride + j] of its old ones,
+ * for j below its count; positions move along, or are j (renumber != 0: keys
+ * are stored without rotation, so their rotation follows).  Slots past the
+ * count keep what they hold.  New pages are none of the old ones.
+ *   tile_seq [n_tiles]   the sequence of each run of nq_pool_move_tokens()
+ *                        new tokens (a sequence's runs are consecutive);
+ *   seq      [n_seq * 5] per sequence its first tile, tokens kept, tokens it
+ *                        had, and where its old and new page numbers start in
+ *   tables               (page numbers);
+ *   kept                 positions in the sequence, as nq_keep_mask lists
+ *                        them (entries outside the sequence are clamped).
+ * All device int32 arrays.
+ */
+int32_t nq_pool_move_tokens(void);
+int nq_pool_compact(const nq_pool* pool, const int32_t* tile_seq, int32_t n_tiles, const int32_t* seq,
+                    const int32_t* tables, const int32_t* kept, int32_t kept_stride, int32_t renumber, void* stream);
+
+/*
+ * Encoded tokens to their slots in one layer: `tokens` is one page of n
+ * tokens (nq_page_encode's output and the tokens' positions); token i goes to
+ * slot slots[i] = page * pool tokens + offset (device int32 array).  Negative
+ * slots and slots past the pool are skipped; slots must be distinct.
+ *
+ * Replaces: NexusQuantPagedAttention.compress_and_cache   vllm_backend.py:622-688
+ *           (the cache side, for pages of a pool)
+ */
+int nq_pool_write(const nq_pool* pool, int32_t layer, const nq_pool* tokens, const int32_t* slots, int32_t n,
+                  void* stream);
+
 /* Library version and the last error message of the calling thread. */
 int nq_abi_version(void);
 const char* nq_last_error(void);

@@ -88,6 +88,15 @@ class AttnDesc(ctypes.Structure):
     ]
 
 
+class Pool(ctypes.Structure):
+    """Mirror of nq_pool in include/nexusquant_amd.h."""
+    _fields_ = [
+        ("layers", ctypes.c_int32), ("pages", ctypes.c_int32), ("heads", ctypes.c_int32),
+        ("tokens", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("key_codes", _P), ("value_codes", _P), ("key_scales", _P), ("value_scales", _P), ("positions", _P),
+    ]
+
+
 # Every exported symbol, with (argtypes, restype).  tests/test_abi.py checks
 # that this list and include/nexusquant_amd.h agree and that the library
 # exports all of them.
@@ -129,6 +138,10 @@ SIGNATURES = {
     "nq_paged_attention": ([ctypes.POINTER(AttnDesc), _P], ctypes.c_int),
     "nq_nibble_pack": ([_P, _I64, _I32, _P, _P], ctypes.c_int),
     "nq_nibble_unpack": ([_P, _I64, _I32, _I32, _P, _P], ctypes.c_int),
+    "nq_pool_copy_pages": ([ctypes.POINTER(Pool), _P, _P, _I32, _P], ctypes.c_int),
+    "nq_pool_move_tokens": ([], ctypes.c_int32),
+    "nq_pool_compact": ([ctypes.POINTER(Pool), _P, _I32, _P, _P, _P, _I32, _I32, _P], ctypes.c_int),
+    "nq_pool_write": ([ctypes.POINTER(Pool), _I32, ctypes.POINTER(Pool), _P, _I32, _P], ctypes.c_int),
     "nq_e8_dequant_matmul": ([_P, _P, _P, _P, _I64, _I32, _I32, _I32, _P], ctypes.c_int),
     "nq_e8_nearest_point": ([_P, _P, _I64, _P], ctypes.c_int),
     "nq_e8_quantize_perhead": ([_P, _P, _I64, _I32, _I32, _P], ctypes.c_int),
