@@ -578,6 +578,35 @@ int nq_e8_stream_values(const int8_t* codes, const uint16_t* scales_f16, int64_t
                         float* out, void* stream);
 
 /*
+ * Causal attention over packed prompts: q [rows, q_heads, head_dim], k and v
+ * [rows, kv_heads, head_dim], sequences one after another along the rows.
+ * Query i of a sequence sees its keys j with i - sliding_window < j <= i (all
+ * j <= i for sliding_window 0): out = softmax(scale * q . k) . v, query head h
+ * reading kv head h / (q_heads / kv_heads).  fp16 or bf16; softmax in fp32,
+ * its weights rounded to the type for the second product.
+ * tiles: device int32 [n_tiles, 4], the nq_prompt_tile_rows() queries of each
+ * tile as {first row of its sequence, the sequence's length, the tile's first
+ * query in it, 0}; rows in no tile are neither read nor written.
+ */
+typedef struct nq_prompt_desc {
+    int32_t q_heads, kv_heads, head_dim;  /* head_dim 64, 128 or 256 */
+    int32_t dtype;                        /* NQ_F16 / NQ_BF16 */
+    int32_t n_tiles;
+    int32_t sliding_window;
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    const int32_t* tiles;
+    int64_t q_stride[2], k_stride[2], v_stride[2], out_stride[2]; /* of a row and of a head, elements */
+    float scale;
+    float reserved_f;
+} nq_prompt_desc;
+
+int32_t nq_prompt_tile_rows(void);
+int nq_prompt_attention(const nq_prompt_desc* desc, void* stream);
+
+/*
  * A pool of equally sized compressed pages: per layer and page the codes and
  * scales of a page (nq_page_desc layout), and one position a token for all
  * layers.  Codes and scales 16-byte aligned.  The host keeps which pages are

@@ -88,6 +88,18 @@ class AttnDesc(ctypes.Structure):
     ]
 
 
+class PromptDesc(ctypes.Structure):
+    """Mirror of nq_prompt_desc in include/nexusquant_amd.h."""
+    _fields_ = [
+        ("q_heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("n_tiles", ctypes.c_int32), ("sliding_window", ctypes.c_int32),
+        ("q", _P), ("k", _P), ("v", _P), ("out", _P), ("tiles", _P),
+        ("q_stride", ctypes.c_int64 * 2), ("k_stride", ctypes.c_int64 * 2), ("v_stride", ctypes.c_int64 * 2),
+        ("out_stride", ctypes.c_int64 * 2),
+        ("scale", ctypes.c_float), ("reserved_f", ctypes.c_float),
+    ]
+
+
 class Pool(ctypes.Structure):
     """Mirror of nq_pool in include/nexusquant_amd.h."""
     _fields_ = [
@@ -138,6 +150,8 @@ SIGNATURES = {
     "nq_paged_attention": ([ctypes.POINTER(AttnDesc), _P], ctypes.c_int),
     "nq_nibble_pack": ([_P, _I64, _I32, _P, _P], ctypes.c_int),
     "nq_nibble_unpack": ([_P, _I64, _I32, _I32, _P, _P], ctypes.c_int),
+    "nq_prompt_tile_rows": ([], ctypes.c_int32),
+    "nq_prompt_attention": ([ctypes.POINTER(PromptDesc), _P], ctypes.c_int),
     "nq_pool_copy_pages": ([ctypes.POINTER(Pool), _P, _P, _I32, _P], ctypes.c_int),
     "nq_pool_move_tokens": ([], ctypes.c_int32),
     "nq_pool_compact": ([ctypes.POINTER(Pool), _P, _I32, _P, _P, _P, _I32, _I32, _P], ctypes.c_int),

@@ -1,0 +1,124 @@
+"""Causal attention over packed prompts (nq_prompt_attention): the prefill's attention of a
+serving batch, before its keys and values are compressed into pages.
+
+scoring.attention_real is the padded form with transformers' eager roundings (and the column
+sums of the scorer); here the softmax stays in fp32 and sequences of different lengths stand
+one after another without padding.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import dataclasses
+from typing import Optional, Sequence
+
+import numpy as np
+import torch
+
+from . import _lib
+from .ops import _addr
+
+_HEAD_DIMS = (64, 128, 256)
+
+
+@dataclasses.dataclass(frozen=True)
+class PromptPlan:
+    """Which rows are whose: made once for a batch's lengths, used by every layer."""
+    lengths: tuple
+    rows: int                     # of all sequences
+    n_tiles: int
+    tiles: Optional[torch.Tensor]  # int32 [n_tiles, 4] on the device
+
+
+def prompt_tiles(lengths: Sequence[int], tile_rows: int) -> np.ndarray:
+    """int32 [n_tiles, 4]: first row, length and first query of each tile, the ones that see most keys first."""
+    n = np.asarray(lengths, dtype=np.int64).reshape(-1)
+    count = -(-n // tile_rows)
+    seq = np.repeat(np.arange(len(n)), count)
+    q0 = (np.arange(len(seq)) - np.repeat(np.cumsum(count) - count, count)) * tile_rows
+    tiles = np.stack([(np.cumsum(n) - n)[seq], n[seq], q0, np.zeros_like(q0)], axis=1)
+    return tiles[np.argsort(-q0, kind="stable")].astype(np.int32)
+
+
+def plan_prompts(lengths: Sequence[int], device=None) -> PromptPlan:
+    """The plan of sequences of `lengths` tokens (0 is allowed), one after another in this order."""
+    lens = tuple(int(x) for x in (lengths.tolist() if torch.is_tensor(lengths) else lengths))
+    if any(x < 0 for x in lens):
+        raise ValueError(f"lengths must not be negative, got {min(lens)}")
+    rows = sum(lens)
+    if rows >= 1 << 31:
+        raise ValueError(f"{rows} rows: a batch takes less than 2^31")
+    dev = torch.device("cuda" if device is None else device)
+    if dev.type != "cuda":
+        raise _lib.NexusQuantError(f"nexusquant_amd runs on MI355X (ROCm) devices only; the plan is for {dev}")
+    tiles = prompt_tiles(lens, int(_lib.load().nq_prompt_tile_rows()))
+    return PromptPlan(lengths=lens, rows=rows, n_tiles=len(tiles),
+                      tiles=torch.from_numpy(tiles).to(dev) if len(tiles) else None)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t with contiguous, 16-byte aligned head vectors (itself when they are)."""
+    if t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, plan: PromptPlan,
+                     scale: Optional[float] = None, sliding_window: Optional[int] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of each packed sequence over itself.
+
+    query [rows, q_heads, head_dim], key and value [rows, kv_heads, head_dim] (fp16 or bf16, q_heads a
+    multiple of kv_heads, head_dim 64, 128 or 256), any strides of rows and heads: slices of one fused
+    projection are read in place.  scale: 1 / sqrt(head_dim) by default.  sliding_window: query i sees
+    keys i - window < j <= i.
+    Returns [rows, q_heads, head_dim].  Rows behind the plan's sequences are left as they are in `out`,
+    and are zero without one.  Inference only: tensors that require a gradient are refused."""
+    lib = _lib.load()
+    for name, t in (("query", query), ("key", key), ("value", value)):
+        _lib.require_device(t, name)
+        if t.dim() != 3:
+            raise ValueError(f"{name} must be [rows, heads, head_dim], got {tuple(t.shape)}")
+    rows, hq, d = query.shape
+    hkv = key.shape[1]
+    if tuple(key.shape) != (rows, hkv, d) or value.shape != key.shape:
+        raise ValueError(f"incompatible query {tuple(query.shape)}, key {tuple(key.shape)} and value {tuple(value.shape)}")
+    if hkv == 0 or hq == 0 or hq % hkv:
+        raise ValueError(f"{hq} query heads are no multiple of {hkv} kv heads")
+    if not (query.dtype == key.dtype == value.dtype) or query.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("query, key and value must share an fp16 or bf16 dtype")
+    if not query.device == key.device == value.device:
+        raise ValueError("query, key and value must be on one device")
+    if d not in _HEAD_DIMS:
+        raise ValueError(f"head_dim {d} unsupported (64, 128, 256)")
+    if rows < plan.rows:
+        raise ValueError(f"the plan's sequences have {plan.rows} rows, the tensors {rows}")
+    if plan.tiles is not None and plan.tiles.device != query.device:
+        raise ValueError(f"the plan is on {plan.tiles.device}, the tensors on {query.device}")
+    if sliding_window is not None and int(sliding_window) <= 0:
+        raise ValueError(f"sliding_window must be positive, got {sliding_window}")
+    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
+        raise NotImplementedError("prompt_attention has no backward pass; call it under torch.no_grad()")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError(f"scale must be positive, got {scale}")
+    if out is None:
+        out = torch.empty(rows, hq, d, dtype=query.dtype, device=query.device)
+        if rows > plan.rows:
+            out[plan.rows:].zero_()
+    elif (tuple(out.shape) != (rows, hq, d) or out.dtype != query.dtype or out.device != query.device
+          or out.stride(2) != 1 or out.stride(0) % 4 or out.stride(1) % 4 or out.data_ptr() % 8):
+        raise ValueError(f"out must be {(rows, hq, d)} {query.dtype} on {query.device} with 8-byte aligned head vectors")
+    if plan.n_tiles == 0:
+        return out
+    q, k, v = _rows(query), _rows(key), _rows(value)
+    window = 0 if sliding_window is None or int(sliding_window) >= max(plan.lengths) else int(sliding_window)
+    two = ctypes.c_int64 * 2
+    desc = _lib.PromptDesc(q_heads=hq, kv_heads=hkv, head_dim=d, dtype=_lib.dtype_code(q.dtype), n_tiles=plan.n_tiles,
+                           sliding_window=window, q=_addr(q), k=_addr(k), v=_addr(v), out=_addr(out),
+                           tiles=_addr(plan.tiles), q_stride=two(*q.stride()[:2]), k_stride=two(*k.stride()[:2]),
+                           v_stride=two(*v.stride()[:2]), out_stride=two(*out.stride()[:2]), scale=scale)
+    with torch.cuda.device(q.device):
+        st = lib.nq_prompt_attention(ctypes.byref(desc), ctypes.c_void_p(_lib.current_stream_handle(q.device)))
+    _lib.check(st, "nq_prompt_attention")
+    return out

@@ -33,6 +33,7 @@ HIPCC_FLAGS = [
 SOURCE_FLAGS = {
     "nq_score.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "nq_keykey.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "nq_prompt.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -1,0 +1,229 @@
+// One pass of softmax attention over tiles of keys and values in LDS: 32 query rows a
+// wave, running maximum and sum, matrix cores for both products.
+//
+// With q the wave's 32 queries, a tile of 32 keys K and its values V:
+//   S^T = K q^T      32x32x16 MFMAs, keys the A operand: lane (n, g) gets its query n's
+//                    logits at the keys acc_row(j, g) = 8 (j / 4) + 4 g + j % 4
+//   p   = 2^(c s - m)  c = scale * log2(e), m >= c max s - kSlack: lane-local
+//   O^T += V^T P^T   P^T is the B operand as it stands (an MFMA's k order is free as long
+//                    as both operands share it: slot (g, i) of step s is key
+//                    16 s + 8 (i / 4) + 4 g + i % 4), V^T the A operand by transposing
+//                    LDS reads (ds_read_b64_tr_b16: 4 keys x 16 coordinates of 16 lanes)
+// so a query's maximum, sum and output stay in the two lanes (n, 0) and (n, 1).
+#pragma once
+
+#include "nq_common.h"
+
+namespace nq {
+namespace flash {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void global_void;
+
+constexpr int kStage = 64;  // keys of a stage: two tiles
+
+// A running maximum may lag the true one by 2^kSlack before the output is rescaled: weights stay
+// at most 256 (sums in fp32, weights in fp16 or bf16 have the room), and the 16 D / 32 multiplies
+// of a rescale run in the first stages of a row only.
+constexpr float kSlack = 8.0f;
+constexpr float kNoMax = -3.0e38f;  // finite, so that a row that has seen no key forms no inf - inf
+
+template <int DT>
+__device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (DT == NQ_F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// two floats rounded to nearest even, packed
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (DT == NQ_F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+}
+template <int DT>
+__device__ __forceinline__ float unpack(uint32_t bits16) {
+    if constexpr (DT == NQ_F16) return f16_bits_to_f32(bits16);
+    else return bf16_bits_to_f32(bits16);
+}
+
+// The values of lanes l and l + 32, in either.  (Elements are taken out before they are cast: a bit
+// cast of a vector's element reads the first one.)
+__device__ __forceinline__ f32x2 halves(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t lo = r[0], hi = r[1];
+    return {__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)};
+}
+__device__ __forceinline__ float both_max(float v) {
+    const f32x2 h = halves(v);
+    return __builtin_fmaxf(h.x, h.y);
+}
+__device__ __forceinline__ float both_sum(float v) {
+    const f32x2 h = halves(v);
+    return h.x + h.y;
+}
+
+__device__ __forceinline__ int acc_row(int j, int g) { return 8 * (j >> 2) + 4 * g + (j & 3); }
+
+// A stage's LDS layout: row r (a key) at byte r * 2 D, its 16-byte chunk c at chunk place
+// c ^ f(r).  Keys are read 32 rows at one chunk (ds_read_b128), values 4 rows at 64 bytes
+// (transposing ds_read_b64); each f spreads its read over all 64 banks.
+template <int D>
+struct Tile {
+    static constexpr int ROWB = 2 * D;
+    static constexpr int UPR = D / 8;           // 16-byte chunks a row
+    static constexpr int BYTES = kStage * ROWB;
+    static constexpr int KS = D / 16;           // MFMA steps of a logit
+    static constexpr int DB = D / 32;           // 32-coordinate blocks of the output
+    static __device__ __forceinline__ int key_swizzle(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
+    static __device__ __forceinline__ int value_swizzle(int r) { return D == 64 ? 4 * ((r >> 1) & 1) : 4 * (r & 3); }
+};
+
+template <int DT, int D>
+struct Rows {
+    using T = Tile<D>;
+    u32x4 q[T::KS];       // lane (n, g): query n, coordinates 16 s + 8 g + 0..7
+    f32x16 o[T::DB];      // lane (n, g): query n, coordinates 32 b + acc_row(j, g)
+    float m, l;           // c * (lagging) maximum; this lane's part of the sum
+    uint32_t k_at, v_at, v_xor;
+
+    __device__ __forceinline__ void init(int lane) {
+        const int n = lane & 31, g = lane >> 5;
+#pragma unroll
+        for (int b = 0; b < T::DB; ++b) o[b] = f32x16{};
+        m = kNoMax;
+        l = 0.0f;
+        // keys: row n of a tile, chunk (2 s + g) ^ swizzle(n); swizzles of rows n and n + 32 agree
+        k_at = (uint32_t)(n * T::ROWB + 16 * (g ^ T::key_swizzle(n)));
+        // values: row 4 g + r of a step, r = lane / 4 % 4; chunk 4 b + 2 (lane / 16 % 2) + lane / 2 % 2
+        const int r = 4 * g + ((lane >> 2) & 3);
+        v_at = (uint32_t)(r * T::ROWB + 16 * (2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) + 8 * (lane & 1));
+        v_xor = (uint32_t)(16 * T::value_swizzle(r));
+    }
+
+    __device__ __forceinline__ f32x16 logits(const char* kbuf, int t) const {
+        f32x16 s = {};
+        const char* const base = kbuf + t * 32 * T::ROWB;
+#pragma unroll
+        for (int i = 0; i < T::KS; ++i)
+            s = mfma<DT>(*reinterpret_cast<const u32x4*>(base + (k_at ^ (uint32_t)(32 * i))), q[i], s);
+        return s;
+    }
+
+    __device__ __forceinline__ u32x4 value_operand(const char* vbuf, int t, int s, int b) const {
+        const uint32_t at = (uint32_t)((t * 32 + 16 * s) * T::ROWB) + ((v_at + 64u * (uint32_t)b) ^ v_xor);
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_void*)(vbuf + at));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_void*)(vbuf + at + 8 * T::ROWB));
+        const u32x2 a = __builtin_bit_cast(u32x2, lo), c = __builtin_bit_cast(u32x2, hi);
+        return u32x4{a.x, a.y, c.x, c.y};
+    }
+
+    // the maximum of the stage's logits (c > 0), and the output rescaled where it passes the slack
+    __device__ __forceinline__ void raise(float mx, float c) {
+        mx = both_max(mx) * c;
+        if (__any(mx > m + kSlack)) {
+            const float to = __builtin_fmaxf(m, mx);
+            const float f = __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            l *= f;
+#pragma unroll
+            for (int b = 0; b < T::DB; ++b) o[b] *= f;
+        }
+    }
+
+    __device__ __forceinline__ void weights(const f32x16& s, float c, uint32_t (&p)[8]) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, -m));
+            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j + 1], c, -m));
+            sum += x;
+            sum += y;
+            p[j / 2] = pack2<DT>(x, y);
+        }
+        l += sum;
+    }
+
+    __device__ __forceinline__ void add_values(const uint32_t (&p)[8], const char* vbuf, int t) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const u32x4 w = {p[4 * s], p[4 * s + 1], p[4 * s + 2], p[4 * s + 3]};
+#pragma unroll
+            for (int b = 0; b < T::DB; ++b) o[b] = mfma<DT>(value_operand(vbuf, t, s, b), w, o[b]);
+        }
+    }
+
+    // Whether a tile of values holds an infinity or a NaN.  A hidden key's weight is zero, but zero
+    // times such a value is NaN, so a tile that hides keys must not hold one for the product above.
+    __device__ __forceinline__ bool tile_odd(const char* vbuf, int t, int lane) const {
+        constexpr uint32_t kExp = DT == NQ_F16 ? 0x7c00u : 0x7f80u;
+        uint32_t odd = 0;
+#pragma unroll
+        for (int i = 0; i < T::UPR / 2; ++i) {  // the tile's 4 D dwords, whichever lane reads which
+            const u32x4 v = *reinterpret_cast<const u32x4*>(vbuf + 32 * t * T::ROWB + 1024 * i + 16 * lane);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) odd |= (uint32_t)((v[k] & kExp) == kExp) | (uint32_t)((v[k] & (kExp << 16)) == (kExp << 16));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        return __any((int)odd);
+    }
+
+    // one stage that every query sees whole
+    __device__ __forceinline__ void stage(const char* kbuf, const char* vbuf, float c) {
+        f32x16 s[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[t] = logits(kbuf, t);
+        float mx = s[0][0];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) mx = __builtin_fmaxf(mx, s[t][j]);
+        raise(mx, c);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            uint32_t p[8];
+            weights(s[t], c, p);
+            add_values(p, vbuf, t);
+        }
+    }
+
+    // One stage of which this lane's query sees the keys lo <= key < hi (of 64).  Returns whether a
+    // tile that was summed holds values that spoil the sums of queries that do not see them.
+    __device__ __forceinline__ bool stage_masked(const char* kbuf, const char* vbuf, float c, int lo, int hi, int lane) {
+        const int g = lane >> 5;
+        bool odd = false;
+#pragma unroll 1
+        for (int t = 0; t < 2; ++t, lo -= 32, hi -= 32) {
+            if (!__any(lo < 32 && hi > 0 && lo < hi)) continue;
+            f32x16 s = logits(kbuf, t);
+            float mx = -__builtin_inff();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int key = acc_row(j, g);
+                s[j] = key >= lo && key < hi ? s[j] : -__builtin_inff();
+                mx = __builtin_fmaxf(mx, s[j]);
+            }
+            raise(mx, c);
+            uint32_t p[8];
+            weights(s, c, p);
+            add_values(p, vbuf, t);
+            odd |= tile_odd(vbuf, t, lane);
+        }
+        return odd;
+    }
+};
+
+}  // namespace flash
+}  // namespace nq

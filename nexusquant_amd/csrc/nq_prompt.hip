@@ -1,0 +1,209 @@
+// Causal attention over packed prompts (grouped heads, optional sliding window) on gfx950:
+// query i of a sequence sees its keys j with i - window < j <= i.
+//
+// A workgroup of 4 waves owns 128 consecutive queries of one sequence and head, 32 a wave,
+// and streams the 64-key stages that they see through two LDS buffers each for keys and
+// values (direct-to-LDS loads, under way while the other buffer is computed on).
+#include "nq_flash.h"
+
+namespace nq {
+
+using namespace flash;
+
+struct PromptArgs {
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    uint16_t* out;
+    const int32_t* tiles;  // [n_tiles * 4]: first row of the sequence, its length, the tile's first query, 0
+    int64_t q_row, k_row, v_row, o_row;      // strides of a token, elements
+    int64_t q_head, k_head, v_head, o_head;  // of a head
+    uint32_t hq, hkv;
+    int32_t window;        // 0: none
+    float c;               // scale * log2(e)
+};
+
+constexpr int kWaitVm0 = 0x0f70;  // vmcnt(0), the other counters left open
+constexpr int kPromptRows = 128;
+
+// Rows row0 .. row0 + 63 of one head to LDS in Tile's layout; rows past the sequence repeat its
+// last one (their weights are zero, and what lies behind the sequence is never read).
+template <int D, bool VALUES>
+__device__ __forceinline__ void load_stage(const uint16_t* base, int64_t stride, int row0, int n, char* buf, int wave, int lane) {
+    using T = Tile<D>;
+#pragma unroll
+    for (int i = 0; i < T::UPR / 4; ++i) {
+        const int w = 4 * i + wave, slot = 64 * w + lane;
+        const int r = slot / T::UPR, place = slot % T::UPR;
+        const int chunk = place ^ (VALUES ? T::value_swizzle(r) : T::key_swizzle(r));
+        const int row = min(row0 + r, n - 1);
+        const uint16_t* src = base + (int64_t)row * stride + 8 * chunk;
+        __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(buf + 1024 * w), 16, 0, 0);
+    }
+}
+
+// The output of a wave's queries again, key by key on the vector ALUs, each query over the keys
+// it sees only: for blocks with an infinity or a NaN among the values of a tile that hides keys.
+// The maxima and sums of the fast pass hold (hidden logits never enter them).
+template <int DT, int D>
+__device__ __forceinline__ void sum_again(Rows<DT, D>& rows, const uint16_t* kb, int64_t k_row, const uint16_t* vb, int64_t v_row,
+                                          float c, int key_first, int key_last, int lo, int hi, int g) {
+    using T = Tile<D>;
+#pragma unroll
+    for (int b = 0; b < T::DB; ++b) rows.o[b] = f32x16{};
+#pragma unroll 1
+    for (int key = key_first; key <= key_last; ++key) {
+        const uint16_t* const kr = kb + key * k_row + 8 * g;
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < T::KS; ++i) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(kr + 16 * i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                s = __builtin_fmaf(unpack<DT>(x[k] & 0xffffu), unpack<DT>(rows.q[i][k] & 0xffffu), s);
+                s = __builtin_fmaf(unpack<DT>(x[k] >> 16), unpack<DT>(rows.q[i][k] >> 16), s);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        s = both_sum(s);
+        if (key < lo || key > hi) continue;
+        const float p = unpack<DT>(pack2<DT>(__builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -rows.m)), 0.0f) & 0xffffu);
+        const uint16_t* const vr = vb + key * v_row + 4 * g;
+#pragma unroll
+        for (int b = 0; b < T::DB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const u32x2 x = *reinterpret_cast<const u32x2*>(vr + 32 * b + 8 * i);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    rows.o[b][4 * i + k] = __builtin_fmaf(p, unpack<DT>((k & 1) ? x[k / 2] >> 16 : x[k / 2] & 0xffffu), rows.o[b][4 * i + k]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    }
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(PromptArgs a) {
+    using T = Tile<D>;
+    __shared__ __align__(16) char k0[T::BYTES];
+    __shared__ __align__(16) char k1[T::BYTES];
+    __shared__ __align__(16) char v0[T::BYTES];
+    __shared__ __align__(16) char v1[T::BYTES];
+    const int lane = threadIdx.x & 63, n = lane & 31, g = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    // kv heads fastest: blocks go to the XCDs in turn, so the query heads of a kv head meet in one
+    // XCD's L2 when the kv heads are a multiple of 8
+    const uint32_t tile = blockIdx.x / a.hq, j = blockIdx.x % a.hq;
+    const uint32_t kh = j % a.hkv, head = kh * (a.hq / a.hkv) + j / a.hkv;
+    const int32_t first = a.tiles[4 * tile], len = a.tiles[4 * tile + 1], q0 = a.tiles[4 * tile + 2];
+    const int q_last = min(q0 + kPromptRows, len) - 1;
+    const int key0 = a.window ? max(q0 - a.window + 1, 0) & ~(kStage - 1) : 0;
+    const int n_stages = (q_last - key0) / kStage + 1;
+    const int my0 = q0 + 32 * wave;               // this wave's first query
+    const bool live = my0 < len;
+    const int my_q = min(my0 + n, len - 1);
+    const int my_last = min(my0 + 31, len - 1);
+
+    const uint16_t* const kb = a.k + first * a.k_row + kh * a.k_head;
+    const uint16_t* const vb = a.v + first * a.v_row + kh * a.v_head;
+    Rows<DT, D> rows;
+    bool odd = false;
+    rows.init(lane);
+    const uint16_t* const qp = a.q + (first + (int64_t)my_q) * a.q_row + head * a.q_head + 8 * g;
+#pragma unroll
+    for (int i = 0; i < T::KS; ++i) rows.q[i] = *reinterpret_cast<const u32x4*>(qp + 16 * i);
+
+    load_stage<D, false>(kb, a.k_row, key0, len, k0, wave, lane);
+    load_stage<D, true>(vb, a.v_row, key0, len, v0, wave, lane);
+    __builtin_amdgcn_s_waitcnt(kWaitVm0);
+    __syncthreads();
+    auto step = [&](int it, const char* ck, const char* cv, char* nk, char* nv) {
+        const int key = key0 + kStage * it;
+        if (it + 1 < n_stages) {
+            load_stage<D, false>(kb, a.k_row, key + kStage, len, nk, wave, lane);
+            load_stage<D, true>(vb, a.v_row, key + kStage, len, nv, wave, lane);
+        }
+        if (live && key <= my_last) {
+            const bool whole = key + kStage - 1 <= my0 && (!a.window || key > my_last - a.window);
+            if (whole) rows.stage(ck, cv, a.c);
+            else odd |= rows.stage_masked(ck, cv, a.c, a.window ? my_q - a.window + 1 - key : 0, my_q + 1 - key, lane);
+        }
+        __builtin_amdgcn_s_waitcnt(kWaitVm0);
+        __syncthreads();
+    };
+#pragma unroll 1
+    for (int it = 0; it < n_stages; it += 2) {
+        step(it, k0, v0, k1, v1);
+        if (it + 1 < n_stages) step(it + 1, k1, v1, k0, v0);
+    }
+    if (odd) sum_again<DT, D>(rows, kb, a.k_row, vb, a.v_row, a.c, key0, my_last, a.window ? my_q - a.window + 1 : 0, my_q, g);
+    if (!live || my0 + n >= len) return;
+    const float r = 1.0f / both_sum(rows.l);
+    uint16_t* const op = a.out + (first + (int64_t)my_q) * a.o_row + head * a.o_head + 4 * g;
+#pragma unroll
+    for (int b = 0; b < T::DB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const u32x2 w = {pack2<DT>(rows.o[b][4 * i] * r, rows.o[b][4 * i + 1] * r),
+                             pack2<DT>(rows.o[b][4 * i + 2] * r, rows.o[b][4 * i + 3] * r)};
+            *reinterpret_cast<u32x2*>(op + 32 * b + 8 * i) = w;
+        }
+}
+
+template <int DT>
+static hipError_t launch_prompt(int32_t d, const PromptArgs& a, uint32_t blocks, hipStream_t s) {
+    switch (d) {
+        case 64: hipLaunchKernelGGL((prompt_kernel<DT, 64>), dim3(blocks), dim3(256), 0, s, a); break;
+        case 128: hipLaunchKernelGGL((prompt_kernel<DT, 128>), dim3(blocks), dim3(256), 0, s, a); break;
+        default: hipLaunchKernelGGL((prompt_kernel<DT, 256>), dim3(blocks), dim3(256), 0, s, a); break;
+    }
+    return hipGetLastError();
+}
+
+}  // namespace nq
+
+extern "C" int32_t nq_prompt_tile_rows(void) { return nq::kPromptRows; }
+
+extern "C" int nq_prompt_attention(const nq_prompt_desc* d, void* stream) {
+    using namespace nq;
+    NQ_CHECK_ARG(d != nullptr, "nq_prompt_attention: desc is NULL");
+    NQ_CHECK_ARG(d->head_dim == 64 || d->head_dim == 128 || d->head_dim == 256,
+                 "nq_prompt_attention: head_dim %d unsupported (64, 128, 256)", d->head_dim);
+    NQ_CHECK_ARG(d->dtype == NQ_F16 || d->dtype == NQ_BF16, "nq_prompt_attention: dtype must be fp16 or bf16");
+    NQ_CHECK_ARG(d->q_heads > 0 && d->kv_heads > 0 && d->q_heads % d->kv_heads == 0,
+                 "nq_prompt_attention: q_heads %d must be a positive multiple of kv_heads %d", d->q_heads, d->kv_heads);
+    NQ_CHECK_ARG(d->n_tiles >= 0 && d->sliding_window >= 0, "nq_prompt_attention: n_tiles %d, sliding_window %d",
+                 d->n_tiles, d->sliding_window);
+    NQ_CHECK_ARG(d->scale > 0.0f && d->scale < 1e30f, "nq_prompt_attention: scale must be positive");
+    if (d->n_tiles == 0) return NQ_OK;
+    NQ_CHECK_ARG(d->q && d->k && d->v && d->out && d->tiles, "nq_prompt_attention: q, k, v, out and tiles are required");
+    NQ_CHECK_ARG((((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v) & 15u) == 0 && ((uintptr_t)d->out & 7u) == 0,
+                 "nq_prompt_attention: q, k and v must be 16-byte aligned, out 8-byte");
+    NQ_CHECK_ARG(((d->q_stride[0] | d->q_stride[1] | d->k_stride[0] | d->k_stride[1] | d->v_stride[0] | d->v_stride[1]) & 7) == 0 &&
+                     ((d->out_stride[0] | d->out_stride[1]) & 3) == 0,
+                 "nq_prompt_attention: strides must keep rows 16-byte aligned (out: 8-byte)");
+    NQ_CHECK_ARG((uint64_t)d->n_tiles * d->q_heads <= max_blocks(256), "nq_prompt_attention: grid too large");
+    PromptArgs a = {};
+    a.q = static_cast<const uint16_t*>(d->q);
+    a.k = static_cast<const uint16_t*>(d->k);
+    a.v = static_cast<const uint16_t*>(d->v);
+    a.out = static_cast<uint16_t*>(d->out);
+    a.tiles = d->tiles;
+    a.q_row = d->q_stride[0];
+    a.q_head = d->q_stride[1];
+    a.k_row = d->k_stride[0];
+    a.k_head = d->k_stride[1];
+    a.v_row = d->v_stride[0];
+    a.v_head = d->v_stride[1];
+    a.o_row = d->out_stride[0];
+    a.o_head = d->out_stride[1];
+    a.hq = (uint32_t)d->q_heads;
+    a.hkv = (uint32_t)d->kv_heads;
+    a.window = d->sliding_window;
+    a.c = d->scale * 1.44269504088896340736f;
+    const uint32_t blocks = (uint32_t)d->n_tiles * a.hq;
+    hipStream_t s = (hipStream_t)stream;
+    NQ_CHECK_HIP(d->dtype == NQ_F16 ? launch_prompt<NQ_F16>(d->head_dim, a, blocks, s)
+                                    : launch_prompt<NQ_BF16>(d->head_dim, a, blocks, s));
+    return NQ_OK;
+}

@@ -19,6 +19,7 @@ streams orders them.  Decode attention over a pool: NexusQuantPagedAttention.pla
 
 from __future__ import annotations
 
+import array
 import ctypes
 import threading
 from typing import List, Optional, Sequence, Tuple
@@ -141,7 +142,12 @@ class CompressedPagePool:
         return -(-int(length) // self.page_tokens)
 
     def _pages(self, pages) -> np.ndarray:
-        p = np.asarray(pages, dtype=np.int64).reshape(-1)
+        # a list of ints by way of array(): two thirds of numpy's own conversion time
+        try:
+            p = (np.frombuffer(array.array("i", pages), dtype=np.int32) if type(pages) is list and pages
+                 else np.asarray(pages, dtype=np.int64).reshape(-1))
+        except OverflowError:
+            raise ValueError(f"page numbers must lie in [0, {self.num_pages})") from None
         if len(p) and (p.min() < 0 or p.max() >= self.num_pages):
             raise ValueError(f"page numbers must lie in [0, {self.num_pages})")
         return p
@@ -151,6 +157,14 @@ class CompressedPagePool:
         if len(p) and self._refs[p].min() < 1:
             raise ValueError(f"{what}: page {int(p[self._refs[p] < 1][0])} is not allocated")
         return p
+
+    def _tally(self, p: np.ndarray):
+        """The pages in p, ascending and each once, and how often each is there."""
+        if 8 * len(p) < self.num_pages:
+            return np.unique(p, return_counts=True)
+        n = np.bincount(p, minlength=self.num_pages)  # 7 us where sorting 6000 pages takes 53
+        p = np.flatnonzero(n)
+        return p, n[p]
 
     def allocate(self, n: int) -> List[int]:
         """n pages with one reference each.  Their contents are whatever they last held."""
@@ -168,14 +182,15 @@ class CompressedPagePool:
     def retain(self, pages: Sequence[int]) -> None:
         """One more reference to each page (to a page listed twice: two)."""
         with self._lock:
-            np.add.at(self._refs, self._in_use(pages, "retain"), 1)
+            p, n = self._tally(self._in_use(pages, "retain"))
+            self._refs[p] += n.astype(np.int32)
 
     def free(self, pages: Sequence[int]) -> None:
         """Drop one reference of each page (of a page listed twice: two); pages without any can be
         allocated again.  Work already queued on the pool's stream still sees them as they were."""
         with self._lock:
-            p, n = np.unique(self._in_use(pages, "free"), return_counts=True)
-            left = self._refs[p] - n
+            p, n = self._tally(self._in_use(pages, "free"))
+            left = self._refs[p] - n.astype(np.int32)
             if len(p) and left.min() < 0:
                 raise ValueError(f"page {int(p[left < 0][0])} is freed more often than it is referenced")
             self._refs[p] = left
@@ -211,6 +226,8 @@ class CompressedPagePool:
         p, length = self._in_use(pages, what), int(length)
         if length < 0 or self.pages_for(length) != len(p):
             raise ValueError(f"{what}: {length} tokens take {self.pages_for(max(length, 0))} pages, got {len(p)}")
+        if len(self._tally(p)[0]) != len(p):
+            raise ValueError(f"{what}: a page stands twice in one sequence")
         return p, length
 
     def fork(self, pages: Sequence[int], length: int, n: int = 1) -> List[List[int]]:
@@ -224,11 +241,11 @@ class CompressedPagePool:
             n = int(n)
             if n < 0:
                 raise ValueError(f"cannot fork {n} branches")
-            table = p.tolist()
+            table = list(pages) if type(pages) is list else p.tolist()
             if n == 0:
                 return []
             if length % self.page_tokens == 0:
-                np.add.at(self._refs, p, n)
+                self._refs[p] += n
                 return [list(table) for _ in range(n)]
             last = self.allocate(n)
             try:
@@ -236,7 +253,7 @@ class CompressedPagePool:
             except Exception:
                 self.free(last)
                 raise
-            np.add.at(self._refs, p[:-1], n)
+            self._refs[p[:-1]] += n
             return [table[:-1] + [x] for x in last]
 
     def compact(self, tables: Sequence[Sequence[int]], lengths: Sequence[int], kept_idx: torch.Tensor, n_kept,
@@ -273,8 +290,8 @@ class CompressedPagePool:
                     raise ValueError(f"sequence {b} keeps {counts[b]} of {n} tokens by a list of {idx.shape[1]}")
                 old.append(p)
             want = [self.pages_for(c) for c in counts]
-            flat = np.concatenate(old) if old else np.zeros(0, dtype=np.int64)
-            held, times = np.unique(flat, return_counts=True)
+            flat = np.concatenate(old) if old else np.zeros(0, dtype=np.int32)
+            held, times = self._tally(flat)
             if np.any(times > self._refs[held]):
                 raise ValueError("compact: a page stands in more tables than it has references")
             new = self.allocate(sum(want))

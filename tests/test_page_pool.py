@@ -79,7 +79,7 @@ def test_fork_shares_full_pages_and_copies_the_last(monkeypatch):
     assert pool.fork(a, 12) == [[0, 1, 2]] and pool.ref_count(2) == 2  # nothing part-filled: nothing copied
     assert len(pool.copied) == 1
     assert pool.fork([], 0, 2) == [[], []] and pool.fork(a, 10, 0) == []
-    for pages, length in ((a, 8), (a, 13), (a[:2], 9), ([8], 1), (a, -1)):
+    for pages, length in ((a, 8), (a, 13), (a[:2], 9), ([8], 1), (a, -1), ([0, 1, 1], 12)):
         with pytest.raises(ValueError):
             pool.fork(pages, length)
     with pytest.raises(ValueError, match="shared"):

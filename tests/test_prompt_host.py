@@ -1,0 +1,77 @@
+"""Host side of packed prompt attention: the tile list and the refusals, without a GPU."""
+
+import ctypes
+import os
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+from nexusquant_amd import _lib
+from nexusquant_amd.attention import PromptPlan, plan_prompts, prompt_attention, prompt_tiles
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.mark.parametrize("lens", [[], [0], [1], [128], [129], [0, 5, 0, 300, 128, 0], [4096, 1, 64]])
+def test_tiles_cover_every_query_once_longest_first(lens):
+    tiles = prompt_tiles(lens, 128)
+    starts = np.concatenate([[0], np.cumsum(lens)])
+    seen = []
+    for first, n, q0, _ in tiles.tolist():
+        b = [i for i in range(len(lens)) if starts[i] == first and lens[i] == n and n]
+        assert b and 0 <= q0 < n and q0 % 128 == 0
+        seen += range(first + q0, first + min(q0 + 128, n))
+    assert sorted(seen) == list(range(sum(lens)))
+    assert list(tiles[:, 2]) == sorted(tiles[:, 2], reverse=True)
+
+
+def test_plan_refusals():
+    with pytest.raises(ValueError):
+        plan_prompts([3, -1], device="cuda")
+    with pytest.raises(ValueError):
+        plan_prompts([1 << 30, 1 << 30], device="cuda")
+    with pytest.raises(_lib.NexusQuantError):
+        plan_prompts([3], device="cpu")
+    x = torch.zeros(4, 2, 64, dtype=torch.float16)
+    with pytest.raises(_lib.NexusQuantError):
+        prompt_attention(x, x, x, PromptPlan((4,), 4, 0, None))
+
+
+def test_prompt_struct_matches_the_c_compiler(tmp_path):
+    names = [f[0] for f in _lib.PromptDesc._fields_]
+    prog = ["#include <stddef.h>", "#include <stdio.h>", f'#include "{ROOT}/include/nexusquant_amd.h"', "int main(void){",
+            'printf("%zu\\n", sizeof(nq_prompt_desc));']
+    prog += [f'printf("%zu\\n", offsetof(nq_prompt_desc, {f}));' for f in names] + ["return 0;}"]
+    (tmp_path / "p.c").write_text("\n".join(prog))
+    subprocess.check_call(["gcc", "-o", str(tmp_path / "p"), str(tmp_path / "p.c")])
+    out = [int(x) for x in subprocess.check_output([str(tmp_path / "p")]).split()]
+    assert out == [ctypes.sizeof(_lib.PromptDesc)] + [getattr(_lib.PromptDesc, f).offset for f in names]
+
+
+def desc(**kw):
+    dummy = ctypes.c_void_p(4096)
+    two = ctypes.c_int64 * 2
+    base = dict(q_heads=8, kv_heads=2, head_dim=128, dtype=_lib.NQ_F16, n_tiles=1, q=dummy, k=dummy, v=dummy, out=dummy,
+                tiles=dummy, q_stride=two(1024, 128), k_stride=two(256, 128), v_stride=two(256, 128),
+                out_stride=two(1024, 128), scale=0.1)
+    return _lib.PromptDesc(**{**base, **kw})
+
+
+@pytest.mark.parametrize("kw", [
+    dict(head_dim=96), dict(dtype=_lib.NQ_F32), dict(q_heads=0), dict(q_heads=7), dict(kv_heads=0), dict(n_tiles=-1),
+    dict(sliding_window=-1), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None),
+    dict(tiles=None), dict(out=ctypes.c_void_p(4100)), dict(v=ctypes.c_void_p(4104)),
+    dict(k_stride=(ctypes.c_int64 * 2)(260, 128)), dict(out_stride=(ctypes.c_int64 * 2)(1024, 130)),
+    dict(n_tiles=1 << 24), dict(q_heads=1 << 30, kv_heads=1)])
+def test_c_entry_refuses(kw):
+    lib = _lib.load()
+    assert lib.nq_prompt_attention(ctypes.byref(desc(**kw)), None) == -1
+    assert lib.nq_last_error().startswith(b"nq_prompt_attention")
+
+
+def test_c_entry_takes_an_empty_batch():
+    lib = _lib.load()
+    assert lib.nq_prompt_attention(ctypes.byref(desc(n_tiles=0, q=None, tiles=None)), None) == 0
+    assert lib.nq_prompt_attention(None, None) == -1
