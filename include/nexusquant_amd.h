@@ -661,6 +661,56 @@ int nq_pool_compact(const nq_pool* pool, const int32_t* tile_seq, int32_t n_tile
 int nq_pool_write(const nq_pool* pool, int32_t layer, const nq_pool* tokens, const int32_t* slots, int32_t n,
                   void* stream);
 
+/*
+ * Decode attention over a pool's pages for rows that share pages: for each
+ * batch row and query head softmax(q . k / scale_divisor) . v over the row's
+ * tokens, k and v the pages' keys and values.  The tokens come as segments: pages that a list of
+ * rows sees whole; a row's tokens are the union of its segments.
+ *   items    [n_items * 8] chunks of segments, up to
+ *            nq_shared_attention_chunk_tokens() tokens each:
+ *              [0] where the segment's pages start in `pages`
+ *              [1] the chunk's first token, counted from there
+ *              [2] its tokens (1 ..)
+ *              [3] where its rows start in `seg_rows` (entries)
+ *              [4] rows, at most nq_shared_attention_rows() / (q_heads / heads)
+ *              [5] the chunk's number in its segment;  [6..7] unused
+ *   pages    page numbers
+ *   seg_rows [entries * 2] batch row, and the row's slot of the segment's
+ *            first chunk
+ *   row_slots [batch + 1] each row's slots, one per chunk that it sees
+ *            (every slot is written by exactly one item)
+ * Device int32 arrays.  query, out: [batch, q_heads, head_dim], fp16 or bf16;
+ * a row without slots is zero.  Rounding: keys to fp16; queries of bf16 to
+ * fp16 after a power of two is taken out; softmax weights and values times
+ * their scale to fp16; sums in fp32.
+ * workspace: nq_shared_attention_workspace(n_slots, q_heads, head_dim) bytes,
+ * 16-byte aligned.
+ */
+typedef struct nq_shared_desc {
+    const nq_pool* pool;
+    int32_t layer, batch, q_heads;
+    int32_t q_dtype;            /* NQ_F16 / NQ_BF16 */
+    int32_t n_items, n_slots;
+    const void* query;
+    void* out;
+    const int32_t* items;
+    const int32_t* pages;
+    const int32_t* seg_rows;
+    const int32_t* row_slots;
+    const float* rope_sin_minus_cos;
+    const float* rope_cos_plus_sin;
+    int64_t rope_n_pos;
+    float hadamard_scale;
+    float scale_divisor;
+    void* workspace;
+    int64_t workspace_bytes;
+} nq_shared_desc;
+
+int32_t nq_shared_attention_chunk_tokens(void);
+int32_t nq_shared_attention_rows(void);
+int64_t nq_shared_attention_workspace(int32_t n_slots, int32_t q_heads, int32_t head_dim);
+int nq_shared_attention(const nq_shared_desc* desc, void* stream);
+
 /* Library version and the last error message of the calling thread. */
 int nq_abi_version(void);
 const char* nq_last_error(void);

@@ -16,7 +16,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .ops import _addr
+from .ops import PlanTensor, _addr
 
 _HEAD_DIMS = (64, 128, 256)
 
@@ -27,7 +27,7 @@ class PromptPlan:
     lengths: tuple
     rows: int                     # of all sequences
     n_tiles: int
-    tiles: Optional[torch.Tensor]  # int32 [n_tiles, 4] on the device
+    tiles: Optional[PlanTensor]   # int32 [n_tiles, 4] on the device
 
 
 def prompt_tiles(lengths: Sequence[int], tile_rows: int) -> np.ndarray:
@@ -53,7 +53,7 @@ def plan_prompts(lengths: Sequence[int], device=None) -> PromptPlan:
         raise _lib.NexusQuantError(f"nexusquant_amd runs on MI355X (ROCm) devices only; the plan is for {dev}")
     tiles = prompt_tiles(lens, int(_lib.load().nq_prompt_tile_rows()))
     return PromptPlan(lengths=lens, rows=rows, n_tiles=len(tiles),
-                      tiles=torch.from_numpy(tiles).to(dev) if len(tiles) else None)
+                      tiles=PlanTensor(tiles.reshape(-1), dev) if len(tiles) else None)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -93,8 +93,8 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         raise ValueError(f"head_dim {d} unsupported (64, 128, 256)")
     if rows < plan.rows:
         raise ValueError(f"the plan's sequences have {plan.rows} rows, the tensors {rows}")
-    if plan.tiles is not None and plan.tiles.device != query.device:
-        raise ValueError(f"the plan is on {plan.tiles.device}, the tensors on {query.device}")
+    if plan.tiles is not None and plan.tiles.tensor.device != query.device:
+        raise ValueError(f"the plan is on {plan.tiles.tensor.device}, the tensors on {query.device}")
     if sliding_window is not None and int(sliding_window) <= 0:
         raise ValueError(f"sliding_window must be positive, got {sliding_window}")
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
@@ -114,11 +114,12 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     q, k, v = _rows(query), _rows(key), _rows(value)
     window = 0 if sliding_window is None or int(sliding_window) >= max(plan.lengths) else int(sliding_window)
     two = ctypes.c_int64 * 2
-    desc = _lib.PromptDesc(q_heads=hq, kv_heads=hkv, head_dim=d, dtype=_lib.dtype_code(q.dtype), n_tiles=plan.n_tiles,
-                           sliding_window=window, q=_addr(q), k=_addr(k), v=_addr(v), out=_addr(out),
-                           tiles=_addr(plan.tiles), q_stride=two(*q.stride()[:2]), k_stride=two(*k.stride()[:2]),
-                           v_stride=two(*v.stride()[:2]), out_stride=two(*out.stride()[:2]), scale=scale)
     with torch.cuda.device(q.device):
+        desc = _lib.PromptDesc(q_heads=hq, kv_heads=hkv, head_dim=d, dtype=_lib.dtype_code(q.dtype),
+                               n_tiles=plan.n_tiles, sliding_window=window, q=_addr(q), k=_addr(k), v=_addr(v),
+                               out=_addr(out), tiles=plan.tiles.address(), q_stride=two(*q.stride()[:2]),
+                               k_stride=two(*k.stride()[:2]), v_stride=two(*v.stride()[:2]),
+                               out_stride=two(*out.stride()[:2]), scale=scale)
         st = lib.nq_prompt_attention(ctypes.byref(desc), ctypes.c_void_p(_lib.current_stream_handle(q.device)))
     _lib.check(st, "nq_prompt_attention")
     return out

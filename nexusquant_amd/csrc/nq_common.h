@@ -83,6 +83,21 @@ __device__ __forceinline__ tab_t table(const uint64_t* p) {
     return (tab_t)a;
 }
 
+// Unsigned division by a launch constant: with l = ceil(log2 d) and the 33-bit multiplier
+// 2^32 + m, m = floor(2^32 (2^l - d) / d) + 1, n / d = (mulhi(n, m) + n) >> l for every 32-bit n.
+struct FastDiv {
+    uint32_t d, m, s;
+};
+inline FastDiv fast_div(uint32_t d) {
+    uint32_t l = 0;
+    while (l < 32 && (1ull << l) < d) ++l;
+    return {d, (uint32_t)(((1ull << 32) * ((1ull << l) - d)) / d + 1), l};
+}
+__device__ __forceinline__ uint32_t div(uint32_t n, const FastDiv& f) {
+    const uint64_t t = (uint64_t)__umulhi(n, f.m) + n;
+    return (uint32_t)(t >> f.s);
+}
+
 // Quad (4-lane) permutes through DPP.  Encoded as quad_perm selectors.
 constexpr int kQuadXor1 = 0xB1;  // [1,0,3,2]
 constexpr int kQuadXor2 = 0x4E;  // [2,3,0,1]

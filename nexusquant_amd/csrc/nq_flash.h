@@ -22,6 +22,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -29,8 +30,6 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) void lds_void;
 typedef const __attribute__((address_space(1))) void global_void;
-
-constexpr int kStage = 64;  // keys of a stage: two tiles
 
 // A running maximum may lag the true one by 2^kSlack before the output is rescaled: weights stay
 // at most 256 (sums in fp32, weights in fp16 or bf16 have the room), and the 16 D / 32 multiplies
@@ -77,14 +76,13 @@ __device__ __forceinline__ float both_sum(float v) {
 
 __device__ __forceinline__ int acc_row(int j, int g) { return 8 * (j >> 2) + 4 * g + (j & 3); }
 
-// A stage's LDS layout: row r (a key) at byte r * 2 D, its 16-byte chunk c at chunk place
+// A tile's LDS layout: row r (a key) at byte r * 2 D, its 16-byte chunk c at chunk place
 // c ^ f(r).  Keys are read 32 rows at one chunk (ds_read_b128), values 4 rows at 64 bytes
 // (transposing ds_read_b64); each f spreads its read over all 64 banks.
 template <int D>
 struct Tile {
     static constexpr int ROWB = 2 * D;
     static constexpr int UPR = D / 8;           // 16-byte chunks a row
-    static constexpr int BYTES = kStage * ROWB;
     static constexpr int KS = D / 16;           // MFMA steps of a logit
     static constexpr int DB = D / 32;           // 32-coordinate blocks of the output
     static __device__ __forceinline__ int key_swizzle(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
@@ -180,48 +178,39 @@ struct Rows {
         return __any((int)odd);
     }
 
-    // one stage that every query sees whole
-    __device__ __forceinline__ void stage(const char* kbuf, const char* vbuf, float c) {
+    // tiles t and t + 1, which every query sees whole
+    __device__ __forceinline__ void two_tiles(const char* kbuf, const char* vbuf, int t, float c) {
         f32x16 s[2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) s[t] = logits(kbuf, t);
+        for (int i = 0; i < 2; ++i) s[i] = logits(kbuf, t + i);
         float mx = s[0][0];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) mx = __builtin_fmaxf(mx, s[t][j]);
+            for (int j = 0; j < 16; ++j) mx = __builtin_fmaxf(mx, s[i][j]);
         raise(mx, c);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int i = 0; i < 2; ++i) {
             uint32_t p[8];
-            weights(s[t], c, p);
-            add_values(p, vbuf, t);
+            weights(s[i], c, p);
+            add_values(p, vbuf, t + i);
         }
     }
 
-    // One stage of which this lane's query sees the keys lo <= key < hi (of 64).  Returns whether a
-    // tile that was summed holds values that spoil the sums of queries that do not see them.
-    __device__ __forceinline__ bool stage_masked(const char* kbuf, const char* vbuf, float c, int lo, int hi, int lane) {
-        const int g = lane >> 5;
-        bool odd = false;
-#pragma unroll 1
-        for (int t = 0; t < 2; ++t, lo -= 32, hi -= 32) {
-            if (!__any(lo < 32 && hi > 0 && lo < hi)) continue;
-            f32x16 s = logits(kbuf, t);
-            float mx = -__builtin_inff();
+    // tile t, of which this lane's query sees the keys lo <= key < hi (of 32)
+    __device__ __forceinline__ void masked_tile(const char* kbuf, const char* vbuf, int t, float c, int lo, int hi, int g) {
+        f32x16 s = logits(kbuf, t);
+        float mx = -__builtin_inff();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int key = acc_row(j, g);
-                s[j] = key >= lo && key < hi ? s[j] : -__builtin_inff();
-                mx = __builtin_fmaxf(mx, s[j]);
-            }
-            raise(mx, c);
-            uint32_t p[8];
-            weights(s, c, p);
-            add_values(p, vbuf, t);
-            odd |= tile_odd(vbuf, t, lane);
+        for (int j = 0; j < 16; ++j) {
+            const int key = acc_row(j, g);
+            s[j] = key >= lo && key < hi ? s[j] : -__builtin_inff();
+            mx = __builtin_fmaxf(mx, s[j]);
         }
-        return odd;
+        raise(mx, c);
+        uint32_t p[8];
+        weights(s, c, p);
+        add_values(p, vbuf, t);
     }
 };
 

@@ -30,16 +30,6 @@ struct PageArgs {
     InlineTabs inl;  // tables given as host arrays
 };
 
-// Four int8 codes (one dword) -> two fp16 pairs, exactly.  XOR 0x80 biases
-// the byte to c + 128; v_perm places it under the fp16 exponent of 1024
-// (0x64 high byte), giving 1024 + c + 128, and one packed add removes 1152.
-__device__ __forceinline__ void codes_to_f16(uint32_t w, half2v& lo, half2v& hi) {
-    const uint32_t u = w ^ 0x80808080u;
-    const half2v bias = {(__fp16)-1152.0f, (__fp16)-1152.0f};
-    lo = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(u, 0x64646464u, 0x00050004u)) + bias;
-    hi = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(u, 0x64646464u, 0x00070006u)) + bias;
-}
-
 template <int D>
 __device__ __forceinline__ uint32_t page_position(const PageArgs& a, uint32_t page, uint32_t row) {
     const int32_t p = reinterpret_cast<const int32_t*>(table(a.positions)[page])[row % a.tokens];

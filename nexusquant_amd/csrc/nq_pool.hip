@@ -12,21 +12,6 @@
 
 namespace nq {
 
-// Unsigned division by a launch constant: with l = ceil(log2 d) and the 33-bit multiplier
-// 2^32 + m, m = floor(2^32 (2^l - d) / d) + 1, n / d = (mulhi(n, m) + n) >> l for every 32-bit n.
-struct FastDiv {
-    uint32_t d, m, s;
-};
-static FastDiv fast_div(uint32_t d) {
-    uint32_t l = 0;
-    while (l < 32 && (1ull << l) < d) ++l;
-    return {d, (uint32_t)(((1ull << 32) * ((1ull << l) - d)) / d + 1), l};
-}
-__device__ __forceinline__ uint32_t div(uint32_t n, const FastDiv& f) {
-    const uint64_t t = (uint64_t)__umulhi(n, f.m) + n;
-    return (uint32_t)(t >> f.s);
-}
-
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct PoolPtrs {

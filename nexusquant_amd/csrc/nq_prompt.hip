@@ -25,6 +25,7 @@ struct PromptArgs {
 
 constexpr int kWaitVm0 = 0x0f70;  // vmcnt(0), the other counters left open
 constexpr int kPromptRows = 128;
+constexpr int kStage = 64;        // keys of a stage: two tiles
 
 // Rows row0 .. row0 + 63 of one head to LDS in Tile's layout; rows past the sequence repeat its
 // last one (their weights are zero, and what lies behind the sequence is never read).
@@ -85,10 +86,10 @@ __device__ __forceinline__ void sum_again(Rows<DT, D>& rows, const uint16_t* kb,
 template <int DT, int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(PromptArgs a) {
     using T = Tile<D>;
-    __shared__ __align__(16) char k0[T::BYTES];
-    __shared__ __align__(16) char k1[T::BYTES];
-    __shared__ __align__(16) char v0[T::BYTES];
-    __shared__ __align__(16) char v1[T::BYTES];
+    __shared__ __align__(16) char k0[kStage * T::ROWB];
+    __shared__ __align__(16) char k1[kStage * T::ROWB];
+    __shared__ __align__(16) char v0[kStage * T::ROWB];
+    __shared__ __align__(16) char v1[kStage * T::ROWB];
     const int lane = threadIdx.x & 63, n = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     // kv heads fastest: blocks go to the XCDs in turn, so the query heads of a kv head meet in one
@@ -125,8 +126,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
         }
         if (live && key <= my_last) {
             const bool whole = key + kStage - 1 <= my0 && (!a.window || key > my_last - a.window);
-            if (whole) rows.stage(ck, cv, a.c);
-            else odd |= rows.stage_masked(ck, cv, a.c, a.window ? my_q - a.window + 1 - key : 0, my_q + 1 - key, lane);
+            if (whole) {
+                rows.two_tiles(ck, cv, 0, a.c);
+            } else {
+                int lo = a.window ? my_q - a.window + 1 - key : 0, hi = my_q + 1 - key;
+#pragma unroll 1
+                for (int t = 0; t < 2; ++t, lo -= 32, hi -= 32) {
+                    if (!__any(lo < 32 && hi > 0)) continue;
+                    rows.masked_tile(ck, cv, t, a.c, lo, hi, g);
+                    odd |= rows.tile_odd(cv, t, lane);
+                }
+            }
         }
         __builtin_amdgcn_s_waitcnt(kWaitVm0);
         __syncthreads();

@@ -117,6 +117,16 @@ __device__ __forceinline__ void store_rows16(uint8_t* dst, uint32_t n_rows, cons
 
 typedef __fp16 half2v __attribute__((ext_vector_type(2)));
 
+// Four int8 codes (one dword) -> two fp16 pairs, exactly.  XOR 0x80 biases
+// the byte to c + 128; v_perm places it under the fp16 exponent of 1024
+// (0x64 high byte), giving 1024 + c + 128, and one packed add removes 1152.
+__device__ __forceinline__ void codes_to_f16(uint32_t w, half2v& lo, half2v& hi) {
+    const uint32_t u = w ^ 0x80808080u;
+    const half2v bias = {(__fp16)-1152.0f, (__fp16)-1152.0f};
+    lo = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(u, 0x64646464u, 0x00050004u)) + bias;
+    hi = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(u, 0x64646464u, 0x00070006u)) + bias;
+}
+
 // A device address as a pointer the compiler knows to be global memory (it is
 // made in the global address space, then cast to a generic pointer, which
 // address-space inference folds back): accesses through it compile to global

@@ -1,0 +1,441 @@
+// Decode attention over a pool's pages for rows that share pages: what several rows begin
+// with is read and decoded once for all of them.
+//
+// The host cuts the rows' tokens into segments: a run of pages and the batch rows that see
+// all its tokens (a shared prefix: many rows; a row's own rest: one).  A workgroup of 4 waves
+// takes a chunk of a segment's tokens, one kv head, and up to 128 of the segment's query rows
+// (batch rows x the kv head's query heads).  Stage by stage (128 tokens) it
+//  1. decodes keys and values into LDS as fp16, all waves together: keys through the int8
+//     matrix cores (nq_keymfma.h), scaled and rotated in fp32; values as codes times their scale, without the transform: it is linear, and the combine kernel
+//     applies it once to a row's sum;
+//  2. attends (nq_flash.h): with more than 64 query rows each wave has 32 of them and all four
+//     tiles of the stage; with up to 64 two waves, with up to 32 four waves share 32 rows and
+//     take the stage's tiles in turn, and their sums are joined in LDS at the end.
+// A partial (maximum, sum, value sum) per query row and chunk goes to the workspace; the
+// combine kernel joins a row's chunks.
+#include "nq_flash.h"
+#include "nq_keymfma.h"
+#include "nq_rowmath.h"
+
+namespace nq {
+
+using namespace flash;
+
+constexpr int kSharedStage = 128;   // tokens
+constexpr int kSharedChunk = 1024;  // most tokens of a chunk: their places and scales stay in LDS
+constexpr int kSharedRows = 128;    // query rows of a workgroup
+
+struct SharedArgs {
+    const uint16_t* query;
+    void* out;
+    const int8_t* kc;
+    const int8_t* vc;
+    const uint16_t* ks;
+    const uint16_t* vs;
+    const int32_t* positions;
+    const int32_t* items;     // [n_items * 8]: pages, first token, tokens, rows, batch rows, chunk
+    const int32_t* pages;     // the segments' page numbers
+    const int32_t* seg_rows;  // per segment and row: batch row, its first slot there
+    const int32_t* row_slots; // [batch + 1]
+    float* part_y;            // [slots, q_heads, D]
+    float* part_ml;           // [slots, q_heads, 2]
+    const float* rope_dm;
+    const float* rope_dp;
+    uint32_t q_heads, kv_heads, rope_n_pos, n_items, tokens;
+    FastDiv by_tokens, by_group;
+    float c;                  // log2(e) / scale_divisor
+    float hscale;
+};
+
+// fp16 queries of a row, and the power of two taken out of them: bf16 ones are scaled so that the
+// row's largest is in [2^14, 2^15), where all of it that counts is exact in fp16 (8 bits of 11; what
+// falls below 2^-24 is 2^-38 of the largest).
+template <int D, int QDT>
+__device__ __forceinline__ float load_query(const uint16_t* p, u32x4 (&q)[Tile<D>::KS]) {
+    constexpr int KS = Tile<D>::KS;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) q[i] = *reinterpret_cast<const u32x4*>(p + 16 * i);
+    if constexpr (QDT == NQ_F16) return 1.0f;
+    float big = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t w = q[i][k];
+            big = __builtin_fmaxf(big, __builtin_fmaxf(__builtin_fabsf(bf16_bits_to_f32(w & 0xffffu)),
+                                                       __builtin_fabsf(bf16_bits_to_f32(w >> 16))));
+        }
+    big = both_max(big);
+    int e = 0;
+    if (big > 0.0f && big < __builtin_inff()) (void)__builtin_frexpf(big, &e);
+    e -= 15;
+    const float f = __builtin_ldexpf(1.0f, -e < 126 ? -e : 126);  // bf16's subnormals: scaled as far as fp32 reaches
+    if (-e > 126) e = -126;
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t w = q[i][k];
+            q[i][k] = pack2<NQ_F16>(bf16_bits_to_f32(w & 0xffffu) * f, bf16_bits_to_f32(w >> 16) * f);
+        }
+    return __builtin_ldexpf(1.0f, e);
+}
+
+template <int D, int QDT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void shared_attn_kernel(SharedArgs a) {
+    using T = Tile<D>;
+    using KM = KeyMfma<D>;
+    constexpr int ROWB = T::ROWB;
+    __shared__ __align__(16) char s_kv[2 * kSharedStage * ROWB];  // keys, values; at the end the waves' sums
+    __shared__ uint32_t s_row[kSharedChunk];    // a token's row of head 0
+    __shared__ uint32_t s_pos[kSharedChunk];    // its rotation table row
+    __shared__ uint32_t s_scale[kSharedChunk];  // its key scale, and its value scale times 2^vexp (fp16)
+    __shared__ float s_max[4], s_m[4][32], s_l[4][32];
+    char* const kbuf = s_kv;
+    char* const vbuf = s_kv + kSharedStage * ROWB;
+
+    const int lane = threadIdx.x & 63, n = lane & 31, g = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    // block 8 i + x runs on XCD x: the kv heads of an item there, one after another, share its rows of
+    // the rotation table in that XCD's L2 (the host puts items of one chunk 8 apart, for its codes)
+    const uint32_t in_xcd = blockIdx.x >> 3, item = (blockIdx.x & 7u) + 8u * (in_xcd / a.kv_heads), kh = in_xcd % a.kv_heads;
+    if (item >= a.n_items) return;  // whole block
+    const int32_t* const it = a.items + 8 * item;
+    const int32_t* const pages = a.pages + it[0];
+    const uint32_t tok0 = (uint32_t)it[1];
+    const int n_tok = it[2];
+    const int32_t* const seg_rows = a.seg_rows + 2 * it[3];
+    const int G = (int)(a.q_heads / a.kv_heads), n_q = it[4] * G, chunk = it[5];
+
+    // ---- the chunk's tokens ----
+    float vmax = 0.0f;
+    const uint32_t head_rows = kh * a.tokens;
+    for (int i = threadIdx.x; i < n_tok; i += 256) {
+        const uint32_t t = tok0 + i, p = div(t, a.by_tokens), off = t - p * a.tokens;
+        const uint32_t page = (uint32_t)pages[p];
+        const uint32_t row = page * a.kv_heads * a.tokens + head_rows + off;
+        const int32_t pos = a.positions[page * a.tokens + off];
+        const uint32_t vs = a.vs[row];
+        s_row[i] = row;
+        s_pos[i] = pos < 0 ? 0u : ((uint32_t)pos >= a.rope_n_pos ? a.rope_n_pos - 1u : (uint32_t)pos);
+        s_scale[i] = a.ks[row] | vs << 16;
+        vmax = __builtin_fmaxf(vmax, __builtin_fabsf(f16_bits_to_f32(vs)));
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) vmax = __builtin_fmaxf(vmax, __shfl_xor(vmax, o, 64));
+    if (lane == 0) s_max[wave] = vmax;
+
+    // ---- this wave's queries ----
+    const int rw = n_q <= 32 ? 1 : n_q <= 64 ? 2 : 4;   // waves with rows of their own
+    const int r0 = 32 * (wave % rw), tile0 = wave / rw * rw;
+    const bool live = r0 < n_q;
+    Rows<NQ_F16, D> rows;
+    rows.init(lane);
+    float c = a.c;
+    {
+        const uint32_t r = (uint32_t)min(r0 + n, n_q - 1), br = div(r, a.by_group);
+        const uint32_t head = kh * G + (r - br * G);
+        c *= load_query<D, QDT>(a.query + ((size_t)(uint32_t)seg_rows[2 * br] * a.q_heads + head) * D + 8 * g, rows.q);
+    }
+    KM km;
+    km.init(lane);
+    __syncthreads();
+    // Values in fp16: the chunk's scales times 2^vexp, the largest then in [128, 256): a value of codes
+    // up to 128 stays below 2^15, and one keeps its 11 bits down to 2^-21 of the largest scale.
+    int vexp = 0;
+    {
+        const float m = __builtin_fmaxf(__builtin_fmaxf(s_max[0], s_max[1]), __builtin_fmaxf(s_max[2], s_max[3]));
+        if (m > 0.0f && m < __builtin_inff()) {
+            (void)__builtin_frexpf(m, &vexp);
+            vexp = 8 - vexp;
+        }
+    }
+    for (int i = threadIdx.x; i < n_tok; i += 256) {
+        const uint32_t w = s_scale[i];
+        s_scale[i] = (w & 0xffffu) | f32_to_f16_bits(__builtin_ldexpf(f16_bits_to_f32(w >> 16), vexp)) << 16;
+    }
+    __syncthreads();
+
+    const int n16 = lane & 15, kg = lane >> 4, quad = lane >> 2, qq = lane & 3;
+    const int from_quad = 4 * (4 * n16 + kg);  // byte address of the lane that loaded this lane's block
+    auto permute = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_ds_bpermute(from_quad, (int)v); };
+    auto permute_f = [&](float v) { return __builtin_bit_cast(float, permute(__builtin_bit_cast(uint32_t, v))); };
+
+    for (int s0 = 0; s0 < n_tok; s0 += kSharedStage) {
+        const int left = min(n_tok - s0, kSharedStage);
+        const int units = 2 * ((left + 31) / 32);  // whole tiles: slots past the chunk repeat its last token
+        // ---- 1. keys: 16 tokens (a unit) of a wave at a time ----
+        for (int u = wave; u < units; u += 4) {
+            const int tq = min(s0 + 16 * u + quad, n_tok - 1), tn = min(s0 + 16 * u + n16, n_tok - 1);
+            uint32_t code[2][KM::NK][KM::W];
+            {
+                const int8_t* const p = a.kc + (size_t)s_row[tq] * D + KM::KPL * qq;
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                    for (int s = 0; s < KM::NK; ++s) {
+                        const uint32_t* const w = reinterpret_cast<const uint32_t*>(p + hf * KM::HALF + s * KM::KB);
+#pragma unroll
+                        for (int i = 0; i < KM::W; ++i) code[hf][s][i] = w[i];
+                    }
+            }
+            const size_t tab = (size_t)s_pos[tq] * (D / 2) + 4 * qq;
+            const float k_scale = (0.5f * f16_bits_to_f32(s_scale[tn] & 0xffffu)) * a.hscale;
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                for (int s = 0; s < KM::NK; ++s)
+#pragma unroll
+                    for (int i = 0; i < KM::W; ++i) code[hf][s][i] = permute(code[hf][s][i]);
+            const int row = 16 * u + n16;
+            char* const to = kbuf + row * ROWB + 8 * (kg & 1);
+#pragma unroll
+            for (int t = 0; t < KM::T; ++t) {
+                const f32x4 tm = *reinterpret_cast<const f32x4*>(a.rope_dm + tab + 16 * t);
+                const f32x4 tp = *reinterpret_cast<const f32x4*>(a.rope_dp + tab + 16 * t);
+                int4v y0 = {0, 0, 0, 0}, y1 = {0, 0, 0, 0};
+#pragma unroll
+                for (int s = 0; s < KM::NK; ++s) {
+                    y0 = km.mul(t, s, lane, code[0][s], y0);
+                    y1 = km.mul(t, s, lane, code[1][s], y1);
+                }
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float m = permute_f(tm[i]), p = permute_f(tp[i]);
+                    const float lo = (float)y0[i] * k_scale, hi = (float)y1[i] * k_scale;
+                    x[i] = __builtin_fmaf(-lo, m, hi * p);
+                    x[4 + i] = __builtin_fmaf(lo, p, hi * m);
+                }
+                // coordinates 16 t + 4 kg + 0..3 and those D / 2 on: half a 16-byte chunk each
+                const int chunk16 = 2 * t + (kg >> 1), f = T::key_swizzle(row);
+                *reinterpret_cast<u32x2*>(to + 16 * (chunk16 ^ f)) = u32x2{pack2<NQ_F16>(x[0], x[1]), pack2<NQ_F16>(x[2], x[3])};
+                *reinterpret_cast<u32x2*>(to + 16 * ((chunk16 + D / 16) ^ f)) =
+                    u32x2{pack2<NQ_F16>(x[4], x[5]), pack2<NQ_F16>(x[6], x[7])};
+            }
+        }
+        // ---- values: 16 codes of a token a lane ----
+        for (int i = threadIdx.x; i < 16 * units * (D / 16); i += 256) {
+            const int row = i / (D / 16), piece = i % (D / 16);
+            const int t = min(s0 + row, n_tok - 1);
+            const u32x4 w = *reinterpret_cast<const u32x4*>(a.vc + (size_t)s_row[t] * D + 16 * piece);
+            const uint32_t sc = s0 + row < n_tok ? s_scale[t] >> 16 : 0u;
+            const half2v s = __builtin_bit_cast(half2v, sc | sc << 16);
+            u32x4 o[2];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                half2v lo, hi;
+                codes_to_f16(w[k], lo, hi);
+                lo *= s;
+                hi *= s;
+                o[k / 2][2 * (k & 1)] = __builtin_bit_cast(uint32_t, lo);
+                o[k / 2][2 * (k & 1) + 1] = __builtin_bit_cast(uint32_t, hi);
+            }
+            const int f = T::value_swizzle(row);
+            *reinterpret_cast<u32x4*>(vbuf + row * ROWB + 16 * ((2 * piece) ^ f)) = o[0];
+            *reinterpret_cast<u32x4*>(vbuf + row * ROWB + 16 * ((2 * piece + 1) ^ f)) = o[1];
+        }
+        __syncthreads();
+        // ---- 2. attention ----
+        if (live) {
+            const int t1 = min(tile0 + rw, units / 2);
+            int t = tile0;
+#pragma unroll 1
+            for (; t + 1 < t1 && 32 * (t + 2) <= left; t += 2) rows.two_tiles(kbuf, vbuf, t, c);
+#pragma unroll 1
+            for (; t < t1; ++t) rows.masked_tile(kbuf, vbuf, t, c, 0, left - 32 * t, g);
+        }
+        __syncthreads();
+    }
+
+    // ---- the waves' sums joined, and written ----
+    const float lsum = both_sum(rows.l);
+    if (g == 0) {
+        s_m[wave][n] = rows.m;
+        s_l[wave][n] = lsum;
+    }
+    __syncthreads();
+    {
+        float m = kNoMax;
+        for (int w = wave % rw; w < 4; w += rw) m = __builtin_fmaxf(m, s_m[w][n]);
+        const float f = __builtin_ldexpf(__builtin_amdgcn_exp2f(rows.m - m), -1 - vexp);
+        // [wave][query][coordinate], 16-byte chunks at chunk ^ query
+        float* const area = reinterpret_cast<float*>(s_kv) + (wave * 32 + n) * D;
+#pragma unroll
+        for (int b = 0; b < T::DB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = (8 * b + 2 * i + g) ^ (n & 15);
+                *reinterpret_cast<f32x4*>(area + 4 * at) = f32x4{rows.o[b][4 * i] * f, rows.o[b][4 * i + 1] * f,
+                                                                 rows.o[b][4 * i + 2] * f, rows.o[b][4 * i + 3] * f};
+            }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n_q * (D / 4); i += 256) {
+        const int r = i / (D / 4), at = i % (D / 4), w0 = r >> 5, q = r & 31;
+        f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = w0; w < 4; w += rw)
+            y += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(s_kv) + (w * 32 + q) * D + 4 * (at ^ (q & 15)));
+        const uint32_t br = div((uint32_t)r, a.by_group);
+        const size_t slot = (size_t)(uint32_t)(seg_rows[2 * br + 1] + chunk) * a.q_heads + kh * G + ((uint32_t)r - br * G);
+        *reinterpret_cast<f32x4*>(a.part_y + slot * D + 4 * at) = y;
+        if (at == 0) {
+            float m = kNoMax, l = 0.0f;
+            for (int w = w0; w < 4; w += rw) m = __builtin_fmaxf(m, s_m[w][q]);
+            for (int w = w0; w < 4; w += rw) l += s_l[w][q] * __builtin_amdgcn_exp2f(s_m[w][q] - m);
+            a.part_ml[2 * slot] = m;
+            a.part_ml[2 * slot + 1] = l;
+        }
+    }
+}
+
+// One (row, query head) a workgroup: its chunks' sums weighted and added in a fixed order, then the
+// Walsh-Hadamard transform, h_D and the softmax's sum.
+template <int D, int QDT>
+__global__ __launch_bounds__(256) void shared_combine_kernel(SharedArgs a) {
+    constexpr int V = D / 4, NG = 256 / V;  // lanes of a chunk's row, chunks at a time
+    __shared__ f32x4 s_y[NG][V];
+    __shared__ float s_l[NG], s_x[D], s_mw[4];
+    const uint32_t row = blockIdx.x / a.q_heads, head = blockIdx.x % a.q_heads;
+    const int c0 = a.row_slots[row], c1 = a.row_slots[row + 1];
+    const int tid = threadIdx.x, grp = tid / V, at = tid % V;
+    float m = kNoMax;
+    for (int s = c0 + tid; s < c1; s += 256) m = __builtin_fmaxf(m, a.part_ml[2 * ((size_t)s * a.q_heads + head)]);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, o, 64));
+    if ((tid & 63) == 0) s_mw[tid >> 6] = m;
+    __syncthreads();
+    m = __builtin_fmaxf(__builtin_fmaxf(s_mw[0], s_mw[1]), __builtin_fmaxf(s_mw[2], s_mw[3]));
+    f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f;
+#pragma unroll 4
+    for (int s = c0 + grp; s < c1; s += NG) {
+        const size_t i = (size_t)s * a.q_heads + head;
+        const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * i] - m);
+        l = __builtin_fmaf(f, a.part_ml[2 * i + 1], l);
+        const f32x4 p = *reinterpret_cast<const f32x4*>(a.part_y + i * D + 4 * at);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] = __builtin_fmaf(f, p[k], y[k]);
+    }
+    s_y[grp][at] = y;
+    if (at == 0) s_l[grp] = l;
+    __syncthreads();
+    if (grp == 0) {
+        for (int i = 1; i < NG; ++i) y += s_y[i][at];
+        const float p0 = y[0] + y[1], p1 = y[0] - y[1], p2 = y[2] + y[3], p3 = y[2] - y[3];
+        *reinterpret_cast<f32x4*>(&s_x[4 * at]) = f32x4{p0 + p2, p1 + p3, p0 - p2, p1 - p3};
+    }
+    __syncthreads();
+#pragma unroll
+    for (int len = 4; len < D; len <<= 1) {
+        if (tid < D / 2) {
+            const int i = (tid / len) * 2 * len + tid % len;
+            const float x0 = s_x[i], x1 = s_x[i + len];
+            s_x[i] = x0 + x1;
+            s_x[i + len] = x0 - x1;
+        }
+        __syncthreads();
+    }
+    if (tid >= D) return;
+    l = s_l[0];
+    for (int i = 1; i < NG; ++i) l += s_l[i];
+    const float v = c1 > c0 ? s_x[tid] * a.hscale / l : 0.0f;  // a row without tokens is zero
+    static_cast<uint16_t*>(a.out)[(size_t)blockIdx.x * D + tid] = (uint16_t)(pack2<QDT>(v, 0.0f) & 0xffffu);
+}
+
+template <int D, int QDT>
+static hipError_t launch_shared(const SharedArgs& a, uint32_t batch, hipStream_t s) {
+    if (a.n_items > 0) {
+        hipLaunchKernelGGL((shared_attn_kernel<D, QDT>), dim3((a.n_items + 7u) / 8u * 8u * a.kv_heads), dim3(256), 0, s, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL((shared_combine_kernel<D, QDT>), dim3(batch * a.q_heads), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+template <int QDT>
+static hipError_t shared_dims(int32_t d, const SharedArgs& a, uint32_t batch, hipStream_t s) {
+    switch (d) {
+        case 64: return launch_shared<64, QDT>(a, batch, s);
+        case 128: return launch_shared<128, QDT>(a, batch, s);
+        default: return launch_shared<256, QDT>(a, batch, s);
+    }
+}
+
+}  // namespace nq
+
+extern "C" int32_t nq_shared_attention_chunk_tokens(void) { return nq::kSharedChunk; }
+extern "C" int32_t nq_shared_attention_rows(void) { return nq::kSharedRows; }
+
+extern "C" int64_t nq_shared_attention_workspace(int32_t n_slots, int32_t q_heads, int32_t head_dim) {
+    if (n_slots <= 0 || q_heads <= 0 || head_dim <= 0) return 0;
+    return (int64_t)n_slots * q_heads * (head_dim + 2) * (int64_t)sizeof(float);
+}
+
+extern "C" int nq_shared_attention(const nq_shared_desc* d, void* stream) {
+    using namespace nq;
+    NQ_CHECK_ARG(d != nullptr && d->pool != nullptr, "nq_shared_attention: desc and pool are required");
+    const nq_pool* p = d->pool;
+    NQ_CHECK_ARG(p->head_dim == 64 || p->head_dim == 128 || p->head_dim == 256,
+                 "nq_shared_attention: head_dim %d unsupported (64, 128, 256)", p->head_dim);
+    NQ_CHECK_ARG(p->layers > 0 && p->pages > 0 && p->heads > 0 && p->tokens > 0 && d->layer >= 0 && d->layer < p->layers,
+                 "nq_shared_attention: bad pool geometry, or layer %d of %d", d->layer, p->layers);
+    NQ_CHECK_ARG((uint64_t)p->pages * p->heads * p->tokens < (1ull << 31),
+                 "nq_shared_attention: a layer must have less than 2^31 token rows");
+    NQ_CHECK_ARG(d->q_dtype == NQ_F16 || d->q_dtype == NQ_BF16, "nq_shared_attention: queries must be fp16 or bf16");
+    NQ_CHECK_ARG(d->batch >= 0 && d->q_heads > 0 && d->q_heads % p->heads == 0 && d->q_heads / p->heads <= kSharedRows,
+                 "nq_shared_attention: q_heads %d must be a multiple of the pool's %d heads, at most %d times", d->q_heads,
+                 p->heads, kSharedRows);
+    NQ_CHECK_ARG(d->n_items >= 0 && d->n_slots >= 0, "nq_shared_attention: n_items %d, n_slots %d", d->n_items, d->n_slots);
+    if (d->batch == 0) return NQ_OK;
+    NQ_CHECK_ARG(d->query && d->out && d->row_slots, "nq_shared_attention: query, out and row_slots are required");
+    NQ_CHECK_ARG(((uintptr_t)d->query & 15u) == 0, "nq_shared_attention: query must be 16-byte aligned");
+    NQ_CHECK_ARG((uint64_t)d->batch * d->q_heads <= max_blocks(256) &&
+                     ((uint64_t)d->n_items + 7) * p->heads <= max_blocks(256), "nq_shared_attention: grid too large");
+    SharedArgs a = {};
+    if (d->n_items > 0) {
+        NQ_CHECK_ARG(d->items && d->pages && d->seg_rows, "nq_shared_attention: the plan's arrays are required");
+        NQ_CHECK_ARG(p->key_codes && p->value_codes && p->key_scales && p->value_scales && p->positions,
+                     "nq_shared_attention: the pool's arrays are required");
+        NQ_CHECK_ARG((((uintptr_t)p->key_codes | (uintptr_t)p->value_codes | (uintptr_t)p->key_scales |
+                       (uintptr_t)p->value_scales) & 15u) == 0 && ((uintptr_t)p->positions & 3u) == 0,
+                     "nq_shared_attention: the pool's codes and scales must be 16-byte aligned");
+        NQ_CHECK_ARG(d->rope_sin_minus_cos && d->rope_cos_plus_sin && d->rope_n_pos > 0 && d->rope_n_pos < (1ll << 31),
+                     "nq_shared_attention: keys need RoPE tables");
+        const int64_t need = nq_shared_attention_workspace(d->n_slots, d->q_heads, p->head_dim);
+        NQ_CHECK_ARG(d->n_slots > 0 && d->workspace != nullptr && d->workspace_bytes >= need &&
+                         ((uintptr_t)d->workspace & 15u) == 0,
+                     "nq_shared_attention: a 16-byte aligned workspace of %lld bytes is needed", (long long)need);
+        NQ_CHECK_ARG(d->scale_divisor > 0.0f, "nq_shared_attention: scale_divisor must be positive");
+    }
+    const size_t rows = (size_t)d->layer * p->pages * p->heads * p->tokens;
+    a.query = static_cast<const uint16_t*>(d->query);
+    a.out = d->out;
+    a.kc = p->key_codes + rows * p->head_dim;
+    a.vc = p->value_codes + rows * p->head_dim;
+    a.ks = static_cast<const uint16_t*>(p->key_scales) + rows;
+    a.vs = static_cast<const uint16_t*>(p->value_scales) + rows;
+    a.positions = p->positions;
+    a.items = d->items;
+    a.pages = d->pages;
+    a.seg_rows = d->seg_rows;
+    a.row_slots = d->row_slots;
+    a.part_y = static_cast<float*>(d->workspace);
+    a.part_ml = a.part_y + (size_t)d->n_slots * d->q_heads * p->head_dim;
+    a.rope_dm = d->rope_sin_minus_cos;
+    a.rope_dp = d->rope_cos_plus_sin;
+    a.q_heads = (uint32_t)d->q_heads;
+    a.kv_heads = (uint32_t)p->heads;
+    a.rope_n_pos = (uint32_t)(d->rope_n_pos > 0 ? d->rope_n_pos : 1);
+    a.n_items = (uint32_t)d->n_items;
+    a.tokens = (uint32_t)p->tokens;
+    a.by_tokens = fast_div(a.tokens);
+    a.by_group = fast_div(a.q_heads / a.kv_heads);
+    a.c = 1.44269504088896340736f / (d->scale_divisor > 0.0f ? d->scale_divisor : 1.0f);
+    a.hscale = d->hadamard_scale;
+    hipStream_t s = (hipStream_t)stream;
+    NQ_CHECK_HIP(d->q_dtype == NQ_F16 ? shared_dims<NQ_F16>(p->head_dim, a, (uint32_t)d->batch, s)
+                                      : shared_dims<NQ_BF16>(p->head_dim, a, (uint32_t)d->batch, s));
+    return NQ_OK;
+}

@@ -7,6 +7,7 @@ import threading
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence, Tuple
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -166,6 +167,35 @@ def _addr(t):
     if t is None:
         return None
     return ctypes.c_void_p(t if isinstance(t, int) else t.data_ptr())
+
+
+def to_device(values: np.ndarray, device) -> torch.Tensor:
+    """int32 values on the device, by way of pinned memory: the copy waits for nothing."""
+    host = torch.empty(len(values), dtype=torch.int32, pin_memory=True)
+    host.numpy()[:] = values
+    return host.to(device, non_blocking=True)
+
+
+class PlanTensor:
+    """A plan's int32 array on the device, for launches on any stream: the first ones on another stream than
+    the one it was copied on wait for the copy, and the array's memory is kept until they have run.  A graph's
+    capture relies on the device having been synchronized since the plan was made (torch.cuda.graph does)."""
+
+    def __init__(self, values: np.ndarray, device):
+        self.device = torch.device(device)
+        with torch.cuda.device(self.device):
+            self.tensor = to_device(values, self.device)
+            self._stream = torch.cuda.current_stream(self.device)
+            self._copied = torch.cuda.Event()
+            self._copied.record(self._stream)
+
+    def address(self) -> int:
+        """For a launch on the device's current stream."""
+        if _lib.current_stream_handle(self.device) != self._stream.cuda_stream and not torch.cuda.is_current_stream_capturing():
+            stream = torch.cuda.current_stream(self.device)
+            stream.wait_event(self._copied)
+            self.tensor.record_stream(stream)
+        return self.tensor.data_ptr()
 
 
 _workspaces: Dict[Tuple[int, int], torch.Tensor] = {}

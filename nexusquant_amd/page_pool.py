@@ -28,18 +28,11 @@ import numpy as np
 import torch
 
 from . import _lib
-from .ops import _addr
+from .ops import _addr, to_device
 from .vllm_backend import CompressedPage
 
 _HEAD_DIMS = (64, 128, 256)
 _FIELDS = ("key_codes", "value_codes", "key_scales", "value_scales", "positions")
-
-
-def to_device(values: np.ndarray, device) -> torch.Tensor:
-    """int32 values on the device, by way of pinned memory: the copy waits for nothing."""
-    host = torch.empty(len(values), dtype=torch.int32, pin_memory=True)
-    host.numpy()[:] = values
-    return host.to(device, non_blocking=True)
 
 
 def _refuse_capture(what: str) -> None:
@@ -123,7 +116,7 @@ class CompressedPagePool:
         self._stack = np.arange(self.num_pages - 1, -1, -1, dtype=np.int32)  # free pages, the next one last
         self._free = self.num_pages
         self._lock = threading.RLock()
-        self._desc = _lib.Pool(layers=self.num_layers, pages=self.num_pages, heads=self.num_heads,
+        self.desc = _lib.Pool(layers=self.num_layers, pages=self.num_pages, heads=self.num_heads,
                                tokens=self.page_tokens, head_dim=self.head_dim, key_codes=_addr(key_codes),
                                value_codes=_addr(value_codes), key_scales=_addr(key_scales),
                                value_scales=_addr(value_scales), positions=_addr(positions))
@@ -152,7 +145,8 @@ class CompressedPagePool:
             raise ValueError(f"page numbers must lie in [0, {self.num_pages})")
         return p
 
-    def _in_use(self, pages, what: str) -> np.ndarray:
+    def in_use(self, pages, what: str = "pages") -> np.ndarray:
+        """The page numbers as an array; raises unless all are allocated."""
         p = self._pages(pages)
         if len(p) and self._refs[p].min() < 1:
             raise ValueError(f"{what}: page {int(p[self._refs[p] < 1][0])} is not allocated")
@@ -182,14 +176,14 @@ class CompressedPagePool:
     def retain(self, pages: Sequence[int]) -> None:
         """One more reference to each page (to a page listed twice: two)."""
         with self._lock:
-            p, n = self._tally(self._in_use(pages, "retain"))
+            p, n = self._tally(self.in_use(pages, "retain"))
             self._refs[p] += n.astype(np.int32)
 
     def free(self, pages: Sequence[int]) -> None:
         """Drop one reference of each page (of a page listed twice: two); pages without any can be
         allocated again.  Work already queued on the pool's stream still sees them as they were."""
         with self._lock:
-            p, n = self._tally(self._in_use(pages, "free"))
+            p, n = self._tally(self.in_use(pages, "free"))
             left = self._refs[p] - n.astype(np.int32)
             if len(p) and left.min() < 0:
                 raise ValueError(f"page {int(p[left < 0][0])} is freed more often than it is referenced")
@@ -205,7 +199,7 @@ class CompressedPagePool:
         dst = np.ascontiguousarray(dst, dtype=np.int32)
         lib = _lib.load()
         with torch.cuda.device(self.device):
-            st = lib.nq_pool_copy_pages(ctypes.byref(self._desc), src.ctypes.data, dst.ctypes.data, len(src),
+            st = lib.nq_pool_copy_pages(ctypes.byref(self.desc), src.ctypes.data, dst.ctypes.data, len(src),
                                         ctypes.c_void_p(_lib.current_stream_handle(self.device)))
         _lib.check(st, "nq_pool_copy_pages")
 
@@ -215,7 +209,7 @@ class CompressedPagePool:
         A page may be read any number of times, written once, and not both; a page with more
         than one reference is not written (its other holders would see it change)."""
         with self._lock:
-            s, d = self._in_use(src, "copy_pages"), self._in_use(dst, "copy_pages")
+            s, d = self.in_use(src, "copy_pages"), self.in_use(dst, "copy_pages")
             if len(s) != len(d):
                 raise ValueError(f"{len(s)} source pages for {len(d)} destinations")
             if len(d) and self._refs[d].max() > 1:
@@ -223,7 +217,7 @@ class CompressedPagePool:
             self._copy(s, d)
 
     def _sequence(self, pages, length: int, what: str) -> Tuple[np.ndarray, int]:
-        p, length = self._in_use(pages, what), int(length)
+        p, length = self.in_use(pages, what), int(length)
         if length < 0 or self.pages_for(length) != len(p):
             raise ValueError(f"{what}: {length} tokens take {self.pages_for(max(length, 0))} pages, got {len(p)}")
         if len(self._tally(p)[0]) != len(p):
@@ -306,7 +300,7 @@ class CompressedPagePool:
                     plan = to_device(np.concatenate([np.repeat(np.arange(batch), tiles), seq, flat, new]), self.device)
                     base = plan.data_ptr()
                     with torch.cuda.device(self.device):
-                        st = lib.nq_pool_compact(ctypes.byref(self._desc), base, n_tiles, base + 4 * n_tiles,
+                        st = lib.nq_pool_compact(ctypes.byref(self.desc), base, n_tiles, base + 4 * n_tiles,
                                                  base + 4 * (n_tiles + len(seq)), _addr(idx), idx.shape[1],
                                                  int(bool(renumber)),
                                                  ctypes.c_void_p(_lib.current_stream_handle(self.device)))
@@ -356,7 +350,7 @@ class CompressedPagePool:
         if n == 0:
             return
         with self._lock:
-            p = self._in_use(np.unique(used // self.page_tokens), "write")
+            p = self.in_use(np.unique(used // self.page_tokens), "write")
             if len(p) and self._refs[p].max() > 1:
                 raise ValueError(f"write: page {int(p[self._refs[p] > 1][0])} is shared and cannot be written")
             with torch.cuda.device(self.device):
@@ -366,7 +360,7 @@ class CompressedPagePool:
                                    key_codes=_addr(page.key_codes), value_codes=_addr(page.value_codes),
                                    key_scales=_addr(page.key_scales), value_scales=_addr(page.value_scales),
                                    positions=_addr(page.positions))
-                st = lib.nq_pool_write(ctypes.byref(self._desc), int(layer), ctypes.byref(tokens), _addr(where), n,
+                st = lib.nq_pool_write(ctypes.byref(self.desc), int(layer), ctypes.byref(tokens), _addr(where), n,
                                        ctypes.c_void_p(_lib.current_stream_handle(self.device)))
             _lib.check(st, "nq_pool_write")
             self.max_position = max(self.max_position, page.max_position or 0)
@@ -374,7 +368,7 @@ class CompressedPagePool:
     def page(self, page: int, layer: int = 0) -> CompressedPage:
         """One page of a layer as a CompressedPage of page_tokens tokens (views, no copy), for
         NexusQuantKVCompressor and NexusQuantPagedAttention.plan."""
-        i = int(self._in_use([page], "page")[0])
+        i = int(self.in_use([page], "page")[0])
         return CompressedPage(key_codes=self.key_codes[layer, i], value_codes=self.value_codes[layer, i],
                               key_scales=self.key_scales[layer, i], value_scales=self.value_scales[layer, i],
                               positions=self.positions[i], num_valid=self.page_tokens, max_position=self.max_position)

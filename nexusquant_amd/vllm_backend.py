@@ -27,7 +27,7 @@ import torch
 
 from . import _lib
 from .hadamard import hadamard_constant
-from .ops import _addr, _PtrArrays
+from .ops import PlanTensor, _addr, _PtrArrays
 from .rope import device_merged_table, device_table
 
 _FP16_BYTES = 2
@@ -461,6 +461,134 @@ class PagedAttentionPlan:
     tokens: int                        # tokens attended over all rows
 
 
+# A segment is shared when that saves at least this many tokens' decoding (its tokens, once for
+# every row but one).
+_MIN_SHARED = 256
+
+
+def shared_segments(tables: Sequence[np.ndarray], lengths: Sequence[int], page_tokens: int,
+                    min_saved: int = _MIN_SHARED) -> List[Tuple[List[int], np.ndarray, int]]:
+    """Cut the rows' tokens into segments (rows, pages, tokens) that their rows see whole.
+
+    tables[b]: row b's pages, lengths[b]: its tokens.  Rows that begin with the same full pages
+    share a segment of these, and those among them that go on alike another one, and so on; a
+    segment of one row is what it has for itself.  Sharing that would save less than min_saved
+    tokens is left to what follows it."""
+    full = [int(n) // page_tokens for n in lengths]
+    out: List[Tuple[List[int], np.ndarray, int]] = []
+
+    def split(rows: List[int], start: int, depth: int) -> None:
+        # the rows agree on their pages before `depth`; those from `start` on are in no segment yet
+        groups: Dict[int, List[int]] = {}
+        for b in rows:
+            if full[b] > depth:
+                groups.setdefault(int(tables[b][depth]), []).append(b)
+            elif lengths[b] > start * page_tokens:
+                out.append(([b], tables[b][start:], int(lengths[b]) - start * page_tokens))
+        for same in groups.values():
+            if len(same) == 1:
+                b = same[0]
+                out.append((same, tables[b][start:], int(lengths[b]) - start * page_tokens))
+                continue
+            most = min(full[b] for b in same)
+            stack = np.stack([tables[b][depth:most] for b in same])
+            differ = np.flatnonzero((stack != stack[0]).any(axis=0))
+            end = depth + int(differ[0]) if len(differ) else most
+            tokens = (end - start) * page_tokens
+            if (len(same) - 1) * tokens >= min_saved:
+                out.append((same, tables[same[0]][start:end], tokens))
+                split(same, end, end)
+            else:
+                split(same, start, end)
+
+    split([b for b in range(len(tables)) if lengths[b] > 0], 0, 0)
+    return out
+
+
+# Workgroups that a launch should have before its chunks stay long: two on each of 256 CUs.
+_SHARED_WORKGROUPS = 512
+_SHARED_STAGE = 128
+
+
+def shared_items(segments, batch: int, tile_rows: int, kv_heads: int, cap: int):
+    """The work list of nq_shared_attention: int32 arrays items, pages, seg_rows, row_slots, and the
+    counts of items and slots.  Chunks are `cap` tokens, halved down to one stage of 128 while the
+    launch would have fewer than _SHARED_WORKGROUPS workgroups."""
+    tiles = [-(-len(rows) // tile_rows) for rows, _, _ in segments]
+    length = cap
+    while length > _SHARED_STAGE and kv_heads * sum(
+            t * -(-n // length) for t, (_, _, n) in zip(tiles, segments)) < _SHARED_WORKGROUPS:
+        length //= 2
+    per_row = np.zeros(batch + 1, dtype=np.int64)
+    chunks = []
+    for rows, _, n in segments:
+        chunks.append(-(-n // length))
+        per_row[np.asarray(rows) + 1] += chunks[-1]
+    row_slots = np.cumsum(per_row)
+    nxt = row_slots[:-1].copy()
+    records, seg_rows, pages = [], [], []
+    at_rows = at_pages = 0
+    order = sorted(range(len(segments)), key=lambda i: -len(segments[i][0]))  # the dear ones first
+    for i in order:
+        rows, seg_pages, n = segments[i]
+        rows = np.asarray(rows)
+        seg_rows.append(np.stack([rows, nxt[rows]], axis=1))
+        nxt[rows] += chunks[i]
+        c = np.arange(chunks[i])
+        r0 = np.arange(tiles[i]) * tile_rows
+        # chunks in eights (one for each XCD), a chunk's row tiles one eight after another
+        cc, rr = np.repeat(c, tiles[i]), np.tile(r0, chunks[i])
+        by = np.lexsort((cc % 8, rr, cc // 8))
+        cc, rr = cc[by], rr[by]
+        rec = np.zeros((len(cc), 8), dtype=np.int64)
+        rec[:, 0] = at_pages
+        rec[:, 1] = cc * length
+        rec[:, 2] = np.minimum(n - cc * length, length)
+        rec[:, 3] = at_rows + rr
+        rec[:, 4] = np.minimum(len(rows) - rr, tile_rows)
+        rec[:, 5] = cc
+        records.append(rec)
+        pages.append(np.asarray(seg_pages))
+        at_rows += len(rows)
+        at_pages += len(seg_pages)
+    empty = np.zeros(0, dtype=np.int64)
+    items = np.concatenate(records).reshape(-1) if records else empty
+    parts = {"items": items, "pages": np.concatenate(pages) if pages else empty,
+             "seg_rows": np.concatenate(seg_rows).reshape(-1) if seg_rows else empty, "row_slots": row_slots}
+    return parts, len(items) // 8, int(row_slots[-1])
+
+
+class SharedAttentionPlan:
+    """Which tokens of a pool each batch row attends to, and which of them rows share: valid for every
+    layer of the pool while the rows' tables and lengths stay the same.  The device arrays are made for a
+    number of query heads, the first time that it is used (before a graph is captured)."""
+
+    def __init__(self, pool, batch: int, segments):
+        self.pool = pool
+        self.batch = batch
+        self.segments = segments
+        self._work: Dict[int, tuple] = {}
+
+    def work(self, q_heads: int):
+        """(device ints, offsets, items, slots) for q_heads query heads."""
+        got = self._work.get(q_heads)
+        if got is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("run_shared: run the plan once before capturing it into a graph")
+            lib = _lib.load()
+            group = q_heads // self.pool.num_heads
+            parts, n_items, n_slots = shared_items(self.segments, self.batch,
+                                                   int(lib.nq_shared_attention_rows()) // group, self.pool.num_heads,
+                                                   int(lib.nq_shared_attention_chunk_tokens()))
+            offsets, at = {}, 0
+            for name, v in parts.items():
+                offsets[name] = at
+                at += len(v)
+            ints = PlanTensor(np.concatenate(list(parts.values())), self.pool.device)
+            got = self._work[q_heads] = (ints, offsets, n_items, n_slots)
+        return got
+
+
 class NexusQuantPagedAttention:
     """Paged attention over compressed pages (vllm_backend.py:543-775)."""
 
@@ -615,6 +743,74 @@ class NexusQuantPagedAttention:
         with torch.cuda.device(dev):
             st = lib.nq_paged_attention(ctypes.byref(desc), _stream(dev))
         _lib.check(st, "nq_paged_attention")
+        return out
+
+    # ----------------------------------------------------- rows that share pages
+
+    def plan_shared(self, pool, block_tables: Sequence[Sequence[int]], context_lens) -> SharedAttentionPlan:
+        """The plan of rows over a CompressedPagePool: row b attends to the first context_lens[b] tokens of
+        its pages block_tables[b] (0: none).  Full pages that several rows begin with, as forks do, are
+        read and decoded once for all of them (shared_segments)."""
+        if pool.head_dim != self.compressor.head_dim:
+            raise ValueError(f"pool head_dim {pool.head_dim} != compressor head_dim {self.compressor.head_dim}")
+        ctx = [int(x) for x in (context_lens.tolist() if torch.is_tensor(context_lens) else context_lens)]
+        if len(ctx) != len(block_tables):
+            raise ValueError(f"{len(block_tables)} block tables for {len(ctx)} context lengths")
+        tables = []
+        for b, n in enumerate(ctx):
+            pages = pool.in_use(block_tables[b], "plan_shared")
+            if not 0 <= n <= len(pages) * pool.page_tokens:
+                raise ValueError(f"row {b}: {n} tokens in {len(pages)} pages of {pool.page_tokens}")
+            tables.append(pages[:pool.pages_for(n)])
+        return SharedAttentionPlan(pool, len(ctx), shared_segments(tables, ctx, pool.page_tokens))
+
+    def run_shared(self, plan: SharedAttentionPlan, query: torch.Tensor, layer: int = 0,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of query (batch, num_heads, head_dim; fp16 or bf16) over a shared plan's tokens in one
+        layer of its pool.  num_heads is a multiple of the pool's heads.  Rows without tokens are zero.
+
+        What a row sees is cut by all rows of the plan: outputs of one row alone and in a batch agree to
+        roundings, not bit for bit.  run() differs in its roundings too (values there are not rounded)."""
+        lib = _lib.load()
+        pool = plan.pool
+        _lib.require_device(query, "query")
+        if query.device != pool.device:
+            raise ValueError(f"query is on {query.device}, the pool on {pool.device}")
+        if query.dim() != 3 or query.shape[0] != plan.batch or query.shape[2] != pool.head_dim:
+            raise ValueError(f"query must be (batch={plan.batch}, num_heads, head_dim={pool.head_dim}), got "
+                             f"{tuple(query.shape)}")
+        if query.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"run_shared takes fp16 or bf16 queries, got {query.dtype}; run() takes fp32 ones")
+        b, hq, d = query.shape
+        rows = int(lib.nq_shared_attention_rows())
+        if hq == 0 or hq % pool.num_heads or hq // pool.num_heads > rows:
+            raise ValueError(f"num_heads {hq} is not a multiple (up to {rows}) of the pool's {pool.num_heads}")
+        if not 0 <= int(layer) < pool.num_layers:
+            raise ValueError(f"layer {layer} of a pool of {pool.num_layers}")
+        if out is None:
+            out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+        elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {query.dtype} tensor {tuple(query.shape)} on {query.device}")
+        q = query.contiguous()
+        if q.data_ptr() % 16:
+            q = q.clone()
+        dev = pool.device
+        with torch.cuda.device(dev):
+            ints, offsets, n_items, n_slots = plan.work(hq)
+            nbytes = lib.nq_shared_attention_workspace(n_slots, hq, d)
+            # of this call alone: calls on other streams and captured graphs have their own
+            ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+            _, _, dm, dp = self.compressor._tables(pool.max_position, dev)
+            base = ints.address()
+            desc = _lib.SharedDesc(
+                pool=ctypes.pointer(pool.desc), layer=int(layer), batch=b, q_heads=hq, q_dtype=_lib.dtype_code(q.dtype),
+                n_items=n_items, n_slots=n_slots, query=_addr(q), out=_addr(out), items=base + 4 * offsets["items"],
+                pages=base + 4 * offsets["pages"], seg_rows=base + 4 * offsets["seg_rows"],
+                row_slots=base + 4 * offsets["row_slots"], rope_sin_minus_cos=_addr(dm), rope_cos_plus_sin=_addr(dp),
+                rope_n_pos=dm.shape[0], hadamard_scale=hadamard_constant(d),
+                scale_divisor=float(np.float32(math.sqrt(d))), workspace=_addr(ws), workspace_bytes=nbytes)
+            st = lib.nq_shared_attention(ctypes.byref(desc), _stream(dev))
+        _lib.check(st, "nq_shared_attention")
         return out
 
     def forward(self, query: torch.Tensor, compressed_key_cache: dict, compressed_value_cache: dict,

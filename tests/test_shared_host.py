@@ -1,0 +1,138 @@
+"""Host side of decode attention over shared pages: segments, work lists and refusals, without a GPU."""
+
+import ctypes
+import os
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+from nexusquant_amd import _lib
+from nexusquant_amd.vllm_backend import (NexusQuantKVCompressor, NexusQuantPagedAttention, SharedAttentionPlan,
+                                         shared_items, shared_segments)
+
+from test_page_pool import c_pool, host_pool
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def pages_of(segments, batch, t):
+    """Per row its (page, tokens) in order of the pages, from the segments."""
+    got = [[] for _ in range(batch)]
+    for rows, pages, n in segments:
+        assert n > 0 and len(pages) >= -(-n // t)
+        for b in rows:
+            got[b] += [(int(p), min(t, n - i * t)) for i, p in enumerate(pages) if i * t < n]
+    return got
+
+
+def cases():
+    a = list(range(100, 140))
+    yield [a[:20], a[:20], a[:20]], [320, 320, 320], 16          # the same rows
+    yield [a[:20] + [1], a[:20] + [2], a[:20] + [3, 4]], [323, 336, 340], 16
+    yield [a[:20], a[:30], [7]], [311, 480, 5], 16               # the shared run ends in the shorter row's part page
+    yield [a[:2] + [1], a[:2] + [2]], [48, 47], 16               # too little to share
+    yield [a[:1] + a[10:30] + [1], a[:1] + a[10:30] + [2], a[:1] + [50, 51]], [340, 350, 40], 16  # nested
+    yield [[], [3], []], [0, 1, 0], 16
+    yield [a[:20] + a[20:40], a[:20] + a[20:40], a[:20] + [1], a[:20] + [2]], [640, 639, 330, 330], 16  # forks of forks
+    yield [[5] * 1, [5] * 1], [1, 1], 1
+
+
+@pytest.mark.parametrize("min_saved", [1, 256, 10 ** 9])
+@pytest.mark.parametrize("tables,lengths,t", list(cases()))
+def test_segments_hold_every_token_of_every_row_once(tables, lengths, t, min_saved):
+    arr = [np.asarray(x[:-(-n // t)], dtype=np.int64) for x, n in zip(tables, lengths)]
+    segs = shared_segments(arr, lengths, t, min_saved)
+    got = pages_of(segs, len(tables), t)
+    for b, n in enumerate(lengths):
+        want = [(int(p), min(t, n - i * t)) for i, p in enumerate(arr[b])]
+        assert sorted(got[b]) == sorted(want)
+    for rows, pages, n in segs:
+        if len(rows) > 1:
+            assert n % t == 0 and (len(rows) - 1) * n >= min_saved
+
+
+def test_what_is_shared_is_in_one_segment():
+    a = np.arange(40)
+    segs = shared_segments([np.r_[a, 50], np.r_[a, 51], np.r_[a, 52]], [650, 656, 641], 16)
+    assert sorted((rows, n) for rows, _, n in segs) == [([0], 10), ([0, 1, 2], 640), ([1], 16), ([2], 1)]
+    # nested: a common start too short by itself goes along with what its branches share
+    x, y = np.arange(100, 130), np.arange(200, 230)
+    segs = shared_segments([np.r_[1, x], np.r_[1, x], np.r_[1, y], np.r_[1, y]], [496] * 4, 16)
+    assert sorted((rows, n) for rows, _, n in segs) == [([0, 1], 496), ([2, 3], 496)]
+
+
+@pytest.mark.parametrize("tile_rows,kv_heads,cap", [(128, 8, 1024), (32, 1, 1024), (1, 2, 256), (16, 64, 128)])
+def test_items_cover_each_rows_tokens_and_slots_once(tile_rows, kv_heads, cap):
+    r = np.random.RandomState(tile_rows)
+    batch = 37
+    segments = [(list(range(20)), np.arange(300), 4800), ([3, 5, 36], np.arange(400, 410), 160)]
+    segments += [([b], np.arange(1000 + 10 * b, 1010 + 10 * b), int(r.randint(1, 160))) for b in range(30)]
+    parts, n_items, n_slots = shared_items(segments, batch, tile_rows, kv_heads, cap)
+    items = parts["items"].reshape(-1, 8)
+    rows = parts["seg_rows"].reshape(-1, 2)
+    assert len(items) == n_items and parts["row_slots"][0] == 0 and parts["row_slots"][-1] == n_slots
+    seen, slots = {}, []
+    for page0, tok0, n, row0, n_rows, chunk, _, _ in items:
+        assert 1 <= n <= cap and 1 <= n_rows <= tile_rows
+        for b, slot0 in rows[row0:row0 + n_rows]:
+            slots.append(slot0 + chunk)
+            assert parts["row_slots"][b] <= slot0 + chunk < parts["row_slots"][b + 1]
+            for t in range(tok0, tok0 + n):
+                key = (int(b), int(parts["pages"][page0 + t // 16]), t % 16)
+                assert key not in seen
+                seen[key] = 1
+    assert sorted(slots) == list(range(n_slots))
+    assert len(seen) == sum(len(s[0]) * s[2] for s in segments)
+
+
+def test_no_rows_and_no_tokens():
+    parts, n_items, n_slots = shared_items([], 3, 128, 8, 1024)
+    assert n_items == 0 and n_slots == 0 and list(parts["row_slots"]) == [0, 0, 0, 0]
+
+
+def test_plan_refuses_bad_tables(monkeypatch):
+    pool = host_pool(monkeypatch, d=64)
+    attn = NexusQuantPagedAttention(NexusQuantKVCompressor(head_dim=64))
+    a = pool.allocate(4)
+    assert sorted(s[2] for s in attn.plan_shared(pool, [a, a[:1], []], [16, 3, 0]).segments) == [3, 16]
+    for tables, ctx in (([a], [17]), ([a], [-1]), ([[9]], [1]), ([a, a], [4]), ([[99]], [1])):
+        with pytest.raises(ValueError):
+            attn.plan_shared(pool, tables, ctx)
+    with pytest.raises(ValueError):
+        NexusQuantPagedAttention(NexusQuantKVCompressor(head_dim=128)).plan_shared(pool, [a], [3])
+    with pytest.raises(_lib.NexusQuantError):
+        attn.run_shared(SharedAttentionPlan(pool, 1, []), torch.zeros(1, 3, 64))
+
+
+def test_shared_struct_matches_the_c_compiler(tmp_path):
+    names = [f[0] for f in _lib.SharedDesc._fields_]
+    prog = ["#include <stddef.h>", "#include <stdio.h>", f'#include "{ROOT}/include/nexusquant_amd.h"', "int main(void){",
+            'printf("%zu\\n", sizeof(nq_shared_desc));']
+    prog += [f'printf("%zu\\n", offsetof(nq_shared_desc, {f}));' for f in names] + ["return 0;}"]
+    (tmp_path / "p.c").write_text("\n".join(prog))
+    subprocess.check_call(["gcc", "-o", str(tmp_path / "p"), str(tmp_path / "p.c")])
+    out = [int(x) for x in subprocess.check_output([str(tmp_path / "p")]).split()]
+    assert out == [ctypes.sizeof(_lib.SharedDesc)] + [getattr(_lib.SharedDesc, f).offset for f in names]
+
+
+@pytest.mark.parametrize("kw,pool_kw", [
+    (dict(layer=1), {}), (dict(layer=-1), {}), (dict(batch=-1), {}), (dict(q_heads=0), {}), (dict(q_heads=3), {}),
+    (dict(q_heads=2 * 129), {}), (dict(q_dtype=_lib.NQ_F32), {}), (dict(n_items=-1), {}), (dict(n_slots=0), {}),
+    (dict(query=None), {}), (dict(query=ctypes.c_void_p(4104)), {}), (dict(out=None), {}), (dict(items=None), {}),
+    (dict(row_slots=None), {}), (dict(rope_sin_minus_cos=None), {}), (dict(rope_n_pos=0), {}),
+    (dict(workspace=None), {}), (dict(workspace_bytes=100), {}), (dict(workspace=ctypes.c_void_p(4100)), {}),
+    (dict(scale_divisor=0.0), {}), (dict(n_items=1 << 30), {}), (dict(batch=1 << 30), {}),
+    ({}, dict(head_dim=96)), ({}, dict(heads=0)), ({}, dict(pages=1 << 27)), ({}, dict(key_codes=None)),
+    ({}, dict(value_codes=ctypes.c_void_p(4104)))])
+def test_c_entry_refuses(kw, pool_kw):
+    lib = _lib.load()
+    dummy = ctypes.c_void_p(4096)
+    base = dict(pool=ctypes.pointer(c_pool(**pool_kw)), layer=0, batch=2, q_heads=4, q_dtype=_lib.NQ_F16, n_items=1,
+                n_slots=2, query=dummy, out=dummy, items=dummy, pages=dummy, seg_rows=dummy, row_slots=dummy,
+                rope_sin_minus_cos=dummy, rope_cos_plus_sin=dummy, rope_n_pos=4096, hadamard_scale=0.1,
+                scale_divisor=11.3, workspace=dummy, workspace_bytes=1 << 20)
+    assert lib.nq_shared_attention(ctypes.byref(_lib.SharedDesc(**{**base, **kw})), None) == -1
+    assert lib.nq_last_error().startswith(b"nq_shared_attention")
+    assert lib.nq_shared_attention(ctypes.byref(_lib.SharedDesc(**{**base, "batch": 0})), None) in (0, -1)
