@@ -244,6 +244,7 @@ def prepare(case, seed):
     if own:
         from nexusquant_amd.vllm_backend import NexusQuantKVCompressor, NexusQuantPagedAttention
         st["pool"] = _own_pool(f)
+        st["pool"].allocate(groups * full + sum(own_pages))
         st["attn"] = NexusQuantPagedAttention(NexusQuantKVCompressor(head_dim=d, bits=case["bits"], rope_base=BASE))
         st["plan"] = st["attn"].plan_shared(st["pool"], tables, ctx)
     else:
