@@ -141,15 +141,26 @@ struct Rows {
         }
     }
 
-    __device__ __forceinline__ void weights(const f32x16& s, float c, uint32_t (&p)[8]) {
+    // SCALED: the weights of the sum of values are times v[key of the tile], in LDS
+    template <bool SCALED>
+    __device__ __forceinline__ void weights(const f32x16& s, float c, uint32_t (&p)[8], const float* v, int g) {
         float sum = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, -m));
-            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j + 1], c, -m));
-            sum += x;
-            sum += y;
-            p[j / 2] = pack2<DT>(x, y);
+        for (int i = 0; i < 4; ++i) {
+            f32x4 f = {1.0f, 1.0f, 1.0f, 1.0f};
+            if constexpr (SCALED) f = *reinterpret_cast<const f32x4*>(v + 8 * i + 4 * g);
+#pragma unroll
+            for (int k = 0; k < 4; k += 2) {
+                float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i + k], c, -m));
+                float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i + k + 1], c, -m));
+                sum += x;
+                sum += y;
+                if constexpr (SCALED) {
+                    x *= f[k];
+                    y *= f[k + 1];
+                }
+                p[2 * i + k / 2] = pack2<DT>(x, y);
+            }
         }
         l += sum;
     }
@@ -179,7 +190,8 @@ struct Rows {
     }
 
     // tiles t and t + 1, which every query sees whole
-    __device__ __forceinline__ void two_tiles(const char* kbuf, const char* vbuf, int t, float c) {
+    template <bool SCALED = false>
+    __device__ __forceinline__ void two_tiles(const char* kbuf, const char* vbuf, int t, float c, int g, const float* v = nullptr) {
         f32x16 s[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) s[i] = logits(kbuf, t + i);
@@ -192,13 +204,15 @@ struct Rows {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             uint32_t p[8];
-            weights(s[i], c, p);
+            weights<SCALED>(s[i], c, p, v + 32 * i, g);
             add_values(p, vbuf, t + i);
         }
     }
 
     // tile t, of which this lane's query sees the keys lo <= key < hi (of 32)
-    __device__ __forceinline__ void masked_tile(const char* kbuf, const char* vbuf, int t, float c, int lo, int hi, int g) {
+    template <bool SCALED = false>
+    __device__ __forceinline__ void masked_tile(const char* kbuf, const char* vbuf, int t, float c, int lo, int hi, int g,
+                                                const float* v = nullptr) {
         f32x16 s = logits(kbuf, t);
         float mx = -__builtin_inff();
 #pragma unroll
@@ -209,7 +223,7 @@ struct Rows {
         }
         raise(mx, c);
         uint32_t p[8];
-        weights(s, c, p);
+        weights<SCALED>(s, c, p, v, g);
         add_values(p, vbuf, t);
     }
 };

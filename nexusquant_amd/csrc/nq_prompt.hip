@@ -127,7 +127,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
         if (live && key <= my_last) {
             const bool whole = key + kStage - 1 <= my0 && (!a.window || key > my_last - a.window);
             if (whole) {
-                rows.two_tiles(ck, cv, 0, a.c);
+                rows.two_tiles(ck, cv, 0, a.c, g);
             } else {
                 int lo = a.window ? my_q - a.window + 1 - key : 0, hi = my_q + 1 - key;
 #pragma unroll 1

@@ -6,8 +6,9 @@
 // takes a chunk of a segment's tokens, one kv head, and up to 128 of the segment's query rows
 // (batch rows x the kv head's query heads).  Stage by stage (128 tokens) it
 //  1. decodes keys and values into LDS as fp16, all waves together: keys through the int8
-//     matrix cores (nq_keymfma.h), scaled and rotated in fp32; values as codes times their scale, without the transform: it is linear, and the combine kernel
-//     applies it once to a row's sum;
+//     matrix cores (nq_keymfma.h), scaled and rotated in fp32; values as their codes: their
+//     scales go with the softmax weights, and the transform, which is linear, with a row's
+//     sum (combine kernel);
 //  2. attends (nq_flash.h): with more than 64 query rows each wave has 32 of them and all four
 //     tiles of the stage; with up to 64 two waves, with up to 32 four waves share 32 rows and
 //     take the stage's tiles in turn, and their sums are joined in LDS at the end.
@@ -89,7 +90,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
     __shared__ __align__(16) char s_kv[2 * kSharedStage * ROWB];  // keys, values; at the end the waves' sums
     __shared__ uint32_t s_row[kSharedChunk];    // a token's row of head 0
     __shared__ uint32_t s_pos[kSharedChunk];    // its rotation table row
-    __shared__ uint32_t s_scale[kSharedChunk];  // its key scale, and its value scale times 2^vexp (fp16)
+    __shared__ __align__(16) float s_vs[kSharedChunk];  // its value scale times 2^vexp
+    __shared__ uint16_t s_ks[kSharedChunk];     // its key scale (fp16)
     __shared__ float s_max[4], s_m[4][32], s_l[4][32];
     char* const kbuf = s_kv;
     char* const vbuf = s_kv + kSharedStage * ROWB;
@@ -115,12 +117,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
         const uint32_t page = (uint32_t)pages[p];
         const uint32_t row = page * a.kv_heads * a.tokens + head_rows + off;
         const int32_t pos = a.positions[page * a.tokens + off];
-        const uint32_t vs = a.vs[row];
+        const float vs = f16_bits_to_f32(a.vs[row]);
         s_row[i] = row;
         s_pos[i] = pos < 0 ? 0u : ((uint32_t)pos >= a.rope_n_pos ? a.rope_n_pos - 1u : (uint32_t)pos);
-        s_scale[i] = a.ks[row] | vs << 16;
-        vmax = __builtin_fmaxf(vmax, __builtin_fabsf(f16_bits_to_f32(vs)));
+        s_ks[i] = a.ks[row];
+        s_vs[i] = vs;
+        vmax = __builtin_fmaxf(vmax, __builtin_fabsf(vs));
     }
+    for (int i = n_tok + threadIdx.x; i < (n_tok + 31) / 32 * 32; i += 256) s_vs[i] = 0.0f;  // slots of the last tile
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) vmax = __builtin_fmaxf(vmax, __shfl_xor(vmax, o, 64));
     if (lane == 0) s_max[wave] = vmax;
@@ -140,20 +144,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
     KM km;
     km.init(lane);
     __syncthreads();
-    // Values in fp16: the chunk's scales times 2^vexp, the largest then in [128, 256): a value of codes
-    // up to 128 stays below 2^15, and one keeps its 11 bits down to 2^-21 of the largest scale.
+    // The values' scales go with the weights, so that the codes are exact in fp16 and one rounding is left.
+    // Times 2^vexp the chunk's largest is in [64, 128): weights (at most 2^kSlack) stay below 2^15, and keep
+    // their 11 bits down to 2^-20 of that.
     int vexp = 0;
     {
         const float m = __builtin_fmaxf(__builtin_fmaxf(s_max[0], s_max[1]), __builtin_fmaxf(s_max[2], s_max[3]));
         if (m > 0.0f && m < __builtin_inff()) {
             (void)__builtin_frexpf(m, &vexp);
-            vexp = 8 - vexp;
+            vexp = 7 - vexp;
         }
     }
-    for (int i = threadIdx.x; i < n_tok; i += 256) {
-        const uint32_t w = s_scale[i];
-        s_scale[i] = (w & 0xffffu) | f32_to_f16_bits(__builtin_ldexpf(f16_bits_to_f32(w >> 16), vexp)) << 16;
-    }
+    for (int i = threadIdx.x; i < n_tok; i += 256) s_vs[i] = __builtin_ldexpf(s_vs[i], vexp);
     __syncthreads();
 
     const int n16 = lane & 15, kg = lane >> 4, quad = lane >> 2, qq = lane & 3;
@@ -180,7 +182,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
                     }
             }
             const size_t tab = (size_t)s_pos[tq] * (D / 2) + 4 * qq;
-            const float k_scale = (0.5f * f16_bits_to_f32(s_scale[tn] & 0xffffu)) * a.hscale;
+            const float k_scale = (0.5f * f16_bits_to_f32(s_ks[tn])) * a.hscale;
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
@@ -219,15 +221,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
             const int row = i / (D / 16), piece = i % (D / 16);
             const int t = min(s0 + row, n_tok - 1);
             const u32x4 w = *reinterpret_cast<const u32x4*>(a.vc + (size_t)s_row[t] * D + 16 * piece);
-            const uint32_t sc = s0 + row < n_tok ? s_scale[t] >> 16 : 0u;
-            const half2v s = __builtin_bit_cast(half2v, sc | sc << 16);
             u32x4 o[2];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 half2v lo, hi;
                 codes_to_f16(w[k], lo, hi);
-                lo *= s;
-                hi *= s;
                 o[k / 2][2 * (k & 1)] = __builtin_bit_cast(uint32_t, lo);
                 o[k / 2][2 * (k & 1) + 1] = __builtin_bit_cast(uint32_t, hi);
             }
@@ -241,9 +239,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
             const int t1 = min(tile0 + rw, units / 2);
             int t = tile0;
 #pragma unroll 1
-            for (; t + 1 < t1 && 32 * (t + 2) <= left; t += 2) rows.two_tiles(kbuf, vbuf, t, c);
+            for (; t + 1 < t1 && 32 * (t + 2) <= left; t += 2) rows.template two_tiles<true>(kbuf, vbuf, t, c, g, s_vs + s0 + 32 * t);
 #pragma unroll 1
-            for (; t < t1; ++t) rows.masked_tile(kbuf, vbuf, t, c, 0, left - 32 * t, g);
+            for (; t < t1; ++t) rows.template masked_tile<true>(kbuf, vbuf, t, c, 0, left - 32 * t, g, s_vs + s0 + 32 * t);
         }
         __syncthreads();
     }

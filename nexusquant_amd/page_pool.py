@@ -28,7 +28,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .ops import _addr, to_device
+from .ops import _addr, on_device, to_device
 from .vllm_backend import CompressedPage
 
 _HEAD_DIMS = (64, 128, 256)
@@ -138,10 +138,10 @@ class CompressedPagePool:
         # a list of ints by way of array(): two thirds of numpy's own conversion time
         try:
             p = (np.frombuffer(array.array("i", pages), dtype=np.int32) if type(pages) is list and pages
-                 else np.asarray(pages, dtype=np.int64).reshape(-1))
+                 else np.asarray(pages, dtype=np.int32).reshape(-1))
         except OverflowError:
             raise ValueError(f"page numbers must lie in [0, {self.num_pages})") from None
-        if len(p) and (p.min() < 0 or p.max() >= self.num_pages):
+        if len(p) and p.view(np.uint32).max() >= self.num_pages:  # a negative number is a large one there
             raise ValueError(f"page numbers must lie in [0, {self.num_pages})")
         return p
 
@@ -155,10 +155,11 @@ class CompressedPagePool:
     def _tally(self, p: np.ndarray):
         """The pages in p, ascending and each once, and how often each is there."""
         if 8 * len(p) < self.num_pages:
-            return np.unique(p, return_counts=True)
+            p, n = np.unique(p, return_counts=True)
+            return p, n.astype(np.int32)
         n = np.bincount(p, minlength=self.num_pages)  # 7 us where sorting 6000 pages takes 53
-        p = np.flatnonzero(n)
-        return p, n[p]
+        p = n.nonzero()[0]
+        return p, n[p].astype(np.int32)
 
     def allocate(self, n: int) -> List[int]:
         """n pages with one reference each.  Their contents are whatever they last held."""
@@ -168,38 +169,42 @@ class CompressedPagePool:
         with self._lock:
             if n > self._free:
                 raise _lib.NexusQuantError(f"{n} pages wanted, {self._free} of {self.num_pages} free")
-            got = self._stack[self._free - n:self._free][::-1]
-            self._free -= n
-            self._refs[got] = 1
-            return got.tolist()
+            return self._take(n).tolist()
+
+    def _take(self, n: int) -> np.ndarray:
+        got = self._stack[self._free - n:self._free][::-1].copy()
+        self._free -= n
+        self._refs[got] = 1
+        return got
+
+    def _drop(self, p: np.ndarray, n: np.ndarray) -> None:
+        left = self._refs[p] - n
+        if len(p) and left.min() < 0:
+            raise ValueError(f"page {int(p[left < 0][0])} is freed more often than it is referenced")
+        self._refs[p] = left
+        gone = p[left == 0][::-1]  # the lowest is allocated next
+        self._stack[self._free:self._free + len(gone)] = gone
+        self._free += len(gone)
 
     def retain(self, pages: Sequence[int]) -> None:
         """One more reference to each page (to a page listed twice: two)."""
         with self._lock:
             p, n = self._tally(self.in_use(pages, "retain"))
-            self._refs[p] += n.astype(np.int32)
+            self._refs[p] += n
 
     def free(self, pages: Sequence[int]) -> None:
         """Drop one reference of each page (of a page listed twice: two); pages without any can be
         allocated again.  Work already queued on the pool's stream still sees them as they were."""
         with self._lock:
-            p, n = self._tally(self.in_use(pages, "free"))
-            left = self._refs[p] - n.astype(np.int32)
-            if len(p) and left.min() < 0:
-                raise ValueError(f"page {int(p[left < 0][0])} is freed more often than it is referenced")
-            self._refs[p] = left
-            gone = p[left == 0][::-1]  # the lowest is allocated next
-            self._stack[self._free:self._free + len(gone)] = gone
-            self._free += len(gone)
+            self._drop(*self._tally(self.in_use(pages, "free")))
 
     # --------------------------------------------------------------- page moves
 
-    def _copy(self, src: np.ndarray, dst: np.ndarray) -> None:
-        src = np.ascontiguousarray(src, dtype=np.int32)
-        dst = np.ascontiguousarray(dst, dtype=np.int32)
+    def _copy(self, src, dst) -> None:
+        s, d = array.array("i", src), array.array("i", dst)  # read during the call
         lib = _lib.load()
-        with torch.cuda.device(self.device):
-            st = lib.nq_pool_copy_pages(ctypes.byref(self.desc), src.ctypes.data, dst.ctypes.data, len(src),
+        with on_device(self.device):
+            st = lib.nq_pool_copy_pages(ctypes.byref(self.desc), s.buffer_info()[0], d.buffer_info()[0], len(s),
                                         ctypes.c_void_p(_lib.current_stream_handle(self.device)))
         _lib.check(st, "nq_pool_copy_pages")
 
@@ -214,7 +219,7 @@ class CompressedPagePool:
                 raise ValueError(f"{len(s)} source pages for {len(d)} destinations")
             if len(d) and self._refs[d].max() > 1:
                 raise ValueError(f"copy_pages: page {int(d[self._refs[d] > 1][0])} is shared and cannot be written")
-            self._copy(s, d)
+            self._copy(s.tolist(), d.tolist())
 
     def _sequence(self, pages, length: int, what: str) -> Tuple[np.ndarray, int]:
         p, length = self.in_use(pages, what), int(length)
@@ -231,19 +236,21 @@ class CompressedPagePool:
         for each branch, so that the sequence and its branches can all go on writing."""
         _refuse_capture("fork")
         with self._lock:
-            p, length = self._sequence(pages, length, "fork")
-            n = int(n)
+            n, length = int(n), int(length)
             if n < 0:
                 raise ValueError(f"cannot fork {n} branches")
-            table = list(pages) if type(pages) is list else p.tolist()
-            if n == 0:
-                return []
+            p = self.in_use(pages, "fork")
+            if length < 0 or self.pages_for(length) != len(p):
+                raise ValueError(f"fork: {length} tokens take {self.pages_for(max(length, 0))} pages, got {len(p)}")
+            if len(self._tally(p)[0]) != len(p):
+                raise ValueError("fork: a page stands twice in one sequence")
+            table = pages if type(pages) is list else p.tolist()
             if length % self.page_tokens == 0:
                 self._refs[p] += n
                 return [list(table) for _ in range(n)]
             last = self.allocate(n)
             try:
-                self._copy(np.full(n, p[-1]), np.asarray(last))
+                self._copy([table[-1]] * n, last)
             except Exception:
                 self.free(last)
                 raise
@@ -270,49 +277,58 @@ class CompressedPagePool:
         if kept_idx.device != self.device:
             raise ValueError(f"kept_idx is on {kept_idx.device}, the pool on {self.device}")
         batch = len(tables)
-        counts = [int(x) for x in (n_kept.tolist() if torch.is_tensor(n_kept) else n_kept)]
-        if not (len(lengths) == len(counts) == kept_idx.shape[0] == batch):
-            raise ValueError(f"{batch} tables, {len(lengths)} lengths, {len(counts)} counts and {kept_idx.shape[0]} "
-                             "rows of kept_idx")
         idx = kept_idx.contiguous()
         step = int(lib.nq_pool_move_tokens())
         with self._lock:
-            old = []
+            # everything that does not need the counts comes before they are read back: the device is
+            # busy with what was queued before
+            had = [int(n) for n in lengths]
+            sizes = [len(t) for t in tables]
+            if not (len(had) == kept_idx.shape[0] == batch):
+                raise ValueError(f"{batch} tables, {len(had)} lengths and {kept_idx.shape[0]} rows of kept_idx")
             for b in range(batch):
-                p, n = self._sequence(tables[b], lengths[b], "compact")
-                if not 0 <= counts[b] <= n or counts[b] > idx.shape[1]:
-                    raise ValueError(f"sequence {b} keeps {counts[b]} of {n} tokens by a list of {idx.shape[1]}")
-                old.append(p)
-            want = [self.pages_for(c) for c in counts]
-            flat = np.concatenate(old) if old else np.zeros(0, dtype=np.int32)
+                if had[b] < 0 or self.pages_for(had[b]) != sizes[b]:
+                    raise ValueError(f"compact: {had[b]} tokens take {self.pages_for(max(had[b], 0))} pages, "
+                                     f"got {sizes[b]}")
+            flat = self.in_use([p for t in tables for p in t] if batch != 1 else tables[0], "compact")
             held, times = self._tally(flat)
-            if np.any(times > self._refs[held]):
+            if len(held) and (self._refs[held] < times).any():
                 raise ValueError("compact: a page stands in more tables than it has references")
-            new = self.allocate(sum(want))
-            at = np.concatenate([[0], np.cumsum(want)]).astype(np.int64)
+            counts = [int(x) for x in (n_kept.tolist() if torch.is_tensor(n_kept) else n_kept)]
+            if len(counts) != batch:
+                raise ValueError(f"{len(counts)} counts for {batch} sequences")
+            seq, tiles, ends = [], [], [0]
+            n_tiles = start = 0
+            for b, k in enumerate(counts):
+                if not 0 <= k <= had[b] or k > idx.shape[1]:
+                    raise ValueError(f"sequence {b} keeps {k} of {had[b]} tokens by a list of {idx.shape[1]}")
+                seq += (n_tiles, k, had[b], start, len(flat) + ends[-1])
+                tiles.append(-(-k // step))
+                n_tiles += tiles[-1]
+                start += sizes[b]
+                ends.append(ends[-1] + self.pages_for(k))
+            if ends[-1] > self._free:
+                raise _lib.NexusQuantError(f"{ends[-1]} pages wanted, {self._free} of {self.num_pages} free")
+            new = self._take(ends[-1])
             try:
-                tiles = [-(-c // step) for c in counts]
-                n_tiles = sum(tiles)
                 if n_tiles:
-                    first = np.concatenate([[0], np.cumsum(tiles)[:-1]])
-                    starts = np.concatenate([[0], np.cumsum([len(p) for p in old])[:-1]])
-                    seq = np.stack([first, counts, lengths, starts, len(flat) + at[:-1]], axis=1).reshape(-1)
-                    plan = to_device(np.concatenate([np.repeat(np.arange(batch), tiles), seq, flat, new]), self.device)
+                    plan = to_device(np.concatenate([np.repeat(np.arange(batch, dtype=np.int32), tiles),
+                                                     np.array(seq, dtype=np.int32), flat, new]), self.device)
                     base = plan.data_ptr()
-                    with torch.cuda.device(self.device):
+                    with on_device(self.device):
                         st = lib.nq_pool_compact(ctypes.byref(self.desc), base, n_tiles, base + 4 * n_tiles,
                                                  base + 4 * (n_tiles + len(seq)), _addr(idx), idx.shape[1],
                                                  int(bool(renumber)),
                                                  ctypes.c_void_p(_lib.current_stream_handle(self.device)))
                     _lib.check(st, "nq_pool_compact")
             except Exception:
-                self.free(new)
+                self._drop(*self._tally(new))
                 raise
-            if len(flat):
-                self.free(flat)
+            self._drop(held, times)
             if renumber and counts:
                 self.max_position = max(self.max_position, max(counts) - 1)
-        return [new[at[b]:at[b + 1]] for b in range(batch)], counts
+        got = new.tolist()
+        return [got[a:b] for a, b in zip(ends, ends[1:])], counts
 
     # ------------------------------------------------------------------- tokens
 
