@@ -672,8 +672,11 @@ int nq_pool_write(const nq_pool* pool, int32_t layer, const nq_pool* tokens, con
  *              [1] the chunk's first token, counted from there
  *              [2] its tokens (1 ..)
  *              [3] where its rows start in `seg_rows` (entries)
- *              [4] rows, at most nq_shared_attention_rows() / (q_heads / heads)
+ *              [4] rows, at most nq_shared_attention_rows(head_dim) / (q_heads / heads)
  *              [5] the chunk's number in its segment;  [6..7] unused
+ *            The first n_many of them may have that many rows; those after
+ *            them have at most nq_shared_attention_few_rows() query rows
+ *            (rows x q_heads / heads).
  *   pages    page numbers
  *   seg_rows [entries * 2] batch row, and the row's slot of the segment's
  *            first chunk
@@ -690,7 +693,8 @@ typedef struct nq_shared_desc {
     const nq_pool* pool;
     int32_t layer, batch, q_heads;
     int32_t q_dtype;            /* NQ_F16 / NQ_BF16 */
-    int32_t n_items, n_slots;
+    int32_t n_items, n_many, n_slots;
+    int32_t reserved;
     const void* query;
     void* out;
     const int32_t* items;
@@ -707,7 +711,8 @@ typedef struct nq_shared_desc {
 } nq_shared_desc;
 
 int32_t nq_shared_attention_chunk_tokens(void);
-int32_t nq_shared_attention_rows(void);
+int32_t nq_shared_attention_rows(int32_t head_dim);
+int32_t nq_shared_attention_few_rows(void);
 int64_t nq_shared_attention_workspace(int32_t n_slots, int32_t q_heads, int32_t head_dim);
 int nq_shared_attention(const nq_shared_desc* desc, void* stream);
 

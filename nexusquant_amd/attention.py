@@ -58,7 +58,7 @@ def plan_prompts(lengths: Sequence[int], device=None) -> PromptPlan:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t with contiguous, 16-byte aligned head vectors (itself when they are)."""
-    if t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0:
+    if t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(0) < 1 << 24 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

@@ -194,12 +194,20 @@ struct Rows {
     __device__ __forceinline__ void two_tiles(const char* kbuf, const char* vbuf, int t, float c, int g, const float* v = nullptr) {
         f32x16 s[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) s[i] = logits(kbuf, t + i);
+        for (int i = 0; i < 2; ++i) s[i] = f32x16{};
+#pragma unroll
+        for (int k = 0; k < T::KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                s[i] = mfma<DT>(*reinterpret_cast<const u32x4*>(kbuf + (t + i) * 32 * T::ROWB + (k_at ^ (uint32_t)(32 * k))), q[k], s[i]);
         float mx = s[0][0];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int j = 0; j < 16; ++j) mx = __builtin_fmaxf(mx, s[i][j]);
+        // the wave that is past its logits goes first, so that a SIMD's waves fall out of step and one's
+        // exponentials run under the other's products
+        __builtin_amdgcn_s_setprio(1);
         raise(mx, c);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -207,6 +215,7 @@ struct Rows {
             weights<SCALED>(s[i], c, p, v + 32 * i, g);
             add_values(p, vbuf, t + i);
         }
+        __builtin_amdgcn_s_setprio(0);
     }
 
     // tile t, of which this lane's query sees the keys lo <= key < hi (of 32)

@@ -27,21 +27,40 @@ constexpr int kWaitVm0 = 0x0f70;  // vmcnt(0), the other counters left open
 constexpr int kPromptRows = 128;
 constexpr int kStage = 64;        // keys of a stage: two tiles
 
-// Rows row0 .. row0 + 63 of one head to LDS in Tile's layout; rows past the sequence repeat its
-// last one (their weights are zero, and what lies behind the sequence is never read).
+// Rows row0 .. row0 + 63 of one head to LDS in Tile's layout, 16 bytes a lane: load i fills the 64
+// slots from 64 (4 i + wave) on.  A lane's rows of successive loads are 2048 / D apart, at the same
+// chunk (but for bit 3 of a key's at D = 256), so a whole stage is a uniform address plus a fixed lane
+// offset.  In the sequence's last stage rows past its end repeat its last one (their weights are
+// zero, and what lies behind the sequence is never read).
 template <int D, bool VALUES>
-__device__ __forceinline__ void load_stage(const uint16_t* base, int64_t stride, int row0, int n, char* buf, int wave, int lane) {
+struct StageLoad {
     using T = Tile<D>;
-#pragma unroll
-    for (int i = 0; i < T::UPR / 4; ++i) {
-        const int w = 4 * i + wave, slot = 64 * w + lane;
-        const int r = slot / T::UPR, place = slot % T::UPR;
-        const int chunk = place ^ (VALUES ? T::value_swizzle(r) : T::key_swizzle(r));
-        const int row = min(row0 + r, n - 1);
-        const uint16_t* src = base + (int64_t)row * stride + 8 * chunk;
-        __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(buf + 1024 * w), 16, 0, 0);
+    static constexpr int STEP = 256 / T::UPR;  // rows
+    int row, chunk;
+    uint32_t off;
+    __device__ __forceinline__ void init(int wave, int lane, int64_t stride) {
+        const int slot = 64 * wave + lane;
+        row = slot / T::UPR;
+        chunk = (slot % T::UPR) ^ (VALUES ? T::value_swizzle(row) : T::key_swizzle(row));
+        off = (uint32_t)row * (uint32_t)(2 * stride) + 16u * chunk;
     }
-}
+    static __device__ __forceinline__ uint32_t flip(int i) { return !VALUES && D == 256 ? 8u * (i & 1) : 0u; }
+    __device__ __forceinline__ void operator()(const uint16_t* base, int64_t stride, int row0, int n, char* buf, int wave) const {
+        if (row0 + kStage <= n) {
+            const char* const from = reinterpret_cast<const char*>(base + (int64_t)row0 * stride);
+#pragma unroll
+            for (int i = 0; i < T::UPR / 4; ++i)
+                __builtin_amdgcn_global_load_lds((global_void*)(from + (int64_t)(STEP * i) * 2 * stride + (off ^ (16u * flip(i)))),
+                                                 (lds_void*)(buf + 1024 * (4 * i + wave)), 16, 0, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < T::UPR / 4; ++i) {
+                const uint16_t* const src = base + (int64_t)min(row0 + row + STEP * i, n - 1) * stride + 8 * (chunk ^ flip(i));
+                __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(buf + 1024 * (4 * i + wave)), 16, 0, 0);
+            }
+        }
+    }
+};
 
 // The output of a wave's queries again, key by key on the vector ALUs, each query over the keys
 // it sees only: for blocks with an infinity or a NaN among the values of a tile that hides keys.
@@ -114,37 +133,62 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
 #pragma unroll
     for (int i = 0; i < T::KS; ++i) rows.q[i] = *reinterpret_cast<const u32x4*>(qp + 16 * i);
 
-    load_stage<D, false>(kb, a.k_row, key0, len, k0, wave, lane);
-    load_stage<D, true>(vb, a.v_row, key0, len, v0, wave, lane);
+    StageLoad<D, false> load_k;
+    StageLoad<D, true> load_v;
+    load_k.init(wave, lane, a.k_row);
+    load_v.init(wave, lane, a.v_row);
+    load_k(kb, a.k_row, key0, len, k0, wave);
+    load_v(vb, a.v_row, key0, len, v0, wave);
     __builtin_amdgcn_s_waitcnt(kWaitVm0);
     __syncthreads();
-    auto step = [&](int it, const char* ck, const char* cv, char* nk, char* nv) {
-        const int key = key0 + kStage * it;
+    auto fetch = [&](int it, char* nk, char* nv) {
         if (it + 1 < n_stages) {
-            load_stage<D, false>(kb, a.k_row, key + kStage, len, nk, wave, lane);
-            load_stage<D, true>(vb, a.v_row, key + kStage, len, nv, wave, lane);
+            load_k(kb, a.k_row, key0 + kStage * (it + 1), len, nk, wave);
+            load_v(vb, a.v_row, key0 + kStage * (it + 1), len, nv, wave);
         }
-        if (live && key <= my_last) {
-            const bool whole = key + kStage - 1 <= my0 && (!a.window || key > my_last - a.window);
-            if (whole) {
-                rows.two_tiles(ck, cv, 0, a.c, g);
-            } else {
-                int lo = a.window ? my_q - a.window + 1 - key : 0, hi = my_q + 1 - key;
-#pragma unroll 1
-                for (int t = 0; t < 2; ++t, lo -= 32, hi -= 32) {
-                    if (!__any(lo < 32 && hi > 0)) continue;
-                    rows.masked_tile(ck, cv, t, a.c, lo, hi, g);
-                    odd |= rows.tile_odd(cv, t, lane);
-                }
-            }
-        }
+    };
+    auto landed = [&] {  // the next stage is in LDS, and this one may be overwritten
         __builtin_amdgcn_s_waitcnt(kWaitVm0);
         __syncthreads();
     };
+    // a stage that hides keys from some queries of the workgroup, or from all of a wave's
+    auto masked = [&](int it, const char* ck, const char* cv, char* nk, char* nv) {
+        fetch(it, nk, nv);
+        const int key = key0 + kStage * it;
+        int lo = a.window ? my_q - a.window + 1 - key : 0, hi = live ? my_q + 1 - key : 0;
 #pragma unroll 1
-    for (int it = 0; it < n_stages; it += 2) {
-        step(it, k0, v0, k1, v1);
-        if (it + 1 < n_stages) step(it + 1, k1, v1, k0, v0);
+        for (int t = 0; t < 2; ++t, lo -= 32, hi -= 32) {
+            if (!__any(lo < 32 && hi > 0)) continue;
+            rows.masked_tile(ck, cv, t, a.c, lo, hi, g);
+            if (__any(lo > 0 || hi < 32)) odd |= rows.tile_odd(cv, t, lane);
+        }
+        landed();
+    };
+    // one that every query of the workgroup sees whole
+    auto whole = [&](int it, const char* ck, const char* cv, char* nk, char* nv) {
+        fetch(it, nk, nv);
+        rows.two_tiles(ck, cv, 0, a.c, g);
+        landed();
+    };
+    // Whole stages are [it0, it1): past every query's window start, before the first query.  They run in a
+    // loop of their own, two a turn: a branch between the two kinds in every stage made the compiler move all
+    // of the output's registers twice a stage (32/8 heads x 16384 x 128 fp16: 2.47 ms with it).
+    const int it0 = a.window ? max((q_last - a.window - key0 + kStage) / kStage, 0) : 0;
+    const int it1 = (q0 - key0) / kStage;
+    int it = 0;
+    while (it < n_stages) {
+        if (!(it & 1) && it >= it0 && it + 1 < it1) {
+#pragma unroll 1
+            do {
+                whole(it, k0, v0, k1, v1);
+                whole(it + 1, k1, v1, k0, v0);
+                it += 2;
+            } while (it + 1 < it1);
+        } else {
+            if (it & 1) masked(it, k1, v1, k0, v0);
+            else masked(it, k0, v0, k1, v1);
+            ++it;
+        }
     }
     if (odd) sum_again<DT, D>(rows, kb, a.k_row, vb, a.v_row, a.c, key0, my_last, a.window ? my_q - a.window + 1 : 0, my_q, g);
     if (!live || my0 + n >= len) return;
@@ -192,6 +236,8 @@ extern "C" int nq_prompt_attention(const nq_prompt_desc* d, void* stream) {
     NQ_CHECK_ARG(((d->q_stride[0] | d->q_stride[1] | d->k_stride[0] | d->k_stride[1] | d->v_stride[0] | d->v_stride[1]) & 7) == 0 &&
                      ((d->out_stride[0] | d->out_stride[1]) & 3) == 0,
                  "nq_prompt_attention: strides must keep rows 16-byte aligned (out: 8-byte)");
+    NQ_CHECK_ARG(d->k_stride[0] >= 0 && d->k_stride[0] < (1 << 24) && d->v_stride[0] >= 0 && d->v_stride[0] < (1 << 24),
+                 "nq_prompt_attention: rows of k and v must be less than 2^24 elements apart");
     NQ_CHECK_ARG((uint64_t)d->n_tiles * d->q_heads <= max_blocks(256), "nq_prompt_attention: grid too large");
     PromptArgs a = {};
     a.q = static_cast<const uint16_t*>(d->q);

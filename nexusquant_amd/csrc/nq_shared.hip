@@ -2,16 +2,15 @@
 // with is read and decoded once for all of them.
 //
 // The host cuts the rows' tokens into segments: a run of pages and the batch rows that see
-// all its tokens (a shared prefix: many rows; a row's own rest: one).  A workgroup of 4 waves
-// takes a chunk of a segment's tokens, one kv head, and up to 128 of the segment's query rows
-// (batch rows x the kv head's query heads).  Stage by stage (128 tokens) it
+// all its tokens (a shared prefix: many rows; a row's own rest: one).  A workgroup takes a
+// chunk of a segment's tokens, one kv head, and up to 256 (head_dim 256: 128) of the segment's
+// query rows (batch rows x the kv head's query heads).  Stage by stage (128 tokens; 64) it
 //  1. decodes keys and values into LDS as fp16, all waves together: keys through the int8
 //     matrix cores (nq_keymfma.h), scaled and rotated in fp32; values as their codes: their
 //     scales go with the softmax weights, and the transform, which is linear, with a row's
 //     sum (combine kernel);
-//  2. attends (nq_flash.h): with more than 64 query rows each wave has 32 of them and all four
-//     tiles of the stage; with up to 64 two waves, with up to 32 four waves share 32 rows and
-//     take the stage's tiles in turn, and their sums are joined in LDS at the end.
+//  2. attends (nq_flash.h): 32 query rows a wave and all tiles of the stage; with fewer rows
+//     several waves share them and split the tiles, and their sums are joined in LDS at the end.
 // A partial (maximum, sum, value sum) per query row and chunk goes to the workspace; the
 // combine kernel joins a row's chunks.
 #include "nq_flash.h"
@@ -22,9 +21,25 @@ namespace nq {
 
 using namespace flash;
 
-constexpr int kSharedStage = 128;   // tokens
 constexpr int kSharedChunk = 1024;  // most tokens of a chunk: their places and scales stay in LDS
-constexpr int kSharedRows = 128;    // query rows of a workgroup
+
+// The shape of a workgroup.  MANY, for segments of more query rows than kFewRows: rows count, so as many as the
+// registers hold (32 a wave) share what is decoded; two stage buffers, 128 KB of LDS at head_dim 128 and 256, so
+// one workgroup on a CU.  Not MANY: decoding counts, and several small workgroups on a CU hide each other's loads.
+template <int D, bool MANY>
+struct Shape {
+    static constexpr int WAVES = MANY && D <= 128 ? 8 : 4;
+    static constexpr int STAGE = MANY && D > 128 ? 64 : 128;  // tokens
+    static constexpr int BUFS = MANY ? 2 : 1;
+    static constexpr int THREADS = 64 * WAVES;
+    static constexpr int TILES = STAGE / 32;
+    static constexpr int ROWS = 32 * WAVES;            // query rows
+    static constexpr int UNITS = STAGE / 16 / WAVES;   // 16-token units of keys a wave
+    static constexpr int PIECES = STAGE * D / 16 / THREADS;  // 16-byte pieces of values a thread
+    static_assert(BUFS * 2 * STAGE * 2 * D >= WAVES * 32 * D * 4, "the waves' sums must fit the stage buffers");
+    static constexpr int PER_SIMD = MANY ? WAVES / 4 : D == 64 ? 3 : D == 128 ? 2 : 1;  // waves
+};
+constexpr int kFewRows = 32;
 
 struct SharedArgs {
     const uint16_t* query;
@@ -42,7 +57,7 @@ struct SharedArgs {
     float* part_ml;           // [slots, q_heads, 2]
     const float* rope_dm;
     const float* rope_dp;
-    uint32_t q_heads, kv_heads, rope_n_pos, n_items, tokens;
+    uint32_t q_heads, kv_heads, rope_n_pos, n_items, tokens;  // n_items: of the launch, from `items` on
     FastDiv by_tokens, by_group;
     float c;                  // log2(e) / scale_divisor
     float hscale;
@@ -82,19 +97,19 @@ __device__ __forceinline__ float load_query(const uint16_t* p, u32x4 (&q)[Tile<D
     return __builtin_ldexpf(1.0f, e);
 }
 
-template <int D, int QDT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void shared_attn_kernel(SharedArgs a) {
+template <int D, int QDT, bool MANY>
+__global__ __launch_bounds__((Shape<D, MANY>::THREADS)) __attribute__((amdgpu_waves_per_eu(Shape<D, MANY>::PER_SIMD))) void
+shared_attn_kernel(SharedArgs a) {
     using T = Tile<D>;
     using KM = KeyMfma<D>;
-    constexpr int ROWB = T::ROWB;
-    __shared__ __align__(16) char s_kv[2 * kSharedStage * ROWB];  // keys, values; at the end the waves' sums
+    using SH = Shape<D, MANY>;
+    constexpr int ROWB = T::ROWB, NT = SH::THREADS, NW = SH::WAVES, STAGE = SH::STAGE;
+    __shared__ __align__(16) char s_kv[SH::BUFS][2 * STAGE * ROWB];  // stages of keys and values; at the end the waves' sums
     __shared__ uint32_t s_row[kSharedChunk];    // a token's row of head 0
     __shared__ uint32_t s_pos[kSharedChunk];    // its rotation table row
     __shared__ __align__(16) float s_vs[kSharedChunk];  // its value scale times 2^vexp
     __shared__ uint16_t s_ks[kSharedChunk];     // its key scale (fp16)
-    __shared__ float s_max[4], s_m[4][32], s_l[4][32];
-    char* const kbuf = s_kv;
-    char* const vbuf = s_kv + kSharedStage * ROWB;
+    __shared__ float s_max[NW], s_m[NW][32], s_l[NW][32];
 
     const int lane = threadIdx.x & 63, n = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -112,7 +127,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
     // ---- the chunk's tokens ----
     float vmax = 0.0f;
     const uint32_t head_rows = kh * a.tokens;
-    for (int i = threadIdx.x; i < n_tok; i += 256) {
+    for (int i = threadIdx.x; i < n_tok; i += NT) {
         const uint32_t t = tok0 + i, p = div(t, a.by_tokens), off = t - p * a.tokens;
         const uint32_t page = (uint32_t)pages[p];
         const uint32_t row = page * a.kv_heads * a.tokens + head_rows + off;
@@ -124,15 +139,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
         s_vs[i] = vs;
         vmax = __builtin_fmaxf(vmax, __builtin_fabsf(vs));
     }
-    for (int i = n_tok + threadIdx.x; i < (n_tok + 31) / 32 * 32; i += 256) s_vs[i] = 0.0f;  // slots of the last tile
+    for (int i = n_tok + threadIdx.x; i < (n_tok + 31) / 32 * 32; i += NT) s_vs[i] = 0.0f;  // slots of the last tile
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) vmax = __builtin_fmaxf(vmax, __shfl_xor(vmax, o, 64));
     if (lane == 0) s_max[wave] = vmax;
 
     // ---- this wave's queries ----
-    const int rw = n_q <= 32 ? 1 : n_q <= 64 ? 2 : 4;   // waves with rows of their own
-    const int r0 = 32 * (wave % rw), tile0 = wave / rw * rw;
-    const bool live = r0 < n_q;
+    int rw = 1;  // waves with rows of their own; the others share these rows and take other tiles
+    while (rw < NW && n_q > 32 * rw) rw *= 2;
+    const int per_wave = SH::TILES * rw < NW ? 1 : SH::TILES * rw / NW;   // tiles of a stage
+    const int r0 = 32 * (wave % rw), tile0 = wave / rw * per_wave;
+    const bool live = r0 < n_q && tile0 < SH::TILES;
     Rows<NQ_F16, D> rows;
     rows.init(lane);
     float c = a.c;
@@ -141,55 +158,95 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
         const uint32_t head = kh * G + (r - br * G);
         c *= load_query<D, QDT>(a.query + ((size_t)(uint32_t)seg_rows[2 * br] * a.q_heads + head) * D + 8 * g, rows.q);
     }
-    KM km;
-    km.init(lane);
     __syncthreads();
     // The values' scales go with the weights, so that the codes are exact in fp16 and one rounding is left.
     // Times 2^vexp the chunk's largest is in [64, 128): weights (at most 2^kSlack) stay below 2^15, and keep
     // their 11 bits down to 2^-20 of that.
     int vexp = 0;
     {
-        const float m = __builtin_fmaxf(__builtin_fmaxf(s_max[0], s_max[1]), __builtin_fmaxf(s_max[2], s_max[3]));
+        float m = s_max[0];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) m = __builtin_fmaxf(m, s_max[w]);
         if (m > 0.0f && m < __builtin_inff()) {
             (void)__builtin_frexpf(m, &vexp);
             vexp = 7 - vexp;
         }
     }
-    for (int i = threadIdx.x; i < n_tok; i += 256) s_vs[i] = __builtin_ldexpf(s_vs[i], vexp);
-    __syncthreads();
+    for (int i = threadIdx.x; i < n_tok; i += NT) s_vs[i] = __builtin_ldexpf(s_vs[i], vexp);  // used after the next barrier
 
-    const int n16 = lane & 15, kg = lane >> 4, quad = lane >> 2, qq = lane & 3;
-    const int from_quad = 4 * (4 * n16 + kg);  // byte address of the lane that loaded this lane's block
-    auto permute = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_ds_bpermute(from_quad, (int)v); };
-    auto permute_f = [&](float v) { return __builtin_bit_cast(float, permute(__builtin_bit_cast(uint32_t, v))); };
-
-    for (int s0 = 0; s0 < n_tok; s0 += kSharedStage) {
-        const int left = min(n_tok - s0, kSharedStage);
-        const int units = 2 * ((left + 31) / 32);  // whole tiles: slots past the chunk repeat its last token
-        // ---- 1. keys: 16 tokens (a unit) of a wave at a time ----
-        for (int u = wave; u < units; u += 4) {
-            const int tq = min(s0 + 16 * u + quad, n_tok - 1), tn = min(s0 + 16 * u + n16, n_tok - 1);
-            uint32_t code[2][KM::NK][KM::W];
-            {
-                const int8_t* const p = a.kc + (size_t)s_row[tq] * D + KM::KPL * qq;
+    // ---- a stage's codes: 16 tokens of keys (a unit), and pieces of values, to registers ----
+    // Loaded a quad per token, 64 consecutive bytes; the MFMA operands want token n16 and 16-byte block
+    // kg in lane 16 kg + n16, so the lanes exchange them when they decode.
+    KM signs;
+    signs.init(lane);
+    uint32_t kcode[2][KM::NK][KM::W];
+    u32x4 vcode[SH::PIECES];
+    auto load_keys = [&](int s0, int u) {
+        const int tq = min(s0 + 16 * (NW * u + wave) + (lane >> 2), n_tok - 1);  // slots past the chunk repeat its last token
+        const int8_t* const p = a.kc + (size_t)s_row[tq] * D + KM::KPL * (lane & 3);
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf)
+        for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-                    for (int s = 0; s < KM::NK; ++s) {
-                        const uint32_t* const w = reinterpret_cast<const uint32_t*>(p + hf * KM::HALF + s * KM::KB);
+            for (int s = 0; s < KM::NK; ++s) {
+                const uint32_t* const w = reinterpret_cast<const uint32_t*>(p + hf * KM::HALF + s * KM::KB);
 #pragma unroll
-                        for (int i = 0; i < KM::W; ++i) code[hf][s][i] = w[i];
-                    }
+                for (int i = 0; i < KM::W; ++i) kcode[hf][s][i] = w[i];
             }
+    };
+    auto load_values = [&](int s0) {
+#pragma unroll
+        for (int i = 0; i < SH::PIECES; ++i) {
+            const int j = NT * i + threadIdx.x, t = min(s0 + j / (D / 16), n_tok - 1);
+            vcode[i] = *reinterpret_cast<const u32x4*>(a.vc + (size_t)s_row[t] * D + 16 * (j % (D / 16)));
+        }
+    };
+    // The stage at s0 to LDS.  MANY: its codes are in registers, and those of the stage after it follow.
+    auto decode = [&](int s0, char* kbuf) {
+        char* const vbuf = kbuf + STAGE * ROWB;
+        // what follows from the lane alone (operand signs, addresses) is worked out again in each stage:
+        // kept across stages it would take 40 registers that the attention needs
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        const int n16 = lane & 15, kg = lane >> 4, quad = lane >> 2, qq = lane & 3;
+        const int from_quad = 4 * (4 * n16 + kg);  // byte address of the lane that loaded this lane's block
+        auto permute = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_ds_bpermute(from_quad, (int)v); };
+        auto permute_f = [&](float v) { return __builtin_bit_cast(float, permute(__builtin_bit_cast(uint32_t, v))); };
+        KM km = signs;
+#pragma unroll
+        for (int w = 0; w < KM::W; ++w) asm volatile("" : "+v"(km.h[w]));
+        const int tid = 64 * wave + lane;
+        if constexpr (!MANY) load_values(s0);
+#pragma unroll
+        for (int i = 0; i < SH::PIECES; ++i) {
+            const int j = NT * i + tid, row = j / (D / 16), piece = j % (D / 16);
+            u32x4 o[2];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                half2v lo, hi;
+                codes_to_f16(vcode[i][k], lo, hi);
+                o[k / 2][2 * (k & 1)] = __builtin_bit_cast(uint32_t, lo);
+                o[k / 2][2 * (k & 1) + 1] = __builtin_bit_cast(uint32_t, hi);
+            }
+            const int f = T::value_swizzle(row);
+            *reinterpret_cast<u32x4*>(vbuf + row * ROWB + 16 * ((2 * piece) ^ f)) = o[0];
+            *reinterpret_cast<u32x4*>(vbuf + row * ROWB + 16 * ((2 * piece + 1) ^ f)) = o[1];
+        }
+        const bool more = MANY && s0 + STAGE < n_tok;
+        if (more) load_values(s0 + STAGE);
+#pragma unroll 1
+        for (int u = 0; u < SH::UNITS; ++u) {
+            const int row = 16 * (NW * u + wave) + n16;
+            const int tq = min(s0 + 16 * (NW * u + wave) + quad, n_tok - 1), tn = min(s0 + row, n_tok - 1);
             const size_t tab = (size_t)s_pos[tq] * (D / 2) + 4 * qq;
             const float k_scale = (0.5f * f16_bits_to_f32(s_ks[tn])) * a.hscale;
+            if constexpr (!MANY) load_keys(s0, u);
+            uint32_t code[2][KM::NK][KM::W];
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
                 for (int s = 0; s < KM::NK; ++s)
 #pragma unroll
-                    for (int i = 0; i < KM::W; ++i) code[hf][s][i] = permute(code[hf][s][i]);
-            const int row = 16 * u + n16;
+                    for (int i = 0; i < KM::W; ++i) code[hf][s][i] = permute(kcode[hf][s][i]);
             char* const to = kbuf + row * ROWB + 8 * (kg & 1);
 #pragma unroll
             for (int t = 0; t < KM::T; ++t) {
@@ -216,34 +273,52 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
                     u32x2{pack2<NQ_F16>(x[4], x[5]), pack2<NQ_F16>(x[6], x[7])};
             }
         }
-        // ---- values: 16 codes of a token a lane ----
-        for (int i = threadIdx.x; i < 16 * units * (D / 16); i += 256) {
-            const int row = i / (D / 16), piece = i % (D / 16);
-            const int t = min(s0 + row, n_tok - 1);
-            const u32x4 w = *reinterpret_cast<const u32x4*>(a.vc + (size_t)s_row[t] * D + 16 * piece);
-            u32x4 o[2];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                half2v lo, hi;
-                codes_to_f16(w[k], lo, hi);
-                o[k / 2][2 * (k & 1)] = __builtin_bit_cast(uint32_t, lo);
-                o[k / 2][2 * (k & 1) + 1] = __builtin_bit_cast(uint32_t, hi);
+        if (more) load_keys(s0 + STAGE, 0);
+    };
+    auto attend = [&](int s0, const char* kbuf) {
+        if (!live) return;
+        asm volatile("" : "+v"(rows.k_at), "+v"(rows.v_at));  // its addresses, as in decode
+        const char* const vbuf = kbuf + STAGE * ROWB;
+        const int left = n_tok - s0;
+        const int t1 = min(tile0 + per_wave, (min(left, STAGE) + 31) / 32);
+        int t = tile0;
+        if constexpr (MANY)
+#pragma unroll 1
+        for (; t + 1 < t1 && 32 * (t + 2) <= left; t += 2)
+            rows.template two_tiles<true>(kbuf, vbuf, t, c, g, s_vs + s0 + 32 * t);
+#pragma unroll 1
+        for (; t < t1; ++t) rows.template masked_tile<true>(kbuf, vbuf, t, c, 0, left - 32 * t, g, s_vs + s0 + 32 * t);
+    };
+
+    if constexpr (MANY) {
+        static_assert(SH::UNITS == 1, "a wave's keys of the next stage are one unit");
+        load_keys(0, 0);
+        load_values(0);
+        // ---- the stages: one is decoded while the one before it is attended to ----
+        // A SIMD's two waves do these in opposite order, so that one's matrix products run under the other's
+        // conversions.
+        decode(0, s_kv[0]);
+        __syncthreads();
+        const bool decode_first = wave >= NW / 2;
+        int at = 0;
+        for (int s0 = 0; s0 < n_tok; s0 += STAGE, at ^= 1) {
+#pragma unroll 1
+            for (int part = 0; part < 2; ++part) {
+                if ((part == 0) == decode_first) {
+                    if (s0 + STAGE < n_tok) decode(s0 + STAGE, s_kv[(at ^ 1) % SH::BUFS]);
+                } else {
+                    attend(s0, s_kv[at % SH::BUFS]);
+                }
             }
-            const int f = T::value_swizzle(row);
-            *reinterpret_cast<u32x4*>(vbuf + row * ROWB + 16 * ((2 * piece) ^ f)) = o[0];
-            *reinterpret_cast<u32x4*>(vbuf + row * ROWB + 16 * ((2 * piece + 1) ^ f)) = o[1];
+            __syncthreads();
         }
-        __syncthreads();
-        // ---- 2. attention ----
-        if (live) {
-            const int t1 = min(tile0 + rw, units / 2);
-            int t = tile0;
-#pragma unroll 1
-            for (; t + 1 < t1 && 32 * (t + 2) <= left; t += 2) rows.template two_tiles<true>(kbuf, vbuf, t, c, g, s_vs + s0 + 32 * t);
-#pragma unroll 1
-            for (; t < t1; ++t) rows.template masked_tile<true>(kbuf, vbuf, t, c, 0, left - 32 * t, g, s_vs + s0 + 32 * t);
+    } else {
+        for (int s0 = 0; s0 < n_tok; s0 += STAGE) {
+            decode(s0, s_kv[0]);
+            __syncthreads();
+            attend(s0, s_kv[0]);
+            __syncthreads();
         }
-        __syncthreads();
     }
 
     // ---- the waves' sums joined, and written ----
@@ -255,7 +330,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
     __syncthreads();
     {
         float m = kNoMax;
-        for (int w = wave % rw; w < 4; w += rw) m = __builtin_fmaxf(m, s_m[w][n]);
+        for (int w = wave % rw; w < NW; w += rw) m = __builtin_fmaxf(m, s_m[w][n]);
         const float f = __builtin_ldexpf(__builtin_amdgcn_exp2f(rows.m - m), -1 - vexp);
         // [wave][query][coordinate], 16-byte chunks at chunk ^ query
         float* const area = reinterpret_cast<float*>(s_kv) + (wave * 32 + n) * D;
@@ -263,24 +338,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
         for (int b = 0; b < T::DB; ++b)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int at = (8 * b + 2 * i + g) ^ (n & 15);
-                *reinterpret_cast<f32x4*>(area + 4 * at) = f32x4{rows.o[b][4 * i] * f, rows.o[b][4 * i + 1] * f,
+                const int to = (8 * b + 2 * i + g) ^ (n & 15);
+                *reinterpret_cast<f32x4*>(area + 4 * to) = f32x4{rows.o[b][4 * i] * f, rows.o[b][4 * i + 1] * f,
                                                                  rows.o[b][4 * i + 2] * f, rows.o[b][4 * i + 3] * f};
             }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < n_q * (D / 4); i += 256) {
-        const int r = i / (D / 4), at = i % (D / 4), w0 = r >> 5, q = r & 31;
+    for (int i = threadIdx.x; i < n_q * (D / 4); i += NT) {
+        const int r = i / (D / 4), j = i % (D / 4), w0 = r >> 5, q = r & 31;
         f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int w = w0; w < 4; w += rw)
-            y += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(s_kv) + (w * 32 + q) * D + 4 * (at ^ (q & 15)));
+        for (int w = w0; w < NW; w += rw)
+            y += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(s_kv) + (w * 32 + q) * D + 4 * (j ^ (q & 15)));
         const uint32_t br = div((uint32_t)r, a.by_group);
         const size_t slot = (size_t)(uint32_t)(seg_rows[2 * br + 1] + chunk) * a.q_heads + kh * G + ((uint32_t)r - br * G);
-        *reinterpret_cast<f32x4*>(a.part_y + slot * D + 4 * at) = y;
-        if (at == 0) {
+        *reinterpret_cast<f32x4*>(a.part_y + slot * D + 4 * j) = y;
+        if (j == 0) {
             float m = kNoMax, l = 0.0f;
-            for (int w = w0; w < 4; w += rw) m = __builtin_fmaxf(m, s_m[w][q]);
-            for (int w = w0; w < 4; w += rw) l += s_l[w][q] * __builtin_amdgcn_exp2f(s_m[w][q] - m);
+            for (int w = w0; w < NW; w += rw) m = __builtin_fmaxf(m, s_m[w][q]);
+            for (int w = w0; w < NW; w += rw) l += s_l[w][q] * __builtin_amdgcn_exp2f(s_m[w][q] - m);
             a.part_ml[2 * slot] = m;
             a.part_ml[2 * slot + 1] = l;
         }
@@ -341,10 +416,22 @@ __global__ __launch_bounds__(256) void shared_combine_kernel(SharedArgs a) {
     static_cast<uint16_t*>(a.out)[(size_t)blockIdx.x * D + tid] = (uint16_t)(pack2<QDT>(v, 0.0f) & 0xffffu);
 }
 
+// items: those of segments of many query rows first, then the others
 template <int D, int QDT>
-static hipError_t launch_shared(const SharedArgs& a, uint32_t batch, hipStream_t s) {
-    if (a.n_items > 0) {
-        hipLaunchKernelGGL((shared_attn_kernel<D, QDT>), dim3((a.n_items + 7u) / 8u * 8u * a.kv_heads), dim3(256), 0, s, a);
+static hipError_t launch_shared(SharedArgs a, uint32_t n_many, uint32_t n_items, uint32_t batch, hipStream_t s) {
+    const int32_t* const items = a.items;
+    if (n_many > 0) {
+        a.n_items = n_many;
+        hipLaunchKernelGGL((shared_attn_kernel<D, QDT, true>), dim3((n_many + 7u) / 8u * 8u * a.kv_heads),
+                           dim3(Shape<D, true>::THREADS), 0, s, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    if (n_items > n_many) {
+        a.items = items + 8 * (size_t)n_many;
+        a.n_items = n_items - n_many;
+        hipLaunchKernelGGL((shared_attn_kernel<D, QDT, false>), dim3((a.n_items + 7u) / 8u * 8u * a.kv_heads),
+                           dim3(Shape<D, false>::THREADS), 0, s, a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
@@ -353,18 +440,22 @@ static hipError_t launch_shared(const SharedArgs& a, uint32_t batch, hipStream_t
 }
 
 template <int QDT>
-static hipError_t shared_dims(int32_t d, const SharedArgs& a, uint32_t batch, hipStream_t s) {
+static hipError_t shared_dims(int32_t d, const SharedArgs& a, uint32_t n_many, uint32_t n_items, uint32_t batch, hipStream_t s) {
     switch (d) {
-        case 64: return launch_shared<64, QDT>(a, batch, s);
-        case 128: return launch_shared<128, QDT>(a, batch, s);
-        default: return launch_shared<256, QDT>(a, batch, s);
+        case 64: return launch_shared<64, QDT>(a, n_many, n_items, batch, s);
+        case 128: return launch_shared<128, QDT>(a, n_many, n_items, batch, s);
+        default: return launch_shared<256, QDT>(a, n_many, n_items, batch, s);
     }
 }
 
 }  // namespace nq
 
 extern "C" int32_t nq_shared_attention_chunk_tokens(void) { return nq::kSharedChunk; }
-extern "C" int32_t nq_shared_attention_rows(void) { return nq::kSharedRows; }
+extern "C" int32_t nq_shared_attention_rows(int32_t head_dim) {
+    return head_dim <= 128 ? nq::Shape<128, true>::ROWS : nq::Shape<256, true>::ROWS;
+}
+
+extern "C" int32_t nq_shared_attention_few_rows(void) { return nq::kFewRows; }
 
 extern "C" int64_t nq_shared_attention_workspace(int32_t n_slots, int32_t q_heads, int32_t head_dim) {
     if (n_slots <= 0 || q_heads <= 0 || head_dim <= 0) return 0;
@@ -382,15 +473,17 @@ extern "C" int nq_shared_attention(const nq_shared_desc* d, void* stream) {
     NQ_CHECK_ARG((uint64_t)p->pages * p->heads * p->tokens < (1ull << 31),
                  "nq_shared_attention: a layer must have less than 2^31 token rows");
     NQ_CHECK_ARG(d->q_dtype == NQ_F16 || d->q_dtype == NQ_BF16, "nq_shared_attention: queries must be fp16 or bf16");
-    NQ_CHECK_ARG(d->batch >= 0 && d->q_heads > 0 && d->q_heads % p->heads == 0 && d->q_heads / p->heads <= kSharedRows,
+    NQ_CHECK_ARG(d->batch >= 0 && d->q_heads > 0 && d->q_heads % p->heads == 0 &&
+                     d->q_heads / p->heads <= nq_shared_attention_rows(p->head_dim),
                  "nq_shared_attention: q_heads %d must be a multiple of the pool's %d heads, at most %d times", d->q_heads,
-                 p->heads, kSharedRows);
-    NQ_CHECK_ARG(d->n_items >= 0 && d->n_slots >= 0, "nq_shared_attention: n_items %d, n_slots %d", d->n_items, d->n_slots);
+                 p->heads, nq_shared_attention_rows(p->head_dim));
+    NQ_CHECK_ARG(d->n_items >= 0 && d->n_slots >= 0 && d->n_many >= 0 && d->n_many <= d->n_items,
+                 "nq_shared_attention: n_items %d, n_many %d, n_slots %d", d->n_items, d->n_many, d->n_slots);
     if (d->batch == 0) return NQ_OK;
     NQ_CHECK_ARG(d->query && d->out && d->row_slots, "nq_shared_attention: query, out and row_slots are required");
     NQ_CHECK_ARG(((uintptr_t)d->query & 15u) == 0, "nq_shared_attention: query must be 16-byte aligned");
     NQ_CHECK_ARG((uint64_t)d->batch * d->q_heads <= max_blocks(256) &&
-                     ((uint64_t)d->n_items + 7) * p->heads <= max_blocks(256), "nq_shared_attention: grid too large");
+                     ((uint64_t)d->n_items + 7) * p->heads <= max_blocks(512), "nq_shared_attention: grid too large");
     SharedArgs a = {};
     if (d->n_items > 0) {
         NQ_CHECK_ARG(d->items && d->pages && d->seg_rows, "nq_shared_attention: the plan's arrays are required");
@@ -426,14 +519,13 @@ extern "C" int nq_shared_attention(const nq_shared_desc* d, void* stream) {
     a.q_heads = (uint32_t)d->q_heads;
     a.kv_heads = (uint32_t)p->heads;
     a.rope_n_pos = (uint32_t)(d->rope_n_pos > 0 ? d->rope_n_pos : 1);
-    a.n_items = (uint32_t)d->n_items;
     a.tokens = (uint32_t)p->tokens;
     a.by_tokens = fast_div(a.tokens);
     a.by_group = fast_div(a.q_heads / a.kv_heads);
     a.c = 1.44269504088896340736f / (d->scale_divisor > 0.0f ? d->scale_divisor : 1.0f);
     a.hscale = d->hadamard_scale;
     hipStream_t s = (hipStream_t)stream;
-    NQ_CHECK_HIP(d->q_dtype == NQ_F16 ? shared_dims<NQ_F16>(p->head_dim, a, (uint32_t)d->batch, s)
-                                      : shared_dims<NQ_BF16>(p->head_dim, a, (uint32_t)d->batch, s));
+    NQ_CHECK_HIP(d->q_dtype == NQ_F16 ? shared_dims<NQ_F16>(p->head_dim, a, (uint32_t)d->n_many, (uint32_t)d->n_items, (uint32_t)d->batch, s)
+                                      : shared_dims<NQ_BF16>(p->head_dim, a, (uint32_t)d->n_many, (uint32_t)d->n_items, (uint32_t)d->batch, s));
     return NQ_OK;
 }

@@ -505,57 +505,62 @@ def shared_segments(tables: Sequence[np.ndarray], lengths: Sequence[int], page_t
     return out
 
 
-# Workgroups that a launch should have before its chunks stay long: two on each of 256 CUs.
-_SHARED_WORKGROUPS = 512
+# Workgroups that a launch should have before its chunks stay long: of segments of many query rows one for
+# each of 256 CUs, of the others two.
+_SHARED_WORKGROUPS = {True: 256, False: 512}
 _SHARED_STAGE = 128
 
 
-def shared_items(segments, batch: int, tile_rows: int, kv_heads: int, cap: int):
-    """The work list of nq_shared_attention: int32 arrays items, pages, seg_rows, row_slots, and the
-    counts of items and slots.  Chunks are `cap` tokens, halved down to one stage of 128 while the
-    launch would have fewer than _SHARED_WORKGROUPS workgroups."""
-    tiles = [-(-len(rows) // tile_rows) for rows, _, _ in segments]
+def _shared_chunk(segments, tiles, kv_heads: int, cap: int, many: bool) -> int:
+    """Chunk length of one kind of segments: `cap` tokens, halved down to one stage of 128 while the launch
+    would have fewer than _SHARED_WORKGROUPS workgroups."""
     length = cap
     while length > _SHARED_STAGE and kv_heads * sum(
-            t * -(-n // length) for t, (_, _, n) in zip(tiles, segments)) < _SHARED_WORKGROUPS:
+            t * -(-n // length) for t, (_, _, n) in zip(tiles, segments)) < _SHARED_WORKGROUPS[many]:
         length //= 2
-    per_row = np.zeros(batch + 1, dtype=np.int64)
-    chunks = []
-    for rows, _, n in segments:
-        chunks.append(-(-n // length))
-        per_row[np.asarray(rows) + 1] += chunks[-1]
+    return length
+
+
+def shared_items(segments, batch: int, group: int, kv_heads: int, cap: int, rows_of_many: int, few_rows: int):
+    """The work list of nq_shared_attention: int32 arrays items, pages, seg_rows, row_slots, and the counts of
+    items, of those among them that come first (of segments of more than few_rows query rows) and of slots."""
+    many = [len(rows) * group > few_rows for rows, _, _ in segments]
+    per_tile = max(1, rows_of_many // group)  # batch rows of a workgroup
+    tiles = [-(-len(rows) // per_tile) for rows, _, _ in segments]
+    length = {}
+    for kind in (True, False):
+        of = [i for i in range(len(segments)) if many[i] == kind]
+        length[kind] = _shared_chunk([segments[i] for i in of], [tiles[i] for i in of], kv_heads, cap, kind)
+    chunks = [-(-s[2] // length[m]) for s, m in zip(segments, many)]
+    per_row = [0] * (batch + 1)
+    for (rows, _, _), c in zip(segments, chunks):
+        for b in rows:
+            per_row[b + 1] += c
     row_slots = np.cumsum(per_row)
-    nxt = row_slots[:-1].copy()
+    nxt = row_slots[:-1].tolist()
     records, seg_rows, pages = [], [], []
-    at_rows = at_pages = 0
-    order = sorted(range(len(segments)), key=lambda i: -len(segments[i][0]))  # the dear ones first
-    for i in order:
+    at_pages = 0
+    # those of many rows first, long ones before short ones
+    for i in sorted(range(len(segments)), key=lambda i: (not many[i], -segments[i][2])):
         rows, seg_pages, n = segments[i]
-        rows = np.asarray(rows)
-        seg_rows.append(np.stack([rows, nxt[rows]], axis=1))
-        nxt[rows] += chunks[i]
-        c = np.arange(chunks[i])
-        r0 = np.arange(tiles[i]) * tile_rows
+        at_rows = len(seg_rows)
+        for b in rows:
+            seg_rows.append((b, nxt[b]))
+            nxt[b] += chunks[i]
         # chunks in eights (one for each XCD), a chunk's row tiles one eight after another
-        cc, rr = np.repeat(c, tiles[i]), np.tile(r0, chunks[i])
-        by = np.lexsort((cc % 8, rr, cc // 8))
-        cc, rr = cc[by], rr[by]
-        rec = np.zeros((len(cc), 8), dtype=np.int64)
-        rec[:, 0] = at_pages
-        rec[:, 1] = cc * length
-        rec[:, 2] = np.minimum(n - cc * length, length)
-        rec[:, 3] = at_rows + rr
-        rec[:, 4] = np.minimum(len(rows) - rr, tile_rows)
-        rec[:, 5] = cc
-        records.append(rec)
-        pages.append(np.asarray(seg_pages))
-        at_rows += len(rows)
+        step = length[many[i]]
+        for c0 in range(0, chunks[i], 8):
+            for r0 in range(0, len(rows), per_tile):
+                for c in range(c0, min(c0 + 8, chunks[i])):
+                    records.append((at_pages, c * step, min(n - c * step, step), at_rows + r0,
+                                    min(len(rows) - r0, per_tile), c, 0, 0))
+        pages.append(np.asarray(seg_pages, dtype=np.int32))
         at_pages += len(seg_pages)
-    empty = np.zeros(0, dtype=np.int64)
-    items = np.concatenate(records).reshape(-1) if records else empty
-    parts = {"items": items, "pages": np.concatenate(pages) if pages else empty,
-             "seg_rows": np.concatenate(seg_rows).reshape(-1) if seg_rows else empty, "row_slots": row_slots}
-    return parts, len(items) // 8, int(row_slots[-1])
+    n_many = sum(t * c for t, c, m in zip(tiles, chunks, many) if m)
+    parts = {"items": np.array(records, dtype=np.int32).reshape(-1),
+             "pages": np.concatenate(pages) if pages else np.zeros(0, dtype=np.int32),
+             "seg_rows": np.array(seg_rows, dtype=np.int32).reshape(-1), "row_slots": row_slots.astype(np.int32)}
+    return parts, len(records), n_many, int(row_slots[-1])
 
 
 class SharedAttentionPlan:
@@ -570,22 +575,23 @@ class SharedAttentionPlan:
         self._work: Dict[int, tuple] = {}
 
     def work(self, q_heads: int):
-        """(device ints, offsets, items, slots) for q_heads query heads."""
+        """(device ints, offsets, items, items of many rows, slots) for q_heads query heads."""
         got = self._work.get(q_heads)
         if got is None:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("run_shared: run the plan once before capturing it into a graph")
             lib = _lib.load()
-            group = q_heads // self.pool.num_heads
-            parts, n_items, n_slots = shared_items(self.segments, self.batch,
-                                                   int(lib.nq_shared_attention_rows()) // group, self.pool.num_heads,
-                                                   int(lib.nq_shared_attention_chunk_tokens()))
+            heads = self.pool.num_heads
+            parts, *counts = shared_items(self.segments, self.batch, q_heads // heads, heads,
+                                          int(lib.nq_shared_attention_chunk_tokens()),
+                                          int(lib.nq_shared_attention_rows(self.pool.head_dim)),
+                                          int(lib.nq_shared_attention_few_rows()))
             offsets, at = {}, 0
             for name, v in parts.items():
                 offsets[name] = at
                 at += len(v)
             ints = PlanTensor(np.concatenate(list(parts.values())), self.pool.device)
-            got = self._work[q_heads] = (ints, offsets, n_items, n_slots)
+            got = self._work[q_heads] = (ints, offsets, *counts)
         return got
 
 
@@ -782,7 +788,7 @@ class NexusQuantPagedAttention:
         if query.dtype not in (torch.float16, torch.bfloat16):
             raise ValueError(f"run_shared takes fp16 or bf16 queries, got {query.dtype}; run() takes fp32 ones")
         b, hq, d = query.shape
-        rows = int(lib.nq_shared_attention_rows())
+        rows = int(lib.nq_shared_attention_rows(d))
         if hq == 0 or hq % pool.num_heads or hq // pool.num_heads > rows:
             raise ValueError(f"num_heads {hq} is not a multiple (up to {rows}) of the pool's {pool.num_heads}")
         if not 0 <= int(layer) < pool.num_layers:
@@ -796,7 +802,7 @@ class NexusQuantPagedAttention:
             q = q.clone()
         dev = pool.device
         with torch.cuda.device(dev):
-            ints, offsets, n_items, n_slots = plan.work(hq)
+            ints, offsets, n_items, n_many, n_slots = plan.work(hq)
             nbytes = lib.nq_shared_attention_workspace(n_slots, hq, d)
             # of this call alone: calls on other streams and captured graphs have their own
             ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
@@ -804,7 +810,7 @@ class NexusQuantPagedAttention:
             base = ints.address()
             desc = _lib.SharedDesc(
                 pool=ctypes.pointer(pool.desc), layer=int(layer), batch=b, q_heads=hq, q_dtype=_lib.dtype_code(q.dtype),
-                n_items=n_items, n_slots=n_slots, query=_addr(q), out=_addr(out), items=base + 4 * offsets["items"],
+                n_items=n_items, n_many=n_many, n_slots=n_slots, query=_addr(q), out=_addr(out), items=base + 4 * offsets["items"],
                 pages=base + 4 * offsets["pages"], seg_rows=base + 4 * offsets["seg_rows"],
                 row_slots=base + 4 * offsets["row_slots"], rope_sin_minus_cos=_addr(dm), rope_cos_plus_sin=_addr(dp),
                 rope_n_pos=dm.shape[0], hadamard_scale=hadamard_constant(d),

@@ -64,6 +64,7 @@ def desc(**kw):
     dict(sliding_window=-1), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None),
     dict(tiles=None), dict(out=ctypes.c_void_p(4100)), dict(v=ctypes.c_void_p(4104)),
     dict(k_stride=(ctypes.c_int64 * 2)(260, 128)), dict(out_stride=(ctypes.c_int64 * 2)(1024, 130)),
+    dict(k_stride=(ctypes.c_int64 * 2)(1 << 24, 128)), dict(v_stride=(ctypes.c_int64 * 2)(-256, 128)),
     dict(n_tiles=1 << 24), dict(q_heads=1 << 30, kv_heads=1)])
 def test_c_entry_refuses(kw):
     lib = _lib.load()

@@ -63,19 +63,20 @@ def test_what_is_shared_is_in_one_segment():
     assert sorted((rows, n) for rows, _, n in segs) == [([0, 1], 496), ([2, 3], 496)]
 
 
-@pytest.mark.parametrize("tile_rows,kv_heads,cap", [(128, 8, 1024), (32, 1, 1024), (1, 2, 256), (16, 64, 128)])
-def test_items_cover_each_rows_tokens_and_slots_once(tile_rows, kv_heads, cap):
-    r = np.random.RandomState(tile_rows)
+@pytest.mark.parametrize("group,kv_heads,cap,most,few", [(1, 8, 1024, 128, 32), (4, 1, 1024, 128, 32), (128, 2, 256, 128, 32),
+                                                         (8, 64, 128, 128, 0), (2, 3, 1024, 256, 1000)])
+def test_items_cover_each_rows_tokens_and_slots_once(group, kv_heads, cap, most, few):
+    r = np.random.RandomState(group)
     batch = 37
     segments = [(list(range(20)), np.arange(300), 4800), ([3, 5, 36], np.arange(400, 410), 160)]
     segments += [([b], np.arange(1000 + 10 * b, 1010 + 10 * b), int(r.randint(1, 160))) for b in range(30)]
-    parts, n_items, n_slots = shared_items(segments, batch, tile_rows, kv_heads, cap)
+    parts, n_items, n_many, n_slots = shared_items(segments, batch, group, kv_heads, cap, most, few)
     items = parts["items"].reshape(-1, 8)
     rows = parts["seg_rows"].reshape(-1, 2)
     assert len(items) == n_items and parts["row_slots"][0] == 0 and parts["row_slots"][-1] == n_slots
     seen, slots = {}, []
-    for page0, tok0, n, row0, n_rows, chunk, _, _ in items:
-        assert 1 <= n <= cap and 1 <= n_rows <= tile_rows
+    for i, (page0, tok0, n, row0, n_rows, chunk, _, _) in enumerate(items):
+        assert 1 <= n <= cap and 1 <= n_rows and n_rows * group <= (most if i < n_many else few)
         for b, slot0 in rows[row0:row0 + n_rows]:
             slots.append(slot0 + chunk)
             assert parts["row_slots"][b] <= slot0 + chunk < parts["row_slots"][b + 1]
@@ -85,11 +86,12 @@ def test_items_cover_each_rows_tokens_and_slots_once(tile_rows, kv_heads, cap):
                 seen[key] = 1
     assert sorted(slots) == list(range(n_slots))
     assert len(seen) == sum(len(s[0]) * s[2] for s in segments)
+    assert n_many == (0 if few == 1000 else n_items if group * 1 > few else n_many) and n_many <= n_items
 
 
 def test_no_rows_and_no_tokens():
-    parts, n_items, n_slots = shared_items([], 3, 128, 8, 1024)
-    assert n_items == 0 and n_slots == 0 and list(parts["row_slots"]) == [0, 0, 0, 0]
+    parts, n_items, n_many, n_slots = shared_items([], 3, 4, 8, 1024, 256, 32)
+    assert n_items == n_many == n_slots == 0 and list(parts["row_slots"]) == [0, 0, 0, 0]
 
 
 def test_plan_refuses_bad_tables(monkeypatch):
@@ -119,7 +121,7 @@ def test_shared_struct_matches_the_c_compiler(tmp_path):
 
 @pytest.mark.parametrize("kw,pool_kw", [
     (dict(layer=1), {}), (dict(layer=-1), {}), (dict(batch=-1), {}), (dict(q_heads=0), {}), (dict(q_heads=3), {}),
-    (dict(q_heads=2 * 129), {}), (dict(q_dtype=_lib.NQ_F32), {}), (dict(n_items=-1), {}), (dict(n_slots=0), {}),
+    (dict(q_heads=2 * 257), {}), (dict(q_dtype=_lib.NQ_F32), {}), (dict(n_items=-1), {}), (dict(n_slots=0), {}), (dict(n_many=2), {}), (dict(n_many=-1), {}),
     (dict(query=None), {}), (dict(query=ctypes.c_void_p(4104)), {}), (dict(out=None), {}), (dict(items=None), {}),
     (dict(row_slots=None), {}), (dict(rope_sin_minus_cos=None), {}), (dict(rope_n_pos=0), {}),
     (dict(workspace=None), {}), (dict(workspace_bytes=100), {}), (dict(workspace=ctypes.c_void_p(4100)), {}),
