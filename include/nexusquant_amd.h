@@ -667,14 +667,14 @@ int nq_pool_write(const nq_pool* pool, int32_t layer, const nq_pool* tokens, con
  * tokens, k and v the pages' keys and values.  The tokens come as segments: pages that a list of
  * rows sees whole; a row's tokens are the union of its segments.
  *   items    [n_items * 8] chunks of segments, up to
- *            nq_shared_attention_chunk_tokens() tokens each:
+ *            nq_shared_attention_chunk_tokens(many) tokens each:
  *              [0] where the segment's pages start in `pages`
  *              [1] the chunk's first token, counted from there
  *              [2] its tokens (1 ..)
  *              [3] where its rows start in `seg_rows` (entries)
  *              [4] rows, at most nq_shared_attention_rows(head_dim) / (q_heads / heads)
  *              [5] the chunk's number in its segment;  [6..7] unused
- *            The first n_many of them may have that many rows; those after
+ *            The first n_many of them (many = 1) may have that many rows; those after
  *            them have at most nq_shared_attention_few_rows() query rows
  *            (rows x q_heads / heads).
  *   pages    page numbers
@@ -710,7 +710,7 @@ typedef struct nq_shared_desc {
     int64_t workspace_bytes;
 } nq_shared_desc;
 
-int32_t nq_shared_attention_chunk_tokens(void);
+int32_t nq_shared_attention_chunk_tokens(int32_t many);
 int32_t nq_shared_attention_rows(int32_t head_dim);
 int32_t nq_shared_attention_few_rows(void);
 int64_t nq_shared_attention_workspace(int32_t n_slots, int32_t q_heads, int32_t head_dim);

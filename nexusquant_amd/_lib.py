@@ -170,7 +170,7 @@ SIGNATURES = {
     "nq_pool_move_tokens": ([], ctypes.c_int32),
     "nq_pool_compact": ([ctypes.POINTER(Pool), _P, _I32, _P, _P, _P, _I32, _I32, _P], ctypes.c_int),
     "nq_pool_write": ([ctypes.POINTER(Pool), _I32, ctypes.POINTER(Pool), _P, _I32, _P], ctypes.c_int),
-    "nq_shared_attention_chunk_tokens": ([], ctypes.c_int32),
+    "nq_shared_attention_chunk_tokens": ([_I32], ctypes.c_int32),
     "nq_shared_attention_rows": ([_I32], ctypes.c_int32),
     "nq_shared_attention_few_rows": ([], ctypes.c_int32),
     "nq_shared_attention_workspace": ([_I32, _I32, _I32], _I64),

@@ -86,7 +86,10 @@ struct Tile {
     static constexpr int KS = D / 16;           // MFMA steps of a logit
     static constexpr int DB = D / 32;           // 32-coordinate blocks of the output
     static __device__ __forceinline__ int key_swizzle(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
-    static __device__ __forceinline__ int value_swizzle(int r) { return D == 64 ? 4 * ((r >> 1) & 1) : 4 * (r & 3); }
+    // (its bit 0 is for writers of two chunks a lane: half of their rows then take the odd one first)
+    static __device__ __forceinline__ int value_swizzle(int r) {
+        return (D == 64 ? 4 * ((r >> 1) & 1) : 4 * (r & 3)) ^ ((r >> 2) & 1);
+    }
 };
 
 template <int DT, int D>

@@ -21,26 +21,24 @@ namespace nq {
 
 using namespace flash;
 
-constexpr int kSharedChunk = 1024;  // most tokens of a chunk: their places and scales stay in LDS
-
-// The shape of a workgroup.  MANY, for segments of more query rows than kFewRows: rows count, so as many as the
-// registers hold (32 a wave) share what is decoded; two stage buffers, 128 KB of LDS at head_dim 128 and 256, so
-// one workgroup on a CU.  Not MANY: decoding counts, and several small workgroups on a CU hide each other's loads.
+// The shape of a workgroup.  MANY: rows count, so as many as the registers hold (32 a wave) share what is decoded,
+// and a stage is decoded under the attention to the one before it; two stage buffers, 128 KB of LDS at head_dim
+// 128 and 256, so one workgroup on a CU.  Not MANY: decoding counts, and several small workgroups on a CU hide
+// each other's loads.  8 kv heads x 128, us: 512 query rows x 32768 tokens 122 (MANY) and 230; 128 rows x
+// 16384 35.0 and 38.9, x 4096 24.8 and 25.5; 64 rows x 8192 23.4 and 23.8; 8 rows (32 heads x 64) 63.6 and 41.
 template <int D, bool MANY>
 struct Shape {
     static constexpr int WAVES = MANY && D <= 128 ? 8 : 4;
     static constexpr int STAGE = MANY && D > 128 ? 64 : 128;  // tokens
     static constexpr int BUFS = MANY ? 2 : 1;
+    static constexpr int CHUNK = MANY ? 2048 : 1024;   // most tokens of a chunk: their places and scales stay in LDS
     static constexpr int THREADS = 64 * WAVES;
     static constexpr int TILES = STAGE / 32;
     static constexpr int ROWS = 32 * WAVES;            // query rows
-    static constexpr int UNITS = STAGE / 16 / WAVES;   // 16-token units of keys a wave
-    static constexpr int PIECES = STAGE * D / 16 / THREADS;  // 16-byte pieces of values a thread
+    static constexpr int UNITS = STAGE / 16 / WAVES;   // 16-token units a wave decodes
     static_assert(BUFS * 2 * STAGE * 2 * D >= WAVES * 32 * D * 4, "the waves' sums must fit the stage buffers");
     static constexpr int PER_SIMD = MANY ? WAVES / 4 : D == 64 ? 3 : D == 128 ? 2 : 1;  // waves
 };
-constexpr int kFewRows = 32;
-
 struct SharedArgs {
     const uint16_t* query;
     void* out;
@@ -63,15 +61,11 @@ struct SharedArgs {
     float hscale;
 };
 
-// fp16 queries of a row, and the power of two taken out of them: bf16 ones are scaled so that the
-// row's largest is in [2^14, 2^15), where all of it that counts is exact in fp16 (8 bits of 11; what
-// falls below 2^-24 is 2^-38 of the largest).
-template <int D, int QDT>
-__device__ __forceinline__ float load_query(const uint16_t* p, u32x4 (&q)[Tile<D>::KS]) {
-    constexpr int KS = Tile<D>::KS;
-#pragma unroll
-    for (int i = 0; i < KS; ++i) q[i] = *reinterpret_cast<const u32x4*>(p + 16 * i);
-    if constexpr (QDT == NQ_F16) return 1.0f;
+// bf16 queries of a row to fp16, and the power of two taken out of them: scaled so that the row's
+// largest is in [2^14, 2^15), where all of it that counts is exact in fp16 (8 bits of 11; what falls
+// below 2^-24 is 2^-38 of the largest).
+template <int KS>
+__device__ __forceinline__ float bf16_queries(u32x4 (&q)[KS]) {
     float big = 0.0f;
 #pragma unroll
     for (int i = 0; i < KS; ++i)
@@ -84,9 +78,8 @@ __device__ __forceinline__ float load_query(const uint16_t* p, u32x4 (&q)[Tile<D
     big = both_max(big);
     int e = 0;
     if (big > 0.0f && big < __builtin_inff()) (void)__builtin_frexpf(big, &e);
-    e -= 15;
-    const float f = __builtin_ldexpf(1.0f, -e < 126 ? -e : 126);  // bf16's subnormals: scaled as far as fp32 reaches
-    if (-e > 126) e = -126;
+    e = max(e - 15, -126);  // bf16's subnormals: scaled as far as fp32 reaches
+    const float f = __builtin_ldexpf(1.0f, -e);
 #pragma unroll
     for (int i = 0; i < KS; ++i)
 #pragma unroll
@@ -105,11 +98,12 @@ shared_attn_kernel(SharedArgs a) {
     using SH = Shape<D, MANY>;
     constexpr int ROWB = T::ROWB, NT = SH::THREADS, NW = SH::WAVES, STAGE = SH::STAGE;
     __shared__ __align__(16) char s_kv[SH::BUFS][2 * STAGE * ROWB];  // stages of keys and values; at the end the waves' sums
-    __shared__ uint32_t s_row[kSharedChunk];    // a token's row of head 0
-    __shared__ uint32_t s_pos[kSharedChunk];    // its rotation table row
-    __shared__ __align__(16) float s_vs[kSharedChunk];  // its value scale times 2^vexp
-    __shared__ uint16_t s_ks[kSharedChunk];     // its key scale (fp16)
+    __shared__ uint32_t s_row[SH::CHUNK];    // a token's row of head 0
+    __shared__ uint32_t s_pos[SH::CHUNK];    // its rotation table row, in bytes
+    __shared__ __align__(16) float s_vs[SH::CHUNK];  // its value scale times 2^vexp
+    __shared__ uint16_t s_ks[SH::CHUNK];     // its key scale (fp16)
     __shared__ float s_max[NW], s_m[NW][32], s_l[NW][32];
+    __shared__ uint32_t s_slot[SH::ROWS];       // a query row's place among the partial sums
 
     const int lane = threadIdx.x & 63, n = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -124,26 +118,8 @@ shared_attn_kernel(SharedArgs a) {
     const int32_t* const seg_rows = a.seg_rows + 2 * it[3];
     const int G = (int)(a.q_heads / a.kv_heads), n_q = it[4] * G, chunk = it[5];
 
-    // ---- the chunk's tokens ----
-    float vmax = 0.0f;
-    const uint32_t head_rows = kh * a.tokens;
-    for (int i = threadIdx.x; i < n_tok; i += NT) {
-        const uint32_t t = tok0 + i, p = div(t, a.by_tokens), off = t - p * a.tokens;
-        const uint32_t page = (uint32_t)pages[p];
-        const uint32_t row = page * a.kv_heads * a.tokens + head_rows + off;
-        const int32_t pos = a.positions[page * a.tokens + off];
-        const float vs = f16_bits_to_f32(a.vs[row]);
-        s_row[i] = row;
-        s_pos[i] = pos < 0 ? 0u : ((uint32_t)pos >= a.rope_n_pos ? a.rope_n_pos - 1u : (uint32_t)pos);
-        s_ks[i] = a.ks[row];
-        s_vs[i] = vs;
-        vmax = __builtin_fmaxf(vmax, __builtin_fabsf(vs));
-    }
-    for (int i = n_tok + threadIdx.x; i < (n_tok + 31) / 32 * 32; i += NT) s_vs[i] = 0.0f;  // slots of the last tile
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) vmax = __builtin_fmaxf(vmax, __shfl_xor(vmax, o, 64));
-    if (lane == 0) s_max[wave] = vmax;
-
+    // The three chains of loads that the first stage waits for run at once: rows -> queries, pages -> codes,
+    // pages -> positions and scales (-> rotation tables).
     // ---- this wave's queries ----
     int rw = 1;  // waves with rows of their own; the others share these rows and take other tiles
     while (rw < NW && n_q > 32 * rw) rw *= 2;
@@ -152,12 +128,78 @@ shared_attn_kernel(SharedArgs a) {
     const bool live = r0 < n_q && tile0 < SH::TILES;
     Rows<NQ_F16, D> rows;
     rows.init(lane);
-    float c = a.c;
     {
         const uint32_t r = (uint32_t)min(r0 + n, n_q - 1), br = div(r, a.by_group);
         const uint32_t head = kh * G + (r - br * G);
-        c *= load_query<D, QDT>(a.query + ((size_t)(uint32_t)seg_rows[2 * br] * a.q_heads + head) * D + 8 * g, rows.q);
+        const uint16_t* const q = a.query + ((size_t)(uint32_t)seg_rows[2 * br] * a.q_heads + head) * D + 8 * g;
+#pragma unroll
+        for (int i = 0; i < T::KS; ++i) rows.q[i] = *reinterpret_cast<const u32x4*>(q + 16 * i);
     }
+
+    // ---- the codes of a unit, 16 tokens, to registers ----
+    // Keys a quad per token, 64 consecutive bytes; the MFMA operands want token n16 and 16-byte block kg in
+    // lane 16 kg + n16, so the lanes exchange them when they decode.
+    constexpr int PIECES = D / 64;  // 16-byte pieces of a unit's values a lane
+    uint32_t kcode[SH::UNITS][2][KM::NK][KM::W];
+    u32x4 vcode[SH::UNITS][PIECES];
+    auto load = [&](int s0, auto&& row_of) {
+#pragma unroll
+        for (int u = 0; u < SH::UNITS; ++u) {
+            const int first = s0 + 16 * (NW * u + wave);
+            const int8_t* const p = a.kc + (size_t)row_of(first + (lane >> 2)) * D + KM::KPL * (lane & 3);
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                for (int s = 0; s < KM::NK; ++s) {
+                    const uint32_t* const w = reinterpret_cast<const uint32_t*>(p + hf * KM::HALF + s * KM::KB);
+#pragma unroll
+                    for (int i = 0; i < KM::W; ++i) kcode[u][hf][s][i] = w[i];
+                }
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const uint32_t j = 64u * i + lane;
+                vcode[u][i] = *reinterpret_cast<const u32x4*>(a.vc + (size_t)row_of(first + j / (D / 16)) * D + 16 * (j % (D / 16)));
+            }
+        }
+    };
+    for (int r = threadIdx.x; r < n_q; r += NT) {
+        const uint32_t br = div((uint32_t)r, a.by_group);
+        s_slot[r] = (uint32_t)(seg_rows[2 * br + 1] + chunk) * a.q_heads + kh * G + ((uint32_t)r - br * G);
+    }
+    // a slot's place: slots past the chunk repeat its last token (with weight 0)
+    const uint32_t head_rows = kh * a.tokens;
+    auto page_of = [&](int i, uint32_t& off) {
+        const uint32_t t = tok0 + min(i, n_tok - 1), p = div(t, a.by_tokens);
+        off = t - p * a.tokens;
+        return (uint32_t)pages[p];
+    };
+    load(0, [&](int i) {
+        uint32_t off;
+        const uint32_t page = page_of(i, off);
+        return page * a.kv_heads * a.tokens + head_rows + off;
+    });
+
+    // ---- the chunk's tokens ----
+    float vmax = 0.0f;
+    const int n_slots = (n_tok + STAGE - 1) / STAGE * STAGE;
+    for (int i = threadIdx.x; i < n_slots; i += NT) {
+        uint32_t off;
+        const uint32_t page = page_of(i, off), row = page * a.kv_heads * a.tokens + head_rows + off;
+        const int32_t pos = a.positions[page * a.tokens + off];
+        const float vs = i < n_tok ? f16_bits_to_f32(a.vs[row]) : 0.0f;
+        s_row[i] = row;
+        s_pos[i] = (pos < 0 ? 0u : ((uint32_t)pos >= a.rope_n_pos ? a.rope_n_pos - 1u : (uint32_t)pos)) * (2u * D);
+        s_ks[i] = a.ks[row];
+        s_vs[i] = vs;
+        vmax = __builtin_fmaxf(vmax, __builtin_fabsf(vs));
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) vmax = __builtin_fmaxf(vmax, __shfl_xor(vmax, o, 64));
+    if (lane == 0) s_max[wave] = vmax;
+    float c = a.c;
+    if constexpr (QDT == NQ_BF16) c *= bf16_queries(rows.q);
+    KM signs;
+    signs.init(lane);
     __syncthreads();
     // The values' scales go with the weights, so that the codes are exact in fp16 and one rounding is left.
     // Times 2^vexp the chunk's largest is in [64, 128): weights (at most 2^kSlack) stay below 2^15, and keep
@@ -172,86 +214,78 @@ shared_attn_kernel(SharedArgs a) {
             vexp = 7 - vexp;
         }
     }
-    for (int i = threadIdx.x; i < n_tok; i += NT) s_vs[i] = __builtin_ldexpf(s_vs[i], vexp);  // used after the next barrier
+    for (int i = threadIdx.x; i < n_slots; i += NT) s_vs[i] = __builtin_ldexpf(s_vs[i], vexp);  // used after the next barrier
 
-    // ---- a stage's codes: 16 tokens of keys (a unit), and pieces of values, to registers ----
-    // Loaded a quad per token, 64 consecutive bytes; the MFMA operands want token n16 and 16-byte block
-    // kg in lane 16 kg + n16, so the lanes exchange them when they decode.
-    KM signs;
-    signs.init(lane);
-    uint32_t kcode[2][KM::NK][KM::W];
-    u32x4 vcode[SH::PIECES];
-    auto load_keys = [&](int s0, int u) {
-        const int tq = min(s0 + 16 * (NW * u + wave) + (lane >> 2), n_tok - 1);  // slots past the chunk repeat its last token
-        const int8_t* const p = a.kc + (size_t)s_row[tq] * D + KM::KPL * (lane & 3);
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-            for (int s = 0; s < KM::NK; ++s) {
-                const uint32_t* const w = reinterpret_cast<const uint32_t*>(p + hf * KM::HALF + s * KM::KB);
-#pragma unroll
-                for (int i = 0; i < KM::W; ++i) kcode[hf][s][i] = w[i];
-            }
-    };
-    auto load_values = [&](int s0) {
-#pragma unroll
-        for (int i = 0; i < SH::PIECES; ++i) {
-            const int j = NT * i + threadIdx.x, t = min(s0 + j / (D / 16), n_tok - 1);
-            vcode[i] = *reinterpret_cast<const u32x4*>(a.vc + (size_t)s_row[t] * D + 16 * (j % (D / 16)));
-        }
-    };
-    // The stage at s0 to LDS.  MANY: its codes are in registers, and those of the stage after it follow.
+    // The stage at s0 to LDS: its codes are in registers, and those of the stage after it follow.
     auto decode = [&](int s0, char* kbuf) {
-        char* const vbuf = kbuf + STAGE * ROWB;
         // what follows from the lane alone (operand signs, addresses) is worked out again in each stage:
         // kept across stages it would take 40 registers that the attention needs
-        int lane = threadIdx.x & 63;
+        uint32_t lane = threadIdx.x;
         asm volatile("" : "+v"(lane));
-        const int n16 = lane & 15, kg = lane >> 4, quad = lane >> 2, qq = lane & 3;
-        const int from_quad = 4 * (4 * n16 + kg);  // byte address of the lane that loaded this lane's block
-        auto permute = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_ds_bpermute(from_quad, (int)v); };
-        auto permute_f = [&](float v) { return __builtin_bit_cast(float, permute(__builtin_bit_cast(uint32_t, v))); };
+        lane &= 63u;
+        const uint32_t n16 = lane & 15u, kg = lane >> 4;
+        const int from_quad = (int)(4 * (4 * n16 + kg));  // byte address of the lane that loaded this lane's block
         KM km = signs;
 #pragma unroll
         for (int w = 0; w < KM::W; ++w) asm volatile("" : "+v"(km.h[w]));
-        const int tid = 64 * wave + lane;
-        if constexpr (!MANY) load_values(s0);
+        // The units' rows of the rotation tables, by way of the LDS that their keys and values will take:
+        // they arrive a row per 16 lanes, and every lane then reads its own coordinates.
 #pragma unroll
-        for (int i = 0; i < SH::PIECES; ++i) {
-            const int j = NT * i + tid, row = j / (D / 16), piece = j % (D / 16);
-            u32x4 o[2];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                half2v lo, hi;
-                codes_to_f16(vcode[i][k], lo, hi);
-                o[k / 2][2 * (k & 1)] = __builtin_bit_cast(uint32_t, lo);
-                o[k / 2][2 * (k & 1) + 1] = __builtin_bit_cast(uint32_t, hi);
-            }
-            const int f = T::value_swizzle(row);
-            *reinterpret_cast<u32x4*>(vbuf + row * ROWB + 16 * ((2 * piece) ^ f)) = o[0];
-            *reinterpret_cast<u32x4*>(vbuf + row * ROWB + 16 * ((2 * piece + 1) ^ f)) = o[1];
-        }
-        const bool more = MANY && s0 + STAGE < n_tok;
-        if (more) load_values(s0 + STAGE);
-#pragma unroll 1
         for (int u = 0; u < SH::UNITS; ++u) {
-            const int row = 16 * (NW * u + wave) + n16;
-            const int tq = min(s0 + 16 * (NW * u + wave) + quad, n_tok - 1), tn = min(s0 + row, n_tok - 1);
-            const size_t tab = (size_t)s_pos[tq] * (D / 2) + 4 * qq;
-            const float k_scale = (0.5f * f16_bits_to_f32(s_ks[tn])) * a.hscale;
-            if constexpr (!MANY) load_keys(s0, u);
+            const int row0 = 16 * (NW * u + wave);
+            char* const krows = kbuf + row0 * ROWB;
+            char* const vrows = krows + STAGE * ROWB;
+#pragma unroll
+            for (int i = 0; i < T::UPR / 4; ++i) {
+                const uint32_t slot = 64u * i + lane, r = slot / T::UPR;
+                const uint32_t tab = s_pos[s0 + row0 + r] + 16u * ((slot % T::UPR) ^ T::key_swizzle(r));
+                __builtin_amdgcn_global_load_lds((global_void*)(reinterpret_cast<const char*>(a.rope_dm) + tab),
+                                                 (lds_void*)(krows + 1024 * i), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((global_void*)(reinterpret_cast<const char*>(a.rope_dp) + tab),
+                                                 (lds_void*)(vrows + 1024 * i), 16, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < SH::UNITS; ++u) {
+            const int row0 = 16 * (NW * u + wave);
+            char* const krows = kbuf + row0 * ROWB;
+            char* const vrows = krows + STAGE * ROWB;
+            const float k_scale = (0.5f * f16_bits_to_f32(s_ks[s0 + row0 + n16])) * a.hscale;
             uint32_t code[2][KM::NK][KM::W];
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
                 for (int s = 0; s < KM::NK; ++s)
 #pragma unroll
-                    for (int i = 0; i < KM::W; ++i) code[hf][s][i] = permute(kcode[hf][s][i]);
-            char* const to = kbuf + row * ROWB + 8 * (kg & 1);
+                    for (int i = 0; i < KM::W; ++i)
+                        code[hf][s][i] = (uint32_t)__builtin_amdgcn_ds_bpermute(from_quad, (int)kcode[u][hf][s][i]);
+            if (u == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tables are this wave's own: no barrier
+            f32x4 tm[KM::T], tp[KM::T];
 #pragma unroll
             for (int t = 0; t < KM::T; ++t) {
-                const f32x4 tm = *reinterpret_cast<const f32x4*>(a.rope_dm + tab + 16 * t);
-                const f32x4 tp = *reinterpret_cast<const f32x4*>(a.rope_dp + tab + 16 * t);
+                const uint32_t at = n16 * ROWB + 16u * ((4u * t + kg) ^ (uint32_t)T::key_swizzle(n16));
+                tm[t] = *reinterpret_cast<const f32x4*>(krows + at);
+                tp[t] = *reinterpret_cast<const f32x4*>(vrows + at);
+            }
+            asm volatile("" ::: "memory");  // a wave's LDS accesses run in order: read before they are written over
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const uint32_t j = 64u * i + lane, r = j / (D / 16), piece = j % (D / 16);
+                u32x4 o[2];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    half2v lo, hi;
+                    codes_to_f16(vcode[u][i][k], lo, hi);
+                    o[k / 2][2 * (k & 1)] = __builtin_bit_cast(uint32_t, lo);
+                    o[k / 2][2 * (k & 1) + 1] = __builtin_bit_cast(uint32_t, hi);
+                }
+                const uint32_t f = T::value_swizzle(r);
+                *reinterpret_cast<u32x4*>(vrows + r * ROWB + 16 * ((2 * piece) ^ f)) = o[0];
+                *reinterpret_cast<u32x4*>(vrows + r * ROWB + 16 * ((2 * piece + 1) ^ f)) = o[1];
+            }
+            char* const to = krows + n16 * ROWB + 8 * (kg & 1);
+#pragma unroll
+            for (int t = 0; t < KM::T; ++t) {
                 int4v y0 = {0, 0, 0, 0}, y1 = {0, 0, 0, 0};
 #pragma unroll
                 for (int s = 0; s < KM::NK; ++s) {
@@ -261,19 +295,19 @@ shared_attn_kernel(SharedArgs a) {
                 float x[8];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float m = permute_f(tm[i]), p = permute_f(tp[i]);
                     const float lo = (float)y0[i] * k_scale, hi = (float)y1[i] * k_scale;
-                    x[i] = __builtin_fmaf(-lo, m, hi * p);
-                    x[4 + i] = __builtin_fmaf(lo, p, hi * m);
+                    x[i] = __builtin_fmaf(-lo, tm[t][i], hi * tp[t][i]);
+                    x[4 + i] = __builtin_fmaf(lo, tp[t][i], hi * tm[t][i]);
                 }
                 // coordinates 16 t + 4 kg + 0..3 and those D / 2 on: half a 16-byte chunk each
-                const int chunk16 = 2 * t + (kg >> 1), f = T::key_swizzle(row);
+                const uint32_t chunk16 = 2u * t + (kg >> 1), f = T::key_swizzle(n16);
                 *reinterpret_cast<u32x2*>(to + 16 * (chunk16 ^ f)) = u32x2{pack2<NQ_F16>(x[0], x[1]), pack2<NQ_F16>(x[2], x[3])};
                 *reinterpret_cast<u32x2*>(to + 16 * ((chunk16 + D / 16) ^ f)) =
                     u32x2{pack2<NQ_F16>(x[4], x[5]), pack2<NQ_F16>(x[6], x[7])};
             }
+            if constexpr (SH::UNITS > 1) __builtin_amdgcn_sched_barrier(0);  // one unit at a time in registers
         }
-        if (more) load_keys(s0 + STAGE, 0);
+        if (s0 + STAGE < n_tok) load(s0 + STAGE, [&](int i) { return s_row[i]; });
     };
     auto attend = [&](int s0, const char* kbuf) {
         if (!live) return;
@@ -291,9 +325,6 @@ shared_attn_kernel(SharedArgs a) {
     };
 
     if constexpr (MANY) {
-        static_assert(SH::UNITS == 1, "a wave's keys of the next stage are one unit");
-        load_keys(0, 0);
-        load_values(0);
         // ---- the stages: one is decoded while the one before it is attended to ----
         // A SIMD's two waves do these in opposite order, so that one's matrix products run under the other's
         // conversions.
@@ -344,21 +375,24 @@ shared_attn_kernel(SharedArgs a) {
             }
     }
     __syncthreads();
+    for (int r = threadIdx.x; r < n_q; r += NT) {
+        const int w0 = r >> 5, q = r & 31;
+        float m = kNoMax, l = 0.0f;
+        for (int w = w0; w < NW; w += rw) m = __builtin_fmaxf(m, s_m[w][q]);
+        for (int w = w0; w < NW; w += rw) l += s_l[w][q] * __builtin_amdgcn_exp2f(s_m[w][q] - m);
+        *reinterpret_cast<f32x2*>(a.part_ml + 2 * (size_t)s_slot[r]) = f32x2{m, l};
+    }
+    const float* const sums = reinterpret_cast<const float*>(s_kv);
+#pragma unroll 4
     for (int i = threadIdx.x; i < n_q * (D / 4); i += NT) {
         const int r = i / (D / 4), j = i % (D / 4), w0 = r >> 5, q = r & 31;
-        f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int w = w0; w < NW; w += rw)
-            y += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(s_kv) + (w * 32 + q) * D + 4 * (j ^ (q & 15)));
-        const uint32_t br = div((uint32_t)r, a.by_group);
-        const size_t slot = (size_t)(uint32_t)(seg_rows[2 * br + 1] + chunk) * a.q_heads + kh * G + ((uint32_t)r - br * G);
-        *reinterpret_cast<f32x4*>(a.part_y + slot * D + 4 * j) = y;
-        if (j == 0) {
-            float m = kNoMax, l = 0.0f;
-            for (int w = w0; w < NW; w += rw) m = __builtin_fmaxf(m, s_m[w][q]);
-            for (int w = w0; w < NW; w += rw) l += s_l[w][q] * __builtin_amdgcn_exp2f(s_m[w][q] - m);
-            a.part_ml[2 * slot] = m;
-            a.part_ml[2 * slot + 1] = l;
-        }
+        f32x4 y = *reinterpret_cast<const f32x4*>(sums + r * D + 4 * (j ^ (q & 15)));
+        for (int w = w0 + rw; w < NW; w += rw) y += *reinterpret_cast<const f32x4*>(sums + (w * 32 + q) * D + 4 * (j ^ (q & 15)));
+        f32x4* const to = reinterpret_cast<f32x4*>(a.part_y + (size_t)s_slot[r] * D + 4 * j);
+        // many rows: more bytes than the next kernel finds in its XCD's L2 (32 rows x 4 heads over 4096 tokens,
+        // 27.7 -> 25.2 us); few: 16.1 us kept there, 16.4 not
+        if constexpr (MANY) __builtin_nontemporal_store(y, to);
+        else *to = y;
     }
 }
 
@@ -450,12 +484,14 @@ static hipError_t shared_dims(int32_t d, const SharedArgs& a, uint32_t n_many, u
 
 }  // namespace nq
 
-extern "C" int32_t nq_shared_attention_chunk_tokens(void) { return nq::kSharedChunk; }
+extern "C" int32_t nq_shared_attention_chunk_tokens(int32_t many) {
+    return many ? nq::Shape<128, true>::CHUNK : nq::Shape<128, false>::CHUNK;
+}
 extern "C" int32_t nq_shared_attention_rows(int32_t head_dim) {
     return head_dim <= 128 ? nq::Shape<128, true>::ROWS : nq::Shape<256, true>::ROWS;
 }
 
-extern "C" int32_t nq_shared_attention_few_rows(void) { return nq::kFewRows; }
+extern "C" int32_t nq_shared_attention_few_rows(void) { return nq::Shape<128, false>::ROWS; }
 
 extern "C" int64_t nq_shared_attention_workspace(int32_t n_slots, int32_t q_heads, int32_t head_dim) {
     if (n_slots <= 0 || q_heads <= 0 || head_dim <= 0) return 0;
@@ -492,8 +528,9 @@ extern "C" int nq_shared_attention(const nq_shared_desc* d, void* stream) {
         NQ_CHECK_ARG((((uintptr_t)p->key_codes | (uintptr_t)p->value_codes | (uintptr_t)p->key_scales |
                        (uintptr_t)p->value_scales) & 15u) == 0 && ((uintptr_t)p->positions & 3u) == 0,
                      "nq_shared_attention: the pool's codes and scales must be 16-byte aligned");
-        NQ_CHECK_ARG(d->rope_sin_minus_cos && d->rope_cos_plus_sin && d->rope_n_pos > 0 && d->rope_n_pos < (1ll << 31),
-                     "nq_shared_attention: keys need RoPE tables");
+        NQ_CHECK_ARG(d->rope_sin_minus_cos && d->rope_cos_plus_sin && d->rope_n_pos > 0 && d->rope_n_pos < (1ll << 31) / p->head_dim,
+                     "nq_shared_attention: keys need RoPE tables, of less than 4 GB each");
+        NQ_CHECK_ARG((uint64_t)d->n_slots * d->q_heads < (1ull << 32), "nq_shared_attention: too many partial sums");
         const int64_t need = nq_shared_attention_workspace(d->n_slots, d->q_heads, p->head_dim);
         NQ_CHECK_ARG(d->n_slots > 0 && d->workspace != nullptr && d->workspace_bytes >= need &&
                          ((uintptr_t)d->workspace & 15u) == 0,

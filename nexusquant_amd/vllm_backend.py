@@ -505,62 +505,73 @@ def shared_segments(tables: Sequence[np.ndarray], lengths: Sequence[int], page_t
     return out
 
 
-# Workgroups that a launch should have before its chunks stay long: of segments of many query rows one for
-# each of 256 CUs, of the others two.
-_SHARED_WORKGROUPS = {True: 256, False: 512}
 _SHARED_STAGE = 128
+# Segments of more query rows than _MANY_ROWS go to the wide workgroups when there are at least
+# _MANY_TOKENS tokens for each of 256 CUs (the small shape takes up to nq_shared_attention_few_rows()):
+# 8 kv heads, 128 query rows, us wide and small: 4096 tokens 24.8 and 25.5, where the rows' own tokens need
+# the small shape's launch anyway; 16384 tokens 35.0 and 38.9.
+_MANY_ROWS = 32
+_MANY_TOKENS = 512
 
 
-def _shared_chunk(segments, tiles, kv_heads: int, cap: int, many: bool) -> int:
-    """Chunk length of one kind of segments: `cap` tokens, halved down to one stage of 128 while the launch
-    would have fewer than _SHARED_WORKGROUPS workgroups."""
-    length = cap
-    while length > _SHARED_STAGE and kv_heads * sum(
-            t * -(-n // length) for t, (_, _, n) in zip(tiles, segments)) < _SHARED_WORKGROUPS[many]:
-        length //= 2
+def _shared_chunk(lengths, tiles, kv_heads: int, cap: int, least: int, workgroups: int) -> int:
+    """Chunk length of segments: the least multiple of a stage with which the launch is one round of
+    `workgroups`.  16 rows x 4 heads over 8192 tokens, us: 512 workgroups 32.3, 256 (chunks of 256) 23.4,
+    128 27.3; 64 rows' own 512 tokens: 512 workgroups 37.3, 1024 41.9, 2048 50.3."""
+    length = min(least, cap)
+    while length < cap and kv_heads * sum(t * -(-n // length) for t, n in zip(tiles, lengths)) > workgroups:
+        length += _SHARED_STAGE
     return length
 
 
-def shared_items(segments, batch: int, group: int, kv_heads: int, cap: int, rows_of_many: int, few_rows: int):
+def shared_items(segments, batch: int, group: int, kv_heads: int, head_dim: int, cap: Dict[bool, int],
+                 rows: Dict[bool, int]):
     """The work list of nq_shared_attention: int32 arrays items, pages, seg_rows, row_slots, and the counts of
-    items, of those among them that come first (of segments of more than few_rows query rows) and of slots."""
-    many = [len(rows) * group > few_rows for rows, _, _ in segments]
-    per_tile = max(1, rows_of_many // group)  # batch rows of a workgroup
-    tiles = [-(-len(rows) // per_tile) for rows, _, _ in segments]
-    length = {}
-    for kind in (True, False):
-        of = [i for i in range(len(segments)) if many[i] == kind]
-        length[kind] = _shared_chunk([segments[i] for i in of], [tiles[i] for i in of], kv_heads, cap, kind)
-    chunks = [-(-s[2] // length[m]) for s, m in zip(segments, many)]
+    items, of those among them that come first (for the wide workgroups) and of slots.  cap, rows: most tokens
+    of a chunk and most query rows of a workgroup, wide (True) and small."""
+    wide = [len(r) * group > _MANY_ROWS for r, _, _ in segments]
+    work = kv_heads * sum(n * -(-len(r) * group // rows[True]) for (r, _, n), w in zip(segments, wide) if w)
+    if work < 256 * _MANY_TOKENS:
+        wide = [len(r) * group > rows[False] for r, _, _ in segments]
+    per_tile = {k: max(1, rows[k] // group) for k in rows}  # batch rows of a workgroup
+    tiles = [-(-len(r) // per_tile[w]) for (r, _, _), w in zip(segments, wide)]
+    step = {}
+    for k in (True, False):
+        of = [i for i in range(len(segments)) if wide[i] == k]
+        # as many workgroups as run at once: LDS leaves one of the wide ones on a CU, of the small 3, 2 or 1
+        slots = 256 if k else 256 * {64: 3, 128: 2}.get(head_dim, 1)
+        step[k] = _shared_chunk([segments[i][2] for i in of], [tiles[i] for i in of], kv_heads, cap[k],
+                                (2 if k else 1) * _SHARED_STAGE, slots)
+    chunks = [-(-s[2] // step[w]) for s, w in zip(segments, wide)]
     per_row = [0] * (batch + 1)
-    for (rows, _, _), c in zip(segments, chunks):
-        for b in rows:
+    for (r, _, _), c in zip(segments, chunks):
+        for b in r:
             per_row[b + 1] += c
     row_slots = np.cumsum(per_row)
     nxt = row_slots[:-1].tolist()
     records, seg_rows, pages = [], [], []
     at_pages = 0
-    # those of many rows first, long ones before short ones
-    for i in sorted(range(len(segments)), key=lambda i: (not many[i], -segments[i][2])):
-        rows, seg_pages, n = segments[i]
+    # the wide ones first, long ones before short ones
+    for i in sorted(range(len(segments)), key=lambda i: (not wide[i], -segments[i][2])):
+        r, seg_pages, n = segments[i]
         at_rows = len(seg_rows)
-        for b in rows:
+        for b in r:
             seg_rows.append((b, nxt[b]))
             nxt[b] += chunks[i]
         # chunks in eights (one for each XCD), a chunk's row tiles one eight after another
-        step = length[many[i]]
+        length, per = step[wide[i]], per_tile[wide[i]]
         for c0 in range(0, chunks[i], 8):
-            for r0 in range(0, len(rows), per_tile):
+            for r0 in range(0, len(r), per):
                 for c in range(c0, min(c0 + 8, chunks[i])):
-                    records.append((at_pages, c * step, min(n - c * step, step), at_rows + r0,
-                                    min(len(rows) - r0, per_tile), c, 0, 0))
+                    records.append((at_pages, c * length, min(n - c * length, length), at_rows + r0,
+                                    min(len(r) - r0, per), c, 0, 0))
         pages.append(np.asarray(seg_pages, dtype=np.int32))
         at_pages += len(seg_pages)
-    n_many = sum(t * c for t, c, m in zip(tiles, chunks, many) if m)
+    n_wide = sum(t * c for t, c, w in zip(tiles, chunks, wide) if w)
     parts = {"items": np.array(records, dtype=np.int32).reshape(-1),
              "pages": np.concatenate(pages) if pages else np.zeros(0, dtype=np.int32),
              "seg_rows": np.array(seg_rows, dtype=np.int32).reshape(-1), "row_slots": row_slots.astype(np.int32)}
-    return parts, len(records), n_many, int(row_slots[-1])
+    return parts, len(records), n_wide, int(row_slots[-1])
 
 
 class SharedAttentionPlan:
@@ -582,10 +593,11 @@ class SharedAttentionPlan:
                 raise RuntimeError("run_shared: run the plan once before capturing it into a graph")
             lib = _lib.load()
             heads = self.pool.num_heads
-            parts, *counts = shared_items(self.segments, self.batch, q_heads // heads, heads,
-                                          int(lib.nq_shared_attention_chunk_tokens()),
-                                          int(lib.nq_shared_attention_rows(self.pool.head_dim)),
-                                          int(lib.nq_shared_attention_few_rows()))
+            parts, *counts = shared_items(
+                self.segments, self.batch, q_heads // heads, heads, self.pool.head_dim,
+                {k: int(lib.nq_shared_attention_chunk_tokens(k)) for k in (True, False)},
+                {True: int(lib.nq_shared_attention_rows(self.pool.head_dim)),
+                 False: int(lib.nq_shared_attention_few_rows())})
             offsets, at = {}, 0
             for name, v in parts.items():
                 offsets[name] = at

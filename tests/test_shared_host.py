@@ -63,21 +63,23 @@ def test_what_is_shared_is_in_one_segment():
     assert sorted((rows, n) for rows, _, n in segs) == [([0, 1], 496), ([2, 3], 496)]
 
 
-@pytest.mark.parametrize("group,kv_heads,cap,most,few", [(1, 8, 1024, 128, 32), (4, 1, 1024, 128, 32), (128, 2, 256, 128, 32),
-                                                         (8, 64, 128, 128, 0), (2, 3, 1024, 256, 1000)])
-def test_items_cover_each_rows_tokens_and_slots_once(group, kv_heads, cap, most, few):
+@pytest.mark.parametrize("group,kv_heads,d,cap,rows", [
+    (1, 8, 128, 1024, (256, 128)), (4, 1, 64, 1024, (256, 128)), (128, 2, 256, 256, (128, 128)),
+    (8, 64, 128, 128, (256, 128)), (2, 3, 128, 1024, (256, 128)), (200, 1, 128, 2048, (256, 128))])
+def test_items_cover_each_rows_tokens_and_slots_once(group, kv_heads, d, cap, rows):
     r = np.random.RandomState(group)
     batch = 37
     segments = [(list(range(20)), np.arange(300), 4800), ([3, 5, 36], np.arange(400, 410), 160)]
     segments += [([b], np.arange(1000 + 10 * b, 1010 + 10 * b), int(r.randint(1, 160))) for b in range(30)]
-    parts, n_items, n_many, n_slots = shared_items(segments, batch, group, kv_heads, cap, most, few)
+    most = dict(zip((True, False), rows))
+    parts, n_items, n_wide, n_slots = shared_items(segments, batch, group, kv_heads, d, {True: cap, False: cap}, most)
     items = parts["items"].reshape(-1, 8)
-    rows = parts["seg_rows"].reshape(-1, 2)
+    where = parts["seg_rows"].reshape(-1, 2)
     assert len(items) == n_items and parts["row_slots"][0] == 0 and parts["row_slots"][-1] == n_slots
     seen, slots = {}, []
     for i, (page0, tok0, n, row0, n_rows, chunk, _, _) in enumerate(items):
-        assert 1 <= n <= cap and 1 <= n_rows and n_rows * group <= (most if i < n_many else few)
-        for b, slot0 in rows[row0:row0 + n_rows]:
+        assert 1 <= n <= cap and 1 <= n_rows and n_rows * group <= most[i < n_wide]
+        for b, slot0 in where[row0:row0 + n_rows]:
             slots.append(slot0 + chunk)
             assert parts["row_slots"][b] <= slot0 + chunk < parts["row_slots"][b + 1]
             for t in range(tok0, tok0 + n):
@@ -86,12 +88,19 @@ def test_items_cover_each_rows_tokens_and_slots_once(group, kv_heads, cap, most,
                 seen[key] = 1
     assert sorted(slots) == list(range(n_slots))
     assert len(seen) == sum(len(s[0]) * s[2] for s in segments)
-    assert n_many == (0 if few == 1000 else n_items if group * 1 > few else n_many) and n_many <= n_items
+
+
+@pytest.mark.parametrize("rows,group,tokens,wide", [(16, 8, 16384, True), (16, 8, 4096, False), (4, 8, 60000, False),
+                                                    (32, 8, 128, True), (1, 200, 16, True)])
+def test_which_segments_take_the_wide_workgroups(rows, group, tokens, wide):
+    segments = [(list(range(rows)), np.arange(tokens // 16), tokens)]
+    _, n_items, n_wide, _ = shared_items(segments, rows, group, 8, 128, {True: 2048, False: 1024}, {True: 256, False: 128})
+    assert n_wide == (n_items if wide else 0)
 
 
 def test_no_rows_and_no_tokens():
-    parts, n_items, n_many, n_slots = shared_items([], 3, 4, 8, 1024, 256, 32)
-    assert n_items == n_many == n_slots == 0 and list(parts["row_slots"]) == [0, 0, 0, 0]
+    parts, n_items, n_wide, n_slots = shared_items([], 3, 4, 8, 128, {True: 2048, False: 1024}, {True: 256, False: 128})
+    assert n_items == n_wide == n_slots == 0 and list(parts["row_slots"]) == [0, 0, 0, 0]
 
 
 def test_plan_refuses_bad_tables(monkeypatch):
