@@ -44,6 +44,7 @@ def copy_np(f, src, dst):
     (2, 2, 1, 64, 4), (2, 3, 24, 128, 7),      # 4- and 16-byte ones
     (1, 8, 16, 128, 1), (5, 4, 7, 256, 33),
     (2, 1, 2, 64, 449), (1, 1, 3, 64, 1000),   # past one launch's pairs
+    (20, 8, 16, 128, 60), (10, 1, 25, 256, 300),  # past the caches
 ])
 def test_copy_pages(layers, heads, tokens, d, n):
     print(f"[gpu] copy layers={layers} heads={heads} tokens={tokens} d={d} n={n}", flush=True)
