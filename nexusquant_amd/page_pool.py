@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import array
 import ctypes
+import struct
 import threading
 from typing import List, Optional, Sequence, Tuple
 
@@ -135,15 +136,18 @@ class CompressedPagePool:
         return -(-int(length) // self.page_tokens)
 
     def _pages(self, pages) -> np.ndarray:
-        # a list of ints by way of array(): two thirds of numpy's own conversion time
-        try:
-            p = (np.frombuffer(array.array("i", pages), dtype=np.int32) if type(pages) is list and pages
-                 else np.asarray(pages, dtype=np.int32).reshape(-1))
-        except OverflowError:
-            raise ValueError(f"page numbers must lie in [0, {self.num_pages})") from None
-        if len(p) and p.view(np.uint32).max() >= self.num_pages:  # a negative number is a large one there
+        # a list of ints by way of struct: a third of numpy's own conversion time
+        if type(pages) is list:
+            try:
+                p = np.frombuffer(struct.pack(f"{len(pages)}i", *pages), dtype=np.int32)
+            except struct.error:
+                raise ValueError(f"page numbers must be integers in [0, {self.num_pages})") from None
+        else:
+            p = np.asarray(pages, dtype=np.int64).reshape(-1)
+        # a negative number is a large one as unsigned
+        if len(p) and p.view(np.uint32 if p.dtype == np.int32 else np.uint64).max() >= self.num_pages:
             raise ValueError(f"page numbers must lie in [0, {self.num_pages})")
-        return p
+        return p.astype(np.int32, copy=False)
 
     def in_use(self, pages, what: str = "pages") -> np.ndarray:
         """The page numbers as an array; raises unless all are allocated."""
@@ -180,7 +184,7 @@ class CompressedPagePool:
     def _drop(self, p: np.ndarray, n: np.ndarray) -> None:
         left = self._refs[p] - n
         if len(p) and left.min() < 0:
-            raise ValueError(f"page {int(p[left < 0][0])} is freed more often than it is referenced")
+            raise ValueError(f"free: page {int(p[left < 0][0])} is not allocated, or freed more often than referenced")
         self._refs[p] = left
         gone = p[left == 0][::-1]  # the lowest is allocated next
         self._stack[self._free:self._free + len(gone)] = gone
@@ -189,14 +193,14 @@ class CompressedPagePool:
     def retain(self, pages: Sequence[int]) -> None:
         """One more reference to each page (to a page listed twice: two)."""
         with self._lock:
-            p, n = self._tally(self.in_use(pages, "retain"))
-            self._refs[p] += n
+            p, n = self._tally(self._pages(pages))
+            self._refs[self.in_use(p, "retain")] += n
 
     def free(self, pages: Sequence[int]) -> None:
         """Drop one reference of each page (of a page listed twice: two); pages without any can be
         allocated again.  Work already queued on the pool's stream still sees them as they were."""
         with self._lock:
-            self._drop(*self._tally(self.in_use(pages, "free")))
+            self._drop(*self._tally(self._pages(pages)))
 
     # --------------------------------------------------------------- page moves
 
