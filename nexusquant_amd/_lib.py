@@ -243,7 +243,7 @@ def current_stream_handle(device) -> int:
     """The current stream's handle on `device` (the raw one: 0.2 us where building a
     torch.cuda.Stream object for it takes 2)."""
     import torch
-    idx = torch.device(device).index
+    idx = device.index if isinstance(device, torch.device) else torch.device(device).index
     if idx is None:
         idx = torch.cuda.current_device()
     return torch._C._cuda_getCurrentRawStream(idx)

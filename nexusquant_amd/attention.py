@@ -10,13 +10,14 @@ from __future__ import annotations
 
 import ctypes
 import dataclasses
+import struct
 from typing import Optional, Sequence
 
 import numpy as np
 import torch
 
 from . import _lib
-from .ops import PlanTensor, _addr
+from .ops import PlanTensor, on_device
 
 _HEAD_DIMS = (64, 128, 256)
 
@@ -56,11 +57,19 @@ def plan_prompts(lengths: Sequence[int], device=None) -> PromptPlan:
                       tiles=PlanTensor(tiles.reshape(-1), dev) if len(tiles) else None)
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t with contiguous, 16-byte aligned head vectors (itself when they are)."""
-    if t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(0) < 1 << 24 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _rows(t: torch.Tensor):
+    """t with contiguous, 16-byte aligned head vectors (itself when they are), its address and strides."""
+    row, head, one = t.stride()
+    at = t.data_ptr()
+    if one != 1 or (row | head) & 7 or row >= 1 << 24 or at & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        row, head, one = t.stride()
+        at = t.data_ptr()
+    return t, at, row, head
+
+
+# nq_prompt_desc, packed in one go (a call's host time counts for short prompts)
+_PACK = struct.Struct("6i5P8q2f")
 
 
 def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, plan: PromptPlan,
@@ -76,25 +85,27 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     and are zero without one.  Inference only: tensors that require a gradient are refused."""
     lib = _lib.load()
     for name, t in (("query", query), ("key", key), ("value", value)):
-        _lib.require_device(t, name)
-        if t.dim() != 3:
-            raise ValueError(f"{name} must be [rows, heads, head_dim], got {tuple(t.shape)}")
-    rows, hq, d = query.shape
-    hkv = key.shape[1]
-    if tuple(key.shape) != (rows, hkv, d) or value.shape != key.shape:
-        raise ValueError(f"incompatible query {tuple(query.shape)}, key {tuple(key.shape)} and value {tuple(value.shape)}")
+        if not t.is_cuda:
+            _lib.require_device(t, name)
+    shape, kv, dtype, dev = query.shape, key.shape, query.dtype, query.device
+    if len(shape) != 3 or len(kv) != 3:
+        raise ValueError(f"query and key must be [rows, heads, head_dim], got {tuple(shape)} and {tuple(kv)}")
+    rows, hq, d = shape
+    hkv = kv[1]
+    if kv[0] != rows or kv[2] != d or value.shape != kv:
+        raise ValueError(f"incompatible query {tuple(shape)}, key {tuple(kv)} and value {tuple(value.shape)}")
     if hkv == 0 or hq == 0 or hq % hkv:
         raise ValueError(f"{hq} query heads are no multiple of {hkv} kv heads")
-    if not (query.dtype == key.dtype == value.dtype) or query.dtype not in (torch.float16, torch.bfloat16):
+    if dtype not in (torch.float16, torch.bfloat16) or key.dtype != dtype or value.dtype != dtype:
         raise ValueError("query, key and value must share an fp16 or bf16 dtype")
-    if not query.device == key.device == value.device:
+    if key.device != dev or value.device != dev:
         raise ValueError("query, key and value must be on one device")
     if d not in _HEAD_DIMS:
         raise ValueError(f"head_dim {d} unsupported (64, 128, 256)")
     if rows < plan.rows:
         raise ValueError(f"the plan's sequences have {plan.rows} rows, the tensors {rows}")
-    if plan.tiles is not None and plan.tiles.tensor.device != query.device:
-        raise ValueError(f"the plan is on {plan.tiles.tensor.device}, the tensors on {query.device}")
+    if plan.tiles is not None and plan.tiles.device != dev:
+        raise ValueError(f"the plan is on {plan.tiles.device}, the tensors on {dev}")
     if sliding_window is not None and int(sliding_window) <= 0:
         raise ValueError(f"sliding_window must be positive, got {sliding_window}")
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
@@ -103,23 +114,23 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     if not 0.0 < scale < 1e30:
         raise ValueError(f"scale must be positive, got {scale}")
     if out is None:
-        out = torch.empty(rows, hq, d, dtype=query.dtype, device=query.device)
+        out = torch.empty(shape, dtype=dtype, device=dev)
         if rows > plan.rows:
             out[plan.rows:].zero_()
-    elif (tuple(out.shape) != (rows, hq, d) or out.dtype != query.dtype or out.device != query.device
+    elif (out.shape != shape or out.dtype != dtype or out.device != dev
           or out.stride(2) != 1 or out.stride(0) % 4 or out.stride(1) % 4 or out.data_ptr() % 8):
-        raise ValueError(f"out must be {(rows, hq, d)} {query.dtype} on {query.device} with 8-byte aligned head vectors")
+        raise ValueError(f"out must be {tuple(shape)} {dtype} on {dev} with 8-byte aligned head vectors")
     if plan.n_tiles == 0:
         return out
-    q, k, v = _rows(query), _rows(key), _rows(value)
+    q, q_at, q_row, q_head = _rows(query)
+    k, k_at, k_row, k_head = _rows(key)
+    v, v_at, v_row, v_head = _rows(value)
+    o_row, o_head, _ = out.stride()
     window = 0 if sliding_window is None or int(sliding_window) >= max(plan.lengths) else int(sliding_window)
-    two = ctypes.c_int64 * 2
-    with torch.cuda.device(q.device):
-        desc = _lib.PromptDesc(q_heads=hq, kv_heads=hkv, head_dim=d, dtype=_lib.dtype_code(q.dtype),
-                               n_tiles=plan.n_tiles, sliding_window=window, q=_addr(q), k=_addr(k), v=_addr(v),
-                               out=_addr(out), tiles=plan.tiles.address(), q_stride=two(*q.stride()[:2]),
-                               k_stride=two(*k.stride()[:2]), v_stride=two(*v.stride()[:2]),
-                               out_stride=two(*out.stride()[:2]), scale=scale)
-        st = lib.nq_prompt_attention(ctypes.byref(desc), ctypes.c_void_p(_lib.current_stream_handle(q.device)))
+    with on_device(dev):
+        desc = _lib.PromptDesc.from_buffer_copy(_PACK.pack(
+            hq, hkv, d, _lib.NQ_F16 if dtype == torch.float16 else _lib.NQ_BF16, plan.n_tiles, window, q_at, k_at, v_at,
+            out.data_ptr(), plan.tiles.address(), q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, scale, 0.0))
+        st = lib.nq_prompt_attention(ctypes.byref(desc), _lib.current_stream_handle(dev))
     _lib.check(st, "nq_prompt_attention")
     return out

@@ -191,20 +191,23 @@ class PlanTensor:
     capture relies on the device having been synchronized since the plan was made (torch.cuda.graph does)."""
 
     def __init__(self, values: np.ndarray, device):
-        self.device = torch.device(device)
+        device = torch.device(device)
+        self.device = device if device.index is not None else torch.device("cuda", torch.cuda.current_device())
         with torch.cuda.device(self.device):
             self.tensor = to_device(values, self.device)
-            self._stream = torch.cuda.current_stream(self.device)
+            stream = torch.cuda.current_stream(self.device)
+            self._stream = stream.cuda_stream
             self._copied = torch.cuda.Event()
-            self._copied.record(self._stream)
+            self._copied.record(stream)
+        self._address = self.tensor.data_ptr()
 
     def address(self) -> int:
         """For a launch on the device's current stream."""
-        if _lib.current_stream_handle(self.device) != self._stream.cuda_stream and not torch.cuda.is_current_stream_capturing():
+        if _lib.current_stream_handle(self.device) != self._stream and not torch.cuda.is_current_stream_capturing():
             stream = torch.cuda.current_stream(self.device)
             stream.wait_event(self._copied)
             self.tensor.record_stream(stream)
-        return self.tensor.data_ptr()
+        return self._address
 
 
 _workspaces: Dict[Tuple[int, int], torch.Tensor] = {}

@@ -20,6 +20,7 @@ from __future__ import annotations
 import ctypes
 import dataclasses
 import math
+import struct
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -27,7 +28,7 @@ import torch
 
 from . import _lib
 from .hadamard import hadamard_constant
-from .ops import PlanTensor, _addr, _PtrArrays
+from .ops import PlanTensor, _addr, _PtrArrays, on_device
 from .rope import device_merged_table, device_table
 
 _FP16_BYTES = 2
@@ -461,19 +462,21 @@ class PagedAttentionPlan:
     tokens: int                        # tokens attended over all rows
 
 
-# A segment is shared when that saves at least this many tokens' decoding (its tokens, once for
-# every row but one).
-_MIN_SHARED = 256
+# What pays to share: a segment of _MIN_TOKENS tokens whose sharing saves _MIN_SAVED tokens' decoding (its tokens,
+# once for every row but one).  8 kv heads x 4, us shared and apart: 32 rows x 128 tokens 17.4 and 15.6, x 256
+# 17.3 and 20.4, x 1024 19.0 and 35.0; 8 rows x 256 14.3 and 14.5, x 1024 14.4 and 19.2; 2 rows x 2048 15.9 and 15.5.
+_MIN_TOKENS = 256
+_MIN_SAVED = 2048
 
 
 def shared_segments(tables: Sequence[np.ndarray], lengths: Sequence[int], page_tokens: int,
-                    min_saved: int = _MIN_SHARED) -> List[Tuple[List[int], np.ndarray, int]]:
+                    min_saved: Optional[int] = None) -> List[Tuple[List[int], np.ndarray, int]]:
     """Cut the rows' tokens into segments (rows, pages, tokens) that their rows see whole.
 
     tables[b]: row b's pages, lengths[b]: its tokens.  Rows that begin with the same full pages
     share a segment of these, and those among them that go on alike another one, and so on; a
     segment of one row is what it has for itself.  Sharing that would save less than min_saved
-    tokens is left to what follows it."""
+    tokens (None: that does not pay) is left to what follows it."""
     full = [int(n) // page_tokens for n in lengths]
     out: List[Tuple[List[int], np.ndarray, int]] = []
 
@@ -495,7 +498,8 @@ def shared_segments(tables: Sequence[np.ndarray], lengths: Sequence[int], page_t
             differ = np.flatnonzero((stack != stack[0]).any(axis=0))
             end = depth + int(differ[0]) if len(differ) else most
             tokens = (end - start) * page_tokens
-            if (len(same) - 1) * tokens >= min_saved:
+            saved = (len(same) - 1) * tokens
+            if saved >= min_saved if min_saved is not None else saved >= _MIN_SAVED and tokens >= _MIN_TOKENS:
                 out.append((same, tables[same[0]][start:end], tokens))
                 split(same, end, end)
             else:
@@ -574,6 +578,10 @@ def shared_items(segments, batch: int, group: int, kv_heads: int, head_dim: int,
     return parts, len(records), n_wide, int(row_slots[-1])
 
 
+# nq_shared_desc, packed in one go
+_SHARED_PACK = struct.Struct("P8i8Pq2fPq")
+
+
 class SharedAttentionPlan:
     """Which tokens of a pool each batch row attends to, and which of them rows share: valid for every
     layer of the pool while the rows' tables and lengths stay the same.  The device arrays are made for a
@@ -600,8 +608,8 @@ class SharedAttentionPlan:
                  False: int(lib.nq_shared_attention_few_rows())})
             offsets, at = {}, 0
             for name, v in parts.items():
-                offsets[name] = at
-                at += len(v)
+                offsets[name] = at  # bytes
+                at += 4 * len(v)
             ints = PlanTensor(np.concatenate(list(parts.values())), self.pool.device)
             got = self._work[q_heads] = (ints, offsets, *counts)
         return got
@@ -614,6 +622,7 @@ class NexusQuantPagedAttention:
         self.compressor = compressor
         self._block_pool: dict = {}
         self._next_block_id: int = 0
+        self._tables: Optional[tuple] = None  # (largest position, device, merged rotation tables) of run_shared
 
     def allocate_block(self) -> int:
         block_id = self._next_block_id
@@ -765,10 +774,12 @@ class NexusQuantPagedAttention:
 
     # ----------------------------------------------------- rows that share pages
 
-    def plan_shared(self, pool, block_tables: Sequence[Sequence[int]], context_lens) -> SharedAttentionPlan:
+    def plan_shared(self, pool, block_tables: Sequence[Sequence[int]], context_lens,
+                    min_saved: Optional[int] = None) -> SharedAttentionPlan:
         """The plan of rows over a CompressedPagePool: row b attends to the first context_lens[b] tokens of
         its pages block_tables[b] (0: none).  Full pages that several rows begin with, as forks do, are
-        read and decoded once for all of them (shared_segments)."""
+        read and decoded once for all of them, where that saves min_saved tokens' decoding (None: where it
+        pays; see shared_segments)."""
         if pool.head_dim != self.compressor.head_dim:
             raise ValueError(f"pool head_dim {pool.head_dim} != compressor head_dim {self.compressor.head_dim}")
         ctx = [int(x) for x in (context_lens.tolist() if torch.is_tensor(context_lens) else context_lens)]
@@ -780,7 +791,15 @@ class NexusQuantPagedAttention:
             if not 0 <= n <= len(pages) * pool.page_tokens:
                 raise ValueError(f"row {b}: {n} tokens in {len(pages)} pages of {pool.page_tokens}")
             tables.append(pages[:pool.pages_for(n)])
-        return SharedAttentionPlan(pool, len(ctx), shared_segments(tables, ctx, pool.page_tokens))
+        return SharedAttentionPlan(pool, len(ctx), shared_segments(tables, ctx, pool.page_tokens, min_saved))
+
+    def _shared_tables(self, max_position: int, dev):
+        """The merged rotation tables, kept here until a larger position needs longer ones."""
+        got = self._tables
+        if got is None or got[0] < max_position or got[1] != dev:
+            _, _, dm, dp = self.compressor._tables(max_position, dev)
+            got = self._tables = (dm.shape[0] - 1, dev, (dm, dp))
+        return got[2]
 
     def run_shared(self, plan: SharedAttentionPlan, query: torch.Tensor, layer: int = 0,
                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -791,43 +810,44 @@ class NexusQuantPagedAttention:
         roundings, not bit for bit.  run() differs in its roundings too (values there are not rounded)."""
         lib = _lib.load()
         pool = plan.pool
-        _lib.require_device(query, "query")
-        if query.device != pool.device:
-            raise ValueError(f"query is on {query.device}, the pool on {pool.device}")
-        if query.dim() != 3 or query.shape[0] != plan.batch or query.shape[2] != pool.head_dim:
+        if not query.is_cuda:
+            _lib.require_device(query, "query")
+        shape, dtype, dev = query.shape, query.dtype, pool.device
+        if query.device != dev:
+            raise ValueError(f"query is on {query.device}, the pool on {dev}")
+        if len(shape) != 3 or shape[0] != plan.batch or shape[2] != pool.head_dim:
             raise ValueError(f"query must be (batch={plan.batch}, num_heads, head_dim={pool.head_dim}), got "
-                             f"{tuple(query.shape)}")
-        if query.dtype not in (torch.float16, torch.bfloat16):
-            raise ValueError(f"run_shared takes fp16 or bf16 queries, got {query.dtype}; run() takes fp32 ones")
-        b, hq, d = query.shape
+                             f"{tuple(shape)}")
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"run_shared takes fp16 or bf16 queries, got {dtype}; run() takes fp32 ones")
+        b, hq, d = shape
         rows = int(lib.nq_shared_attention_rows(d))
         if hq == 0 or hq % pool.num_heads or hq // pool.num_heads > rows:
             raise ValueError(f"num_heads {hq} is not a multiple (up to {rows}) of the pool's {pool.num_heads}")
         if not 0 <= int(layer) < pool.num_layers:
             raise ValueError(f"layer {layer} of a pool of {pool.num_layers}")
+        if pool.head_dim != self.compressor.head_dim:
+            raise ValueError(f"pool head_dim {pool.head_dim} != compressor head_dim {self.compressor.head_dim}")
         if out is None:
-            out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-        elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous {query.dtype} tensor {tuple(query.shape)} on {query.device}")
+            out = torch.empty(shape, dtype=dtype, device=dev)
+        elif out.shape != shape or out.dtype != dtype or out.device != dev or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {dtype} tensor {tuple(shape)} on {dev}")
         q = query.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()
-        dev = pool.device
-        with torch.cuda.device(dev):
+        with on_device(dev):
             ints, offsets, n_items, n_many, n_slots = plan.work(hq)
             nbytes = lib.nq_shared_attention_workspace(n_slots, hq, d)
             # of this call alone: calls on other streams and captured graphs have their own
             ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-            _, _, dm, dp = self.compressor._tables(pool.max_position, dev)
+            dm, dp = self._shared_tables(pool.max_position, dev)
             base = ints.address()
-            desc = _lib.SharedDesc(
-                pool=ctypes.pointer(pool.desc), layer=int(layer), batch=b, q_heads=hq, q_dtype=_lib.dtype_code(q.dtype),
-                n_items=n_items, n_many=n_many, n_slots=n_slots, query=_addr(q), out=_addr(out), items=base + 4 * offsets["items"],
-                pages=base + 4 * offsets["pages"], seg_rows=base + 4 * offsets["seg_rows"],
-                row_slots=base + 4 * offsets["row_slots"], rope_sin_minus_cos=_addr(dm), rope_cos_plus_sin=_addr(dp),
-                rope_n_pos=dm.shape[0], hadamard_scale=hadamard_constant(d),
-                scale_divisor=float(np.float32(math.sqrt(d))), workspace=_addr(ws), workspace_bytes=nbytes)
-            st = lib.nq_shared_attention(ctypes.byref(desc), _stream(dev))
+            desc = _lib.SharedDesc.from_buffer_copy(_SHARED_PACK.pack(
+                ctypes.addressof(pool.desc), int(layer), b, hq, _lib.dtype_code(dtype), n_items, n_many, n_slots, 0,
+                q.data_ptr(), out.data_ptr(), base + offsets["items"], base + offsets["pages"],
+                base + offsets["seg_rows"], base + offsets["row_slots"], dm.data_ptr(), dp.data_ptr(), dm.shape[0],
+                hadamard_constant(d), float(np.float32(math.sqrt(d))), ws.data_ptr(), nbytes))
+            st = lib.nq_shared_attention(ctypes.byref(desc), _lib.current_stream_handle(dev))
         _lib.check(st, "nq_shared_attention")
         return out
 

@@ -72,8 +72,8 @@ def row_oracle(pool, layer, table, n, q):
     return out.reshape(-1, d), tol.reshape(-1, d)
 
 
-def check(attn, pool, tables, ctx, q, layer=0, **kw):
-    plan = attn.plan_shared(pool, tables, ctx)
+def check(attn, pool, tables, ctx, q, layer=0, min_saved=1, **kw):
+    plan = attn.plan_shared(pool, tables, ctx, min_saved=min_saved)  # 1: whatever can be shared is
     got = attn.run_shared(plan, q, layer=layer, **kw)
     assert got.shape == q.shape and got.dtype == q.dtype
     u = torch.finfo(q.dtype).eps / 2
@@ -128,7 +128,11 @@ def test_forked_rows(heads, group, d, tokens, dtype, rows, prefix):
     tables, ctx = forks(pool, prefix, [int(x) for x in r.randint(0, 130, rows)])
     tables.append([])
     ctx.append(0)  # an idle row
-    check(attention(d), pool, tables, ctx, queries(rows + 1, heads * group, d, dtype, seed=rows))
+    q = queries(rows + 1, heads * group, d, dtype, seed=rows)
+    for min_saved in (1, None, 1 << 40):
+        plan, _ = check(attention(d), pool, tables, ctx, q, min_saved=min_saved)
+        shared = [s for s in plan.segments if len(s[0]) > 1]
+        assert shared if min_saved == 1 and rows > 1 else not shared or min_saved is None
 
 
 @pytest.mark.parametrize("n", [1, 15, 16, 17, 31, 32, 33, 127, 128, 129, 1023, 1024, 1025, 2500])
@@ -155,7 +159,7 @@ def test_nested_prefixes_layers_and_scattered_positions():
     pool.max_position = 80000
     tables, ctx = [x for x, _ in more], [n for _, n in more]
     plan, _ = check(attention(128), pool, tables, ctx, queries(6, 8, 128, torch.float16), layer=2)
-    assert len([s for s in plan.segments if len(s[0]) > 1]) == 1
+    assert sorted(len(s[0]) for s in plan.segments if len(s[0]) > 1) == [3, 3, 6]  # forks of forks
     attn = attention(128)
     for layer in range(3):
         check(attn, pool, tables, ctx, queries(6, 8, 128, torch.bfloat16, seed=layer), layer=layer)
@@ -224,7 +228,7 @@ def test_two_streams_graph_and_repeat():
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
-        fresh = attn.plan_shared(pool, tables, ctx)
+        fresh = attn.plan_shared(pool, tables, ctx, min_saved=1)
         a = attn.run_shared(fresh, q)
         b = attn.run_shared(plan, q)
     c = attn.run_shared(fresh, q)  # a plan made on the other stream
@@ -302,7 +306,7 @@ def test_a_serving_run():
             k, v = (torch.randn(5, h, d, generator=g).half().to(DEV) for _ in range(2))
             pool.write(attn.compressor, where, k, v, ctx, layer=layer)
         ctx = [n + 1 for n in ctx]
-        shared = attn.plan_shared(pool, branches, ctx)
+        shared = attn.plan_shared(pool, branches, ctx, min_saved=1)
         for layer in range(layers):
             check(attn, pool, branches, ctx, queries(5, h * grp, d, torch.float16, seed=step), layer=layer)
             attn.run_shared(shared, queries(5, h * grp, d, torch.float16), layer=layer)
@@ -315,3 +319,14 @@ def test_a_serving_run():
     check(attn, pool, branches, ctx, queries(5, h * grp, d, torch.bfloat16, seed=9), layer=1)
     pool.free([p for x in branches for p in x])
     assert pool.free_pages == pool.num_pages
+
+
+@pytest.mark.parametrize("heads,group,d,rows,prefix", [(8, 8, 128, 40, 4112), (8, 4, 64, 24, 17000), (4, 4, 256, 33, 9000),
+                                                       (2, 32, 128, 5, 1500), (1, 200, 128, 2, 700)])
+def test_wide_workgroups(heads, group, d, rows, prefix):
+    """Segments of many query rows: stages decoded under the attention to the one before, several row tiles."""
+    print(f"[gpu] shared wide {heads}x{group} d={d} rows={rows} prefix={prefix}", flush=True)
+    pool = make_pool(1, prefix // 16 + 2 + 8 * rows, heads, 16, d, seed=rows)
+    tables, ctx = forks(pool, prefix, [7 * i % 90 for i in range(rows)])
+    plan, _ = check(attention(d), pool, tables, ctx, queries(rows, heads * group, d, torch.float16, seed=rows))
+    assert plan.work(heads * group)[3] > 0

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from nexusquant_amd import _lib
-from nexusquant_amd.attention import PromptPlan, plan_prompts, prompt_attention, prompt_tiles
+from nexusquant_amd.attention import _PACK, PromptPlan, plan_prompts, prompt_attention, prompt_tiles
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -47,6 +47,7 @@ def test_prompt_struct_matches_the_c_compiler(tmp_path):
     (tmp_path / "p.c").write_text("\n".join(prog))
     subprocess.check_call(["gcc", "-o", str(tmp_path / "p"), str(tmp_path / "p.c")])
     out = [int(x) for x in subprocess.check_output([str(tmp_path / "p")]).split()]
+    assert _PACK.size == ctypes.sizeof(_lib.PromptDesc)
     assert out == [ctypes.sizeof(_lib.PromptDesc)] + [getattr(_lib.PromptDesc, f).offset for f in names]
 
 

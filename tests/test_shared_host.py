@@ -9,8 +9,8 @@ import pytest
 import torch
 
 from nexusquant_amd import _lib
-from nexusquant_amd.vllm_backend import (NexusQuantKVCompressor, NexusQuantPagedAttention, SharedAttentionPlan,
-                                         shared_items, shared_segments)
+from nexusquant_amd.vllm_backend import (_SHARED_PACK, NexusQuantKVCompressor, NexusQuantPagedAttention,
+                                         SharedAttentionPlan, shared_items, shared_segments)
 
 from test_page_pool import c_pool, host_pool
 
@@ -55,12 +55,20 @@ def test_segments_hold_every_token_of_every_row_once(tables, lengths, t, min_sav
 
 def test_what_is_shared_is_in_one_segment():
     a = np.arange(40)
-    segs = shared_segments([np.r_[a, 50], np.r_[a, 51], np.r_[a, 52]], [650, 656, 641], 16)
+    segs = shared_segments([np.r_[a, 50], np.r_[a, 51], np.r_[a, 52]], [650, 656, 641], 16, 256)
     assert sorted((rows, n) for rows, _, n in segs) == [([0], 10), ([0, 1, 2], 640), ([1], 16), ([2], 1)]
     # nested: a common start too short by itself goes along with what its branches share
     x, y = np.arange(100, 130), np.arange(200, 230)
-    segs = shared_segments([np.r_[1, x], np.r_[1, x], np.r_[1, y], np.r_[1, y]], [496] * 4, 16)
+    segs = shared_segments([np.r_[1, x], np.r_[1, x], np.r_[1, y], np.r_[1, y]], [496] * 4, 16, 256)
     assert sorted((rows, n) for rows, _, n in segs) == [([0, 1], 496), ([2, 3], 496)]
+
+
+@pytest.mark.parametrize("rows,tokens,pays", [(32, 128, False), (32, 256, True), (9, 256, True), (8, 256, False),
+                                              (2, 2048, True), (2, 2032, False)])
+def test_what_pays_is_shared(rows, tokens, pays):
+    table = np.arange(tokens // 16)
+    segs = shared_segments([table] * rows, [tokens] * rows, 16)
+    assert len(segs) == (1 if pays else rows)
 
 
 @pytest.mark.parametrize("group,kv_heads,d,cap,rows", [
@@ -125,6 +133,7 @@ def test_shared_struct_matches_the_c_compiler(tmp_path):
     (tmp_path / "p.c").write_text("\n".join(prog))
     subprocess.check_call(["gcc", "-o", str(tmp_path / "p"), str(tmp_path / "p.c")])
     out = [int(x) for x in subprocess.check_output([str(tmp_path / "p")]).split()]
+    assert _SHARED_PACK.size == ctypes.sizeof(_lib.SharedDesc)
     assert out == [ctypes.sizeof(_lib.SharedDesc)] + [getattr(_lib.SharedDesc, f).offset for f in names]
 
 
