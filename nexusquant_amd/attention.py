@@ -82,7 +82,7 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     projection are read in place.  scale: 1 / sqrt(head_dim) by default.  sliding_window: query i sees
     keys i - window < j <= i.
     Returns [rows, q_heads, head_dim].  Rows behind the plan's sequences are left as they are in `out`,
-    and are zero without one.  Inference only: tensors that require a gradient are refused."""
+    and are zero without one; `out` may be `query`, and must not overlap key or value.  Inference only: tensors that require a gradient are refused."""
     lib = _lib.load()
     for name, t in (("query", query), ("key", key), ("value", value)):
         if not t.is_cuda:
@@ -118,8 +118,9 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         if rows > plan.rows:
             out[plan.rows:].zero_()
     elif (out.shape != shape or out.dtype != dtype or out.device != dev
-          or out.stride(2) != 1 or out.stride(0) % 4 or out.stride(1) % 4 or out.data_ptr() % 8):
-        raise ValueError(f"out must be {tuple(shape)} {dtype} on {dev} with 8-byte aligned head vectors")
+          or out.stride(2) != 1 or out.stride(0) % 4 or out.stride(1) % 4 or out.data_ptr() % 8
+          or (rows > 1 and out.stride(0) == 0) or (hq > 1 and out.stride(1) == 0)):
+        raise ValueError(f"out must be {tuple(shape)} {dtype} on {dev} with 8-byte aligned head vectors of their own")
     if plan.n_tiles == 0:
         return out
     q, q_at, q_row, q_head = _rows(query)

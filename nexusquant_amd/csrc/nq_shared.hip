@@ -114,9 +114,11 @@ shared_attn_kernel(SharedArgs a) {
     const int32_t* const it = a.items + 8 * item;
     const int32_t* const pages = a.pages + it[0];
     const uint32_t tok0 = (uint32_t)it[1];
-    const int n_tok = it[2];
     const int32_t* const seg_rows = a.seg_rows + 2 * it[3];
-    const int G = (int)(a.q_heads / a.kv_heads), n_q = it[4] * G, chunk = it[5];
+    const int G = (int)(a.q_heads / a.kv_heads), chunk = it[5];
+    // what LDS is sized for, whatever a plan from elsewhere holds
+    const int n_tok = (int)min(max((uint32_t)it[2], 1u), (uint32_t)SH::CHUNK);
+    const int n_q = (int)min(max((uint32_t)it[4] * (uint32_t)G, 1u), (uint32_t)SH::ROWS);
 
     // The three chains of loads that the first stage waits for run at once: rows -> queries, pages -> codes,
     // pages -> positions and scales (-> rotation tables).
@@ -515,6 +517,9 @@ extern "C" int nq_shared_attention(const nq_shared_desc* d, void* stream) {
                  p->heads, nq_shared_attention_rows(p->head_dim));
     NQ_CHECK_ARG(d->n_items >= 0 && d->n_slots >= 0 && d->n_many >= 0 && d->n_many <= d->n_items,
                  "nq_shared_attention: n_items %d, n_many %d, n_slots %d", d->n_items, d->n_many, d->n_slots);
+    NQ_CHECK_ARG(d->n_many == d->n_items || d->q_heads / p->heads <= nq_shared_attention_few_rows(),
+                 "nq_shared_attention: over %d query heads per kv head, every item belongs to the n_many of many rows",
+                 nq_shared_attention_few_rows());
     if (d->batch == 0) return NQ_OK;
     NQ_CHECK_ARG(d->query && d->out && d->row_slots, "nq_shared_attention: query, out and row_slots are required");
     NQ_CHECK_ARG(((uintptr_t)d->query & 15u) == 0, "nq_shared_attention: query must be 16-byte aligned");

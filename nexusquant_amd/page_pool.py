@@ -143,7 +143,10 @@ class CompressedPagePool:
             except struct.error:
                 raise ValueError(f"page numbers must be integers in [0, {self.num_pages})") from None
         else:
-            p = np.asarray(pages, dtype=np.int64).reshape(-1)
+            p = np.asarray(pages).reshape(-1)
+            if len(p) and p.dtype.kind not in "iu":
+                raise ValueError(f"page numbers must be integers, got {p.dtype}")
+            p = p.astype(np.int64, copy=False)
         # a negative number is a large one as unsigned
         if len(p) and p.view(np.uint32 if p.dtype == np.int32 else np.uint64).max() >= self.num_pages:
             raise ValueError(f"page numbers must lie in [0, {self.num_pages})")
@@ -360,7 +363,10 @@ class CompressedPagePool:
                              f"{tuple(keys.shape)} / {tuple(values.shape)}")
         if keys.device != self.device or values.device != self.device:
             raise ValueError(f"keys are on {keys.device}, values on {values.device}, the pool on {self.device}")
-        s = np.asarray(slots.tolist() if torch.is_tensor(slots) else slots, dtype=np.int64).reshape(-1)
+        s = np.asarray(slots.tolist() if torch.is_tensor(slots) else slots).reshape(-1)
+        if len(s) and s.dtype.kind not in "iu":
+            raise ValueError(f"slots must be integers, got {s.dtype}")
+        s = s.astype(np.int64, copy=False)
         n = keys.shape[0]
         if len(s) != n:
             raise ValueError(f"{len(s)} slots for {n} tokens")

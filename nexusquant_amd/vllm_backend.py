@@ -480,8 +480,10 @@ def shared_segments(tables: Sequence[np.ndarray], lengths: Sequence[int], page_t
     full = [int(n) // page_tokens for n in lengths]
     out: List[Tuple[List[int], np.ndarray, int]] = []
 
-    def split(rows: List[int], start: int, depth: int) -> None:
-        # the rows agree on their pages before `depth`; those from `start` on are in no segment yet
+    # (rows, start, depth): the rows agree on their pages before `depth`; those from `start` on are in no segment yet
+    todo = [([b for b in range(len(tables)) if lengths[b] > 0], 0, 0)]
+    while todo:
+        rows, start, depth = todo.pop()
         groups: Dict[int, List[int]] = {}
         for b in rows:
             if full[b] > depth:
@@ -501,11 +503,9 @@ def shared_segments(tables: Sequence[np.ndarray], lengths: Sequence[int], page_t
             saved = (len(same) - 1) * tokens
             if saved >= min_saved if min_saved is not None else saved >= _MIN_SAVED and tokens >= _MIN_TOKENS:
                 out.append((same, tables[same[0]][start:end], tokens))
-                split(same, end, end)
+                todo.append((same, end, end))
             else:
-                split(same, start, end)
-
-    split([b for b in range(len(tables)) if lengths[b] > 0], 0, 0)
+                todo.append((same, start, end))
     return out
 
 
@@ -592,6 +592,7 @@ class SharedAttentionPlan:
         self.batch = batch
         self.segments = segments
         self._work: Dict[int, tuple] = {}
+        self._tables: list = []  # rotation tables that calls with this plan have read: a captured graph goes on reading them
 
     def work(self, q_heads: int):
         """(device ints, offsets, items, items of many rows, slots) for q_heads query heads."""
@@ -777,7 +778,7 @@ class NexusQuantPagedAttention:
     def plan_shared(self, pool, block_tables: Sequence[Sequence[int]], context_lens,
                     min_saved: Optional[int] = None) -> SharedAttentionPlan:
         """The plan of rows over a CompressedPagePool: row b attends to the first context_lens[b] tokens of
-        its pages block_tables[b] (0: none).  Full pages that several rows begin with, as forks do, are
+        its pages block_tables[b] (0: none; entries past those tokens are padding).  Full pages that several rows begin with, as forks do, are
         read and decoded once for all of them, where that saves min_saved tokens' decoding (None: where it
         pays; see shared_segments)."""
         if pool.head_dim != self.compressor.head_dim:
@@ -787,10 +788,10 @@ class NexusQuantPagedAttention:
             raise ValueError(f"{len(block_tables)} block tables for {len(ctx)} context lengths")
         tables = []
         for b, n in enumerate(ctx):
-            pages = pool.in_use(block_tables[b], "plan_shared")
-            if not 0 <= n <= len(pages) * pool.page_tokens:
-                raise ValueError(f"row {b}: {n} tokens in {len(pages)} pages of {pool.page_tokens}")
-            tables.append(pages[:pool.pages_for(n)])
+            table = block_tables[b]
+            if not 0 <= n <= len(table) * pool.page_tokens:
+                raise ValueError(f"row {b}: {n} tokens in {len(table)} pages of {pool.page_tokens}")
+            tables.append(pool.in_use(table[:pool.pages_for(n)], "plan_shared"))  # what follows is padding
         return SharedAttentionPlan(pool, len(ctx), shared_segments(tables, ctx, pool.page_tokens, min_saved))
 
     def _shared_tables(self, max_position: int, dev):
@@ -807,7 +808,10 @@ class NexusQuantPagedAttention:
         layer of its pool.  num_heads is a multiple of the pool's heads.  Rows without tokens are zero.
 
         What a row sees is cut by all rows of the plan: outputs of one row alone and in a batch agree to
-        roundings, not bit for bit.  run() differs in its roundings too (values there are not rounded)."""
+        roundings, not bit for bit.  run() differs in its roundings too (values there are not rounded).
+        A captured graph reads the plan's arrays and the rotation tables of the positions up to
+        pool.max_position as they were: keep the plan while it is replayed, and capture again once a token
+        of a larger position is stored."""
         lib = _lib.load()
         pool = plan.pool
         if not query.is_cuda:
@@ -820,6 +824,8 @@ class NexusQuantPagedAttention:
                              f"{tuple(shape)}")
         if dtype not in (torch.float16, torch.bfloat16):
             raise ValueError(f"run_shared takes fp16 or bf16 queries, got {dtype}; run() takes fp32 ones")
+        if query.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError("run_shared has no backward pass; call it under torch.no_grad()")
         b, hq, d = shape
         rows = int(lib.nq_shared_attention_rows(d))
         if hq == 0 or hq % pool.num_heads or hq // pool.num_heads > rows:
@@ -840,7 +846,10 @@ class NexusQuantPagedAttention:
             nbytes = lib.nq_shared_attention_workspace(n_slots, hq, d)
             # of this call alone: calls on other streams and captured graphs have their own
             ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-            dm, dp = self._shared_tables(pool.max_position, dev)
+            tables = self._shared_tables(pool.max_position, dev)
+            if not plan._tables or plan._tables[-1] is not tables:
+                plan._tables.append(tables)
+            dm, dp = tables
             base = ints.address()
             desc = _lib.SharedDesc.from_buffer_copy(_SHARED_PACK.pack(
                 ctypes.addressof(pool.desc), int(layer), b, hq, _lib.dtype_code(dtype), n_items, n_many, n_slots, 0,

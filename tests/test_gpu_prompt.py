@@ -141,6 +141,19 @@ def test_layouts():
     assert torch.equal(prompt_attention(q, one, one, plan), prompt_attention(q, one.contiguous(), one.contiguous(), plan))
 
 
+def test_output_in_place_of_the_query():
+    from nexusquant_amd.attention import plan_prompts, prompt_attention
+    print("[gpu] prompt in place", flush=True)
+    lens = [200, 1, 129]
+    q, k, v = inputs(330, 4, 2, 128, torch.bfloat16, seed=8)
+    v[150:200] = float("nan")  # hidden from the first queries of their tile: summed again after the fast pass
+    plan = plan_prompts(lens, device=DEV)
+    want = prompt_attention(q, k, v, plan)
+    got = prompt_attention(q, k, v, plan, out=q)
+    assert got is q and torch.equal(q.isnan(), want.isnan()) and torch.equal(q.nan_to_num(), want.nan_to_num())
+    assert bool(want[150:200].isnan().all()) and not bool(want[:150].isnan().any())
+
+
 def test_stream_graph_and_repeat():
     from nexusquant_amd.attention import plan_prompts, prompt_attention
     print("[gpu] prompt stream and graph", flush=True)
@@ -179,6 +192,8 @@ def test_refusals():
                  lambda: prompt_attention(q, k, v, plan, scale=-1.0),
                  lambda: prompt_attention(q, k, v, plan, scale=float("nan")),
                  lambda: prompt_attention(q[0], k, v, plan),
+                 lambda: prompt_attention(q, k, v, plan, out=torch.empty_like(q[:1]).expand(20, -1, -1)),
+                 lambda: prompt_attention(q, k, v, plan, out=torch.empty_like(q[:, :1]).expand(-1, 4, -1)),
                  lambda: prompt_attention(q, k, v, plan, out=torch.empty(20, 4, 64, device=DEV))):
         with pytest.raises(ValueError):
             call()

@@ -253,6 +253,30 @@ def test_two_streams_graph_and_repeat():
         assert all(torch.equal(out, want) for _, out in graphs)
 
 
+def test_a_graphs_tables_outlive_longer_ones():
+    """A token of a larger position makes longer rotation tables; a graph captured before reads its own."""
+    from nexusquant_amd import rope
+    print("[gpu] shared graph and longer tables", flush=True)
+    pool = make_pool(1, 60, 2, 16, 64, seed=12)
+    tables, ctx = forks(pool, 400, [5, 60])
+    attn = attention(64)
+    q = queries(2, 8, 64, torch.float16)
+    plan, want = check(attn, pool, tables, ctx, q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attn.run_shared(plan, q)
+    rope.clear_cache()
+    pool.max_position = 9000
+    again = attn.run_shared(attn.plan_shared(pool, tables, ctx, min_saved=1), q)
+    fill = [torch.full((4096, 32), float("nan"), device=DEV) for _ in range(8)]  # where freed tables would have been
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(again, want)
+    del fill
+
+
 def test_refusals():
     print("[gpu] shared refusals", flush=True)
     pool = make_pool(2, 20, 2, 16, 64, seed=10)
@@ -267,6 +291,9 @@ def test_refusals():
                  lambda: attn.run_shared(plan, queries(1, 2 * 257, 64, torch.float16))):
         with pytest.raises(ValueError):
             call()
+    with pytest.raises(NotImplementedError, match="backward"):
+        attn.run_shared(plan, q.requires_grad_())
+    q = q.detach()
     empty = attn.plan_shared(pool, [[], []], [0, 0])
     assert bool((attn.run_shared(empty, queries(2, 4, 64, torch.float16)) == 0).all())
     assert attn.run_shared(attn.plan_shared(pool, [], []), q[:0]).shape == (0, 4, 64)

@@ -63,7 +63,8 @@ def test_wrong_page_numbers_are_refused_and_change_nothing(monkeypatch):
                  lambda: pool.free([-1]), lambda: pool.retain([7]), lambda: pool.copy_pages([0], [5]),
                  lambda: pool.copy_pages([0], [0, 1]), lambda: pool.page(9), lambda: pool.allocate(-1),
                  lambda: pool.slots(a, 0, 9), lambda: pool.slots(a, -1, 2), lambda: pool.free([1 << 40]),
-                 lambda: pool.free([0.5]), lambda: pool.free(np.array([1 << 32])), lambda: pool.retain((-1,))):
+                 lambda: pool.free([0.5]), lambda: pool.free(np.array([1 << 32])), lambda: pool.retain((-1,)),
+                 lambda: pool.retain((0.5,)), lambda: pool.free(np.array([0.0]))):
         with pytest.raises(ValueError):
             call()
     with pytest.raises(_lib.NexusQuantError, match="8 of 10 free"):

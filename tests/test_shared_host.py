@@ -71,6 +71,18 @@ def test_what_pays_is_shared(rows, tokens, pays):
     assert len(segs) == (1 if pays else rows)
 
 
+def test_rows_that_end_one_after_another_are_cut_without_recursion():
+    """2000 rows, each a page longer than the one before: a branch at every page."""
+    pages = np.arange(2000)
+    lengths = [i + 1 for i in range(2000)]
+    segs = shared_segments([pages[:n] for n in lengths], lengths, 1, 1)
+    seen = np.zeros(2000, dtype=int)
+    for rows, seg_pages, n in segs:
+        assert n == len(seg_pages)
+        seen[rows] += n
+    assert list(seen) == lengths and len(segs) == 2000
+
+
 @pytest.mark.parametrize("group,kv_heads,d,cap,rows", [
     (1, 8, 128, 1024, (256, 128)), (4, 1, 64, 1024, (256, 128)), (128, 2, 256, 256, (128, 128)),
     (8, 64, 128, 128, (256, 128)), (2, 3, 128, 1024, (256, 128)), (200, 1, 128, 2048, (256, 128))])
@@ -116,6 +128,13 @@ def test_plan_refuses_bad_tables(monkeypatch):
     attn = NexusQuantPagedAttention(NexusQuantKVCompressor(head_dim=64))
     a = pool.allocate(4)
     assert sorted(s[2] for s in attn.plan_shared(pool, [a, a[:1], []], [16, 3, 0]).segments) == [3, 16]
+    # a rectangular table: what stands behind a row's tokens is padding
+    padded = np.array([a, a[:1] + [-1, 0, 99], [-1] * 4])
+    assert sorted(s[2] for s in attn.plan_shared(pool, padded, [16, 4, 0]).segments) == [4, 16]
+    assert sorted(s[2] for s in attn.plan_shared(pool, torch.from_numpy(padded), torch.tensor([16, 4, 0])).segments) == [4, 16]
+    for tables, ctx in ((padded, [16, 5, 0]), ([[0.5]], [1]), ([np.array([0.5])], [1])):
+        with pytest.raises(ValueError):
+            attn.plan_shared(pool, tables, ctx)
     for tables, ctx in (([a], [17]), ([a], [-1]), ([[9]], [1]), ([a, a], [4]), ([[99]], [1])):
         with pytest.raises(ValueError):
             attn.plan_shared(pool, tables, ctx)
@@ -156,3 +175,13 @@ def test_c_entry_refuses(kw, pool_kw):
     assert lib.nq_shared_attention(ctypes.byref(_lib.SharedDesc(**{**base, **kw})), None) == -1
     assert lib.nq_last_error().startswith(b"nq_shared_attention")
     assert lib.nq_shared_attention(ctypes.byref(_lib.SharedDesc(**{**base, "batch": 0})), None) in (0, -1)
+
+
+def test_c_entry_refuses_wide_groups_among_small_items():
+    """A kv head of more query heads than a small workgroup has rows: its items all belong to the wide ones."""
+    lib = _lib.load()
+    dummy = ctypes.c_void_p(4096)
+    desc = dict(pool=ctypes.pointer(c_pool()), layer=0, batch=1, q_heads=c_pool().heads * 129, q_dtype=_lib.NQ_F16, n_items=2,
+                n_many=1, n_slots=2, query=dummy, out=dummy, items=dummy, pages=dummy, seg_rows=dummy, row_slots=dummy)
+    assert lib.nq_shared_attention(ctypes.byref(_lib.SharedDesc(**desc)), None) == -1
+    assert b"over 128 query heads" in lib.nq_last_error()
