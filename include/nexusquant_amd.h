@@ -636,30 +636,34 @@ int nq_pool_copy_pages(const nq_pool* pool, const int32_t* src, const int32_t* d
  * for j below its count; positions move along, or are j (renumber != 0: keys
  * are stored without rotation, so their rotation follows).  Slots past the
  * count keep what they hold.  New pages are none of the old ones.
- *   tile_seq [n_tiles]   the sequence of each run of nq_pool_move_tokens()
- *                        new tokens (a sequence's runs are consecutive);
- *   seq      [n_seq * 5] per sequence its first tile, tokens kept, tokens it
- *                        had, and where its old and new page numbers start in
- *   tables               (page numbers);
- *   kept                 positions in the sequence, as nq_keep_mask lists
- *                        them (entries outside the sequence are clamped).
- * All device int32 arrays.
+ * plan: plan_ints int32, one after another
+ *   [n_tiles]    the sequence of each run of nq_pool_move_tokens() new tokens
+ *                (a sequence's runs are consecutive);
+ *   [n_seq * 5]  per sequence its first tile, tokens kept, tokens it had, and
+ *                where its old and new page numbers start in what follows;
+ *   page numbers.
+ * plan_on_host != 0: a host array of at most nq_pool_host_ints(), read
+ * during the call; otherwise a device array.
+ * kept (device): positions in the sequence, as nq_keep_mask lists them
+ * (entries outside the sequence are clamped).
  */
 int32_t nq_pool_move_tokens(void);
-int nq_pool_compact(const nq_pool* pool, const int32_t* tile_seq, int32_t n_tiles, const int32_t* seq,
-                    const int32_t* tables, const int32_t* kept, int32_t kept_stride, int32_t renumber, void* stream);
+int32_t nq_pool_host_ints(void);
+int nq_pool_compact(const nq_pool* pool, const int32_t* plan, int32_t plan_ints, int32_t plan_on_host, int32_t n_tiles,
+                    int32_t n_seq, const int32_t* kept, int32_t kept_stride, int32_t renumber, void* stream);
 
 /*
  * Encoded tokens to their slots in one layer: `tokens` is one page of n
  * tokens (nq_page_encode's output and the tokens' positions); token i goes to
- * slot slots[i] = page * pool tokens + offset (device int32 array).  Negative
+ * slot slots[i] = page * pool tokens + offset (int32; a host array of at most
+ * nq_pool_host_ints(), read during the call, or a device array).  Negative
  * slots and slots past the pool are skipped; slots must be distinct.
  *
  * Replaces: NexusQuantPagedAttention.compress_and_cache   vllm_backend.py:622-688
  *           (the cache side, for pages of a pool)
  */
-int nq_pool_write(const nq_pool* pool, int32_t layer, const nq_pool* tokens, const int32_t* slots, int32_t n,
-                  void* stream);
+int nq_pool_write(const nq_pool* pool, int32_t layer, const nq_pool* tokens, const int32_t* slots,
+                  int32_t slots_on_host, int32_t n, void* stream);
 
 /*
  * Decode attention over a pool's pages for rows that share pages: for each

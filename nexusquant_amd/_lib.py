@@ -168,8 +168,9 @@ SIGNATURES = {
     "nq_prompt_attention": ([ctypes.POINTER(PromptDesc), _P], ctypes.c_int),
     "nq_pool_copy_pages": ([ctypes.POINTER(Pool), _P, _P, _I32, _P], ctypes.c_int),
     "nq_pool_move_tokens": ([], ctypes.c_int32),
-    "nq_pool_compact": ([ctypes.POINTER(Pool), _P, _I32, _P, _P, _P, _I32, _I32, _P], ctypes.c_int),
-    "nq_pool_write": ([ctypes.POINTER(Pool), _I32, ctypes.POINTER(Pool), _P, _I32, _P], ctypes.c_int),
+    "nq_pool_host_ints": ([], ctypes.c_int32),
+    "nq_pool_compact": ([ctypes.POINTER(Pool), _P, _I32, _I32, _I32, _I32, _P, _I32, _I32, _P], ctypes.c_int),
+    "nq_pool_write": ([ctypes.POINTER(Pool), _I32, ctypes.POINTER(Pool), _P, _I32, _I32, _P], ctypes.c_int),
     "nq_shared_attention_chunk_tokens": ([_I32], ctypes.c_int32),
     "nq_shared_attention_rows": ([_I32], ctypes.c_int32),
     "nq_shared_attention_few_rows": ([], ctypes.c_int32),

@@ -96,6 +96,10 @@ __global__ __launch_bounds__(256) void pool_copy_kernel(CopyArgs a, uint32_t lay
 
 constexpr int kMoveTokens = 64;  // tokens of a workgroup
 
+// A compaction's plan, or a write's slots, of at most this many integers travel in the launch's arguments: the copy to
+// the device ahead of it and what it waits for were 11 us of a call of 8191 tokens in one layer (90 us with it, 81 without).
+constexpr int kPlanInts = 896;
+
 // A source of token rows: pages of `tokens` rows a head.
 struct MoveArgs {
     PoolPtrs src, dst;
@@ -104,22 +108,25 @@ struct MoveArgs {
     uint32_t head_split;              // workgroups that share a tile's heads
     uint32_t n;                       // writes: tokens in all
     int32_t renumber;
-    // compaction: per tile its sequence, per sequence {first tile, tokens kept, tokens it had, src table, dst table}
-    const int32_t* tile_seq;
-    const int32_t* seq;
-    const int32_t* tables;
+    // compaction: per tile its sequence, per sequence {first tile, tokens kept, tokens it had, src table, dst table},
+    // and from there on the tables; writes: the slot of each token, negative: none
+    const int32_t* plan;
+    uint32_t seq_at, tables_at;
     const int32_t* kept;
     uint32_t kept_stride;
-    // writes: the slot of each token, negative: none
-    const int32_t* slots;
-    uint32_t slot_end;
+    uint32_t slot_end;                // writes: of the pool
 };
+struct InlineArgs : MoveArgs {
+    int32_t ints[kPlanInts];
+};
+__device__ __forceinline__ int32_t plan_at(const MoveArgs& a, uint32_t i) { return a.plan[i]; }
+__device__ __forceinline__ int32_t plan_at(const InlineArgs& a, uint32_t i) { return a.ints[i]; }
 
 // Rows of D bytes: D / 16 lanes a row.  The workgroup's token slots are worked out once, into
 // LDS, and serve every head of its share: keys and values of a head are 2 * 64 rows, moved as
 // 16-byte pieces with all of a thread's loads ahead of its stores.
-template <int D, bool COMPACT>
-__global__ __launch_bounds__(256) void pool_move_kernel(MoveArgs a) {
+template <int D, bool COMPACT, typename Args>
+__global__ __launch_bounds__(256) void pool_move_kernel(Args a) {
     constexpr int UR = D / 16;                    // 16-byte units a row
     constexpr int PER = kMoveTokens * UR / 256;   // of a role and head, per thread
     __shared__ uint64_t s_src[kMoveTokens], s_dst[kMoveTokens];  // row index of head 0, page by page
@@ -127,17 +134,19 @@ __global__ __launch_bounds__(256) void pool_move_kernel(MoveArgs a) {
     const uint32_t layer = blockIdx.y;
     uint32_t n_tok;
     if constexpr (COMPACT) {
-        const int32_t sq = a.tile_seq[tile];
-        const int32_t* const s = a.seq + 5 * sq;
-        const uint32_t first = (tile - (uint32_t)s[0]) * kMoveTokens;
-        n_tok = min((uint32_t)s[1] - first, (uint32_t)kMoveTokens);
+        const int32_t sq = plan_at(a, tile);
+        const uint32_t s = a.seq_at + 5u * (uint32_t)sq;
+        const uint32_t first = (tile - (uint32_t)plan_at(a, s)) * kMoveTokens;
+        n_tok = min((uint32_t)plan_at(a, s + 1) - first, (uint32_t)kMoveTokens);
         if (threadIdx.x < n_tok) {
             const uint32_t j = first + threadIdx.x;
+            const int32_t had = plan_at(a, s + 2);
             int32_t i = a.kept[(size_t)sq * a.kept_stride + j];
-            i = i < 0 ? 0 : (i >= s[2] ? s[2] - 1 : i);  // the caller's list; clamped, so no page is read past its sequence
+            i = i < 0 ? 0 : (i >= had ? had - 1 : i);  // the caller's list; clamped, so no page is read past its sequence
             const uint32_t sp = (uint32_t)i / a.src_tokens, so = (uint32_t)i % a.src_tokens;
             const uint32_t dp = j / a.dst_tokens, d0 = j % a.dst_tokens;
-            const uint64_t spage = (uint32_t)a.tables[s[3] + sp], dpage = (uint32_t)a.tables[s[4] + dp];
+            const uint64_t spage = (uint32_t)plan_at(a, a.tables_at + (uint32_t)plan_at(a, s + 3) + sp);
+            const uint64_t dpage = (uint32_t)plan_at(a, a.tables_at + (uint32_t)plan_at(a, s + 4) + dp);
             s_src[threadIdx.x] = spage * a.heads * a.src_tokens + so;
             s_dst[threadIdx.x] = dpage * a.heads * a.dst_tokens + d0;
             if (layer == 0 && part == 0)
@@ -149,7 +158,7 @@ __global__ __launch_bounds__(256) void pool_move_kernel(MoveArgs a) {
         n_tok = min(a.n - first, (uint32_t)kMoveTokens);
         if (threadIdx.x < n_tok) {
             const uint32_t j = first + threadIdx.x;
-            const int32_t slot = a.slots[j];
+            const int32_t slot = plan_at(a, j);
             const bool ok = slot >= 0 && (uint32_t)slot < a.slot_end;
             const uint64_t dp = ok ? (uint32_t)slot / a.dst_tokens : 0u, d0 = ok ? (uint32_t)slot % a.dst_tokens : 0u;
             s_src[threadIdx.x] = j;  // one page of n tokens a head
@@ -193,15 +202,24 @@ static uint32_t head_split(uint32_t heads, uint64_t tiles) {
     return split < heads ? split : heads;
 }
 
-template <bool COMPACT>
-static hipError_t launch_move(const MoveArgs& a, uint32_t tiles, uint32_t layers, hipStream_t s) {
+template <bool COMPACT, typename Args>
+static hipError_t launch_move(const Args& a, uint32_t tiles, uint32_t layers, hipStream_t s) {
     const dim3 grid(tiles * a.head_split, layers);
     switch (a.d) {
-        case 64: hipLaunchKernelGGL((pool_move_kernel<64, COMPACT>), grid, dim3(256), 0, s, a); break;
-        case 128: hipLaunchKernelGGL((pool_move_kernel<128, COMPACT>), grid, dim3(256), 0, s, a); break;
-        default: hipLaunchKernelGGL((pool_move_kernel<256, COMPACT>), grid, dim3(256), 0, s, a); break;
+        case 64: hipLaunchKernelGGL((pool_move_kernel<64, COMPACT, Args>), grid, dim3(256), 0, s, a); break;
+        case 128: hipLaunchKernelGGL((pool_move_kernel<128, COMPACT, Args>), grid, dim3(256), 0, s, a); break;
+        default: hipLaunchKernelGGL((pool_move_kernel<256, COMPACT, Args>), grid, dim3(256), 0, s, a); break;
     }
     return hipGetLastError();
+}
+
+template <bool COMPACT>
+static hipError_t launch_plan(const MoveArgs& a, bool on_host, uint32_t ints, uint32_t tiles, uint32_t layers, hipStream_t s) {
+    if (!on_host) return launch_move<COMPACT>(a, tiles, layers, s);
+    InlineArgs in = {};
+    static_cast<MoveArgs&>(in) = a;
+    memcpy(in.ints, a.plan, (size_t)ints * sizeof(int32_t));
+    return launch_move<COMPACT>(in, tiles, layers, s);
 }
 
 template <typename ScaleUnit>
@@ -307,33 +325,38 @@ extern "C" int nq_pool_copy_pages(const nq_pool* p, const int32_t* src, const in
 
 extern "C" int32_t nq_pool_move_tokens(void) { return nq::kMoveTokens; }
 
-extern "C" int nq_pool_compact(const nq_pool* p, const int32_t* tile_seq, int32_t n_tiles, const int32_t* seq,
-                               const int32_t* tables, const int32_t* kept, int32_t kept_stride, int32_t renumber,
-                               void* stream) {
+extern "C" int32_t nq_pool_host_ints(void) { return nq::kPlanInts; }
+
+extern "C" int nq_pool_compact(const nq_pool* p, const int32_t* plan, int32_t plan_ints, int32_t plan_on_host, int32_t n_tiles,
+                               int32_t n_seq, const int32_t* kept, int32_t kept_stride, int32_t renumber, void* stream) {
     using namespace nq;
     if (int st = check_pool(p, "nq_pool_compact")) return st;
     NQ_CHECK_ARG(n_tiles >= 0 && kept_stride >= 0, "nq_pool_compact: n_tiles %d, kept_stride %d", n_tiles, kept_stride);
     if (n_tiles == 0) return NQ_OK;
-    NQ_CHECK_ARG(tile_seq && seq && tables && kept, "nq_pool_compact: the plan's arrays and the kept list are required");
+    NQ_CHECK_ARG(plan && kept, "nq_pool_compact: the plan and the kept list are required");
+    NQ_CHECK_ARG(n_seq > 0 && plan_ints > 0 && (int64_t)n_tiles + 5ll * n_seq <= plan_ints,
+                 "nq_pool_compact: %d integers hold no plan of %d tiles and %d sequences", plan_ints, n_tiles, n_seq);
+    NQ_CHECK_ARG(!plan_on_host || plan_ints <= kPlanInts, "nq_pool_compact: a host plan has at most %d integers, got %d",
+                 kPlanInts, plan_ints);
     MoveArgs a = {};
     a.src = a.dst = pool_ptrs(p);
     a.src_tokens = a.dst_tokens = (uint32_t)p->tokens;
     a.heads = (uint32_t)p->heads;
     a.d = (uint32_t)p->head_dim;
     a.renumber = renumber;
-    a.tile_seq = tile_seq;
-    a.seq = seq;
-    a.tables = tables;
+    a.plan = plan;
+    a.seq_at = (uint32_t)n_tiles;
+    a.tables_at = (uint32_t)n_tiles + 5u * (uint32_t)n_seq;
     a.kept = kept;
     a.kept_stride = (uint32_t)kept_stride;
     a.head_split = head_split(a.heads, (uint64_t)n_tiles * p->layers);
     NQ_CHECK_ARG((uint64_t)n_tiles * a.head_split <= max_blocks(256), "nq_pool_compact: grid too large");
-    NQ_CHECK_HIP(launch_move<true>(a, (uint32_t)n_tiles, (uint32_t)p->layers, (hipStream_t)stream));
+    NQ_CHECK_HIP(launch_plan<true>(a, plan_on_host, (uint32_t)plan_ints, (uint32_t)n_tiles, (uint32_t)p->layers, (hipStream_t)stream));
     return NQ_OK;
 }
 
-extern "C" int nq_pool_write(const nq_pool* p, int32_t layer, const nq_pool* tokens, const int32_t* slots, int32_t n,
-                             void* stream) {
+extern "C" int nq_pool_write(const nq_pool* p, int32_t layer, const nq_pool* tokens, const int32_t* slots,
+                             int32_t slots_on_host, int32_t n, void* stream) {
     using namespace nq;
     if (int st = check_pool(p, "nq_pool_write")) return st;
     NQ_CHECK_ARG(n >= 0 && layer >= 0 && layer < p->layers, "nq_pool_write: n %d, layer %d of %d", n, layer, p->layers);
@@ -343,6 +366,7 @@ extern "C" int nq_pool_write(const nq_pool* p, int32_t layer, const nq_pool* tok
                      tokens->head_dim == p->head_dim,
                  "nq_pool_write: the tokens must be one page of n tokens of the pool's heads and head_dim");
     NQ_CHECK_ARG(slots != nullptr, "nq_pool_write: slots are required");
+    NQ_CHECK_ARG(!slots_on_host || n <= kPlanInts, "nq_pool_write: a host array has at most %d slots, got %d", kPlanInts, n);
     MoveArgs a = {};
     a.src = pool_ptrs(tokens);
     a.dst = pool_ptrs(p);
@@ -356,11 +380,11 @@ extern "C" int nq_pool_write(const nq_pool* p, int32_t layer, const nq_pool* tok
     a.heads = (uint32_t)p->heads;
     a.d = (uint32_t)p->head_dim;
     a.n = (uint32_t)n;
-    a.slots = slots;
+    a.plan = slots;
     a.slot_end = (uint32_t)p->pages * (uint32_t)p->tokens;
     const uint32_t tiles = ((uint32_t)n + kMoveTokens - 1) / kMoveTokens;
     a.head_split = head_split(a.heads, tiles);
     NQ_CHECK_ARG((uint64_t)tiles * a.head_split <= max_blocks(256), "nq_pool_write: grid too large");
-    NQ_CHECK_HIP(launch_move<false>(a, tiles, 1u, (hipStream_t)stream));
+    NQ_CHECK_HIP(launch_plan<false>(a, slots_on_host, (uint32_t)n, tiles, 1u, (hipStream_t)stream));
     return NQ_OK;
 }

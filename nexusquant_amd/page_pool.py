@@ -319,12 +319,14 @@ class CompressedPagePool:
             new = self._take(ends[-1])
             try:
                 if n_tiles:
-                    plan = to_device(np.concatenate([np.repeat(np.arange(batch, dtype=np.int32), tiles),
-                                                     np.array(seq, dtype=np.int32), flat, new]), self.device)
-                    base = plan.data_ptr()
+                    plan = np.concatenate([np.repeat(np.arange(batch, dtype=np.int32), tiles),
+                                           np.array(seq, dtype=np.int32), flat, new])
+                    host = len(plan) <= lib.nq_pool_host_ints()
+                    if not host:
+                        plan = to_device(plan, self.device)
                     with on_device(self.device):
-                        st = lib.nq_pool_compact(ctypes.byref(self.desc), base, n_tiles, base + 4 * n_tiles,
-                                                 base + 4 * (n_tiles + len(seq)), _addr(idx), idx.shape[1],
+                        st = lib.nq_pool_compact(ctypes.byref(self.desc), plan.ctypes.data if host else plan.data_ptr(),
+                                                 len(plan), host, n_tiles, batch, _addr(idx), idx.shape[1],
                                                  int(bool(renumber)),
                                                  ctypes.c_void_p(_lib.current_stream_handle(self.device)))
                     _lib.check(st, "nq_pool_compact")
@@ -381,12 +383,16 @@ class CompressedPagePool:
                 raise ValueError(f"write: page {int(p[self._refs[p] > 1][0])} is shared and cannot be written")
             with torch.cuda.device(self.device):
                 page = compressor.compress_page(keys.permute(1, 0, 2), values.permute(1, 0, 2), positions)
-                where = to_device(s, self.device)
+                host = n <= lib.nq_pool_host_ints()
+                where = np.maximum(s, -1).astype(np.int32)
+                if not host:
+                    where = to_device(where, self.device)
                 tokens = _lib.Pool(layers=1, pages=1, heads=self.num_heads, tokens=n, head_dim=self.head_dim,
                                    key_codes=_addr(page.key_codes), value_codes=_addr(page.value_codes),
                                    key_scales=_addr(page.key_scales), value_scales=_addr(page.value_scales),
                                    positions=_addr(page.positions))
-                st = lib.nq_pool_write(ctypes.byref(self.desc), int(layer), ctypes.byref(tokens), _addr(where), n,
+                st = lib.nq_pool_write(ctypes.byref(self.desc), int(layer), ctypes.byref(tokens),
+                                       where.ctypes.data if host else where.data_ptr(), host, n,
                                        ctypes.c_void_p(_lib.current_stream_handle(self.device)))
             _lib.check(st, "nq_pool_write")
             self.max_position = max(self.max_position, page.max_position or 0)

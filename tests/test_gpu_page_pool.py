@@ -104,6 +104,7 @@ def compact_np(f, tables, kept_idx, n_kept, new, t, renumber):
     (3, 4, 24, 64, [200, 3, 129], 0.6, False),
     (1, 8, 64, 128, [1000], 0.75, True),
     (2, 1, 1, 64, [150, 70], 0.3, False),                 # one token a page
+    (1, 1, 4, 64, [4001, 3], 0.25, True),                 # a plan past what a launch's arguments hold
 ])
 def test_compact(layers, heads, tokens, d, lens, rate, renumber):
     print(f"[gpu] compact {lens} tokens={tokens} rate={rate}", flush=True)
@@ -188,7 +189,8 @@ def test_compact_refusals():
 
 
 @pytest.mark.parametrize("heads,tokens,d,dtype,n", [(2, 16, 128, torch.float16, 1), (1, 7, 64, torch.bfloat16, 40),
-                                                    (8, 16, 128, torch.bfloat16, 130), (3, 5, 256, torch.float32, 65)])
+                                                    (8, 16, 128, torch.bfloat16, 130), (3, 5, 256, torch.float32, 65),
+                                                    (1, 16, 64, torch.float16, 1000)])
 def test_write_stores_what_the_page_encoder_makes(heads, tokens, d, dtype, n):
     from nexusquant_amd.vllm_backend import NexusQuantKVCompressor
     print(f"[gpu] write heads={heads} tokens={tokens} d={d} n={n}", flush=True)
@@ -240,7 +242,7 @@ def test_write_refusals():
         with pytest.raises(ValueError):
             call()
     pool.write(comp, [], k[:0], k[:0], [])
-    pool.write(comp, [-1, -1], k, k, [0, 1])
+    pool.write(comp, [-1, -(1 << 40)], k, k, [0, 1])
     assert_same(pool, before)
 
 

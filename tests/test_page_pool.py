@@ -170,19 +170,22 @@ def test_pool_entry_points_refuse_bad_geometry():
                dict(key_codes=ctypes.c_void_p(4104)), dict(layers=65536), dict(pages=1 << 27),
                dict(heads=1 << 14, tokens=1 << 14)):
         assert lib.nq_pool_copy_pages(ctypes.byref(c_pool(**kw)), s, s, 1, None) == -1, kw
-        assert lib.nq_pool_compact(ctypes.byref(c_pool(**kw)), dummy, 1, dummy, dummy, dummy, 8, 0, None) == -1, kw
-        assert lib.nq_pool_write(ctypes.byref(c_pool(**kw)), 0, ctypes.byref(c_pool(pages=1)), dummy, 16, None) == -1, kw
+        assert lib.nq_pool_compact(ctypes.byref(c_pool(**kw)), dummy, 100, 0, 1, 1, dummy, 8, 0, None) == -1, kw
+        assert lib.nq_pool_write(ctypes.byref(c_pool(**kw)), 0, ctypes.byref(c_pool(pages=1)), dummy, 0, 16, None) == -1, kw
     ok = ctypes.byref(c_pool())
     assert lib.nq_pool_copy_pages(None, s, s, 1, None) == -1
     assert lib.nq_pool_copy_pages(ok, s, s, -1, None) == -1
     assert lib.nq_pool_copy_pages(ok, None, s, 1, None) == -1
     assert lib.nq_pool_copy_pages(ok, None, None, 0, None) == 0
-    assert lib.nq_pool_compact(ok, None, 0, None, None, None, 0, 0, None) == 0
-    assert lib.nq_pool_compact(ok, dummy, 1, None, dummy, dummy, 8, 0, None) == -1
-    assert lib.nq_pool_compact(ok, dummy, -1, dummy, dummy, dummy, 8, 0, None) == -1
+    assert lib.nq_pool_compact(ok, None, 0, 0, 0, 0, None, 0, 0, None) == 0
+    for kw in (dict(plan=None), dict(kept=None), dict(n_tiles=-1), dict(n_seq=0), dict(plan_ints=5), dict(stride=-1),
+               dict(plan_ints=lib.nq_pool_host_ints() + 1, on_host=1)):
+        x = {**dict(plan=dummy, plan_ints=100, on_host=0, n_tiles=1, n_seq=1, kept=dummy, stride=8), **kw}
+        assert lib.nq_pool_compact(ok, *x.values(), 0, None) == -1, kw
+        assert lib.nq_last_error().startswith(b"nq_pool_compact")
     one = ctypes.byref(c_pool(pages=1))
-    assert lib.nq_pool_write(ok, 0, None, None, 0, None) == 0
-    assert lib.nq_pool_write(ok, 1, one, dummy, 16, None) == -1       # no such layer
-    assert lib.nq_pool_write(ok, 0, one, dummy, 15, None) == -1       # not one page of n tokens
-    assert lib.nq_pool_write(ok, 0, ctypes.byref(c_pool(pages=1, heads=4)), dummy, 16, None) == -1
-    assert lib.nq_pool_write(ok, 0, one, None, 16, None) == -1
+    assert lib.nq_pool_write(ok, 0, None, None, 0, 0, None) == 0
+    assert lib.nq_pool_write(ok, 1, one, dummy, 0, 16, None) == -1       # no such layer
+    assert lib.nq_pool_write(ok, 0, one, dummy, 0, 15, None) == -1       # not one page of n tokens
+    assert lib.nq_pool_write(ok, 0, ctypes.byref(c_pool(pages=1, heads=4)), dummy, 0, 16, None) == -1
+    assert lib.nq_pool_write(ok, 0, one, None, 0, 16, None) == -1
