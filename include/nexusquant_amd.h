@@ -670,17 +670,15 @@ int nq_pool_write(const nq_pool* pool, int32_t layer, const nq_pool* tokens, con
  * batch row and query head softmax(q . k / scale_divisor) . v over the row's
  * tokens, k and v the pages' keys and values.  The tokens come as segments: pages that a list of
  * rows sees whole; a row's tokens are the union of its segments.
- *   items    [n_items * 8] chunks of segments, up to
- *            nq_shared_attention_chunk_tokens(many) tokens each:
+ *   items    [n_items * 8] chunks of segments: the first n_many of kind 0, the
+ *            last n_few of kind 2, those between of kind 1
  *              [0] where the segment's pages start in `pages`
  *              [1] the chunk's first token, counted from there
- *              [2] its tokens (1 ..)
+ *              [2] its tokens, 1 .. nq_shared_attention_chunk_tokens(kind)
  *              [3] where its rows start in `seg_rows` (entries)
- *              [4] rows, at most nq_shared_attention_rows(head_dim) / (q_heads / heads)
+ *              [4] rows; times q_heads / heads at most
+ *                  nq_shared_attention_rows(head_dim, kind)
  *              [5] the chunk's number in its segment;  [6..7] unused
- *            The first n_many of them (many = 1) may have that many rows; those after
- *            them have at most nq_shared_attention_few_rows() query rows
- *            (rows x q_heads / heads).
  *   pages    page numbers
  *   seg_rows [entries * 2] batch row, and the row's slot of the segment's
  *            first chunk
@@ -697,8 +695,7 @@ typedef struct nq_shared_desc {
     const nq_pool* pool;
     int32_t layer, batch, q_heads;
     int32_t q_dtype;            /* NQ_F16 / NQ_BF16 */
-    int32_t n_items, n_many, n_slots;
-    int32_t reserved;
+    int32_t n_items, n_many, n_few, n_slots;
     const void* query;
     void* out;
     const int32_t* items;
@@ -714,9 +711,8 @@ typedef struct nq_shared_desc {
     int64_t workspace_bytes;
 } nq_shared_desc;
 
-int32_t nq_shared_attention_chunk_tokens(int32_t many);
-int32_t nq_shared_attention_rows(int32_t head_dim);
-int32_t nq_shared_attention_few_rows(void);
+int32_t nq_shared_attention_chunk_tokens(int32_t kind);
+int32_t nq_shared_attention_rows(int32_t head_dim, int32_t kind);
 int64_t nq_shared_attention_workspace(int32_t n_slots, int32_t q_heads, int32_t head_dim);
 int nq_shared_attention(const nq_shared_desc* desc, void* stream);
 

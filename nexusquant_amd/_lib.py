@@ -115,7 +115,7 @@ class SharedDesc(ctypes.Structure):
         ("pool", ctypes.POINTER(Pool)),
         ("layer", ctypes.c_int32), ("batch", ctypes.c_int32), ("q_heads", ctypes.c_int32),
         ("q_dtype", ctypes.c_int32), ("n_items", ctypes.c_int32), ("n_many", ctypes.c_int32),
-        ("n_slots", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("n_few", ctypes.c_int32), ("n_slots", ctypes.c_int32),
         ("query", _P), ("out", _P), ("items", _P), ("pages", _P), ("seg_rows", _P), ("row_slots", _P),
         ("rope_sin_minus_cos", _P), ("rope_cos_plus_sin", _P), ("rope_n_pos", ctypes.c_int64),
         ("hadamard_scale", ctypes.c_float), ("scale_divisor", ctypes.c_float),
@@ -172,8 +172,7 @@ SIGNATURES = {
     "nq_pool_compact": ([ctypes.POINTER(Pool), _P, _I32, _I32, _I32, _I32, _P, _I32, _I32, _P], ctypes.c_int),
     "nq_pool_write": ([ctypes.POINTER(Pool), _I32, ctypes.POINTER(Pool), _P, _I32, _I32, _P], ctypes.c_int),
     "nq_shared_attention_chunk_tokens": ([_I32], ctypes.c_int32),
-    "nq_shared_attention_rows": ([_I32], ctypes.c_int32),
-    "nq_shared_attention_few_rows": ([], ctypes.c_int32),
+    "nq_shared_attention_rows": ([_I32, _I32], ctypes.c_int32),
     "nq_shared_attention_workspace": ([_I32, _I32, _I32], _I64),
     "nq_shared_attention": ([ctypes.POINTER(SharedDesc), _P], ctypes.c_int),
     "nq_e8_dequant_matmul": ([_P, _P, _P, _P, _I64, _I32, _I32, _I32, _P], ctypes.c_int),

@@ -1,10 +1,11 @@
 // Decode attention over a pool's pages for rows that share pages: what several rows begin
 // with is read and decoded once for all of them.
 //
-// The host cuts the rows' tokens into segments: a run of pages and the batch rows that see
-// all its tokens (a shared prefix: many rows; a row's own rest: one).  A workgroup takes a
-// chunk of a segment's tokens, one kv head, and up to 256 (head_dim 256: 128) of the segment's
-// query rows (batch rows x the kv head's query heads).  Stage by stage (128 tokens; 64) it
+// The host cuts the rows' tokens into segments: a run of pages and the batch rows that see all its
+// tokens (a shared prefix: many rows; a row's own rest: one).  A workgroup takes a chunk of a segment's
+// tokens, one kv head, and the segment's query rows (batch rows x the kv head's query heads), up to 16 of
+// them (few_attn_kernel, below), 128 or 256 (shared_attn_kernel, two shapes).  The latter, stage by stage
+// (128 tokens; 64),
 //  1. decodes keys and values into LDS as fp16, all waves together: keys through the int8
 //     matrix cores (nq_keymfma.h), scaled and rotated in fp32; values as their codes: their
 //     scales go with the softmax weights, and the transform, which is linear, with a row's
@@ -13,6 +14,10 @@
 //     several waves share them and split the tiles, and their sums are joined in LDS at the end.
 // A partial (maximum, sum, value sum) per query row and chunk goes to the workspace; the
 // combine kernel joins a row's chunks.
+//
+// What bounds it: 512 query rows of 8 kv heads x 128 over 32768 tokens, 122 us (560 TFLOP/s): the products by
+// themselves take 105 of them (every wave reads every key and value from LDS), decoding by itself 78, and they run
+// under each other only in part.  Few rows: see there.
 #include "nq_flash.h"
 #include "nq_keymfma.h"
 #include "nq_rowmath.h"
@@ -25,7 +30,7 @@ using namespace flash;
 // and a stage is decoded under the attention to the one before it; two stage buffers, 128 KB of LDS at head_dim
 // 128 and 256, so one workgroup on a CU.  Not MANY: decoding counts, and several small workgroups on a CU hide
 // each other's loads.  8 kv heads x 128, us: 512 query rows x 32768 tokens 122 (MANY) and 230; 128 rows x
-// 16384 35.0 and 38.9, x 4096 24.8 and 25.5; 64 rows x 8192 23.4 and 23.8; 8 rows (32 heads x 64) 63.6 and 41.
+// 16384 35.0 and 38.9, x 4096 24.8 and 25.5; 64 rows x 8192 23.4 and 23.8.
 template <int D, bool MANY>
 struct Shape {
     static constexpr int WAVES = MANY && D <= 128 ? 8 : 4;
@@ -64,30 +69,42 @@ struct SharedArgs {
 // bf16 queries of a row to fp16, and the power of two taken out of them: scaled so that the row's
 // largest is in [2^14, 2^15), where all of it that counts is exact in fp16 (8 bits of 11; what falls
 // below 2^-24 is 2^-38 of the largest).
-template <int KS>
-__device__ __forceinline__ float bf16_queries(u32x4 (&q)[KS]) {
+template <typename Words, typename Max>
+__device__ __forceinline__ float bf16_queries(Words& q, Max row_max) {
+    constexpr int N = sizeof(Words) / 4;
+    uint32_t* const words = reinterpret_cast<uint32_t*>(&q);
     float big = 0.0f;
 #pragma unroll
-    for (int i = 0; i < KS; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint32_t w = q[i][k];
-            big = __builtin_fmaxf(big, __builtin_fmaxf(__builtin_fabsf(bf16_bits_to_f32(w & 0xffffu)),
-                                                       __builtin_fabsf(bf16_bits_to_f32(w >> 16))));
-        }
-    big = both_max(big);
+    for (int i = 0; i < N; ++i) {
+        const uint32_t w = words[i];
+        big = __builtin_fmaxf(big, __builtin_fmaxf(__builtin_fabsf(bf16_bits_to_f32(w & 0xffffu)),
+                                                   __builtin_fabsf(bf16_bits_to_f32(w >> 16))));
+    }
+    big = row_max(big);
     int e = 0;
     if (big > 0.0f && big < __builtin_inff()) (void)__builtin_frexpf(big, &e);
     e = max(e - 15, -126);  // bf16's subnormals: scaled as far as fp32 reaches
     const float f = __builtin_ldexpf(1.0f, -e);
 #pragma unroll
-    for (int i = 0; i < KS; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint32_t w = q[i][k];
-            q[i][k] = pack2<NQ_F16>(bf16_bits_to_f32(w & 0xffffu) * f, bf16_bits_to_f32(w >> 16) * f);
-        }
+    for (int i = 0; i < N; ++i) {
+        const uint32_t w = words[i];
+        words[i] = pack2<NQ_F16>(bf16_bits_to_f32(w & 0xffffu) * f, bf16_bits_to_f32(w >> 16) * f);
+    }
     return __builtin_ldexpf(1.0f, e);
+}
+
+// The values' scales go with the weights, so that the codes are exact in fp16 and one rounding is left.
+// Times 2^vexp the chunk's largest is in [64, 128): weights (at most 2^kSlack) stay below 2^15, and keep
+// their 11 bits down to 2^-20 of that.
+template <int NW>
+__device__ __forceinline__ int value_exponent(const float (&wave_max)[NW]) {
+    float m = wave_max[0];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) m = __builtin_fmaxf(m, wave_max[w]);
+    int e = 0;
+    if (!(m > 0.0f && m < __builtin_inff())) return 0;
+    (void)__builtin_frexpf(m, &e);
+    return 7 - e;
 }
 
 template <int D, int QDT, bool MANY>
@@ -147,7 +164,7 @@ shared_attn_kernel(SharedArgs a) {
     auto load = [&](int s0, auto&& row_of) {
 #pragma unroll
         for (int u = 0; u < SH::UNITS; ++u) {
-            const int first = s0 + 16 * (NW * u + wave);
+            const int first = s0 + 16 * (SH::UNITS * wave + u);
             const int8_t* const p = a.kc + (size_t)row_of(first + (lane >> 2)) * D + KM::KPL * (lane & 3);
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf)
@@ -199,23 +216,11 @@ shared_attn_kernel(SharedArgs a) {
     for (int o = 32; o >= 1; o >>= 1) vmax = __builtin_fmaxf(vmax, __shfl_xor(vmax, o, 64));
     if (lane == 0) s_max[wave] = vmax;
     float c = a.c;
-    if constexpr (QDT == NQ_BF16) c *= bf16_queries(rows.q);
+    if constexpr (QDT == NQ_BF16) c *= bf16_queries(rows.q, [](float v) { return both_max(v); });
     KM signs;
     signs.init(lane);
     __syncthreads();
-    // The values' scales go with the weights, so that the codes are exact in fp16 and one rounding is left.
-    // Times 2^vexp the chunk's largest is in [64, 128): weights (at most 2^kSlack) stay below 2^15, and keep
-    // their 11 bits down to 2^-20 of that.
-    int vexp = 0;
-    {
-        float m = s_max[0];
-#pragma unroll
-        for (int w = 1; w < NW; ++w) m = __builtin_fmaxf(m, s_max[w]);
-        if (m > 0.0f && m < __builtin_inff()) {
-            (void)__builtin_frexpf(m, &vexp);
-            vexp = 7 - vexp;
-        }
-    }
+    const int vexp = value_exponent<NW>(s_max);
     for (int i = threadIdx.x; i < n_slots; i += NT) s_vs[i] = __builtin_ldexpf(s_vs[i], vexp);  // used after the next barrier
 
     // The stage at s0 to LDS: its codes are in registers, and those of the stage after it follow.
@@ -234,7 +239,7 @@ shared_attn_kernel(SharedArgs a) {
         // they arrive a row per 16 lanes, and every lane then reads its own coordinates.
 #pragma unroll
         for (int u = 0; u < SH::UNITS; ++u) {
-            const int row0 = 16 * (NW * u + wave);
+            const int row0 = 16 * (SH::UNITS * wave + u);
             char* const krows = kbuf + row0 * ROWB;
             char* const vrows = krows + STAGE * ROWB;
 #pragma unroll
@@ -249,7 +254,7 @@ shared_attn_kernel(SharedArgs a) {
         }
 #pragma unroll
         for (int u = 0; u < SH::UNITS; ++u) {
-            const int row0 = 16 * (NW * u + wave);
+            const int row0 = 16 * (SH::UNITS * wave + u);
             char* const krows = kbuf + row0 * ROWB;
             char* const vrows = krows + STAGE * ROWB;
             const float k_scale = (0.5f * f16_bits_to_f32(s_ks[s0 + row0 + n16])) * a.hscale;
@@ -346,12 +351,18 @@ shared_attn_kernel(SharedArgs a) {
             __syncthreads();
         }
     } else {
+        // Up to 32 rows: every wave has all of them and attends to the tokens that it decoded itself.  Its LDS accesses
+        // run in order, so the waves need no barriers and drift apart, one's loads under another's work (3 to 5 %).
+        const bool alone = rw == 1;
         for (int s0 = 0; s0 < n_tok; s0 += STAGE) {
             decode(s0, s_kv[0]);
-            __syncthreads();
+            if (alone) asm volatile("" ::: "memory");
+            else __syncthreads();
             attend(s0, s_kv[0]);
-            __syncthreads();
+            if (alone) asm volatile("" ::: "memory");
+            else __syncthreads();
         }
+        if (alone) __syncthreads();  // the sums go over the other waves' stages
     }
 
     // ---- the waves' sums joined, and written ----
@@ -396,6 +407,306 @@ shared_attn_kernel(SharedArgs a) {
         if constexpr (MANY) __builtin_nontemporal_store(y, to);
         else *to = y;
     }
+}
+
+// ------------------------------------------------------------------- few rows ----
+
+// Up to 16 query rows of a kv head: a wave takes 16 tokens at a time through 16x16x16 MFMAs, from their codes to the
+// output without LDS between.  The int8 products leave a key's coordinates 16 t + 4 kg + i with lane (token, kg), which is
+// how the next product takes its A operand: S = K q^T comes out as lane (query, kg) with tokens 4 kg + i, which is how
+// P^T goes into O^T += V^T P^T.  For V^T lane (n, kg) reads the D / 16 bytes from D / 16 n on of tokens 4 kg + i and
+// turns them four by four, so tile j of the output is coordinates D / 16 r + j.  Keys stay without scales, which go with
+// the logits (sums of codes are below 2 D 127: they fit fp16).  Waves need no barriers; what a wave's next 16 tokens need
+// is loaded into registers as soon as they are free, without a branch, so that the waits count only what they must.
+//
+// us here and in the small shape above: 2 rows x 2 heads of 32 kv heads x 128 over 6352 own tokens 39.7 and 51.8 (2.7
+// TB/s of codes and scales), 64 x 8 of 8 over 512 28.8 and 35.8, 3 x 8 of 8 x 256 over 9184 40.6 and 71, 1 x 8 of 8 x 128
+// over 131072 106 and 118.  Loads alone take 29 of the first's 39.7; the rest is conversions (some 280 vector
+// instructions for 16 tokens of a head) and rows of the rotation table, twice the bytes of the codes, from L2.
+template <int D>
+struct Few {
+    static constexpr int WAVES = 4, ROWS = 16;
+    static constexpr int CHUNK = 1024;  // most tokens of a chunk
+    static constexpr int PER_SIMD = D == 64 ? 4 : D == 128 ? 3 : 2;
+};
+
+// over the lanes n, n + 16, n + 32, n + 48
+__device__ __forceinline__ f32x2 rows16(float v) {  // the values of lanes n and n ^ 16
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t lo = r[0], hi = r[1];
+    return {__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)};
+}
+__device__ __forceinline__ float four_max(float v) {
+    const f32x2 h = rows16(v);
+    return both_max(__builtin_fmaxf(h.x, h.y));
+}
+__device__ __forceinline__ float four_sum(float v) {
+    const f32x2 h = rows16(v);
+    return both_sum(h.x + h.y);
+}
+
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 mfma16(u32x2 a, u32x2 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+}
+
+template <int D, int QDT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Few<D>::PER_SIMD))) void few_attn_kernel(SharedArgs a) {
+    using KM = KeyMfma<D>;
+    using F = Few<D>;
+    constexpr int T = KM::T, NW = F::WAVES, NT = 64 * NW;
+    constexpr int TILES = D / 16, VW = D / 64;  // tiles of the output; dwords of a token's values a lane
+    __shared__ uint32_t s_row[F::CHUNK];
+    __shared__ uint32_t s_pos[F::CHUNK];
+    __shared__ __align__(16) float s_vs[F::CHUNK];
+    __shared__ __align__(8) uint16_t s_ks[F::CHUNK];
+    __shared__ float s_max[NW], s_m[NW / 2][16], s_l[NW / 2][16];
+    __shared__ f32x4 s_o[NW / 2][TILES][64];
+
+    const int lane = threadIdx.x & 63, n16 = lane & 15, kg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t in_xcd = blockIdx.x >> 3, item = (blockIdx.x & 7u) + 8u * (in_xcd / a.kv_heads), kh = in_xcd % a.kv_heads;
+    if (item >= a.n_items) return;  // whole block
+    const int32_t* const it = a.items + 8 * item;
+    const int32_t* const pages = a.pages + it[0];
+    const uint32_t tok0 = (uint32_t)it[1];
+    const int32_t* const seg_rows = a.seg_rows + 2 * it[3];
+    const int G = (int)(a.q_heads / a.kv_heads), chunk = it[5];
+    // what LDS is sized for, whatever a plan from elsewhere holds
+    const int n_tok = (int)min(max((uint32_t)it[2], 1u), (uint32_t)F::CHUNK);
+    const int n_q = (int)min(max((uint32_t)it[4] * (uint32_t)G, 1u), (uint32_t)F::ROWS);
+    const int n_units = (n_tok + 15) / 16, last = 16 * n_units - 1;
+
+    // ---- queries: B operands of coordinates 16 t + 4 kg + 0..3 of either half ----
+    u32x2 q[2][T];
+    {
+        const uint32_t my_r = (uint32_t)min(n16, n_q - 1), my_br = div(my_r, a.by_group), my_head = kh * G + (my_r - my_br * G);
+        const uint16_t* const p = a.query + ((size_t)(uint32_t)seg_rows[2 * my_br] * a.q_heads + my_head) * D + 4 * kg;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int t = 0; t < T; ++t) q[hf][t] = *reinterpret_cast<const u32x2*>(p + hf * (D / 2) + 16 * t);
+    }
+
+    // ---- the chunk's tokens; places past it repeat its last (with weight 0) ----
+    auto row_of = [&](int i, uint32_t& page, uint32_t& off) {
+        const uint32_t t = tok0 + min(i, n_tok - 1), p = div(t, a.by_tokens);
+        off = t - p * a.tokens;
+        page = (uint32_t)pages[p];
+        return (page * a.kv_heads + kh) * a.tokens + off;
+    };
+    // Key codes a quad per token, 64 consecutive bytes, tables likewise: the operands want lane (token, kg), so the lanes
+    // exchange them when they are used.
+    uint32_t kcode[2][KM::NK][KM::W], vcode[4][VW];
+    constexpr int DEPTH = T <= 4 ? T : 2;  // tiles of the tables on their way (registers)
+    static_assert(T % DEPTH == 0, "a tile keeps its registers from token to token");
+    f32x4 tm[DEPTH], tp[DEPTH];
+    auto load_keys = [&](uint32_t lane, uint32_t row) {  // row: of token lane / 4
+        const int8_t* const p = a.kc + (size_t)row * D + KM::KPL * (lane & 3u);
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int s = 0; s < KM::NK; ++s) {
+                const uint32_t* const w = reinterpret_cast<const uint32_t*>(p + hf * KM::HALF + s * KM::KB);
+#pragma unroll
+                for (int i = 0; i < KM::W; ++i) kcode[hf][s][i] = w[i];
+            }
+    };
+    auto load_table = [&](int t, uint32_t tab) {
+        tm[t % DEPTH] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(a.rope_dm) + (tab + 64u * t));
+        tp[t % DEPTH] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(a.rope_dp) + (tab + 64u * t));
+    };
+    auto load_values = [&](uint32_t n16, int i, uint32_t row) {  // row: of token 4 kg + i
+        const uint32_t* const w = reinterpret_cast<const uint32_t*>(a.vc + (size_t)row * D + (D / 16) * n16);
+#pragma unroll
+        for (int k = 0; k < VW; ++k) vcode[i][k] = w[k];
+    };
+    {
+        uint32_t page, off;
+        load_keys(lane, row_of(16 * wave + (lane >> 2), page, off));
+    }
+    float vmax = 0.0f;
+    for (int i = threadIdx.x; i <= last; i += NT) {
+        uint32_t page, off;
+        const uint32_t row = row_of(i, page, off);
+        const int32_t pos = a.positions[page * a.tokens + off];
+        const float vs = i < n_tok ? f16_bits_to_f32(a.vs[row]) : 0.0f;
+        s_row[i] = row;
+        s_pos[i] = (pos < 0 ? 0u : ((uint32_t)pos >= a.rope_n_pos ? a.rope_n_pos - 1u : (uint32_t)pos)) * (2u * D);
+        s_ks[i] = a.ks[row];
+        s_vs[i] = vs;
+        vmax = __builtin_fmaxf(vmax, __builtin_fabsf(vs));
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) vmax = __builtin_fmaxf(vmax, __shfl_xor(vmax, o, 64));
+    if (lane == 0) s_max[wave] = vmax;
+    float c = a.c * (0.5f * a.hscale);
+    if constexpr (QDT == NQ_BF16) c *= bf16_queries(q, [](float v) { return four_max(v); });
+    KM signs;
+    signs.init(lane);
+    __syncthreads();
+    const int vexp = value_exponent<NW>(s_max);  // used with the weights, not in place: no second pass over s_vs
+
+    uint32_t tab;
+    {
+        const int first = min(16 * wave, last - 15);
+        tab = s_pos[first + (lane >> 2)] + 16u * (lane & 3);
+#pragma unroll
+        for (int t = 0; t < DEPTH; ++t) load_table(t, tab);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_values(n16, i, s_row[first + 4 * kg + i]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+
+    f32x4 o[TILES];
+#pragma unroll
+    for (int j = 0; j < TILES; ++j) o[j] = f32x4{};
+    float m = kNoMax, l = 0.0f;
+    const float vmul = __builtin_ldexpf(1.0f, vexp);
+#pragma unroll 1
+    for (int u = wave; u < n_units; u += NW) {
+        // what follows from the lane alone is worked out again each time, as in decode
+        uint32_t lane = threadIdx.x;
+        asm volatile("" : "+v"(lane));
+        lane &= 63u;
+        const uint32_t n16 = lane & 15u, kg = lane >> 4;
+        const int from_quad = (int)(4 * (4 * n16 + kg));  // byte address of the lane that loaded this lane's block
+        KM km = signs;
+#pragma unroll
+        for (int w = 0; w < KM::W; ++w) asm volatile("" : "+v"(km.h[w]));
+        const int next = 16 * min(u + NW, n_units - 1);
+        uint32_t code[2][KM::NK][KM::W];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int s = 0; s < KM::NK; ++s)
+#pragma unroll
+                for (int i = 0; i < KM::W; ++i) code[hf][s][i] = (uint32_t)__builtin_amdgcn_ds_bpermute(from_quad, (int)kcode[hf][s][i]);
+        load_keys(lane, s_row[next + (lane >> 2)]);
+        const uint32_t next_tab = s_pos[next + (lane >> 2)] + 16u * (lane & 3u);
+        __builtin_amdgcn_sched_barrier(0);
+        f32x4 s = {};
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            f32x4 dm, dp;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = tm[t % DEPTH][i], y = tp[t % DEPTH][i];  // (an element is taken out before it is cast)
+                dm[i] = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(from_quad, __builtin_bit_cast(int, x)));
+                dp[i] = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(from_quad, __builtin_bit_cast(int, y)));
+            }
+            if (t + DEPTH < T) load_table(t + DEPTH, tab);
+            else load_table(t + DEPTH - T, next_tab);
+            int4v y0 = {0, 0, 0, 0}, y1 = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < KM::NK; ++k) {
+                y0 = km.mul(t, k, lane, code[0][k], y0);
+                y1 = km.mul(t, k, lane, code[1][k], y1);
+            }
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float lo = (float)y0[i], hi = (float)y1[i];
+                x[i] = __builtin_fmaf(-lo, dm[i], hi * dp[i]);
+                x[4 + i] = __builtin_fmaf(lo, dp[i], hi * dm[i]);
+            }
+            s = mfma16(u32x2{pack2<NQ_F16>(x[0], x[1]), pack2<NQ_F16>(x[2], x[3])}, q[0][t], s);
+            s = mfma16(u32x2{pack2<NQ_F16>(x[4], x[5]), pack2<NQ_F16>(x[6], x[7])}, q[1][t], s);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        tab = next_tab;
+        // ---- weights ----
+        const int at = 16 * u + 4 * (int)kg, left = n_tok - at;
+        const u32x2 kw = *reinterpret_cast<const u32x2*>(s_ks + at);
+        const f32x4 vs = *reinterpret_cast<const f32x4*>(s_vs + at);
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = s[i] * f16_bits_to_f32((i & 1) ? kw[i / 2] >> 16 : kw[i / 2] & 0xffffu);
+            s[i] = i < left ? x * c : -__builtin_inff();
+            mx = __builtin_fmaxf(mx, s[i]);
+        }
+        if (__any(mx > m + kSlack)) {
+            const float to = __builtin_fmaxf(m, four_max(mx));
+            const float f = __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            l *= f;
+#pragma unroll
+            for (int j = 0; j < TILES; ++j) o[j] *= f;
+        }
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(s[i] - m);
+            l += p[i];
+            p[i] *= vs[i] * vmul;
+        }
+        const u32x2 w = {pack2<NQ_F16>(p[0], p[1]), pack2<NQ_F16>(p[2], p[3])};
+        // ---- values: bytes to fp16 as codes_to_f16, four tokens of a coordinate together ----
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+            uint32_t x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = vcode[i][k] ^ 0x80808080u;
+            const uint32_t pairs[2][2] = {{__builtin_amdgcn_perm(x[1], x[0], 0x05010400u), __builtin_amdgcn_perm(x[3], x[2], 0x05010400u)},
+                                          {__builtin_amdgcn_perm(x[1], x[0], 0x07030602u), __builtin_amdgcn_perm(x[3], x[2], 0x07030602u)}};
+            const half2v bias = {(__fp16)-1152.0f, (__fp16)-1152.0f};
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const uint32_t sel = (b & 1) ? 0x00070006u : 0x00050004u;
+                const half2v v0 = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(pairs[b / 2][0], 0x64646464u, sel)) + bias;
+                const half2v v1 = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(pairs[b / 2][1], 0x64646464u, sel)) + bias;
+                o[4 * k + b] = mfma16(u32x2{__builtin_bit_cast(uint32_t, v0), __builtin_bit_cast(uint32_t, v1)}, w, o[4 * k + b]);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_values(n16, i, s_row[next + 4 * kg + i]);
+    }
+
+    // ---- the waves' sums joined: the upper half's into the lower half's, twice ----
+    uint32_t end_lane = threadIdx.x;  // as in the loop: nothing of the lane is kept over it
+    asm volatile("" : "+v"(end_lane));
+    const int lane2 = end_lane & 63, n = lane2 & 15, g = lane2 >> 4;
+    l = four_sum(l);
+#pragma unroll
+    for (int step = NW / 2; step >= 1; step >>= 1) {
+        if (wave >= step && wave < 2 * step) {
+#pragma unroll
+            for (int j = 0; j < TILES; ++j) s_o[wave - step][j][lane2] = o[j];
+            if (g == 0) {
+                s_m[wave - step][n] = m;
+                s_l[wave - step][n] = l;
+            }
+        }
+        __syncthreads();
+        if (wave < step) {
+            const float mo = s_m[wave][n], to = __builtin_fmaxf(m, mo);
+            const float f = __builtin_amdgcn_exp2f(m - to), fo = __builtin_amdgcn_exp2f(mo - to);
+            m = to;
+            l = l * f + s_l[wave][n] * fo;
+#pragma unroll
+            for (int j = 0; j < TILES; ++j) {
+                const f32x4 y = s_o[wave][j][lane2];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[j][i] = __builtin_fmaf(y[i], fo, o[j][i] * f);
+            }
+        }
+        __syncthreads();
+    }
+    if (wave > 0 || n >= n_q) return;
+    const uint32_t my_br = div((uint32_t)n, a.by_group), my_head = kh * G + ((uint32_t)n - my_br * G);
+    const size_t slot = (size_t)(uint32_t)(seg_rows[2 * my_br + 1] + chunk) * a.q_heads + my_head;
+    if (g == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * slot) = f32x2{m, l};
+    const float f = __builtin_ldexpf(0.5f, -vexp);
+    float* const y = a.part_y + slot * D + (D / 16) * 4 * g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < VW; ++k)
+            *reinterpret_cast<f32x4*>(y + (D / 16) * i + 4 * k) = f32x4{o[4 * k][i] * f, o[4 * k + 1][i] * f, o[4 * k + 2][i] * f, o[4 * k + 3][i] * f};
 }
 
 // One (row, query head) a workgroup: its chunks' sums weighted and added in a fixed order, then the
@@ -452,48 +763,42 @@ __global__ __launch_bounds__(256) void shared_combine_kernel(SharedArgs a) {
     static_cast<uint16_t*>(a.out)[(size_t)blockIdx.x * D + tid] = (uint16_t)(pack2<QDT>(v, 0.0f) & 0xffffu);
 }
 
-// items: those of segments of many query rows first, then the others
+// items: those of segments of many query rows first, those of few last
 template <int D, int QDT>
-static hipError_t launch_shared(SharedArgs a, uint32_t n_many, uint32_t n_items, uint32_t batch, hipStream_t s) {
-    const int32_t* const items = a.items;
-    if (n_many > 0) {
-        a.n_items = n_many;
-        hipLaunchKernelGGL((shared_attn_kernel<D, QDT, true>), dim3((n_many + 7u) / 8u * 8u * a.kv_heads),
-                           dim3(Shape<D, true>::THREADS), 0, s, a);
+static hipError_t launch_shared(SharedArgs a, const uint32_t (&n)[3], uint32_t batch, hipStream_t s) {
+    for (int k = 0; k < 3; ++k) {
+        if (n[k] == 0) continue;
+        a.n_items = n[k];
+        const dim3 grid((n[k] + 7u) / 8u * 8u * a.kv_heads);
+        if (k == 0) hipLaunchKernelGGL((shared_attn_kernel<D, QDT, true>), grid, dim3(Shape<D, true>::THREADS), 0, s, a);
+        else if (k == 1) hipLaunchKernelGGL((shared_attn_kernel<D, QDT, false>), grid, dim3(Shape<D, false>::THREADS), 0, s, a);
+        else hipLaunchKernelGGL((few_attn_kernel<D, QDT>), grid, dim3(64 * Few<D>::WAVES), 0, s, a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-    }
-    if (n_items > n_many) {
-        a.items = items + 8 * (size_t)n_many;
-        a.n_items = n_items - n_many;
-        hipLaunchKernelGGL((shared_attn_kernel<D, QDT, false>), dim3((a.n_items + 7u) / 8u * 8u * a.kv_heads),
-                           dim3(Shape<D, false>::THREADS), 0, s, a);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
+        a.items += 8 * (size_t)n[k];
     }
     hipLaunchKernelGGL((shared_combine_kernel<D, QDT>), dim3(batch * a.q_heads), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
 template <int QDT>
-static hipError_t shared_dims(int32_t d, const SharedArgs& a, uint32_t n_many, uint32_t n_items, uint32_t batch, hipStream_t s) {
+static hipError_t shared_dims(int32_t d, const SharedArgs& a, const uint32_t (&n)[3], uint32_t batch, hipStream_t s) {
     switch (d) {
-        case 64: return launch_shared<64, QDT>(a, n_many, n_items, batch, s);
-        case 128: return launch_shared<128, QDT>(a, n_many, n_items, batch, s);
-        default: return launch_shared<256, QDT>(a, n_many, n_items, batch, s);
+        case 64: return launch_shared<64, QDT>(a, n, batch, s);
+        case 128: return launch_shared<128, QDT>(a, n, batch, s);
+        default: return launch_shared<256, QDT>(a, n, batch, s);
     }
 }
 
 }  // namespace nq
 
-extern "C" int32_t nq_shared_attention_chunk_tokens(int32_t many) {
-    return many ? nq::Shape<128, true>::CHUNK : nq::Shape<128, false>::CHUNK;
+extern "C" int32_t nq_shared_attention_chunk_tokens(int32_t kind) {
+    return kind == 0 ? nq::Shape<128, true>::CHUNK : kind == 1 ? nq::Shape<128, false>::CHUNK : nq::Few<128>::CHUNK;
 }
-extern "C" int32_t nq_shared_attention_rows(int32_t head_dim) {
-    return head_dim <= 128 ? nq::Shape<128, true>::ROWS : nq::Shape<256, true>::ROWS;
+extern "C" int32_t nq_shared_attention_rows(int32_t head_dim, int32_t kind) {
+    if (kind == 0) return head_dim <= 128 ? nq::Shape<128, true>::ROWS : nq::Shape<256, true>::ROWS;
+    return kind == 1 ? nq::Shape<128, false>::ROWS : nq::Few<128>::ROWS;
 }
-
-extern "C" int32_t nq_shared_attention_few_rows(void) { return nq::Shape<128, false>::ROWS; }
 
 extern "C" int64_t nq_shared_attention_workspace(int32_t n_slots, int32_t q_heads, int32_t head_dim) {
     if (n_slots <= 0 || q_heads <= 0 || head_dim <= 0) return 0;
@@ -512,14 +817,16 @@ extern "C" int nq_shared_attention(const nq_shared_desc* d, void* stream) {
                  "nq_shared_attention: a layer must have less than 2^31 token rows");
     NQ_CHECK_ARG(d->q_dtype == NQ_F16 || d->q_dtype == NQ_BF16, "nq_shared_attention: queries must be fp16 or bf16");
     NQ_CHECK_ARG(d->batch >= 0 && d->q_heads > 0 && d->q_heads % p->heads == 0 &&
-                     d->q_heads / p->heads <= nq_shared_attention_rows(p->head_dim),
+                     d->q_heads / p->heads <= nq_shared_attention_rows(p->head_dim, 0),
                  "nq_shared_attention: q_heads %d must be a multiple of the pool's %d heads, at most %d times", d->q_heads,
-                 p->heads, nq_shared_attention_rows(p->head_dim));
-    NQ_CHECK_ARG(d->n_items >= 0 && d->n_slots >= 0 && d->n_many >= 0 && d->n_many <= d->n_items,
-                 "nq_shared_attention: n_items %d, n_many %d, n_slots %d", d->n_items, d->n_many, d->n_slots);
-    NQ_CHECK_ARG(d->n_many == d->n_items || d->q_heads / p->heads <= nq_shared_attention_few_rows(),
-                 "nq_shared_attention: over %d query heads per kv head, every item belongs to the n_many of many rows",
-                 nq_shared_attention_few_rows());
+                 p->heads, nq_shared_attention_rows(p->head_dim, 0));
+    NQ_CHECK_ARG(d->n_items >= 0 && d->n_slots >= 0 && d->n_many >= 0 && d->n_few >= 0 &&
+                     (int64_t)d->n_many + d->n_few <= d->n_items,
+                 "nq_shared_attention: n_items %d, n_many %d, n_few %d, n_slots %d", d->n_items, d->n_many, d->n_few, d->n_slots);
+    for (int k = 1; k < 3; ++k)
+        NQ_CHECK_ARG((k == 1 ? d->n_items - d->n_many - d->n_few : d->n_few) == 0 ||
+                         d->q_heads / p->heads <= nq_shared_attention_rows(p->head_dim, k),
+                     "nq_shared_attention: %d query heads per kv head are too many for items of kind %d", d->q_heads / p->heads, k);
     if (d->batch == 0) return NQ_OK;
     NQ_CHECK_ARG(d->query && d->out && d->row_slots, "nq_shared_attention: query, out and row_slots are required");
     NQ_CHECK_ARG(((uintptr_t)d->query & 15u) == 0, "nq_shared_attention: query must be 16-byte aligned");
@@ -567,7 +874,8 @@ extern "C" int nq_shared_attention(const nq_shared_desc* d, void* stream) {
     a.c = 1.44269504088896340736f / (d->scale_divisor > 0.0f ? d->scale_divisor : 1.0f);
     a.hscale = d->hadamard_scale;
     hipStream_t s = (hipStream_t)stream;
-    NQ_CHECK_HIP(d->q_dtype == NQ_F16 ? shared_dims<NQ_F16>(p->head_dim, a, (uint32_t)d->n_many, (uint32_t)d->n_items, (uint32_t)d->batch, s)
-                                      : shared_dims<NQ_BF16>(p->head_dim, a, (uint32_t)d->n_many, (uint32_t)d->n_items, (uint32_t)d->batch, s));
+    const uint32_t n[3] = {(uint32_t)d->n_many, (uint32_t)(d->n_items - d->n_many - d->n_few), (uint32_t)d->n_few};
+    NQ_CHECK_HIP(d->q_dtype == NQ_F16 ? shared_dims<NQ_F16>(p->head_dim, a, n, (uint32_t)d->batch, s)
+                                      : shared_dims<NQ_BF16>(p->head_dim, a, n, (uint32_t)d->batch, s));
     return NQ_OK;
 }

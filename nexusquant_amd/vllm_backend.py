@@ -462,21 +462,20 @@ class PagedAttentionPlan:
     tokens: int                        # tokens attended over all rows
 
 
-# What pays to share: a segment of _MIN_TOKENS tokens whose sharing saves _MIN_SAVED tokens' decoding (its tokens,
-# once for every row but one).  8 kv heads x 4, us shared and apart: 32 rows x 128 tokens 17.4 and 15.6, x 256
-# 17.3 and 20.4, x 1024 19.0 and 35.0; 8 rows x 256 14.3 and 14.5, x 1024 14.4 and 19.2; 2 rows x 2048 15.9 and 15.5.
-_MIN_TOKENS = 256
-_MIN_SAVED = 2048
+# What pays to share: sharing that saves this many tokens' decoding, counted in every kv head (a segment's tokens, once
+# for every row but one).  us shared and apart: 8 kv heads x 4, 32 rows x 256 tokens 18.7 and 15.8, x 512 18.0 and
+# 19.2, 8 rows x 1024 15.3 and 15.5, x 2048 15.9 and 18.4; 32 x 1, 16 rows x 128 15.6 and 15.9, x 256 15.7 and 20.5.
+_MIN_SAVED = 1 << 16
 
 
 def shared_segments(tables: Sequence[np.ndarray], lengths: Sequence[int], page_tokens: int,
-                    min_saved: Optional[int] = None) -> List[Tuple[List[int], np.ndarray, int]]:
+                    min_saved: int) -> List[Tuple[List[int], np.ndarray, int]]:
     """Cut the rows' tokens into segments (rows, pages, tokens) that their rows see whole.
 
     tables[b]: row b's pages, lengths[b]: its tokens.  Rows that begin with the same full pages
     share a segment of these, and those among them that go on alike another one, and so on; a
     segment of one row is what it has for itself.  Sharing that would save less than min_saved
-    tokens (None: that does not pay) is left to what follows it."""
+    tokens is left to what follows it."""
     full = [int(n) // page_tokens for n in lengths]
     out: List[Tuple[List[int], np.ndarray, int]] = []
 
@@ -500,8 +499,7 @@ def shared_segments(tables: Sequence[np.ndarray], lengths: Sequence[int], page_t
             differ = np.flatnonzero((stack != stack[0]).any(axis=0))
             end = depth + int(differ[0]) if len(differ) else most
             tokens = (end - start) * page_tokens
-            saved = (len(same) - 1) * tokens
-            if saved >= min_saved if min_saved is not None else saved >= _MIN_SAVED and tokens >= _MIN_TOKENS:
+            if (len(same) - 1) * tokens >= min_saved:
                 out.append((same, tables[same[0]][start:end], tokens))
                 todo.append((same, end, end))
             else:
@@ -509,44 +507,56 @@ def shared_segments(tables: Sequence[np.ndarray], lengths: Sequence[int], page_t
     return out
 
 
-_SHARED_STAGE = 128
-# Segments of more query rows than _MANY_ROWS go to the wide workgroups when there are at least
-# _MANY_TOKENS tokens for each of 256 CUs (the small shape takes up to nq_shared_attention_few_rows()):
-# 8 kv heads, 128 query rows, us wide and small: 4096 tokens 24.8 and 25.5, where the rows' own tokens need
-# the small shape's launch anyway; 16384 tokens 35.0 and 38.9.
+# Tokens that a workgroup takes at a time, by kind, and the least of a chunk: 4 rows of 4 heads over 992 tokens in
+# chunks of 64 11.2 us, of 128 11.8.
+_SHARED_STAGE = (128, 128, 64)
+_SHARED_LEAST = (256, 128, 64)
+# The kinds of segments, by query rows (batch rows x query heads of a kv head): many (wide workgroups), some, few.
+# Few are up to nq_shared_attention_rows(d, 2) of them: 8 kv heads x 128, us few and some: 64 rows x 8 heads over 512
+# own tokens 28.8 and 35.8, 3 x 8 over 9184 at head_dim 256 40.6 and 71, 8 x 1 over 8192 at 64 18.8 and 22.9.
+# Segments of more than _MANY_ROWS count as many when there are at least _MANY_TOKENS tokens for each of 256 CUs
+# (some are up to nq_shared_attention_rows(d, 1)): 8 kv heads, 128 query rows, us many and some: 4096 tokens 24.8 and
+# 25.5, 16384 tokens 35.0 and 38.9.
+_MANY, _SOME, _FEW = 0, 1, 2
 _MANY_ROWS = 32
 _MANY_TOKENS = 512
+# Few go along with some, where there are any, unless they have _FEW_TOKENS tokens for each CU: a launch less.  32 rows
+# of 4 heads over a shared 4096 tokens and 256 own ones: 26 us, with a launch for the own ones 36.
+_FEW_TOKENS = 1024
 
 
-def _shared_chunk(lengths, tiles, kv_heads: int, cap: int, least: int, workgroups: int) -> int:
-    """Chunk length of segments: the least multiple of a stage with which the launch is one round of
+def _shared_chunk(lengths, tiles, kv_heads: int, cap: int, least: int, stage: int, workgroups: int) -> int:
+    """Chunk length of segments: the least multiple of `stage` with which the launch is one round of
     `workgroups`.  16 rows x 4 heads over 8192 tokens, us: 512 workgroups 32.3, 256 (chunks of 256) 23.4,
-    128 27.3; 64 rows' own 512 tokens: 512 workgroups 37.3, 1024 41.9, 2048 50.3."""
+    128 27.3; 64 rows' own 512 tokens: 512 workgroups 28.8, 1024 31.9."""
     length = min(least, cap)
     while length < cap and kv_heads * sum(t * -(-n // length) for t, n in zip(tiles, lengths)) > workgroups:
-        length += _SHARED_STAGE
+        length += stage
     return length
 
 
-def shared_items(segments, batch: int, group: int, kv_heads: int, head_dim: int, cap: Dict[bool, int],
-                 rows: Dict[bool, int]):
+def shared_items(segments, batch: int, group: int, kv_heads: int, head_dim: int, cap: Sequence[int],
+                 rows: Sequence[int]):
     """The work list of nq_shared_attention: int32 arrays items, pages, seg_rows, row_slots, and the counts of
-    items, of those among them that come first (for the wide workgroups) and of slots.  cap, rows: most tokens
-    of a chunk and most query rows of a workgroup, wide (True) and small."""
-    wide = [len(r) * group > _MANY_ROWS for r, _, _ in segments]
-    work = kv_heads * sum(n * -(-len(r) * group // rows[True]) for (r, _, n), w in zip(segments, wide) if w)
+    items, of those of segments of many rows (they come first), of few (last) and of slots.  cap, rows: most
+    tokens of a chunk and most query rows of a workgroup, by kind."""
+    queries = [len(r) * group for r, _, _ in segments]
+    kind = [_FEW if q <= rows[_FEW] else _MANY if q > _MANY_ROWS else _SOME for q in queries]
+    work = kv_heads * sum(s[2] * -(-q // rows[_MANY]) for s, q, k in zip(segments, queries, kind) if k == _MANY)
     if work < 256 * _MANY_TOKENS:
-        wide = [len(r) * group > rows[False] for r, _, _ in segments]
-    per_tile = {k: max(1, rows[k] // group) for k in rows}  # batch rows of a workgroup
-    tiles = [-(-len(r) // per_tile[w]) for (r, _, _), w in zip(segments, wide)]
-    step = {}
-    for k in (True, False):
-        of = [i for i in range(len(segments)) if wide[i] == k]
-        # as many workgroups as run at once: LDS leaves one of the wide ones on a CU, of the small 3, 2 or 1
-        slots = 256 if k else 256 * {64: 3, 128: 2}.get(head_dim, 1)
-        step[k] = _shared_chunk([segments[i][2] for i in of], [tiles[i] for i in of], kv_heads, cap[k],
-                                (2 if k else 1) * _SHARED_STAGE, slots)
-    chunks = [-(-s[2] // step[w]) for s, w in zip(segments, wide)]
+        kind = [_SOME if k == _MANY and q <= rows[_SOME] else k for k, q in zip(kind, queries)]
+    if _SOME in kind and kv_heads * sum(s[2] for s, k in zip(segments, kind) if k == _FEW) < 256 * _FEW_TOKENS:
+        kind = [_SOME if k == _FEW else k for k in kind]
+    per_tile = [max(1, n // group) for n in rows]  # batch rows of a workgroup
+    tiles = [-(-len(s[0]) // per_tile[k]) for s, k in zip(segments, kind)]
+    # as many workgroups as run at once: LDS leaves one of the wide ones on a CU, LDS or registers those of the others
+    at_once = (1, {64: 3, 128: 2}.get(head_dim, 1), {64: 4, 128: 3}.get(head_dim, 2))
+    step = []
+    for k in (_MANY, _SOME, _FEW):
+        of = [i for i in range(len(segments)) if kind[i] == k]
+        step.append(_shared_chunk([segments[i][2] for i in of], [tiles[i] for i in of], kv_heads, cap[k],
+                                  _SHARED_LEAST[k], _SHARED_STAGE[k], 256 * at_once[k]))
+    chunks = [-(-s[2] // step[k]) for s, k in zip(segments, kind)]
     per_row = [0] * (batch + 1)
     for (r, _, _), c in zip(segments, chunks):
         for b in r:
@@ -555,15 +565,15 @@ def shared_items(segments, batch: int, group: int, kv_heads: int, head_dim: int,
     nxt = row_slots[:-1].tolist()
     records, seg_rows, pages = [], [], []
     at_pages = 0
-    # the wide ones first, long ones before short ones
-    for i in sorted(range(len(segments)), key=lambda i: (not wide[i], -segments[i][2])):
+    # by kind, long ones before short ones
+    for i in sorted(range(len(segments)), key=lambda i: (kind[i], -segments[i][2])):
         r, seg_pages, n = segments[i]
         at_rows = len(seg_rows)
         for b in r:
             seg_rows.append((b, nxt[b]))
             nxt[b] += chunks[i]
         # chunks in eights (one for each XCD), a chunk's row tiles one eight after another
-        length, per = step[wide[i]], per_tile[wide[i]]
+        length, per = step[kind[i]], per_tile[kind[i]]
         for c0 in range(0, chunks[i], 8):
             for r0 in range(0, len(r), per):
                 for c in range(c0, min(c0 + 8, chunks[i])):
@@ -571,11 +581,11 @@ def shared_items(segments, batch: int, group: int, kv_heads: int, head_dim: int,
                                     min(len(r) - r0, per), c, 0, 0))
         pages.append(np.asarray(seg_pages, dtype=np.int32))
         at_pages += len(seg_pages)
-    n_wide = sum(t * c for t, c, w in zip(tiles, chunks, wide) if w)
+    n_kind = [sum(t * c for t, c, x in zip(tiles, chunks, kind) if x == k) for k in (_MANY, _FEW)]
     parts = {"items": np.array(records, dtype=np.int32).reshape(-1),
              "pages": np.concatenate(pages) if pages else np.zeros(0, dtype=np.int32),
              "seg_rows": np.array(seg_rows, dtype=np.int32).reshape(-1), "row_slots": row_slots.astype(np.int32)}
-    return parts, len(records), n_wide, int(row_slots[-1])
+    return parts, len(records), n_kind[0], n_kind[1], int(row_slots[-1])
 
 
 # nq_shared_desc, packed in one go
@@ -595,7 +605,7 @@ class SharedAttentionPlan:
         self._tables: list = []  # rotation tables that calls with this plan have read: a captured graph goes on reading them
 
     def work(self, q_heads: int):
-        """(device ints, offsets, items, items of many rows, slots) for q_heads query heads."""
+        """(device ints, offsets, items, items of many rows, of few, slots) for q_heads query heads."""
         got = self._work.get(q_heads)
         if got is None:
             if torch.cuda.is_current_stream_capturing():
@@ -604,9 +614,8 @@ class SharedAttentionPlan:
             heads = self.pool.num_heads
             parts, *counts = shared_items(
                 self.segments, self.batch, q_heads // heads, heads, self.pool.head_dim,
-                {k: int(lib.nq_shared_attention_chunk_tokens(k)) for k in (True, False)},
-                {True: int(lib.nq_shared_attention_rows(self.pool.head_dim)),
-                 False: int(lib.nq_shared_attention_few_rows())})
+                [int(lib.nq_shared_attention_chunk_tokens(k)) for k in range(3)],
+                [int(lib.nq_shared_attention_rows(self.pool.head_dim, k)) for k in range(3)])
             offsets, at = {}, 0
             for name, v in parts.items():
                 offsets[name] = at  # bytes
@@ -779,8 +788,8 @@ class NexusQuantPagedAttention:
                     min_saved: Optional[int] = None) -> SharedAttentionPlan:
         """The plan of rows over a CompressedPagePool: row b attends to the first context_lens[b] tokens of
         its pages block_tables[b] (0: none; entries past those tokens are padding).  Full pages that several rows begin with, as forks do, are
-        read and decoded once for all of them, where that saves min_saved tokens' decoding (None: where it
-        pays; see shared_segments)."""
+        read and decoded once for all of them, where that saves min_saved tokens' decoding (None: what pays,
+        65536 over the pool's heads)."""
         if pool.head_dim != self.compressor.head_dim:
             raise ValueError(f"pool head_dim {pool.head_dim} != compressor head_dim {self.compressor.head_dim}")
         ctx = [int(x) for x in (context_lens.tolist() if torch.is_tensor(context_lens) else context_lens)]
@@ -792,6 +801,8 @@ class NexusQuantPagedAttention:
             if not 0 <= n <= len(table) * pool.page_tokens:
                 raise ValueError(f"row {b}: {n} tokens in {len(table)} pages of {pool.page_tokens}")
             tables.append(pool.in_use(table[:pool.pages_for(n)], "plan_shared"))  # what follows is padding
+        if min_saved is None:
+            min_saved = -(-_MIN_SAVED // pool.num_heads)
         return SharedAttentionPlan(pool, len(ctx), shared_segments(tables, ctx, pool.page_tokens, min_saved))
 
     def _shared_tables(self, max_position: int, dev):
@@ -827,7 +838,7 @@ class NexusQuantPagedAttention:
         if query.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("run_shared has no backward pass; call it under torch.no_grad()")
         b, hq, d = shape
-        rows = int(lib.nq_shared_attention_rows(d))
+        rows = int(lib.nq_shared_attention_rows(d, _MANY))
         if hq == 0 or hq % pool.num_heads or hq // pool.num_heads > rows:
             raise ValueError(f"num_heads {hq} is not a multiple (up to {rows}) of the pool's {pool.num_heads}")
         if not 0 <= int(layer) < pool.num_layers:
@@ -842,7 +853,7 @@ class NexusQuantPagedAttention:
         if q.data_ptr() % 16:
             q = q.clone()
         with on_device(dev):
-            ints, offsets, n_items, n_many, n_slots = plan.work(hq)
+            ints, offsets, n_items, n_many, n_few, n_slots = plan.work(hq)
             nbytes = lib.nq_shared_attention_workspace(n_slots, hq, d)
             # of this call alone: calls on other streams and captured graphs have their own
             ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
@@ -852,7 +863,7 @@ class NexusQuantPagedAttention:
             dm, dp = tables
             base = ints.address()
             desc = _lib.SharedDesc.from_buffer_copy(_SHARED_PACK.pack(
-                ctypes.addressof(pool.desc), int(layer), b, hq, _lib.dtype_code(dtype), n_items, n_many, n_slots, 0,
+                ctypes.addressof(pool.desc), int(layer), b, hq, _lib.dtype_code(dtype), n_items, n_many, n_few, n_slots,
                 q.data_ptr(), out.data_ptr(), base + offsets["items"], base + offsets["pages"],
                 base + offsets["seg_rows"], base + offsets["row_slots"], dm.data_ptr(), dp.data_ptr(), dm.shape[0],
                 hadamard_constant(d), float(np.float32(math.sqrt(d))), ws.data_ptr(), nbytes))

@@ -63,12 +63,14 @@ def test_what_is_shared_is_in_one_segment():
     assert sorted((rows, n) for rows, _, n in segs) == [([0, 1], 496), ([2, 3], 496)]
 
 
-@pytest.mark.parametrize("rows,tokens,pays", [(32, 128, False), (32, 256, True), (9, 256, True), (8, 256, False),
-                                              (2, 2048, True), (2, 2032, False)])
-def test_what_pays_is_shared(rows, tokens, pays):
-    table = np.arange(tokens // 16)
-    segs = shared_segments([table] * rows, [tokens] * rows, 16)
-    assert len(segs) == (1 if pays else rows)
+@pytest.mark.parametrize("heads,rows,tokens,pays", [(8, 32, 256, False), (8, 32, 272, True), (8, 9, 1024, True),
+                                                    (8, 9, 1008, False), (16, 2, 4096, True), (16, 2, 4080, False)])
+def test_what_pays_is_shared(monkeypatch, heads, rows, tokens, pays):
+    pool = host_pool(monkeypatch, layers=1, pages=tokens // 16, heads=heads, tokens=16)
+    table = pool.allocate(tokens // 16)
+    attn = NexusQuantPagedAttention(NexusQuantKVCompressor(head_dim=64))
+    assert len(attn.plan_shared(pool, [table] * rows, [tokens] * rows).segments) == (1 if pays else rows)
+    assert len(attn.plan_shared(pool, [table] * rows, [tokens] * rows, min_saved=1).segments) == 1
 
 
 def test_rows_that_end_one_after_another_are_cut_without_recursion():
@@ -84,21 +86,21 @@ def test_rows_that_end_one_after_another_are_cut_without_recursion():
 
 
 @pytest.mark.parametrize("group,kv_heads,d,cap,rows", [
-    (1, 8, 128, 1024, (256, 128)), (4, 1, 64, 1024, (256, 128)), (128, 2, 256, 256, (128, 128)),
-    (8, 64, 128, 128, (256, 128)), (2, 3, 128, 1024, (256, 128)), (200, 1, 128, 2048, (256, 128))])
+    (1, 8, 128, 1024, (256, 128, 16)), (4, 1, 64, 1024, (256, 128, 16)), (128, 2, 256, 256, (128, 128, 16)),
+    (8, 64, 128, 128, (256, 128, 16)), (2, 3, 128, 1024, (256, 128, 16)), (200, 1, 128, 2048, (256, 128, 16))])
 def test_items_cover_each_rows_tokens_and_slots_once(group, kv_heads, d, cap, rows):
     r = np.random.RandomState(group)
     batch = 37
     segments = [(list(range(20)), np.arange(300), 4800), ([3, 5, 36], np.arange(400, 410), 160)]
     segments += [([b], np.arange(1000 + 10 * b, 1010 + 10 * b), int(r.randint(1, 160))) for b in range(30)]
-    most = dict(zip((True, False), rows))
-    parts, n_items, n_wide, n_slots = shared_items(segments, batch, group, kv_heads, d, {True: cap, False: cap}, most)
+    parts, n_items, n_many, n_few, n_slots = shared_items(segments, batch, group, kv_heads, d, [cap] * 3, rows)
     items = parts["items"].reshape(-1, 8)
     where = parts["seg_rows"].reshape(-1, 2)
     assert len(items) == n_items and parts["row_slots"][0] == 0 and parts["row_slots"][-1] == n_slots
     seen, slots = {}, []
     for i, (page0, tok0, n, row0, n_rows, chunk, _, _) in enumerate(items):
-        assert 1 <= n <= cap and 1 <= n_rows and n_rows * group <= most[i < n_wide]
+        most = rows[0 if i < n_many else 2 if i >= n_items - n_few else 1]
+        assert 1 <= n <= cap and 1 <= n_rows and n_rows * group <= most
         for b, slot0 in where[row0:row0 + n_rows]:
             slots.append(slot0 + chunk)
             assert parts["row_slots"][b] <= slot0 + chunk < parts["row_slots"][b + 1]
@@ -110,17 +112,17 @@ def test_items_cover_each_rows_tokens_and_slots_once(group, kv_heads, d, cap, ro
     assert len(seen) == sum(len(s[0]) * s[2] for s in segments)
 
 
-@pytest.mark.parametrize("rows,group,tokens,wide", [(16, 8, 16384, True), (16, 8, 4096, False), (4, 8, 60000, False),
-                                                    (32, 8, 128, True), (1, 200, 16, True)])
-def test_which_segments_take_the_wide_workgroups(rows, group, tokens, wide):
+@pytest.mark.parametrize("rows,group,tokens,kind", [(16, 8, 16384, 0), (16, 8, 4096, 1), (4, 8, 60000, 1), (32, 8, 128, 0),
+                                                    (1, 200, 16, 0), (2, 8, 60000, 2), (16, 1, 16, 2), (17, 1, 16, 1)])
+def test_which_kind_a_segment_is(rows, group, tokens, kind):
     segments = [(list(range(rows)), np.arange(tokens // 16), tokens)]
-    _, n_items, n_wide, _ = shared_items(segments, rows, group, 8, 128, {True: 2048, False: 1024}, {True: 256, False: 128})
-    assert n_wide == (n_items if wide else 0)
+    _, n_items, n_many, n_few, _ = shared_items(segments, rows, group, 8, 128, (2048, 1024, 1024), (256, 128, 16))
+    assert (n_many, n_items - n_many - n_few, n_few) == tuple(n_items if k == kind else 0 for k in range(3))
 
 
 def test_no_rows_and_no_tokens():
-    parts, n_items, n_wide, n_slots = shared_items([], 3, 4, 8, 128, {True: 2048, False: 1024}, {True: 256, False: 128})
-    assert n_items == n_wide == n_slots == 0 and list(parts["row_slots"]) == [0, 0, 0, 0]
+    parts, *counts = shared_items([], 3, 4, 8, 128, (2048, 1024, 1024), (256, 128, 16))
+    assert counts == [0, 0, 0, 0] and list(parts["row_slots"]) == [0, 0, 0, 0]
 
 
 def test_plan_refuses_bad_tables(monkeypatch):
@@ -159,6 +161,7 @@ def test_shared_struct_matches_the_c_compiler(tmp_path):
 @pytest.mark.parametrize("kw,pool_kw", [
     (dict(layer=1), {}), (dict(layer=-1), {}), (dict(batch=-1), {}), (dict(q_heads=0), {}), (dict(q_heads=3), {}),
     (dict(q_heads=2 * 257), {}), (dict(q_dtype=_lib.NQ_F32), {}), (dict(n_items=-1), {}), (dict(n_slots=0), {}), (dict(n_many=2), {}), (dict(n_many=-1), {}),
+    (dict(n_few=2), {}), (dict(n_few=-1), {}), (dict(n_few=1, n_many=1), {}), (dict(n_few=1, q_heads=34), {}),
     (dict(query=None), {}), (dict(query=ctypes.c_void_p(4104)), {}), (dict(out=None), {}), (dict(items=None), {}),
     (dict(row_slots=None), {}), (dict(rope_sin_minus_cos=None), {}), (dict(rope_n_pos=0), {}),
     (dict(workspace=None), {}), (dict(workspace_bytes=100), {}), (dict(workspace=ctypes.c_void_p(4100)), {}),
@@ -177,11 +180,12 @@ def test_c_entry_refuses(kw, pool_kw):
     assert lib.nq_shared_attention(ctypes.byref(_lib.SharedDesc(**{**base, "batch": 0})), None) in (0, -1)
 
 
-def test_c_entry_refuses_wide_groups_among_small_items():
-    """A kv head of more query heads than a small workgroup has rows: its items all belong to the wide ones."""
+def test_c_entry_refuses_groups_that_a_kind_does_not_take():
     lib = _lib.load()
     dummy = ctypes.c_void_p(4096)
-    desc = dict(pool=ctypes.pointer(c_pool()), layer=0, batch=1, q_heads=c_pool().heads * 129, q_dtype=_lib.NQ_F16, n_items=2,
-                n_many=1, n_slots=2, query=dummy, out=dummy, items=dummy, pages=dummy, seg_rows=dummy, row_slots=dummy)
-    assert lib.nq_shared_attention(ctypes.byref(_lib.SharedDesc(**desc)), None) == -1
-    assert b"over 128 query heads" in lib.nq_last_error()
+    for n_many, n_few, group in ((1, 0, 129), (0, 2, 17), (1, 1, 17)):
+        desc = dict(pool=ctypes.pointer(c_pool()), layer=0, batch=1, q_heads=c_pool().heads * group, q_dtype=_lib.NQ_F16,
+                    n_items=2, n_many=n_many, n_few=n_few, n_slots=2, query=dummy, out=dummy, items=dummy, pages=dummy,
+                    seg_rows=dummy, row_slots=dummy)
+        assert lib.nq_shared_attention(ctypes.byref(_lib.SharedDesc(**desc)), None) == -1
+        assert b"too many for items of kind" in lib.nq_last_error()
