@@ -165,7 +165,7 @@ SIGNATURES = {
     "nq_nibble_pack": ([_P, _I64, _I32, _P, _P], ctypes.c_int),
     "nq_nibble_unpack": ([_P, _I64, _I32, _I32, _P, _P], ctypes.c_int),
     "nq_prompt_tile_rows": ([], ctypes.c_int32),
-    "nq_prompt_attention": ([ctypes.POINTER(PromptDesc), _P], ctypes.c_int),
+    "nq_prompt_attention": ([_P, _P], ctypes.c_int),
     "nq_pool_copy_pages": ([ctypes.POINTER(Pool), _P, _P, _I32, _P], ctypes.c_int),
     "nq_pool_move_tokens": ([], ctypes.c_int32),
     "nq_pool_host_ints": ([], ctypes.c_int32),
@@ -174,7 +174,7 @@ SIGNATURES = {
     "nq_shared_attention_chunk_tokens": ([_I32], ctypes.c_int32),
     "nq_shared_attention_rows": ([_I32, _I32], ctypes.c_int32),
     "nq_shared_attention_workspace": ([_I32, _I32, _I32], _I64),
-    "nq_shared_attention": ([ctypes.POINTER(SharedDesc), _P], ctypes.c_int),
+    "nq_shared_attention": ([_P, _P], ctypes.c_int),
     "nq_e8_dequant_matmul": ([_P, _P, _P, _P, _I64, _I32, _I32, _I32, _P], ctypes.c_int),
     "nq_e8_nearest_point": ([_P, _P, _I64, _P], ctypes.c_int),
     "nq_e8_quantize_perhead": ([_P, _P, _I64, _I32, _I32, _P], ctypes.c_int),

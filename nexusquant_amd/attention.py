@@ -8,7 +8,6 @@ one after another without padding.
 
 from __future__ import annotations
 
-import ctypes
 import dataclasses
 import struct
 from typing import Optional, Sequence
@@ -68,7 +67,7 @@ def _rows(t: torch.Tensor):
     return t, at, row, head
 
 
-# nq_prompt_desc, packed in one go (a call's host time counts for short prompts)
+# nq_prompt_desc, packed in one go and passed as bytes (a call's host time counts for short prompts)
 _PACK = struct.Struct("6i5P8q2f")
 
 
@@ -129,9 +128,9 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     o_row, o_head, _ = out.stride()
     window = 0 if sliding_window is None or int(sliding_window) >= max(plan.lengths) else int(sliding_window)
     with on_device(dev):
-        desc = _lib.PromptDesc.from_buffer_copy(_PACK.pack(
+        st = lib.nq_prompt_attention(_PACK.pack(
             hq, hkv, d, _lib.NQ_F16 if dtype == torch.float16 else _lib.NQ_BF16, plan.n_tiles, window, q_at, k_at, v_at,
-            out.data_ptr(), plan.tiles.address(), q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, scale, 0.0))
-        st = lib.nq_prompt_attention(ctypes.byref(desc), _lib.current_stream_handle(dev))
+            out.data_ptr(), plan.tiles.address(), q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, scale, 0.0),
+            _lib.current_stream_handle(dev))
     _lib.check(st, "nq_prompt_attention")
     return out

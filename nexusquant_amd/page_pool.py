@@ -121,6 +121,7 @@ class CompressedPagePool:
                                tokens=self.page_tokens, head_dim=self.head_dim, key_codes=_addr(key_codes),
                                value_codes=_addr(value_codes), key_scales=_addr(key_scales),
                                value_scales=_addr(value_scales), positions=_addr(positions))
+        self.desc_at = ctypes.addressof(self.desc)
 
     # ------------------------------------------------------------- page numbers
 

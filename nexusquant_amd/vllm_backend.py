@@ -588,8 +588,16 @@ def shared_items(segments, batch: int, group: int, kv_heads: int, head_dim: int,
     return parts, len(records), n_kind[0], n_kind[1], int(row_slots[-1])
 
 
-# nq_shared_desc, packed in one go
+# nq_shared_desc, packed in one go and passed as bytes
 _SHARED_PACK = struct.Struct("P8i8Pq2fPq")
+
+
+class _SharedTables:
+    """Merged rotation tables, and their addresses and length."""
+
+    def __init__(self, dm: torch.Tensor, dp: torch.Tensor):
+        self.tensors = (dm, dp)
+        self.args = (dm.data_ptr(), dp.data_ptr(), dm.shape[0])
 
 
 class SharedAttentionPlan:
@@ -605,23 +613,27 @@ class SharedAttentionPlan:
         self._tables: list = []  # rotation tables that calls with this plan have read: a captured graph goes on reading them
 
     def work(self, q_heads: int):
-        """(device ints, offsets, items, items of many rows, of few, slots) for q_heads query heads."""
+        """(device ints, what nq_shared_desc holds that all calls share: counts, the arrays' places in the ints, factors
+        and workspace bytes) for q_heads query heads."""
         got = self._work.get(q_heads)
         if got is None:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("run_shared: run the plan once before capturing it into a graph")
+            with on_device(self.pool.device):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("run_shared: run the plan once before capturing it into a graph")
             lib = _lib.load()
-            heads = self.pool.num_heads
-            parts, *counts = shared_items(
-                self.segments, self.batch, q_heads // heads, heads, self.pool.head_dim,
-                [int(lib.nq_shared_attention_chunk_tokens(k)) for k in range(3)],
-                [int(lib.nq_shared_attention_rows(self.pool.head_dim, k)) for k in range(3)])
-            offsets, at = {}, 0
-            for name, v in parts.items():
-                offsets[name] = at  # bytes
+            heads, d = self.pool.num_heads, self.pool.head_dim
+            most = [int(lib.nq_shared_attention_rows(d, k)) for k in range(3)]
+            if q_heads == 0 or q_heads % heads or q_heads // heads > most[_MANY]:
+                raise ValueError(f"num_heads {q_heads} is not a multiple (up to {most[_MANY]}) of the pool's {heads}")
+            parts, *counts = shared_items(self.segments, self.batch, q_heads // heads, heads, d,
+                                          [int(lib.nq_shared_attention_chunk_tokens(k)) for k in range(3)], most)
+            places, at = [], 0
+            for v in parts.values():
+                places.append(at)  # bytes
                 at += 4 * len(v)
             ints = PlanTensor(np.concatenate(list(parts.values())), self.pool.device)
-            got = self._work[q_heads] = (ints, offsets, *counts)
+            got = self._work[q_heads] = (ints, counts, places, (hadamard_constant(d), float(np.float32(math.sqrt(d)))),
+                                         int(lib.nq_shared_attention_workspace(counts[-1], q_heads, d)))
         return got
 
 
@@ -810,7 +822,7 @@ class NexusQuantPagedAttention:
         got = self._tables
         if got is None or got[0] < max_position or got[1] != dev:
             _, _, dm, dp = self.compressor._tables(max_position, dev)
-            got = self._tables = (dm.shape[0] - 1, dev, (dm, dp))
+            got = self._tables = (dm.shape[0] - 1, dev, _SharedTables(dm, dp))
         return got[2]
 
     def run_shared(self, plan: SharedAttentionPlan, query: torch.Tensor, layer: int = 0,
@@ -837,10 +849,8 @@ class NexusQuantPagedAttention:
             raise ValueError(f"run_shared takes fp16 or bf16 queries, got {dtype}; run() takes fp32 ones")
         if query.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("run_shared has no backward pass; call it under torch.no_grad()")
-        b, hq, d = shape
-        rows = int(lib.nq_shared_attention_rows(d, _MANY))
-        if hq == 0 or hq % pool.num_heads or hq // pool.num_heads > rows:
-            raise ValueError(f"num_heads {hq} is not a multiple (up to {rows}) of the pool's {pool.num_heads}")
+        hq = shape[1]
+        ints, counts, places, factors, nbytes = plan._work.get(hq) or plan.work(hq)
         if not 0 <= int(layer) < pool.num_layers:
             raise ValueError(f"layer {layer} of a pool of {pool.num_layers}")
         if pool.head_dim != self.compressor.head_dim:
@@ -852,22 +862,19 @@ class NexusQuantPagedAttention:
         q = query.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()
+        # of this call alone: calls on other streams and captured graphs have their own
+        ws = torch.empty(nbytes or 16, dtype=torch.uint8, device=dev)
+        tables = self._shared_tables(pool.max_position, dev)
+        if not plan._tables or plan._tables[-1] is not tables:
+            plan._tables.append(tables)
+        dm, dp, n_pos = tables.args
+        items, pages, seg_rows, row_slots = places
         with on_device(dev):
-            ints, offsets, n_items, n_many, n_few, n_slots = plan.work(hq)
-            nbytes = lib.nq_shared_attention_workspace(n_slots, hq, d)
-            # of this call alone: calls on other streams and captured graphs have their own
-            ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-            tables = self._shared_tables(pool.max_position, dev)
-            if not plan._tables or plan._tables[-1] is not tables:
-                plan._tables.append(tables)
-            dm, dp = tables
             base = ints.address()
-            desc = _lib.SharedDesc.from_buffer_copy(_SHARED_PACK.pack(
-                ctypes.addressof(pool.desc), int(layer), b, hq, _lib.dtype_code(dtype), n_items, n_many, n_few, n_slots,
-                q.data_ptr(), out.data_ptr(), base + offsets["items"], base + offsets["pages"],
-                base + offsets["seg_rows"], base + offsets["row_slots"], dm.data_ptr(), dp.data_ptr(), dm.shape[0],
-                hadamard_constant(d), float(np.float32(math.sqrt(d))), ws.data_ptr(), nbytes))
-            st = lib.nq_shared_attention(ctypes.byref(desc), _lib.current_stream_handle(dev))
+            st = lib.nq_shared_attention(_SHARED_PACK.pack(
+                pool.desc_at, int(layer), shape[0], hq, _lib.NQ_F16 if dtype == torch.float16 else _lib.NQ_BF16, *counts,
+                q.data_ptr(), out.data_ptr(), base + items, base + pages, base + seg_rows, base + row_slots, dm, dp, n_pos,
+                *factors, ws.data_ptr(), nbytes), _lib.current_stream_handle(dev))
         _lib.check(st, "nq_shared_attention")
         return out
 

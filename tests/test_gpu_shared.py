@@ -356,4 +356,4 @@ def test_wide_workgroups(heads, group, d, rows, prefix):
     pool = make_pool(1, prefix // 16 + 2 + 8 * rows, heads, 16, d, seed=rows)
     tables, ctx = forks(pool, prefix, [7 * i % 90 for i in range(rows)])
     plan, _ = check(attention(d), pool, tables, ctx, queries(rows, heads * group, d, torch.float16, seed=rows))
-    assert plan.work(heads * group)[3] > 0
+    assert plan.work(heads * group)[1][1] > 0  # items of many rows
