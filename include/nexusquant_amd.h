@@ -678,7 +678,9 @@ int nq_pool_write(const nq_pool* pool, int32_t layer, const nq_pool* tokens, con
  *              [3] where its rows start in `seg_rows` (entries)
  *              [4] rows; times q_heads / heads at most
  *                  nq_shared_attention_rows(head_dim, kind)
- *              [5] the chunk's number in its segment;  [6..7] unused
+ *              [5] the chunk's number in its segment
+ *              [6] kind 1: not 0 where the item is within kind 2's bounds and
+ *                  is to be computed as one of these;  [7] unused
  *   pages    page numbers
  *   seg_rows [entries * 2] batch row, and the row's slot of the segment's
  *            first chunk

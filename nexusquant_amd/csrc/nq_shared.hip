@@ -107,6 +107,324 @@ __device__ __forceinline__ int value_exponent(const float (&wave_max)[NW]) {
     return 7 - e;
 }
 
+// ------------------------------------------------------------------- few rows ----
+
+// Up to 16 query rows of a kv head: a wave takes 16 tokens at a time through 16x16x16 MFMAs, from their codes to the
+// output without LDS between.  The int8 products leave a key's coordinates 16 t + 4 kg + i with lane (token, kg), which is
+// how the next product takes its A operand: S = K q^T comes out as lane (query, kg) with tokens 4 kg + i, which is how
+// P^T goes into O^T += V^T P^T.  For V^T lane (n, kg) reads the D / 16 bytes from D / 16 n on of tokens 4 kg + i and
+// turns them four by four, so tile j of the output is coordinates D / 16 r + j.  Keys stay without scales, which go with
+// the logits (sums of codes are below 2 D 127: they fit fp16).  Waves need no barriers; what a wave's next 16 tokens need
+// is loaded into registers as soon as they are free, without a branch, so that the waits count only what they must.
+//
+// us here and in the small shape above: 2 rows x 2 heads of 32 kv heads x 128 over 6352 own tokens 39.7 and 51.8 (2.7
+// TB/s of codes and scales), 64 x 8 of 8 over 512 28.8 and 35.8, 3 x 8 of 8 x 256 over 9184 40.6 and 71, 1 x 8 of 8 x 128
+// over 131072 106 and 118.  Loads alone take 29 of the first's 39.7; the rest is conversions (some 280 vector
+// instructions for 16 tokens of a head) and rows of the rotation table, twice the bytes of the codes, from L2.
+template <int D>
+struct Few {
+    static constexpr int WAVES = 4, ROWS = 16;
+    static constexpr int CHUNK = 1024;  // most tokens of a chunk
+    static constexpr int PER_SIMD = D == 64 ? 4 : D == 128 ? 3 : 2;
+};
+
+// over the lanes n, n + 16, n + 32, n + 48
+__device__ __forceinline__ f32x2 rows16(float v) {  // the values of lanes n and n ^ 16
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t lo = r[0], hi = r[1];
+    return {__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)};
+}
+__device__ __forceinline__ float four_max(float v) {
+    const f32x2 h = rows16(v);
+    return both_max(__builtin_fmaxf(h.x, h.y));
+}
+__device__ __forceinline__ float four_sum(float v) {
+    const f32x2 h = rows16(v);
+    return both_sum(h.x + h.y);
+}
+
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 mfma16(u32x2 a, u32x2 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+}
+
+template <int D>
+struct FewLds {
+    float vs[Few<D>::CHUNK];     // a token's value scale
+    uint32_t row[Few<D>::CHUNK]; // its row of this head
+    uint32_t pos[Few<D>::CHUNK]; // its rotation table row, in bytes
+    f32x4 o[Few<D>::WAVES / 2][D / 16][64];
+    uint16_t ks[Few<D>::CHUNK];  // its key scale (fp16)
+    float max[Few<D>::WAVES], m[Few<D>::WAVES / 2][16], l[Few<D>::WAVES / 2][16];
+};
+
+template <int D, int QDT>
+__device__ __forceinline__ void few_chunk(const SharedArgs& a, FewLds<D>& lds, const int32_t* it, uint32_t kh) {
+    using KM = KeyMfma<D>;
+    using F = Few<D>;
+    constexpr int T = KM::T, NW = F::WAVES, NT = 64 * NW;
+    constexpr int TILES = D / 16, VW = D / 64;  // tiles of the output; dwords of a token's values a lane
+    auto& s_row = lds.row;
+    auto& s_pos = lds.pos;
+    auto& s_vs = lds.vs;
+    auto& s_ks = lds.ks;
+    auto& s_max = lds.max;
+    auto& s_m = lds.m;
+    auto& s_l = lds.l;
+    auto& s_o = lds.o;
+
+    const int lane = threadIdx.x & 63, n16 = lane & 15, kg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int32_t* const pages = a.pages + it[0];
+    const uint32_t tok0 = (uint32_t)it[1];
+    const int32_t* const seg_rows = a.seg_rows + 2 * it[3];
+    const int G = (int)(a.q_heads / a.kv_heads), chunk = it[5];
+    // what LDS is sized for, whatever a plan from elsewhere holds
+    const int n_tok = (int)min(max((uint32_t)it[2], 1u), (uint32_t)F::CHUNK);
+    const int n_q = (int)min(max((uint32_t)it[4] * (uint32_t)G, 1u), (uint32_t)F::ROWS);
+    const int n_units = (n_tok + 15) / 16, last = 16 * n_units - 1;
+
+    // ---- queries: B operands of coordinates 16 t + 4 kg + 0..3 of either half ----
+    u32x2 q[2][T];
+    {
+        const uint32_t my_r = (uint32_t)min(n16, n_q - 1), my_br = div(my_r, a.by_group), my_head = kh * G + (my_r - my_br * G);
+        const uint16_t* const p = a.query + ((size_t)(uint32_t)seg_rows[2 * my_br] * a.q_heads + my_head) * D + 4 * kg;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int t = 0; t < T; ++t) q[hf][t] = *reinterpret_cast<const u32x2*>(p + hf * (D / 2) + 16 * t);
+    }
+
+    // ---- the chunk's tokens; places past it repeat its last (with weight 0) ----
+    auto row_of = [&](int i, uint32_t& page, uint32_t& off) {
+        const uint32_t t = tok0 + min(i, n_tok - 1), p = div(t, a.by_tokens);
+        off = t - p * a.tokens;
+        page = (uint32_t)pages[p];
+        return (page * a.kv_heads + kh) * a.tokens + off;
+    };
+    // Key codes a quad per token, 64 consecutive bytes, tables likewise: the operands want lane (token, kg), so the lanes
+    // exchange them when they are used.
+    uint32_t kcode[2][KM::NK][KM::W], vcode[4][VW];
+    constexpr int DEPTH = T <= 4 ? T : 2;  // tiles of the tables on their way (registers)
+    static_assert(T % DEPTH == 0, "a tile keeps its registers from token to token");
+    f32x4 tm[DEPTH], tp[DEPTH];
+    auto load_keys = [&](uint32_t lane, uint32_t row) {  // row: of token lane / 4
+        const int8_t* const p = a.kc + (size_t)row * D + KM::KPL * (lane & 3u);
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int s = 0; s < KM::NK; ++s) {
+                const uint32_t* const w = reinterpret_cast<const uint32_t*>(p + hf * KM::HALF + s * KM::KB);
+#pragma unroll
+                for (int i = 0; i < KM::W; ++i) kcode[hf][s][i] = w[i];
+            }
+    };
+    auto load_table = [&](int t, uint32_t tab) {
+        tm[t % DEPTH] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(a.rope_dm) + (tab + 64u * t));
+        tp[t % DEPTH] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(a.rope_dp) + (tab + 64u * t));
+    };
+    auto load_values = [&](uint32_t n16, int i, uint32_t row) {  // row: of token 4 kg + i
+        const uint32_t* const w = reinterpret_cast<const uint32_t*>(a.vc + (size_t)row * D + (D / 16) * n16);
+#pragma unroll
+        for (int k = 0; k < VW; ++k) vcode[i][k] = w[k];
+    };
+    {
+        uint32_t page, off;
+        load_keys(lane, row_of(16 * wave + (lane >> 2), page, off));
+    }
+    float vmax = 0.0f;
+    for (int i = threadIdx.x; i <= last; i += NT) {
+        uint32_t page, off;
+        const uint32_t row = row_of(i, page, off);
+        const int32_t pos = a.positions[page * a.tokens + off];
+        const float vs = i < n_tok ? f16_bits_to_f32(a.vs[row]) : 0.0f;
+        s_row[i] = row;
+        s_pos[i] = (pos < 0 ? 0u : ((uint32_t)pos >= a.rope_n_pos ? a.rope_n_pos - 1u : (uint32_t)pos)) * (2u * D);
+        s_ks[i] = a.ks[row];
+        s_vs[i] = vs;
+        vmax = __builtin_fmaxf(vmax, __builtin_fabsf(vs));
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) vmax = __builtin_fmaxf(vmax, __shfl_xor(vmax, o, 64));
+    if (lane == 0) s_max[wave] = vmax;
+    float c = a.c * (0.5f * a.hscale);
+    if constexpr (QDT == NQ_BF16) c *= bf16_queries(q, [](float v) { return four_max(v); });
+    KM signs;
+    signs.init(lane);
+    __syncthreads();
+    const int vexp = value_exponent<NW>(s_max);  // used with the weights, not in place: no second pass over s_vs
+
+    uint32_t tab;
+    {
+        const int first = min(16 * wave, last - 15);
+        tab = s_pos[first + (lane >> 2)] + 16u * (lane & 3);
+#pragma unroll
+        for (int t = 0; t < DEPTH; ++t) load_table(t, tab);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_values(n16, i, s_row[first + 4 * kg + i]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+
+    f32x4 o[TILES];
+#pragma unroll
+    for (int j = 0; j < TILES; ++j) o[j] = f32x4{};
+    float m = kNoMax, l = 0.0f;
+    const float vmul = __builtin_ldexpf(1.0f, vexp);
+#pragma unroll 1
+    for (int u = wave; u < n_units; u += NW) {
+        // what follows from the lane alone is worked out again each time, as in decode
+        uint32_t lane = threadIdx.x;
+        asm volatile("" : "+v"(lane));
+        lane &= 63u;
+        const uint32_t n16 = lane & 15u, kg = lane >> 4;
+        const int from_quad = (int)(4 * (4 * n16 + kg));  // byte address of the lane that loaded this lane's block
+        KM km = signs;
+#pragma unroll
+        for (int w = 0; w < KM::W; ++w) asm volatile("" : "+v"(km.h[w]));
+        const int next = 16 * min(u + NW, n_units - 1);
+        uint32_t code[2][KM::NK][KM::W];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int s = 0; s < KM::NK; ++s)
+#pragma unroll
+                for (int i = 0; i < KM::W; ++i) code[hf][s][i] = (uint32_t)__builtin_amdgcn_ds_bpermute(from_quad, (int)kcode[hf][s][i]);
+        load_keys(lane, s_row[next + (lane >> 2)]);
+        const uint32_t next_tab = s_pos[next + (lane >> 2)] + 16u * (lane & 3u);
+        __builtin_amdgcn_sched_barrier(0);
+        f32x4 s = {};
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            f32x4 dm, dp;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = tm[t % DEPTH][i], y = tp[t % DEPTH][i];  // (an element is taken out before it is cast)
+                dm[i] = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(from_quad, __builtin_bit_cast(int, x)));
+                dp[i] = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(from_quad, __builtin_bit_cast(int, y)));
+            }
+            if (t + DEPTH < T) load_table(t + DEPTH, tab);
+            else load_table(t + DEPTH - T, next_tab);
+            int4v y0 = {0, 0, 0, 0}, y1 = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < KM::NK; ++k) {
+                y0 = km.mul(t, k, lane, code[0][k], y0);
+                y1 = km.mul(t, k, lane, code[1][k], y1);
+            }
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float lo = (float)y0[i], hi = (float)y1[i];
+                x[i] = __builtin_fmaf(-lo, dm[i], hi * dp[i]);
+                x[4 + i] = __builtin_fmaf(lo, dp[i], hi * dm[i]);
+            }
+            s = mfma16(u32x2{pack2<NQ_F16>(x[0], x[1]), pack2<NQ_F16>(x[2], x[3])}, q[0][t], s);
+            s = mfma16(u32x2{pack2<NQ_F16>(x[4], x[5]), pack2<NQ_F16>(x[6], x[7])}, q[1][t], s);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        tab = next_tab;
+        // ---- weights ----
+        const int at = 16 * u + 4 * (int)kg, left = n_tok - at;
+        const u32x2 kw = *reinterpret_cast<const u32x2*>(s_ks + at);
+        const f32x4 vs = *reinterpret_cast<const f32x4*>(s_vs + at);
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = s[i] * f16_bits_to_f32((i & 1) ? kw[i / 2] >> 16 : kw[i / 2] & 0xffffu);
+            s[i] = i < left ? x * c : -__builtin_inff();
+            mx = __builtin_fmaxf(mx, s[i]);
+        }
+        if (__any(mx > m + kSlack)) {
+            const float to = __builtin_fmaxf(m, four_max(mx));
+            const float f = __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            l *= f;
+#pragma unroll
+            for (int j = 0; j < TILES; ++j) o[j] *= f;
+        }
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(s[i] - m);
+            l += p[i];
+            p[i] *= vs[i] * vmul;
+        }
+        const u32x2 w = {pack2<NQ_F16>(p[0], p[1]), pack2<NQ_F16>(p[2], p[3])};
+        // ---- values: bytes to fp16 as codes_to_f16, four tokens of a coordinate together ----
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+            uint32_t x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = vcode[i][k] ^ 0x80808080u;
+            const uint32_t pairs[2][2] = {{__builtin_amdgcn_perm(x[1], x[0], 0x05010400u), __builtin_amdgcn_perm(x[3], x[2], 0x05010400u)},
+                                          {__builtin_amdgcn_perm(x[1], x[0], 0x07030602u), __builtin_amdgcn_perm(x[3], x[2], 0x07030602u)}};
+            const half2v bias = {(__fp16)-1152.0f, (__fp16)-1152.0f};
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const uint32_t sel = (b & 1) ? 0x00070006u : 0x00050004u;
+                const half2v v0 = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(pairs[b / 2][0], 0x64646464u, sel)) + bias;
+                const half2v v1 = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(pairs[b / 2][1], 0x64646464u, sel)) + bias;
+                o[4 * k + b] = mfma16(u32x2{__builtin_bit_cast(uint32_t, v0), __builtin_bit_cast(uint32_t, v1)}, w, o[4 * k + b]);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_values(n16, i, s_row[next + 4 * kg + i]);
+    }
+
+    // ---- the waves' sums joined: the upper half's into the lower half's, twice ----
+    uint32_t end_lane = threadIdx.x;  // as in the loop: nothing of the lane is kept over it
+    asm volatile("" : "+v"(end_lane));
+    const int lane2 = end_lane & 63, n = lane2 & 15, g = lane2 >> 4;
+    l = four_sum(l);
+#pragma unroll
+    for (int step = NW / 2; step >= 1; step >>= 1) {
+        if (wave >= step && wave < 2 * step) {
+#pragma unroll
+            for (int j = 0; j < TILES; ++j) s_o[wave - step][j][lane2] = o[j];
+            if (g == 0) {
+                s_m[wave - step][n] = m;
+                s_l[wave - step][n] = l;
+            }
+        }
+        __syncthreads();
+        if (wave < step) {
+            const float mo = s_m[wave][n], to = __builtin_fmaxf(m, mo);
+            const float f = __builtin_amdgcn_exp2f(m - to), fo = __builtin_amdgcn_exp2f(mo - to);
+            m = to;
+            l = l * f + s_l[wave][n] * fo;
+#pragma unroll
+            for (int j = 0; j < TILES; ++j) {
+                const f32x4 y = s_o[wave][j][lane2];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[j][i] = __builtin_fmaf(y[i], fo, o[j][i] * f);
+            }
+        }
+        __syncthreads();
+    }
+    if (wave > 0 || n >= n_q) return;
+    const uint32_t my_br = div((uint32_t)n, a.by_group), my_head = kh * G + ((uint32_t)n - my_br * G);
+    const size_t slot = (size_t)(uint32_t)(seg_rows[2 * my_br + 1] + chunk) * a.q_heads + my_head;
+    if (g == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * slot) = f32x2{m, l};
+    const float f = __builtin_ldexpf(0.5f, -vexp);
+    float* const y = a.part_y + slot * D + (D / 16) * 4 * g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < VW; ++k)
+            *reinterpret_cast<f32x4*>(y + (D / 16) * i + 4 * k) = f32x4{o[4 * k][i] * f, o[4 * k + 1][i] * f, o[4 * k + 2][i] * f, o[4 * k + 3][i] * f};
+}
+
+template <int D, int QDT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Few<D>::PER_SIMD))) void few_attn_kernel(SharedArgs a) {
+    __shared__ __align__(16) FewLds<D> lds;
+    const uint32_t in_xcd = blockIdx.x >> 3, item = (blockIdx.x & 7u) + 8u * (in_xcd / a.kv_heads);  // as in shared_attn_kernel
+    if (item < a.n_items) few_chunk<D, QDT>(a, lds, a.items + 8 * item, in_xcd % a.kv_heads);
+}
+
+// -------------------------------------------------------------- some rows, many ----
+
 template <int D, int QDT, bool MANY>
 __global__ __launch_bounds__((Shape<D, MANY>::THREADS)) __attribute__((amdgpu_waves_per_eu(Shape<D, MANY>::PER_SIMD))) void
 shared_attn_kernel(SharedArgs a) {
@@ -129,6 +447,13 @@ shared_attn_kernel(SharedArgs a) {
     const uint32_t in_xcd = blockIdx.x >> 3, item = (blockIdx.x & 7u) + 8u * (in_xcd / a.kv_heads), kh = in_xcd % a.kv_heads;
     if (item >= a.n_items) return;  // whole block
     const int32_t* const it = a.items + 8 * item;
+    if constexpr (!MANY) {
+        static_assert(sizeof(FewLds<D>) <= sizeof(s_kv) && 64 * Few<D>::WAVES == NT, "a chunk of few rows in this launch");
+        if (it[6] != 0) {
+            few_chunk<D, QDT>(a, *reinterpret_cast<FewLds<D>*>(&s_kv), it, kh);
+            return;
+        }
+    }
     const int32_t* const pages = a.pages + it[0];
     const uint32_t tok0 = (uint32_t)it[1];
     const int32_t* const seg_rows = a.seg_rows + 2 * it[3];
@@ -407,306 +732,6 @@ shared_attn_kernel(SharedArgs a) {
         if constexpr (MANY) __builtin_nontemporal_store(y, to);
         else *to = y;
     }
-}
-
-// ------------------------------------------------------------------- few rows ----
-
-// Up to 16 query rows of a kv head: a wave takes 16 tokens at a time through 16x16x16 MFMAs, from their codes to the
-// output without LDS between.  The int8 products leave a key's coordinates 16 t + 4 kg + i with lane (token, kg), which is
-// how the next product takes its A operand: S = K q^T comes out as lane (query, kg) with tokens 4 kg + i, which is how
-// P^T goes into O^T += V^T P^T.  For V^T lane (n, kg) reads the D / 16 bytes from D / 16 n on of tokens 4 kg + i and
-// turns them four by four, so tile j of the output is coordinates D / 16 r + j.  Keys stay without scales, which go with
-// the logits (sums of codes are below 2 D 127: they fit fp16).  Waves need no barriers; what a wave's next 16 tokens need
-// is loaded into registers as soon as they are free, without a branch, so that the waits count only what they must.
-//
-// us here and in the small shape above: 2 rows x 2 heads of 32 kv heads x 128 over 6352 own tokens 39.7 and 51.8 (2.7
-// TB/s of codes and scales), 64 x 8 of 8 over 512 28.8 and 35.8, 3 x 8 of 8 x 256 over 9184 40.6 and 71, 1 x 8 of 8 x 128
-// over 131072 106 and 118.  Loads alone take 29 of the first's 39.7; the rest is conversions (some 280 vector
-// instructions for 16 tokens of a head) and rows of the rotation table, twice the bytes of the codes, from L2.
-template <int D>
-struct Few {
-    static constexpr int WAVES = 4, ROWS = 16;
-    static constexpr int CHUNK = 1024;  // most tokens of a chunk
-    static constexpr int PER_SIMD = D == 64 ? 4 : D == 128 ? 3 : 2;
-};
-
-// over the lanes n, n + 16, n + 32, n + 48
-__device__ __forceinline__ f32x2 rows16(float v) {  // the values of lanes n and n ^ 16
-    const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const uint32_t lo = r[0], hi = r[1];
-    return {__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)};
-}
-__device__ __forceinline__ float four_max(float v) {
-    const f32x2 h = rows16(v);
-    return both_max(__builtin_fmaxf(h.x, h.y));
-}
-__device__ __forceinline__ float four_sum(float v) {
-    const f32x2 h = rows16(v);
-    return both_sum(h.x + h.y);
-}
-
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ f32x4 mfma16(u32x2 a, u32x2 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
-}
-
-template <int D, int QDT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Few<D>::PER_SIMD))) void few_attn_kernel(SharedArgs a) {
-    using KM = KeyMfma<D>;
-    using F = Few<D>;
-    constexpr int T = KM::T, NW = F::WAVES, NT = 64 * NW;
-    constexpr int TILES = D / 16, VW = D / 64;  // tiles of the output; dwords of a token's values a lane
-    __shared__ uint32_t s_row[F::CHUNK];
-    __shared__ uint32_t s_pos[F::CHUNK];
-    __shared__ __align__(16) float s_vs[F::CHUNK];
-    __shared__ __align__(8) uint16_t s_ks[F::CHUNK];
-    __shared__ float s_max[NW], s_m[NW / 2][16], s_l[NW / 2][16];
-    __shared__ f32x4 s_o[NW / 2][TILES][64];
-
-    const int lane = threadIdx.x & 63, n16 = lane & 15, kg = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const uint32_t in_xcd = blockIdx.x >> 3, item = (blockIdx.x & 7u) + 8u * (in_xcd / a.kv_heads), kh = in_xcd % a.kv_heads;
-    if (item >= a.n_items) return;  // whole block
-    const int32_t* const it = a.items + 8 * item;
-    const int32_t* const pages = a.pages + it[0];
-    const uint32_t tok0 = (uint32_t)it[1];
-    const int32_t* const seg_rows = a.seg_rows + 2 * it[3];
-    const int G = (int)(a.q_heads / a.kv_heads), chunk = it[5];
-    // what LDS is sized for, whatever a plan from elsewhere holds
-    const int n_tok = (int)min(max((uint32_t)it[2], 1u), (uint32_t)F::CHUNK);
-    const int n_q = (int)min(max((uint32_t)it[4] * (uint32_t)G, 1u), (uint32_t)F::ROWS);
-    const int n_units = (n_tok + 15) / 16, last = 16 * n_units - 1;
-
-    // ---- queries: B operands of coordinates 16 t + 4 kg + 0..3 of either half ----
-    u32x2 q[2][T];
-    {
-        const uint32_t my_r = (uint32_t)min(n16, n_q - 1), my_br = div(my_r, a.by_group), my_head = kh * G + (my_r - my_br * G);
-        const uint16_t* const p = a.query + ((size_t)(uint32_t)seg_rows[2 * my_br] * a.q_heads + my_head) * D + 4 * kg;
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-            for (int t = 0; t < T; ++t) q[hf][t] = *reinterpret_cast<const u32x2*>(p + hf * (D / 2) + 16 * t);
-    }
-
-    // ---- the chunk's tokens; places past it repeat its last (with weight 0) ----
-    auto row_of = [&](int i, uint32_t& page, uint32_t& off) {
-        const uint32_t t = tok0 + min(i, n_tok - 1), p = div(t, a.by_tokens);
-        off = t - p * a.tokens;
-        page = (uint32_t)pages[p];
-        return (page * a.kv_heads + kh) * a.tokens + off;
-    };
-    // Key codes a quad per token, 64 consecutive bytes, tables likewise: the operands want lane (token, kg), so the lanes
-    // exchange them when they are used.
-    uint32_t kcode[2][KM::NK][KM::W], vcode[4][VW];
-    constexpr int DEPTH = T <= 4 ? T : 2;  // tiles of the tables on their way (registers)
-    static_assert(T % DEPTH == 0, "a tile keeps its registers from token to token");
-    f32x4 tm[DEPTH], tp[DEPTH];
-    auto load_keys = [&](uint32_t lane, uint32_t row) {  // row: of token lane / 4
-        const int8_t* const p = a.kc + (size_t)row * D + KM::KPL * (lane & 3u);
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-            for (int s = 0; s < KM::NK; ++s) {
-                const uint32_t* const w = reinterpret_cast<const uint32_t*>(p + hf * KM::HALF + s * KM::KB);
-#pragma unroll
-                for (int i = 0; i < KM::W; ++i) kcode[hf][s][i] = w[i];
-            }
-    };
-    auto load_table = [&](int t, uint32_t tab) {
-        tm[t % DEPTH] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(a.rope_dm) + (tab + 64u * t));
-        tp[t % DEPTH] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(a.rope_dp) + (tab + 64u * t));
-    };
-    auto load_values = [&](uint32_t n16, int i, uint32_t row) {  // row: of token 4 kg + i
-        const uint32_t* const w = reinterpret_cast<const uint32_t*>(a.vc + (size_t)row * D + (D / 16) * n16);
-#pragma unroll
-        for (int k = 0; k < VW; ++k) vcode[i][k] = w[k];
-    };
-    {
-        uint32_t page, off;
-        load_keys(lane, row_of(16 * wave + (lane >> 2), page, off));
-    }
-    float vmax = 0.0f;
-    for (int i = threadIdx.x; i <= last; i += NT) {
-        uint32_t page, off;
-        const uint32_t row = row_of(i, page, off);
-        const int32_t pos = a.positions[page * a.tokens + off];
-        const float vs = i < n_tok ? f16_bits_to_f32(a.vs[row]) : 0.0f;
-        s_row[i] = row;
-        s_pos[i] = (pos < 0 ? 0u : ((uint32_t)pos >= a.rope_n_pos ? a.rope_n_pos - 1u : (uint32_t)pos)) * (2u * D);
-        s_ks[i] = a.ks[row];
-        s_vs[i] = vs;
-        vmax = __builtin_fmaxf(vmax, __builtin_fabsf(vs));
-    }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) vmax = __builtin_fmaxf(vmax, __shfl_xor(vmax, o, 64));
-    if (lane == 0) s_max[wave] = vmax;
-    float c = a.c * (0.5f * a.hscale);
-    if constexpr (QDT == NQ_BF16) c *= bf16_queries(q, [](float v) { return four_max(v); });
-    KM signs;
-    signs.init(lane);
-    __syncthreads();
-    const int vexp = value_exponent<NW>(s_max);  // used with the weights, not in place: no second pass over s_vs
-
-    uint32_t tab;
-    {
-        const int first = min(16 * wave, last - 15);
-        tab = s_pos[first + (lane >> 2)] + 16u * (lane & 3);
-#pragma unroll
-        for (int t = 0; t < DEPTH; ++t) load_table(t, tab);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) load_values(n16, i, s_row[first + 4 * kg + i]);
-        __builtin_amdgcn_sched_barrier(0);
-    }
-
-    f32x4 o[TILES];
-#pragma unroll
-    for (int j = 0; j < TILES; ++j) o[j] = f32x4{};
-    float m = kNoMax, l = 0.0f;
-    const float vmul = __builtin_ldexpf(1.0f, vexp);
-#pragma unroll 1
-    for (int u = wave; u < n_units; u += NW) {
-        // what follows from the lane alone is worked out again each time, as in decode
-        uint32_t lane = threadIdx.x;
-        asm volatile("" : "+v"(lane));
-        lane &= 63u;
-        const uint32_t n16 = lane & 15u, kg = lane >> 4;
-        const int from_quad = (int)(4 * (4 * n16 + kg));  // byte address of the lane that loaded this lane's block
-        KM km = signs;
-#pragma unroll
-        for (int w = 0; w < KM::W; ++w) asm volatile("" : "+v"(km.h[w]));
-        const int next = 16 * min(u + NW, n_units - 1);
-        uint32_t code[2][KM::NK][KM::W];
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-            for (int s = 0; s < KM::NK; ++s)
-#pragma unroll
-                for (int i = 0; i < KM::W; ++i) code[hf][s][i] = (uint32_t)__builtin_amdgcn_ds_bpermute(from_quad, (int)kcode[hf][s][i]);
-        load_keys(lane, s_row[next + (lane >> 2)]);
-        const uint32_t next_tab = s_pos[next + (lane >> 2)] + 16u * (lane & 3u);
-        __builtin_amdgcn_sched_barrier(0);
-        f32x4 s = {};
-#pragma unroll
-        for (int t = 0; t < T; ++t) {
-            f32x4 dm, dp;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = tm[t % DEPTH][i], y = tp[t % DEPTH][i];  // (an element is taken out before it is cast)
-                dm[i] = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(from_quad, __builtin_bit_cast(int, x)));
-                dp[i] = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(from_quad, __builtin_bit_cast(int, y)));
-            }
-            if (t + DEPTH < T) load_table(t + DEPTH, tab);
-            else load_table(t + DEPTH - T, next_tab);
-            int4v y0 = {0, 0, 0, 0}, y1 = {0, 0, 0, 0};
-#pragma unroll
-            for (int k = 0; k < KM::NK; ++k) {
-                y0 = km.mul(t, k, lane, code[0][k], y0);
-                y1 = km.mul(t, k, lane, code[1][k], y1);
-            }
-            float x[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float lo = (float)y0[i], hi = (float)y1[i];
-                x[i] = __builtin_fmaf(-lo, dm[i], hi * dp[i]);
-                x[4 + i] = __builtin_fmaf(lo, dp[i], hi * dm[i]);
-            }
-            s = mfma16(u32x2{pack2<NQ_F16>(x[0], x[1]), pack2<NQ_F16>(x[2], x[3])}, q[0][t], s);
-            s = mfma16(u32x2{pack2<NQ_F16>(x[4], x[5]), pack2<NQ_F16>(x[6], x[7])}, q[1][t], s);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        tab = next_tab;
-        // ---- weights ----
-        const int at = 16 * u + 4 * (int)kg, left = n_tok - at;
-        const u32x2 kw = *reinterpret_cast<const u32x2*>(s_ks + at);
-        const f32x4 vs = *reinterpret_cast<const f32x4*>(s_vs + at);
-        float mx = -__builtin_inff();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float x = s[i] * f16_bits_to_f32((i & 1) ? kw[i / 2] >> 16 : kw[i / 2] & 0xffffu);
-            s[i] = i < left ? x * c : -__builtin_inff();
-            mx = __builtin_fmaxf(mx, s[i]);
-        }
-        if (__any(mx > m + kSlack)) {
-            const float to = __builtin_fmaxf(m, four_max(mx));
-            const float f = __builtin_amdgcn_exp2f(m - to);
-            m = to;
-            l *= f;
-#pragma unroll
-            for (int j = 0; j < TILES; ++j) o[j] *= f;
-        }
-        float p[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(s[i] - m);
-            l += p[i];
-            p[i] *= vs[i] * vmul;
-        }
-        const u32x2 w = {pack2<NQ_F16>(p[0], p[1]), pack2<NQ_F16>(p[2], p[3])};
-        // ---- values: bytes to fp16 as codes_to_f16, four tokens of a coordinate together ----
-#pragma unroll
-        for (int k = 0; k < VW; ++k) {
-            uint32_t x[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = vcode[i][k] ^ 0x80808080u;
-            const uint32_t pairs[2][2] = {{__builtin_amdgcn_perm(x[1], x[0], 0x05010400u), __builtin_amdgcn_perm(x[3], x[2], 0x05010400u)},
-                                          {__builtin_amdgcn_perm(x[1], x[0], 0x07030602u), __builtin_amdgcn_perm(x[3], x[2], 0x07030602u)}};
-            const half2v bias = {(__fp16)-1152.0f, (__fp16)-1152.0f};
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const uint32_t sel = (b & 1) ? 0x00070006u : 0x00050004u;
-                const half2v v0 = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(pairs[b / 2][0], 0x64646464u, sel)) + bias;
-                const half2v v1 = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(pairs[b / 2][1], 0x64646464u, sel)) + bias;
-                o[4 * k + b] = mfma16(u32x2{__builtin_bit_cast(uint32_t, v0), __builtin_bit_cast(uint32_t, v1)}, w, o[4 * k + b]);
-            }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) load_values(n16, i, s_row[next + 4 * kg + i]);
-    }
-
-    // ---- the waves' sums joined: the upper half's into the lower half's, twice ----
-    uint32_t end_lane = threadIdx.x;  // as in the loop: nothing of the lane is kept over it
-    asm volatile("" : "+v"(end_lane));
-    const int lane2 = end_lane & 63, n = lane2 & 15, g = lane2 >> 4;
-    l = four_sum(l);
-#pragma unroll
-    for (int step = NW / 2; step >= 1; step >>= 1) {
-        if (wave >= step && wave < 2 * step) {
-#pragma unroll
-            for (int j = 0; j < TILES; ++j) s_o[wave - step][j][lane2] = o[j];
-            if (g == 0) {
-                s_m[wave - step][n] = m;
-                s_l[wave - step][n] = l;
-            }
-        }
-        __syncthreads();
-        if (wave < step) {
-            const float mo = s_m[wave][n], to = __builtin_fmaxf(m, mo);
-            const float f = __builtin_amdgcn_exp2f(m - to), fo = __builtin_amdgcn_exp2f(mo - to);
-            m = to;
-            l = l * f + s_l[wave][n] * fo;
-#pragma unroll
-            for (int j = 0; j < TILES; ++j) {
-                const f32x4 y = s_o[wave][j][lane2];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[j][i] = __builtin_fmaf(y[i], fo, o[j][i] * f);
-            }
-        }
-        __syncthreads();
-    }
-    if (wave > 0 || n >= n_q) return;
-    const uint32_t my_br = div((uint32_t)n, a.by_group), my_head = kh * G + ((uint32_t)n - my_br * G);
-    const size_t slot = (size_t)(uint32_t)(seg_rows[2 * my_br + 1] + chunk) * a.q_heads + my_head;
-    if (g == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * slot) = f32x2{m, l};
-    const float f = __builtin_ldexpf(0.5f, -vexp);
-    float* const y = a.part_y + slot * D + (D / 16) * 4 * g;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int k = 0; k < VW; ++k)
-            *reinterpret_cast<f32x4*>(y + (D / 16) * i + 4 * k) = f32x4{o[4 * k][i] * f, o[4 * k + 1][i] * f, o[4 * k + 2][i] * f, o[4 * k + 3][i] * f};
 }
 
 // One (row, query head) a workgroup: its chunks' sums weighted and added in a fixed order, then the

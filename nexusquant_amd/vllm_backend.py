@@ -520,8 +520,9 @@ _SHARED_LEAST = (256, 128, 64)
 _MANY, _SOME, _FEW = 0, 1, 2
 _MANY_ROWS = 32
 _MANY_TOKENS = 512
-# Few go along with some, where there are any, unless they have _FEW_TOKENS tokens for each CU: a launch less.  32 rows
-# of 4 heads over a shared 4096 tokens and 256 own ones: 26 us, with a launch for the own ones 36.
+# Few go into the launch of some, where there are any, unless they have _FEW_TOKENS tokens for each CU: 32 rows of 4
+# heads over a shared 4096 tokens and 256 own ones 25.7 us, with a launch for the own ones 36, as some themselves
+# 26.3.  (The shared ones in chunks of one stage, the own ones in longer ones: 27.4.)
 _FEW_TOKENS = 1024
 
 
@@ -545,18 +546,19 @@ def shared_items(segments, batch: int, group: int, kv_heads: int, head_dim: int,
     work = kv_heads * sum(s[2] * -(-q // rows[_MANY]) for s, q, k in zip(segments, queries, kind) if k == _MANY)
     if work < 256 * _MANY_TOKENS:
         kind = [_SOME if k == _MANY and q <= rows[_SOME] else k for k, q in zip(kind, queries)]
+    launch = kind
     if _SOME in kind and kv_heads * sum(s[2] for s, k in zip(segments, kind) if k == _FEW) < 256 * _FEW_TOKENS:
-        kind = [_SOME if k == _FEW else k for k in kind]
+        launch = [_SOME if k == _FEW else k for k in kind]
     per_tile = [max(1, n // group) for n in rows]  # batch rows of a workgroup
     tiles = [-(-len(s[0]) // per_tile[k]) for s, k in zip(segments, kind)]
     # as many workgroups as run at once: LDS leaves one of the wide ones on a CU, LDS or registers those of the others
     at_once = (1, {64: 3, 128: 2}.get(head_dim, 1), {64: 4, 128: 3}.get(head_dim, 2))
     step = []
     for k in (_MANY, _SOME, _FEW):
-        of = [i for i in range(len(segments)) if kind[i] == k]
+        of = [i for i in range(len(segments)) if launch[i] == k]
         step.append(_shared_chunk([segments[i][2] for i in of], [tiles[i] for i in of], kv_heads, cap[k],
                                   _SHARED_LEAST[k], _SHARED_STAGE[k], 256 * at_once[k]))
-    chunks = [-(-s[2] // step[k]) for s, k in zip(segments, kind)]
+    chunks = [-(-s[2] // step[k]) for s, k in zip(segments, launch)]
     per_row = [0] * (batch + 1)
     for (r, _, _), c in zip(segments, chunks):
         for b in r:
@@ -566,22 +568,22 @@ def shared_items(segments, batch: int, group: int, kv_heads: int, head_dim: int,
     records, seg_rows, pages = [], [], []
     at_pages = 0
     # by kind, long ones before short ones
-    for i in sorted(range(len(segments)), key=lambda i: (kind[i], -segments[i][2])):
+    for i in sorted(range(len(segments)), key=lambda i: (launch[i], -segments[i][2])):
         r, seg_pages, n = segments[i]
         at_rows = len(seg_rows)
         for b in r:
             seg_rows.append((b, nxt[b]))
             nxt[b] += chunks[i]
         # chunks in eights (one for each XCD), a chunk's row tiles one eight after another
-        length, per = step[kind[i]], per_tile[kind[i]]
+        length, per, few = step[launch[i]], per_tile[kind[i]], int(launch[i] != kind[i])
         for c0 in range(0, chunks[i], 8):
             for r0 in range(0, len(r), per):
                 for c in range(c0, min(c0 + 8, chunks[i])):
                     records.append((at_pages, c * length, min(n - c * length, length), at_rows + r0,
-                                    min(len(r) - r0, per), c, 0, 0))
+                                    min(len(r) - r0, per), c, few, 0))
         pages.append(np.asarray(seg_pages, dtype=np.int32))
         at_pages += len(seg_pages)
-    n_kind = [sum(t * c for t, c, x in zip(tiles, chunks, kind) if x == k) for k in (_MANY, _FEW)]
+    n_kind = [sum(t * c for t, c, x in zip(tiles, chunks, launch) if x == k) for k in (_MANY, _FEW)]
     parts = {"items": np.array(records, dtype=np.int32).reshape(-1),
              "pages": np.concatenate(pages) if pages else np.zeros(0, dtype=np.int32),
              "seg_rows": np.array(seg_rows, dtype=np.int32).reshape(-1), "row_slots": row_slots.astype(np.int32)}

@@ -98,8 +98,8 @@ def test_items_cover_each_rows_tokens_and_slots_once(group, kv_heads, d, cap, ro
     where = parts["seg_rows"].reshape(-1, 2)
     assert len(items) == n_items and parts["row_slots"][0] == 0 and parts["row_slots"][-1] == n_slots
     seen, slots = {}, []
-    for i, (page0, tok0, n, row0, n_rows, chunk, _, _) in enumerate(items):
-        most = rows[0 if i < n_many else 2 if i >= n_items - n_few else 1]
+    for i, (page0, tok0, n, row0, n_rows, chunk, few, _) in enumerate(items):
+        most = rows[0 if i < n_many else 2 if few or i >= n_items - n_few else 1]
         assert 1 <= n <= cap and 1 <= n_rows and n_rows * group <= most
         for b, slot0 in where[row0:row0 + n_rows]:
             slots.append(slot0 + chunk)
