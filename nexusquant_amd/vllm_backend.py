@@ -520,10 +520,12 @@ _SHARED_LEAST = (256, 128, 64)
 _MANY, _SOME, _FEW = 0, 1, 2
 _MANY_ROWS = 32
 _MANY_TOKENS = 512
-# Few go into the launch of some, where there are any, unless they have _FEW_TOKENS tokens for each CU: 32 rows of 4
-# heads over a shared 4096 tokens and 256 own ones 25.7 us, with a launch for the own ones 36, as some themselves
-# 26.3.  (The shared ones in chunks of one stage, the own ones in longer ones: 27.4.)
-_FEW_TOKENS = 1024
+# Few go into the launch of some, where there are any, as long as they have less than this many tokens for each CU (each
+# segment counted as 128 at least).  A shared 4096 tokens of 128 query rows and own ones, us together and with a launch
+# for the own ones: 8 kv heads x 128, 512 a CU 36.9 and 40.0, 1024 60 and 47; x 64, 768 24.0 and 27.7, 1536 35.9 and
+# 36.0; 4 x 256, 128 39.2 and 44.8, 256 60.5 and 47.7.  32 rows of 4 heads and 256 own tokens: 25.7 us together, 26.3
+# with the own ones as some, 36 with a launch of their own.
+_FEW_TOKENS = {64: 1536, 128: 768, 256: 192}
 
 
 def _shared_chunk(lengths, tiles, kv_heads: int, cap: int, least: int, stage: int, workgroups: int) -> int:
@@ -547,7 +549,8 @@ def shared_items(segments, batch: int, group: int, kv_heads: int, head_dim: int,
     if work < 256 * _MANY_TOKENS:
         kind = [_SOME if k == _MANY and q <= rows[_SOME] else k for k, q in zip(kind, queries)]
     launch = kind
-    if _SOME in kind and kv_heads * sum(s[2] for s, k in zip(segments, kind) if k == _FEW) < 256 * _FEW_TOKENS:
+    few_tokens = kv_heads * sum(max(s[2], 128) for s, k in zip(segments, kind) if k == _FEW)
+    if _SOME in kind and few_tokens < 256 * _FEW_TOKENS[head_dim]:
         launch = [_SOME if k == _FEW else k for k in kind]
     per_tile = [max(1, n // group) for n in rows]  # batch rows of a workgroup
     tiles = [-(-len(s[0]) // per_tile[k]) for s, k in zip(segments, kind)]

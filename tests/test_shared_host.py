@@ -120,6 +120,16 @@ def test_which_kind_a_segment_is(rows, group, tokens, kind):
     assert (n_many, n_items - n_many - n_few, n_few) == tuple(n_items if k == kind else 0 for k in range(3))
 
 
+@pytest.mark.parametrize("rows,own,together", [(32, 256, True), (32, 1024, False), (300, 1, False)])
+def test_few_go_along_with_some(rows, own, together):
+    segments = [(list(range(16)), np.arange(64), 1024)]
+    segments += [([b], np.arange(100, 100 + -(-own // 16)), own) for b in range(rows)]
+    parts, n_items, n_many, n_few, _ = shared_items(segments, rows, 8, 8, 128, (2048, 1024, 1024), (256, 128, 16))
+    flagged = parts["items"].reshape(-1, 8)[:, 6]
+    assert n_many == 0 and (n_few == 0) == together
+    assert flagged.sum() == (n_items - (flagged == 0).sum() if together else 0) and (flagged.any() == together)
+
+
 def test_no_rows_and_no_tokens():
     parts, *counts = shared_items([], 3, 4, 8, 128, (2048, 1024, 1024), (256, 128, 16))
     assert counts == [0, 0, 0, 0] and list(parts["row_slots"]) == [0, 0, 0, 0]
