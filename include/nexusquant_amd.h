@@ -689,7 +689,7 @@ int nq_pool_write(const nq_pool* pool, int32_t layer, const nq_pool* tokens, con
  * Device int32 arrays.  query, out: [batch, q_heads, head_dim], fp16 or bf16;
  * a row without slots is zero.  Rounding: keys to fp16; queries of bf16 to
  * fp16 after a power of two is taken out; softmax weights times the values'
- * scales to fp16; sums in fp32.
+ * scales to fp16 (kind 2: to twice fp16's 11 bits); sums in fp32.
  * workspace: nq_shared_attention_workspace(n_slots, q_heads, head_dim) bytes,
  * 16-byte aligned.
  */
