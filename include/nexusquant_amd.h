@@ -600,10 +600,13 @@ typedef struct nq_prompt_desc {
     const int32_t* tiles;
     int64_t q_stride[2], k_stride[2], v_stride[2], out_stride[2]; /* of a row and of a head, elements */
     float scale;
-    float reserved_f;
+    int32_t n_split;   /* workgroups that share a tile's keys, 1 .. 64 */
+    void* workspace;   /* nq_prompt_workspace() bytes, 16-byte aligned (n_split 1: none) */
+    int64_t workspace_bytes;
 } nq_prompt_desc;
 
 int32_t nq_prompt_tile_rows(void);
+int64_t nq_prompt_workspace(int32_t n_tiles, int32_t q_heads, int32_t head_dim, int32_t n_split);
 int nq_prompt_attention(const nq_prompt_desc* desc, void* stream);
 
 /*

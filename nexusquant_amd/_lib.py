@@ -96,7 +96,7 @@ class PromptDesc(ctypes.Structure):
         ("q", _P), ("k", _P), ("v", _P), ("out", _P), ("tiles", _P),
         ("q_stride", ctypes.c_int64 * 2), ("k_stride", ctypes.c_int64 * 2), ("v_stride", ctypes.c_int64 * 2),
         ("out_stride", ctypes.c_int64 * 2),
-        ("scale", ctypes.c_float), ("reserved_f", ctypes.c_float),
+        ("scale", ctypes.c_float), ("n_split", ctypes.c_int32), ("workspace", _P), ("workspace_bytes", ctypes.c_int64),
     ]
 
 
@@ -165,6 +165,7 @@ SIGNATURES = {
     "nq_nibble_pack": ([_P, _I64, _I32, _P, _P], ctypes.c_int),
     "nq_nibble_unpack": ([_P, _I64, _I32, _I32, _P, _P], ctypes.c_int),
     "nq_prompt_tile_rows": ([], ctypes.c_int32),
+    "nq_prompt_workspace": ([_I32, _I32, _I32, _I32], _I64),
     "nq_prompt_attention": ([_P, _P], ctypes.c_int),
     "nq_pool_copy_pages": ([ctypes.POINTER(Pool), _P, _P, _I32, _P], ctypes.c_int),
     "nq_pool_move_tokens": ([], ctypes.c_int32),

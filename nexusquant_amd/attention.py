@@ -68,7 +68,20 @@ def _rows(t: torch.Tensor):
 
 
 # nq_prompt_desc, packed in one go and passed as bytes (a call's host time counts for short prompts)
-_PACK = struct.Struct("6i5P8q2f")
+_PACK = struct.Struct("6i5P8qfiPq")
+
+
+# Few tiles and heads: several workgroups share a tile's keys, as many as run at once (two on a CU, at head_dim 256 one),
+# with _SPLIT_STAGES stages of 64 keys each at least.  us without and with, one prompt: 2188 tokens of 4 heads x 256 100
+# and 51, x 128 46 and 28, 8192 of one head 149 and 42, 4096 of 8 87 and 68, 700 of 8 x 64 14.2 and 13.8.
+_SPLIT_TO = {64: 512, 128: 512, 256: 256}
+_SPLIT_STAGES = 3
+_STAGE = 64
+
+
+def _splits(workgroups: int, keys: int, head_dim: int) -> int:
+    """Workgroups that share a tile's keys when the launch has `workgroups` without and tiles see up to `keys` keys."""
+    return max(1, min(_SPLIT_TO[head_dim] // workgroups, -(-keys // _STAGE) // _SPLIT_STAGES, 64))
 
 
 def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, plan: PromptPlan,
@@ -127,10 +140,18 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     v, v_at, v_row, v_head = _rows(value)
     o_row, o_head, _ = out.stride()
     window = 0 if sliding_window is None or int(sliding_window) >= max(plan.lengths) else int(sliding_window)
+    split, ws, nbytes = 1, None, 0
+    if plan.n_tiles * hq <= _SPLIT_TO[d] // 2:
+        longest = max(plan.lengths)
+        split = _splits(plan.n_tiles * hq, min(longest, window + 128) if window else longest, d)
+        if split > 1:
+            nbytes = lib.nq_prompt_workspace(plan.n_tiles, hq, d, split)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)  # of this call alone
     with on_device(dev):
         st = lib.nq_prompt_attention(_PACK.pack(
             hq, hkv, d, _lib.NQ_F16 if dtype == torch.float16 else _lib.NQ_BF16, plan.n_tiles, window, q_at, k_at, v_at,
-            out.data_ptr(), plan.tiles.address(), q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, scale, 0.0),
+            out.data_ptr(), plan.tiles.address(), q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, scale, split,
+            0 if ws is None else ws.data_ptr(), nbytes),
             _lib.current_stream_handle(dev))
     _lib.check(st, "nq_prompt_attention")
     return out

@@ -3,7 +3,13 @@
 //
 // A workgroup of 4 waves owns 128 consecutive queries of one sequence and head, 32 a wave,
 // and streams the 64-key stages that they see through two LDS buffers each for keys and
-// values (direct-to-LDS loads, under way while the other buffer is computed on).
+// values (direct-to-LDS loads, under way while the other buffer is computed on).  128 queries
+// and 64 keys are what two workgroups on a CU leave of registers and LDS at head_dim 128.
+//
+// What bounds it: at 16384 tokens of 32 / 8 heads x 128, 1030 TFLOP/s (2.12 ms); with half of the LDS
+// reads 6 % less, without exponentials 5 %, so nothing by itself.  At head_dim 64 exponentials
+// take half of the products' time (640 TFLOP/s), at 256 a SIMD holds one wave (590).  Short
+// prompts are bound by the latency of their few stages: 12 us for up to 190 tokens.
 #include "nq_flash.h"
 
 namespace nq {
@@ -21,6 +27,9 @@ struct PromptArgs {
     uint32_t hq, hkv;
     int32_t window;        // 0: none
     float c;               // scale * log2(e)
+    uint32_t n_split;      // workgroups that share a tile's keys
+    float* part_o;         // [workgroups, 128, D]: their sums
+    float* part_ml;        // [workgroups, 128, 2]: their maxima and sums of weights
 };
 
 constexpr int kWaitVm0 = 0x0f70;  // vmcnt(0), the other counters left open
@@ -102,7 +111,8 @@ __device__ __forceinline__ void sum_again(Rows<DT, D>& rows, const uint16_t* kb,
     }
 }
 
-template <int DT, int D>
+// SPLIT: a tile's stages go to n_split workgroups, whose sums prompt_join_kernel joins.
+template <int DT, int D, bool SPLIT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(PromptArgs a) {
     using T = Tile<D>;
     __shared__ __align__(16) char k0[kStage * T::ROWB];
@@ -113,12 +123,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     // kv heads fastest: blocks go to the XCDs in turn, so the query heads of a kv head meet in one
     // XCD's L2 when the kv heads are a multiple of 8
-    const uint32_t tile = blockIdx.x / a.hq, j = blockIdx.x % a.hq;
+    const uint32_t part = blockIdx.x / a.hq, j = blockIdx.x % a.hq, tile = SPLIT ? part / a.n_split : part;
     const uint32_t kh = j % a.hkv, head = kh * (a.hq / a.hkv) + j / a.hkv;
     const int32_t first = a.tiles[4 * tile], len = a.tiles[4 * tile + 1], q0 = a.tiles[4 * tile + 2];
     const int q_last = min(q0 + kPromptRows, len) - 1;
-    const int key0 = a.window ? max(q0 - a.window + 1, 0) & ~(kStage - 1) : 0;
-    const int n_stages = (q_last - key0) / kStage + 1;
+    int key0 = a.window ? max(q0 - a.window + 1, 0) & ~(kStage - 1) : 0;
+    int n_stages = (q_last - key0) / kStage + 1;
+    if constexpr (SPLIT) {
+        const int per = (n_stages + (int)a.n_split - 1) / (int)a.n_split, before = per * (int)(part - tile * a.n_split);
+        key0 += kStage * before;
+        n_stages = min(per, n_stages - before);
+        if (n_stages <= 0) {  // whole block: no keys
+            if (threadIdx.x < kPromptRows) *reinterpret_cast<f32x2*>(a.part_ml + 2 * ((size_t)blockIdx.x * kPromptRows + threadIdx.x)) = f32x2{kNoMax, 0.0f};
+            return;
+        }
+    }
     const int my0 = q0 + 32 * wave;               // this wave's first query
     const bool live = my0 < len;
     const int my_q = min(my0 + n, len - 1);
@@ -174,7 +193,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
     // loop of their own, two a turn: a branch between the two kinds in every stage made the compiler move all
     // of the output's registers twice a stage (32/8 heads x 16384 x 128 fp16: 2.47 ms with it).
     const int it0 = a.window ? max((q_last - a.window - key0 + kStage) / kStage, 0) : 0;
-    const int it1 = (q0 - key0) / kStage;
+    const int it1 = min((q0 - key0) / kStage, n_stages);  // (a part of the keys may end before the first query)
     int it = 0;
     while (it < n_stages) {
         if (!(it & 1) && it >= it0 && it + 1 < it1) {
@@ -190,8 +209,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
             ++it;
         }
     }
-    if (odd) sum_again<DT, D>(rows, kb, a.k_row, vb, a.v_row, a.c, key0, my_last, a.window ? my_q - a.window + 1 : 0, my_q, g);
+    if (odd) sum_again<DT, D>(rows, kb, a.k_row, vb, a.v_row, a.c, key0, SPLIT ? min(my_last, key0 + kStage * n_stages - 1) : my_last, a.window ? my_q - a.window + 1 : 0, my_q, g);
     if (!live || my0 + n >= len) return;
+    if constexpr (SPLIT) {
+        const size_t at = (size_t)blockIdx.x * kPromptRows + 32 * wave + n;
+        const float l = both_sum(rows.l);
+        if (g == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * at) = f32x2{rows.m, l};
+        float* const to = a.part_o + at * D + 4 * g;
+#pragma unroll
+        for (int b = 0; b < T::DB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f32x4*>(to + 32 * b + 8 * i) = f32x4{rows.o[b][4 * i], rows.o[b][4 * i + 1], rows.o[b][4 * i + 2], rows.o[b][4 * i + 3]};
+        return;
+    }
     const float r = 1.0f / both_sum(rows.l);
     uint16_t* const op = a.out + (first + (int64_t)my_q) * a.o_row + head * a.o_head + 4 * g;
 #pragma unroll
@@ -204,19 +235,65 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
         }
 }
 
-template <int DT>
-static hipError_t launch_prompt(int32_t d, const PromptArgs& a, uint32_t blocks, hipStream_t s) {
-    switch (d) {
-        case 64: hipLaunchKernelGGL((prompt_kernel<DT, 64>), dim3(blocks), dim3(256), 0, s, a); break;
-        case 128: hipLaunchKernelGGL((prompt_kernel<DT, 128>), dim3(blocks), dim3(256), 0, s, a); break;
-        default: hipLaunchKernelGGL((prompt_kernel<DT, 256>), dim3(blocks), dim3(256), 0, s, a); break;
+// The parts of a tile and head joined, in their order: 1024 / D rows a workgroup, four coordinates a lane.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a) {
+    constexpr int LANES = D / 4, ROWS = 256 / LANES, BLOCKS = kPromptRows / ROWS;
+    const uint32_t wg = blockIdx.x / BLOCKS, tile = wg / a.hq, j = wg % a.hq;
+    const uint32_t head = j % a.hkv * (a.hq / a.hkv) + j / a.hkv;
+    const int32_t first = a.tiles[4 * tile], len = a.tiles[4 * tile + 1], q0 = a.tiles[4 * tile + 2];
+    const int r = (int)(blockIdx.x % BLOCKS) * ROWS + (int)threadIdx.x / LANES, at = threadIdx.x % LANES;
+    if (q0 + r >= len) return;
+    const size_t row0 = ((size_t)tile * a.n_split * a.hq + j) * kPromptRows + r, step = (size_t)a.hq * kPromptRows;
+    float m = kNoMax, l = 0.0f;
+#pragma unroll 4
+    for (uint32_t s = 0; s < a.n_split; ++s) m = __builtin_fmaxf(m, a.part_ml[2 * (row0 + s * step)]);
+    f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (uint32_t s = 0; s < a.n_split; ++s) {
+        const size_t row = row0 + s * step;
+        const f32x2 ml = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * row);
+        const f32x4 o = *reinterpret_cast<const f32x4*>(a.part_o + row * D + 4 * at);
+        const float f = __builtin_amdgcn_exp2f(ml.x - m);
+        l = __builtin_fmaf(ml.y, f, l);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] = ml.y == 0.0f ? y[k] : __builtin_fmaf(o[k], f, y[k]);  // no keys: no sums are written
     }
+    const float d = 1.0f / l;
+    *reinterpret_cast<u32x2*>(a.out + (first + (int64_t)(q0 + r)) * a.o_row + head * a.o_head + 4 * at) =
+        u32x2{pack2<DT>(y[0] * d, y[1] * d), pack2<DT>(y[2] * d, y[3] * d)};
+}
+
+template <int DT, int D>
+static hipError_t launch_prompt(const PromptArgs& a, uint32_t blocks, hipStream_t s) {
+    if (a.n_split <= 1) {
+        hipLaunchKernelGGL((prompt_kernel<DT, D, false>), dim3(blocks), dim3(256), 0, s, a);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL((prompt_kernel<DT, D, true>), dim3(blocks * a.n_split), dim3(256), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((prompt_join_kernel<DT, D>), dim3(blocks * (kPromptRows * D / 1024)), dim3(256), 0, s, a);
     return hipGetLastError();
+}
+
+template <int DT>
+static hipError_t prompt_dims(int32_t d, const PromptArgs& a, uint32_t blocks, hipStream_t s) {
+    switch (d) {
+        case 64: return launch_prompt<DT, 64>(a, blocks, s);
+        case 128: return launch_prompt<DT, 128>(a, blocks, s);
+        default: return launch_prompt<DT, 256>(a, blocks, s);
+    }
 }
 
 }  // namespace nq
 
 extern "C" int32_t nq_prompt_tile_rows(void) { return nq::kPromptRows; }
+
+extern "C" int64_t nq_prompt_workspace(int32_t n_tiles, int32_t q_heads, int32_t head_dim, int32_t n_split) {
+    if (n_tiles <= 0 || q_heads <= 0 || head_dim <= 0 || n_split <= 1) return 0;
+    return (int64_t)n_tiles * q_heads * n_split * nq::kPromptRows * (head_dim + 2) * (int64_t)sizeof(float);
+}
 
 extern "C" int nq_prompt_attention(const nq_prompt_desc* d, void* stream) {
     using namespace nq;
@@ -238,7 +315,11 @@ extern "C" int nq_prompt_attention(const nq_prompt_desc* d, void* stream) {
                  "nq_prompt_attention: strides must keep rows 16-byte aligned (out: 8-byte)");
     NQ_CHECK_ARG(d->k_stride[0] >= 0 && d->k_stride[0] < (1 << 24) && d->v_stride[0] >= 0 && d->v_stride[0] < (1 << 24),
                  "nq_prompt_attention: rows of k and v must be less than 2^24 elements apart");
-    NQ_CHECK_ARG((uint64_t)d->n_tiles * d->q_heads <= max_blocks(256), "nq_prompt_attention: grid too large");
+    NQ_CHECK_ARG(d->n_split >= 1 && d->n_split <= 64, "nq_prompt_attention: n_split %d (1 .. 64)", d->n_split);
+    NQ_CHECK_ARG((uint64_t)d->n_tiles * d->q_heads * d->n_split <= max_blocks(256), "nq_prompt_attention: grid too large");
+    const int64_t need = nq_prompt_workspace(d->n_tiles, d->q_heads, d->head_dim, d->n_split);
+    NQ_CHECK_ARG(need == 0 || (d->workspace != nullptr && d->workspace_bytes >= need && ((uintptr_t)d->workspace & 15u) == 0),
+                 "nq_prompt_attention: a 16-byte aligned workspace of %lld bytes is needed", (long long)need);
     PromptArgs a = {};
     a.q = static_cast<const uint16_t*>(d->q);
     a.k = static_cast<const uint16_t*>(d->k);
@@ -258,8 +339,11 @@ extern "C" int nq_prompt_attention(const nq_prompt_desc* d, void* stream) {
     a.window = d->sliding_window;
     a.c = d->scale * 1.44269504088896340736f;
     const uint32_t blocks = (uint32_t)d->n_tiles * a.hq;
+    a.n_split = (uint32_t)d->n_split;
+    a.part_o = static_cast<float*>(d->workspace);
+    a.part_ml = a.part_o + (size_t)blocks * a.n_split * kPromptRows * d->head_dim;
     hipStream_t s = (hipStream_t)stream;
-    NQ_CHECK_HIP(d->dtype == NQ_F16 ? launch_prompt<NQ_F16>(d->head_dim, a, blocks, s)
-                                    : launch_prompt<NQ_BF16>(d->head_dim, a, blocks, s));
+    NQ_CHECK_HIP(d->dtype == NQ_F16 ? prompt_dims<NQ_F16>(d->head_dim, a, blocks, s)
+                                    : prompt_dims<NQ_BF16>(d->head_dim, a, blocks, s));
     return NQ_OK;
 }

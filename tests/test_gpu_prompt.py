@@ -1,7 +1,8 @@
 """Packed prompt attention against the formula in 64 bits.
 
 Tolerance: with u = eps(T) / 2 the kernel rounds each weight once (at most u of it) and each
-result once (u of it); logits are fp32 sums of D products, so a weight's exponent is off by at
+result once (u of it, or half a step of the type's subnormal numbers, which below finfo.tiny are
+tiny * eps apart whatever the result: 2^-25 for fp16); logits are fp32 sums of D products, so a weight's exponent is off by at
 most D 2^-24 of the sum of |q k| scale (twice, through the denominator); sums over n keys in
 fp32 and the exponential's 2^-22 are added.  Nothing else is rounded."""
 
@@ -30,7 +31,8 @@ def oracle(q, k, v, lens, scale, window):
             out[a:a + n, h] = p @ vv
             big = torch.where(seen, qq.abs() @ kk.abs().T * scale, 0.0).amax(-1, keepdim=True)
             rel = u + 2 * (q.shape[2] + 2) * 2 ** -24 * big + n * 2 ** -24 + 2 ** -21
-            tol[a:a + n, h] = rel * (p @ vv.abs()) + u * out[a:a + n, h].abs()
+            step = torch.finfo(q.dtype).tiny * u
+            tol[a:a + n, h] = rel * (p @ vv.abs()) + (u * out[a:a + n, h].abs()).clamp_min(step)
         a += n
     return out, tol
 
@@ -139,6 +141,33 @@ def test_layouts():
     assert torch.equal(wide[:, 2:6], want) and bool((wide[:, :2] == 3).all()) and bool((wide[:, 6:] == 3).all())
     one = k[:, :1].expand(-1, 2, -1)  # one stored head under two
     assert torch.equal(prompt_attention(q, one, one, plan), prompt_attention(q, one.contiguous(), one.contiguous(), plan))
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(1, 1, 64, torch.bfloat16), (2, 1, 128, torch.float16), (2, 2, 256, torch.bfloat16)])
+@pytest.mark.parametrize("lens,window", [([513], None), ([1300, 5, 0, 129], None), ([2500], 700), ([1000, 640], 1), ([1, 3000], None)])
+def test_few_tiles_share_their_keys(hq, hkv, d, dtype, lens, window):
+    from nexusquant_amd.attention import _splits, plan_prompts, prompt_attention
+    print(f"[gpu] prompt split {hq}/{hkv} d={d} {dtype} {lens} {window}", flush=True)
+    q, k, v = inputs(sum(lens), hq, hkv, d, dtype, seed=len(lens))
+    plan = plan_prompts(lens, device=DEV)
+    assert window or _splits(plan.n_tiles * hq, max(lens), d) > 1
+    want = check(q, k, v, lens, window=window)
+    assert torch.equal(prompt_attention(q, k, v, plan, sliding_window=window), want)  # joined in a fixed order
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = prompt_attention(q, k, v, plan, sliding_window=window)
+    for _ in range(2):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    # what the first half of the last sequence does not see (its last queries are summed again, in other roundings)
+    at = sum(lens) - lens[-1] // 2
+    if lens[-1] > 1:
+        ref, tol = oracle(q, k, v, lens, d ** -0.5, window)
+        v[at:, -1], k[at + 1:, -1] = float("inf"), float("nan")
+        got = prompt_attention(q, k, v, plan, sliding_window=window)
+        assert bool(((got.double() - ref).abs() <= tol)[:at].all()) and bool(got[at + 1:, -1].isnan().all())
 
 
 def test_output_in_place_of_the_query():

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from nexusquant_amd import _lib
-from nexusquant_amd.attention import _PACK, PromptPlan, plan_prompts, prompt_attention, prompt_tiles
+from nexusquant_amd.attention import PromptPlan, _PACK, _splits, plan_prompts, prompt_attention, prompt_tiles
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -56,7 +56,7 @@ def desc(**kw):
     two = ctypes.c_int64 * 2
     base = dict(q_heads=8, kv_heads=2, head_dim=128, dtype=_lib.NQ_F16, n_tiles=1, q=dummy, k=dummy, v=dummy, out=dummy,
                 tiles=dummy, q_stride=two(1024, 128), k_stride=two(256, 128), v_stride=two(256, 128),
-                out_stride=two(1024, 128), scale=0.1)
+                out_stride=two(1024, 128), scale=0.1, n_split=1)
     return _lib.PromptDesc(**{**base, **kw})
 
 
@@ -66,11 +66,20 @@ def desc(**kw):
     dict(tiles=None), dict(out=ctypes.c_void_p(4100)), dict(v=ctypes.c_void_p(4104)),
     dict(k_stride=(ctypes.c_int64 * 2)(260, 128)), dict(out_stride=(ctypes.c_int64 * 2)(1024, 130)),
     dict(k_stride=(ctypes.c_int64 * 2)(1 << 24, 128)), dict(v_stride=(ctypes.c_int64 * 2)(-256, 128)),
-    dict(n_tiles=1 << 24), dict(q_heads=1 << 30, kv_heads=1)])
+    dict(n_tiles=1 << 24), dict(q_heads=1 << 30, kv_heads=1), dict(n_split=0), dict(n_split=65), dict(n_split=2),
+    dict(n_split=2, workspace=ctypes.c_void_p(4096), workspace_bytes=100),
+    dict(n_split=2, workspace=ctypes.c_void_p(4100), workspace_bytes=1 << 30)])
 def test_c_entry_refuses(kw):
     lib = _lib.load()
     assert lib.nq_prompt_attention(ctypes.byref(desc(**kw)), None) == -1
     assert lib.nq_last_error().startswith(b"nq_prompt_attention")
+
+
+@pytest.mark.parametrize("workgroups,keys,d,want", [(1, 64, 128, 1), (1, 511, 64, 2), (1, 1 << 20, 128, 64), (64, 4096, 128, 8),
+                                                    (128, 4096, 64, 4), (128, 4096, 256, 2), (100, 4096, 256, 2),
+                                                    (129, 4096, 256, 1), (72, 500, 128, 2), (72, 200, 128, 1)])
+def test_how_many_workgroups_share_a_tiles_keys(workgroups, keys, d, want):
+    assert _splits(workgroups, keys, d) == want
 
 
 def test_c_entry_takes_an_empty_batch():
