@@ -147,17 +147,23 @@ class CompressedPagePool:
             p = np.asarray(pages).reshape(-1)
             if len(p) and p.dtype.kind not in "iu":
                 raise ValueError(f"page numbers must be integers, got {p.dtype}")
-            p = p.astype(np.int64, copy=False)
-        # a negative number is a large one as unsigned
-        if len(p) and p.view(np.uint32 if p.dtype == np.int32 else np.uint64).max() >= self.num_pages:
+            if len(p) and (p.min() < 0 or p.max() >= self.num_pages):
+                raise ValueError(f"page numbers must lie in [0, {self.num_pages})")
+            return p.astype(np.int32, copy=False)
+        if len(p) and p.view(np.uint32).max() >= self.num_pages:  # a negative number is a large one as unsigned
             raise ValueError(f"page numbers must lie in [0, {self.num_pages})")
-        return p.astype(np.int32, copy=False)
+        return p
+
+    def _referenced(self, p: np.ndarray, what: str) -> np.ndarray:
+        refs = self._refs[p]
+        if len(p) and refs.min() < 1:
+            raise ValueError(f"{what}: page {int(p[refs < 1][0])} is not allocated")
+        return refs
 
     def in_use(self, pages, what: str = "pages") -> np.ndarray:
         """The page numbers as an array; raises unless all are allocated."""
         p = self._pages(pages)
-        if len(p) and self._refs[p].min() < 1:
-            raise ValueError(f"{what}: page {int(p[self._refs[p] < 1][0])} is not allocated")
+        self._referenced(p, what)
         return p
 
     def _tally(self, p: np.ndarray):
@@ -198,7 +204,7 @@ class CompressedPagePool:
         """One more reference to each page (to a page listed twice: two)."""
         with self._lock:
             p, n = self._tally(self._pages(pages))
-            self._refs[self.in_use(p, "retain")] += n
+            self._refs[p] = self._referenced(p, "retain") + n
 
     def free(self, pages: Sequence[int]) -> None:
         """Drop one reference of each page (of a page listed twice: two); pages without any can be
@@ -298,9 +304,9 @@ class CompressedPagePool:
                 if had[b] < 0 or self.pages_for(had[b]) != sizes[b]:
                     raise ValueError(f"compact: {had[b]} tokens take {self.pages_for(max(had[b], 0))} pages, "
                                      f"got {sizes[b]}")
-            flat = self.in_use([p for t in tables for p in t] if batch != 1 else tables[0], "compact")
+            flat = self._pages([p for t in tables for p in t] if batch != 1 else tables[0])
             held, times = self._tally(flat)
-            if len(held) and (self._refs[held] < times).any():
+            if (self._referenced(held, "compact") < times).any():
                 raise ValueError("compact: a page stands in more tables than it has references")
             counts = [int(x) for x in (n_kept.tolist() if torch.is_tensor(n_kept) else n_kept)]
             if len(counts) != batch:
