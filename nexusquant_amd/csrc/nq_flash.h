@@ -177,21 +177,6 @@ struct Rows {
         }
     }
 
-    // Whether a tile of values holds an infinity or a NaN.  A hidden key's weight is zero, but zero
-    // times such a value is NaN, so a tile that hides keys must not hold one for the product above.
-    __device__ __forceinline__ bool tile_odd(const char* vbuf, int t, int lane) const {
-        constexpr uint32_t kExp = DT == NQ_F16 ? 0x7c00u : 0x7f80u;
-        uint32_t odd = 0;
-#pragma unroll
-        for (int i = 0; i < T::UPR / 2; ++i) {  // the tile's 4 D dwords, whichever lane reads which
-            const u32x4 v = *reinterpret_cast<const u32x4*>(vbuf + 32 * t * T::ROWB + 1024 * i + 16 * lane);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) odd |= (uint32_t)((v[k] & kExp) == kExp) | (uint32_t)((v[k] & (kExp << 16)) == (kExp << 16));
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        return __any((int)odd);
-    }
-
     // tiles t and t + 1, which every query sees whole
     template <bool SCALED = false>
     __device__ __forceinline__ void two_tiles(const char* kbuf, const char* vbuf, int t, float c, int g, const float* v = nullptr) {
