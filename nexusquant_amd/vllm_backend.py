@@ -862,8 +862,8 @@ class NexusQuantPagedAttention:
             raise ValueError(f"pool head_dim {pool.head_dim} != compressor head_dim {self.compressor.head_dim}")
         if out is None:
             out = torch.empty(shape, dtype=dtype, device=dev)
-        elif out.shape != shape or out.dtype != dtype or out.device != dev or not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous {dtype} tensor {tuple(shape)} on {dev}")
+        elif out.shape != shape or out.dtype != dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 8:
+            raise ValueError(f"out must be a contiguous, 8-byte aligned {dtype} tensor {tuple(shape)} on {dev}")
         q = query.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()

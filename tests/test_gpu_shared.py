@@ -288,6 +288,7 @@ def test_refusals():
                  lambda: attn.run_shared(plan, q[..., :32]), lambda: attn.run_shared(plan, q.expand(2, -1, -1)),
                  lambda: attn.run_shared(plan, q, layer=2), lambda: attn.run_shared(plan, q, layer=-1),
                  lambda: attn.run_shared(plan, q, out=torch.empty_like(q.float())),
+                 lambda: attn.run_shared(plan, q, out=torch.empty(257, dtype=torch.float16, device=DEV)[1:].view(1, 4, 64)),
                  lambda: attn.run_shared(plan, queries(1, 2 * 257, 64, torch.float16))):
         with pytest.raises(ValueError):
             call()

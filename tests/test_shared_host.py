@@ -172,7 +172,7 @@ def test_shared_struct_matches_the_c_compiler(tmp_path):
     (dict(layer=1), {}), (dict(layer=-1), {}), (dict(batch=-1), {}), (dict(q_heads=0), {}), (dict(q_heads=3), {}),
     (dict(q_heads=2 * 257), {}), (dict(q_dtype=_lib.NQ_F32), {}), (dict(n_items=-1), {}), (dict(n_slots=0), {}), (dict(n_many=2), {}), (dict(n_many=-1), {}),
     (dict(n_few=2), {}), (dict(n_few=-1), {}), (dict(n_few=1, n_many=1), {}), (dict(n_few=1, q_heads=34), {}),
-    (dict(query=None), {}), (dict(query=ctypes.c_void_p(4104)), {}), (dict(out=None), {}), (dict(items=None), {}),
+    (dict(query=None), {}), (dict(query=ctypes.c_void_p(4104)), {}), (dict(out=None), {}), (dict(out=ctypes.c_void_p(4100)), {}), (dict(items=None), {}),
     (dict(row_slots=None), {}), (dict(rope_sin_minus_cos=None), {}), (dict(rope_n_pos=0), {}),
     (dict(workspace=None), {}), (dict(workspace_bytes=100), {}), (dict(workspace=ctypes.c_void_p(4100)), {}),
     (dict(scale_divisor=0.0), {}), (dict(n_items=1 << 30), {}), (dict(batch=1 << 30), {}),
