@@ -23,7 +23,7 @@ import array
 import ctypes
 import struct
 import threading
-from typing import List, Optional, Sequence, Tuple
+from typing import List, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -235,14 +235,6 @@ class CompressedPagePool:
                 raise ValueError(f"copy_pages: page {int(d[self._refs[d] > 1][0])} is shared and cannot be written")
             self._copy(s.tolist(), d.tolist())
 
-    def _sequence(self, pages, length: int, what: str) -> Tuple[np.ndarray, int]:
-        p, length = self.in_use(pages, what), int(length)
-        if length < 0 or self.pages_for(length) != len(p):
-            raise ValueError(f"{what}: {length} tokens take {self.pages_for(max(length, 0))} pages, got {len(p)}")
-        if len(self._tally(p)[0]) != len(p):
-            raise ValueError(f"{what}: a page stands twice in one sequence")
-        return p, length
-
     def fork(self, pages: Sequence[int], length: int, n: int = 1) -> List[List[int]]:
         """Page lists of n branches of the sequence (`pages` holding `length` tokens).
 
@@ -256,9 +248,9 @@ class CompressedPagePool:
             p = self.in_use(pages, "fork")
             if length < 0 or self.pages_for(length) != len(p):
                 raise ValueError(f"fork: {length} tokens take {self.pages_for(max(length, 0))} pages, got {len(p)}")
-            if len(self._tally(p)[0]) != len(p):
-                raise ValueError("fork: a page stands twice in one sequence")
             table = pages if type(pages) is list else p.tolist()
+            if len(set(table)) != len(table):
+                raise ValueError("fork: a page stands twice in one sequence")
             if length % self.page_tokens == 0:
                 self._refs[p] += n
                 return [list(table) for _ in range(n)]
