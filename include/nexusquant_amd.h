@@ -689,8 +689,8 @@ int nq_pool_write(const nq_pool* pool, int32_t layer, const nq_pool* tokens, con
  *            first chunk
  *   row_slots [batch + 1] each row's slots, one per chunk that it sees
  *            (every slot is written by exactly one item)
- * Device int32 arrays.  query, out: [batch, q_heads, head_dim], fp16 or bf16;
- * a row without slots is zero.  Rounding: keys to fp16; queries of bf16 to
+ * Device int32 arrays.  query, out: [batch, q_heads, head_dim], fp16 or bf16,
+ * 16- and 8-byte aligned; a row without slots is zero.  Rounding: keys to fp16; queries of bf16 to
  * fp16 after a power of two is taken out; softmax weights times the values'
  * scales to fp16 (kind 2: to twice fp16's 11 bits); sums in fp32.
  * workspace: nq_shared_attention_workspace(n_slots, q_heads, head_dim) bytes,

@@ -94,7 +94,8 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     projection are read in place.  scale: 1 / sqrt(head_dim) by default.  sliding_window: query i sees
     keys i - window < j <= i.
     Returns [rows, q_heads, head_dim].  Rows behind the plan's sequences are left as they are in `out`,
-    and are zero without one; `out` may be `query`, and must not overlap key or value.  Inference only: tensors that require a gradient are refused."""
+    and are zero without one; `out` may be `query`, and must not overlap key or value.  Inference only:
+    tensors that require a gradient are refused."""
     lib = _lib.load()
     for name, t in (("query", query), ("key", key), ("value", value)):
         if not t.is_cuda:

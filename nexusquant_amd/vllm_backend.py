@@ -649,7 +649,7 @@ class NexusQuantPagedAttention:
         self.compressor = compressor
         self._block_pool: dict = {}
         self._next_block_id: int = 0
-        self._tables: Optional[tuple] = None  # (largest position, device, merged rotation tables) of run_shared
+        self._tables: Dict[torch.device, _SharedTables] = {}  # of run_shared
 
     def allocate_block(self) -> int:
         block_id = self._next_block_id
@@ -804,9 +804,9 @@ class NexusQuantPagedAttention:
     def plan_shared(self, pool, block_tables: Sequence[Sequence[int]], context_lens,
                     min_saved: Optional[int] = None) -> SharedAttentionPlan:
         """The plan of rows over a CompressedPagePool: row b attends to the first context_lens[b] tokens of
-        its pages block_tables[b] (0: none; entries past those tokens are padding).  Full pages that several rows begin with, as forks do, are
-        read and decoded once for all of them, where that saves min_saved tokens' decoding (None: what pays,
-        65536 over the pool's heads)."""
+        its pages block_tables[b] (0: none; entries past those tokens are padding).  Full pages that several
+        rows begin with, as forks do, are read and decoded once for all of them, where that saves min_saved
+        tokens' decoding (None: what pays, 65536 over the pool's heads)."""
         if pool.head_dim != self.compressor.head_dim:
             raise ValueError(f"pool head_dim {pool.head_dim} != compressor head_dim {self.compressor.head_dim}")
         ctx = [int(x) for x in (context_lens.tolist() if torch.is_tensor(context_lens) else context_lens)]
@@ -822,13 +822,13 @@ class NexusQuantPagedAttention:
             min_saved = -(-_MIN_SAVED // pool.num_heads)
         return SharedAttentionPlan(pool, len(ctx), shared_segments(tables, ctx, pool.page_tokens, min_saved))
 
-    def _shared_tables(self, max_position: int, dev):
-        """The merged rotation tables, kept here until a larger position needs longer ones."""
-        got = self._tables
-        if got is None or got[0] < max_position or got[1] != dev:
+    def _shared_tables(self, max_position: int, dev) -> _SharedTables:
+        """A device's merged rotation tables, kept here until a larger position needs longer ones."""
+        got = self._tables.get(dev)
+        if got is None or got.args[2] <= max_position:
             _, _, dm, dp = self.compressor._tables(max_position, dev)
-            got = self._tables = (dm.shape[0] - 1, dev, _SharedTables(dm, dp))
-        return got[2]
+            got = self._tables[dev] = _SharedTables(dm, dp)
+        return got
 
     def run_shared(self, plan: SharedAttentionPlan, query: torch.Tensor, layer: int = 0,
                    out: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -156,6 +156,24 @@ def test_plan_refuses_bad_tables(monkeypatch):
         attn.run_shared(SharedAttentionPlan(pool, 1, []), torch.zeros(1, 3, 64))
 
 
+def test_rotation_tables_are_kept_by_device_and_grow(monkeypatch):
+    attn = NexusQuantPagedAttention(NexusQuantKVCompressor(head_dim=64))
+    made = []
+
+    def tables(max_position, dev):
+        made.append((max_position, dev))
+        n = -(-(max_position + 1) // 4096) * 4096
+        return None, None, torch.zeros(n, 1), torch.zeros(n, 1)
+    monkeypatch.setattr(attn.compressor, "_tables", tables)
+    a, b = torch.device("cuda", 0), torch.device("cuda", 1)
+    one, two = attn._shared_tables(100, a), attn._shared_tables(4095, b)
+    for _ in range(3):  # pools on two devices in turn
+        assert attn._shared_tables(4095, a) is one and attn._shared_tables(7, b) is two
+    assert len(made) == 2 and one.args[2] == 4096
+    assert attn._shared_tables(4096, a).args[2] == 8192 and attn._shared_tables(5000, a).args[2] == 8192
+    assert len(made) == 3
+
+
 def test_shared_struct_matches_the_c_compiler(tmp_path):
     names = [f[0] for f in _lib.SharedDesc._fields_]
     prog = ["#include <stddef.h>", "#include <stdio.h>", f'#include "{ROOT}/include/nexusquant_amd.h"', "int main(void){",
