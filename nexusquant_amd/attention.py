@@ -127,7 +127,7 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     if not 0.0 < scale < 1e30:
         raise ValueError(f"scale must be positive, got {scale}")
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=dev)
+        out = query.new_empty(shape)
         if rows > plan.rows:
             out[plan.rows:].zero_()
     elif (out.shape != shape or out.dtype != dtype or out.device != dev

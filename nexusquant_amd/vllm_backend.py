@@ -860,13 +860,13 @@ class NexusQuantPagedAttention:
             raise ValueError(f"layer {layer} of a pool of {pool.num_layers}")
         if pool.head_dim != self.compressor.head_dim:
             raise ValueError(f"pool head_dim {pool.head_dim} != compressor head_dim {self.compressor.head_dim}")
-        if out is None:
-            out = torch.empty(shape, dtype=dtype, device=dev)
-        elif out.shape != shape or out.dtype != dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 8:
-            raise ValueError(f"out must be a contiguous, 8-byte aligned {dtype} tensor {tuple(shape)} on {dev}")
         q = query.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()
+        if out is None:
+            out = torch.empty_like(q)
+        elif out.shape != shape or out.dtype != dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 8:
+            raise ValueError(f"out must be a contiguous, 8-byte aligned {dtype} tensor {tuple(shape)} on {dev}")
         # of this call alone: calls on other streams and captured graphs have their own
         ws = torch.empty(nbytes or 16, dtype=torch.uint8, device=dev)
         tables = self._shared_tables(pool.max_position, dev)
