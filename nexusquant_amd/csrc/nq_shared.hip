@@ -551,7 +551,9 @@ shared_attn_kernel(SharedArgs a) {
     signs.init(lane);
     __syncthreads();
     const int vexp = value_exponent<NW>(s_max);
-    for (int i = threadIdx.x; i < n_slots; i += NT) s_vs[i] = __builtin_ldexpf(s_vs[i], vexp);  // used after the next barrier
+    for (int i = threadIdx.x; i < n_slots; i += NT) s_vs[i] = __builtin_ldexpf(s_vs[i], vexp);
+    // Other waves use them: MANY behind the barrier after its first decode, the others' waves may go on by themselves.
+    if constexpr (!MANY) __syncthreads();
 
     // The stage at s0 to LDS: its codes are in registers, and those of the stage after it follow.
     auto decode = [&](int s0, char* kbuf) {

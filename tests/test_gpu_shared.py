@@ -358,3 +358,22 @@ def test_wide_workgroups(heads, group, d, rows, prefix):
     tables, ctx = forks(pool, prefix, [7 * i % 90 for i in range(rows)])
     plan, _ = check(attention(d), pool, tables, ctx, queries(rows, heads * group, d, torch.float16, seed=rows))
     assert plan.work(heads * group)[1][1] > 0  # items of many rows
+
+
+@pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16), (128, torch.float16), (256, torch.bfloat16)])
+@pytest.mark.parametrize("heads,group,rows,prefix", [(8, 4, 8, 1040), (2, 17, 1, 2100), (2, 16, 2, 515), (1, 32, 1, 130),
+                                                     (8, 1, 31, 4100)])
+def test_seventeen_to_thirty_two_query_rows(heads, group, rows, prefix, d, dtype):
+    """Every wave of a workgroup has all of these rows and goes on by itself: what the others stored for it (places,
+    scales in units of the chunk's largest) must be there.  (Outputs of fp16 stay clear of its subnormals.)"""
+    print(f"[gpu] shared alone {heads}x{group} d={d} {dtype} rows={rows} prefix={prefix}", flush=True)
+    for scale_mul in (2.0 ** -12 if dtype == torch.bfloat16 else 2000.0, 1.0):
+        pool = make_pool(1, prefix // 16 + 2 + 8 * rows, heads, 16, d, seed=rows, scale_mul=scale_mul)
+        tables, ctx = forks(pool, prefix, [11 * i % 70 for i in range(rows)])
+        q = queries(rows, heads * group, d, dtype, seed=prefix)
+        plan, want = check(attention(d), pool, tables, ctx, q)
+        items = plan.work(heads * group)[1]
+        assert items[1] == 0 and items[0] > items[2]  # some are of neither many rows nor few
+        attn = attention(d)
+        for _ in range(3):
+            assert torch.equal(attn.run_shared(plan, q), want)
