@@ -13,6 +13,7 @@
 #pragma once
 
 #include "nq_common.h"
+#include "nq_tile.h"
 
 namespace nq {
 namespace flash {
@@ -75,22 +76,6 @@ __device__ __forceinline__ float both_sum(float v) {
 }
 
 __device__ __forceinline__ int acc_row(int j, int g) { return 8 * (j >> 2) + 4 * g + (j & 3); }
-
-// A tile's LDS layout: row r (a key) at byte r * 2 D, its 16-byte chunk c at chunk place
-// c ^ f(r).  Keys are read 32 rows at one chunk (ds_read_b128), values 4 rows at 64 bytes
-// (transposing ds_read_b64); each f spreads its read over all 64 banks.
-template <int D>
-struct Tile {
-    static constexpr int ROWB = 2 * D;
-    static constexpr int UPR = D / 8;           // 16-byte chunks a row
-    static constexpr int KS = D / 16;           // MFMA steps of a logit
-    static constexpr int DB = D / 32;           // 32-coordinate blocks of the output
-    static __device__ __forceinline__ int key_swizzle(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
-    // (its bit 0 is for writers of two chunks a lane: half of their rows then take the odd one first)
-    static __device__ __forceinline__ int value_swizzle(int r) {
-        return (D == 64 ? 4 * ((r >> 1) & 1) : 4 * (r & 3)) ^ ((r >> 2) & 1);
-    }
-};
 
 template <int DT, int D>
 struct Rows {

@@ -36,35 +36,31 @@ constexpr int kWaitVm0 = 0x0f70;  // vmcnt(0), the other counters left open
 constexpr int kPromptRows = 128;
 constexpr int kStage = 64;        // keys of a stage: two tiles
 
-// Rows row0 .. row0 + 63 of one head to LDS in Tile's layout, 16 bytes a lane: load i fills the 64
-// slots from 64 (4 i + wave) on.  A lane's rows of successive loads are 2048 / D apart, at the same
-// chunk (but for bit 3 of a key's at D = 256), so a whole stage is a uniform address plus a fixed lane
-// offset.  In the sequence's last stage rows past its end repeat its last one (their weights are
-// zero, and what lies behind the sequence is never read).
+// Rows row0 .. row0 + 63 of one head to LDS in Tile's layout (StagePieces), 16 bytes a lane.  A whole stage
+// is a uniform address plus a lane's fixed offsets.  In the sequence's last stage rows past its end repeat
+// its last one (their weights are zero, and what lies behind the sequence is never read).
 template <int D, bool VALUES>
 struct StageLoad {
     using T = Tile<D>;
-    static constexpr int STEP = 256 / T::UPR;  // rows
-    int row, chunk;
-    uint32_t off;
+    using P = StagePieces<D, VALUES>;
+    int thread;
+    uint32_t off[P::PERIOD];
     __device__ __forceinline__ void init(int wave, int lane, int64_t stride) {
-        const int slot = 64 * wave + lane;
-        row = slot / T::UPR;
-        chunk = (slot % T::UPR) ^ (VALUES ? T::value_swizzle(row) : T::key_swizzle(row));
-        off = (uint32_t)row * (uint32_t)(2 * stride) + 16u * chunk;
+        thread = 64 * wave + lane;
+#pragma unroll
+        for (int i = 0; i < P::PERIOD; ++i) off[i] = P::offset(thread, i, stride);
     }
-    static __device__ __forceinline__ uint32_t flip(int i) { return !VALUES && D == 256 ? 8u * (i & 1) : 0u; }
     __device__ __forceinline__ void operator()(const uint16_t* base, int64_t stride, int row0, int n, char* buf, int wave) const {
         if (row0 + kStage <= n) {
             const char* const from = reinterpret_cast<const char*>(base + (int64_t)row0 * stride);
 #pragma unroll
             for (int i = 0; i < T::UPR / 4; ++i)
-                __builtin_amdgcn_global_load_lds((global_void*)(from + (int64_t)(STEP * i) * 2 * stride + (off ^ (16u * flip(i)))),
+                __builtin_amdgcn_global_load_lds((global_void*)(from + (int64_t)(P::STEP * i) * 2 * stride + off[i % P::PERIOD]),
                                                  (lds_void*)(buf + 1024 * (4 * i + wave)), 16, 0, 0);
         } else {
 #pragma unroll
             for (int i = 0; i < T::UPR / 4; ++i) {
-                const uint16_t* const src = base + (int64_t)min(row0 + row + STEP * i, n - 1) * stride + 8 * (chunk ^ flip(i));
+                const uint16_t* const src = base + (int64_t)min(row0 + P::row(thread, i), n - 1) * stride + 8 * P::chunk(thread, i);
                 __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(buf + 1024 * (4 * i + wave)), 16, 0, 0);
             }
         }

@@ -232,3 +232,27 @@ def test_refusals():
     with pytest.raises(NexusQuantError):
         prompt_attention(q, k.cpu(), v, plan)
     assert prompt_attention(q[:0], k[:0], v[:0], plan_prompts([0, 0], device=DEV)).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("d,widths", [(256, (264, 320)), (256, (832, 1032)), (256, (384, 256)), (128, (136, 200)), (64, (72, 104))])
+@pytest.mark.parametrize("hq,hkv,lens", [(1, 1, [513]), (2, 2, [700, 0, 65]), (34, 2, [450, 130])])
+def test_row_strides_of_any_multiple_of_eight(d, widths, hq, hkv, lens):
+    """Keys and values in wider rows: the same bytes read, so the same results as from rows next to one another."""
+    from nexusquant_amd.attention import _SPLIT_TO, plan_prompts, prompt_attention
+    print(f"[gpu] prompt strides d={d} {widths} {hq}/{hkv} {lens}", flush=True)
+    q, k, v = inputs(sum(lens), hq, hkv, d, torch.float16, seed=d + hq)
+    plan = plan_prompts(lens, device=DEV)
+    assert (plan.n_tiles * hq <= _SPLIT_TO[d] // 2) == (hq < 34 or d < 256)
+    want = check(q, k, v, lens)
+
+    def padded(x, width, pad):
+        wide = torch.full((x.shape[0], hkv * width + pad), 5.0, dtype=x.dtype, device=DEV)
+        y = wide[:, :hkv * width].view(x.shape[0], hkv, width)[..., :d]
+        y.copy_(x)
+        assert y.stride() == (hkv * width + pad, width, 1)
+        return y
+    for pad in (0, 8, 40):
+        for window in (None, 100):
+            ref = want if window is None else prompt_attention(q, k, v, plan, sliding_window=window)
+            got = prompt_attention(q, padded(k, widths[0], pad), padded(v, widths[1], pad), plan, sliding_window=window)
+            assert torch.equal(got, ref), (pad, window)

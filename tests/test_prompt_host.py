@@ -86,3 +86,38 @@ def test_c_entry_takes_an_empty_batch():
     lib = _lib.load()
     assert lib.nq_prompt_attention(ctypes.byref(desc(n_tiles=0, q=None, tiles=None)), None) == 0
     assert lib.nq_prompt_attention(None, None) == -1
+
+
+def test_a_stages_pieces_come_from_their_rows_whatever_the_stride(tmp_path):
+    """Every lane's piece of every load of a stage, replayed through the kernel's own formulas: its place in LDS holds
+    the chunk that the readers' layout wants there, read at row * stride + chunk."""
+    (tmp_path / "p.cpp").write_text("""
+#include <stdio.h>
+#include "nq_tile.h"
+using namespace nq::flash;
+template <int D, bool VALUES> int check(long long stride) {
+    using P = StagePieces<D, VALUES>;
+    int bad = 0;
+    for (int i = 0; i < Tile<D>::UPR / 4; ++i)
+        for (int s = 0; s < 256; ++s) {
+            const int place = 256 * i + s, row = place / Tile<D>::UPR;
+            const int chunk = place % Tile<D>::UPR ^ (VALUES ? Tile<D>::value_swizzle(row) : Tile<D>::key_swizzle(row));
+            const long long want = 2 * stride * row + 16 * chunk;
+            bad += 2 * stride * P::STEP * i + (long long)P::offset(s, i % P::PERIOD, stride) != want;  // a whole stage's
+            bad += 2 * (stride * P::row(s, i) + 8 * P::chunk(s, i)) != want;                           // the last one's
+        }
+    return bad;
+}
+int main(void) {
+    int bad = 0;
+    const long long strides[] = {0, 64, 72, 128, 136, 256, 264, 320, 384, 832, 1032, 8200, (1 << 24) - 8};
+    for (long long s : strides)
+        bad += check<64, false>(s) + check<64, true>(s) + check<128, false>(s) + check<128, true>(s) + check<256, false>(s) +
+               check<256, true>(s);
+    printf("%d\\n", bad);
+    return bad != 0;
+}
+""")
+    subprocess.check_call(["g++", "-std=c++17", "-I", os.path.join(ROOT, "nexusquant_amd", "csrc"), "-o", str(tmp_path / "p"),
+                           str(tmp_path / "p.cpp")])
+    assert subprocess.run([str(tmp_path / "p")], capture_output=True, text=True).stdout == "0\n"
