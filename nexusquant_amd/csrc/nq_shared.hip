@@ -691,7 +691,8 @@ shared_attn_kernel(SharedArgs a) {
             if (alone) asm volatile("" ::: "memory");
             else __syncthreads();
             attend(s0, s_kv[0]);
-            if (alone) asm volatile("" ::: "memory");
+            // the next stage's tables come by DMA into the rows that were read here, in no order with these reads
+            if (alone) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             else __syncthreads();
         }
         if (alone) __syncthreads();  // the sums go over the other waves' stages
