@@ -615,7 +615,7 @@ class SharedAttentionPlan:
         self.batch = batch
         self.segments = segments
         self._work: Dict[int, tuple] = {}
-        self._tables: list = []  # rotation tables that calls with this plan have read: a captured graph goes on reading them
+        self._tables: Dict[int, _SharedTables] = {}  # by id, each once, however many attentions use the plan in turn
 
     def work(self, q_heads: int):
         """(device ints, what nq_shared_desc holds that all calls share: counts, the arrays' places in the ints, factors
@@ -640,6 +640,11 @@ class SharedAttentionPlan:
             got = self._work[q_heads] = (ints, counts, places, (hadamard_constant(d), float(np.float32(math.sqrt(d)))),
                                          int(lib.nq_shared_attention_workspace(counts[-1], q_heads, d)))
         return got
+
+    def reads(self, tables: _SharedTables):
+        """Arguments of a call that reads these tables.  They are kept with the plan: a captured graph goes on reading them."""
+        self._tables[id(tables)] = tables
+        return tables.args
 
 
 class NexusQuantPagedAttention:
@@ -870,9 +875,7 @@ class NexusQuantPagedAttention:
         # of this call alone: calls on other streams and captured graphs have their own
         ws = torch.empty(nbytes or 16, dtype=torch.uint8, device=dev)
         tables = self._shared_tables(pool.max_position, dev)
-        if not plan._tables or plan._tables[-1] is not tables:
-            plan._tables.append(tables)
-        dm, dp, n_pos = tables.args
+        dm, dp, n_pos = plan.reads(tables)
         items, pages, seg_rows, row_slots = places
         with on_device(dev):
             base = ints.address()

@@ -377,3 +377,19 @@ def test_seventeen_to_thirty_two_query_rows(heads, group, rows, prefix, d, dtype
         attn = attention(d)
         for _ in range(3):
             assert torch.equal(attn.run_shared(plan, q), want)
+
+
+def test_two_attentions_over_one_plan():
+    """Layers of local and global rotation: each attention reads its own tables, and the plan keeps one of each."""
+    from nexusquant_amd.vllm_backend import NexusQuantKVCompressor, NexusQuantPagedAttention
+    print("[gpu] shared two attentions", flush=True)
+    pool = make_pool(1, 60, 2, 16, 64, seed=13)
+    tables, ctx = forks(pool, 400, [5, 60])
+    one, two = attention(64), NexusQuantPagedAttention(NexusQuantKVCompressor(head_dim=64, bits=3, rope_base=10000.0))
+    q = queries(2, 8, 64, torch.float16)
+    plan, want = check(one, pool, tables, ctx, q)
+    other = two.run_shared(plan, q)
+    assert not torch.equal(other, want)
+    for _ in range(20):
+        assert torch.equal(one.run_shared(plan, q), want) and torch.equal(two.run_shared(plan, q), other)
+    assert len(plan._tables) == 2

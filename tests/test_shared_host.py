@@ -10,7 +10,7 @@ import torch
 
 from nexusquant_amd import _lib
 from nexusquant_amd.vllm_backend import (_SHARED_PACK, NexusQuantKVCompressor, NexusQuantPagedAttention,
-                                         SharedAttentionPlan, shared_items, shared_segments)
+                                         SharedAttentionPlan, _SharedTables, shared_items, shared_segments)
 
 from test_page_pool import c_pool, host_pool
 
@@ -172,6 +172,15 @@ def test_rotation_tables_are_kept_by_device_and_grow(monkeypatch):
     assert len(made) == 2 and one.args[2] == 4096
     assert attn._shared_tables(4096, a).args[2] == 8192 and attn._shared_tables(5000, a).args[2] == 8192
     assert len(made) == 3
+
+
+def test_a_plan_keeps_each_table_once():
+    """Two attentions (local and global rotation bases) that use one plan in turn: a table for each, not for each call."""
+    plan = SharedAttentionPlan(None, 1, [])
+    one, two = (_SharedTables(torch.zeros(4096, 1), torch.zeros(4096, 1)) for _ in range(2))
+    for _ in range(50):
+        assert plan.reads(one) == one.args and plan.reads(two) == two.args
+    assert list(plan._tables.values()) == [one, two]
 
 
 def test_shared_struct_matches_the_c_compiler(tmp_path):
