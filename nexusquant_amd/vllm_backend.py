@@ -654,7 +654,7 @@ class NexusQuantPagedAttention:
         self.compressor = compressor
         self._block_pool: dict = {}
         self._next_block_id: int = 0
-        self._tables: Dict[torch.device, _SharedTables] = {}  # of run_shared
+        self._tables: Dict[tuple, _SharedTables] = {}  # of run_shared, by (device, head_dim, rope_base)
 
     def allocate_block(self) -> int:
         block_id = self._next_block_id
@@ -829,10 +829,12 @@ class NexusQuantPagedAttention:
 
     def _shared_tables(self, max_position: int, dev) -> _SharedTables:
         """A device's merged rotation tables, kept here until a larger position needs longer ones."""
-        got = self._tables.get(dev)
+        comp = self.compressor  # may be another one, or of another base, than in the call before
+        key = dev, comp.head_dim, comp.rope_base
+        got = self._tables.get(key)
         if got is None or got.args[2] <= max_position:
-            _, _, dm, dp = self.compressor._tables(max_position, dev)
-            got = self._tables[dev] = _SharedTables(dm, dp)
+            _, _, dm, dp = comp._tables(max_position, dev)
+            got = self._tables[key] = _SharedTables(dm, dp)
         return got
 
     def run_shared(self, plan: SharedAttentionPlan, query: torch.Tensor, layer: int = 0,

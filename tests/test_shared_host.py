@@ -174,6 +174,26 @@ def test_rotation_tables_are_kept_by_device_and_grow(monkeypatch):
     assert len(made) == 3
 
 
+def test_rotation_tables_are_the_compressors(monkeypatch):
+    """Another compressor on the same attention, and another base of the same one: their tables, as run() reads them."""
+    from nexusquant_amd.rope import device_merged_table
+    attn = NexusQuantPagedAttention(NexusQuantKVCompressor(head_dim=64, rope_base=10000.0))
+    cpu = torch.device("cpu")
+
+    def is_of(tables, d, base):
+        return all(torch.equal(a, b) for a, b in zip(tables.tensors, device_merged_table(4096, d, base, None, cpu)))
+    first = attn._shared_tables(100, cpu)
+    assert is_of(first, 64, 10000.0)
+    attn.compressor = NexusQuantKVCompressor(head_dim=64, rope_base=500000.0)
+    assert is_of(attn._shared_tables(100, cpu), 64, 500000.0)
+    attn.compressor.rope_base = 1000000.0
+    assert is_of(attn._shared_tables(100, cpu), 64, 1000000.0)
+    attn.compressor = NexusQuantKVCompressor(head_dim=128, rope_base=10000.0)
+    assert is_of(attn._shared_tables(100, cpu), 128, 10000.0)
+    attn.compressor = NexusQuantKVCompressor(head_dim=64, rope_base=10000.0)
+    assert attn._shared_tables(100, cpu) is first
+
+
 def test_a_plan_keeps_each_table_once():
     """Two attentions (local and global rotation bases) that use one plan in turn: a table for each, not for each call."""
     plan = SharedAttentionPlan(None, 1, [])
