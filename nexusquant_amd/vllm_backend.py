@@ -603,6 +603,18 @@ class _SharedTables:
     def __init__(self, dm: torch.Tensor, dp: torch.Tensor):
         self.tensors = (dm, dp)
         self.args = (dm.data_ptr(), dp.data_ptr(), dm.shape[0])
+        self._streams: set = set()
+
+    def read_on(self, device) -> int:
+        """The device's current stream's handle, for a launch that reads the tables: their memory, once dropped, is not
+        given to others before what this stream had queued until then has run.  (A captured graph's plan keeps them.)"""
+        handle = _lib.current_stream_handle(device)
+        if handle not in self._streams and not torch.cuda.is_current_stream_capturing():
+            stream = torch.cuda.current_stream(device)
+            for t in self.tensors:
+                t.record_stream(stream)
+            self._streams.add(handle)
+        return handle
 
 
 class SharedAttentionPlan:
@@ -884,7 +896,7 @@ class NexusQuantPagedAttention:
             st = lib.nq_shared_attention(_SHARED_PACK.pack(
                 pool.desc_at, int(layer), shape[0], hq, _lib.NQ_F16 if dtype == torch.float16 else _lib.NQ_BF16, *counts,
                 q.data_ptr(), out.data_ptr(), base + items, base + pages, base + seg_rows, base + row_slots, dm, dp, n_pos,
-                *factors, ws.data_ptr(), nbytes), _lib.current_stream_handle(dev))
+                *factors, ws.data_ptr(), nbytes), tables.read_on(dev))
         _lib.check(st, "nq_shared_attention")
         return out
 

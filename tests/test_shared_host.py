@@ -194,6 +194,32 @@ def test_rotation_tables_are_the_compressors(monkeypatch):
     assert attn._shared_tables(100, cpu) is first
 
 
+def test_rotation_tables_are_recorded_on_the_streams_that_read_them(monkeypatch):
+    """Dropped tables (longer ones took their place) must outlive what other streams had queued; once a stream will do."""
+    class Table:
+        shape = (4096, 32)
+        seen = None
+
+        def data_ptr(self):
+            return 4096
+
+        def record_stream(self, stream):
+            self.seen = (self.seen or []) + [stream]
+    now, capturing = [7], [False]
+    monkeypatch.setattr(_lib, "current_stream_handle", lambda dev: now[0])
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda dev: f"stream {now[0]}")
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    tables = _SharedTables(Table(), Table())
+    for now[0] in (7, 9, 7, 9):
+        assert tables.read_on(torch.device("cuda", 0)) == now[0]
+    now[0], capturing[0] = 11, True  # a capture: the graph's plan keeps the tables
+    assert tables.read_on(torch.device("cuda", 0)) == 11
+    assert all(t.seen == ["stream 7", "stream 9"] for t in tables.tensors)
+    capturing[0] = False
+    tables.read_on(torch.device("cuda", 0))
+    assert all(t.seen == ["stream 7", "stream 9", "stream 11"] for t in tables.tensors)
+
+
 def test_a_plan_keeps_each_table_once():
     """Two attentions (local and global rotation bases) that use one plan in turn: a table for each, not for each call."""
     plan = SharedAttentionPlan(None, 1, [])
