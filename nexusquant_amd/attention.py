@@ -41,7 +41,8 @@ def prompt_tiles(lengths: Sequence[int], tile_rows: int) -> np.ndarray:
 
 
 def plan_prompts(lengths: Sequence[int], device=None) -> PromptPlan:
-    """The plan of sequences of `lengths` tokens (0 is allowed), one after another in this order."""
+    """The plan of sequences of `lengths` tokens (0 is allowed), one after another in this order.
+    Made before a graph is captured, not in the capture."""
     lens = tuple(int(x) for x in (lengths.tolist() if torch.is_tensor(lengths) else lengths))
     if any(x < 0 for x in lens):
         raise ValueError(f"lengths must not be negative, got {min(lens)}")

@@ -194,6 +194,9 @@ class PlanTensor:
         device = torch.device(device)
         self.device = device if device.index is not None else torch.device("cuda", torch.cuda.current_device())
         with torch.cuda.device(self.device):
+            if torch.cuda.is_current_stream_capturing():
+                # replays would copy again, from pinned memory that others hold by then
+                raise RuntimeError("a plan's arrays cannot be copied to the device in a graph: make the plan before capturing")
             self.tensor = to_device(values, self.device)
             stream = torch.cuda.current_stream(self.device)
             self._stream = stream.cuda_stream

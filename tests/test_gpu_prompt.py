@@ -256,3 +256,22 @@ def test_row_strides_of_any_multiple_of_eight(d, widths, hq, hkv, lens):
             ref = want if window is None else prompt_attention(q, k, v, plan, sliding_window=window)
             got = prompt_attention(q, padded(k, widths[0], pad), padded(v, widths[1], pad), plan, sliding_window=window)
             assert torch.equal(got, ref), (pad, window)
+
+
+def test_a_plan_is_made_before_a_capture():
+    """The refusal leaves the capture as it was: its graph is whole."""
+    from nexusquant_amd.attention import plan_prompts, prompt_attention
+    print("[gpu] prompt plan in a capture", flush=True)
+    q, k, v = inputs(150, 4, 2, 64, torch.float16, seed=21)
+    plan = plan_prompts([150], device=DEV)
+    want = prompt_attention(q, k, v, plan)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="before capturing"):
+            plan_prompts([150], device=DEV)
+        out = prompt_attention(q, k, v, plan)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)

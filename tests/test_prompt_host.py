@@ -121,3 +121,13 @@ int main(void) {
     subprocess.check_call(["g++", "-std=c++17", "-I", os.path.join(ROOT, "nexusquant_amd", "csrc"), "-o", str(tmp_path / "p"),
                            str(tmp_path / "p.cpp")])
     assert subprocess.run([str(tmp_path / "p")], capture_output=True, text=True).stdout == "0\n"
+
+
+def test_plans_are_not_made_in_a_capture(monkeypatch):
+    """The copy to the device would become part of the graph, from pinned memory that is given to others afterwards."""
+    import contextlib
+    monkeypatch.setattr(torch.cuda, "device", lambda dev: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before capturing"):
+        plan_prompts([3, 200], device="cuda:0")
+    assert plan_prompts([0, 0], device="cuda:0").n_tiles == 0  # nothing to copy
