@@ -69,6 +69,12 @@ def _scaling_key(rope_scaling: Optional[dict]) -> str:
     return "null" if rope_scaling is None else json.dumps(rope_scaling, sort_keys=True, default=str)
 
 
+def _before_capture(n_pos: int, device: torch.device) -> None:
+    if device.type == "cuda" and torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"rotation tables of {n_pos} positions are not on {device} yet and cannot be copied there in a "
+                           "graph: make the call once before capturing")
+
+
 def device_table(n_pos: int, head_dim: int, base: float, rope_scaling: Optional[dict],
                  device) -> Tuple[torch.Tensor, torch.Tensor]:
     """Cached device copy of host_table covering at least n_pos positions."""
@@ -78,6 +84,7 @@ def device_table(n_pos: int, head_dim: int, base: float, rope_scaling: Optional[
         hit = _cache.get(key)
         if hit is not None and hit[0].shape[0] >= n_pos:
             return hit
+        _before_capture(n_pos, device)
         n = max(_ROUND, -(-n_pos // _ROUND) * _ROUND)
         c, s = host_table(n, head_dim, base, rope_scaling)
         tab = (c.to(device), s.to(device))
@@ -96,6 +103,7 @@ def device_merged_table(n_pos: int, head_dim: int, base: float, rope_scaling: Op
         hit = _cache.get(key)
         if hit is not None and hit[0].shape[0] >= n_pos:
             return hit
+        _before_capture(n_pos, device)
         n = max(_ROUND, -(-n_pos // _ROUND) * _ROUND)
         c, s = host_table(n, head_dim, base, rope_scaling)
         tab = ((s - c).to(device), (c + s).to(device))

@@ -857,8 +857,8 @@ class NexusQuantPagedAttention:
         What a row sees is cut by all rows of the plan: outputs of one row alone and in a batch agree to
         roundings, not bit for bit.  run() differs in its roundings too (values there are not rounded).
         A captured graph reads the plan's arrays and the rotation tables of the positions up to
-        pool.max_position as they were: keep the plan while it is replayed, and capture again once a token
-        of a larger position is stored."""
+        pool.max_position as they were: keep the plan while it is replayed, and capture again, after a call
+        outside of a capture, once a token of a larger position is stored."""
         lib = _lib.load()
         pool = plan.pool
         if not query.is_cuda:

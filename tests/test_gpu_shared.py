@@ -393,3 +393,32 @@ def test_two_attentions_over_one_plan():
     for _ in range(20):
         assert torch.equal(one.run_shared(plan, q), want) and torch.equal(two.run_shared(plan, q), other)
     assert len(plan._tables) == 2
+
+
+def test_longer_tables_are_made_before_a_capture():
+    """A larger position than the tables reach: refused in a capture, which stays whole; one call before it, and it is not."""
+    from nexusquant_amd import rope
+    print("[gpu] shared longer tables in a capture", flush=True)
+    rope.clear_cache()
+    pool = make_pool(1, 60, 2, 16, 64, seed=14)
+    tables, ctx = forks(pool, 400, [5, 60])
+    attn = attention(64)
+    q = queries(2, 8, 64, torch.float16)
+    plan, want = check(attn, pool, tables, ctx, q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attn.run_shared(plan, q)
+        pool.max_position = 5000
+        with pytest.raises(RuntimeError, match="before capturing"):
+            attn.run_shared(plan, q)
+    longer = torch.cuda.CUDAGraph()
+    attn.run_shared(plan, q)
+    with torch.cuda.graph(longer):
+        out2 = attn.run_shared(plan, q)
+    for _ in range(3):
+        out.zero_()
+        out2.zero_()
+        graph.replay()
+        longer.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(out2, want)

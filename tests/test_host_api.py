@@ -54,3 +54,21 @@ def test_quant_only_level_resolution():
     assert (q.key_levels, q.value_levels) == (8, 4)
     q = nq.NexusQuantQuantOnly(bits=2)
     assert (q.key_levels, q.value_levels) == (4, 4)
+
+
+def test_rotation_tables_are_not_made_in_a_capture(monkeypatch):
+    """Their copy to the device would end the capture; tables that are there already are given in one, too."""
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    rope.clear_cache()
+    dev = torch.device("cuda", 0)
+    for make in (rope.device_table, rope.device_merged_table):
+        with pytest.raises(RuntimeError, match="before capturing"):
+            make(10, 64, 10000.0, None, dev)
+        make(10, 64, 10000.0, None, "cpu")
+    have = torch.zeros(4096, 32), torch.zeros(4096, 32)
+    monkeypatch.setitem(rope._cache, (64, 10000.0, "null", dev), have)
+    assert rope.device_table(4096, 64, 10000.0, None, dev) is have
+    with pytest.raises(RuntimeError, match="4097 positions"):
+        rope.device_table(4097, 64, 10000.0, None, dev)
+    rope.clear_cache()
