@@ -583,7 +583,8 @@ int nq_e8_stream_values(const int8_t* codes, const uint16_t* scales_f16, int64_t
  * Query i of a sequence sees its keys j with i - sliding_window < j <= i (all
  * j <= i for sliding_window 0): out = softmax(scale * q . k) . v, query head h
  * reading kv head h / (q_heads / kv_heads).  fp16 or bf16; softmax in fp32,
- * its weights rounded to the type for the second product.
+ * its weights rounded to the type for the second product (fp16: 11 bits of
+ * those down to 2^-21 of a row's largest, steps of 2^-31 of it below).
  * tiles: device int32 [n_tiles, 4], the nq_prompt_tile_rows() queries of each
  * tile as {first row of its sequence, the sequence's length, the tile's first
  * query in it, 0}; rows in no tile are neither read nor written.

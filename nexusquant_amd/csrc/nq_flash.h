@@ -4,7 +4,7 @@
 // With q the wave's 32 queries, a tile of 32 keys K and its values V:
 //   S^T = K q^T      32x32x16 MFMAs, keys the A operand: lane (n, g) gets its query n's
 //                    logits at the keys acc_row(j, g) = 8 (j / 4) + 4 g + j % 4
-//   p   = 2^(c s - m)  c = scale * log2(e), m >= c max s - kSlack: lane-local
+//   p   = 2^(c s - m)  c = scale * log2(e), m >= c max s - kSlack - LIFT: lane-local
 //   O^T += V^T P^T   P^T is the B operand as it stands (an MFMA's k order is free as long
 //                    as both operands share it: slot (g, i) of step s is key
 //                    16 s + 8 (i / 4) + 4 g + i % 4), V^T the A operand by transposing
@@ -32,9 +32,9 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) void lds_void;
 typedef const __attribute__((address_space(1))) void global_void;
 
-// A running maximum may lag the true one by 2^kSlack before the output is rescaled: weights stay
-// at most 256 (sums in fp32, weights in fp16 or bf16 have the room), and the 16 D / 32 multiplies
-// of a rescale run in the first stages of a row only.
+// A running maximum may lag the true one by 2^kSlack before the output is rescaled: weights stay at
+// most 256 times what they are at the maximum (sums in fp32, weights in fp16 or bf16 have the room), and
+// the 16 D / 32 multiplies of a rescale run in the first stages of a row only.
 constexpr float kSlack = 8.0f;
 constexpr float kNoMax = -3.0e38f;  // finite, so that a row that has seen no key forms no inf - inf
 
@@ -82,7 +82,7 @@ struct Rows {
     using T = Tile<D>;
     u32x4 q[T::KS];       // lane (n, g): query n, coordinates 16 s + 8 g + 0..7
     f32x16 o[T::DB];      // lane (n, g): query n, coordinates 32 b + acc_row(j, g)
-    float m, l;           // c * (lagging) maximum; this lane's part of the sum
+    float m, l;           // c * (lagging) maximum - LIFT; this lane's part of the sum
     uint32_t k_at, v_at, v_xor;
 
     __device__ __forceinline__ void init(int lane) {
@@ -116,11 +116,18 @@ struct Rows {
         return u32x4{a.x, a.y, c.x, c.y};
     }
 
+    // What m is below the maximum.  fp16 weights are up to 2^(kSlack + LIFT) = 2^15 then, and keep their 11 bits down to
+    // 2^-21 of a row's largest; without it 2^-14: a first token that takes nearly all of the weight leaves little above
+    // that to the others, and where its values are near zero they are the output.  (Scales of their own, SCALED, do this.)
+    template <bool SCALED>
+    static constexpr float LIFT = DT == NQ_F16 && !SCALED ? 7.0f : 0.0f;
+
     // the maximum of the stage's logits (c > 0), and the output rescaled where it passes the slack
+    template <bool SCALED>
     __device__ __forceinline__ void raise(float mx, float c) {
         mx = both_max(mx) * c;
-        if (__any(mx > m + kSlack)) {
-            const float to = __builtin_fmaxf(m, mx);
+        if (__any(mx > m + (kSlack + LIFT<SCALED>))) {
+            const float to = __builtin_fmaxf(m, mx - LIFT<SCALED>);
             const float f = __builtin_amdgcn_exp2f(m - to);
             m = to;
             l *= f;
@@ -181,7 +188,7 @@ struct Rows {
         // the wave that is past its logits goes first, so that a SIMD's waves fall out of step and one's
         // exponentials run under the other's products
         __builtin_amdgcn_s_setprio(1);
-        raise(mx, c);
+        raise<SCALED>(mx, c);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             uint32_t p[8];
@@ -203,7 +210,7 @@ struct Rows {
             s[j] = key >= lo && key < hi ? s[j] : -__builtin_inff();
             mx = __builtin_fmaxf(mx, s[j]);
         }
-        raise(mx, c);
+        raise<SCALED>(mx, c);
         uint32_t p[8];
         weights<SCALED>(s, c, p, v, g);
         add_values(p, vbuf, t);

@@ -275,3 +275,24 @@ def test_a_plan_is_made_before_a_capture():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("hq,d,dtype", [(1, 128, torch.float16), (32, 128, torch.float16), (1, 64, torch.float16),
+                                        (40, 64, torch.float16), (2, 256, torch.float16), (18, 256, torch.float16),
+                                        (32, 128, torch.bfloat16)])
+@pytest.mark.parametrize("logit", [-9.375, -12.1875, -14.25])
+def test_many_small_weights_beside_one_large(hq, d, dtype, logit):
+    """A first token that takes nearly all of the weight and has a value of zero, and many that share the rest, alike (so
+    that their weights' roundings add up): a fp16 weight keeps its 11 bits down to 2^-21 of the largest, e^-14.25 among
+    them, though it is 11 steps of fp16's smallest number as it stands."""
+    print(f"[gpu] prompt small weights {hq} d={d} {dtype} {logit}", flush=True)
+    n = 1100
+    q, k, v = (x.contiguous() for x in inputs(n, hq, 1, d, dtype, seed=hq + d))
+    v.add_(3.0)
+    v[0] = 0
+    q.zero_()
+    k.zero_()
+    q[..., 0] = 1.0
+    k[1:, :, 0] = logit
+    check(q, k, v, [n], scale=1.0)
+    check(q, k, v, [n], scale=1.0, window=700)
