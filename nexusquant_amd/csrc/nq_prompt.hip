@@ -317,7 +317,11 @@ extern "C" int nq_prompt_attention(const nq_prompt_desc* d, void* stream) {
     NQ_CHECK_ARG(d->k_stride[0] >= 0 && d->k_stride[0] < (1 << 24) && d->v_stride[0] >= 0 && d->v_stride[0] < (1 << 24),
                  "nq_prompt_attention: rows of k and v must be less than 2^24 elements apart");
     NQ_CHECK_ARG(d->n_split >= 1 && d->n_split <= 64, "nq_prompt_attention: n_split %d (1 .. 64)", d->n_split);
-    NQ_CHECK_ARG((uint64_t)d->n_tiles * d->q_heads * d->n_split <= max_blocks(256), "nq_prompt_attention: grid too large");
+    // the tiles' parts, and where there are several the workgroups that join them
+    const uint64_t blocks64 = (uint64_t)d->n_tiles * d->q_heads;
+    NQ_CHECK_ARG(blocks64 <= max_blocks(256) && blocks64 * d->n_split <= max_blocks(256) &&
+                     (d->n_split == 1 || blocks64 * (kPromptRows * d->head_dim / 1024) <= max_blocks(256)),
+                 "nq_prompt_attention: grid too large");
     const int64_t need = nq_prompt_workspace(d->n_tiles, d->q_heads, d->head_dim, d->n_split);
     NQ_CHECK_ARG(need == 0 || (d->workspace != nullptr && d->workspace_bytes >= need && ((uintptr_t)d->workspace & 15u) == 0),
                  "nq_prompt_attention: a 16-byte aligned workspace of %lld bytes is needed", (long long)need);
@@ -339,7 +343,7 @@ extern "C" int nq_prompt_attention(const nq_prompt_desc* d, void* stream) {
     a.hkv = (uint32_t)d->kv_heads;
     a.window = d->sliding_window;
     a.c = d->scale * 1.44269504088896340736f;
-    const uint32_t blocks = (uint32_t)d->n_tiles * a.hq;
+    const uint32_t blocks = (uint32_t)blocks64;
     a.n_split = (uint32_t)d->n_split;
     a.part_o = static_cast<float*>(d->workspace);
     a.part_ml = a.part_o + (size_t)blocks * a.n_split * kPromptRows * d->head_dim;

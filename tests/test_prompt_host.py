@@ -131,3 +131,22 @@ def test_plans_are_not_made_in_a_capture(monkeypatch):
     with pytest.raises(RuntimeError, match="before capturing"):
         plan_prompts([3, 200], device="cuda:0")
     assert plan_prompts([0, 0], device="cuda:0").n_tiles == 0  # nothing to copy
+
+
+@pytest.mark.parametrize("d,per_tile", [(64, 8), (128, 16), (256, 32)])
+def test_c_entry_refuses_more_tiles_than_their_join_takes(d, per_tile):
+    """The join has 128 D / 1024 workgroups of 256 threads for each tile and head: 2^32 threads at most.  (The calls within
+    it end at their missing workspace.)"""
+    lib = _lib.load()
+    most = (2 ** 32 - 1) // 256 // per_tile // 8  # tiles of 8 heads
+    for n_tiles, why in ((most, b"workspace"), (most + 1, b"grid too large")):
+        x = desc(head_dim=d, n_tiles=n_tiles, n_split=2)
+        assert lib.nq_prompt_attention(ctypes.byref(x), None) == -1
+        assert why in lib.nq_last_error(), (n_tiles, lib.nq_last_error())
+
+
+def test_c_entry_refuses_products_past_64_bits():
+    lib = _lib.load()
+    x = desc(n_tiles=1 << 30, q_heads=1 << 30, kv_heads=1, n_split=16)  # 2^64 workgroups
+    assert lib.nq_prompt_attention(ctypes.byref(x), None) == -1
+    assert b"grid too large" in lib.nq_last_error()
