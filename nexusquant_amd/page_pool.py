@@ -351,8 +351,8 @@ class CompressedPagePool:
     def write(self, compressor, slots: Sequence[int], keys: torch.Tensor, values: torch.Tensor, positions,
               layer: int = 0) -> None:
         """Encode tokens and store them in one layer: keys, values [tokens, heads, head_dim], keys rotated
-        to `positions` [tokens]; token i goes to slots[i], -1 skips it (a padded batch).  Slots are distinct
-        and in pages of one reference."""
+        to `positions` [tokens]; token i goes to slots[i], -1 skips it (a padded batch), whatever its position.
+        Slots are distinct and in pages of one reference."""
         _refuse_capture("write")
         lib = _lib.load()
         if compressor.head_dim != self.head_dim:
@@ -376,6 +376,10 @@ class CompressedPagePool:
             raise ValueError("write: slots must be distinct")
         if n == 0:
             return
+        if len(used) < n:  # padding: its positions, -1 or large ones among them, are nobody's
+            pos = torch.as_tensor(positions).reshape(-1)
+            if len(pos) == n:
+                positions = pos.masked_fill(torch.from_numpy(s < 0).to(pos.device), 0)
         with self._lock:
             p = self.in_use(np.unique(used // self.page_tokens), "write")
             if len(p) and self._refs[p].max() > 1:

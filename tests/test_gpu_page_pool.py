@@ -286,3 +286,36 @@ def test_pages_of_a_pool_are_the_compressors_pages():
     got = comp.decompress_page(pool.page(2, layer=1))
     want = comp.decompress_page(comp.compress_page(k.permute(1, 0, 2), v.permute(1, 0, 2), range(100, 116)))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("where", ["list", "cpu", "device"])
+def test_positions_of_skipped_tokens_do_not_count(where):
+    """A padded batch: -1 and far positions where nothing is stored are not refused and do not lengthen the tables."""
+    from nexusquant_amd.vllm_backend import NexusQuantKVCompressor
+    print(f"[gpu] write padding positions ({where})", flush=True)
+    pool = random_pool(1, 6, 2, 4, 64, seed=3)
+    pool.positions.zero_()
+    pool.max_position = 0
+    pool.allocate(3)
+    comp = NexusQuantKVCompressor(head_dim=64)
+    k = torch.randn(5, 2, 64, generator=torch.Generator().manual_seed(1)).half().to(DEV)
+    slots, pos = [3, -1, 9, -1, 4], [7, -1, 8, (1 << 31) - 1, 9]
+    want = snapshot(pool)
+    kept = [0, 2, 4]
+    page = comp.compress_page(k[kept].permute(1, 0, 2), k[kept].permute(1, 0, 2), [7, 8, 9])
+    for j, i in enumerate(kept):
+        at = slots[i] // 4, slots[i] % 4
+        for name in FIELDS[:4]:
+            want[name][0, at[0], :, at[1]] = getattr(page, name)[:, j].cpu().numpy()
+        want["positions"][at] = pos[i]
+    given = pos if where == "list" else torch.tensor(pos, dtype=torch.int32, device=DEV if where == "device" else "cpu")
+    pool.write(comp, slots, k, k, given)
+    assert_same(pool, want)
+    assert pool.max_position == 9
+    if where != "list":
+        assert given.tolist() == pos  # the caller's are left as they are
+    with pytest.raises(ValueError):
+        pool.write(comp, slots, k, k, [7, -1, -8, 0, 9])  # a stored one
+    with pytest.raises(ValueError):
+        pool.write(comp, slots, k, k, [7, -1, 8])
+    assert_same(pool, want)
