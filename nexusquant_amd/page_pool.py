@@ -367,6 +367,8 @@ class CompressedPagePool:
         s = np.asarray(slots.tolist() if torch.is_tensor(slots) else slots).reshape(-1)
         if len(s) and s.dtype.kind not in "iu":
             raise ValueError(f"slots must be integers, got {s.dtype}")
+        if len(s) and s.max() >= self.num_pages * self.page_tokens:  # (as the type they came in)
+            raise ValueError(f"slots must lie below {self.num_pages * self.page_tokens}")
         s = s.astype(np.int64, copy=False)
         n = keys.shape[0]
         if len(s) != n:

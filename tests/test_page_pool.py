@@ -189,3 +189,16 @@ def test_pool_entry_points_refuse_bad_geometry():
     assert lib.nq_pool_write(ok, 0, one, dummy, 0, 15, None) == -1       # not one page of n tokens
     assert lib.nq_pool_write(ok, 0, ctypes.byref(c_pool(pages=1, heads=4)), dummy, 0, 16, None) == -1
     assert lib.nq_pool_write(ok, 0, one, None, 0, 16, None) == -1
+
+
+def test_write_refuses_slots_past_the_pool(monkeypatch):
+    """Unsigned numbers past 2^63 among them: negative ones are skipped, and these are none."""
+    from nexusquant_amd.vllm_backend import NexusQuantKVCompressor
+    pool = host_pool(monkeypatch)
+    pool.allocate(2)
+    k = torch.zeros(2, 3, 64, dtype=torch.float16)
+    for slots in (np.array([0, (1 << 64) - 1], dtype=np.uint64), [0, 40], torch.tensor([40, 0]), [0, 1 << 62]):
+        with pytest.raises(ValueError, match="below 40"):
+            pool.write(NexusQuantKVCompressor(head_dim=64), slots, k, k, [0, 1])
+    with pytest.raises(ValueError, match="integers"):
+        pool.write(NexusQuantKVCompressor(head_dim=64), [0, 1 << 64], k, k, [0, 1])
