@@ -248,7 +248,7 @@ class CompressedPagePool:
             p = self.in_use(pages, "fork")
             if length < 0 or self.pages_for(length) != len(p):
                 raise ValueError(f"fork: {length} tokens take {self.pages_for(max(length, 0))} pages, got {len(p)}")
-            table = pages if type(pages) is list else p.tolist()
+            table = p.tolist()  # plain integers, whatever the list held (a 0-d tensor equals no other in a set)
             if len(set(table)) != len(table):
                 raise ValueError("fork: a page stands twice in one sequence")
             if length % self.page_tokens == 0:

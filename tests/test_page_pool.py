@@ -202,3 +202,18 @@ def test_write_refuses_slots_past_the_pool(monkeypatch):
             pool.write(NexusQuantKVCompressor(head_dim=64), slots, k, k, [0, 1])
     with pytest.raises(ValueError, match="integers"):
         pool.write(NexusQuantKVCompressor(head_dim=64), [0, 1 << 64], k, k, [0, 1])
+
+
+def test_fork_of_a_tables_row(monkeypatch):
+    """list(block_table[b]): 0-d tensors, of which no two are equal in a set; numpy's integers."""
+    pool = host_pool(monkeypatch)
+    a = torch.tensor(pool.allocate(3), dtype=torch.int32)
+    for row in (list(a), list(a.numpy()), a, a.numpy(), tuple(a.tolist())):
+        kids = pool.fork(row, 10, 2)
+        assert [x[:2] for x in kids] == [[0, 1]] * 2 and all(type(p) is int for x in kids for p in x)
+        pool.free([p for x in kids for p in x])
+    twice = [a[0], a[1], a[1].clone()]
+    for row in (twice, [int(p) for p in twice]):
+        with pytest.raises(ValueError, match="twice"):
+            pool.fork(row, 12)
+    assert [pool.ref_count(p) for p in range(3)] == [1, 1, 1] and pool.free_pages == 7
