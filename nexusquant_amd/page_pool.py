@@ -36,9 +36,11 @@ _HEAD_DIMS = (64, 128, 256)
 _FIELDS = ("key_codes", "value_codes", "key_scales", "value_scales", "positions")
 
 
-def _refuse_capture(what: str) -> None:
-    if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError(f"{what} changes the pool's host state and cannot be captured into a graph")
+def _refuse_capture(what: str, device: torch.device) -> None:
+    if torch.cuda.is_initialized():
+        with on_device(device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"{what} changes the pool's host state and cannot be captured into a graph")
 
 
 class CompressedPagePool:
@@ -240,7 +242,7 @@ class CompressedPagePool:
 
         Full pages are shared (one more reference a branch); a part-filled last page is copied
         for each branch, so that the sequence and its branches can all go on writing."""
-        _refuse_capture("fork")
+        _refuse_capture("fork", self.device)
         with self._lock:
             n, length = int(n), int(length)
             if n < 0:
@@ -275,7 +277,7 @@ class CompressedPagePool:
         position j, keys re-rotated (truncation).  Positions in the list must lie in their
         sequence (the kernel clamps them).  Needs the new pages free beside the old ones.
         Returns the new tables and lengths."""
-        _refuse_capture("compact")
+        _refuse_capture("compact", self.device)
         lib = _lib.load()
         _lib.require_device(kept_idx, "kept_idx")
         if kept_idx.dtype != torch.int32 or kept_idx.dim() != 2:
@@ -353,7 +355,7 @@ class CompressedPagePool:
         """Encode tokens and store them in one layer: keys, values [tokens, heads, head_dim], keys rotated
         to `positions` [tokens]; token i goes to slots[i], -1 skips it (a padded batch), whatever its position.
         Slots are distinct and in pages of one reference."""
-        _refuse_capture("write")
+        _refuse_capture("write", self.device)
         lib = _lib.load()
         if compressor.head_dim != self.head_dim:
             raise ValueError(f"compressor head_dim {compressor.head_dim} != pool head_dim {self.head_dim}")

@@ -217,3 +217,32 @@ def test_fork_of_a_tables_row(monkeypatch):
         with pytest.raises(ValueError, match="twice"):
             pool.fork(row, 12)
     assert [pool.ref_count(p) for p in range(3)] == [1, 1, 1] and pool.free_pages == 7
+
+
+def test_a_capture_on_the_pools_device_is_seen_from_another_current_one(monkeypatch):
+    """The launches go to the pool's device's current stream, so it is that one that may be capturing."""
+    now = [0]
+
+    class Device:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.was, now[0] = now[0], self.index
+
+        def __exit__(self, *_):
+            now[0] = self.was
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now[0] == 1)
+    pool = host_pool(monkeypatch)
+    a = pool.allocate(3)
+    pool.device = torch.device("cuda", 1)
+    for call in (lambda: pool.fork(a, 12), lambda: pool.compact([a], [12], torch.zeros(1, 12, dtype=torch.int32), [3]),
+                 lambda: pool.write(None, [0], None, None, [0])):
+        with pytest.raises(RuntimeError, match="captured"):
+            call()
+    assert now == [0] and pool.free_pages == 7 and pool.ref_count(0) == 1
+    pool.device = torch.device("cuda", 0)
+    assert pool.fork(a, 12) == [a]
