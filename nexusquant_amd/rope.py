@@ -70,9 +70,11 @@ def _scaling_key(rope_scaling: Optional[dict]) -> str:
 
 
 def _before_capture(n_pos: int, device: torch.device) -> None:
-    if device.type == "cuda" and torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError(f"rotation tables of {n_pos} positions are not on {device} yet and cannot be copied there in a "
-                           "graph: make the call once before capturing")
+    if device.type == "cuda" and torch.cuda.is_initialized():
+        with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"rotation tables of {n_pos} positions are not on {device} yet and cannot be copied "
+                                   "there in a graph: make the call once before capturing")
 
 
 def device_table(n_pos: int, head_dim: int, base: float, rope_scaling: Optional[dict],

@@ -58,10 +58,22 @@ def test_quant_only_level_resolution():
 
 def test_rotation_tables_are_not_made_in_a_capture(monkeypatch):
     """Their copy to the device would end the capture; tables that are there already are given in one, too."""
+    now = [0]
+
+    class Device:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.was, now[0] = now[0], self.index
+
+        def __exit__(self, *_):
+            now[0] = self.was
     monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now == [1])
     rope.clear_cache()
-    dev = torch.device("cuda", 0)
+    dev = torch.device("cuda", 1)  # the one that is capturing, not the current one
     for make in (rope.device_table, rope.device_merged_table):
         with pytest.raises(RuntimeError, match="before capturing"):
             make(10, 64, 10000.0, None, dev)
