@@ -68,6 +68,20 @@ def _rows(t: torch.Tensor):
     return t, at, row, head
 
 
+def _apart(t: torch.Tensor) -> bool:
+    """Whether no two head vectors of t share memory."""
+    (n, m, d), (row, head, _) = t.shape, t.stride()
+    if n <= 1 or m <= 1:
+        return (n <= 1 or row >= d) and (m <= 1 or head >= d)
+    if row < d or head < d:
+        return False
+    if row >= (m - 1) * head + d or head >= (n - 1) * row + d:  # heads within rows, or rows within heads
+        return True
+    # interleaved: the rows nearest to each head's distance, from below and from above
+    return not any((i < n and j * head - i * row < d) or (i + 1 < n and (i + 1) * row - j * head < d)
+                   for j in range(1, m) for i in (j * head // row,))
+
+
 # nq_prompt_desc, packed in one go and passed as bytes (a call's host time counts for short prompts)
 _PACK = struct.Struct("6i5P8qfiPq")
 
@@ -132,8 +146,7 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         if rows > plan.rows:
             out[plan.rows:].zero_()
     elif (out.shape != shape or out.dtype != dtype or out.device != dev
-          or out.stride(2) != 1 or out.stride(0) % 4 or out.stride(1) % 4 or out.data_ptr() % 8
-          or (rows > 1 and out.stride(0) == 0) or (hq > 1 and out.stride(1) == 0)):
+          or out.stride(2) != 1 or out.stride(0) % 4 or out.stride(1) % 4 or out.data_ptr() % 8 or not _apart(out)):
         raise ValueError(f"out must be {tuple(shape)} {dtype} on {dev} with 8-byte aligned head vectors of their own")
     if plan.n_tiles == 0:
         return out

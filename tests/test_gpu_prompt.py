@@ -296,3 +296,18 @@ def test_many_small_weights_beside_one_large(hq, d, dtype, logit):
     k[1:, :, 0] = logit
     check(q, k, v, [n], scale=1.0)
     check(q, k, v, [n], scale=1.0, window=700)
+
+
+def test_overlapping_outputs_are_refused():
+    from nexusquant_amd.attention import plan_prompts, prompt_attention
+    print("[gpu] prompt overlapping outputs", flush=True)
+    q, k, v = inputs(20, 4, 2, 64, torch.float16, seed=31)
+    plan = plan_prompts([20], device=DEV)
+    buf = torch.zeros(20 * 4 * 64 * 2, dtype=torch.float16, device=DEV)
+    for row, head in ((32, 1280), (192, 64), (256, 32), (64, 64)):
+        with pytest.raises(ValueError, match="of their own"):
+            prompt_attention(q, k, v, plan, out=torch.as_strided(buf, (20, 4, 64), (row, head, 1)))
+    assert not bool(buf.any())
+    want = prompt_attention(q, k, v, plan)
+    for row, head in ((256, 64), (64, 1280), (264, 64), (68, 1360)):  # rows within heads, too, and with gaps
+        assert torch.equal(prompt_attention(q, k, v, plan, out=torch.as_strided(buf, (20, 4, 64), (row, head, 1))), want)

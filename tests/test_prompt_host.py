@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from nexusquant_amd import _lib
-from nexusquant_amd.attention import PromptPlan, _PACK, _splits, plan_prompts, prompt_attention, prompt_tiles
+from nexusquant_amd.attention import PromptPlan, _PACK, _apart, _splits, plan_prompts, prompt_attention, prompt_tiles
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -150,3 +150,21 @@ def test_c_entry_refuses_products_past_64_bits():
     x = desc(n_tiles=1 << 30, q_heads=1 << 30, kv_heads=1, n_split=16)  # 2^64 workgroups
     assert lib.nq_prompt_attention(ctypes.byref(x), None) == -1
     assert b"grid too large" in lib.nq_last_error()
+
+
+def test_outputs_whose_head_vectors_overlap_are_seen():
+    """Against the list of all addresses."""
+    def overlap(rows, heads, row, head, d=8):
+        at = [r * row + h * head for r in range(rows) for h in range(heads)]
+        return len({a + i for a in at for i in range(d)}) < len(at) * d
+    seen = set()
+    for rows in range(1, 5):
+        for heads in range(1, 5):
+            for row in range(0, 52, 4):
+                for head in range(0, 52, 4):
+                    t = torch.as_strided(torch.zeros(400), (rows, heads, 8), (row, head, 1))
+                    want = not overlap(rows, heads, row, head)
+                    assert _apart(t) == want, (rows, heads, row, head)
+                    nested = row >= (heads - 1) * head + 8 or head >= (rows - 1) * row + 8
+                    seen.add((want, nested))
+    assert len(seen) == 4  # interleaved ones that are apart, too
