@@ -422,3 +422,32 @@ def test_longer_tables_are_made_before_a_capture():
         longer.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(out2, want)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("heads,group,rows,prefix,kind", [(2, 4, 3, 1500, "few"), (2, 4, 8, 1500, "some"),
+                                                          (8, 4, 24, 4096, "some"), (8, 8, 40, 6000, "many")])
+def test_values_are_exact_and_weights_of_few_rows_nearly(heads, group, rows, prefix, kind, d):
+    """Queries of zero weigh all tokens alike, so keys' roundings do not count, and values' would be all there is to see.
+    Values are exact codes: a weight times its scale is rounded (U; U^2 for few rows, which keep what that rounds off, in fp16
+    too), or is off by half of fp16's smallest step where the chunk's largest is at least 2^6: 2^-31 of the largest a token, 2^-20
+    for a chunk's 2048.  Sums in fp32, in the transformed domain: 2^-20 of the tokens' 2-norms."""
+    print(f"[gpu] shared values {kind} {heads}x{group} d={d} rows={rows} prefix={prefix}", flush=True)
+    pool = make_pool(1, prefix // 16 + 2 + 8 * rows, heads, 16, d, seed=rows + d)
+    tables, ctx = forks(pool, prefix, [0] * rows)
+    q = torch.zeros(rows, heads * group, d, dtype=torch.float16, device=DEV)
+    attn = attention(d)
+    plan = attn.plan_shared(pool, tables, ctx, min_saved=1)
+    n_items, n_many, n_few, _ = plan.work(heads * group)[1]
+    assert {"few": n_few == n_items, "some": n_many == 0 and n_few < n_items, "many": n_many > 0}[kind]
+    got = attn.run_shared(plan, q)
+    w = U ** 2 if kind == "few" else U
+    for b in range(0, rows, 7):
+        pages = torch.tensor(tables[b], device=DEV)
+        v = pool.value_codes[0, pages].double() / 2 * pool.value_scales[0, pages].double()[..., None]
+        v = walsh(v.transpose(0, 1).reshape(heads, -1, d)[:, :ctx[b]])
+        want = v.mean(1)
+        tol = (w + 2 ** -20) * v.abs().mean(1) + 2 ** -19 * v.norm(dim=-1).amax(-1, keepdim=True)
+        want, tol = (x.repeat_interleave(group, 0) for x in (want, tol))
+        off = (got[b].double() - want).abs() - tol - (U * want.abs()).clamp_min(2.0 ** -25)
+        assert bool((off <= 0).all()), (b, off.max().item())
