@@ -87,8 +87,8 @@ _PACK = struct.Struct("6i5P8qfiPq")
 
 
 # Few tiles and heads: several workgroups share a tile's keys, as many as run at once (two on a CU, at head_dim 256 one),
-# with _SPLIT_STAGES stages of 64 keys each at least.  us without and with, one prompt: 2188 tokens of 4 heads x 256 100
-# and 51, x 128 46 and 28, 8192 of one head 149 and 42, 4096 of 8 87 and 68, 700 of 8 x 64 14.2 and 13.8.
+# with _SPLIT_STAGES stages of 64 keys each at least.  us without and with, one prompt: 2188 tokens of 4 heads x 256 95
+# and 49, x 128 45 and 28, 8192 of one head 148 and 42, 4096 of 8 80 and 65, 2048 of 8 x 64 32 and 23, 700 13.5 and 13.8.
 _SPLIT_TO = {64: 512, 128: 512, 256: 256}
 _SPLIT_STAGES = 3
 _STAGE = 64

@@ -6,10 +6,12 @@
 // values (direct-to-LDS loads, under way while the other buffer is computed on).  128 queries
 // and 64 keys are what two workgroups on a CU leave of registers and LDS at head_dim 128.
 //
-// What bounds it: at 16384 tokens of 32 / 8 heads x 128, 1030 TFLOP/s (2.12 ms); with half of the LDS
-// reads 6 % less, without exponentials 5 %, so nothing by itself.  At head_dim 64 exponentials
-// take half of the products' time (640 TFLOP/s), at 256 a SIMD holds one wave (590).  Short
-// prompts are bound by the latency of their few stages: 10.7 us for up to 190 tokens.
+// What bounds it: at 16384 tokens of 32 / 8 heads x 128, fp16, 2.15 to 2.26 ms by card (975 to 1020
+// TFLOP/s; bf16 1090); with half of the LDS reads 6 % less, without exponentials 5 %, so nothing by
+// itself.  At head_dim 64 exponentials take half of the products' time (890, bf16 940), at 256 a SIMD
+// holds one wave (810; 4096 tokens 720).  A window of 1024 tokens leaves many of a workgroup's stages
+// masked: 760 TFLOP/s of what is seen, 530 at 256.  Short prompts are bound by the latency of their
+// few stages: 10.6 us for up to 190 tokens.
 #include "nq_flash.h"
 
 namespace nq {

@@ -15,9 +15,14 @@
 // A partial (maximum, sum, value sum) per query row and chunk goes to the workspace; the
 // combine kernel joins a row's chunks.
 //
-// What bounds it: 512 query rows of 8 kv heads x 128 over 32768 tokens, 122 us (560 TFLOP/s): the products by
-// themselves take 105 of them (every wave reads every key and value from LDS), decoding by itself 78, and they run
-// under each other only in part.  Few rows: see there.
+// What bounds it: 512 query rows of 8 kv heads x 128 over 32768 tokens, a call 107 to 112 us by card (610 to 640
+// TFLOP/s): 92 without the decoding (every wave reads every key and value from LDS), 67 without the attention, and they
+// run under each other only in part.  Few rows: see there.
+//
+// Weights times scales keep fp16's 11 bits here; twice as many, as few rows have, are a second product for the values.
+// us and error of fp16 outputs (2.1e-4 is their own rounding) with 11 and with 22, head_dim 128: 32 query rows x 32768
+// tokens 34.2, 3.3e-4 and 34.7, 2.6e-4; 128 x 4096 24.8, 3.3e-4 and 26.1, 2.7e-4; 512 x 32768 107, 3.4e-4 and 129,
+// 2.7e-4.  The other half of what is above 2.1e-4 is the keys'.
 #include "nq_flash.h"
 #include "nq_keymfma.h"
 #include "nq_rowmath.h"
@@ -29,8 +34,8 @@ using namespace flash;
 // The shape of a workgroup.  MANY: rows count, so as many as the registers hold (32 a wave) share what is decoded,
 // and a stage is decoded under the attention to the one before it; two stage buffers, 128 KB of LDS at head_dim
 // 128 and 256, so one workgroup on a CU.  Not MANY: decoding counts, and several small workgroups on a CU hide
-// each other's loads.  8 kv heads x 128, us: 512 query rows x 32768 tokens 122 (MANY) and 230; 128 rows x
-// 16384 35.0 and 38.9, x 4096 24.8 and 25.5; 64 rows x 8192 23.4 and 23.8.
+// each other's loads.  8 kv heads x 128, us a call: 512 query rows x 32768 tokens 107 (MANY) and 146; 128 rows x
+// 16384 31.1 and 34.4, x 4096 21.7 and 24.0; 64 rows x 8192 21.2 and 24.5, x 4096 19.5 and 18.1.
 template <int D, bool MANY>
 struct Shape {
     static constexpr int WAVES = MANY && D <= 128 ? 8 : 4;
@@ -117,9 +122,9 @@ __device__ __forceinline__ int value_exponent(const float (&wave_max)[NW]) {
 // the logits (sums of codes are below 2 D 127: they fit fp16).  Waves need no barriers; what a wave's next 16 tokens need
 // is loaded into registers as soon as they are free, without a branch, so that the waits count only what they must.
 //
-// us here and in the small shape above: 2 rows x 2 heads of 32 kv heads x 128 over 6352 own tokens 39.7 and 51.8 (2.7
-// TB/s of codes and scales), 64 x 8 of 8 over 512 28.8 and 35.8, 3 x 8 of 8 x 256 over 9184 40.6 and 71, 1 x 8 of 8 x 128
-// over 131072 106 and 118.  Loads alone take 29 of the first's 39.7; the rest is conversions (some 280 vector
+// us a call here and in the small shape above: 2 rows x 2 heads of 32 kv heads x 128 over 6352 own tokens 33.8 and 43.5
+// (3.1 TB/s of codes and scales), 64 x 8 of 8 over 512 27.4 and 33.4, 3 x 8 of 8 x 256 over 9184 38.3 and 66.2, 1 x 8 of 8
+// x 128 over 131072 97 and 107.  Loads alone take some 70 % of the first's; the rest is conversions (some 280 vector
 // instructions for 16 tokens of a head) and rows of the rotation table, twice the bytes of the codes, from L2.
 template <int D>
 struct Few {

@@ -463,8 +463,8 @@ class PagedAttentionPlan:
 
 
 # What pays to share: sharing that saves this many tokens' decoding, counted in every kv head (a segment's tokens, once
-# for every row but one).  us shared and apart: 8 kv heads x 4, 32 rows x 256 tokens 18.7 and 15.8, x 512 18.0 and
-# 19.2, 8 rows x 1024 15.3 and 15.5, x 2048 15.9 and 18.4; 32 x 1, 16 rows x 128 15.6 and 15.9, x 256 15.7 and 20.5.
+# for every row but one).  us shared and apart: 8 kv heads x 4, 32 rows x 256 tokens 15.6 and 13.4, x 512 15.9 and
+# 17.1, 8 rows x 1024 13.3 and 13.2, x 2048 14.1 and 18.6; 32 x 1, 16 rows x 128 11.2 and 12.6, x 256 11.9 and 15.7.
 _MIN_SAVED = 1 << 16
 
 
@@ -513,17 +513,18 @@ _SHARED_STAGE = (128, 128, 64)
 _SHARED_LEAST = (256, 128, 64)
 # The kinds of segments, by query rows (batch rows x query heads of a kv head): many (wide workgroups), some, few.
 # Few are up to nq_shared_attention_rows(d, 2) of them: 8 kv heads x 128, us few and some: 64 rows x 8 heads over 512
-# own tokens 28.8 and 35.8, 3 x 8 over 9184 at head_dim 256 40.6 and 71, 8 x 1 over 8192 at 64 18.8 and 22.9.
+# own tokens 27.4 and 33.4, 3 x 8 over 9184 at head_dim 256 38.3 and 66.2, 8 x 1 over 8192 at 64 24.4 and 31.4.
 # Segments of more than _MANY_ROWS count as many when there are at least _MANY_TOKENS tokens for each of 256 CUs
-# (some are up to nq_shared_attention_rows(d, 1)): 8 kv heads, 128 query rows, us many and some: 4096 tokens 24.8 and
-# 25.5, 16384 tokens 35.0 and 38.9.
+# (some are up to nq_shared_attention_rows(d, 1)): 8 kv heads x 128, us many and some: 128 query rows over 16384 shared
+# tokens 31.1 and 34.4, over 4096 21.7 and 24.0, but with 256 own tokens a row, which go along with some, 32.4 and 25.1;
+# 64 query rows over 4096 19.5 and 18.1.
 _MANY, _SOME, _FEW = 0, 1, 2
 _MANY_ROWS = 32
 _MANY_TOKENS = 512
 # Few go into the launch of some, where there are any, as long as they have less than this many tokens for each CU (each
 # segment counted as 128 at least).  A shared 4096 tokens of 128 query rows and own ones, us together and with a launch
-# for the own ones: 8 kv heads x 128, 512 a CU 36.9 and 40.0, 1024 60 and 47; x 64, 768 24.0 and 27.7, 1536 35.9 and
-# 36.0; 4 x 256, 128 39.2 and 44.8, 256 60.5 and 47.7.  32 rows of 4 heads and 256 own tokens: 25.7 us together, 26.3
+# for the own ones: 8 kv heads x 128, 512 a CU 35.1 and 38.7, 1024 57.8 and 44.2; x 64, 768 23.5 and 29.2, 1536 34.3 and
+# 34.9; 4 x 256, 128 38.0 and 43.7, 256 59.3 and 47.2.  32 rows of 4 heads and 256 own tokens: 25.7 us together, 26.3
 # with the own ones as some, 36 with a launch of their own.
 _FEW_TOKENS = {64: 1536, 128: 768, 256: 192}
 
@@ -855,7 +856,8 @@ class NexusQuantPagedAttention:
         layer of its pool.  num_heads is a multiple of the pool's heads.  Rows without tokens are zero.
 
         What a row sees is cut by all rows of the plan: outputs of one row alone and in a batch agree to
-        roundings, not bit for bit.  run() differs in its roundings too (values there are not rounded).
+        roundings, not bit for bit.  Values are exact codes, as in run(); weights keep 22 bits there and for segments of
+        up to 16 query rows here, fp16's 11 for wider ones.
         A captured graph reads the plan's arrays and the rotation tables of the positions up to
         pool.max_position as they were: keep the plan while it is replayed, and capture again, after a call
         outside of a capture, once a token of a larger position is stored."""
