@@ -9,7 +9,7 @@ Families:
 With `own` false each is computed in elementary torch operations; with `own` true through the package's entry points.
 
 The 4-bit form of a vector x of d coordinates: t = H x (H the orthonormal Sylvester matrix), s = fp16(max|t| / 7.5),
-n = clamp(floor(t / s + 8), 0, 15); it stands for H ((n - 7.5) s).  Keys are stored rotated.
+n = clamp(floor(t / s + 8.5), 0, 15); it stands for H ((n - 8) s).  Keys are stored rotated.
 """
 
 import math
@@ -157,7 +157,7 @@ def _fields(g, pages, heads, tokens, d):
     for name in ("key", "value"):
         byte = torch.zeros(shape + (d // 2,), dtype=torch.uint8, device=DEV)
         for shift in (0, 4):
-            n = torch.empty(byte.shape, dtype=torch.float16, device=DEV).normal_(8.0, 2.6, generator=g)
+            n = torch.empty(byte.shape, dtype=torch.float16, device=DEV).normal_(8.5, 2.6, generator=g)
             byte |= n.floor_().clamp_(0, 15).to(torch.uint8) << shift
         out[name + "_codes"] = byte
         out[name + "_scales"] = (torch.rand(shape, device=DEV, generator=g) * 0.2 + 0.3).half()
@@ -278,13 +278,13 @@ def _encode(x, hadamard):
     """Codes and scales of vectors; in 64 bits, since a value next to a border takes one code or the other."""
     y = torch.matmul(x.double(), hadamard)
     s = (y.abs().amax(-1, keepdim=True) / 7.5).half()
-    n = torch.floor(y / torch.where(s == 0, 1.0, s.double()) + 8.0).clamp_(0, 15).to(torch.uint8)
+    n = torch.floor(y / torch.where(s == 0, 1.0, s.double()) + 8.5).clamp_(0, 15).to(torch.uint8)
     return n[..., 0::2] | (n[..., 1::2] << 4), s[..., 0]
 
 
 def _decode(codes, scales, hadamard):
     n = torch.stack([codes & 15, codes >> 4], dim=-1).flatten(-2)
-    return torch.matmul((n.to(hadamard.dtype) - 7.5) * scales.to(hadamard.dtype)[..., None], hadamard)
+    return torch.matmul((n.to(hadamard.dtype) - 8) * scales.to(hadamard.dtype)[..., None], hadamard)
 
 
 def _plain_append(st):
@@ -417,7 +417,7 @@ def exact(case, seed):
         for x in (_turned(st["k"], st, 1) if case["axes"] else st["k"].double(), st["v"].double()):
             t = _walsh(x[:st["live"]])
             s = (t.abs().amax(-1, keepdim=True) / 7.5).half().double()
-            level = torch.floor(t / s).clamp(-8, 7) + 0.5  # a step's middle
+            level = torch.floor(t / s + 0.5).clamp(-8, 7)
             out.append(_walsh(torch.where(s > 0, level * s, 0.0)))
         return out
     f = st["fields"]
@@ -433,7 +433,7 @@ def exact(case, seed):
                 codes = f[name + "_codes"][0, pages].transpose(0, 1).flatten(1, 2)[:, :n]
                 x = torch.empty(*codes.shape[:2], d, dtype=torch.float64, device=DEV)
                 x[..., 0::2], x[..., 1::2] = codes % 16, codes // 16
-                return _walsh((x - 7.5) * f[name + "_scales"][0, pages].transpose(0, 1).flatten(1)[:, :n, None].double())
+                return _walsh((x - 8) * f[name + "_scales"][0, pages].transpose(0, 1).flatten(1)[:, :n, None].double())
 
             k, v = whole("key"), whole("value")
             j = torch.arange(n, device=DEV)
