@@ -618,7 +618,7 @@ int nq_prompt_attention(const nq_prompt_desc* desc, void* stream);
  */
 typedef struct nq_pool {
     int32_t layers, pages, heads, tokens, head_dim; /* head_dim 64, 128 or 256 */
-    int32_t reserved;
+    int32_t reserved;     /* 0; 4: a pool of 4 bits a coordinate, see nq_fourbit_append */
     int8_t* key_codes;    /* [layers, pages, heads, tokens, head_dim] */
     int8_t* value_codes;
     void* key_scales;     /* fp16 [layers, pages, heads, tokens] */
@@ -721,6 +721,118 @@ int32_t nq_shared_attention_chunk_tokens(int32_t kind);
 int32_t nq_shared_attention_rows(int32_t head_dim, int32_t kind);
 int64_t nq_shared_attention_workspace(int32_t n_slots, int32_t q_heads, int32_t head_dim);
 int nq_shared_attention(const nq_shared_desc* desc, void* stream);
+
+/*
+ * Rotary positions: out [rows, 2, half] fp32 is cos, then sin, of
+ * positions[axis_of[i] * axis_stride + r] * inv_freq[i] (the fp32 product of
+ * fp32 numbers), for half <= 128 frequencies of up to 255 axes.  positions:
+ * device int32 or int64; inv_freq, axis_of: HOST arrays of `half`, read during
+ * the call.
+ */
+int nq_rotation(const void* positions, int32_t int64_positions, int32_t axes, int64_t axis_stride, int64_t rows,
+                int32_t half, const float* inv_freq, const uint8_t* axis_of, float* out, void* stream);
+
+/*
+ * Queries and keys rotated by nq_rotation's angles [rows, 2, head_dim / 2]:
+ * (a, b) = (x[i], x[i + head_dim / 2]) becomes (a cos - b sin, b cos + a sin),
+ * with inverse != 0 (a cos + b sin, b cos - a sin), the forward's gradient.
+ * fp16, bf16 or fp32, rounded once.  Strides of a row and of a head in
+ * elements; head vectors 16-byte aligned.  An output may be its own input.
+ *
+ * Replaces: forward_rope / inverse_rope    rope_utils.py:75-249 (one axis)
+ */
+typedef struct nq_rotate_desc {
+    int32_t rows, q_heads, k_heads, head_dim; /* head_dim 64, 128 or 256 */
+    int32_t dtype, inverse;
+    const void* q;
+    const void* k;
+    void* q_out;
+    void* k_out;
+    const float* angles;
+    int64_t q_stride[2], k_stride[2], q_out_stride[2], k_out_stride[2];
+} nq_rotate_desc;
+int nq_rotate(const nq_rotate_desc* desc, void* stream);
+
+/*
+ * A pool whose pages hold 4 bits a coordinate is an nq_pool with reserved 4,
+ * codes of head_dim / 2 bytes a row (uint8) and positions NULL.  A row x of d coordinates is held as t = H x, H the orthonormal
+ * Walsh-Hadamard matrix: scale s = fp16(max |t| / 7.5) (at most 65504; NaN
+ * where t is not finite) and n = clamp(floor(t / s + 8.5), 0, 15), coordinate i
+ * in nibble i % 2 of byte i / 2.  It stands for H ((n - 8) s).
+ * nq_pool_copy_pages and nq_pool_compact (renumber 0) take such pools.
+ *
+ * nq_fourbit_append encodes tokens into their slots of a layer: keys [rows,
+ * heads, d] rotated by angles (NULL: not), values as they are; queries
+ * [rows, q_heads, d] (0 heads: none) are rotated into q_out.  slots: device
+ * int32 [rows], page * tokens + offset; negative ones and those past the pool
+ * are skipped; distinct.  Strides of a row and of a head in elements, head
+ * vectors 16-byte aligned; q_out may be q.
+ *
+ * nq_fourbit_read writes what slots stand for, keys and values [n, heads, d]
+ * of type dtype; rows of skipped slots are zero.
+ */
+typedef struct nq_fourbit_append_desc {
+    const nq_pool* pool;
+    int32_t layer, rows, q_heads, dtype; /* NQ_F16 / NQ_BF16 */
+    const void* q;
+    const void* k;
+    const void* v;
+    void* q_out;
+    const float* angles;
+    const int32_t* slots;
+    int64_t q_stride[2], k_stride[2], v_stride[2], q_out_stride[2];
+    float hadamard_scale;
+    int32_t reserved;
+} nq_fourbit_append_desc;
+int nq_fourbit_append(const nq_fourbit_append_desc* desc, void* stream);
+int nq_fourbit_read(const nq_pool* pool, int32_t layer, const int32_t* slots, int32_t n, int32_t dtype,
+                    float hadamard_scale, void* keys, void* values, void* stream);
+
+/*
+ * Attention of packed queries over such a pool: softmax(scale * q . k) . v
+ * over the tokens that a query sees, query head h reading kv head
+ * h / (q_heads / heads).  A sequence's queries see its tokens up to
+ * last + (causal ? i : 0), i the query's number, and with sliding_window W the
+ * last W of them; a query that sees none is zero.
+ *   items  [(n_wide + n_few) * 12] a tile of a sequence's rows (a row: a query
+ *          token and one of the q_heads / heads heads of a kv head, heads
+ *          fastest) and a chunk of its tokens: those of up to
+ *          nq_fourbit_rows(0) rows, then those of up to nq_fourbit_rows(1)
+ *          rows and nq_fourbit_chunk_tokens() tokens
+ *            [0] where the sequence's pages start in `pages`
+ *            [1] the chunk's first token   [2] its tokens, 1 or more
+ *            [3] the sequence's first query row   [4] the tile's first row
+ *            [5] its rows, 1 or more
+ *            [6], [7] query token i's partial sums of this chunk are slot
+ *                [6] + i * [7]
+ *            [8] the last token that query token 0 sees
+ *   joins  [n_joins * 4] query row, its first slot, its slots (consecutive; 0:
+ *          the row is zero), 0
+ * Device int32 arrays.  query, out: fp16 or bf16, strides of a row and of a
+ * head in elements, head vectors 16- and 8-byte aligned; rows in no join are
+ * left as they are; out may be query.  workspace: nq_fourbit_workspace(n_slots,
+ * q_heads, d) bytes, 16-byte aligned.
+ */
+typedef struct nq_fourbit_desc {
+    const nq_pool* pool;
+    int32_t layer, q_heads, q_dtype; /* NQ_F16 / NQ_BF16 */
+    int32_t n_wide, n_few, n_joins, n_slots;
+    int32_t causal, sliding_window;
+    float scale, hadamard_scale;
+    int32_t reserved;
+    const void* query;
+    void* out;
+    const int32_t* items;
+    const int32_t* pages;
+    const int32_t* joins;
+    int64_t q_stride[2], out_stride[2];
+    void* workspace;
+    int64_t workspace_bytes;
+} nq_fourbit_desc;
+int32_t nq_fourbit_rows(int32_t kind);
+int32_t nq_fourbit_chunk_tokens(void);
+int64_t nq_fourbit_workspace(int32_t n_slots, int32_t q_heads, int32_t head_dim);
+int nq_fourbit_attention(const nq_fourbit_desc* desc, void* stream);
 
 /* Library version and the last error message of the calling thread. */
 int nq_abi_version(void);

@@ -34,6 +34,7 @@ SOURCE_FLAGS = {
     "nq_score.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "nq_keykey.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "nq_prompt.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "nq_fourbit.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "nq_shared.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 

@@ -128,7 +128,7 @@ __device__ __forceinline__ int32_t plan_at(const InlineArgs& a, uint32_t i) { re
 template <int D, bool COMPACT, typename Args>
 __global__ __launch_bounds__(256) void pool_move_kernel(Args a) {
     constexpr int UR = D / 16;                    // 16-byte units a row
-    constexpr int PER = kMoveTokens * UR / 256;   // of a role and head, per thread
+    constexpr int PER = (kMoveTokens * UR + 255) / 256;  // of a role and head, per thread (D 32: half of the threads have one)
     __shared__ uint64_t s_src[kMoveTokens], s_dst[kMoveTokens];  // row index of head 0, page by page
     const uint32_t tile = blockIdx.x / a.head_split, part = blockIdx.x % a.head_split;
     const uint32_t layer = blockIdx.y;
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(256) void pool_move_kernel(Args a) {
             const uint64_t dpage = (uint32_t)plan_at(a, a.tables_at + (uint32_t)plan_at(a, s + 4) + dp);
             s_src[threadIdx.x] = spage * a.heads * a.src_tokens + so;
             s_dst[threadIdx.x] = dpage * a.heads * a.dst_tokens + d0;
-            if (layer == 0 && part == 0)
+            if (layer == 0 && part == 0 && a.dst.positions)
                 a.dst.positions[dpage * a.dst_tokens + d0] =
                     a.renumber ? (int32_t)j : a.src.positions[spage * a.src_tokens + so];
         }
@@ -206,6 +206,9 @@ template <bool COMPACT, typename Args>
 static hipError_t launch_move(const Args& a, uint32_t tiles, uint32_t layers, hipStream_t s) {
     const dim3 grid(tiles * a.head_split, layers);
     switch (a.d) {
+        case 32:
+            if constexpr (COMPACT) hipLaunchKernelGGL((pool_move_kernel<32, COMPACT, Args>), grid, dim3(256), 0, s, a);
+            break;
         case 64: hipLaunchKernelGGL((pool_move_kernel<64, COMPACT, Args>), grid, dim3(256), 0, s, a); break;
         case 128: hipLaunchKernelGGL((pool_move_kernel<128, COMPACT, Args>), grid, dim3(256), 0, s, a); break;
         default: hipLaunchKernelGGL((pool_move_kernel<256, COMPACT, Args>), grid, dim3(256), 0, s, a); break;
@@ -228,6 +231,10 @@ static void launch_copy(dim3 grid, hipStream_t s, const CopyArgs& a, uint32_t la
     else hipLaunchKernelGGL((pool_copy_kernel<ScaleUnit, false>), grid, dim3(256), 0, s, a, layers);
 }
 
+// A row's bytes of codes: a pool of 4 bits a coordinate has half of them, and no positions.
+static bool four_bit(const nq_pool* p) { return p->reserved == 4; }
+static uint32_t row_bytes(const nq_pool* p) { return (uint32_t)(four_bit(p) ? p->head_dim / 2 : p->head_dim); }
+
 static int check_pool(const nq_pool* p, const char* who) {
     NQ_CHECK_ARG(p != nullptr, "%s: pool is NULL", who);
     NQ_CHECK_ARG(p->head_dim == 64 || p->head_dim == 128 || p->head_dim == 256,
@@ -238,7 +245,7 @@ static int check_pool(const nq_pool* p, const char* who) {
     NQ_CHECK_ARG((uint64_t)p->heads * p->tokens * p->head_dim < (1ull << 31) &&
                      (uint64_t)p->pages * p->tokens < (1ull << 31),
                  "%s: a page's codes and the pool's slots must each stay below 2^31", who);
-    NQ_CHECK_ARG(p->key_codes && p->value_codes && p->key_scales && p->value_scales && p->positions,
+    NQ_CHECK_ARG(p->key_codes && p->value_codes && p->key_scales && p->value_scales && (p->positions || four_bit(p)),
                  "%s: the pool's arrays are required", who);
     NQ_CHECK_ARG((((uintptr_t)p->key_codes | (uintptr_t)p->value_codes | (uintptr_t)p->key_scales |
                    (uintptr_t)p->value_scales) & 15u) == 0 && ((uintptr_t)p->positions & 3u) == 0,
@@ -288,7 +295,7 @@ extern "C" int nq_pool_copy_pages(const nq_pool* p, const int32_t* src, const in
 
     CopyArgs a = {};
     a.p = pool_ptrs(p);
-    a.code_bytes = (uint32_t)p->heads * p->tokens * p->head_dim;
+    a.code_bytes = (uint32_t)p->heads * p->tokens * row_bytes(p);
     a.scale_bytes = (uint32_t)p->heads * p->tokens * 2u;
     a.tokens = (uint32_t)p->tokens;
     // scales in the widest pieces that every page's offset allows
@@ -310,7 +317,7 @@ extern "C" int nq_pool_copy_pages(const nq_pool* p, const int32_t* src, const in
         const uint32_t pages = 2u * (uint32_t)p->layers * a.pairs;
         a.code_units = pages * (a.code_bytes / 16);
         a.scale_units = pages * (a.scale_bytes / width);
-        a.pos_units = a.pairs * a.tokens;
+        a.pos_units = four_bit(p) ? 0u : a.pairs * a.tokens;
         a.code_blocks = (a.code_units + 1023u) / 1024u;
         a.scale_blocks = (a.scale_units + 1023u) / 1024u;
         const dim3 grid(a.code_blocks + a.scale_blocks + (a.pos_units + 255u) / 256u);
@@ -334,6 +341,7 @@ extern "C" int nq_pool_compact(const nq_pool* p, const int32_t* plan, int32_t pl
     NQ_CHECK_ARG(n_tiles >= 0 && kept_stride >= 0, "nq_pool_compact: n_tiles %d, kept_stride %d", n_tiles, kept_stride);
     if (n_tiles == 0) return NQ_OK;
     NQ_CHECK_ARG(plan && kept, "nq_pool_compact: the plan and the kept list are required");
+    NQ_CHECK_ARG(!four_bit(p) || !renumber, "nq_pool_compact: a pool of 4 bits a coordinate stores keys rotated and cannot renumber");
     NQ_CHECK_ARG(n_seq > 0 && plan_ints > 0 && (int64_t)n_tiles + 5ll * n_seq <= plan_ints,
                  "nq_pool_compact: %d integers hold no plan of %d tiles and %d sequences", plan_ints, n_tiles, n_seq);
     NQ_CHECK_ARG(!plan_on_host || plan_ints <= kPlanInts, "nq_pool_compact: a host plan has at most %d integers, got %d",
@@ -342,7 +350,7 @@ extern "C" int nq_pool_compact(const nq_pool* p, const int32_t* plan, int32_t pl
     a.src = a.dst = pool_ptrs(p);
     a.src_tokens = a.dst_tokens = (uint32_t)p->tokens;
     a.heads = (uint32_t)p->heads;
-    a.d = (uint32_t)p->head_dim;
+    a.d = row_bytes(p);
     a.renumber = renumber;
     a.plan = plan;
     a.seq_at = (uint32_t)n_tiles;
@@ -359,10 +367,11 @@ extern "C" int nq_pool_write(const nq_pool* p, int32_t layer, const nq_pool* tok
                              int32_t slots_on_host, int32_t n, void* stream) {
     using namespace nq;
     if (int st = check_pool(p, "nq_pool_write")) return st;
+    NQ_CHECK_ARG(!four_bit(p), "nq_pool_write: a pool of 4 bits a coordinate is written by nq_fourbit_append");
     NQ_CHECK_ARG(n >= 0 && layer >= 0 && layer < p->layers, "nq_pool_write: n %d, layer %d of %d", n, layer, p->layers);
     if (n == 0) return NQ_OK;
     if (int st = check_pool(tokens, "nq_pool_write")) return st;
-    NQ_CHECK_ARG(tokens->layers == 1 && tokens->pages == 1 && tokens->tokens == n && tokens->heads == p->heads &&
+    NQ_CHECK_ARG(!four_bit(tokens) && tokens->layers == 1 && tokens->pages == 1 && tokens->tokens == n && tokens->heads == p->heads &&
                      tokens->head_dim == p->head_dim,
                  "nq_pool_write: the tokens must be one page of n tokens of the pool's heads and head_dim");
     NQ_CHECK_ARG(slots != nullptr, "nq_pool_write: slots are required");

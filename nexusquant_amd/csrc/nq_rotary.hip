@@ -1,0 +1,461 @@
+// Rotary positions with one or several axes, and new tokens into a cache held in 4 bits with their rotation on the way.
+//
+//   angles   cos, sin of pos[axis(i)] * inv_freq[i], once for all layers of a step
+//   rotate   (a, b) = (x[i], x[i + d / 2]) -> (a c - b s, b c + a s); the inverse, its gradient, with -s
+//   append   queries rotated; keys rotated, transformed, encoded and stored in their slots; values likewise, unrotated
+//   read     what slots hold, as values again
+// Bytes bound all of them where there are many rows, the launch where there are few.
+#include "nq_fourbit.h"
+#include "nq_rowmath.h"
+
+namespace nq {
+
+// ----------------------------------------------------------------- angles ----
+
+struct AngleArgs {
+    const void* positions;  // [axes, rows], int32 or int64
+    float* out;             // [rows, 2, half]: cosines, sines
+    int64_t stride;         // of an axis, elements
+    uint32_t rows, half;
+    FastDiv by_half;
+    int32_t wide;           // int64 positions
+    float freq[128];
+    uint8_t axis[128];
+};
+
+// The angle is the fp32 product of fp32 numbers, as models form it; its cosine and sine are taken in 64 bits and rounded
+// once (an angle of 10^5 has no digit to lose to a reduction in fp32).
+__global__ __launch_bounds__(256) void rotation_kernel(AngleArgs a) {
+    const uint32_t u = blockIdx.x * 256u + threadIdx.x;
+    if (u >= a.rows * a.half) return;
+    const uint32_t r = div(u, a.by_half), i = u - r * a.half;
+    const int64_t at = (int64_t)a.axis[i] * a.stride + r;
+    const float pos = a.wide ? (float)static_cast<const int64_t*>(a.positions)[at] : (float)static_cast<const int32_t*>(a.positions)[at];
+    double s, c;
+    sincos((double)(pos * a.freq[i]), &s, &c);
+    float* const o = a.out + (size_t)r * 2u * a.half + i;
+    o[0] = (float)c;
+    o[a.half] = (float)s;
+}
+
+// ----------------------------------------------------------------- rotate ----
+
+struct RotateArgs {
+    const uint8_t* x[2];    // queries, keys
+    uint8_t* y[2];
+    int64_t x_row[2], x_head[2], y_row[2], y_head[2];  // strides, bytes
+    const float* angles;    // [rows, 2, d / 2]
+    uint32_t rows, heads[2], parts;
+    float sign;             // -1: the inverse
+};
+
+template <int DT>
+__device__ __forceinline__ void store8(uint8_t* p, const float (&x)[8]) {
+    if constexpr (DT == NQ_F32) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const f32x2 v = {x[2 * k], x[2 * k + 1]};
+            if constexpr (DT == NQ_F16) w[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+            else w[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+        }
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// D / 16 lanes a row, eight pairs a lane: its cosines and sines stay in registers for the heads of the block's part.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
+    constexpr int LANES = D / 16, ROWS = 256 / LANES, SIZE = DT == NQ_F32 ? 4 : 2, UNROLL = DT == NQ_F32 ? 2 : 4;
+    const uint32_t row = (blockIdx.x / a.parts) * ROWS + threadIdx.x / LANES, part = blockIdx.x % a.parts, at = threadIdx.x % LANES;
+    if (row >= a.rows) return;
+    float c[8], s[8];
+    const float* const t = a.angles + (size_t)row * D + 8 * at;
+    load8f(t, c);
+    load8f(t + D / 2, s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] *= a.sign;
+    const uint32_t n = a.heads[0] + a.heads[1];
+#pragma unroll UNROLL
+    for (uint32_t h = part; h < n; h += a.parts) {
+        const bool key = h >= a.heads[0];
+        const uint32_t head = key ? h - a.heads[0] : h;
+        const uint8_t* const x = a.x[key] + row * a.x_row[key] + head * a.x_head[key] + 8 * SIZE * at;
+        uint8_t* const y = a.y[key] + row * a.y_row[key] + head * a.y_head[key] + 8 * SIZE * at;
+        float lo[8], hi[8], u[8], v[8];
+        load8<DT>(x, 0, lo);
+        load8<DT>(x, D / 2, hi);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            u[i] = __builtin_fmaf(lo[i], c[i], -(hi[i] * s[i]));
+            v[i] = __builtin_fmaf(hi[i], c[i], lo[i] * s[i]);
+        }
+        store8<DT>(y, u);
+        store8<DT>(y + D / 2 * SIZE, v);
+    }
+}
+
+// ----------------------------------------------------------------- append ----
+
+struct AppendArgs {
+    const uint8_t* x[3];                // keys, values, queries
+    int64_t row[3], head[3];            // strides, bytes
+    uint8_t* out;                       // rotated queries
+    int64_t out_row, out_head;
+    const float* angles;                // [rows, 2, d / 2], or NULL
+    const int32_t* slots;               // [rows]
+    FourBitRows pool;
+    uint32_t rows, q_heads, kv_heads;
+    uint32_t batches, waves;            // of 16 heads a token; waves that share a token's
+    uint32_t tokens, slot_end;
+    FastDiv by_tokens;
+    float hscale;
+};
+
+// A wave takes a token, and its heads sixteen at a time, a quad a head (nq_rowmath.h): keys, then values, then queries.
+// The token's cosines and sines stay in registers.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
+    constexpr int C = D / 32, HC = C / 2;
+    const int lane = threadIdx.x & 63, q = lane & 3;
+    const uint32_t wave = blockIdx.x * 4u + (threadIdx.x >> 6), token = wave / a.waves;
+    if (token >= a.rows) return;  // whole wave
+    float cs[HC][8], sn[HC][8];
+#pragma unroll
+    for (int c = 0; c < HC; ++c) {
+        if (a.angles) {
+            const float* const t = a.angles + (size_t)token * D + 32 * c + 8 * q;
+            load8f(t, cs[c]);
+            load8f(t + D / 2, sn[c]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                cs[c][i] = 1.0f;
+                sn[c][i] = 0.0f;
+            }
+        }
+    }
+    const int32_t slot = a.slots[token];
+    const bool stored = slot >= 0 && (uint32_t)slot < a.slot_end;
+    const uint32_t page = stored ? div((uint32_t)slot, a.by_tokens) : 0u, off = stored ? (uint32_t)slot - page * a.tokens : 0u;
+    const uint32_t total = 2u * a.kv_heads + a.q_heads;
+    for (uint32_t batch = wave % a.waves; batch < a.batches; batch += a.waves) {
+        const uint32_t want = 16u * batch + ((uint32_t)lane >> 2), h = min(want, total - 1u);
+        const uint32_t role = h < a.kv_heads ? 0u : h < 2u * a.kv_heads ? 1u : 2u;
+        const uint32_t head = h - role * a.kv_heads;
+        const int64_t row = role == 0 ? a.row[0] : role == 1 ? a.row[1] : a.row[2], step = role == 0 ? a.head[0] : role == 1 ? a.head[1] : a.head[2];
+        const uint8_t* const base = role == 0 ? a.x[0] : role == 1 ? a.x[1] : a.x[2];
+        const uint8_t* const x = base + token * row + head * step;
+        float v[C][8];
+#pragma unroll
+        for (int c = 0; c < C; ++c) load8<DT>(x, 32 * c + 8 * q, v[c]);
+        if (role != 1 && a.angles) {
+#pragma unroll
+            for (int c = 0; c < HC; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float lo = v[c][i], hi = v[c + HC][i];
+                    v[c][i] = __builtin_fmaf(lo, cs[c][i], -(hi * sn[c][i]));
+                    v[c + HC][i] = __builtin_fmaf(hi, cs[c][i], lo * sn[c][i]);
+                }
+        }
+        if (role == 2) {
+            if (want == h) {
+                uint8_t* const o = a.out + token * a.out_row + head * a.out_head;
+#pragma unroll
+                for (int c = 0; c < C; ++c) store8<DT>(o + 2 * (32 * c + 8 * q), v[c]);
+            }
+        }
+        if (16u * batch >= 2u * a.kv_heads) continue;  // whole wave: queries alone
+        fwht_row<C>(v, q);
+        // the largest |t| as an integer: infinities and NaNs are larger than any number
+        uint32_t big = 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[c][i] *= a.hscale;
+                big = max(big, __builtin_bit_cast(uint32_t, v[c][i]) & 0x7fffffffu);
+            }
+        big = max(big, dpp_u32<kQuadXor1>(big));
+        big = max(big, dpp_u32<kQuadXor2>(big));
+        const bool finite = big < 0x7f800000u;
+        const float amax = finite ? __builtin_bit_cast(float, big) : 0.0f;
+        const uint32_t s16 = f32_to_f16_bits(__builtin_fminf(amax / 7.5f, 65504.0f));
+        const float s = f16_bits_to_f32(s16);
+        const float inv = (s > 0.0f ? 1.0f / s : 0.0f) * quad_sign(q);  // the transform's sign (nq_rowmath.h)
+        uint32_t w[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            w[c] = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y = __builtin_fminf(__builtin_fmaxf(v[c][i] * inv + 8.5f, 0.0f), 15.0f);
+                w[c] |= (uint32_t)y << (4 * i);  // (truncates; what is past 15 is level 15)
+            }
+        }
+        if (stored && role < 2 && want == h) {
+            const size_t to = ((size_t)page * a.kv_heads + head) * a.tokens + off;
+            uint32_t* const codes = reinterpret_cast<uint32_t*>((role ? a.pool.codes[1] : a.pool.codes[0]) + to * (D / 2)) + q;
+#pragma unroll
+            for (int c = 0; c < C; ++c) codes[4 * c] = w[c];
+            if (q == 0) (role ? a.pool.scales[1] : a.pool.scales[0])[to] = finite ? (uint16_t)s16 : (uint16_t)0x7e00u;
+        }
+    }
+}
+
+// ------------------------------------------------------------------- read ----
+
+struct ReadArgs {
+    uint8_t* out[2];        // [rows, kv_heads, d]
+    const int32_t* slots;
+    FourBitRows pool;
+    uint32_t rows, kv_heads, tokens, slot_end;
+    FastDiv by_tokens, by_heads;
+    float hscale;
+};
+
+// A quad a row and role; sums of n - 8 are whole numbers of at most 2048, so fp16 holds them exactly, and each coordinate is rounded by its scale and by its type.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
+    constexpr int C = D / 32, SIZE = DT == NQ_F32 ? 4 : 2;
+    const int q = threadIdx.x & 3;
+    const uint32_t u = blockIdx.x * 64u + (threadIdx.x >> 2), n = a.rows * a.kv_heads, r = min(u, n - 1u);
+    const uint32_t token = div(r, a.by_heads), head = r - token * a.kv_heads;
+    const int32_t slot = a.slots[token];
+    const bool stored = slot >= 0 && (uint32_t)slot < a.slot_end;
+    const uint32_t page = stored ? div((uint32_t)slot, a.by_tokens) : 0u, off = stored ? (uint32_t)slot - page * a.tokens : 0u;
+    const size_t at = ((size_t)page * a.kv_heads + head) * a.tokens + off;
+#pragma unroll
+    for (int role = 0; role < 2; ++role) {
+        const uint32_t* const codes = reinterpret_cast<const uint32_t*>(a.pool.codes[role] + at * (D / 2)) + q;
+        half2v h[C][4];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const uint32_t w = codes[4 * c];
+            const half2v bias = {(__fp16)-kNibbleBias, (__fp16)-kNibbleBias};
+            const uint32_t p[4] = {nibble_pair<0>(w), nibble_pair<1>(w), nibble_pair<2>(w), nibble_pair<3>(w)};
+            // (0, 4), (1, 5), (2, 6), (3, 7) to (0, 1), (2, 3), (4, 5), (6, 7)
+            h[c][0] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(p[1], p[0], 0x05040100u)) + bias;
+            h[c][1] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(p[3], p[2], 0x05040100u)) + bias;
+            h[c][2] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(p[1], p[0], 0x07060302u)) + bias;
+            h[c][3] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(p[3], p[2], 0x07060302u)) + bias;
+        }
+        const float f = f16_bits_to_f32(a.pool.scales[role][at]) * a.hscale * quad_sign(q);
+        fwht_row_f16<C>(h, q);
+        if (u >= n) continue;
+        uint8_t* const o = a.out[role] + (size_t)r * D * SIZE;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                x[2 * k] = stored ? (float)h[c][k].x * f : 0.0f;
+                x[2 * k + 1] = stored ? (float)h[c][k].y * f : 0.0f;
+            }
+            store8<DT>(o + SIZE * (32 * c + 8 * q), x);
+        }
+    }
+}
+
+int check_fourbit_pool(const nq_pool* p, int32_t layer, const char* who) {
+    NQ_CHECK_ARG(p != nullptr, "%s: pool is NULL", who);
+    NQ_CHECK_ARG(p->reserved == 4, "%s: the pool holds 8 bits a coordinate", who);
+    NQ_CHECK_ARG(p->head_dim == 64 || p->head_dim == 128 || p->head_dim == 256, "%s: head_dim %d unsupported (64, 128, 256)", who, p->head_dim);
+    NQ_CHECK_ARG(p->layers > 0 && p->pages > 0 && p->heads > 0 && p->tokens > 0 && layer >= 0 && layer < p->layers,
+                 "%s: bad pool geometry, or layer %d of %d", who, layer, p->layers);
+    NQ_CHECK_ARG((uint64_t)p->pages * p->heads * p->tokens < (1ull << 31), "%s: a layer must have less than 2^31 token rows", who);
+    NQ_CHECK_ARG(p->key_codes && p->value_codes && p->key_scales && p->value_scales, "%s: the pool's arrays are required", who);
+    NQ_CHECK_ARG((((uintptr_t)p->key_codes | (uintptr_t)p->value_codes | (uintptr_t)p->key_scales | (uintptr_t)p->value_scales) & 15u) == 0,
+                 "%s: the pool's codes and scales must be 16-byte aligned", who);
+    return NQ_OK;
+}
+
+FourBitRows fourbit_rows(const nq_pool* p, int32_t layer) {
+    const size_t rows = (size_t)layer * p->pages * p->heads * p->tokens;
+    FourBitRows r = {};
+    r.codes[0] = reinterpret_cast<uint8_t*>(p->key_codes) + rows * (p->head_dim / 2);
+    r.codes[1] = reinterpret_cast<uint8_t*>(p->value_codes) + rows * (p->head_dim / 2);
+    r.scales[0] = static_cast<uint16_t*>(p->key_scales) + rows;
+    r.scales[1] = static_cast<uint16_t*>(p->value_scales) + rows;
+    return r;
+}
+
+#define NQ_BY_DIM(KERNEL, DT, d, ...)                                                     \
+    switch (d) {                                                                          \
+        case 64: hipLaunchKernelGGL((KERNEL<DT, 64>), __VA_ARGS__); break;                \
+        case 128: hipLaunchKernelGGL((KERNEL<DT, 128>), __VA_ARGS__); break;              \
+        default: hipLaunchKernelGGL((KERNEL<DT, 256>), __VA_ARGS__); break;               \
+    }
+
+// Blocks that share a row's heads: one until the launch has fewer than 1024.
+static uint32_t share(uint64_t blocks, uint32_t most) {
+    uint32_t n = 1;
+    while (n < most && blocks * n < 1024) n *= 2;
+    return n < most ? n : most;
+}
+
+}  // namespace nq
+
+extern "C" int nq_rotation(const void* positions, int32_t int64_positions, int32_t axes, int64_t axis_stride, int64_t rows,
+                           int32_t half, const float* inv_freq, const uint8_t* axis_of, float* out, void* stream) {
+    using namespace nq;
+    NQ_CHECK_ARG(axes >= 1 && axes <= 255 && rows >= 0 && half >= 1 && half <= 128, "nq_rotation: axes %d, rows %lld, half %d", axes,
+                 (long long)rows, half);
+    NQ_CHECK_ARG((uint64_t)rows * half < (1ull << 32) - 256, "nq_rotation: %lld rows are too many", (long long)rows);
+    if (rows == 0) return NQ_OK;
+    NQ_CHECK_ARG(positions && inv_freq && axis_of && out, "nq_rotation: positions, inv_freq, axis_of and out are required");
+    AngleArgs a = {};
+    a.positions = positions;
+    a.out = out;
+    a.stride = axis_stride;
+    a.rows = (uint32_t)rows;
+    a.half = (uint32_t)half;
+    a.by_half = fast_div((uint32_t)half);
+    a.wide = int64_positions;
+    for (int32_t i = 0; i < half; ++i) {
+        NQ_CHECK_ARG(axis_of[i] < axes, "nq_rotation: frequency %d is of axis %d of %d", i, axis_of[i], axes);
+        a.freq[i] = inv_freq[i];
+        a.axis[i] = axis_of[i];
+    }
+    hipLaunchKernelGGL(rotation_kernel, dim3((uint32_t)(((uint64_t)rows * half + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a);
+    NQ_CHECK_HIP(hipGetLastError());
+    return NQ_OK;
+}
+
+extern "C" int nq_rotate(const nq_rotate_desc* d, void* stream) {
+    using namespace nq;
+    NQ_CHECK_ARG(d != nullptr, "nq_rotate: desc is NULL");
+    NQ_CHECK_ARG(d->head_dim == 64 || d->head_dim == 128 || d->head_dim == 256, "nq_rotate: head_dim %d unsupported (64, 128, 256)", d->head_dim);
+    NQ_CHECK_ARG(d->dtype == NQ_F16 || d->dtype == NQ_BF16 || d->dtype == NQ_F32, "nq_rotate: unknown dtype %d", d->dtype);
+    NQ_CHECK_ARG(d->rows >= 0 && d->q_heads >= 0 && d->k_heads >= 0, "nq_rotate: rows %d, q_heads %d, k_heads %d", d->rows, d->q_heads, d->k_heads);
+    if (d->rows == 0 || d->q_heads + (int64_t)d->k_heads == 0) return NQ_OK;
+    NQ_CHECK_ARG((int64_t)d->q_heads + d->k_heads < (1ll << 31), "nq_rotate: too many heads");
+    NQ_CHECK_ARG(d->angles && (d->q_heads == 0 || (d->q && d->q_out)) && (d->k_heads == 0 || (d->k && d->k_out)),
+                 "nq_rotate: angles, and inputs and outputs of all heads, are required");
+    const int64_t size = d->dtype == NQ_F32 ? 4 : 2;
+    const int64_t all = (d->q_stride[0] | d->q_stride[1] | d->k_stride[0] | d->k_stride[1] | d->q_out_stride[0] | d->q_out_stride[1] |
+                         d->k_out_stride[0] | d->k_out_stride[1]) * size;
+    NQ_CHECK_ARG(((all | (int64_t)(uintptr_t)d->q | (int64_t)(uintptr_t)d->k | (int64_t)(uintptr_t)d->q_out | (int64_t)(uintptr_t)d->k_out |
+                   (int64_t)(uintptr_t)d->angles) & 15) == 0,
+                 "nq_rotate: head vectors and angles must be 16-byte aligned");
+    RotateArgs a = {};
+    a.x[0] = static_cast<const uint8_t*>(d->q);
+    a.x[1] = static_cast<const uint8_t*>(d->k);
+    a.y[0] = static_cast<uint8_t*>(d->q_out);
+    a.y[1] = static_cast<uint8_t*>(d->k_out);
+    a.x_row[0] = d->q_stride[0] * size;
+    a.x_head[0] = d->q_stride[1] * size;
+    a.x_row[1] = d->k_stride[0] * size;
+    a.x_head[1] = d->k_stride[1] * size;
+    a.y_row[0] = d->q_out_stride[0] * size;
+    a.y_head[0] = d->q_out_stride[1] * size;
+    a.y_row[1] = d->k_out_stride[0] * size;
+    a.y_head[1] = d->k_out_stride[1] * size;
+    a.angles = d->angles;
+    a.rows = (uint32_t)d->rows;
+    a.heads[0] = (uint32_t)d->q_heads;
+    a.heads[1] = (uint32_t)d->k_heads;
+    a.sign = d->inverse ? -1.0f : 1.0f;
+    const uint32_t per = 256u / (uint32_t)(d->head_dim / 16);
+    const uint64_t blocks = ((uint64_t)d->rows + per - 1) / per;
+    a.parts = share(blocks, a.heads[0] + a.heads[1]);
+    NQ_CHECK_ARG(blocks * a.parts <= max_blocks(256), "nq_rotate: grid too large");
+    const dim3 grid((uint32_t)(blocks * a.parts));
+    hipStream_t s = (hipStream_t)stream;
+    if (d->dtype == NQ_F16) NQ_BY_DIM(rotate_kernel, NQ_F16, d->head_dim, grid, dim3(256), 0, s, a)
+    else if (d->dtype == NQ_BF16) NQ_BY_DIM(rotate_kernel, NQ_BF16, d->head_dim, grid, dim3(256), 0, s, a)
+    else NQ_BY_DIM(rotate_kernel, NQ_F32, d->head_dim, grid, dim3(256), 0, s, a)
+    NQ_CHECK_HIP(hipGetLastError());
+    return NQ_OK;
+}
+
+extern "C" int nq_fourbit_append(const nq_fourbit_append_desc* d, void* stream) {
+    using namespace nq;
+    NQ_CHECK_ARG(d != nullptr, "nq_fourbit_append: desc is NULL");
+    if (int st = check_fourbit_pool(d->pool, d->layer, "nq_fourbit_append")) return st;
+    const nq_pool* p = d->pool;
+    const int32_t dim = p->head_dim;
+    NQ_CHECK_ARG(d->dtype == NQ_F16 || d->dtype == NQ_BF16, "nq_fourbit_append: dtype must be fp16 or bf16");
+    NQ_CHECK_ARG(d->rows >= 0 && d->q_heads >= 0, "nq_fourbit_append: rows %d, q_heads %d", d->rows, d->q_heads);
+    if (d->rows == 0) return NQ_OK;
+    NQ_CHECK_ARG(d->k && d->v && d->slots && (d->q_heads == 0 || (d->q && d->q_out && d->angles)),
+                 "nq_fourbit_append: keys, values, slots, and for queries an output and angles, are required");
+    const int64_t all = d->k_stride[0] | d->k_stride[1] | d->v_stride[0] | d->v_stride[1] | d->q_stride[0] | d->q_stride[1] |
+                        d->q_out_stride[0] | d->q_out_stride[1];
+    NQ_CHECK_ARG(((2 * all | (int64_t)(uintptr_t)d->k | (int64_t)(uintptr_t)d->v | (int64_t)(uintptr_t)d->q | (int64_t)(uintptr_t)d->q_out |
+                   (int64_t)(uintptr_t)d->angles) & 15) == 0,
+                 "nq_fourbit_append: head vectors and angles must be 16-byte aligned");
+    AppendArgs a = {};
+    a.x[0] = static_cast<const uint8_t*>(d->k);
+    a.x[1] = static_cast<const uint8_t*>(d->v);
+    a.x[2] = static_cast<const uint8_t*>(d->q);
+    const int64_t* const strides[3] = {d->k_stride, d->v_stride, d->q_stride};
+    for (int i = 0; i < 3; ++i) {
+        a.row[i] = 2 * strides[i][0];
+        a.head[i] = 2 * strides[i][1];
+    }
+    a.out = static_cast<uint8_t*>(d->q_out);
+    a.out_row = 2 * d->q_out_stride[0];
+    a.out_head = 2 * d->q_out_stride[1];
+    a.angles = d->angles;
+    a.slots = d->slots;
+    a.pool = fourbit_rows(p, d->layer);
+    a.rows = (uint32_t)d->rows;
+    a.q_heads = (uint32_t)d->q_heads;
+    a.kv_heads = (uint32_t)p->heads;
+    NQ_CHECK_ARG(2ll * p->heads + d->q_heads < (1ll << 30), "nq_fourbit_append: too many heads");
+    a.batches = (2u * a.kv_heads + a.q_heads + 15u) / 16u;
+    a.waves = share(((uint64_t)d->rows + 3) / 4, a.batches);
+    a.tokens = (uint32_t)p->tokens;
+    a.slot_end = (uint32_t)p->pages * (uint32_t)p->tokens;
+    a.by_tokens = fast_div(a.tokens);
+    a.hscale = d->hadamard_scale;
+    const uint64_t blocks = ((uint64_t)d->rows * a.waves + 3) / 4;
+    NQ_CHECK_ARG(blocks <= max_blocks(256) && (uint64_t)d->rows * a.waves < (1ull << 32), "nq_fourbit_append: grid too large");
+    const dim3 grid((uint32_t)blocks);
+    hipStream_t s = (hipStream_t)stream;
+    if (d->dtype == NQ_F16) NQ_BY_DIM(append_kernel, NQ_F16, dim, grid, dim3(256), 0, s, a)
+    else NQ_BY_DIM(append_kernel, NQ_BF16, dim, grid, dim3(256), 0, s, a)
+    NQ_CHECK_HIP(hipGetLastError());
+    return NQ_OK;
+}
+
+extern "C" int nq_fourbit_read(const nq_pool* p, int32_t layer, const int32_t* slots, int32_t n, int32_t dtype, float hadamard_scale,
+                               void* keys, void* values, void* stream) {
+    using namespace nq;
+    if (int st = check_fourbit_pool(p, layer, "nq_fourbit_read")) return st;
+    NQ_CHECK_ARG(dtype == NQ_F16 || dtype == NQ_BF16 || dtype == NQ_F32, "nq_fourbit_read: unknown dtype %d", dtype);
+    NQ_CHECK_ARG(n >= 0 && (uint64_t)n * p->heads < (1ull << 32) - 64, "nq_fourbit_read: %d rows of %d heads", n, p->heads);
+    if (n == 0) return NQ_OK;
+    NQ_CHECK_ARG(slots && keys && values, "nq_fourbit_read: slots, keys and values are required");
+    NQ_CHECK_ARG((((uintptr_t)keys | (uintptr_t)values) & 15u) == 0, "nq_fourbit_read: keys and values must be 16-byte aligned");
+    ReadArgs a = {};
+    a.out[0] = static_cast<uint8_t*>(keys);
+    a.out[1] = static_cast<uint8_t*>(values);
+    a.slots = slots;
+    a.pool = fourbit_rows(p, layer);
+    a.rows = (uint32_t)n;
+    a.kv_heads = (uint32_t)p->heads;
+    a.tokens = (uint32_t)p->tokens;
+    a.slot_end = (uint32_t)p->pages * (uint32_t)p->tokens;
+    a.by_tokens = fast_div(a.tokens);
+    a.by_heads = fast_div(a.kv_heads);
+    a.hscale = hadamard_scale;
+    const uint64_t blocks = ((uint64_t)n * p->heads + 63) / 64;
+    NQ_CHECK_ARG(blocks <= max_blocks(256), "nq_fourbit_read: grid too large");
+    const dim3 grid((uint32_t)blocks);
+    const int32_t dim = p->head_dim;
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == NQ_F16) NQ_BY_DIM(read_kernel, NQ_F16, dim, grid, dim3(256), 0, s, a)
+    else if (dtype == NQ_BF16) NQ_BY_DIM(read_kernel, NQ_BF16, dim, grid, dim3(256), 0, s, a)
+    else NQ_BY_DIM(read_kernel, NQ_F32, dim, grid, dim3(256), 0, s, a)
+    NQ_CHECK_HIP(hipGetLastError());
+    return NQ_OK;
+}

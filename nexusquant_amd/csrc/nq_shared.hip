@@ -846,6 +846,7 @@ extern "C" int nq_shared_attention(const nq_shared_desc* d, void* stream) {
     using namespace nq;
     NQ_CHECK_ARG(d != nullptr && d->pool != nullptr, "nq_shared_attention: desc and pool are required");
     const nq_pool* p = d->pool;
+    NQ_CHECK_ARG(p->reserved == 0, "nq_shared_attention: a pool of 4 bits a coordinate is read by nq_fourbit_attention");
     NQ_CHECK_ARG(p->head_dim == 64 || p->head_dim == 128 || p->head_dim == 256,
                  "nq_shared_attention: head_dim %d unsupported (64, 128, 256)", p->head_dim);
     NQ_CHECK_ARG(p->layers > 0 && p->pages > 0 && p->heads > 0 && p->tokens > 0 && d->layer >= 0 && d->layer < p->layers,

@@ -1,0 +1,412 @@
+"""A cache held in 4 bits: a pool of pages, what writes it, and the attentions that read it.
+
+CompressedPagePool (page_pool.py) keeps keys without rotation, 8 bits a coordinate; its
+attention turns every key it reads.  Here keys are stored rotated and both keys and values
+as their Walsh-Hadamard transform in 16 levels with one fp16 scale a token and head: half the
+bytes (66 of 130 at head_dim 128), and an attention that undoes nothing a token.  What that
+gives up is re-rotation: compact keeps positions.
+
+    pool = FourBitPagePool(num_pages, num_heads=8, page_tokens=16, head_dim=128, num_layers=32)
+    rotation = plan_rotation(positions, 128, base=500000.0)      # once a step, for all layers
+    slots = pool.plan_slots(new_slots)
+    step = pool.plan_attention(tables, lengths)                  # lengths with the new tokens
+    q = pool.append(slots, key, value, rotation=rotation, query=query, layer=layer)
+    y = pool.attend(step, q, layer=layer)
+"""
+
+from __future__ import annotations
+
+import struct
+from typing import Dict, List, Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+
+from . import _lib
+from .hadamard import hadamard_constant
+from .ops import PlanTensor, on_device
+from .page_pool import PagePool
+from .rotary import Rotation, aligned, check_out, same_or_apart
+
+_HEAD_DIMS = (64, 128, 256)
+_DTYPES = (torch.float16, torch.bfloat16)
+
+
+class SlotPlan:
+    """Which slots some rows of tokens are stored in: made once a step, used by every layer."""
+
+    def __init__(self, pool: "FourBitPagePool", slots: np.ndarray):
+        self.pool = pool
+        self.rows = len(slots)
+        self.pages = np.unique(slots[slots >= 0] // pool.page_tokens)
+        self.slots = PlanTensor(slots.astype(np.int32), pool.device) if len(slots) else None
+        self.writable_at = -1  # the pool's references when its pages were found to be the sequence's own
+
+
+class FourBitAttentionPlan:
+    """Which tokens of a pool each query sees: valid for every layer while tables and lengths stay the same.
+    The device arrays are made for a number of query heads, the first time that it is used (before a graph is captured)."""
+
+    def __init__(self, pool: "FourBitPagePool", tables: List[np.ndarray], lengths: Sequence[int], queries: Sequence[int],
+                 causal: bool, window: int):
+        self.pool = pool
+        self.lengths, self.queries = tuple(lengths), tuple(queries)
+        self.causal, self.window = causal, window
+        self.rows = sum(queries)
+        self._tables = tables
+        self._work: Dict[int, tuple] = {}
+
+    def work(self, q_heads: int) -> tuple:
+        """(device ints, their places in bytes, counts of wide and few items and joins, slots, workspace bytes) for q_heads
+        query heads."""
+        got = self._work.get(q_heads)
+        if got is None:
+            pool = self.pool
+            with on_device(pool.device):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("attend: run the plan once before capturing it into a graph")
+            if q_heads == 0 or q_heads % pool.num_heads:
+                raise ValueError(f"num_heads {q_heads} is not a multiple of the pool's {pool.num_heads}")
+            lib = _lib.load()
+            parts, counts = attention_items([len(t) for t in self._tables], self.lengths, self.queries, self.causal, self.window,
+                                            q_heads // pool.num_heads, pool.num_heads, pool.head_dim,
+                                            [int(lib.nq_fourbit_rows(k)) for k in range(2)], int(lib.nq_fourbit_chunk_tokens()))
+            parts = [parts[0], np.concatenate(self._tables) if self._tables else np.zeros(0, np.int32), parts[1]]
+            places, at = [], 0
+            for v in parts:
+                places.append(at)
+                at += 4 * len(v)
+            ints = PlanTensor(np.concatenate(parts).astype(np.int32), pool.device) if at else None
+            got = self._work[q_heads] = (ints, places, counts, int(lib.nq_fourbit_workspace(counts[3], q_heads, pool.head_dim)))
+        return got
+
+
+# Workgroups of a launch that run at once (by registers), and the least tokens of a chunk.
+_AT_ONCE = {64: 1024, 128: 1024, 256: 512}
+_WIDE_AT_ONCE = {64: 768, 128: 512, 256: 256}
+_FEW_STEP, _WIDE_STEP, _WIDE_LEAST = 128, 64, 256
+
+
+def _chunk(spans: np.ndarray, heads: int, step: int, least: int, most: int, workgroups: int) -> int:
+    """Tokens of a chunk: the least multiple of `step`, `least` or more, with which the launch is one round of `workgroups`;
+    the longest span's where none is."""
+    lo, hi = -(-least // step), -(-min(most, max(int(spans.max()), least)) // step)
+    while lo < hi:
+        mid = (lo + hi) // 2
+        if heads * int((-(-spans // (mid * step))).sum()) > workgroups:
+            lo = mid + 1
+        else:
+            hi = mid
+    return min(lo * step, most)
+
+
+def attention_items(pages: Sequence[int], lengths: Sequence[int], queries: Sequence[int], causal: bool, window: int, group: int,
+                    heads: int, head_dim: int, rows: Sequence[int], most_tokens: int):
+    """The work list of nq_fourbit_attention, (items, joins) as flat int32 arrays, and the counts of wide items, few items,
+    joins and slots.
+
+    pages[b], lengths[b], queries[b]: a sequence's pages in the list, tokens and query tokens.  rows: most rows of a wide and
+    of a few tile; most_tokens: of a few tile's chunk."""
+    tiles = []  # kind, sequence, first query token, one past the last, first row, rows, first token, one past the last
+    joins = []
+    first_row = first_page = 0
+    starts, firsts = [], []
+    for b, (n, q) in enumerate(zip(lengths, queries)):
+        firsts.append(first_row)
+        starts.append(first_page)
+        joins += [(first_row + i, 0, 0, 0) for i in range(q)]
+        first_row += q
+        first_page += pages[b]
+        if n == 0 or q == 0:
+            continue
+        per = max(1, rows[0] // group) if q * group > rows[1] else q  # query tokens of a tile
+        for i0 in range(0, q, per):
+            i1 = min(i0 + per, q)
+            end = n - q + i1 if causal else n
+            start = max(0, n - q + i0 - window + 1) if window else 0
+            few = int((i1 - i0) * group <= rows[1])
+            for r0 in range(i0 * group, i1 * group, rows[0]):  # (more heads than a tile has rows: several, cut alike)
+                tiles.append((few, b, i0, i1, r0, min(rows[0], i1 * group - r0), start, end))
+    if not tiles:
+        return (np.zeros(0, np.int32), np.array(joins, np.int32).reshape(-1)), (0, 0, len(joins), 0)
+    t = np.array(tiles, dtype=np.int64)
+    t = t[np.lexsort((t[:, 6] - t[:, 7], t[:, 0]))]  # wide ones first, long ones before short ones
+    kind, span = t[:, 0], t[:, 7] - t[:, 6]
+    length = np.empty(len(t), np.int64)
+    few = kind == 1
+    if few.any():
+        length[few] = _chunk(span[few], heads, _FEW_STEP, _FEW_STEP, most_tokens, _AT_ONCE[head_dim])
+    if (~few).any():
+        length[~few] = _chunk(span[~few], heads, _WIDE_STEP, _WIDE_LEAST, 1 << 30, _WIDE_AT_ONCE[head_dim])
+    chunks = -(-span // length)
+    items, slots = [], 0
+    base: Dict[tuple, int] = {}
+    for k in range(len(t)):
+        _, b, i0, i1, r0, n_rows, start, end = (int(x) for x in t[k])
+        c, step = int(chunks[k]), int(length[k])
+        at = base.get((b, i0))
+        if at is None:
+            at = base[(b, i0)] = slots
+            slots += (i1 - i0) * c
+            for i in range(i0, i1):
+                joins[firsts[b] + i] = (firsts[b] + i, at + (i - i0) * c, c, 0)
+        last = lengths[b] - queries[b] if causal else lengths[b] - 1
+        for j in range(c):
+            first = start + j * step
+            items.append((starts[b], first, min(step, end - first), firsts[b], r0, n_rows, at - i0 * c + j, c, last, 0, 0, 0))
+    if slots >= 1 << 31:
+        raise ValueError("too many partial sums: split the queries over several plans")
+    n_few = int(chunks[few].sum())
+    return ((np.array(items, np.int32).reshape(-1), np.array(joins, np.int32).reshape(-1)),
+            (len(items) - n_few, n_few, len(joins), slots))
+
+
+# nq_fourbit_append_desc and nq_fourbit_desc, packed in one go and passed as bytes
+_APPEND_PACK = struct.Struct("P4i6P8qfi")
+_ATTEND_PACK = struct.Struct("P9i2fi5P4qPq")
+
+
+class FourBitPagePool(PagePool):
+    """num_pages pages of page_tokens tokens for num_heads kv heads, in num_layers layers, 4 bits a coordinate.
+
+    key_codes, value_codes    uint8 [layers, pages, heads, tokens, head_dim / 2], coordinate 2 i the low nibble of byte i
+    key_scales, value_scales  fp16 [layers, pages, heads, tokens]
+
+    A vector x is held as t = H x (H the orthonormal Walsh-Hadamard matrix): scale = fp16(max |t| / 7.5), nibble
+    n = clamp(floor(t / scale + 8.5), 0, 15), which stands for H ((n - 8) scale): half a scale off at most.  A vector with an infinity or a NaN has a
+    NaN scale; queries that see it get NaN.
+
+    Page numbers, fork, copy_pages, free: as CompressedPagePool.  compact keeps positions (keys are stored rotated)."""
+
+    def __init__(self, num_pages: int, num_heads: int, page_tokens: int, head_dim: int, num_layers: int = 1, device=None):
+        shape = (int(num_layers), int(num_pages), int(num_heads), int(page_tokens))
+        if min(shape) < 1:
+            raise ValueError(f"layers, pages, heads and tokens must be positive (got {shape})")
+        dev = torch.device("cuda" if device is None else device)
+        if dev.type != "cuda":
+            raise _lib.NexusQuantError(f"nexusquant_amd runs on MI355X (ROCm) devices only; the pool is on {dev}")
+        self._check_shape(shape, int(head_dim))
+        codes = shape + (int(head_dim) // 2,)
+        self._adopt(*(torch.zeros(codes, dtype=torch.uint8, device=dev) for _ in range(2)),
+                    *(torch.zeros(shape, dtype=torch.float16, device=dev) for _ in range(2)))
+
+    @classmethod
+    def from_tensors(cls, key_codes: torch.Tensor, value_codes: torch.Tensor, key_scales: torch.Tensor,
+                     value_scales: torch.Tensor) -> "FourBitPagePool":
+        """A pool over fields that exist already (used, not copied); all its pages are free."""
+        for name, t, dt, dims in (("key_codes", key_codes, torch.uint8, 5), ("value_codes", value_codes, torch.uint8, 5),
+                                  ("key_scales", key_scales, torch.float16, 4),
+                                  ("value_scales", value_scales, torch.float16, 4)):
+            if t.dtype != dt:
+                raise TypeError(f"{name} must be {dt}, got {t.dtype}")
+            if t.dim() != dims or not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f"{name} must be a contiguous, 16-byte aligned {dims}-d tensor, got {tuple(t.shape)}")
+            _lib.require_device(t, name)
+            if t.device != key_codes.device:
+                raise ValueError(f"{name} is on {t.device}, key_codes on {key_codes.device}")
+        shape = tuple(key_codes.shape[:4])
+        if min(shape) < 1:
+            raise ValueError(f"layers, pages, heads and tokens must be positive (got {shape})")
+        if value_codes.shape != key_codes.shape or tuple(key_scales.shape) != shape or tuple(value_scales.shape) != shape:
+            raise ValueError("fields must be [layers, pages, heads, tokens(, head_dim / 2)] of one shape")
+        cls._check_shape(shape, 2 * key_codes.shape[4])
+        pool = cls.__new__(cls)
+        pool._adopt(key_codes, value_codes, key_scales, value_scales)
+        return pool
+
+    @staticmethod
+    def _check_shape(shape, head_dim: int) -> None:
+        layers, pages, heads, tokens = shape
+        if head_dim not in _HEAD_DIMS:
+            raise NotImplementedError(f"head_dim {head_dim}: the gfx950 4-bit kernels take 64, 128 or 256")
+        if layers > 65535 or heads * tokens * head_dim >= 1 << 31 or pages * heads * tokens >= 1 << 31:
+            raise ValueError("a pool takes 65535 layers, pages of less than 2^31 coordinates and less than 2^31 "
+                             f"token rows a layer (got {shape})")
+
+    def _adopt(self, key_codes, value_codes, key_scales, value_scales) -> None:
+        self.key_codes, self.value_codes = key_codes, value_codes
+        self.key_scales, self.value_scales = key_scales, value_scales
+        self.head_dim = 2 * key_codes.shape[4]
+        self._start(key_codes, value_codes, key_scales, value_scales, None, bits=4)
+
+    def compact(self, tables: Sequence[Sequence[int]], lengths: Sequence[int], kept_idx: torch.Tensor, n_kept,
+                renumber: bool = False) -> Tuple[List[List[int]], List[int]]:
+        """As CompressedPagePool.compact; tokens keep their positions."""
+        if renumber:
+            raise ValueError("a pool in 4 bits stores keys rotated: renumber=True cannot rotate them again")
+        return super().compact(tables, lengths, kept_idx, n_kept)
+
+    # ------------------------------------------------------------------- tokens
+
+    def plan_slots(self, slots: Sequence[int]) -> SlotPlan:
+        """A plan of token i in slots[i] (page * page_tokens + offset, as `slots` gives them; -1: nowhere, a padded
+        batch).  Slots are distinct and in allocated pages.  Made before a graph is captured, not in the capture."""
+        s = np.asarray(slots.tolist() if torch.is_tensor(slots) else slots).reshape(-1)
+        if len(s) and s.dtype.kind not in "iu":
+            raise ValueError(f"slots must be integers, got {s.dtype}")
+        if len(s) and s.max() >= self.num_pages * self.page_tokens:  # (as the type they came in)
+            raise ValueError(f"slots must lie below {self.num_pages * self.page_tokens}")
+        s = np.maximum(s.astype(np.int64, copy=False), -1)
+        used = s[s >= 0]
+        if len(np.unique(used)) != len(used):
+            raise ValueError("plan_slots: slots must be distinct")
+        with self._lock:
+            self.in_use(np.unique(used // self.page_tokens), "plan_slots")
+        return SlotPlan(self, s)
+
+    def _check_plan(self, plan, kind, what: str, layer: int) -> None:
+        if not isinstance(plan, kind) or plan.pool is not self:
+            raise ValueError(f"{what}: the plan is not one of this pool")
+        if not 0 <= int(layer) < self.num_layers:
+            raise ValueError(f"layer {layer} of a pool of {self.num_layers}")
+
+    def append(self, plan: SlotPlan, key: torch.Tensor, value: torch.Tensor, rotation: Optional[Rotation] = None,
+               query: Optional[torch.Tensor] = None, layer: int = 0, out: Optional[torch.Tensor] = None
+               ) -> Optional[torch.Tensor]:
+        """Rotate, encode and store tokens in one layer: key, value [rows, heads, head_dim] (fp16 or bf16, any strides of
+        rows and heads) into the plan's slots, keys rotated by `rotation` (None: as they are, an encoder's states).
+        query [rows, q_heads, head_dim] is rotated along and returned, into `out` where that is given (it may be query).
+        The pages must have one reference.  One launch, without host work on the tokens: it can be captured into a graph;
+        replays then store into the same slots."""
+        self._check_plan(plan, SlotPlan, "append", layer)
+        dtype, dev, rows, d = key.dtype, self.device, plan.rows, self.head_dim
+        tensors = [("key", key), ("value", value)] + ([] if query is None else [("query", query)])
+        for name, t in tensors:
+            _lib.require_device(t, name)
+            if t.dim() != 3 or t.shape[0] != rows or t.shape[2] != d or (name != "query" and t.shape[1] != self.num_heads):
+                heads = "q_heads" if name == "query" else self.num_heads
+                raise ValueError(f"{name} must be ({rows} tokens, {heads}, {d}), got {tuple(t.shape)}")
+            if t.dtype != dtype or dtype not in _DTYPES:
+                raise ValueError(f"key, value and query must share an fp16 or bf16 dtype, got {t.dtype}")
+            if t.device != dev:
+                raise ValueError(f"{name} is on {t.device}, the pool on {dev}")
+        if torch.is_grad_enabled() and any(t.requires_grad for _, t in tensors):
+            raise NotImplementedError("append has no backward pass; call it under torch.no_grad()")
+        if rotation is None:
+            if query is not None:
+                raise ValueError("append: a query is rotated along with the keys; without a rotation it is not taken")
+        elif rotation.rows != rows or rotation.head_dim != d or rotation.device != dev:
+            raise ValueError(f"append: a rotation of {rotation.rows} rows of {rotation.head_dim} on {rotation.device} for {rows} of "
+                             f"{d} on {dev}")
+        if out is not None:
+            if query is None:
+                raise ValueError("append: out is the query's")
+            check_out(out, query, "out")
+            if not same_or_apart(out, query) or not all(same_or_apart(out, t) and out.data_ptr() != t.data_ptr()
+                                                        for t in (key, value) if t.numel()):
+                raise ValueError("append: out may be query itself, and must not overlap query, key or value otherwise")
+        with self._lock:
+            if plan.writable_at != self._changes:
+                if len(plan.pages):
+                    refs = self._referenced(plan.pages, "append")
+                    if refs.max() > 1:
+                        raise ValueError(f"append: page {int(plan.pages[refs > 1][0])} is shared and cannot be written")
+                plan.writable_at = self._changes
+            if query is not None and out is None:
+                out = torch.empty(query.shape, dtype=dtype, device=dev)
+            if rows == 0:
+                return out
+            k, v = aligned(key), aligned(value)
+            q = None if query is None else aligned(query)
+            none = (0, 0)
+            with on_device(dev):
+                st = _lib.load().nq_fourbit_append(_APPEND_PACK.pack(
+                    self.desc_at, int(layer), rows, 0 if q is None else q.shape[1], _lib.dtype_code(dtype),
+                    0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if q is None else out.data_ptr(),
+                    0 if rotation is None else rotation.angles.data_ptr(), plan.slots.address(),
+                    *(none if q is None else q.stride()[:2]), *k.stride()[:2], *v.stride()[:2],
+                    *(none if q is None else out.stride()[:2]), hadamard_constant(d), 0), _lib.current_stream_handle(dev))
+            _lib.check(st, "nq_fourbit_append")
+        return out
+
+    def read(self, plan: SlotPlan, layer: int = 0, dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(keys, values) [rows, heads, head_dim] that the plan's slots stand for, keys rotated as they were stored; fp16,
+        bf16 or fp32.  Rows of slot -1 are zero."""
+        self._check_plan(plan, SlotPlan, "read", layer)
+        code = _lib.dtype_code(dtype)
+        keys, values = (torch.empty(plan.rows, self.num_heads, self.head_dim, dtype=dtype, device=self.device) for _ in range(2))
+        if plan.rows:
+            with on_device(self.device):
+                st = _lib.load().nq_fourbit_read(self.desc, int(layer), plan.slots.address(), plan.rows, code,
+                                                 hadamard_constant(self.head_dim), keys.data_ptr(), values.data_ptr(),
+                                                 _lib.current_stream_handle(self.device))
+            _lib.check(st, "nq_fourbit_read")
+        return keys, values
+
+    # ---------------------------------------------------------------- attention
+
+    def plan_attention(self, tables: Sequence[Sequence[int]], lengths: Sequence[int], queries: Optional[Sequence[int]] = None,
+                       causal: bool = True, sliding_window: Optional[int] = None) -> FourBitAttentionPlan:
+        """The plan of packed queries over sequences of this pool.
+
+        Sequence b holds lengths[b] tokens in its pages tables[b] (entries past those are padding) and has queries[b]
+        query rows (None: one each), one sequence's after another's.  causal: they are its last tokens', and query i sees
+        the tokens up to its own, with sliding_window the last so many of them.  causal=False: every query sees all of the
+        sequence's tokens, whatever their numbers (cross attention to an encoder's states).  A sequence without tokens:
+        its queries' rows are zero."""
+        lens = [int(n) for n in (lengths.tolist() if torch.is_tensor(lengths) else lengths)]
+        news = [1] * len(lens) if queries is None else \
+            [int(n) for n in (queries.tolist() if torch.is_tensor(queries) else queries)]
+        if not len(tables) == len(lens) == len(news):
+            raise ValueError(f"{len(tables)} tables, {len(lens)} lengths and {len(news)} numbers of queries")
+        if sliding_window is not None and (int(sliding_window) <= 0 or not causal):
+            raise ValueError(f"sliding_window must be positive, and needs causal queries, got {sliding_window}")
+        flat = []
+        for b, (n, q) in enumerate(zip(lens, news)):
+            if not 0 <= n <= len(tables[b]) * self.page_tokens:
+                raise ValueError(f"sequence {b}: {n} tokens in {len(tables[b])} pages of {self.page_tokens}")
+            if q < 0 or (causal and q > n > 0):
+                raise ValueError(f"sequence {b}: {q} queries of {n} tokens")
+            flat.append(self.in_use(tables[b][:self.pages_for(n)], "plan_attention"))
+        if sum(news) >= 1 << 31:
+            raise ValueError(f"{sum(news)} query rows: a plan takes less than 2^31")
+        window = 0 if sliding_window is None or int(sliding_window) >= max(lens, default=0) else int(sliding_window)
+        return FourBitAttentionPlan(self, flat, lens, news, bool(causal), window)
+
+    def attend(self, plan: FourBitAttentionPlan, query: torch.Tensor, layer: int = 0, scale: Optional[float] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of query [rows, q_heads, head_dim] (fp16 or bf16, q_heads a multiple of the pool's, any strides of rows
+        and heads) over the plan's tokens in one layer.  scale: 1 / sqrt(head_dim) by default.
+
+        Returns [rows, q_heads, head_dim].  Rows behind the plan's are left as they are in `out`, and are zero without one;
+        `out` may be query.  Codes are exact in the products; queries (transformed) and weights are rounded to twice fp16's
+        11 bits where a kv head has up to 16 rows of a sequence, to 11 where it has more.  How a row's tokens are cut follows
+        from the whole plan: outputs of one row alone and in a batch agree to roundings.
+        A captured graph reads the plan's arrays: keep the plan while it is replayed.  Inference only."""
+        self._check_plan(plan, FourBitAttentionPlan, "attend", layer)
+        _lib.require_device(query, "query")
+        shape, dtype, dev = query.shape, query.dtype, self.device
+        if query.device != dev:
+            raise ValueError(f"query is on {query.device}, the pool on {dev}")
+        if len(shape) != 3 or shape[0] < plan.rows or shape[2] != self.head_dim:
+            raise ValueError(f"query must be ({plan.rows} rows or more, num_heads, {self.head_dim}), got {tuple(shape)}")
+        if dtype not in _DTYPES:
+            raise ValueError(f"attend takes fp16 or bf16 queries, got {dtype}")
+        if query.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError("attend has no backward pass; call it under torch.no_grad()")
+        scale = self.head_dim ** -0.5 if scale is None else float(scale)
+        if not 0.0 < scale < 1e30:
+            raise ValueError(f"scale must be positive, got {scale}")
+        hq = shape[1]
+        ints, places, counts, nbytes = plan._work.get(hq) or plan.work(hq)
+        if out is None:
+            out = torch.empty(shape, dtype=dtype, device=dev)
+            if shape[0] > plan.rows:
+                out[plan.rows:].zero_()
+        else:
+            check_out(out, query, "out", align=8)
+            if not same_or_apart(out, query):
+                raise ValueError("attend: out may be query itself, and must not overlap it otherwise")
+        if ints is None or plan.rows == 0:
+            return out
+        q = aligned(query)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None  # of this call alone
+        with on_device(dev):
+            base = ints.address()
+            st = _lib.load().nq_fourbit_attention(_ATTEND_PACK.pack(
+                self.desc_at, int(layer), hq, _lib.NQ_F16 if dtype == torch.float16 else _lib.NQ_BF16, *counts,
+                int(plan.causal), plan.window, scale, hadamard_constant(self.head_dim), 0, q.data_ptr(), out.data_ptr(),
+                base + places[0], base + places[1], base + places[2], *q.stride()[:2], *out.stride()[:2],
+                0 if ws is None else ws.data_ptr(), nbytes), _lib.current_stream_handle(dev))
+        _lib.check(st, "nq_fourbit_attention")
+        return out

@@ -43,86 +43,24 @@ def _refuse_capture(what: str, device: torch.device) -> None:
                 raise RuntimeError(f"{what} changes the pool's host state and cannot be captured into a graph")
 
 
-class CompressedPagePool:
-    """num_pages pages of page_tokens tokens for num_heads kv heads, in num_layers layers.
+class PagePool:
+    """The page numbers of a pool, their references, and its whole pages and tokens moved.
 
-    key_codes, value_codes    int8 [layers, pages, heads, tokens, head_dim]
-    key_scales, value_scales  fp16 [layers, pages, heads, tokens]
-    positions                 int32 [pages, tokens], shared by the layers
-    max_position              no stored position is larger (write() keeps it; raise it
-                              after writing into `positions` directly)
-    """
+    What a page holds is the subclass's: it sets head_dim and calls _start with its fields, codes
+    [layers, pages, heads, tokens, bytes] and scales [layers, pages, heads, tokens]."""
 
-    def __init__(self, num_pages: int, num_heads: int, page_tokens: int, head_dim: int, num_layers: int = 1,
-                 device=None):
-        shape = (int(num_layers), int(num_pages), int(num_heads), int(page_tokens))
-        if min(shape) < 1:
-            raise ValueError(f"layers, pages, heads and tokens must be positive (got {shape})")
-        dev = torch.device("cuda" if device is None else device)
-        if dev.type != "cuda":
-            raise _lib.NexusQuantError(f"nexusquant_amd runs on MI355X (ROCm) devices only; the pool is on {dev}")
-        self._check_shape(shape, int(head_dim))
-        self._adopt(torch.zeros(shape + (int(head_dim),), dtype=torch.int8, device=dev),
-                    torch.zeros(shape + (int(head_dim),), dtype=torch.int8, device=dev),
-                    torch.zeros(shape, dtype=torch.float16, device=dev),
-                    torch.zeros(shape, dtype=torch.float16, device=dev),
-                    torch.zeros(shape[1], shape[3], dtype=torch.int32, device=dev))
-        self.max_position = 0
-
-    @classmethod
-    def from_tensors(cls, key_codes: torch.Tensor, value_codes: torch.Tensor, key_scales: torch.Tensor,
-                     value_scales: torch.Tensor, positions: torch.Tensor) -> "CompressedPagePool":
-        """A pool over fields that exist already (used, not copied); all its pages are free.
-        Reads the largest position back."""
-        for name, t, dt, dims in (("key_codes", key_codes, torch.int8, 5), ("value_codes", value_codes, torch.int8, 5),
-                                  ("key_scales", key_scales, torch.float16, 4),
-                                  ("value_scales", value_scales, torch.float16, 4),
-                                  ("positions", positions, torch.int32, 2)):
-            if t.dtype != dt:
-                raise TypeError(f"{name} must be {dt}, got {t.dtype}")
-            if t.dim() != dims or not t.is_contiguous() or t.data_ptr() % 16:
-                raise ValueError(f"{name} must be a contiguous, 16-byte aligned {dims}-d tensor, got {tuple(t.shape)}")
-            _lib.require_device(t, name)
-            if t.device != key_codes.device:
-                raise ValueError(f"{name} is on {t.device}, key_codes on {key_codes.device}")
-        shape = tuple(key_codes.shape[:4])
-        if min(shape) < 1:
-            raise ValueError(f"layers, pages, heads and tokens must be positive (got {shape})")
-        if (value_codes.shape != key_codes.shape or tuple(key_scales.shape) != shape
-                or tuple(value_scales.shape) != shape or tuple(positions.shape) != (shape[1], shape[3])):
-            raise ValueError("fields must be [layers, pages, heads, tokens(, head_dim)] and [pages, tokens] of one shape")
-        cls._check_shape(shape, key_codes.shape[4])
-        lo, hi = torch.stack(torch.aminmax(positions)).tolist()
-        if lo < 0:
-            raise ValueError("positions must be non-negative")
-        pool = cls.__new__(cls)
-        pool._adopt(key_codes, value_codes, key_scales, value_scales, positions)
-        pool.max_position = hi
-        return pool
-
-    @staticmethod
-    def _check_shape(shape, head_dim: int) -> None:
-        layers, pages, heads, tokens = shape
-        if head_dim not in _HEAD_DIMS:
-            raise NotImplementedError(f"head_dim {head_dim}: the gfx950 page kernels take 64, 128 or 256")
-        if layers > 65535 or heads * tokens * head_dim >= 1 << 31 or pages * heads * tokens >= 1 << 31:
-            raise ValueError("a pool takes 65535 layers, pages of less than 2^31 bytes of codes and less than 2^31 "
-                             f"token rows a layer (got {shape})")
-
-    def _adopt(self, key_codes, value_codes, key_scales, value_scales, positions) -> None:
-        self.key_codes, self.value_codes = key_codes, value_codes
-        self.key_scales, self.value_scales = key_scales, value_scales
-        self.positions = positions
-        self.num_layers, self.num_pages, self.num_heads, self.page_tokens, self.head_dim = key_codes.shape
+    def _start(self, key_codes, value_codes, key_scales, value_scales, positions, bits: int = 0) -> None:
+        self.num_layers, self.num_pages, self.num_heads, self.page_tokens = key_codes.shape[:4]
         self.device = key_codes.device
         self._refs = np.zeros(self.num_pages, dtype=np.int32)
+        self._changes = 0  # of the references
         self._stack = np.arange(self.num_pages - 1, -1, -1, dtype=np.int32)  # free pages, the next one last
         self._free = self.num_pages
         self._lock = threading.RLock()
         self.desc = _lib.Pool(layers=self.num_layers, pages=self.num_pages, heads=self.num_heads,
-                               tokens=self.page_tokens, head_dim=self.head_dim, key_codes=_addr(key_codes),
-                               value_codes=_addr(value_codes), key_scales=_addr(key_scales),
-                               value_scales=_addr(value_scales), positions=_addr(positions))
+                              tokens=self.page_tokens, head_dim=self.head_dim, reserved=bits, key_codes=_addr(key_codes),
+                              value_codes=_addr(value_codes), key_scales=_addr(key_scales),
+                              value_scales=_addr(value_scales), positions=_addr(positions))
         self.desc_at = ctypes.addressof(self.desc)
 
     # ------------------------------------------------------------- page numbers
@@ -191,6 +129,7 @@ class CompressedPagePool:
         got = self._stack[self._free - n:self._free][::-1].copy()
         self._free -= n
         self._refs[got] = 1
+        self._changes += 1
         return got
 
     def _drop(self, p: np.ndarray, n: np.ndarray) -> None:
@@ -198,6 +137,7 @@ class CompressedPagePool:
         if len(p) and left.min() < 0:
             raise ValueError(f"free: page {int(p[left < 0][0])} is not allocated, or freed more often than referenced")
         self._refs[p] = left
+        self._changes += 1
         gone = p[left == 0][::-1]  # the lowest is allocated next
         self._stack[self._free:self._free + len(gone)] = gone
         self._free += len(gone)
@@ -207,6 +147,7 @@ class CompressedPagePool:
         with self._lock:
             p, n = self._tally(self._pages(pages))
             self._refs[p] = self._referenced(p, "retain") + n
+            self._changes += 1
 
     def free(self, pages: Sequence[int]) -> None:
         """Drop one reference of each page (of a page listed twice: two); pages without any can be
@@ -255,6 +196,7 @@ class CompressedPagePool:
                 raise ValueError("fork: a page stands twice in one sequence")
             if length % self.page_tokens == 0:
                 self._refs[p] += n
+                self._changes += 1
                 return [list(table) for _ in range(n)]
             last = self.allocate(n)
             try:
@@ -263,6 +205,7 @@ class CompressedPagePool:
                 self.free(last)
                 raise
             self._refs[p[:-1]] += n
+            self._changes += 1
             return [table[:-1] + [x] for x in last]
 
     def compact(self, tables: Sequence[Sequence[int]], lengths: Sequence[int], kept_idx: torch.Tensor, n_kept,
@@ -340,8 +283,6 @@ class CompressedPagePool:
         got = new.tolist()
         return [got[a:b] for a, b in zip(ends, ends[1:])], counts
 
-    # ------------------------------------------------------------------- tokens
-
     def slots(self, pages: Sequence[int], start: int, stop: int) -> List[int]:
         """Slots (page * page_tokens + offset) of a sequence's tokens start .. stop - 1."""
         p = self._pages(pages)
@@ -349,6 +290,82 @@ class CompressedPagePool:
         if len(i) and (i[0] < 0 or i[-1] >= len(p) * self.page_tokens):
             raise ValueError(f"tokens {start} .. {stop} do not lie in {len(p)} pages of {self.page_tokens}")
         return (p[i // self.page_tokens] * self.page_tokens + i % self.page_tokens).tolist()
+
+
+class CompressedPagePool(PagePool):
+    """num_pages pages of page_tokens tokens for num_heads kv heads, in num_layers layers.
+
+    key_codes, value_codes    int8 [layers, pages, heads, tokens, head_dim]
+    key_scales, value_scales  fp16 [layers, pages, heads, tokens]
+    positions                 int32 [pages, tokens], shared by the layers
+    max_position              no stored position is larger (write() keeps it; raise it
+                              after writing into `positions` directly)
+    """
+
+    def __init__(self, num_pages: int, num_heads: int, page_tokens: int, head_dim: int, num_layers: int = 1,
+                 device=None):
+        shape = (int(num_layers), int(num_pages), int(num_heads), int(page_tokens))
+        if min(shape) < 1:
+            raise ValueError(f"layers, pages, heads and tokens must be positive (got {shape})")
+        dev = torch.device("cuda" if device is None else device)
+        if dev.type != "cuda":
+            raise _lib.NexusQuantError(f"nexusquant_amd runs on MI355X (ROCm) devices only; the pool is on {dev}")
+        self._check_shape(shape, int(head_dim))
+        self._adopt(torch.zeros(shape + (int(head_dim),), dtype=torch.int8, device=dev),
+                    torch.zeros(shape + (int(head_dim),), dtype=torch.int8, device=dev),
+                    torch.zeros(shape, dtype=torch.float16, device=dev),
+                    torch.zeros(shape, dtype=torch.float16, device=dev),
+                    torch.zeros(shape[1], shape[3], dtype=torch.int32, device=dev))
+        self.max_position = 0
+
+    @classmethod
+    def from_tensors(cls, key_codes: torch.Tensor, value_codes: torch.Tensor, key_scales: torch.Tensor,
+                     value_scales: torch.Tensor, positions: torch.Tensor) -> "CompressedPagePool":
+        """A pool over fields that exist already (used, not copied); all its pages are free.
+        Reads the largest position back."""
+        for name, t, dt, dims in (("key_codes", key_codes, torch.int8, 5), ("value_codes", value_codes, torch.int8, 5),
+                                  ("key_scales", key_scales, torch.float16, 4),
+                                  ("value_scales", value_scales, torch.float16, 4),
+                                  ("positions", positions, torch.int32, 2)):
+            if t.dtype != dt:
+                raise TypeError(f"{name} must be {dt}, got {t.dtype}")
+            if t.dim() != dims or not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f"{name} must be a contiguous, 16-byte aligned {dims}-d tensor, got {tuple(t.shape)}")
+            _lib.require_device(t, name)
+            if t.device != key_codes.device:
+                raise ValueError(f"{name} is on {t.device}, key_codes on {key_codes.device}")
+        shape = tuple(key_codes.shape[:4])
+        if min(shape) < 1:
+            raise ValueError(f"layers, pages, heads and tokens must be positive (got {shape})")
+        if (value_codes.shape != key_codes.shape or tuple(key_scales.shape) != shape
+                or tuple(value_scales.shape) != shape or tuple(positions.shape) != (shape[1], shape[3])):
+            raise ValueError("fields must be [layers, pages, heads, tokens(, head_dim)] and [pages, tokens] of one shape")
+        cls._check_shape(shape, key_codes.shape[4])
+        lo, hi = torch.stack(torch.aminmax(positions)).tolist()
+        if lo < 0:
+            raise ValueError("positions must be non-negative")
+        pool = cls.__new__(cls)
+        pool._adopt(key_codes, value_codes, key_scales, value_scales, positions)
+        pool.max_position = hi
+        return pool
+
+    @staticmethod
+    def _check_shape(shape, head_dim: int) -> None:
+        layers, pages, heads, tokens = shape
+        if head_dim not in _HEAD_DIMS:
+            raise NotImplementedError(f"head_dim {head_dim}: the gfx950 page kernels take 64, 128 or 256")
+        if layers > 65535 or heads * tokens * head_dim >= 1 << 31 or pages * heads * tokens >= 1 << 31:
+            raise ValueError("a pool takes 65535 layers, pages of less than 2^31 bytes of codes and less than 2^31 "
+                             f"token rows a layer (got {shape})")
+
+    def _adopt(self, key_codes, value_codes, key_scales, value_scales, positions) -> None:
+        self.key_codes, self.value_codes = key_codes, value_codes
+        self.key_scales, self.value_scales = key_scales, value_scales
+        self.positions = positions
+        self.head_dim = key_codes.shape[4]
+        self._start(key_codes, value_codes, key_scales, value_scales, positions)
+
+    # ------------------------------------------------------------------- tokens
 
     def write(self, compressor, slots: Sequence[int], keys: torch.Tensor, values: torch.Tensor, positions,
               layer: int = 0) -> None:

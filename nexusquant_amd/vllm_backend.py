@@ -825,6 +825,8 @@ class NexusQuantPagedAttention:
         its pages block_tables[b] (0: none; entries past those tokens are padding).  Full pages that several
         rows begin with, as forks do, are read and decoded once for all of them, where that saves min_saved
         tokens' decoding (None: what pays, 65536 over the pool's heads)."""
+        if pool.desc.reserved:
+            raise ValueError("plan_shared takes a CompressedPagePool; a pool in 4 bits has an attention of its own (attend)")
         if pool.head_dim != self.compressor.head_dim:
             raise ValueError(f"pool head_dim {pool.head_dim} != compressor head_dim {self.compressor.head_dim}")
         ctx = [int(x) for x in (context_lens.tolist() if torch.is_tensor(context_lens) else context_lens)]

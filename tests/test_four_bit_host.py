@@ -1,0 +1,205 @@
+"""The work lists of attention over a cache in 4 bits, page numbers, and the C entry points' refusals, without a GPU."""
+
+import ctypes
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from nexusquant_amd import _lib, four_bit
+from oracle import four_bit as ref
+
+
+def replay(pages, lengths, queries, causal, window, group, heads, d):
+    """Every row's tokens and slots as the kernels go through the lists."""
+    lib = _lib.load()
+    most = [lib.nq_fourbit_rows(0), lib.nq_fourbit_rows(1)]
+    cap = lib.nq_fourbit_chunk_tokens()
+    (items, joins), (n_wide, n_few, n_joins, n_slots) = four_bit.attention_items(pages, lengths, queries, causal, window, group,
+                                                                                  heads, d, most, cap)
+    items, joins = items.reshape(-1, 12), joins.reshape(-1, 4)
+    assert len(items) == n_wide + n_few and len(joins) == n_joins == sum(queries)
+    first_row = np.concatenate([[0], np.cumsum(queries)])
+    first_page = np.concatenate([[0], np.cumsum(pages)])
+    seen = {}      # (query row, head in group): how often each token
+    written = {}   # slot, head in group
+    for k, it in enumerate(items):
+        page, tok0, n_tok, q_row0, r0, n_rows, slot0, slots, last = it[:9].tolist()
+        few = k >= n_wide
+        assert 1 <= n_rows <= most[1 if few else 0] and n_tok >= 1 and (not few or n_tok <= cap)
+        b = next(b for b in range(len(lengths)) if queries[b] and first_row[b] == q_row0)
+        assert first_page[b] == page and 0 <= tok0 and tok0 + n_tok <= lengths[b]
+        for r in range(r0, r0 + n_rows):
+            i, h = divmod(r, group)
+            assert i < queries[b]
+            hi = last + (i if causal else 0)
+            lo = max(hi - window + 1, 0) if window else 0
+            got = seen.setdefault((q_row0 + i, h), np.zeros(lengths[b], int))
+            got[max(lo, tok0):min(hi + 1, tok0 + n_tok)] += 1
+            slot = slot0 + i * slots
+            assert 0 <= slot < n_slots and (slot, h) not in written
+            written[slot, h] = q_row0 + i
+    joined = set()
+    for row, at, c, _ in joins.tolist():
+        assert row not in joined
+        joined.add(row)
+        for s in range(at, at + c):
+            assert all(written[s, h] == row for h in range(group))
+    assert sum(c for _, _, c, _ in joins.tolist()) * group == len(written)
+    for b, (n, q) in enumerate(zip(lengths, queries)):
+        mask = ref.seen(n, q, causal, window).numpy() if n else None
+        for i in range(q):
+            for h in range(group):
+                got = seen.get((first_row[b] + i, h))
+                assert (got is None) if not n else np.array_equal(got, mask[i].astype(int)), (b, i, h)
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_every_row_sees_its_tokens_once(seed):
+    r = random.Random(seed)
+    group, heads, d = r.choice([1, 2, 3, 4, 8, 16, 17, 130, 300]), r.choice([1, 2, 8, 40]), r.choice([64, 128, 256])
+    causal = r.random() < 0.6
+    lengths = [r.choice([0, 1, r.randint(1, 60), r.randint(1, 1500)]) for _ in range(r.randint(1, 5))]
+    queries = [r.choice([0, 1, 1, r.randint(1, 9), r.randint(1, 300 if group < 16 else 5)]) for _ in lengths]
+    if causal:
+        queries = [min(q, n) if n else q for q, n in zip(queries, lengths)]
+    window = r.choice([0, 0, 1, r.randint(1, 100)]) if causal else 0
+    replay([-(-n // 16) for n in lengths], lengths, queries, causal, window, group, heads, d)
+
+
+def test_long_sequences_and_many():
+    replay([8192], [131072], [1], True, 0, 8, 8, 128)
+    replay([512] * 3, [8192] * 3, [200, 1, 3], True, 0, 2, 8, 128)
+    replay([32] * 64, [500] * 64, [1] * 64, True, 0, 4, 8, 128)
+    replay([], [], [], True, 0, 4, 8, 128)
+    replay([0], [0], [3], True, 0, 4, 8, 128)
+
+
+def cpu_pool(pages=6, heads=2, tokens=16, d=128, layers=1):
+    """A pool without a device, for what is checked before one is needed."""
+    pool = four_bit.FourBitPagePool.__new__(four_bit.FourBitPagePool)
+    shape = (layers, pages, heads, tokens)
+    pool._adopt(*(torch.zeros(shape + (d // 2,), dtype=torch.uint8) for _ in range(2)),
+                *(torch.zeros(shape, dtype=torch.float16) for _ in range(2)))
+    return pool
+
+
+def test_pool_shapes():
+    pool = cpu_pool()
+    assert (pool.head_dim, pool.page_tokens, pool.num_heads, pool.num_pages, pool.free_pages) == (128, 16, 2, 6, 6)
+    assert pool.desc.head_dim == 128 and pool.desc.reserved == 4 and not pool.desc.positions
+    with pytest.raises(ValueError, match="positive"):
+        four_bit.FourBitPagePool(0, 2, 16, 128)
+    with pytest.raises(_lib.NexusQuantError):
+        four_bit.FourBitPagePool(4, 2, 16, 128, device="cpu")
+    for shape, d in (((1, 4, 2, 16), 96), ((1, 1 << 25, 8, 16), 128), ((65536, 1, 1, 1), 64), ((1, 1, 1 << 13, 1 << 13), 128)):
+        with pytest.raises((ValueError, NotImplementedError)):
+            four_bit.FourBitPagePool._check_shape(shape, d)
+    with pytest.raises(_lib.NexusQuantError):
+        z = torch.zeros(1, 2, 2, 16, 64, dtype=torch.uint8)
+        s = torch.zeros(1, 2, 2, 16, dtype=torch.float16)
+        four_bit.FourBitPagePool.from_tensors(z, z, s, s)
+    with pytest.raises(TypeError):
+        four_bit.FourBitPagePool.from_tensors(z.to(torch.int8), z, s, s)
+    with pytest.raises(ValueError):
+        four_bit.FourBitPagePool.from_tensors(z[..., ::2], z, s, s)
+
+
+def test_plans_check_page_numbers():
+    pool = cpu_pool()
+    t = pool.allocate(2)
+    for tables, lengths in (([t], [33]), ([t], [-1]), ([[4]], [3]), ([t], [3, 4]), ([[99]], [3])):
+        with pytest.raises(ValueError):
+            pool.plan_attention(tables, lengths)
+    with pytest.raises(ValueError):
+        pool.plan_attention([t], [20], [21])
+    with pytest.raises(ValueError):
+        pool.plan_attention([t], [20], causal=False, sliding_window=3)
+    plan = pool.plan_attention([t + [77]], [20], [3], sliding_window=20)
+    assert plan.rows == 3 and plan.window == 0 and plan._tables[0].tolist() == t
+    for bad in ([0, 0], [96], [40], [0.5]):
+        with pytest.raises(ValueError):
+            pool.plan_slots(bad)
+
+
+def test_references_are_counted_as_changes():
+    pool = cpu_pool()
+    seen = [pool._changes]
+
+    def changed():
+        seen.append(pool._changes)
+        return seen[-1] != seen[-2]
+
+    t = pool.allocate(2)
+    assert changed()
+    pool.retain(t)
+    assert changed()
+    pool.free(t)
+    assert changed()
+    pool.fork(t, 32, n=1)
+    assert changed()
+
+
+def test_entry_points_refuse_bad_arguments():
+    lib = _lib.load()
+    at = 4096
+
+    def c_pool(**kw):
+        f = dict(layers=2, pages=4, heads=2, tokens=16, head_dim=128, reserved=4, key_codes=at, value_codes=at, key_scales=at, value_scales=at)
+        return _lib.Pool(**{**f, **kw})
+
+    def append(pool=None, layer=0, rows=3, hq=2, dtype=0, q=at, k=at, v=at, out=at, angles=at, slots=at, strides=(256, 128) * 4):
+        pool = c_pool() if pool is None else pool
+        return lib.nq_fourbit_append(four_bit._APPEND_PACK.pack(ctypes.addressof(pool), layer, rows, hq, dtype, q, k, v, out, angles,
+                                                                slots, *strides, 1.0, 0), None)
+
+    def read(pool=None, layer=0, slots=at, n=3, dtype=0, keys=at, values=at):
+        return lib.nq_fourbit_read(c_pool() if pool is None else pool, layer, slots, n, dtype, 1.0, keys, values, None)
+
+    def attend(pool=None, layer=0, hq=4, dtype=0, counts=(1, 1, 1, 2), window=0, scale=0.1, q=at, out=at, items=at, pages=at, joins=at,
+               strides=(512, 128) * 2, ws=at, nbytes=1 << 20):
+        pool = c_pool() if pool is None else pool
+        return lib.nq_fourbit_attention(four_bit._ATTEND_PACK.pack(
+            ctypes.addressof(pool), layer, hq, dtype, *counts, 1, window, scale, 0.1, 0, q, out, items, pages, joins, *strides, ws, nbytes), None)
+
+    assert lib.nq_fourbit_append(None, None) == lib.nq_fourbit_attention(None, None) == -1
+    for kw in (dict(head_dim=96), dict(layers=0), dict(pages=0), dict(heads=-1), dict(tokens=0), dict(key_codes=None),
+               dict(value_scales=None), dict(key_codes=at + 8), dict(pages=1 << 27), dict(reserved=0), dict(reserved=8)):
+        for call in (append, read, attend):
+            assert call(pool=c_pool(**kw)) == -1, kw
+    for call in (append, read, attend):
+        assert call(layer=2) == call(layer=-1) == -1
+    for kw in (dict(rows=-1), dict(hq=-1), dict(dtype=2), dict(k=0), dict(v=0), dict(slots=0), dict(q=0), dict(out=0), dict(angles=0),
+               dict(k=at + 2), dict(out=at + 8), dict(angles=at + 4), dict(strides=(256, 124) + (256, 128) * 3)):
+        assert append(**kw) == -1, kw
+    for kw in (dict(slots=0), dict(n=-1), dict(dtype=3), dict(keys=0), dict(values=0), dict(values=at + 8), dict(n=(1 << 31) - 1)):
+        assert read(**kw) == -1, kw
+    for kw in (dict(hq=0), dict(hq=3), dict(dtype=2), dict(counts=(-1, 1, 1, 1)), dict(counts=(1, 1, -1, 1)), dict(window=-1),
+               dict(scale=0.0), dict(scale=float("nan")), dict(q=0), dict(out=0), dict(items=0), dict(pages=0), dict(joins=0), dict(q=at + 8),
+               dict(out=at + 4), dict(strides=(512, 124, 512, 128)), dict(strides=(512, 128, 512, 126)), dict(ws=0), dict(nbytes=16),
+               dict(ws=at + 8), dict(counts=(1 << 30, 1 << 30, 1, 1)), dict(counts=(1, 1, 1 << 28, 1))):
+        assert attend(**kw) == -1, kw
+    assert append(rows=0) == read(n=0) == attend(counts=(0, 0, 0, 0)) == 0
+    # pools of the other kind
+    assert lib.nq_pool_compact(c_pool(), at, 100, 0, 1, 1, at, 8, 1, None) == -1 and b"renumber" in lib.nq_last_error()
+    assert lib.nq_pool_write(c_pool(), 0, c_pool(), at, 0, 3, None) == -1
+
+
+def test_descriptors_match_the_c_compiler(tmp_path):
+    """The packed formats' sizes and the places of their last fields equal gcc's on the header."""
+    import os
+    import subprocess
+    from nexusquant_amd import rotary
+    header = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "nexusquant_amd.h")
+    fields = [("nq_rotate_desc", "k_out_stride", rotary._PACK), ("nq_fourbit_append_desc", "hadamard_scale", four_bit._APPEND_PACK),
+              ("nq_fourbit_append_desc", "q_stride", None), ("nq_fourbit_desc", "query", None), ("nq_fourbit_desc", "workspace_bytes", four_bit._ATTEND_PACK)]
+    src = tmp_path / "layout.c"
+    src.write_text(f'#include <stddef.h>\n#include <stdio.h>\n#include "{header}"\nint main(void){{' + "".join(
+        f'printf("%zu %zu\\n", sizeof({s}), offsetof({s}, {f}));' for s, f, _ in fields) + "return 0;}")
+    subprocess.check_call(["gcc", "-o", str(tmp_path / "layout"), str(src)])
+    out = [tuple(int(x) for x in line.split()) for line in subprocess.check_output([str(tmp_path / "layout")]).decode().splitlines()]
+    assert all(size == pack.size for (size, _), (_, _, pack) in zip(out, fields) if pack is not None)
+    import struct
+    assert out[0][1] == struct.calcsize("6i5P6q") and out[1][1] == struct.calcsize("P4i6P8q") and out[2][1] == struct.calcsize("P4i6P")
+    assert out[3][1] == struct.calcsize("P9i2fi") + (-struct.calcsize("P9i2fi")) % 8 and out[4][1] == struct.calcsize("P9i2fi5P4qP")

@@ -1,0 +1,510 @@
+"""A cache held in 4 bits against 64 bits: what is stored, what is read, and attention over it."""
+
+import math
+
+import pytest
+import torch
+
+from nexusquant_amd import FourBitPagePool, plan_rotation, rotate
+from nexusquant_amd.rope import inv_freq
+from nexusquant_amd.rotary import frequency_axes
+from oracle import four_bit as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+def fill(pool, seed):
+    """Random codes and scales in all of a pool."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    for c in (pool.key_codes, pool.value_codes):
+        c.copy_(torch.randint(0, 256, c.shape, device="cuda", generator=g, dtype=torch.uint8))
+    for s in (pool.key_scales, pool.value_scales):
+        s.copy_(torch.rand(s.shape, device="cuda", generator=g) * 0.3 + 0.05)
+
+
+def sequences(pool, lens, seed):
+    """Allocated, shuffled tables."""
+    need = [pool.pages_for(n) for n in lens]
+    pages = torch.tensor(pool.allocate(sum(need)))
+    pages = pages[torch.randperm(len(pages), generator=torch.Generator().manual_seed(seed))].tolist()
+    tables = []
+    for n in need:
+        tables.append(pages[:n])
+        pages = pages[n:]
+    return tables
+
+
+# ----------------------------------------------------------- append and read --
+
+def check_stored(codes, scales, t, terms):
+    """Stored levels of t = H x, as 64 bits have it.  32 bits are off by at most `terms` 2^-24 of |x| sums over sqrt(d) (a
+    butterfly's sums, one rounding a stage, the rotation's and two products), the scale by half a step of fp16 more."""
+    d = t.shape[-1]
+    off = terms * 2.0 ** -24 * ref.walsh(t).abs().sum(-1) / math.sqrt(d) + 1e-30
+    m = t.abs().amax(-1) / 7.5
+    s = scales.double()
+    half = torch.where(m < 2.0 ** -14, 2.0 ** -25, m * 2.0 ** -11)
+    assert ((s - m.clamp(max=65504.0)).abs() <= half + off).all()
+    y = t / torch.where(s == 0, 1.0, s)[..., None]
+    # levels end at 7: with s >= (m / 7.5) (1 - 2^-11), or held at 65504, what lies past 7.5 s is still held as 7 (the format's
+    # own bound there is 0.5 + 7.5 2^-11)
+    clipped = y.clamp(-8.0, 7.5)
+    good = (ref.unpack(codes) - clipped).abs() <= 0.5 + (off / torch.where(s == 0, 1.0, s))[..., None] + 2.0 ** -20
+    assert (good | (s == 0)[..., None]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,heads,hq,tokens,rows,axes", [
+    (64, 1, 1, 16, 1, 1), (128, 8, 32, 16, 33, 3), (256, 3, 6, 8, 17, 1), (128, 5, 0, 24, 40, 0), (64, 20, 20, 32, 100, 1),
+    (128, 2, 14, 16, 7, 1), (256, 8, 0, 16, 130, 0), (128, 16, 64, 64, 300, 2)])
+def test_append_and_read(dtype, d, heads, hq, tokens, rows, axes):
+    T = TYPES[dtype]
+    g = torch.Generator(device="cuda").manual_seed(d + rows)
+    pool = FourBitPagePool(rows // tokens + 5, heads, tokens, d, num_layers=3)
+    fill(pool, 1)
+    before = [x.clone() for x in (pool.key_codes, pool.value_codes, pool.key_scales, pool.value_scales)]
+    pages = pool.allocate(rows // tokens + 3)
+    order = torch.randperm(len(pages) * tokens, generator=torch.Generator().manual_seed(rows)).tolist()
+    slots = [pages[i // tokens] * tokens + i % tokens for i in order[:rows]]
+    if rows > 5:
+        slots[3] = slots[rows - 1] = -1
+    qkv = torch.randn(rows, hq + 2 * heads, d, device="cuda", generator=g).to(T)
+    q, k, v = qkv[:, :hq], qkv[:, hq:hq + heads], qkv[:, hq + heads:]
+    rotation, turned_q, turned_k = None, q.cpu().double(), k.cpu().double()
+    if axes:
+        sections = [d // 2 - (axes - 1) * (d // 8)] + [d // 8] * (axes - 1)
+        pos = torch.stack([torch.arange(rows) * (a + 1) + 17 for a in range(axes)])
+        rotation = plan_rotation(pos.cuda(), d, base=500000.0, sections=sections)
+        ang = ref.angles(pos, inv_freq(d, 500000.0), frequency_axes(d, sections, False))
+        turned_q, turned_k = ref.rotate(turned_q, ang), ref.rotate(turned_k, ang)
+    plan = pool.plan_slots(slots)
+    got = pool.append(plan, k, v, rotation=rotation, query=q if hq else None, layer=1)
+    if hq:
+        assert torch.equal(got, rotate(q, None, rotation)[0])
+    else:
+        assert got is None
+    live = torch.tensor([i for i, s in enumerate(slots) if s >= 0])
+    at = torch.tensor(slots)[live]
+    kc, vc, ks, vs = (x.cpu() for x in (pool.key_codes, pool.value_codes, pool.key_scales, pool.value_scales))
+    for c, s, x in ((kc, ks, turned_k), (vc, vs, v.cpu().double())):
+        check_stored(c[1, at // tokens, :, at % tokens], s[1, at // tokens, :, at % tokens], ref.walsh(x[live]), 16)
+    # nothing else was written
+    for now, was in zip((kc, vc, ks, vs), before):
+        was = was.cpu()
+        was[1, at // tokens, :, at % tokens] = now[1, at // tokens, :, at % tokens]
+        assert torch.equal(now, was)
+    for out_type in (torch.float16, torch.bfloat16, torch.float32):
+        keys, values = pool.read(plan, layer=1, dtype=out_type)
+        for y, c, s in ((keys, kc, ks), (values, vc, vs)):
+            want = ref.decode(c[1, at // tokens, :, at % tokens], s[1, at // tokens, :, at % tokens])
+            off = (y.cpu().double()[live] - want).abs()
+            # its type's rounding, the product of scale and 1 / sqrt(d) and that with a whole number
+            assert (off <= want.abs() * (torch.finfo(out_type).eps / 2 + 4 * 2.0 ** -24) + 2.0 ** -25).all()
+            assert (y.cpu()[[i for i, p in enumerate(slots) if p < 0]] == 0).all()
+
+
+def test_rows_that_are_zero_tiny_huge_or_not_finite():
+    d = 128
+    pool = FourBitPagePool(2, 1, 16, d)
+    pages = pool.allocate(1)
+    for T, tiny, huge in ((torch.float16, 2.0 ** -24, 65504.0), (torch.bfloat16, 1e-30, 1e30)):
+        x = torch.zeros(16, 1, d, dtype=T)
+        g = torch.Generator().manual_seed(1)
+        x[1] = torch.randn(1, d, generator=g)
+        x[2, 0, 5] = tiny
+        x[3] = huge
+        x[4, 0, 7] = math.inf
+        x[5, 0, 9] = math.nan
+        x[6, 0, :2] = torch.tensor([math.inf, -math.inf])
+        x[7] = torch.randn(1, d, generator=g) * 3e-5
+        plan = pool.plan_slots([pages[0] * 16 + i for i in range(16)])
+        pool.append(plan, x.cuda(), x.cuda())
+        codes, scales = pool.key_codes[0, pages[0], 0].cpu(), pool.key_scales[0, pages[0], 0].cpu()
+        assert torch.equal(pool.value_codes[0, pages[0], 0].cpu(), codes)
+        assert scales[0] == 0 and scales[4:7].isnan().all() and scales[[0, 1, 2, 3, 7]].isfinite().all()
+        keys, values = (y.cpu() for y in pool.read(plan, dtype=torch.float32))
+        assert (keys[0] == 0).all() and (keys[8:] == 0).all() and keys[4:7].isnan().all() and values[4:7].isnan().all()
+        check_stored(codes[[1, 7]], scales[[1, 7]], ref.walsh(x[[1, 7], 0].double()), 16)
+        assert keys[2].abs().max() <= 2 * tiny + 2.0 ** -24 and keys[3].isfinite().all()
+        # A constant row is one coordinate of its transform, huge sqrt(d), and 65504 sqrt(128) / 7.5 = 98813 is past fp16 for
+        # both types: the scale is held at 65504, the level at 7, and the other 127 levels at zero.
+        assert scales[3] == 65504
+        assert (keys[3] - 7 * 65504.0 / math.sqrt(d)).abs().max() <= 7 * 65504.0 / math.sqrt(d) * 4 * 2.0 ** -24
+
+
+# ----------------------------------------------------------------- attention --
+
+def check_attention(pool, tables, lens, queries, q, got, dtype, causal=True, window=0, scale=None, layer=0, few=None):
+    """Every row against 64 bits, by the bound of what the kernels round (oracle/four_bit.py) plus half a step of the output."""
+    d = pool.head_dim
+    fields = [x[layer].cpu() for x in (pool.key_codes, pool.key_scales, pool.value_codes, pool.value_scales)]
+    row = 0
+    for table, n, m in zip(tables, lens, queries):
+        if m and n:
+            kl, ks = ref.sequence(fields[0], fields[1], table, n)
+            vl, vs = ref.sequence(fields[2], fields[3], table, n)
+            mask = ref.seen(n, m, causal, window)
+            want, bound = ref.attend(q[row:row + m].cpu(), kl, ks, vl, vs, mask, d ** -0.5 if scale is None else scale)
+            narrow = m * (q.shape[1] // pool.num_heads) <= 16 if few is None else few
+            # 22 bits are a step of 2^-22 of what fp16 holds in full; below that 2^-25 of a row's largest (in 2^14 .. 2^15)
+            u = 2.0 ** -21 if narrow else 2.0 ** -11
+            off = (got[row:row + m].cpu().double() - want).abs()
+            lim = bound(u, u) + want.abs() * torch.finfo(dtype).eps / 2 + 2.0 ** -25
+            assert (off <= lim).all(), (n, m, float((off - lim).max()))
+            # and as a whole much nearer: roundings are independent, a norm's is eps / 2 / sqrt(3) for the output's
+            rel = float(off.norm() / want.norm())
+            assert rel <= (torch.finfo(dtype).eps / 2 if narrow else torch.finfo(dtype).eps / 2 + 3 * 2.0 ** -11), rel
+        else:
+            assert (got[row:row + m] == 0).all()
+        row += m
+
+
+CASES = [
+    # heads, group, d, tokens a page, lengths, queries, causal, window
+    (1, 1, 64, 16, [1], [1], True, 0),
+    (8, 4, 128, 16, [1, 15, 16, 17, 33, 0, 255], None, True, 0),
+    (2, 8, 256, 8, [7, 100, 1025], None, True, 0),
+    (4, 1, 64, 32, [2049, 31, 700], None, True, 0),
+    (2, 16, 128, 24, [513, 64], None, True, 0),
+    (1, 24, 128, 16, [300, 5], None, True, 0),            # more heads than a few tile has rows
+    (1, 160, 64, 16, [77, 130], None, True, 0),           # more than a wide tile has
+    (8, 4, 128, 16, [40, 129, 1000], [4, 4, 3], True, 0),
+    (2, 4, 128, 16, [40, 129, 1000], [5, 33, 40], True, 0),
+    (2, 4, 256, 16, [64, 129, 400], [64, 1, 100], True, 0),
+    (4, 2, 64, 64, [1000, 200, 64], [130, 200, 64], True, 0),
+    (2, 5, 128, 16, [333, 50], [27, 50], True, 0),        # a group that divides no tile
+    (8, 4, 128, 16, [1000, 64, 3], None, True, 17),
+    (2, 4, 128, 16, [1000, 300], [100, 300], True, 70),
+    (2, 2, 64, 16, [500, 65], [30, 65], True, 1),
+    (20, 1, 64, 32, [1500, 3, 0, 64], [1, 1, 1, 1], False, 0),
+    (4, 1, 64, 32, [150, 3, 0, 64], [223, 2, 5, 17], False, 0),
+    (2, 4, 128, 16, [100, 1], [60, 0], False, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,group,d,tokens,lens,queries,causal,window", CASES)
+def test_attention(dtype, heads, group, d, tokens, lens, queries, causal, window):
+    T = TYPES[dtype]
+    pool = FourBitPagePool(sum(-(-n // tokens) for n in lens) + 3, heads, tokens, d, num_layers=2)
+    fill(pool, d + len(lens))
+    tables = sequences(pool, lens, 5)
+    new = queries or [1] * len(lens)
+    g = torch.Generator(device="cuda").manual_seed(11)
+    q = torch.randn(sum(new), heads * group, d, device="cuda", generator=g).to(T)
+    plan = pool.plan_attention(tables, lens, queries, causal=causal, sliding_window=window or None)
+    got = pool.attend(plan, q, layer=1)
+    check_attention(pool, tables, lens, new, q, got, T, causal, window, layer=1)
+    # what no query sees changes nothing, whatever it holds: slots behind a sequence, other pages, tokens before a window
+    hidden = torch.ones(pool.key_scales.shape[1:], dtype=torch.bool)
+    for table, n, m in zip(tables, lens, new):
+        if n and m:
+            some = ref.seen(n, m, causal, window).any(0)
+            for i in some.nonzero().flatten().tolist():
+                hidden[table[i // tokens], :, i % tokens] = False
+    for s in (pool.key_scales, pool.value_scales):
+        s[1][hidden.cuda()] = math.nan
+        s[0] = math.nan
+    assert torch.equal(pool.attend(plan, q, layer=1), got)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("queries", [1, 4, 40])
+def test_what_some_queries_do_not_see_may_be_anything(dtype, queries):
+    """A NaN or infinite scale at a sequence's last token reaches the last query alone."""
+    T = TYPES[dtype]
+    n = 150
+    pool = FourBitPagePool(12, 2, 16, 128)
+    fill(pool, 2)
+    tables = sequences(pool, [n], 1)
+    q = torch.randn(queries, 8, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(T)
+    plan = pool.plan_attention(tables, [n], [queries])
+    want = pool.attend(plan, q)
+    for field in (pool.key_scales, pool.value_scales):
+        for bad in (math.nan, math.inf):
+            slot = tables[0][(n - 1) // 16], (n - 1) % 16
+            was = field[0, slot[0], 1, slot[1]].clone()
+            field[0, slot[0], 1, slot[1]] = bad
+            got = pool.attend(plan, q)
+            # (when a row's maximum rises the rows beside it are rescaled too, so theirs may be rounded in another place)
+            check_attention(pool, tables, [n - 1], [queries - 1], q[:-1], got[:-1], T, few=4 * queries <= 16)
+            assert torch.equal(got[-1, :4], want[-1, :4])
+            # (a key's infinite scale times a negative sum is a logit of -inf, and a weight of zero)
+            assert not got[-1, 4:].isfinite().all() or (field is pool.key_scales and bad == math.inf)
+            field[0, slot[0], 1, slot[1]] = was
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scales_and_queries_of_all_sizes(dtype):
+    """A first token that takes nearly all weight with small values beside later ones with large ones; large and small queries."""
+    T = TYPES[dtype]
+    for queries in (1, 40):
+        n = 700
+        pool = FourBitPagePool(50, 1, 16, 128)
+        fill(pool, 3)
+        tables = sequences(pool, [n], 1)
+        first, later = tables[0][0], tables[0][20]
+        pool.value_scales[0, first, 0, 0] = 2.0 ** -14
+        pool.value_scales[0, later] *= 1000.0
+        pool.key_scales[0, first, 0, 0] = 4.0
+        g = torch.Generator(device="cuda").manual_seed(1)
+        for factor in (1.0, 2.0 ** -12, 30.0):
+            q = (torch.randn(queries, 4, 128, device="cuda", generator=g) * factor).to(T)
+            plan = pool.plan_attention(tables, [n], [queries])
+            got = pool.attend(plan, q)
+            kl, ks = ref.sequence(pool.key_codes[0].cpu(), pool.key_scales[0].cpu(), tables[0], n)
+            vl, vs = ref.sequence(pool.value_codes[0].cpu(), pool.value_scales[0].cpu(), tables[0], n)
+            want, bound = ref.attend(q.cpu(), kl, ks, vl, vs, ref.seen(n, queries, True, 0), 128 ** -0.5)
+            u = 2.0 ** -21 if queries == 1 else 2.0 ** -11
+            assert ((got.cpu().double() - want).abs() <= bound(u, u) + want.abs() * torch.finfo(T).eps / 2 + 2.0 ** -25).all()
+
+
+def test_scale_window_strides_and_rows_behind():
+    pool = FourBitPagePool(20, 2, 16, 128)
+    fill(pool, 4)
+    lens, new = [100, 150], [3, 30]
+    tables = sequences(pool, lens, 2)
+    qkv = torch.randn(40, 12, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).half()
+    plan = pool.plan_attention([t + [999] for t in tables], lens, new)  # (entries past a sequence's tokens are padding)
+    got = pool.attend(plan, qkv[:, :8], scale=0.11)
+    check_attention(pool, tables, lens, new, qkv[:, :8], got, torch.float16, scale=0.11)
+    assert (got[33:] == 0).all()
+    out = torch.full((40, 10, 128), 5.0, device="cuda").half()
+    assert pool.attend(plan, qkv[:, :8], scale=0.11, out=out[:, 1:9]).data_ptr() == out[:, 1:9].data_ptr()
+    assert torch.equal(out[:33, 1:9], got[:33]) and (out[33:] == 5.0).all() and (out[:, 0] == 5.0).all() and (out[:, 9] == 5.0).all()
+    heads_first = qkv[:, :8].transpose(0, 1).contiguous()
+    assert torch.equal(pool.attend(plan, heads_first.transpose(0, 1), scale=0.11), got)
+    odd = torch.empty(40 * 8 * 128 + 1, device="cuda", dtype=torch.float16)[1:].view(40, 8, 128).copy_(qkv[:, :8])
+    assert torch.equal(pool.attend(plan, odd, scale=0.11), got)
+    own = qkv[:, :8].clone()
+    assert pool.attend(plan, own, scale=0.11, out=own) is own and torch.equal(own[:33], got[:33]) and torch.equal(own[33:], qkv[33:, :8])
+    assert torch.equal(pool.attend(pool.plan_attention(tables, lens, new, sliding_window=150), qkv[:, :8], scale=0.11), got)
+    empty = pool.plan_attention([], [])
+    assert pool.attend(empty, qkv[:0, :8]).shape == (0, 8, 128) and (pool.attend(empty, qkv[:4, :8]) == 0).all()
+
+
+def test_decode_steps_as_they_are_used():
+    """Prompts appended at once, then tokens one at a time, with positions of three axes; forks, eviction."""
+    d, heads, hq, T = 128, 2, 8, torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(9)
+    pool = FourBitPagePool(64, heads, 16, d, num_layers=2)
+    lens = [37, 64]
+    tables = [pool.allocate(pool.pages_for(n)) for n in lens]
+    sections = [24, 20, 20]
+
+    def step(tables, start, stop):
+        """Tokens start[b] .. stop[b] of every sequence through both layers: outputs of the last."""
+        rows = [b - a for a, b in zip(start, stop)]
+        pos = torch.cat([torch.stack([torch.arange(a, b), torch.arange(a, b) // 2, torch.arange(a, b) % 7]) for a, b in zip(start, stop)], dim=1)
+        rotation = plan_rotation(pos.cuda(), d, sections=sections, interleaved=True)
+        slots = pool.plan_slots([s for t, a, b in zip(tables, start, stop) for s in pool.slots(t, a, b)])
+        plan = pool.plan_attention(tables, stop, rows)
+        for layer in range(2):
+            qkv = torch.randn(sum(rows), hq + 2 * heads, d, device="cuda", generator=g).to(T)
+            q = pool.append(slots, qkv[:, hq:hq + heads], qkv[:, hq + heads:], rotation=rotation, query=qkv[:, :hq], layer=layer)
+            out = pool.attend(plan, q, layer=layer)
+            check_attention(pool, tables, stop, rows, q, out, T, layer=layer)
+        return out
+
+    step(tables, [0, 0], lens)
+    for i in range(3):
+        for b in range(2):
+            if pool.pages_for(lens[b] + 1) > len(tables[b]):
+                tables[b] += pool.allocate(1)
+        step(tables, lens, [n + 1 for n in lens])
+        lens = [n + 1 for n in lens]
+    kids = pool.fork(tables[0], lens[0], n=2)
+    assert pool.ref_count(tables[0][0]) == 3 and pool.ref_count(tables[0][-1]) == 1
+    with pytest.raises(ValueError, match="shared"):
+        pool.append(pool.plan_slots(pool.slots(kids[0], 0, 1)), torch.zeros(1, heads, d, device="cuda", dtype=T),
+                    torch.zeros(1, heads, d, device="cuda", dtype=T))
+    for now in (pool.key_codes, pool.value_codes, pool.key_scales, pool.value_scales):
+        assert torch.equal(now[:, kids[1][-1]], now[:, tables[0][-1]])
+    step(kids, [lens[0]] * 2, [lens[0] + 1] * 2)
+    pool.free(kids[0])
+    pool.free(kids[1])
+    # every third token leaves
+    kept = torch.arange(lens[1])[torch.arange(lens[1]) % 3 != 1].int()
+    old = pool.read(pool.plan_slots(pool.slots(tables[1], 0, lens[1])), layer=1)
+    (new,), (count,) = pool.compact([tables[1]], [lens[1]], kept[None].cuda(), [len(kept)])
+    assert count == len(kept)
+    now = pool.read(pool.plan_slots(pool.slots(new, 0, count)), layer=1)
+    assert all(torch.equal(a[kept.long().cuda()], b) for a, b in zip(old, now))
+    with pytest.raises(ValueError, match="rotated"):
+        pool.compact([new], [count], kept[None].cuda(), [1], renumber=True)
+    free = pool.free_pages
+    pool.free(new)
+    pool.free(tables[0])
+    assert pool.free_pages == 64 and free < 64
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_whole_pages_copied_and_compacted_in_every_layer(d):
+    pool = FourBitPagePool(12, 3, 8, d, num_layers=3)
+    fill(pool, 7)
+    pages = pool.allocate(8)
+    fields = (pool.key_codes, pool.value_codes, pool.key_scales, pool.value_scales)
+    was = [x.clone() for x in fields]
+    pool.copy_pages([pages[0], pages[0], pages[3]], [pages[5], pages[1], pages[7]])
+    for now, old in zip(fields, was):
+        old[:, [pages[5], pages[1], pages[7]]] = old[:, [pages[0], pages[0], pages[3]]]
+        assert torch.equal(now, old)
+    table, n = pages[:4], 29
+    kept = torch.tensor([0, 2, 3, 9, 11, 12, 20, 27, 28], dtype=torch.int32)
+    (new,), _ = pool.compact([table], [n], kept[None].cuda(), torch.tensor([9], device="cuda"))
+    for now, old in zip(fields, was):
+        for j, i in enumerate(kept.tolist()):
+            assert torch.equal(now[:, new[j // 8], :, j % 8], old[:, table[i // 8], :, i % 8])
+
+
+def test_graphs_and_streams():
+    d, heads, hq = 128, 2, 8
+    g = torch.Generator(device="cuda").manual_seed(3)
+    pool = FourBitPagePool(40, heads, 16, d)
+    fill(pool, 5)
+    lens = [200, 77, 130]
+    tables = sequences(pool, lens, 1)
+    slots = pool.plan_slots([pool.slots(t, n - 1, n)[0] for t, n in zip(tables, lens)])
+    plan = pool.plan_attention(tables, lens)
+    wide = pool.plan_attention(tables, lens, [40, 30, 50])
+    pos = torch.tensor([n - 1 for n in lens], device="cuda")
+    qkv = torch.randn(3, hq + 2 * heads, d, device="cuda", generator=g).half()
+    many = torch.randn(120, hq, d, device="cuda", generator=g).half()
+
+    def step():
+        rotation = plan_rotation(pos, d)
+        q = pool.append(slots, qkv[:, hq:hq + heads], qkv[:, hq + heads:], rotation=rotation, query=qkv[:, :hq])
+        return q, pool.attend(plan, q), pool.attend(wide, many), *pool.read(slots)
+
+    step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):  # two graphs at a time have workspaces of their own
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        graphs.append((graph, got))
+    for i in range(4):
+        qkv.copy_(torch.randn(qkv.shape, device="cuda", generator=g))
+        pos.add_(3)
+        many.copy_(torch.randn(many.shape, device="cuda", generator=g))
+        want = [x.clone() for x in step()]
+        torch.cuda.synchronize()
+        for x in (pool.key_codes, pool.value_codes):
+            x[0, tables[0][-1]].zero_()  # the replay writes its slots again
+        pool.append(slots, qkv[:, hq:hq + heads], qkv[:, hq + heads:], rotation=plan_rotation(pos, d))
+        want = [x.clone() for x in step()]
+        for graph, got in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, got in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    fresh = pool.plan_attention(tables, lens)
+    with torch.cuda.stream(side):
+        got = pool.attend(fresh, qkv[:, :hq]), pool.attend(plan, qkv[:, :hq])
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], pool.attend(plan, qkv[:, :hq]))
+    new = pool.plan_attention(tables, lens)
+    with pytest.raises(RuntimeError, match="before capturing"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            pool.attend(new, qkv[:, :hq])
+    torch.cuda.synchronize()
+
+
+def test_offsets_past_32_bits():
+    """Pages whose codes lie past 4 GiB of their field."""
+    d, heads, tokens = 256, 8, 16
+    pages = 300000  # 4.9 GB of keys' codes
+    shape = (1, pages, heads, tokens)
+    codes = [torch.empty(shape + (d // 2,), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    scales = [torch.zeros(shape, dtype=torch.float16, device="cuda") for _ in range(2)]
+    pool = FourBitPagePool.from_tensors(*codes, *scales)
+    pool.allocate(pages)
+    tables = [[pages - 1, 3, pages - 2, pages - 7], [pages - 4, pages - 9]]
+    lens = [60, 23]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    slots = pool.plan_slots([s for t, n in zip(tables, lens) for s in pool.slots(t, 0, n)])
+    k, v = (torch.randn(83, heads, d, device="cuda", generator=g).half() for _ in range(2))
+    pool.append(slots, k, v)
+    keys, values = pool.read(slots)
+    assert (keys - k).float().norm() < 0.2 * k.float().norm() and (values - v).float().norm() < 0.2 * v.float().norm()
+    for new in ([1, 1], [50, 23]):
+        q = torch.randn(sum(new), heads * 2, d, device="cuda", generator=g).half()
+        got = pool.attend(pool.plan_attention(tables, lens, new), q)
+        row = 0
+        for t, n, m in zip(tables, lens, new):
+            at = torch.tensor(t, device="cuda")
+            kl, ks, vl, vs = (x for c, s in ((codes[0], scales[0]), (codes[1], scales[1]))
+                              for x in ref.sequence(c[0][at].cpu(), s[0][at].cpu(), range(len(t)), n))
+            want, bound = ref.attend(q[row:row + m].cpu(), kl, ks, vl, vs, ref.seen(n, m, True, 0), d ** -0.5)
+            off = (got[row:row + m].cpu().double() - want).abs()
+            assert (off <= bound(2.0 ** -11, 2.0 ** -11) + want.abs() * 2.0 ** -11 + 2.0 ** -25).all()
+            row += m
+
+
+def test_one_call_does_not_change_with_the_next():
+    """Outputs twice on the same inputs are the same bits: sums have one order."""
+    pool = FourBitPagePool(300, 4, 16, 128)
+    fill(pool, 8)
+    lens = [2000, 31, 900]
+    tables = sequences(pool, lens, 3)
+    for new in ([1, 1, 1], [40, 31, 50]):
+        plan = pool.plan_attention(tables, lens, new)
+        q = torch.randn(sum(new), 16, 128, device="cuda").bfloat16()
+        first = pool.attend(plan, q)
+        for _ in range(5):
+            assert torch.equal(pool.attend(plan, q), first)
+
+
+def test_refusals():
+    pool = FourBitPagePool(8, 2, 16, 128, num_layers=2)
+    other = FourBitPagePool(8, 2, 16, 128)
+    t = pool.allocate(3)
+    other.allocate(3)
+    plan = pool.plan_slots([t[0] * 16, t[1] * 16 + 3])
+    k = torch.randn(2, 2, 128, device="cuda").half()
+    q = torch.randn(2, 4, 128, device="cuda").half()
+    r = plan_rotation([0, 1], 128)
+    for bad in ([t[0] * 16, t[0] * 16], [8 * 16], [1.5], [t[2] * 16 + 16], [(1 << 40)]):
+        with pytest.raises(ValueError):
+            pool.plan_slots(bad)
+    with pytest.raises(ValueError, match="not one of this pool"):
+        other.append(plan, k, k)
+    for args in ((k[:1], k), (k, k[:, :1]), (k.bfloat16(), k), (k.float(), k.float()), (k[:, :, :64], k[:, :, :64])):
+        with pytest.raises(ValueError):
+            pool.append(plan, *args)
+    for kw in (dict(query=q), dict(rotation=plan_rotation([0], 128)), dict(rotation=plan_rotation([0, 1], 64)),
+               dict(layer=2), dict(layer=-1), dict(rotation=r, query=q.bfloat16()), dict(rotation=r, query=q[:1]),
+               dict(rotation=r, out=q), dict(rotation=r, query=q, out=q[:, :2]), dict(rotation=r, query=q[:, :2], out=k)):
+        with pytest.raises(ValueError):
+            pool.append(plan, k, k, **kw)
+    with pytest.raises(NotImplementedError):
+        pool.append(plan, k.clone().requires_grad_(), k)
+    with pytest.raises(Exception, match="device"):
+        pool.append(plan, k.cpu(), k)
+    pool.free([t[1]])
+    with pytest.raises(ValueError, match="not allocated"):
+        pool.append(plan, k, k)
+    for args in (([t[:1]], [17]), ([t[:1]], [-1]), ([[5]], [3]), ([t[:1]], [3, 4])):
+        with pytest.raises(ValueError):
+            pool.plan_attention(*args)
+    for kw in (dict(queries=[9]), dict(queries=[-1]), dict(sliding_window=0), dict(causal=False, sliding_window=4), dict(queries=[1, 1])):
+        with pytest.raises(ValueError):
+            pool.plan_attention([t[:1]], [8], **kw)
+    step = pool.plan_attention([t[:1]], [8])
+    for bad in (q[:1].float(), q[:1, :3], q[:0], q[:1, :, :64], q[:1, :0]):
+        with pytest.raises(ValueError):
+            pool.attend(step, bad)
+    for kw in (dict(scale=0.0), dict(scale=math.nan), dict(layer=2), dict(out=q), dict(out=q[1:].bfloat16()), dict(out=q[:1, :4, ::2])):
+        with pytest.raises(ValueError):
+            pool.attend(step, q[:1], **kw)
+    with pytest.raises(ValueError):
+        pool.attend(step, q, out=torch.empty(1, device="cuda").half().expand(2, 4, 128))
+    with pytest.raises(ValueError):
+        other.attend(step, q[:1])
+    with pytest.raises(NotImplementedError):
+        pool.attend(step, q[:1].clone().requires_grad_())

@@ -1,0 +1,69 @@
+"""Arguments of plan_rotation, and the C entry points' refusals, without a GPU."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from nexusquant_amd import _lib, rotary
+
+
+def test_frequencies_belong_to_their_axes():
+    f = rotary.frequency_axes
+    assert f(64, None, False).tolist() == [0] * 32
+    assert f(64, [8, 12, 12], False).tolist() == [0] * 8 + [1] * 12 + [2] * 12
+    got = f(128, [24, 20, 20], True)
+    assert got[:60].tolist() == [0, 1, 2] * 20 and got[60:].tolist() == [0] * 4
+    assert f(64, [16, 16], True).tolist() == [0, 1] * 16
+    assert f(64, [32, 0], True).tolist() == [0] * 32
+    for sections, interleaved in (([8, 8], False), ([40, -8], False), ([], False), ([8, 24], True), ([8, 12, 12], True)):
+        with pytest.raises(ValueError):
+            f(64, sections, interleaved)
+
+
+def test_arguments_are_checked_before_any_device():
+    with pytest.raises(ValueError, match="head_dim"):
+        rotary.plan_rotation([1, 2], 96)
+    with pytest.raises(TypeError):
+        rotary.plan_rotation([1.5], 64)
+    with pytest.raises(TypeError):
+        rotary.plan_rotation([True], 64)
+    with pytest.raises(_lib.NexusQuantError):
+        rotary.plan_rotation([1], 64, device="cpu")
+
+
+def test_which_outputs_are_apart():
+    x = torch.empty(6, 8, 16)
+    apart = rotary.same_or_apart
+    assert apart(x, x) and apart(x[:, :4], x[:, 4:]) and apart(x[:3], x[3:])
+    assert not apart(x[:, :4], x[:, 3:]) and not apart(x[:, :5], x[:, 2:3]) and not apart(x, x[1:])
+    assert apart(x, torch.empty(6, 8, 16)) and apart(x[:0], x)
+    assert not apart(x, x.transpose(0, 1))
+    own = rotary.vectors_apart
+    assert own(x) and own(x.transpose(0, 1)) and own(x[:, ::2]) and own(x[:1].expand(1, 8, 16))
+    assert not own(x[:, :1].expand(6, 8, 16)) and not own(x[:1].expand(6, 8, 16))
+    assert not own(torch.empty(6 * 8 * 16).as_strided((6, 8, 16), (16, 16, 1)))
+
+
+def test_entry_points_refuse_bad_arguments():
+    lib = _lib.load()
+    freq, axis = np.ones(64, np.float32), np.zeros(64, np.uint8)
+    dummy = ctypes.c_void_p(4096)
+
+    def rotation(axes=1, rows=4, half=64, positions=dummy, out=dummy, axis=axis):
+        return lib.nq_rotation(positions, 0, axes, rows, rows, half, freq.ctypes.data, axis.ctypes.data, out, None)
+
+    assert rotation(axes=0) == rotation(axes=256) == rotation(rows=-1) == rotation(half=0) == rotation(half=129) == -1
+    assert rotation(rows=1 << 27) == rotation(positions=None) == rotation(out=None) == rotation(axis=axis + 1) == -1
+    assert rotation(rows=0) == 0
+
+    def desc(rows=4, hq=2, hk=1, d=64, dtype=0, q=4096, k=4096, qo=8192, ko=8192, angles=4096, strides=(128, 64) * 4):
+        return rotary._PACK.pack(rows, hq, hk, d, dtype, 0, q, k, qo, ko, angles, *strides)
+
+    assert lib.nq_rotate(None, None) == -1
+    for kw in (dict(rows=-1), dict(hq=-1), dict(hk=-2), dict(d=96), dict(dtype=3), dict(q=0), dict(ko=0), dict(angles=0),
+               dict(q=4098), dict(angles=4100), dict(strides=(128, 60) + (128, 64) * 3), dict(strides=(128, 64) * 3 + (1, 64)),
+               dict(rows=(1 << 31) - 1, hq=1 << 20)):
+        assert lib.nq_rotate(desc(**kw), None) == -1, kw
+    assert lib.nq_rotate(desc(rows=0), None) == lib.nq_rotate(desc(hq=0, hk=0), None) == 0
