@@ -804,7 +804,8 @@ int nq_fourbit_read(const nq_pool* pool, int32_t layer, const int32_t* slots, in
  *            [3] the sequence's first query row   [4] the tile's first row
  *            [5] its rows, 1 or more
  *            [6], [7] query token i's partial sums of this chunk are slot
- *                [6] + i * [7]
+ *                [6] + i * [7]; [7] 0: the chunk has all that the rows see, and
+ *                they go to out
  *            [8] the last token that query token 0 sees
  *   joins  [n_joins * 4] query row, its first slot, its slots (consecutive; 0:
  *          the row is zero), 0
@@ -819,7 +820,7 @@ typedef struct nq_fourbit_desc {
     int32_t n_wide, n_few, n_joins, n_slots;
     int32_t causal, sliding_window;
     float scale, hadamard_scale;
-    int32_t reserved;
+    int32_t most_chunks; /* of a join */
     const void* query;
     void* out;
     const int32_t* items;

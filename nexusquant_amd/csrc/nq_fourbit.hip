@@ -10,6 +10,8 @@
 // and its tokens into chunks.  A workgroup takes a tile, a chunk and a kv head: up to 16 rows few_kernel, more wide_kernel.
 // A partial (maximum, sum, value sum) per row and chunk goes to the workspace; join_kernel joins a row's, transforms and
 // rounds.
+#include <type_traits>
+
 #include "nq_flash.h"
 #include "nq_fourbit.h"
 
@@ -93,23 +95,98 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
 // A scale, or 0 for one that is not finite: what those who see it get of it must not change what others get.
 __device__ __forceinline__ float finite_scale(uint16_t bits) { return (bits & 0x7c00u) == 0x7c00u ? 0.0f : f16_bits_to_f32(bits); }
 
-// The power of two that takes a row's largest |v| into [2^14, 2^15), as an exponent; 0 for what has none.
-__device__ __forceinline__ int row_exponent(float big) {
-    int e = 0;
-    if (big > 0.0f && big < __builtin_inff()) (void)__builtin_frexpf(big, &e);
-    return min(max(15 - e, -126), 126);
+// ----------------------------------------------------------------------- queries ----
+
+// A query's transform as whole numbers of 16 bits, 32512 its largest coordinate, in two int8 digits of base 256 (high: -127
+// .. 127, low: -128 .. 127).  Codes are whole numbers too, so a logit's sum is exact in 32 bits, and what is rounded off of a
+// coordinate, 2^-16 of the largest, is the only error.
+constexpr float kQueryMax = 32512.0f;
+
+// What multiplies a row's coordinates, and what then multiplies its logits, from its largest |coordinate| as bits (an
+// infinity or a NaN is larger than any number: its row's logits are NaN).
+__device__ __forceinline__ void query_scale(uint32_t big, float& to_int, float& from_int) {
+    const float b = __builtin_bit_cast(float, max(big, 0x0da24260u));  // 1e-30
+    to_int = kQueryMax / b;
+    from_int = b / (16.0f * kQueryMax);  // (levels come 16 times as large)
+}
+
+// 16 coordinates in the order in which the codes' bytes come out of two words (Bytes): the high and the low digits' bytes.
+__device__ __forceinline__ void query_digits(const float (&x)[16], float to_int, u32x4& high, u32x4& low) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int odd = 0; odd < 2; ++odd) {
+            uint32_t h = 0, l = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int q = (int)__builtin_rintf(x[8 * w + 2 * k + odd] * to_int);
+                const int hi = (q + 128) >> 8;
+                h |= (uint32_t)(hi & 0xff) << (8 * k);
+                l |= (uint32_t)(q & 0xff) << (8 * k);  // q - 256 hi
+            }
+            high[2 * w + odd] = h;
+            low[2 * w + odd] = l;
+        }
+}
+
+// Constants in registers that the compiler must not know: a VALU instruction takes no two literals, and with them a mask and
+// what follows it are two.
+struct Bytes {  // the levels of a word's nibbles as int8, times 16: coordinates 0, 2, 4, 6 and 1, 3, 5, 7
+    uint32_t mask, sign;
+    __device__ __forceinline__ void init() {
+        mask = 0xf0f0f0f0u;
+        sign = 0x80808080u;
+        asm volatile("" : "+s"(mask));
+        asm volatile("" : "+v"(sign));
+    }
+    __device__ __forceinline__ uint32_t even(uint32_t w) const { return ((w << 4) & mask) ^ sign; }
+    __device__ __forceinline__ uint32_t odd(uint32_t w) const { return (w & mask) ^ sign; }
+};
+struct Pairs {  // nibbles j and j + 4 of a word as fp16 values 16 + n (nq_fourbit.h)
+    uint32_t mask, sixteen;
+    __device__ __forceinline__ void init() {
+        mask = 0x03C003C0u;
+        sixteen = 0x4C004C00u;
+        asm volatile("" : "+s"(mask));
+        asm volatile("" : "+v"(sixteen));
+    }
+    template <int J>
+    __device__ __forceinline__ uint32_t get(uint32_t w) const {
+        constexpr int at = 6 - 4 * J;
+        const uint32_t x = at >= 0 ? w << (at >= 0 ? at : 0) : w >> (at < 0 ? -at : 0);
+        return (x & mask) | sixteen;
+    }
+};
+
+// What a row's logits are multiplied by: above zero (what is not seen is -infinity, times zero a NaN), or NaN.
+__device__ __forceinline__ float logit_factor(float c) { return c < 1.2e-38f ? 1.2e-38f : c; }
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+template <int N>
+__device__ __forceinline__ void butterflies(float (&x)[N]) {
+#pragma unroll
+    for (int len = 1; len < N; len <<= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (i & len) continue;
+            const float u = x[i], v = x[i + len];
+            x[i] = u + v;
+            x[i + len] = u - v;
+        }
 }
 
 // ------------------------------------------------------------------- few rows ----
 
-// A wave takes 32 tokens at a time through 16x16x32 MFMAs, from their codes to the output without LDS between:
-//   S = K q~^T     A: lane (token m, kg) the D / 32 words of its row from D / 32 kg on, a word a step; B: queries alike
-//   O^T = V^T P^T  S came out as lane (query, kg) with tokens 4 kg + 0..3 of either half, which is the B operand as it
-//                  stands; A: lane (m, kg) the D / 16 nibbles from D / 16 m on of these eight tokens, nibble j of all of
-//                  them the operand of output tile j
-// Codes stand in the operands as 16 + n.  The 24 too much of each comes off by the logits' first accumulator,
-// -24 sum q~, and by one more tile of ones, which sums the weights.  Queries and weights go in twice, as fp16 and what
-// that rounds off: 22 bits.
+// A wave takes 32 tokens at a time, from their codes to the output without LDS between:
+//   S = K q~^T     16x16x64 int8 products, A: lane (token m, kg) the D / 32 words of its row from D / 32 kg on; B: queries'
+//                  digits alike
+//   O^T = V^T P^T  16x16x32 fp16 products; S came out as lane (query, kg) with tokens 4 kg + 0..3 of either half, which is
+//                  the B operand as it stands; A: lane (m, kg) the D / 16 nibbles from D / 16 m on of these eight tokens,
+//                  nibble j of all of them the operand of output tile j
+// Values' codes stand in the operand as 16 + n; the 24 too much of each comes off by one more tile of ones, which sums the
+// weights.  Weights go in twice, as fp16 and what that rounds off: 22 bits.
 template <int D>
 struct FewShape {
     static constexpr int WAVES = 4, ROWS = 16;
@@ -120,15 +197,15 @@ struct FewShape {
 template <int D>
 struct FewLds {
     f32x4 o[FewShape<D>::WAVES / 2][D / 16][64];
-    uint32_t row[FewShape<D>::CHUNK];  // a token's row of this head
-    uint16_t ks[FewShape<D>::CHUNK], vs[FewShape<D>::CHUNK];  // its scales (fp16)
+    uint32_t row[FewShape<D>::CHUNK];                      // a token's row of this head
+    float ks[FewShape<D>::CHUNK], vs[FewShape<D>::CHUNK];  // its scales
     float max[FewShape<D>::WAVES], m[FewShape<D>::WAVES / 2][16], l[FewShape<D>::WAVES / 2][16];
 };
 
 template <int D, int QDT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>::PER_SIMD))) void few_kernel(FourBitArgs a) {
     using F = FewShape<D>;
-    constexpr int KS = D / 32, TILES = D / 16, NW = F::WAVES, NT = 64 * NW, RB = D / 2;
+    constexpr int KW = D / 32, KS = D / 64, TILES = D / 16, NW = F::WAVES, NT = 64 * NW, RB = D / 2;
     constexpr int VW = D == 256 ? 2 : 1;  // words of a token's values a lane (head_dim 64: half of one)
     __shared__ __align__(16) FewLds<D> lds;
     const int lane = threadIdx.x & 63, n16 = lane & 15, kg = lane >> 4;
@@ -138,20 +215,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
     const int n_units = (it.n_tok + 31) / 32, last_place = 32 * n_units - 1;
 
     // ---- the chunk's tokens: places past it repeat its last (no row sees them) ----
-    uint32_t kcode[2][KS], vcode[8][VW];
+    uint32_t kcode[2][KW], vcode[8][VW];
     auto row_of = [&](int i) {
         const uint32_t t = (uint32_t)(it.tok0 + min(i, it.n_tok - 1)), p = div(t, a.by_tokens);
         return ((uint32_t)it.pages[p] * a.kv_heads + kh) * a.tokens + (t - p * a.tokens);
     };
+    const uint8_t* const kbase = a.pool.codes[0] + 4 * KW * kg;
+    const uint8_t* const vbase = a.pool.codes[1] + (D == 64 ? 4 * (n16 >> 1) : 4 * VW * n16);
     auto load_keys = [&](int half, uint32_t row) {
-        const uint32_t* const p = reinterpret_cast<const uint32_t*>(a.pool.codes[0] + (size_t)row * RB + 4 * KS * kg);
-        if constexpr (KS == 2) {
+        const uint32_t* const p = reinterpret_cast<const uint32_t*>(kbase + (size_t)row * RB);
+        if constexpr (KW == 2) {
             const u32x2 w = *reinterpret_cast<const u32x2*>(p);
             kcode[half][0] = w.x;
             kcode[half][1] = w.y;
         } else {
 #pragma unroll
-            for (int s = 0; s < KS; s += 4) {
+            for (int s = 0; s < KW; s += 4) {
                 const u32x4 w = *reinterpret_cast<const u32x4*>(p + s);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) kcode[half][s + i] = w[i];
@@ -159,11 +238,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
         }
     };
     auto load_values = [&](int i, uint32_t row) {
-        const uint8_t* const p = a.pool.codes[1] + (size_t)row * RB;
-        if constexpr (D == 64) vcode[i][0] = *reinterpret_cast<const uint32_t*>(p + 4 * (n16 >> 1));
-        else if constexpr (D == 128) vcode[i][0] = *reinterpret_cast<const uint32_t*>(p + 4 * n16);
+        const uint8_t* const p = vbase + (size_t)row * RB;
+        if constexpr (VW == 1) vcode[i][0] = *reinterpret_cast<const uint32_t*>(p);
         else {
-            const u32x2 w = *reinterpret_cast<const u32x2*>(p + 8 * n16);
+            const u32x2 w = *reinterpret_cast<const u32x2*>(p);
             vcode[i][0] = w.x;
             vcode[i][VW - 1] = w.y;
         }
@@ -173,16 +251,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
 
     // ---- queries: lane (query n16, kg) coordinates D / 4 kg .. + D / 4 - 1 ----
     const RowAt my = row_at(a, (uint32_t)(it.r0 + min(n16, it.n_rows - 1)), kh);
-    float x[KS][8];
+    float x[D / 4];
     {
         const uint16_t* const p = a.query + (int64_t)(it.q_row0 + (int)my.token) * a.q_row + my.head * a.q_head + (D / 4) * kg;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
+        for (int s = 0; s < D / 32; ++s) {
             const u32x4 w = *reinterpret_cast<const u32x4*>(p + 8 * s);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                x[s][2 * k] = unpack<QDT>(w[k] & 0xffffu);
-                x[s][2 * k + 1] = unpack<QDT>(w[k] >> 16);
+                x[8 * s + 2 * k] = unpack<QDT>(w[k] & 0xffffu);
+                x[8 * s + 2 * k + 1] = unpack<QDT>(w[k] >> 16);
             }
         }
     }
@@ -190,79 +268,50 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
     for (int i = threadIdx.x; i <= last_place; i += NT) {
         const uint32_t row = row_of(i);
         lds.row[i] = row;
-        lds.ks[i] = a.pool.scales[0][row];
+        lds.ks[i] = f16_bits_to_f32(a.pool.scales[0][row]);
         const uint16_t vs = a.pool.scales[1][row];
-        lds.vs[i] = vs;
+        lds.vs[i] = f16_bits_to_f32(vs);
         vmax = __builtin_fmaxf(vmax, finite_scale(vs));
     }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) vmax = __builtin_fmaxf(vmax, __shfl_xor(vmax, o, 64));
     if (lane == 0) lds.max[wave] = vmax;
 
-    // the transform over coordinate bits 0..2 (in a step), then the steps, then kg
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int len = 1; len < 8; len <<= 1)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (i & len) continue;
-                const float u = x[s][i], v = x[s][i + len];
-                x[s][i] = u + v;
-                x[s][i + len] = u - v;
-            }
-#pragma unroll
-    for (int len = 1; len < KS; len <<= 1)
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            if (s & len) continue;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float u = x[s][i], v = x[s + len][i];
-                x[s][i] = u + v;
-                x[s + len][i] = u - v;
-            }
-        }
+    // the transform: a lane's own coordinate bits, then kg's
+    butterflies(x);
     const float sign16 = (lane & 16) ? -1.0f : 1.0f, sign32 = (lane & 32) ? -1.0f : 1.0f;
-    float big = 0.0f;
+    uint32_t big = 0;
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const f32x2 h = rows16(x[s][i]);
-            const f32x2 g = halves(__builtin_fmaf(h.y, sign16, h.x));
-            x[s][i] = __builtin_fmaf(g.y, sign32, g.x);
-            big = __builtin_fmaxf(big, __builtin_fabsf(x[s][i]));
-        }
-    const int qexp = row_exponent(four_max(big));
+    for (int i = 0; i < D / 4; ++i) {
+        const f32x2 h = rows16(x[i]);
+        const f32x2 g = halves(__builtin_fmaf(h.y, sign16, h.x));
+        x[i] = __builtin_fmaf(g.y, sign32, g.x);
+        big = max(big, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
+    }
+    big = max(big, (uint32_t)__shfl_xor((int)big, 16, 64));
+    big = max(big, (uint32_t)__shfl_xor((int)big, 32, 64));
+    float to_int, from_int;
+    query_scale(big, to_int, from_int);
     u32x4 qh[KS], ql[KS];
-    float qsum = 0.0f;
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+    for (int s = 0; s < KS; ++s) {
+        float part[16];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {  // the pair (j, j + 4) of a word's nibbles
-            const float u = __builtin_ldexpf(x[s][j], qexp), v = __builtin_ldexpf(x[s][j + 4], qexp);
-            qh[s][j] = pack2<NQ_F16>(u, v);
-            const float uh = f16_bits_to_f32(qh[s][j] & 0xffffu), vh = f16_bits_to_f32(qh[s][j] >> 16);
-            ql[s][j] = pack2<NQ_F16>(u - uh, v - vh);
-            qsum += (uh + vh) + (f16_bits_to_f32(ql[s][j] & 0xffffu) + f16_bits_to_f32(ql[s][j] >> 16));
-        }
-    const float s_first = -kNibbleBias * four_sum(qsum);
-    const float c = __builtin_ldexpf(a.c, -qexp);
+        for (int i = 0; i < 16; ++i) part[i] = x[16 * s + i];
+        query_digits(part, to_int, qh[s], ql[s]);
+    }
+    const float c = logit_factor(a.c * from_int);
     int lo, hi;
     seen_by(a, it, my.token, lo, hi);
     __syncthreads();
     // The values' scales go with the weights: times 2^vexp the chunk's largest is in [64, 128), so weights (2^kSlack at
-    // most) stay below 2^15.
+    // most) stay below 2^15.  The power of two is in the sum of weights as well: nothing takes it out again.
     float vall = lds.max[0];
 #pragma unroll
     for (int w = 1; w < NW; ++w) vall = __builtin_fmaxf(vall, lds.max[w]);
     int vexp = 0;
-    if (vall > 0.0f) {
-        (void)__builtin_frexpf(vall, &vexp);
-        vexp = 7 - vexp;
-    }
-    const float vmul = __builtin_ldexpf(1.0f, vexp);
+    if (vall > 0.0f) (void)__builtin_frexpf(vall, &vexp);
+    const float lift = vall > 0.0f ? (float)(7 - vexp) : 0.0f;
     auto values_at = [&](int first) {
         const uint32_t* const r = lds.row + first + 4 * kg;
         const u32x4 r0 = *reinterpret_cast<const u32x4*>(r), r1 = *reinterpret_cast<const u32x4*>(r + 16);
@@ -276,42 +325,44 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
     f32x4 o[TILES], wsum = {};
 #pragma unroll
     for (int j = 0; j < TILES; ++j) o[j] = f32x4{};
-    float m = kNoMax, l = 0.0f;
+    float m = kNoMax, l = 0.0f;  // m: c * (lagging) maximum - lift
+    Bytes bytes;
+    Pairs pairs;
+    bytes.init();
+    pairs.init();
     const uint32_t pick_lo = D == 64 && (n16 & 1) ? 0x07060302u : 0x05040100u;
     const u32x4 ones = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
-#pragma unroll 1
-    for (int u = wave; u < n_units; u += NW) {
+    auto unit = [&](int u, auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
         const int next = 32 * min(u + NW, n_units - 1);
         // ---- logits of 16 tokens twice ----
-        f32x4 s[2];
+        float p[8], mx = -__builtin_inff();
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            s[t] = f32x4{s_first, s_first, s_first, s_first};
+            i32x4 sh = {}, sl = {};
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                const uint32_t w = kcode[t][k];
-                const u32x4 v = {nibble_pair<0>(w), nibble_pair<1>(w), nibble_pair<2>(w), nibble_pair<3>(w)};
-                s[t] = mfma16(v, qh[k], mfma16(v, ql[k], s[t]));
+                const uint32_t w0 = kcode[t][2 * k], w1 = kcode[t][2 * k + 1];
+                const i32x4 v = {(int)bytes.even(w0), (int)bytes.odd(w0), (int)bytes.even(w1), (int)bytes.odd(w1)};
+                sh = __builtin_amdgcn_mfma_i32_16x16x64_i8(v, __builtin_bit_cast(i32x4, qh[k]), sh, 0, 0, 0);
+                sl = __builtin_amdgcn_mfma_i32_16x16x64_i8(v, __builtin_bit_cast(i32x4, ql[k]), sl, 0, 0, 0);
+            }
+            const int at = 32 * u + 16 * t + 4 * kg;
+            const f32x4 ks = *reinterpret_cast<const f32x4*>(lds.ks + at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v = (float)((sh[i] << 8) + sl[i]) * ks[i];
+                if constexpr (MASKED) v = at + i >= lo && at + i <= hi ? v : -__builtin_inff();
+                p[4 * t + i] = v;
+                mx = __builtin_fmaxf(mx, v);
             }
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t) load_keys(t, lds.row[next + 16 * t + n16]);
         // ---- weights ----
-        float p[8], mx = -__builtin_inff();
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int at = 32 * u + 16 * t + 4 * kg;
-            const u32x2 kw = *reinterpret_cast<const u32x2*>(lds.ks + at);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float v = s[t][i] * f16_bits_to_f32((i & 1) ? kw[i / 2] >> 16 : kw[i / 2] & 0xffffu) * c;
-                const bool seen = at + i >= lo && at + i <= hi;
-                p[4 * t + i] = seen ? v : -__builtin_inff();
-                mx = __builtin_fmaxf(mx, p[4 * t + i]);
-            }
-        }
-        if (__any(mx > m + kSlack)) {
-            const float to = __builtin_fmaxf(m, four_max(mx));
+        mx *= c;
+        if (__any(mx > m + lift + kSlack)) {
+            const float to = __builtin_fmaxf(m, four_max(mx) - lift);
             const float f = __builtin_amdgcn_exp2f(m - to);
             m = to;
             l *= f;
@@ -323,13 +374,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int at = 32 * u + 16 * t + 4 * kg;
-            const u32x2 vw = *reinterpret_cast<const u32x2*>(lds.vs + at);
+            const f32x4 vs = *reinterpret_cast<const f32x4*>(lds.vs + at);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float e = __builtin_amdgcn_exp2f(p[4 * t + i] - m);
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(p[4 * t + i], c, -m));
                 l += e;
-                const float v = e * f16_bits_to_f32((i & 1) ? vw[i / 2] >> 16 : vw[i / 2] & 0xffffu) * vmul;
-                p[4 * t + i] = at + i >= lo && at + i <= hi ? v : 0.0f;  // (a scale that is not seen may be NaN)
+                const float v = e * vs[i];
+                p[4 * t + i] = !MASKED || (at + i >= lo && at + i <= hi) ? v : 0.0f;  // (a scale that is not seen may be NaN)
             }
         }
 #pragma unroll
@@ -343,21 +394,37 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
         for (int k = 0; k < VW; ++k)
 #pragma unroll
             for (int half = 0; half < (D == 64 ? 1 : 2); ++half) {
-                uint32_t x4[4];
+                uint32_t y[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    x4[i] = __builtin_amdgcn_perm(vcode[2 * i + 1][k], vcode[2 * i][k], half ? 0x07060302u : pick_lo);
+                    y[i] = __builtin_amdgcn_perm(vcode[2 * i + 1][k], vcode[2 * i][k], half ? 0x07060302u : pick_lo);
                 auto tile = [&](int j, u32x4 v) {
                     f32x4& to = o[8 * k + 4 * half + j];
                     to = mfma16(v, rest, mfma16(v, w, to));
                 };
-                tile(0, u32x4{nibble_pair<0>(x4[0]), nibble_pair<0>(x4[1]), nibble_pair<0>(x4[2]), nibble_pair<0>(x4[3])});
-                tile(1, u32x4{nibble_pair<1>(x4[0]), nibble_pair<1>(x4[1]), nibble_pair<1>(x4[2]), nibble_pair<1>(x4[3])});
-                tile(2, u32x4{nibble_pair<2>(x4[0]), nibble_pair<2>(x4[1]), nibble_pair<2>(x4[2]), nibble_pair<2>(x4[3])});
-                tile(3, u32x4{nibble_pair<3>(x4[0]), nibble_pair<3>(x4[1]), nibble_pair<3>(x4[2]), nibble_pair<3>(x4[3])});
+                tile(0, u32x4{pairs.get<0>(y[0]), pairs.get<0>(y[1]), pairs.get<0>(y[2]), pairs.get<0>(y[3])});
+                tile(1, u32x4{pairs.get<1>(y[0]), pairs.get<1>(y[1]), pairs.get<1>(y[2]), pairs.get<1>(y[3])});
+                tile(2, u32x4{pairs.get<2>(y[0]), pairs.get<2>(y[1]), pairs.get<2>(y[2]), pairs.get<2>(y[3])});
+                tile(3, u32x4{pairs.get<3>(y[0]), pairs.get<3>(y[1]), pairs.get<3>(y[2]), pairs.get<3>(y[3])});
             }
         values_at(next);
+    };
+    // Units that every row sees whole are [u0, u1).
+    int u0, u1;
+    {
+        int a0, a1, b0, b1;
+        seen_by(a, it, div((uint32_t)it.r0, a.by_group), a0, a1);
+        seen_by(a, it, div((uint32_t)(it.r0 + it.n_rows - 1), a.by_group), b0, b1);
+        u0 = (b0 + 31) / 32;
+        u1 = (a1 + 1) / 32;
     }
+    int u = wave;
+#pragma unroll 1
+    for (; u < min(u0, n_units); u += NW) unit(u, std::true_type{});
+#pragma unroll 1
+    for (; u < u1; u += NW) unit(u, std::false_type{});
+#pragma unroll 1
+    for (; u < n_units; u += NW) unit(u, std::true_type{});
 #pragma unroll
     for (int j = 0; j < TILES; ++j)
 #pragma unroll
@@ -388,79 +455,109 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
                 for (int i = 0; i < 4; ++i) o[j][i] = __builtin_fmaf(y[i], fo, o[j][i] * f);
             }
         }
-        __syncthreads();
+        if (step > 1) __syncthreads();
     }
-    if (wave > 0 || n16 >= it.n_rows) return;
+    if (wave > 0) return;
+    // lane (n, kg), register i of tile j: coordinate TILES (4 kg + i) + j
+    if (it.slots == 0) {  // the row's only chunk: transformed and rounded here
+        float y[4 * TILES];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < TILES; ++j) y[TILES * i + j] = o[j][i];
+        butterflies(y);
+        const float f = l == 0.0f ? 0.0f : a.hscale / l;
+#pragma unroll
+        for (int i = 0; i < 4 * TILES; ++i) {
+            const f32x2 h = rows16(y[i]);
+            const f32x2 g = halves(__builtin_fmaf(h.y, sign16, h.x));
+            y[i] = __builtin_fmaf(g.y, sign32, g.x) * f;
+        }
+        if (n16 >= it.n_rows) return;
+        uint16_t* const to = a.out + (int64_t)(it.q_row0 + (int)my.token) * a.o_row + my.head * a.o_head + 4 * TILES * kg;
+#pragma unroll
+        for (int i = 0; i < 4 * TILES; i += 4)
+            *reinterpret_cast<u32x2*>(to + i) = u32x2{pack2<QDT>(y[i], y[i + 1]), pack2<QDT>(y[i + 2], y[i + 3])};
+        return;
+    }
+    if (n16 >= it.n_rows) return;
     const size_t slot = (size_t)(uint32_t)(it.slot0 + (int)my.token * it.slots) * a.q_heads + my.head;
     if (kg == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * slot) = f32x2{m, l};
-    const float f = __builtin_ldexpf(1.0f, -vexp);
-    // lane (n, kg), register i of tile j: coordinate D / 16 (4 kg + i) + j
     float* const y = a.part_y + slot * D + TILES * 4 * kg;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < TILES; j += 4)
-            *reinterpret_cast<f32x4*>(y + TILES * i + j) = f32x4{o[j][i] * f, o[j + 1][i] * f, o[j + 2][i] * f, o[j + 3][i] * f};
+            *reinterpret_cast<f32x4*>(y + TILES * i + j) = f32x4{o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]};
 }
 
-// One (query token, head) a workgroup: its chunks' sums weighted and added in a fixed order, then the transform, h and the
-// softmax's sum.  A row that saw nothing is zero.
-template <int D, int QDT>
-__global__ __launch_bounds__(256) void fourbit_join_kernel(FourBitArgs a) {
-    constexpr int V = D / 4, NG = 256 / V;  // lanes of a chunk's row, chunks at a time
-    __shared__ f32x4 s_y[NG][V];
-    __shared__ float s_l[NG];
-    const uint32_t which = blockIdx.x / a.q_heads, head = blockIdx.x % a.q_heads;
+// ----------------------------------------------------------------------- joins ----
+
+// The chunks' sums of a (query token, head) weighted and added in a fixed order, then the transform, h and the softmax's sum.
+// A row that saw nothing is zero.  WIDE: a workgroup for it, D / 4 lanes a chunk; else a wave, all lanes a chunk (2900 tokens
+// of 20 heads x 64 in one to three chunks: 59 us with workgroups).
+template <int D, int QDT, bool WIDE>
+__global__ __launch_bounds__(256) void fourbit_join_kernel(FourBitArgs a, uint32_t n) {
+    constexpr int V = WIDE ? 4 : D / 64, LANES = D / V, NG = (WIDE ? 256 : 64) / LANES;  // chunks at a time
+    __shared__ float s_y[WIDE ? NG : 1][WIDE ? D : 1], s_l[NG];
+    const uint32_t unit = WIDE ? blockIdx.x : 4u * blockIdx.x + (threadIdx.x >> 6);
+    if (unit >= n) return;  // whole wave, and not WIDE's
+    const uint32_t which = unit / a.q_heads, head = unit - which * a.q_heads;
     const int32_t row = a.joins[4 * which], c0 = a.joins[4 * which + 1], c1 = c0 + a.joins[4 * which + 2];
-    const int tid = threadIdx.x, grp = tid / V, at = tid % V;
+    const int tid = WIDE ? (int)threadIdx.x : (int)(threadIdx.x & 63), grp = tid / LANES, at = tid % LANES;
     float m = kNoMax;
     for (int s = c0 + (tid & 63); s < c1; s += 64) m = __builtin_fmaxf(m, a.part_ml[2 * ((size_t)s * a.q_heads + head)]);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, o, 64));
-    f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-    float l = 0.0f;
+    float y[V] = {}, l = 0.0f;
 #pragma unroll 4
     for (int s = c0 + grp; s < c1; s += NG) {
         const size_t i = (size_t)s * a.q_heads + head;
         const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * i] - m);
         l = __builtin_fmaf(f, a.part_ml[2 * i + 1], l);
-        const f32x4 p = *reinterpret_cast<const f32x4*>(a.part_y + i * D + 4 * at);
+        const float* const p = a.part_y + i * D + V * at;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) y[k] = __builtin_fmaf(f, p[k], y[k]);
+        for (int k = 0; k < V; ++k) y[k] = __builtin_fmaf(f, p[k], y[k]);
     }
-    s_y[grp][at] = y;
-    if (at == 0) s_l[grp] = l;
-    __syncthreads();
-    if (tid >= 64) return;
-    // the first wave: lane's coordinates 4 at .. 4 at + 3 (head_dim 64 and 128: several times over)
-    y = s_y[0][at];
-    l = s_l[0];
-    for (int i = 1; i < NG; ++i) {
-        y += s_y[i][at];
-        l += s_l[i];
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) s_y[grp][V * at + k] = y[k];
+        if (at == 0) s_l[grp] = l;
+        __syncthreads();
+        if (tid >= 64) return;
+        // the first wave: lane's coordinates 4 at .. 4 at + 3 (head_dim 64 and 128: several times over)
+        l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < V; ++k) y[k] = 0.0f;
+        for (int i = 0; i < NG; ++i) {
+            l += s_l[i];
+#pragma unroll
+            for (int k = 0; k < V; ++k) y[k] += s_y[i][V * at + k];
+        }
     }
-    const float p0 = y[0] + y[1], p1 = y[0] - y[1], p2 = y[2] + y[3], p3 = y[2] - y[3];
-    y = f32x4{p0 + p2, p1 + p3, p0 - p2, p1 - p3};
+    butterflies(y);
 #pragma unroll
-    for (int o = 1; o < V; o <<= 1)
+    for (int o = 1; o < LANES; o <<= 1)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < V; ++k) {
             const float mine = y[k], other = __shfl_xor(mine, o, 64);
             y[k] = (at & o) ? other - mine : mine + other;
         }
-    if (tid >= V) return;
+    if (tid >= LANES) return;
     const float f = l == 0.0f ? 0.0f : a.hscale / l;
-    *reinterpret_cast<u32x2*>(a.out + (int64_t)row * a.o_row + head * a.o_head + 4 * at) =
-        u32x2{pack2<QDT>(y[0] * f, y[1] * f), pack2<QDT>(y[2] * f, y[3] * f)};
+    uint16_t* const to = a.out + (int64_t)row * a.o_row + head * a.o_head + V * at;
+    if constexpr (V == 1) *to = (uint16_t)pack2<QDT>(y[0] * f, 0.0f);
+#pragma unroll
+    for (int k = 0; k + 1 < V; k += 2) *reinterpret_cast<uint32_t*>(to + k) = pack2<QDT>(y[k] * f, y[k + 1] * f);
 }
 
 // ------------------------------------------------------------------ many rows ----
 
-// 32 rows a wave (nq_flash.h), 64 tokens a stage in one of two LDS buffers: codes come into registers a stage ahead, go to
-// LDS as fp16 (n - 8, exactly) while the other buffer is attended to, and their scales as fp32: the keys' times the
-// logits, the values' times the weights.  With few rows several waves share them and split a stage's two tiles; their sums
-// are joined in LDS.
-// A stage's words are kept in the order of nibble_pair: place 2 j of 8 is coordinate j, place 2 j + 1 coordinate j + 4.
+// 32 rows a wave, 64 tokens a stage in one of two LDS buffers: codes come into registers a stage ahead and go to LDS while the
+// other buffer is attended to, keys as int8 levels times 16, values as fp16 levels, exactly.  S^T = K q~^T on 32x32x32 int8
+// products of two digits, O^T += V^T P^T as in nq_flash.h (Rows).  Scales go to LDS as fp32: the keys' times the logits, the
+// values' times the weights.  With few rows several waves share them and split a stage's two tiles; the upper tile's sums are
+// then joined to the lower's in LDS.
 constexpr int kWideStage = 64;
 
 template <int D, int NW>
@@ -469,8 +566,16 @@ struct WideShape {
     static constexpr int UNITS = 4 * D;                            // 16-byte pieces of a stage's codes
     static constexpr int PER = (UNITS + THREADS - 1) / THREADS;    // a thread
     static constexpr int LOOKUPS = UNITS / 2 > THREADS ? UNITS / 2 / THREADS : 1;  // rows of a thread's pieces
-    static constexpr int PER_SIMD = D == 256 ? 1 : NW / 4 > 2 ? NW / 4 : 2;
+    static constexpr int KEYS = kWideStage * D, BUF = KEYS + 2 * kWideStage * D;   // bytes
+    static constexpr int JOIN = NW / 2 * 32 * D * 4;
+    static constexpr int LDS = 2 * BUF > JOIN ? 2 * BUF : JOIN;
+    static constexpr int PER_SIMD = D == 256 ? 1 : 2;
 };
+// 16-byte chunk c of key row r stands at c ^ key_place(r): 16 rows at one chunk lie in all 64 banks.
+template <int D>
+__device__ __forceinline__ constexpr int key_place(int r) {
+    return D == 64 ? (r >> 2) & 3 : D == 128 ? (r >> 1) & 7 : r & 15;
+}
 
 template <int D, int QDT, int NW>
 __global__ __launch_bounds__((WideShape<D, NW>::THREADS)) __attribute__((amdgpu_waves_per_eu(WideShape<D, NW>::PER_SIMD))) void
@@ -478,12 +583,12 @@ wide_kernel(FourBitArgs a) {
     using T = Tile<D>;
     using W = WideShape<D, NW>;
     constexpr int ROWB = T::ROWB, NT = W::THREADS, RB = D / 2, PR = D / 32;  // pieces a row
+    constexpr int QS = D / 32;                                               // steps of a logit
     static_assert(W::LOOKUPS == 1 || W::PER == 2 * W::LOOKUPS, "keys' and values' pieces of a thread are of the same rows");
-    __shared__ __align__(16) char s_kv[2][2 * kWideStage * ROWB];
+    __shared__ __align__(16) char s_kv[W::LDS];
     __shared__ __align__(16) float s_k[2][kWideStage], s_v[2][kWideStage];
     __shared__ int s_exp[2];
-    __shared__ float s_m[NW][32], s_l[NW][32];
-    static_assert(sizeof(s_kv) >= NW * 32 * D * 4, "the waves' sums must fit the stage buffers");
+    __shared__ float s_m[NW / 2][32], s_l[NW / 2][32];
 
     const int lane = threadIdx.x & 63, n = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -523,32 +628,46 @@ wide_kernel(FourBitArgs a) {
             vs = a.pool.scales[1][row];
         }
     };
+    Bytes bytes;
+    Pairs pairs;
+    bytes.init();
+    pairs.init();
     // The values' scales times 2^(7 - e), e the exponent of the largest so far: weights (2^kSlack at most) stay below 2^15.
     // e grows seldom; the sums are then rescaled.
     int vexp = -40;
     auto store = [&](int buf) {
-        char* const kv = s_kv[buf];
+        char* const kv = s_kv + buf * W::BUF;
 #pragma unroll
         for (int i = 0; i < W::PER; ++i) {
             const int u = i * NT + (int)threadIdx.x;
             if (W::UNITS % NT == 0 || u < W::UNITS) {
-                const bool value = u >= W::UNITS / 2;
-                const int r = piece_row(i), f = value ? T::value_swizzle(r) : T::key_swizzle(r);
-                char* const to = kv + (value ? kWideStage * ROWB : 0) + r * ROWB;
+                const int r = piece_row(i);
+                if (u < W::UNITS / 2) {
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const uint32_t x = code[i][w];
-                    const f16x2 bias = {(_Float16)-kNibbleBias, (_Float16)-kNibbleBias};
-                    const f16x2 p[4] = {__builtin_bit_cast(f16x2, nibble_pair<0>(x)) + bias, __builtin_bit_cast(f16x2, nibble_pair<1>(x)) + bias,
-                                        __builtin_bit_cast(f16x2, nibble_pair<2>(x)) + bias, __builtin_bit_cast(f16x2, nibble_pair<3>(x)) + bias};
-                    *reinterpret_cast<u32x4*>(to + 16 * ((4 * (u % PR) + w) ^ f)) =
-                        u32x4{__builtin_bit_cast(uint32_t, p[0]), __builtin_bit_cast(uint32_t, p[1]), __builtin_bit_cast(uint32_t, p[2]),
-                              __builtin_bit_cast(uint32_t, p[3])};
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t w0 = code[i][2 * h], w1 = code[i][2 * h + 1];
+                        *reinterpret_cast<u32x4*>(kv + r * D + 16 * ((2 * (u % PR) + h) ^ key_place<D>(r))) =
+                            u32x4{bytes.even(w0), bytes.odd(w0), bytes.even(w1), bytes.odd(w1)};
+                    }
+                } else {
+                    char* const to = kv + W::KEYS + r * ROWB;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t x = code[i][w];
+                        const f16x2 bias = {(_Float16)-kNibbleBias, (_Float16)-kNibbleBias};
+                        const uint32_t p[4] = {__builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, pairs.get<0>(x)) + bias),
+                                               __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, pairs.get<1>(x)) + bias),
+                                               __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, pairs.get<2>(x)) + bias),
+                                               __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, pairs.get<3>(x)) + bias)};
+                        // (0, 4), (1, 5), (2, 6), (3, 7) to (0, 1), (2, 3), (4, 5), (6, 7)
+                        *reinterpret_cast<u32x4*>(to + 16 * ((4 * (u % PR) + w) ^ T::value_swizzle(r))) =
+                            u32x4{__builtin_amdgcn_perm(p[1], p[0], 0x05040100u), __builtin_amdgcn_perm(p[3], p[2], 0x05040100u),
+                                  __builtin_amdgcn_perm(p[1], p[0], 0x07060302u), __builtin_amdgcn_perm(p[3], p[2], 0x07060302u)};
+                    }
                 }
             }
         }
         if (wave == 0) {
-            const float v = f16_bits_to_f32(vs);
             float big = finite_scale(vs);
 #pragma unroll
             for (int o = 32; o >= 1; o >>= 1) big = __builtin_fmaxf(big, __shfl_xor(big, o, 64));
@@ -558,7 +677,7 @@ wide_kernel(FourBitArgs a) {
                 vexp = max(vexp, e);
             }
             s_k[buf][lane] = f16_bits_to_f32(ks);
-            s_v[buf][lane] = __builtin_ldexpf(v, 7 - vexp);
+            s_v[buf][lane] = __builtin_ldexpf(f16_bits_to_f32(vs), 7 - vexp);
             if (lane == 0) s_exp[buf] = vexp;
         }
     };
@@ -566,84 +685,75 @@ wide_kernel(FourBitArgs a) {
     load();
     look_up(1);
 
-    // ---- this wave's queries ----
+    // ---- this wave's queries: lane (n, g) coordinates 32 s + 16 g .. + 15 ----
     int rw = 1;  // waves with rows of their own; the others share these rows and take the other tile of a stage
     while (rw < NW && it.n_rows > 32 * rw) rw *= 2;
     const int r0 = 32 * (wave % rw), tile0 = rw == NW ? 0 : wave / rw, tiles = rw == NW ? 2 : 1;
     const bool live = r0 < it.n_rows && tile0 < 2;
-    Rows<NQ_F16, D> rows;
+    Rows<NQ_F16, D> rows;  // its queries: the high digits, then the low ones
     float c;
     int lo, hi;
     {
         const RowAt my = row_at(a, (uint32_t)(it.r0 + min(r0 + n, it.n_rows - 1)), kh);
         seen_by(a, it, my.token, lo, hi);
-        const uint16_t* const p = a.query + (int64_t)(it.q_row0 + (int)my.token) * a.q_row + my.head * a.q_head + 8 * g;
-        float x[T::KS][8];
+        const uint16_t* const p = a.query + (int64_t)(it.q_row0 + (int)my.token) * a.q_row + my.head * a.q_head + 16 * g;
+        float x[16 * QS];
 #pragma unroll
-        for (int s = 0; s < T::KS; ++s) {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(p + 16 * s);
+        for (int s = 0; s < 2 * QS; ++s) {
+            const u32x4 w = *reinterpret_cast<const u32x4*>(p + 32 * (s >> 1) + 8 * (s & 1));
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                x[s][2 * k] = unpack<QDT>(w[k] & 0xffffu);
-                x[s][2 * k + 1] = unpack<QDT>(w[k] >> 16);
+                x[8 * s + 2 * k] = unpack<QDT>(w[k] & 0xffffu);
+                x[8 * s + 2 * k + 1] = unpack<QDT>(w[k] >> 16);
             }
         }
-        // the transform: coordinate bits 0..2 (in a lane's eight), 4.. (the steps), 3 (the other half of the wave)
-#pragma unroll
-        for (int s = 0; s < T::KS; ++s)
-#pragma unroll
-            for (int len = 1; len < 8; len <<= 1)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (i & len) continue;
-                    const float u = x[s][i], v = x[s][i + len];
-                    x[s][i] = u + v;
-                    x[s][i + len] = u - v;
-                }
-#pragma unroll
-        for (int len = 1; len < T::KS; len <<= 1)
-#pragma unroll
-            for (int s = 0; s < T::KS; ++s) {
-                if (s & len) continue;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float u = x[s][i], v = x[s + len][i];
-                    x[s][i] = u + v;
-                    x[s + len][i] = u - v;
-                }
-            }
+        butterflies(x);
         const float sign = g ? -1.0f : 1.0f;
-        float big = 0.0f;
+        uint32_t big = 0;
 #pragma unroll
-        for (int s = 0; s < T::KS; ++s)
+        for (int i = 0; i < 16 * QS; ++i) {
+            const f32x2 h = halves(x[i]);
+            x[i] = __builtin_fmaf(h.y, sign, h.x);
+            big = max(big, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
+        }
+        big = max(big, (uint32_t)__shfl_xor((int)big, 32, 64));
+        float to_int, from_int;
+        query_scale(big, to_int, from_int);
+        c = logit_factor(a.c * from_int);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const f32x2 h = halves(x[s][i]);
-                x[s][i] = __builtin_fmaf(h.y, sign, h.x);
-                big = __builtin_fmaxf(big, __builtin_fabsf(x[s][i]));
-            }
-        const int qexp = row_exponent(both_max(big));
-        c = __builtin_ldexpf(a.c, -qexp);
-        rows.init(lane);
+        for (int s = 0; s < QS; ++s) {
+            float part[16];
 #pragma unroll
-        for (int s = 0; s < T::KS; ++s)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                rows.q[s][j] = pack2<NQ_F16>(__builtin_ldexpf(x[s][j], qexp), __builtin_ldexpf(x[s][j + 4], qexp));
+            for (int i = 0; i < 16; ++i) part[i] = x[16 * s + i];
+            query_digits(part, to_int, rows.q[s], rows.q[QS + s]);
+        }
     }
+    rows.init(lane);
+    const uint32_t k_at = (uint32_t)(n * D + 16 * (g ^ key_place<D>(n)));  // row n of a tile, chunk (2 s + g) ^ its place
     store(0);
     load();
     look_up(2);
     __syncthreads();
     int cur = s_exp[0];
 
-    auto scaled = [&](f32x16& s, const float* k) {
+    auto logits = [&](int buf, int t) {
+        const char* const base = s_kv + buf * W::BUF + 32 * D * t;
+        i32x16 sh = {}, sl = {};
+#pragma unroll
+        for (int s = 0; s < QS; ++s) {
+            const i32x4 k = *reinterpret_cast<const i32x4*>(base + (k_at ^ (uint32_t)(32 * s)));
+            sh = __builtin_amdgcn_mfma_i32_32x32x32_i8(k, __builtin_bit_cast(i32x4, rows.q[s]), sh, 0, 0, 0);
+            sl = __builtin_amdgcn_mfma_i32_32x32x32_i8(k, __builtin_bit_cast(i32x4, rows.q[QS + s]), sl, 0, 0, 0);
+        }
+        const float* const f = s_k[buf] + 32 * t + 4 * g;
+        f32x16 x;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const f32x4 f = *reinterpret_cast<const f32x4*>(k + 8 * i + 4 * g);
+            const f32x4 scale = *reinterpret_cast<const f32x4*>(f + 8 * i);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[4 * i + j] *= f[j];
+            for (int j = 0; j < 4; ++j) x[4 * i + j] = (float)((sh[4 * i + j] << 8) + sl[4 * i + j]) * scale[j];
         }
+        return x;
     };
     auto begin = [&](int buf) {
         const int e = s_exp[buf];
@@ -657,32 +767,26 @@ wide_kernel(FourBitArgs a) {
     // a stage that every row of the workgroup sees whole
     auto whole = [&](int buf) {
         if (!live) return;
-        const char* const kbuf = s_kv[buf];
-        const char* const vbuf = kbuf + kWideStage * ROWB;
 #pragma unroll 1
         for (int t = tile0; t < tile0 + tiles; ++t) {
-            f32x16 s = rows.logits(kbuf, t);
-            scaled(s, s_k[buf] + 32 * t);
+            const f32x16 s = logits(buf, t);
             float mx = s[0];
 #pragma unroll
             for (int j = 1; j < 16; ++j) mx = __builtin_fmaxf(mx, s[j]);
             rows.template raise<true>(mx, c);
             uint32_t p[8];
             rows.template weights<true>(s, c, p, s_v[buf] + 32 * t, g);
-            rows.add_values(p, vbuf, t);
+            rows.add_values(p, s_kv + buf * W::BUF + W::KEYS, t);
         }
     };
     // one that hides tokens from some rows: what they do not see enters neither their maximum nor their sums, whatever it holds
     auto masked = [&](int buf, int first) {
         if (!live) return;
-        const char* const kbuf = s_kv[buf];
-        const char* const vbuf = kbuf + kWideStage * ROWB;
 #pragma unroll 1
         for (int t = tile0; t < tile0 + tiles; ++t) {
             const int from = lo - (first + 32 * t), to = hi - (first + 32 * t);
             if (!__any(from < 32 && to >= 0)) continue;
-            f32x16 s = rows.logits(kbuf, t);
-            scaled(s, s_k[buf] + 32 * t);
+            f32x16 s = logits(buf, t);
             float mx = -__builtin_inff();
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
@@ -708,7 +812,7 @@ wide_kernel(FourBitArgs a) {
                 p[2 * i + 1] = pack2<NQ_F16>(x[2], x[3]);
             }
             rows.l += sum;
-            rows.add_values(p, vbuf, t);
+            rows.add_values(p, s_kv + buf * W::BUF + W::KEYS, t);
         }
     };
     auto end = [&](int stage) {  // the next stage to the other buffer, the one after it into registers
@@ -748,56 +852,85 @@ wide_kernel(FourBitArgs a) {
         end(at);
     }
 
-    // ---- the waves' sums joined, and written ----
-    const float lsum = both_sum(rows.l);
-    if (g == 0) {
-        s_m[wave][n] = rows.m;
-        s_l[wave][n] = lsum;
-    }
-    __syncthreads();
-    {
-        float m = kNoMax;
-        for (int w = wave % rw; w < NW; w += rw) m = __builtin_fmaxf(m, s_m[w][n]);
-        const float f = __builtin_ldexpf(__builtin_amdgcn_exp2f(rows.m - m), cur - 7);
-        // [wave][row][place], 16-byte chunks at chunk ^ row
-        float* const area = reinterpret_cast<float*>(&s_kv[0][0]) + (wave * 32 + n) * D;
+    // ---- the upper tile's sums joined to the lower's (the stages' last barrier is behind all reads of them) ----
+    float l = both_sum(rows.l), m = rows.m;
+    uint32_t end_lane = threadIdx.x;  // what follows from the lane is worked out again: nothing of it is kept over the loops
+    asm volatile("" : "+v"(end_lane));
+    const int n2 = end_lane & 31, g2 = (end_lane >> 5) & 1;
+    const RowAt to_row = row_at(a, (uint32_t)(it.r0 + min(r0 + n2, it.n_rows - 1)), kh);
+    if (rw < NW) {
+        // [wave][row][coordinate], 16-byte chunks at chunk ^ row
+        float* const area = reinterpret_cast<float*>(s_kv) + ((wave % rw) * 32 + n2) * D;
+        if (live && tile0 == 1) {
+            if (g2 == 0) {
+                s_m[wave % rw][n2] = m;
+                s_l[wave % rw][n2] = l;
+            }
+#pragma unroll
+            for (int b = 0; b < T::DB; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<f32x4*>(area + 4 * ((8 * b + 2 * i + g2) ^ (n2 & 15))) =
+                        f32x4{rows.o[b][4 * i], rows.o[b][4 * i + 1], rows.o[b][4 * i + 2], rows.o[b][4 * i + 3]};
+        }
+        __syncthreads();
+        if (tile0 != 0) return;
+        const float mo = s_m[wave][n2], to = __builtin_fmaxf(m, mo);
+        const float f = __builtin_amdgcn_exp2f(m - to), fo = __builtin_amdgcn_exp2f(mo - to);
+        m = to;
+        l = l * f + s_l[wave][n2] * fo;
 #pragma unroll
         for (int b = 0; b < T::DB; ++b)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int to = (8 * b + 2 * i + g) ^ (n & 15);
-                *reinterpret_cast<f32x4*>(area + 4 * to) = f32x4{rows.o[b][4 * i] * f, rows.o[b][4 * i + 1] * f,
-                                                                 rows.o[b][4 * i + 2] * f, rows.o[b][4 * i + 3] * f};
+                const f32x4 y = *reinterpret_cast<const f32x4*>(area + 4 * ((8 * b + 2 * i + g2) ^ (n2 & 15)));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) rows.o[b][4 * i + k] = __builtin_fmaf(y[k], fo, rows.o[b][4 * i + k] * f);
             }
     }
-    __syncthreads();
-    auto slot_of = [&](int r) {
-        const RowAt my = row_at(a, (uint32_t)(it.r0 + r), kh);
-        return (size_t)(uint32_t)(it.slot0 + (int)my.token * it.slots) * a.q_heads + my.head;
-    };
-    for (int r = threadIdx.x; r < it.n_rows; r += NT) {
-        const int w0 = r >> 5, q = r & 31;
-        float m = kNoMax, l = 0.0f;
-        for (int w = w0; w < NW; w += rw) m = __builtin_fmaxf(m, s_m[w][q]);
-        for (int w = w0; w < NW; w += rw) l += s_l[w][q] * __builtin_amdgcn_exp2f(s_m[w][q] - m);
-        *reinterpret_cast<f32x2*>(a.part_ml + 2 * slot_of(r)) = f32x2{m, l};
-    }
-    const float* const sums = reinterpret_cast<const float*>(&s_kv[0][0]);
-    for (int i = threadIdx.x; i < it.n_rows * (D / 8); i += NT) {
-        const int r = i / (D / 8), j = i % (D / 8), w0 = r >> 5, q = r & 31;
-        f32x4 y0 = {}, y1 = {};
-        for (int w = w0; w < NW; w += rw) {
-            y0 += *reinterpret_cast<const f32x4*>(sums + (w * 32 + q) * D + 4 * ((2 * j) ^ (q & 15)));
-            y1 += *reinterpret_cast<const f32x4*>(sums + (w * 32 + q) * D + 4 * ((2 * j + 1) ^ (q & 15)));
+    const float unscale = __builtin_ldexpf(1.0f, cur - 7);
+    // lane (n, g), register 4 i + k of block b: coordinate 32 b + 8 i + 4 g + k
+    if (it.slots == 0) {  // the row's only chunk: transformed and rounded here
+        float y[16 * T::DB];
+#pragma unroll
+        for (int b = 0; b < T::DB; ++b)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) y[16 * b + j] = rows.o[b][j];
+        butterflies(y);
+        const float sign = g2 ? -1.0f : 1.0f, f = l == 0.0f ? 0.0f : a.hscale * unscale / l;
+#pragma unroll
+        for (int i = 0; i < 16 * T::DB; ++i) {
+            const f32x2 h = halves(y[i]);
+            y[i] = __builtin_fmaf(h.y, sign, h.x) * f;
         }
-        float* const to = a.part_y + slot_of(r) * D + 8 * j;  // places to coordinates
-        *reinterpret_cast<f32x4*>(to) = f32x4{y0[0], y0[2], y1[0], y1[2]};
-        *reinterpret_cast<f32x4*>(to + 4) = f32x4{y0[1], y0[3], y1[1], y1[3]};
+        if (r0 + n2 >= it.n_rows) return;
+        uint16_t* const to = a.out + (int64_t)(it.q_row0 + (int)to_row.token) * a.o_row + to_row.head * a.o_head + 4 * g2;
+#pragma unroll
+        for (int b = 0; b < T::DB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float* const v = y + 16 * b + 4 * i;
+                *reinterpret_cast<u32x2*>(to + 32 * b + 8 * i) = u32x2{pack2<QDT>(v[0], v[1]), pack2<QDT>(v[2], v[3])};
+            }
+        return;
     }
+    if (r0 + n2 >= it.n_rows) return;
+    const size_t slot = (size_t)(uint32_t)(it.slot0 + (int)to_row.token * it.slots) * a.q_heads + to_row.head;
+    if (g2 == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * slot) = f32x2{m, l};
+    float* const to = a.part_y + slot * D + 4 * g2;
+#pragma unroll
+    for (int b = 0; b < T::DB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<f32x4*>(to + 32 * b + 8 * i) = f32x4{rows.o[b][4 * i] * unscale, rows.o[b][4 * i + 1] * unscale,
+                                                                   rows.o[b][4 * i + 2] * unscale, rows.o[b][4 * i + 3] * unscale};
 }
 
+// Rows of at most this many chunks are joined a wave each.
+constexpr uint32_t kWaveChunks = 16;
+
 template <int D, int QDT>
-static hipError_t launch_fourbit(FourBitArgs a, uint32_t n_wide, uint32_t n_few, uint32_t n_joins, hipStream_t s) {
+static hipError_t launch_fourbit(FourBitArgs a, uint32_t n_wide, uint32_t n_few, uint32_t n_joins, uint32_t most_chunks, hipStream_t s) {
     if (n_wide > 0) hipLaunchKernelGGL((wide_kernel<D, QDT, 4>), dim3(n_wide * a.kv_heads), dim3(256), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -805,16 +938,20 @@ static hipError_t launch_fourbit(FourBitArgs a, uint32_t n_wide, uint32_t n_few,
     if (n_few > 0) hipLaunchKernelGGL((few_kernel<D, QDT>), dim3(n_few * a.kv_heads), dim3(256), 0, s, a);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (n_joins > 0) hipLaunchKernelGGL((fourbit_join_kernel<D, QDT>), dim3(n_joins * a.q_heads), dim3(256), 0, s, a);
+    if (n_joins > 0) {
+        const uint32_t n = n_joins * a.q_heads;
+        if (most_chunks > kWaveChunks) hipLaunchKernelGGL((fourbit_join_kernel<D, QDT, true>), dim3(n), dim3(256), 0, s, a, n);
+        else hipLaunchKernelGGL((fourbit_join_kernel<D, QDT, false>), dim3((n + 3) / 4), dim3(256), 0, s, a, n);
+    }
     return hipGetLastError();
 }
 
 template <int QDT>
-static hipError_t fourbit_dims(int32_t d, const FourBitArgs& a, uint32_t n_wide, uint32_t n_few, uint32_t n_joins, hipStream_t s) {
+static hipError_t fourbit_dims(int32_t d, const FourBitArgs& a, uint32_t n_wide, uint32_t n_few, uint32_t n_joins, uint32_t most_chunks, hipStream_t s) {
     switch (d) {
-        case 64: return launch_fourbit<64, QDT>(a, n_wide, n_few, n_joins, s);
-        case 128: return launch_fourbit<128, QDT>(a, n_wide, n_few, n_joins, s);
-        default: return launch_fourbit<256, QDT>(a, n_wide, n_few, n_joins, s);
+        case 64: return launch_fourbit<64, QDT>(a, n_wide, n_few, n_joins, most_chunks, s);
+        case 128: return launch_fourbit<128, QDT>(a, n_wide, n_few, n_joins, most_chunks, s);
+        default: return launch_fourbit<256, QDT>(a, n_wide, n_few, n_joins, most_chunks, s);
     }
 }
 
@@ -838,7 +975,7 @@ extern "C" int nq_fourbit_attention(const nq_fourbit_desc* d, void* stream) {
     NQ_CHECK_ARG(d->q_dtype == NQ_F16 || d->q_dtype == NQ_BF16, "nq_fourbit_attention: queries must be fp16 or bf16");
     NQ_CHECK_ARG(d->q_heads > 0 && d->q_heads % p->heads == 0, "nq_fourbit_attention: q_heads %d must be a positive multiple of the pool's %d",
                  d->q_heads, p->heads);
-    NQ_CHECK_ARG(d->n_wide >= 0 && d->n_few >= 0 && d->n_joins >= 0 && d->n_slots >= 0 && d->sliding_window >= 0,
+    NQ_CHECK_ARG(d->n_wide >= 0 && d->n_few >= 0 && d->n_joins >= 0 && d->n_slots >= 0 && d->most_chunks >= 0 && d->sliding_window >= 0,
                  "nq_fourbit_attention: n_wide %d, n_few %d, n_joins %d, n_slots %d, sliding_window %d", d->n_wide, d->n_few, d->n_joins,
                  d->n_slots, d->sliding_window);
     NQ_CHECK_ARG(d->scale > 0.0f && d->scale < 1e30f, "nq_fourbit_attention: scale must be positive");
@@ -880,7 +1017,7 @@ extern "C" int nq_fourbit_attention(const nq_fourbit_desc* d, void* stream) {
     a.hscale = d->hadamard_scale;
     a.c = d->scale * 1.44269504088896340736f * d->hadamard_scale;
     hipStream_t s = (hipStream_t)stream;
-    NQ_CHECK_HIP(d->q_dtype == NQ_F16 ? fourbit_dims<NQ_F16>(dim, a, (uint32_t)d->n_wide, (uint32_t)d->n_few, (uint32_t)d->n_joins, s)
-                                      : fourbit_dims<NQ_BF16>(dim, a, (uint32_t)d->n_wide, (uint32_t)d->n_few, (uint32_t)d->n_joins, s));
+    NQ_CHECK_HIP(d->q_dtype == NQ_F16 ? fourbit_dims<NQ_F16>(dim, a, (uint32_t)d->n_wide, (uint32_t)d->n_few, (uint32_t)d->n_joins, (uint32_t)d->most_chunks, s)
+                                      : fourbit_dims<NQ_BF16>(dim, a, (uint32_t)d->n_wide, (uint32_t)d->n_few, (uint32_t)d->n_joins, (uint32_t)d->most_chunks, s));
     return NQ_OK;
 }

@@ -57,7 +57,7 @@ class FourBitAttentionPlan:
         self._work: Dict[int, tuple] = {}
 
     def work(self, q_heads: int) -> tuple:
-        """(device ints, their places in bytes, counts of wide and few items and joins, slots, workspace bytes) for q_heads
+        """(device ints, their places in bytes, (wide and few items, joins, slots, most chunks), workspace bytes) for q_heads
         query heads."""
         got = self._work.get(q_heads)
         if got is None:
@@ -103,7 +103,7 @@ def _chunk(spans: np.ndarray, heads: int, step: int, least: int, most: int, work
 def attention_items(pages: Sequence[int], lengths: Sequence[int], queries: Sequence[int], causal: bool, window: int, group: int,
                     heads: int, head_dim: int, rows: Sequence[int], most_tokens: int):
     """The work list of nq_fourbit_attention, (items, joins) as flat int32 arrays, and the counts of wide items, few items,
-    joins and slots.
+    joins, slots and the most chunks of a tile.
 
     pages[b], lengths[b], queries[b]: a sequence's pages in the list, tokens and query tokens.  rows: most rows of a wide and
     of a few tile; most_tokens: of a few tile's chunk."""
@@ -114,7 +114,8 @@ def attention_items(pages: Sequence[int], lengths: Sequence[int], queries: Seque
     for b, (n, q) in enumerate(zip(lengths, queries)):
         firsts.append(first_row)
         starts.append(first_page)
-        joins += [(first_row + i, 0, 0, 0) for i in range(q)]
+        if n == 0:
+            joins += [(first_row + i, 0, 0, 0) for i in range(q)]
         first_row += q
         first_page += pages[b]
         if n == 0 or q == 0:
@@ -128,7 +129,7 @@ def attention_items(pages: Sequence[int], lengths: Sequence[int], queries: Seque
             for r0 in range(i0 * group, i1 * group, rows[0]):  # (more heads than a tile has rows: several, cut alike)
                 tiles.append((few, b, i0, i1, r0, min(rows[0], i1 * group - r0), start, end))
     if not tiles:
-        return (np.zeros(0, np.int32), np.array(joins, np.int32).reshape(-1)), (0, 0, len(joins), 0)
+        return (np.zeros(0, np.int32), np.array(joins, np.int32).reshape(-1)), (0, 0, len(joins), 0, 0)
     t = np.array(tiles, dtype=np.int64)
     t = t[np.lexsort((t[:, 6] - t[:, 7], t[:, 0]))]  # wide ones first, long ones before short ones
     kind, span = t[:, 0], t[:, 7] - t[:, 6]
@@ -144,13 +145,15 @@ def attention_items(pages: Sequence[int], lengths: Sequence[int], queries: Seque
     for k in range(len(t)):
         _, b, i0, i1, r0, n_rows, start, end = (int(x) for x in t[k])
         c, step = int(chunks[k]), int(length[k])
+        last = lengths[b] - queries[b] if causal else lengths[b] - 1
+        if c == 1:  # nothing to join
+            items.append((starts[b], start, end - start, firsts[b], r0, n_rows, 0, 0, last, 0, 0, 0))
+            continue
         at = base.get((b, i0))
         if at is None:
             at = base[(b, i0)] = slots
             slots += (i1 - i0) * c
-            for i in range(i0, i1):
-                joins[firsts[b] + i] = (firsts[b] + i, at + (i - i0) * c, c, 0)
-        last = lengths[b] - queries[b] if causal else lengths[b] - 1
+            joins += [(firsts[b] + i, at + (i - i0) * c, c, 0) for i in range(i0, i1)]
         for j in range(c):
             first = start + j * step
             items.append((starts[b], first, min(step, end - first), firsts[b], r0, n_rows, at - i0 * c + j, c, last, 0, 0, 0))
@@ -158,7 +161,7 @@ def attention_items(pages: Sequence[int], lengths: Sequence[int], queries: Seque
         raise ValueError("too many partial sums: split the queries over several plans")
     n_few = int(chunks[few].sum())
     return ((np.array(items, np.int32).reshape(-1), np.array(joins, np.int32).reshape(-1)),
-            (len(items) - n_few, n_few, len(joins), slots))
+            (len(items) - n_few, n_few, len(joins), slots, int(chunks.max())))
 
 
 # nq_fourbit_append_desc and nq_fourbit_desc, packed in one go and passed as bytes
@@ -404,8 +407,8 @@ class FourBitPagePool(PagePool):
         with on_device(dev):
             base = ints.address()
             st = _lib.load().nq_fourbit_attention(_ATTEND_PACK.pack(
-                self.desc_at, int(layer), hq, _lib.NQ_F16 if dtype == torch.float16 else _lib.NQ_BF16, *counts,
-                int(plan.causal), plan.window, scale, hadamard_constant(self.head_dim), 0, q.data_ptr(), out.data_ptr(),
+                self.desc_at, int(layer), hq, _lib.NQ_F16 if dtype == torch.float16 else _lib.NQ_BF16, *counts[:4],
+                int(plan.causal), plan.window, scale, hadamard_constant(self.head_dim), counts[4], q.data_ptr(), out.data_ptr(),
                 base + places[0], base + places[1], base + places[2], *q.stride()[:2], *out.stride()[:2],
                 0 if ws is None else ws.data_ptr(), nbytes), _lib.current_stream_handle(dev))
         _lib.check(st, "nq_fourbit_attention")

@@ -16,14 +16,15 @@ def replay(pages, lengths, queries, causal, window, group, heads, d):
     lib = _lib.load()
     most = [lib.nq_fourbit_rows(0), lib.nq_fourbit_rows(1)]
     cap = lib.nq_fourbit_chunk_tokens()
-    (items, joins), (n_wide, n_few, n_joins, n_slots) = four_bit.attention_items(pages, lengths, queries, causal, window, group,
+    (items, joins), (n_wide, n_few, n_joins, n_slots, most_chunks) = four_bit.attention_items(pages, lengths, queries, causal, window, group,
                                                                                   heads, d, most, cap)
     items, joins = items.reshape(-1, 12), joins.reshape(-1, 4)
-    assert len(items) == n_wide + n_few and len(joins) == n_joins == sum(queries)
+    assert len(items) == n_wide + n_few and len(joins) == n_joins
     first_row = np.concatenate([[0], np.cumsum(queries)])
     first_page = np.concatenate([[0], np.cumsum(pages)])
     seen = {}      # (query row, head in group): how often each token
     written = {}   # slot, head in group
+    direct = set()  # (query row, head in group) without a join
     for k, it in enumerate(items):
         page, tok0, n_tok, q_row0, r0, n_rows, slot0, slots, last = it[:9].tolist()
         few = k >= n_wide
@@ -37,6 +38,10 @@ def replay(pages, lengths, queries, causal, window, group, heads, d):
             lo = max(hi - window + 1, 0) if window else 0
             got = seen.setdefault((q_row0 + i, h), np.zeros(lengths[b], int))
             got[max(lo, tok0):min(hi + 1, tok0 + n_tok)] += 1
+            if slots == 0:
+                assert (q_row0 + i, h) not in direct
+                direct.add((q_row0 + i, h))
+                continue
             slot = slot0 + i * slots
             assert 0 <= slot < n_slots and (slot, h) not in written
             written[slot, h] = q_row0 + i
@@ -46,7 +51,9 @@ def replay(pages, lengths, queries, causal, window, group, heads, d):
         joined.add(row)
         for s in range(at, at + c):
             assert all(written[s, h] == row for h in range(group))
-    assert sum(c for _, _, c, _ in joins.tolist()) * group == len(written)
+    assert sum(c for _, _, c, _ in joins.tolist()) * group == len(written) and all(c <= most_chunks for _, _, c, _ in joins.tolist())
+    rows = {(r, h) for r in joined for h in range(group)}
+    assert not rows & direct and rows | direct == {(r, h) for r in range(sum(queries)) for h in range(group)}
     for b, (n, q) in enumerate(zip(lengths, queries)):
         mask = ref.seen(n, q, causal, window).numpy() if n else None
         for i in range(q):
