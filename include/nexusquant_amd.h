@@ -798,7 +798,6 @@ int nq_fourbit_read(const nq_pool* pool, int32_t layer, const int32_t* slots, in
  *          token and one of the q_heads / heads heads of a kv head, heads
  *          fastest) and a chunk of its tokens: those of up to
  *          nq_fourbit_rows(0) rows, then those of up to nq_fourbit_rows(1)
- *          rows and nq_fourbit_chunk_tokens() tokens
  *            [0] where the sequence's pages start in `pages`
  *            [1] the chunk's first token   [2] its tokens, 1 or more
  *            [3] the sequence's first query row   [4] the tile's first row
@@ -831,7 +830,6 @@ typedef struct nq_fourbit_desc {
     int64_t workspace_bytes;
 } nq_fourbit_desc;
 int32_t nq_fourbit_rows(int32_t kind);
-int32_t nq_fourbit_chunk_tokens(void);
 int64_t nq_fourbit_workspace(int32_t n_slots, int32_t q_heads, int32_t head_dim);
 int nq_fourbit_attention(const nq_fourbit_desc* desc, void* stream);
 

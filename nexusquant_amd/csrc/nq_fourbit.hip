@@ -187,20 +187,79 @@ __device__ __forceinline__ void butterflies(float (&x)[N]) {
 //                  nibble j of all of them the operand of output tile j
 // Values' codes stand in the operand as 16 + n; the 24 too much of each comes off by one more tile of ones, which sums the
 // weights.  Weights go in twice, as fp16 and what that rounds off: 22 bits.
+//
+// Where a section's tokens are and their scales stand in LDS, in one of three places: the next section's are written in the
+// middle of this one, behind a barrier there a wave's last unit asks for the next section's first codes, and a wave that is
+// ahead writes the section after that one, which no wave reads yet.
 template <int D>
 struct FewShape {
     static constexpr int WAVES = 4, ROWS = 16;
-    static constexpr int CHUNK = 1024;  // most tokens of a chunk
+    static constexpr int SECTION = 512, UNITS = SECTION / 32;  // tokens, and units of 32
     static constexpr int PER_SIMD = D == 256 ? 2 : 4;
 };
 
 template <int D>
 struct FewLds {
-    f32x4 o[FewShape<D>::WAVES / 2][D / 16][64];
-    uint32_t row[FewShape<D>::CHUNK];                      // a token's row of this head
-    float ks[FewShape<D>::CHUNK], vs[FewShape<D>::CHUNK];  // its scales
-    float max[FewShape<D>::WAVES], m[FewShape<D>::WAVES / 2][16], l[FewShape<D>::WAVES / 2][16];
+    using F = FewShape<D>;
+    f32x4 o[F::WAVES / 2][D / 16][64];
+    uint32_t row[3][F::SECTION];                 // a token's row of this head
+    float ks[3][F::SECTION], vs[3][F::SECTION];  // its scales
+    uint8_t q[2][16][D + 16];                    // the queries' digits, high and low
+    float factor[16], max[3][F::WAVES], m[F::WAVES / 2][16], l[F::WAVES / 2][16];
 };
+
+// The transform of 16 rows, four a wave: lane (bits 2, 3: row; 0, 1 and 4, 5: j) coordinates D / 16 j .. of one, so that all
+// exchanges are lane permutations.  Digits and factors go to LDS.
+template <int D, int QDT>
+__device__ __forceinline__ void few_queries(const FourBitArgs& a, const Item& it, uint32_t kh, FewLds<D>& lds, int lane, int wave) {
+    constexpr int N = D / 16;
+    const int r = 4 * wave + ((lane >> 2) & 3), j = (lane & 3) | ((lane >> 4) << 2);
+    const RowAt at = row_at(a, (uint32_t)(it.r0 + min(r, it.n_rows - 1)), kh);
+    const uint16_t* const p = a.query + (int64_t)(it.q_row0 + (int)at.token) * a.q_row + at.head * a.q_head + N * j;
+    float x[N];
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(p + i);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint32_t both = w[k];
+            x[i + 2 * k] = unpack<QDT>(both & 0xffffu);
+            x[i + 2 * k + 1] = unpack<QDT>(both >> 16);
+        }
+    }
+    butterflies(x);
+    const float s0 = (lane & 1) ? -1.0f : 1.0f, s1 = (lane & 2) ? -1.0f : 1.0f, s4 = (lane & 16) ? -1.0f : 1.0f, s5 = (lane & 32) ? -1.0f : 1.0f;
+    uint32_t big = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        x[i] = __builtin_fmaf(x[i], s0, dpp_f32<kQuadXor1>(x[i]));
+        x[i] = __builtin_fmaf(x[i], s1, dpp_f32<kQuadXor2>(x[i]));
+        const f32x2 h = rows16(x[i]);
+        const f32x2 g = halves(__builtin_fmaf(h.y, s4, h.x));
+        x[i] = __builtin_fmaf(g.y, s5, g.x);
+        big = max(big, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
+    }
+    big = max(big, dpp_u32<kQuadXor1>(big));
+    big = max(big, dpp_u32<kQuadXor2>(big));
+    big = max(big, (uint32_t)__shfl_xor((int)big, 16, 64));
+    big = max(big, (uint32_t)__shfl_xor((int)big, 32, 64));
+    float to_int, from_int;
+    query_scale(big, to_int, from_int);
+    if (j == 0) lds.factor[r] = from_int;
+    // places of a word's coordinates: the even ones' bytes, then the odd ones'
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        int q[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) q[k] = (int)__builtin_rintf(x[i + k] * to_int);
+        const int coordinate = N * j + i, word = coordinate & ~7, place = (coordinate & 7) >> 1;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            lds.q[0][r][word + 4 * k + place] = (uint8_t)((q[k] + 128) >> 8);
+            lds.q[1][r][word + 4 * k + place] = (uint8_t)q[k];
+        }
+    }
+}
 
 template <int D, int QDT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>::PER_SIMD))) void few_kernel(FourBitArgs a) {
@@ -211,15 +270,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
     const int lane = threadIdx.x & 63, n16 = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t item = div(blockIdx.x, a.by_kv), kh = blockIdx.x - item * a.kv_heads;
-    const Item it = item_of(a, item, F::ROWS, F::CHUNK);
-    const int n_units = (it.n_tok + 31) / 32, last_place = 32 * n_units - 1;
+    const Item it = item_of(a, item, F::ROWS, 0x7fffffff);
+    const int n_units = (it.n_tok + 31) / 32, n_sections = (n_units + F::UNITS - 1) / F::UNITS;
 
-    // ---- the chunk's tokens: places past it repeat its last (no row sees them) ----
+    // ---- tokens: places past the chunk repeat its last (no row sees them) ----
     uint32_t kcode[2][KW], vcode[8][VW];
-    auto row_of = [&](int i) {
+    auto page_of = [&](int i, uint32_t& off) {
         const uint32_t t = (uint32_t)(it.tok0 + min(i, it.n_tok - 1)), p = div(t, a.by_tokens);
-        return ((uint32_t)it.pages[p] * a.kv_heads + kh) * a.tokens + (t - p * a.tokens);
+        off = t - p * a.tokens;
+        return (uint32_t)it.pages[p];
     };
+    auto row_in = [&](uint32_t page, uint32_t off) { return (page * a.kv_heads + kh) * a.tokens + off; };
     const uint8_t* const kbase = a.pool.codes[0] + 4 * KW * kg;
     const uint8_t* const vbase = a.pool.codes[1] + (D == 64 ? 4 * (n16 >> 1) : 4 * VW * n16);
     auto load_keys = [&](int half, uint32_t row) {
@@ -246,95 +307,109 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
             vcode[i][VW - 1] = w.y;
         }
     };
+    // A section's places, two a thread: pages, then rows and scales, then LDS, each asked for before it is needed.
+    constexpr int PER = F::SECTION / NT;
+    uint32_t page[PER], off[PER], row[PER];
+    uint16_t ks[PER], vs[PER];
+    auto look_up = [&](int section) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) load_keys(t, row_of(32 * wave + 16 * t + n16));
-
-    // ---- queries: lane (query n16, kg) coordinates D / 4 kg .. + D / 4 - 1 ----
-    const RowAt my = row_at(a, (uint32_t)(it.r0 + min(n16, it.n_rows - 1)), kh);
-    float x[D / 4];
-    {
-        const uint16_t* const p = a.query + (int64_t)(it.q_row0 + (int)my.token) * a.q_row + my.head * a.q_head + (D / 4) * kg;
+        for (int i = 0; i < PER; ++i) page[i] = page_of(F::SECTION * section + NT * i + (int)threadIdx.x, off[i]);
+    };
+    auto load_scales = [&] {
 #pragma unroll
-        for (int s = 0; s < D / 32; ++s) {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(p + 8 * s);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                x[8 * s + 2 * k] = unpack<QDT>(w[k] & 0xffffu);
-                x[8 * s + 2 * k + 1] = unpack<QDT>(w[k] >> 16);
-            }
+        for (int i = 0; i < PER; ++i) {
+            row[i] = row_in(page[i], off[i]);
+            ks[i] = a.pool.scales[0][row[i]];
+            vs[i] = a.pool.scales[1][row[i]];
         }
-    }
-    float vmax = 0.0f;
-    for (int i = threadIdx.x; i <= last_place; i += NT) {
-        const uint32_t row = row_of(i);
-        lds.row[i] = row;
-        lds.ks[i] = f16_bits_to_f32(a.pool.scales[0][row]);
-        const uint16_t vs = a.pool.scales[1][row];
-        lds.vs[i] = f16_bits_to_f32(vs);
-        vmax = __builtin_fmaxf(vmax, finite_scale(vs));
-    }
+    };
+    auto write = [&](int place) {
+        float big = 0.0f;
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) vmax = __builtin_fmaxf(vmax, __shfl_xor(vmax, o, 64));
-    if (lane == 0) lds.max[wave] = vmax;
-
-    // the transform: a lane's own coordinate bits, then kg's
-    butterflies(x);
-    const float sign16 = (lane & 16) ? -1.0f : 1.0f, sign32 = (lane & 32) ? -1.0f : 1.0f;
-    uint32_t big = 0;
+        for (int i = 0; i < PER; ++i) {
+            const int at = NT * i + (int)threadIdx.x;
+            lds.row[place][at] = row[i];
+            lds.ks[place][at] = f16_bits_to_f32(ks[i]);
+            lds.vs[place][at] = f16_bits_to_f32(vs[i]);
+            big = __builtin_fmaxf(big, finite_scale(vs[i]));
+        }
 #pragma unroll
-    for (int i = 0; i < D / 4; ++i) {
-        const f32x2 h = rows16(x[i]);
-        const f32x2 g = halves(__builtin_fmaf(h.y, sign16, h.x));
-        x[i] = __builtin_fmaf(g.y, sign32, g.x);
-        big = max(big, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
+        for (int o = 32; o >= 1; o >>= 1) big = __builtin_fmaxf(big, __shfl_xor(big, o, 64));
+        if (lane == 0) lds.max[place][wave] = big;
+    };
+    look_up(0);
+    {
+        uint32_t first_page[2], first_off[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) first_page[t] = page_of(32 * wave + 16 * t + n16, first_off[t]);
+        load_scales();
+#pragma unroll
+        for (int t = 0; t < 2; ++t) load_keys(t, row_in(first_page[t], first_off[t]));
     }
-    big = max(big, (uint32_t)__shfl_xor((int)big, 16, 64));
-    big = max(big, (uint32_t)__shfl_xor((int)big, 32, 64));
-    float to_int, from_int;
-    query_scale(big, to_int, from_int);
-    u32x4 qh[KS], ql[KS];
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-        float part[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) part[i] = x[16 * s + i];
-        query_digits(part, to_int, qh[s], ql[s]);
-    }
-    const float c = logit_factor(a.c * from_int);
+    few_queries<D, QDT>(a, it, kh, lds, lane, wave);
+    write(0);
+    look_up(1);
+    const RowAt my = row_at(a, (uint32_t)(it.r0 + min(n16, it.n_rows - 1)), kh);
     int lo, hi;
     seen_by(a, it, my.token, lo, hi);
     __syncthreads();
-    // The values' scales go with the weights: times 2^vexp the chunk's largest is in [64, 128), so weights (2^kSlack at
-    // most) stay below 2^15.  The power of two is in the sum of weights as well: nothing takes it out again.
-    float vall = lds.max[0];
+    u32x4 qh[KS], ql[KS];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) vall = __builtin_fmaxf(vall, lds.max[w]);
-    int vexp = 0;
-    if (vall > 0.0f) (void)__builtin_frexpf(vall, &vexp);
-    const float lift = vall > 0.0f ? (float)(7 - vexp) : 0.0f;
-    auto values_at = [&](int first) {
-        const uint32_t* const r = lds.row + first + 4 * kg;
-        const u32x4 r0 = *reinterpret_cast<const u32x4*>(r), r1 = *reinterpret_cast<const u32x4*>(r + 16);
+    for (int s = 0; s < KS; ++s) {
+        qh[s] = *reinterpret_cast<const u32x4*>(&lds.q[0][n16][(D / 4) * kg + 16 * s]);
+        ql[s] = *reinterpret_cast<const u32x4*>(&lds.q[1][n16][(D / 4) * kg + 16 * s]);
+    }
+    const float c = logit_factor(a.c * lds.factor[n16]);
+    auto values_at = [&](const uint32_t* first) {
+        const u32x4 r0 = *reinterpret_cast<const u32x4*>(first + 4 * kg), r1 = *reinterpret_cast<const u32x4*>(first + 16 + 4 * kg);
 #pragma unroll
         for (int i = 0; i < 4; ++i) load_values(i, r0[i]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) load_values(4 + i, r1[i]);
     };
-    values_at(min(32 * wave, 32 * (n_units - 1)));
+    values_at(lds.row[0] + 32 * min(wave, n_units - 1));
+    load_scales();
+    look_up(2);
 
     f32x4 o[TILES], wsum = {};
 #pragma unroll
     for (int j = 0; j < TILES; ++j) o[j] = f32x4{};
-    float m = kNoMax, l = 0.0f;  // m: c * (lagging) maximum - lift
+    // m: c * (lagging) maximum - lift.  The values' scales go with the weights: times 2^lift the largest so far is in
+    // [64, 128), so weights (2^kSlack at most) stay below 2^15.  The power of two is in the sum of weights as well.
+    float m = kNoMax, l = 0.0f, lift = 31.0f;
     Bytes bytes;
     Pairs pairs;
     bytes.init();
     pairs.init();
     const uint32_t pick_lo = D == 64 && (n16 & 1) ? 0x07060302u : 0x05040100u;
     const u32x4 ones = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+    auto rescale = [&](float f) {
+        l *= f;
+        wsum *= f;
+#pragma unroll
+        for (int j = 0; j < TILES; ++j) o[j] *= f;
+    };
+    auto lower = [&](int place) {  // a section's scales may be larger than those before
+        float big = lds.max[place][0];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) big = __builtin_fmaxf(big, lds.max[place][w]);
+        int e = -24;
+        if (big > 0.0f) (void)__builtin_frexpf(big, &e);
+        const float to = __builtin_fminf(lift, (float)(7 - e));
+        if (to < lift) {
+            rescale(__builtin_amdgcn_exp2f(to - lift));
+            m += lift - to;
+            lift = to;
+        }
+    };
+    int place = 0, next_place = 1;  // of this section and the next
+    lower(0);
     auto unit = [&](int u, auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
-        const int next = 32 * min(u + NW, n_units - 1);
+        const int in = u % F::UNITS, first = 32 * in;  // within the section; its last unit of this wave is UNITS - NW + wave
+        const bool last = in >= F::UNITS - NW;
+        const int ahead = u + NW < n_units ? (last ? 32 * wave : first + 32 * NW) : first;
+        const uint32_t* const next = lds.row[last && u + NW < n_units ? next_place : place] + ahead;
         // ---- logits of 16 tokens twice ----
         float p[8], mx = -__builtin_inff();
 #pragma unroll
@@ -348,38 +423,34 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
                 sl = __builtin_amdgcn_mfma_i32_16x16x64_i8(v, __builtin_bit_cast(i32x4, ql[k]), sl, 0, 0, 0);
             }
             const int at = 32 * u + 16 * t + 4 * kg;
-            const f32x4 ks = *reinterpret_cast<const f32x4*>(lds.ks + at);
+            const f32x4 scale = *reinterpret_cast<const f32x4*>(lds.ks[place] + first + 16 * t + 4 * kg);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float v = (float)((sh[i] << 8) + sl[i]) * ks[i];
+                float v = (float)((sh[i] << 8) + sl[i]) * scale[i];
                 if constexpr (MASKED) v = at + i >= lo && at + i <= hi ? v : -__builtin_inff();
                 p[4 * t + i] = v;
                 mx = __builtin_fmaxf(mx, v);
             }
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t) load_keys(t, lds.row[next + 16 * t + n16]);
+        for (int t = 0; t < 2; ++t) load_keys(t, next[16 * t + n16]);
         // ---- weights ----
         mx *= c;
         if (__any(mx > m + lift + kSlack)) {
             const float to = __builtin_fmaxf(m, four_max(mx) - lift);
-            const float f = __builtin_amdgcn_exp2f(m - to);
+            rescale(__builtin_amdgcn_exp2f(m - to));
             m = to;
-            l *= f;
-            wsum *= f;
-#pragma unroll
-            for (int j = 0; j < TILES; ++j) o[j] *= f;
         }
         u32x4 w, rest;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int at = 32 * u + 16 * t + 4 * kg;
-            const f32x4 vs = *reinterpret_cast<const f32x4*>(lds.vs + at);
+            const f32x4 scale = *reinterpret_cast<const f32x4*>(lds.vs[place] + first + 16 * t + 4 * kg);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(p[4 * t + i], c, -m));
                 l += e;
-                const float v = e * vs[i];
+                const float v = e * scale[i];
                 p[4 * t + i] = !MASKED || (at + i >= lo && at + i <= hi) ? v : 0.0f;  // (a scale that is not seen may be NaN)
             }
         }
@@ -408,6 +479,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
                 tile(3, u32x4{pairs.get<3>(y[0]), pairs.get<3>(y[1]), pairs.get<3>(y[2]), pairs.get<3>(y[3])});
             }
         values_at(next);
+        if (last && u + NW < n_units) {  // the next section's scales
+            place = next_place;
+            next_place = next_place == 2 ? 0 : next_place + 1;
+            lower(place);
+        }
+    };
+    // In the middle of a section that another one follows (so that every wave has all its units of it): the next one to LDS.
+    auto middle = [&](int u) {
+        const int section = u / F::UNITS;
+        if (u % F::UNITS / NW != F::UNITS / NW / 2 || section + 1 >= n_sections) return;
+        write(next_place);
+        load_scales();
+        look_up(section + 3);
+        __syncthreads();
     };
     // Units that every row sees whole are [u0, u1).
     int u0, u1;
@@ -420,11 +505,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
     }
     int u = wave;
 #pragma unroll 1
-    for (; u < min(u0, n_units); u += NW) unit(u, std::true_type{});
+    for (; u < min(u0, n_units); u += NW) {
+        middle(u);
+        unit(u, std::true_type{});
+    }
 #pragma unroll 1
-    for (; u < u1; u += NW) unit(u, std::false_type{});
+    for (; u < u1; u += NW) {
+        middle(u);
+        unit(u, std::false_type{});
+    }
 #pragma unroll 1
-    for (; u < n_units; u += NW) unit(u, std::true_type{});
+    for (; u < n_units; u += NW) {
+        middle(u);
+        unit(u, std::true_type{});
+    }
 #pragma unroll
     for (int j = 0; j < TILES; ++j)
 #pragma unroll
@@ -467,6 +561,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
             for (int j = 0; j < TILES; ++j) y[TILES * i + j] = o[j][i];
         butterflies(y);
         const float f = l == 0.0f ? 0.0f : a.hscale / l;
+        const float sign16 = (lane & 16) ? -1.0f : 1.0f, sign32 = (lane & 32) ? -1.0f : 1.0f;
 #pragma unroll
         for (int i = 0; i < 4 * TILES; ++i) {
             const f32x2 h = rows16(y[i]);
@@ -958,8 +1053,6 @@ static hipError_t fourbit_dims(int32_t d, const FourBitArgs& a, uint32_t n_wide,
 }  // namespace nq
 
 extern "C" int32_t nq_fourbit_rows(int32_t kind) { return kind == 0 ? nq::WideShape<128, 4>::ROWS : nq::FewShape<128>::ROWS; }
-
-extern "C" int32_t nq_fourbit_chunk_tokens(void) { return nq::FewShape<128>::CHUNK; }
 
 extern "C" int64_t nq_fourbit_workspace(int32_t n_slots, int32_t q_heads, int32_t head_dim) {
     if (n_slots <= 0 || q_heads <= 0 || head_dim <= 0) return 0;

@@ -70,7 +70,7 @@ class FourBitAttentionPlan:
             lib = _lib.load()
             parts, counts = attention_items([len(t) for t in self._tables], self.lengths, self.queries, self.causal, self.window,
                                             q_heads // pool.num_heads, pool.num_heads, pool.head_dim,
-                                            [int(lib.nq_fourbit_rows(k)) for k in range(2)], int(lib.nq_fourbit_chunk_tokens()))
+                                            [int(lib.nq_fourbit_rows(k)) for k in range(2)])
             parts = [parts[0], np.concatenate(self._tables) if self._tables else np.zeros(0, np.int32), parts[1]]
             places, at = [], 0
             for v in parts:
@@ -87,26 +87,26 @@ _WIDE_AT_ONCE = {64: 768, 128: 512, 256: 256}
 _FEW_STEP, _WIDE_STEP, _WIDE_LEAST = 128, 64, 256
 
 
-def _chunk(spans: np.ndarray, heads: int, step: int, least: int, most: int, workgroups: int) -> int:
+def _chunk(spans: np.ndarray, heads: int, step: int, least: int, workgroups: int) -> int:
     """Tokens of a chunk: the least multiple of `step`, `least` or more, with which the launch is one round of `workgroups`;
     the longest span's where none is."""
-    lo, hi = -(-least // step), -(-min(most, max(int(spans.max()), least)) // step)
+    lo, hi = -(-least // step), -(-max(int(spans.max()), least) // step)
     while lo < hi:
         mid = (lo + hi) // 2
         if heads * int((-(-spans // (mid * step))).sum()) > workgroups:
             lo = mid + 1
         else:
             hi = mid
-    return min(lo * step, most)
+    return lo * step
 
 
 def attention_items(pages: Sequence[int], lengths: Sequence[int], queries: Sequence[int], causal: bool, window: int, group: int,
-                    heads: int, head_dim: int, rows: Sequence[int], most_tokens: int):
+                    heads: int, head_dim: int, rows: Sequence[int]):
     """The work list of nq_fourbit_attention, (items, joins) as flat int32 arrays, and the counts of wide items, few items,
     joins, slots and the most chunks of a tile.
 
     pages[b], lengths[b], queries[b]: a sequence's pages in the list, tokens and query tokens.  rows: most rows of a wide and
-    of a few tile; most_tokens: of a few tile's chunk."""
+    of a few tile."""
     tiles = []  # kind, sequence, first query token, one past the last, first row, rows, first token, one past the last
     joins = []
     first_row = first_page = 0
@@ -136,9 +136,9 @@ def attention_items(pages: Sequence[int], lengths: Sequence[int], queries: Seque
     length = np.empty(len(t), np.int64)
     few = kind == 1
     if few.any():
-        length[few] = _chunk(span[few], heads, _FEW_STEP, _FEW_STEP, most_tokens, _AT_ONCE[head_dim])
+        length[few] = _chunk(span[few], heads, _FEW_STEP, _FEW_STEP, _AT_ONCE[head_dim])
     if (~few).any():
-        length[~few] = _chunk(span[~few], heads, _WIDE_STEP, _WIDE_LEAST, 1 << 30, _WIDE_AT_ONCE[head_dim])
+        length[~few] = _chunk(span[~few], heads, _WIDE_STEP, _WIDE_LEAST, _WIDE_AT_ONCE[head_dim])
     chunks = -(-span // length)
     items, slots = [], 0
     base: Dict[tuple, int] = {}

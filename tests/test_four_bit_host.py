@@ -15,9 +15,8 @@ def replay(pages, lengths, queries, causal, window, group, heads, d):
     """Every row's tokens and slots as the kernels go through the lists."""
     lib = _lib.load()
     most = [lib.nq_fourbit_rows(0), lib.nq_fourbit_rows(1)]
-    cap = lib.nq_fourbit_chunk_tokens()
     (items, joins), (n_wide, n_few, n_joins, n_slots, most_chunks) = four_bit.attention_items(pages, lengths, queries, causal, window, group,
-                                                                                  heads, d, most, cap)
+                                                                                               heads, d, most)
     items, joins = items.reshape(-1, 12), joins.reshape(-1, 4)
     assert len(items) == n_wide + n_few and len(joins) == n_joins
     first_row = np.concatenate([[0], np.cumsum(queries)])
@@ -28,7 +27,7 @@ def replay(pages, lengths, queries, causal, window, group, heads, d):
     for k, it in enumerate(items):
         page, tok0, n_tok, q_row0, r0, n_rows, slot0, slots, last = it[:9].tolist()
         few = k >= n_wide
-        assert 1 <= n_rows <= most[1 if few else 0] and n_tok >= 1 and (not few or n_tok <= cap)
+        assert 1 <= n_rows <= most[1 if few else 0] and n_tok >= 1
         b = next(b for b in range(len(lengths)) if queries[b] and first_row[b] == q_row0)
         assert first_page[b] == page and 0 <= tok0 and tok0 + n_tok <= lengths[b]
         for r in range(r0, r0 + n_rows):
