@@ -794,10 +794,10 @@ int nq_fourbit_read(const nq_pool* pool, int32_t layer, const int32_t* slots, in
  * h / (q_heads / heads).  A sequence's queries see its tokens up to
  * last + (causal ? i : 0), i the query's number, and with sliding_window W the
  * last W of them; a query that sees none is zero.
- *   items  [(n_wide + n_few) * 12] a tile of a sequence's rows (a row: a query
- *          token and one of the q_heads / heads heads of a kv head, heads
- *          fastest) and a chunk of its tokens: those of up to
- *          nq_fourbit_rows(0) rows, then those of up to nq_fourbit_rows(1)
+ *   items  [n * 12] a tile of a sequence's rows (a row: a query token and one
+ *          of the q_heads / heads heads of a kv head, heads fastest) and a
+ *          chunk of its tokens: n_items[k] tiles of up to
+ *          nq_fourbit_rows(head_dim, k) rows, k 0, 1, 2
  *            [0] where the sequence's pages start in `pages`
  *            [1] the chunk's first token   [2] its tokens, 1 or more
  *            [3] the sequence's first query row   [4] the tile's first row
@@ -816,7 +816,7 @@ int nq_fourbit_read(const nq_pool* pool, int32_t layer, const int32_t* slots, in
 typedef struct nq_fourbit_desc {
     const nq_pool* pool;
     int32_t layer, q_heads, q_dtype; /* NQ_F16 / NQ_BF16 */
-    int32_t n_wide, n_few, n_joins, n_slots;
+    int32_t n_items[3], n_joins, n_slots;
     int32_t causal, sliding_window;
     float scale, hadamard_scale;
     int32_t most_chunks; /* of a join */
@@ -829,7 +829,7 @@ typedef struct nq_fourbit_desc {
     void* workspace;
     int64_t workspace_bytes;
 } nq_fourbit_desc;
-int32_t nq_fourbit_rows(int32_t kind);
+int32_t nq_fourbit_rows(int32_t head_dim, int32_t kind);
 int64_t nq_fourbit_workspace(int32_t n_slots, int32_t q_heads, int32_t head_dim);
 int nq_fourbit_attention(const nq_fourbit_desc* desc, void* stream);
 

@@ -180,7 +180,7 @@ SIGNATURES = {
     "nq_rotate": ([_P, _P], ctypes.c_int),
     "nq_fourbit_append": ([_P, _P], ctypes.c_int),
     "nq_fourbit_read": ([ctypes.POINTER(Pool), _I32, _P, _I32, _I32, _F32, _P, _P, _P], ctypes.c_int),
-    "nq_fourbit_rows": ([_I32], ctypes.c_int32),
+    "nq_fourbit_rows": ([_I32, _I32], ctypes.c_int32),
     "nq_fourbit_workspace": ([_I32, _I32, _I32], _I64),
     "nq_fourbit_attention": ([_P, _P], ctypes.c_int),
     "nq_e8_dequant_matmul": ([_P, _P, _P, _P, _I64, _I32, _I32, _I32, _P], ctypes.c_int),

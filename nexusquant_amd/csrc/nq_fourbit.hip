@@ -1021,18 +1021,25 @@ wide_kernel(FourBitArgs a) {
                                                                    rows.o[b][4 * i + 2] * unscale, rows.o[b][4 * i + 3] * unscale};
 }
 
+// Waves of a workgroup of many rows: at head_dim 256 registers leave one wave a SIMD.
+template <int D>
+constexpr int kManyWaves = D == 256 ? 4 : 8;
+
 // Rows of at most this many chunks are joined a wave each.
 constexpr uint32_t kWaveChunks = 16;
 
 template <int D, int QDT>
-static hipError_t launch_fourbit(FourBitArgs a, uint32_t n_wide, uint32_t n_few, uint32_t n_joins, uint32_t most_chunks, hipStream_t s) {
-    if (n_wide > 0) hipLaunchKernelGGL((wide_kernel<D, QDT, 4>), dim3(n_wide * a.kv_heads), dim3(256), 0, s, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    a.items += (size_t)kItemInts * n_wide;
-    if (n_few > 0) hipLaunchKernelGGL((few_kernel<D, QDT>), dim3(n_few * a.kv_heads), dim3(256), 0, s, a);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
+static hipError_t launch_fourbit(FourBitArgs a, const uint32_t (&n_items)[3], uint32_t n_joins, uint32_t most_chunks, hipStream_t s) {
+    for (int k = 0; k < 3; ++k) {
+        if (n_items[k] == 0) continue;
+        const dim3 grid(n_items[k] * a.kv_heads);
+        if (k == 0) hipLaunchKernelGGL((wide_kernel<D, QDT, kManyWaves<D>>), grid, dim3(64 * kManyWaves<D>), 0, s, a);
+        else if (k == 1) hipLaunchKernelGGL((wide_kernel<D, QDT, 4>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((few_kernel<D, QDT>), grid, dim3(256), 0, s, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        a.items += (size_t)kItemInts * n_items[k];
+    }
     if (n_joins > 0) {
         const uint32_t n = n_joins * a.q_heads;
         if (most_chunks > kWaveChunks) hipLaunchKernelGGL((fourbit_join_kernel<D, QDT, true>), dim3(n), dim3(256), 0, s, a, n);
@@ -1042,17 +1049,20 @@ static hipError_t launch_fourbit(FourBitArgs a, uint32_t n_wide, uint32_t n_few,
 }
 
 template <int QDT>
-static hipError_t fourbit_dims(int32_t d, const FourBitArgs& a, uint32_t n_wide, uint32_t n_few, uint32_t n_joins, uint32_t most_chunks, hipStream_t s) {
+static hipError_t fourbit_dims(int32_t d, const FourBitArgs& a, const uint32_t (&n_items)[3], uint32_t n_joins, uint32_t most_chunks, hipStream_t s) {
     switch (d) {
-        case 64: return launch_fourbit<64, QDT>(a, n_wide, n_few, n_joins, most_chunks, s);
-        case 128: return launch_fourbit<128, QDT>(a, n_wide, n_few, n_joins, most_chunks, s);
-        default: return launch_fourbit<256, QDT>(a, n_wide, n_few, n_joins, most_chunks, s);
+        case 64: return launch_fourbit<64, QDT>(a, n_items, n_joins, most_chunks, s);
+        case 128: return launch_fourbit<128, QDT>(a, n_items, n_joins, most_chunks, s);
+        default: return launch_fourbit<256, QDT>(a, n_items, n_joins, most_chunks, s);
     }
 }
 
 }  // namespace nq
 
-extern "C" int32_t nq_fourbit_rows(int32_t kind) { return kind == 0 ? nq::WideShape<128, 4>::ROWS : nq::FewShape<128>::ROWS; }
+extern "C" int32_t nq_fourbit_rows(int32_t head_dim, int32_t kind) {
+    if (kind == 2) return nq::FewShape<128>::ROWS;
+    return kind == 0 && head_dim <= 128 ? 32 * nq::kManyWaves<128> : nq::WideShape<128, 4>::ROWS;
+}
 
 extern "C" int64_t nq_fourbit_workspace(int32_t n_slots, int32_t q_heads, int32_t head_dim) {
     if (n_slots <= 0 || q_heads <= 0 || head_dim <= 0) return 0;
@@ -1068,18 +1078,18 @@ extern "C" int nq_fourbit_attention(const nq_fourbit_desc* d, void* stream) {
     NQ_CHECK_ARG(d->q_dtype == NQ_F16 || d->q_dtype == NQ_BF16, "nq_fourbit_attention: queries must be fp16 or bf16");
     NQ_CHECK_ARG(d->q_heads > 0 && d->q_heads % p->heads == 0, "nq_fourbit_attention: q_heads %d must be a positive multiple of the pool's %d",
                  d->q_heads, p->heads);
-    NQ_CHECK_ARG(d->n_wide >= 0 && d->n_few >= 0 && d->n_joins >= 0 && d->n_slots >= 0 && d->most_chunks >= 0 && d->sliding_window >= 0,
-                 "nq_fourbit_attention: n_wide %d, n_few %d, n_joins %d, n_slots %d, sliding_window %d", d->n_wide, d->n_few, d->n_joins,
-                 d->n_slots, d->sliding_window);
+    NQ_CHECK_ARG(d->n_items[0] >= 0 && d->n_items[1] >= 0 && d->n_items[2] >= 0 && d->n_joins >= 0 && d->n_slots >= 0 && d->most_chunks >= 0 && d->sliding_window >= 0,
+                 "nq_fourbit_attention: n_items %d, %d, %d, n_joins %d, n_slots %d, most_chunks %d, sliding_window %d", d->n_items[0],
+                 d->n_items[1], d->n_items[2], d->n_joins, d->n_slots, d->most_chunks, d->sliding_window);
     NQ_CHECK_ARG(d->scale > 0.0f && d->scale < 1e30f, "nq_fourbit_attention: scale must be positive");
-    const int64_t n_items = (int64_t)d->n_wide + d->n_few;
+    const int64_t n_items = (int64_t)d->n_items[0] + d->n_items[1] + d->n_items[2];
     if (n_items == 0 && d->n_joins == 0) return NQ_OK;
     NQ_CHECK_ARG(d->query && d->out && (n_items == 0 || (d->items && d->pages)) && (d->n_joins == 0 || d->joins),
                  "nq_fourbit_attention: query, out and the plan's arrays are required");
     NQ_CHECK_ARG(((uintptr_t)d->query & 15u) == 0 && ((uintptr_t)d->out & 7u) == 0 && ((d->q_stride[0] | d->q_stride[1]) & 7) == 0 &&
                      ((d->out_stride[0] | d->out_stride[1]) & 3) == 0,
                  "nq_fourbit_attention: query rows must be 16-byte aligned, out's 8-byte");
-    NQ_CHECK_ARG((uint64_t)n_items * p->heads <= max_blocks(256) && (uint64_t)d->n_joins * d->q_heads <= max_blocks(256),
+    NQ_CHECK_ARG((uint64_t)n_items * p->heads <= max_blocks(512) && (uint64_t)d->n_joins * d->q_heads <= max_blocks(256),
                  "nq_fourbit_attention: grid too large");
     NQ_CHECK_ARG((uint64_t)d->n_slots * d->q_heads < (1ull << 32), "nq_fourbit_attention: too many partial sums");
     const int64_t need = nq_fourbit_workspace(d->n_slots, d->q_heads, dim);
@@ -1110,7 +1120,8 @@ extern "C" int nq_fourbit_attention(const nq_fourbit_desc* d, void* stream) {
     a.hscale = d->hadamard_scale;
     a.c = d->scale * 1.44269504088896340736f * d->hadamard_scale;
     hipStream_t s = (hipStream_t)stream;
-    NQ_CHECK_HIP(d->q_dtype == NQ_F16 ? fourbit_dims<NQ_F16>(dim, a, (uint32_t)d->n_wide, (uint32_t)d->n_few, (uint32_t)d->n_joins, (uint32_t)d->most_chunks, s)
-                                      : fourbit_dims<NQ_BF16>(dim, a, (uint32_t)d->n_wide, (uint32_t)d->n_few, (uint32_t)d->n_joins, (uint32_t)d->most_chunks, s));
+    const uint32_t n[3] = {(uint32_t)d->n_items[0], (uint32_t)d->n_items[1], (uint32_t)d->n_items[2]};
+    NQ_CHECK_HIP(d->q_dtype == NQ_F16 ? fourbit_dims<NQ_F16>(dim, a, n, (uint32_t)d->n_joins, (uint32_t)d->most_chunks, s)
+                                      : fourbit_dims<NQ_BF16>(dim, a, n, (uint32_t)d->n_joins, (uint32_t)d->most_chunks, s));
     return NQ_OK;
 }

@@ -57,7 +57,7 @@ class FourBitAttentionPlan:
         self._work: Dict[int, tuple] = {}
 
     def work(self, q_heads: int) -> tuple:
-        """(device ints, their places in bytes, (wide and few items, joins, slots, most chunks), workspace bytes) for q_heads
+        """(device ints, their places in bytes, (items by kind, joins, slots, most chunks), workspace bytes) for q_heads
         query heads."""
         got = self._work.get(q_heads)
         if got is None:
@@ -70,21 +70,36 @@ class FourBitAttentionPlan:
             lib = _lib.load()
             parts, counts = attention_items([len(t) for t in self._tables], self.lengths, self.queries, self.causal, self.window,
                                             q_heads // pool.num_heads, pool.num_heads, pool.head_dim,
-                                            [int(lib.nq_fourbit_rows(k)) for k in range(2)])
+                                            [int(lib.nq_fourbit_rows(pool.head_dim, k)) for k in range(3)])
             parts = [parts[0], np.concatenate(self._tables) if self._tables else np.zeros(0, np.int32), parts[1]]
             places, at = [], 0
             for v in parts:
                 places.append(at)
                 at += 4 * len(v)
             ints = PlanTensor(np.concatenate(parts).astype(np.int32), pool.device) if at else None
-            got = self._work[q_heads] = (ints, places, counts, int(lib.nq_fourbit_workspace(counts[3], q_heads, pool.head_dim)))
+            got = self._work[q_heads] = (ints, places, counts, int(lib.nq_fourbit_workspace(counts[4], q_heads, pool.head_dim)))
         return got
 
 
-# Workgroups of a launch that run at once (by registers), and the least tokens of a chunk.
-_AT_ONCE = {64: 1024, 128: 1024, 256: 512}
-_WIDE_AT_ONCE = {64: 768, 128: 512, 256: 256}
-_FEW_STEP, _WIDE_STEP, _WIDE_LEAST = 128, 64, 256
+# Tiles of a sequence's rows (query tokens x query heads of a kv head) by kind: many, some, few; tokens that a workgroup takes
+# at a time, and the least of a chunk.
+_MANY, _SOME, _FEW = 0, 1, 2
+_STEP = (64, 64, 128)
+_LEAST = (256, 256, 128)
+_WIDE_AT_ONCE = {64: 512, 128: 512, 256: 256}
+
+
+def _workgroups(kind: int, spans: np.ndarray, heads: int, head_dim: int) -> int:
+    """How many workgroups a launch is cut into (or fewer, where its tiles see few tokens).
+
+    Few rows: 1024 run at once (at head_dim 256 512).  With more than that a ragged batch ends evenly, with fewer there is
+    less to join, or nothing, where a chunk has all of a sequence.  us with 512, 1024 and 2048: 64 rows up to 8192 tokens of
+    8 x 128 86, 80, 77; one row of 131072 34, 33, 37; 8 rows of 4096 15.3, 17.3, 20.8; 24 rows up to 1500 of 20 x 64 13.0,
+    16.4, 18.2; 32 rows up to 8192 of 4 x 256 33, 38, 39."""
+    if kind != _FEW:
+        return _WIDE_AT_ONCE[head_dim] // (2 if kind == _MANY else 1)
+    work = heads * int(spans.sum()) * head_dim // 128
+    return 2048 if work >= 2048 * 1024 else 1024 if work >= 1024 * 512 and head_dim < 256 else 512
 
 
 def _chunk(spans: np.ndarray, heads: int, step: int, least: int, workgroups: int) -> int:
@@ -102,11 +117,11 @@ def _chunk(spans: np.ndarray, heads: int, step: int, least: int, workgroups: int
 
 def attention_items(pages: Sequence[int], lengths: Sequence[int], queries: Sequence[int], causal: bool, window: int, group: int,
                     heads: int, head_dim: int, rows: Sequence[int]):
-    """The work list of nq_fourbit_attention, (items, joins) as flat int32 arrays, and the counts of wide items, few items,
-    joins, slots and the most chunks of a tile.
+    """The work list of nq_fourbit_attention, (items, joins) as flat int32 arrays, and the counts of items by
+    kind, joins, slots and the most chunks of a tile.
 
-    pages[b], lengths[b], queries[b]: a sequence's pages in the list, tokens and query tokens.  rows: most rows of a wide and
-    of a few tile."""
+    pages[b], lengths[b], queries[b]: a sequence's pages in the list, tokens and query tokens.  rows: most rows of a
+    tile by kind (many, some, few)."""
     tiles = []  # kind, sequence, first query token, one past the last, first row, rows, first token, one past the last
     joins = []
     first_row = first_page = 0
@@ -120,25 +135,23 @@ def attention_items(pages: Sequence[int], lengths: Sequence[int], queries: Seque
         first_page += pages[b]
         if n == 0 or q == 0:
             continue
-        per = max(1, rows[0] // group) if q * group > rows[1] else q  # query tokens of a tile
+        per = max(1, rows[0] // group)  # query tokens of a tile
         for i0 in range(0, q, per):
             i1 = min(i0 + per, q)
             end = n - q + i1 if causal else n
             start = max(0, n - q + i0 - window + 1) if window else 0
-            few = int((i1 - i0) * group <= rows[1])
+            kind = max(k for k in range(3) if k == 0 or (i1 - i0) * group <= rows[k])
             for r0 in range(i0 * group, i1 * group, rows[0]):  # (more heads than a tile has rows: several, cut alike)
-                tiles.append((few, b, i0, i1, r0, min(rows[0], i1 * group - r0), start, end))
+                tiles.append((kind, b, i0, i1, r0, min(rows[0], i1 * group - r0), start, end))
     if not tiles:
-        return (np.zeros(0, np.int32), np.array(joins, np.int32).reshape(-1)), (0, 0, len(joins), 0, 0)
+        return (np.zeros(0, np.int32), np.array(joins, np.int32).reshape(-1)), (0, 0, 0, len(joins), 0, 0)
     t = np.array(tiles, dtype=np.int64)
-    t = t[np.lexsort((t[:, 6] - t[:, 7], t[:, 0]))]  # wide ones first, long ones before short ones
+    t = t[np.lexsort((t[:, 6] - t[:, 7], t[:, 0]))]  # by kind, long ones before short ones
     kind, span = t[:, 0], t[:, 7] - t[:, 6]
     length = np.empty(len(t), np.int64)
-    few = kind == 1
-    if few.any():
-        length[few] = _chunk(span[few], heads, _FEW_STEP, _FEW_STEP, _AT_ONCE[head_dim])
-    if (~few).any():
-        length[~few] = _chunk(span[~few], heads, _WIDE_STEP, _WIDE_LEAST, _WIDE_AT_ONCE[head_dim])
+    for k in range(3):
+        if (kind == k).any():
+            length[kind == k] = _chunk(span[kind == k], heads, _STEP[k], _LEAST[k], _workgroups(k, span[kind == k], heads, head_dim))
     chunks = -(-span // length)
     items, slots = [], 0
     base: Dict[tuple, int] = {}
@@ -159,14 +172,14 @@ def attention_items(pages: Sequence[int], lengths: Sequence[int], queries: Seque
             items.append((starts[b], first, min(step, end - first), firsts[b], r0, n_rows, at - i0 * c + j, c, last, 0, 0, 0))
     if slots >= 1 << 31:
         raise ValueError("too many partial sums: split the queries over several plans")
-    n_few = int(chunks[few].sum())
+    n_items = [int(chunks[kind == k].sum()) for k in range(3)]
     return ((np.array(items, np.int32).reshape(-1), np.array(joins, np.int32).reshape(-1)),
-            (len(items) - n_few, n_few, len(joins), slots, int(chunks.max())))
+            (*n_items, len(joins), slots, int(chunks.max())))
 
 
 # nq_fourbit_append_desc and nq_fourbit_desc, packed in one go and passed as bytes
 _APPEND_PACK = struct.Struct("P4i6P8qfi")
-_ATTEND_PACK = struct.Struct("P9i2fi5P4qPq")
+_ATTEND_PACK = struct.Struct("P10i2fi5P4qPq")
 
 
 class FourBitPagePool(PagePool):
@@ -407,8 +420,8 @@ class FourBitPagePool(PagePool):
         with on_device(dev):
             base = ints.address()
             st = _lib.load().nq_fourbit_attention(_ATTEND_PACK.pack(
-                self.desc_at, int(layer), hq, _lib.NQ_F16 if dtype == torch.float16 else _lib.NQ_BF16, *counts[:4],
-                int(plan.causal), plan.window, scale, hadamard_constant(self.head_dim), counts[4], q.data_ptr(), out.data_ptr(),
+                self.desc_at, int(layer), hq, _lib.NQ_F16 if dtype == torch.float16 else _lib.NQ_BF16, *counts[:5],
+                int(plan.causal), plan.window, scale, hadamard_constant(self.head_dim), counts[5], q.data_ptr(), out.data_ptr(),
                 base + places[0], base + places[1], base + places[2], *q.stride()[:2], *out.stride()[:2],
                 0 if ws is None else ws.data_ptr(), nbytes), _lib.current_stream_handle(dev))
         _lib.check(st, "nq_fourbit_attention")

@@ -14,11 +14,12 @@ from oracle import four_bit as ref
 def replay(pages, lengths, queries, causal, window, group, heads, d):
     """Every row's tokens and slots as the kernels go through the lists."""
     lib = _lib.load()
-    most = [lib.nq_fourbit_rows(0), lib.nq_fourbit_rows(1)]
-    (items, joins), (n_wide, n_few, n_joins, n_slots, most_chunks) = four_bit.attention_items(pages, lengths, queries, causal, window, group,
+    most = [lib.nq_fourbit_rows(d, k) for k in range(3)]
+    (items, joins), (*n_items, n_joins, n_slots, most_chunks) = four_bit.attention_items(pages, lengths, queries, causal, window, group,
                                                                                                heads, d, most)
     items, joins = items.reshape(-1, 12), joins.reshape(-1, 4)
-    assert len(items) == n_wide + n_few and len(joins) == n_joins
+    assert len(items) == sum(n_items) and len(joins) == n_joins
+    kinds = np.repeat([0, 1, 2], n_items)
     first_row = np.concatenate([[0], np.cumsum(queries)])
     first_page = np.concatenate([[0], np.cumsum(pages)])
     seen = {}      # (query row, head in group): how often each token
@@ -26,8 +27,7 @@ def replay(pages, lengths, queries, causal, window, group, heads, d):
     direct = set()  # (query row, head in group) without a join
     for k, it in enumerate(items):
         page, tok0, n_tok, q_row0, r0, n_rows, slot0, slots, last = it[:9].tolist()
-        few = k >= n_wide
-        assert 1 <= n_rows <= most[1 if few else 0] and n_tok >= 1
+        assert 1 <= n_rows <= most[kinds[k]] and n_tok >= 1
         b = next(b for b in range(len(lengths)) if queries[b] and first_row[b] == q_row0)
         assert first_page[b] == page and 0 <= tok0 and tok0 + n_tok <= lengths[b]
         for r in range(r0, r0 + n_rows):
@@ -163,7 +163,7 @@ def test_entry_points_refuse_bad_arguments():
     def read(pool=None, layer=0, slots=at, n=3, dtype=0, keys=at, values=at):
         return lib.nq_fourbit_read(c_pool() if pool is None else pool, layer, slots, n, dtype, 1.0, keys, values, None)
 
-    def attend(pool=None, layer=0, hq=4, dtype=0, counts=(1, 1, 1, 2), window=0, scale=0.1, q=at, out=at, items=at, pages=at, joins=at,
+    def attend(pool=None, layer=0, hq=4, dtype=0, counts=(1, 1, 1, 1, 2), window=0, scale=0.1, q=at, out=at, items=at, pages=at, joins=at,
                strides=(512, 128) * 2, ws=at, nbytes=1 << 20):
         pool = c_pool() if pool is None else pool
         return lib.nq_fourbit_attention(four_bit._ATTEND_PACK.pack(
@@ -181,12 +181,12 @@ def test_entry_points_refuse_bad_arguments():
         assert append(**kw) == -1, kw
     for kw in (dict(slots=0), dict(n=-1), dict(dtype=3), dict(keys=0), dict(values=0), dict(values=at + 8), dict(n=(1 << 31) - 1)):
         assert read(**kw) == -1, kw
-    for kw in (dict(hq=0), dict(hq=3), dict(dtype=2), dict(counts=(-1, 1, 1, 1)), dict(counts=(1, 1, -1, 1)), dict(window=-1),
+    for kw in (dict(hq=0), dict(hq=3), dict(dtype=2), dict(counts=(-1, 1, 1, 1, 1)), dict(counts=(1, 1, -1, 1, 1)), dict(counts=(1, 1, 1, -1, 1)), dict(window=-1),
                dict(scale=0.0), dict(scale=float("nan")), dict(q=0), dict(out=0), dict(items=0), dict(pages=0), dict(joins=0), dict(q=at + 8),
                dict(out=at + 4), dict(strides=(512, 124, 512, 128)), dict(strides=(512, 128, 512, 126)), dict(ws=0), dict(nbytes=16),
-               dict(ws=at + 8), dict(counts=(1 << 30, 1 << 30, 1, 1)), dict(counts=(1, 1, 1 << 28, 1))):
+               dict(ws=at + 8), dict(counts=(1 << 30, 1 << 30, 1, 1, 1)), dict(counts=(1, 1, 1, 1 << 28, 1))):
         assert attend(**kw) == -1, kw
-    assert append(rows=0) == read(n=0) == attend(counts=(0, 0, 0, 0)) == 0
+    assert append(rows=0) == read(n=0) == attend(counts=(0, 0, 0, 0, 0)) == 0
     # pools of the other kind
     assert lib.nq_pool_compact(c_pool(), at, 100, 0, 1, 1, at, 8, 1, None) == -1 and b"renumber" in lib.nq_last_error()
     assert lib.nq_pool_write(c_pool(), 0, c_pool(), at, 0, 3, None) == -1
@@ -208,4 +208,4 @@ def test_descriptors_match_the_c_compiler(tmp_path):
     assert all(size == pack.size for (size, _), (_, _, pack) in zip(out, fields) if pack is not None)
     import struct
     assert out[0][1] == struct.calcsize("6i5P6q") and out[1][1] == struct.calcsize("P4i6P8q") and out[2][1] == struct.calcsize("P4i6P")
-    assert out[3][1] == struct.calcsize("P9i2fi") + (-struct.calcsize("P9i2fi")) % 8 and out[4][1] == struct.calcsize("P9i2fi5P4qP")
+    assert out[3][1] == struct.calcsize("P10i2fi") + (-struct.calcsize("P10i2fi")) % 8 and out[4][1] == struct.calcsize("P10i2fi5P4qP")
