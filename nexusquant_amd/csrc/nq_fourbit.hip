@@ -824,31 +824,49 @@ wide_kernel(FourBitArgs a) {
         }
     }
     rows.init(lane);
-    const uint32_t k_at = (uint32_t)(n * D + 16 * (g ^ key_place<D>(n)));  // row n of a tile, chunk (2 s + g) ^ its place
+    // A lane's places in a tile: of row n of the keys its chunks 2 s + g, of the values' rows block b's coordinates.  With the
+    // buffer and the tile known when this is compiled the rest of an address is in the instruction.
+    uint32_t k_at[QS], v_at[T::DB];
+#pragma unroll
+    for (int s = 0; s < QS; ++s) k_at[s] = (uint32_t)(n * D + 16 * ((2 * s + g) ^ key_place<D>(n)));
+#pragma unroll
+    for (int b = 0; b < T::DB; ++b) v_at[b] = (rows.v_at + 64u * (uint32_t)b) ^ rows.v_xor;
     store(0);
     load();
     look_up(2);
     __syncthreads();
     int cur = s_exp[0];
 
-    auto logits = [&](int buf, int t) {
-        const char* const base = s_kv + buf * W::BUF + 32 * D * t;
+    auto logits = [&](const char* kbuf, const float* scales) {
         i32x16 sh = {}, sl = {};
 #pragma unroll
         for (int s = 0; s < QS; ++s) {
-            const i32x4 k = *reinterpret_cast<const i32x4*>(base + (k_at ^ (uint32_t)(32 * s)));
+            const i32x4 k = *reinterpret_cast<const i32x4*>(kbuf + k_at[s]);
             sh = __builtin_amdgcn_mfma_i32_32x32x32_i8(k, __builtin_bit_cast(i32x4, rows.q[s]), sh, 0, 0, 0);
             sl = __builtin_amdgcn_mfma_i32_32x32x32_i8(k, __builtin_bit_cast(i32x4, rows.q[QS + s]), sl, 0, 0, 0);
         }
-        const float* const f = s_k[buf] + 32 * t + 4 * g;
         f32x16 x;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const f32x4 scale = *reinterpret_cast<const f32x4*>(f + 8 * i);
+            const f32x4 scale = *reinterpret_cast<const f32x4*>(scales + 8 * i + 4 * g);
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[4 * i + j] = (float)((sh[4 * i + j] << 8) + sl[4 * i + j]) * scale[j];
         }
         return x;
+    };
+    auto add_values = [&](const uint32_t (&p)[8], const char* vbuf) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const u32x4 w = {p[4 * s], p[4 * s + 1], p[4 * s + 2], p[4 * s + 3]};
+#pragma unroll
+            for (int b = 0; b < T::DB; ++b) {
+                const char* const from = vbuf + 16 * s * ROWB + v_at[b];
+                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_void*)from);
+                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_void*)(from + 8 * ROWB));
+                const u32x2 u = __builtin_bit_cast(u32x2, x), v = __builtin_bit_cast(u32x2, y);
+                rows.o[b] = mfma<NQ_F16>(u32x4{u.x, u.y, v.x, v.y}, w, rows.o[b]);
+            }
+        }
     };
     auto begin = [&](int buf) {
         const int e = s_exp[buf];
@@ -859,20 +877,21 @@ wide_kernel(FourBitArgs a) {
             for (int b = 0; b < T::DB; ++b) rows.o[b] *= f;
         }
     };
-    // a stage that every row of the workgroup sees whole
+    // tile t of a stage that every row of the workgroup sees whole
+    auto whole_tile = [&](const char* kv, const float* sk, const float* sv, int t) {
+        const f32x16 s = logits(kv + 32 * D * t, sk + 32 * t);
+        float mx = s[0];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) mx = __builtin_fmaxf(mx, s[j]);
+        rows.template raise<true>(mx, c);
+        uint32_t p[8];
+        rows.template weights<true>(s, c, p, sv + 32 * t, g);
+        add_values(p, kv + W::KEYS + 32 * ROWB * t);
+    };
     auto whole = [&](int buf) {
         if (!live) return;
 #pragma unroll 1
-        for (int t = tile0; t < tile0 + tiles; ++t) {
-            const f32x16 s = logits(buf, t);
-            float mx = s[0];
-#pragma unroll
-            for (int j = 1; j < 16; ++j) mx = __builtin_fmaxf(mx, s[j]);
-            rows.template raise<true>(mx, c);
-            uint32_t p[8];
-            rows.template weights<true>(s, c, p, s_v[buf] + 32 * t, g);
-            rows.add_values(p, s_kv + buf * W::BUF + W::KEYS, t);
-        }
+        for (int t = tile0; t < tile0 + tiles; ++t) whole_tile(s_kv + buf * W::BUF, s_k[buf], s_v[buf], t);
     };
     // one that hides tokens from some rows: what they do not see enters neither their maximum nor their sums, whatever it holds
     auto masked = [&](int buf, int first) {
@@ -881,7 +900,7 @@ wide_kernel(FourBitArgs a) {
         for (int t = tile0; t < tile0 + tiles; ++t) {
             const int from = lo - (first + 32 * t), to = hi - (first + 32 * t);
             if (!__any(from < 32 && to >= 0)) continue;
-            f32x16 s = logits(buf, t);
+            f32x16 s = logits(s_kv + buf * W::BUF + 32 * D * t, s_k[buf] + 32 * t);
             float mx = -__builtin_inff();
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
@@ -907,7 +926,7 @@ wide_kernel(FourBitArgs a) {
                 p[2 * i + 1] = pack2<NQ_F16>(x[2], x[3]);
             }
             rows.l += sum;
-            rows.add_values(p, s_kv + buf * W::BUF + W::KEYS, t);
+            add_values(p, s_kv + buf * W::BUF + W::KEYS + 32 * ROWB * t);
         }
     };
     auto end = [&](int stage) {  // the next stage to the other buffer, the one after it into registers
@@ -933,6 +952,25 @@ wide_kernel(FourBitArgs a) {
         begin(at & 1);
         masked(at & 1, kWideStage * at);
         end(at);
+    }
+    if (tiles == 2 && r0 < it.n_rows) {
+        if ((at & 1) && at < it1) {
+            begin(1);
+            whole(1);
+            end(at);
+            ++at;
+        }
+#pragma unroll 1
+        for (; at + 1 < it1; at += 2) {
+            begin(0);
+            whole_tile(s_kv, s_k[0], s_v[0], 0);
+            whole_tile(s_kv, s_k[0], s_v[0], 1);
+            end(at);
+            begin(1);
+            whole_tile(s_kv + W::BUF, s_k[1], s_v[1], 0);
+            whole_tile(s_kv + W::BUF, s_k[1], s_v[1], 1);
+            end(at + 1);
+        }
     }
 #pragma unroll 1
     for (; at < it1; ++at) {

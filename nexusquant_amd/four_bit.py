@@ -81,38 +81,66 @@ class FourBitAttentionPlan:
         return got
 
 
-# Tiles of a sequence's rows (query tokens x query heads of a kv head) by kind: many, some, few; tokens that a workgroup takes
-# at a time, and the least of a chunk.
+# Tiles of a sequence's rows (query tokens x query heads of a kv head) by kind: many, some, few.
 _MANY, _SOME, _FEW = 0, 1, 2
-_STEP = (64, 64, 128)
-_LEAST = (256, 256, 128)
-_WIDE_AT_ONCE = {64: 512, 128: 512, 256: 256}
+# Where no sequence has this many rows tiles are of some: 24 sequences of up to 223 rows over 1500 tokens of 20 x 64 57 us, with
+# tiles of many 78 (they leave half of the CUs idle); 2048 x 4 rows over 32768 of 8 x 128 1340 and 1204 (what is decoded
+# serves twice the rows).
+_MANY_ROWS = 512
+_FEW_STEP = 128  # tokens that a workgroup takes at a time
+_STAGE, _LEAST = 64, 256  # of wider tiles, and the least of a chunk
+_AT_ONCE = ({64: 256, 128: 256, 256: 256}, {64: 512, 128: 512, 256: 256})  # workgroups of many and of some rows
+_STAGE_US = {64: 1.8, 128: 2.3, 256: 3.7}
+_START_STAGES = 3  # what a workgroup's start and end cost
 
 
-def _workgroups(kind: int, spans: np.ndarray, heads: int, head_dim: int) -> int:
-    """How many workgroups a launch is cut into (or fewer, where its tiles see few tokens).
+def _even(spans: np.ndarray, most: int, step: int):
+    """(chunks, tokens of a chunk) of each span: as few chunks of at most `most` tokens as it takes, all alike but for a
+    multiple of `step`."""
+    chunks = -(-spans // most)
+    each = -(-spans // (chunks * step)) * step
+    return -(-spans // each), each
 
-    Few rows: 1024 run at once (at head_dim 256 512).  With more than that a ragged batch ends evenly, with fewer there is
-    less to join, or nothing, where a chunk has all of a sequence.  us with 512, 1024 and 2048: 64 rows up to 8192 tokens of
-    8 x 128 86, 80, 77; one row of 131072 34, 33, 37; 8 rows of 4096 15.3, 17.3, 20.8; 24 rows up to 1500 of 20 x 64 13.0,
-    16.4, 18.2; 32 rows up to 8192 of 4 x 256 33, 38, 39."""
-    if kind != _FEW:
-        return _WIDE_AT_ONCE[head_dim] // (2 if kind == _MANY else 1)
+
+def _few_chunks(spans: np.ndarray, heads: int, head_dim: int):
+    """Chunks of few rows, of the least length with which the launch is so many workgroups.
+
+    1024 run at once (at head_dim 256 512).  With more than that a ragged batch ends evenly, with fewer there is less to
+    join, or nothing, where a chunk has all of a sequence.  us with 512, 1024 and 2048: 64 rows up to 8192 tokens of 8 x 128
+    86, 80, 77; one row of 131072 34, 33, 37; 8 rows of 4096 15.3, 17.3, 20.8; 24 rows up to 1500 of 20 x 64 13.0, 16.4,
+    18.2; 32 rows up to 8192 of 4 x 256 33, 38, 39."""
     work = heads * int(spans.sum()) * head_dim // 128
-    return 2048 if work >= 2048 * 1024 else 1024 if work >= 1024 * 512 and head_dim < 256 else 512
-
-
-def _chunk(spans: np.ndarray, heads: int, step: int, least: int, workgroups: int) -> int:
-    """Tokens of a chunk: the least multiple of `step`, `least` or more, with which the launch is one round of `workgroups`;
-    the longest span's where none is."""
-    lo, hi = -(-least // step), -(-max(int(spans.max()), least) // step)
+    workgroups = 2048 if work >= 2048 * 1024 else 1024 if work >= 1024 * 512 and head_dim < 256 else 512
+    lo, hi = 1, -(-int(spans.max()) // _FEW_STEP)
     while lo < hi:
         mid = (lo + hi) // 2
-        if heads * int((-(-spans // (mid * step))).sum()) > workgroups:
+        if heads * int((-(-spans // (mid * _FEW_STEP))).sum()) > workgroups:
             lo = mid + 1
         else:
             hi = mid
-    return lo * step
+    return _even(spans, lo * _FEW_STEP, _FEW_STEP)
+
+
+def _wide_chunks(spans: np.ndarray, rows: np.ndarray, heads: int, head_dim: int, at_once: int):
+    """Chunks of many or some rows, by what the launch would take: where all workgroups run at once the longest, else their
+    share of the work and half a chunk until the last has ended; and the sums that are joined."""
+    longest = int(spans.max())
+    best = float("inf")
+    for cut in (1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 32, 48, 64, 128):
+        length = max(_LEAST, -(-longest // (cut * _STAGE)) * _STAGE)
+        chunks, each = _even(spans, length, _STAGE)
+        n = heads * int(chunks.sum())
+        stages = heads * float(spans.sum()) / _STAGE + n * _START_STAGES
+        most = float(np.minimum(spans, each).max()) / _STAGE
+        us = _STAGE_US[head_dim] * (most + _START_STAGES if n <= at_once else stages / at_once + most / 2)
+        split = chunks > 1
+        if split.any():
+            us += 5.0 + heads * head_dim * 8.0 * float((rows * chunks)[split].sum()) / 3.5e6
+        if us < best:
+            best, found = us, (chunks, each)
+        if length == _LEAST:
+            break
+    return found
 
 
 def attention_items(pages: Sequence[int], lengths: Sequence[int], queries: Sequence[int], causal: bool, window: int, group: int,
@@ -126,6 +154,7 @@ def attention_items(pages: Sequence[int], lengths: Sequence[int], queries: Seque
     joins = []
     first_row = first_page = 0
     starts, firsts = [], []
+    wide = rows[_MANY if max(queries, default=0) * group >= _MANY_ROWS else _SOME]  # one kind beside few: launches follow each other
     for b, (n, q) in enumerate(zip(lengths, queries)):
         firsts.append(first_row)
         starts.append(first_page)
@@ -135,29 +164,30 @@ def attention_items(pages: Sequence[int], lengths: Sequence[int], queries: Seque
         first_page += pages[b]
         if n == 0 or q == 0:
             continue
-        per = max(1, rows[0] // group)  # query tokens of a tile
+        per = max(1, wide // group)  # query tokens of a tile
         for i0 in range(0, q, per):
             i1 = min(i0 + per, q)
             end = n - q + i1 if causal else n
             start = max(0, n - q + i0 - window + 1) if window else 0
-            kind = max(k for k in range(3) if k == 0 or (i1 - i0) * group <= rows[k])
-            for r0 in range(i0 * group, i1 * group, rows[0]):  # (more heads than a tile has rows: several, cut alike)
-                tiles.append((kind, b, i0, i1, r0, min(rows[0], i1 * group - r0), start, end))
+            kind = _FEW if (i1 - i0) * group <= rows[_FEW] else _MANY if wide > rows[_SOME] else _SOME
+            for r0 in range(i0 * group, i1 * group, wide):  # (more heads than a tile has rows: several, cut alike)
+                tiles.append((kind, b, i0, i1, r0, min(wide, i1 * group - r0), start, end))
     if not tiles:
         return (np.zeros(0, np.int32), np.array(joins, np.int32).reshape(-1)), (0, 0, 0, len(joins), 0, 0)
     t = np.array(tiles, dtype=np.int64)
     t = t[np.lexsort((t[:, 6] - t[:, 7], t[:, 0]))]  # by kind, long ones before short ones
     kind, span = t[:, 0], t[:, 7] - t[:, 6]
-    length = np.empty(len(t), np.int64)
+    chunks, each = np.empty(len(t), np.int64), np.empty(len(t), np.int64)
     for k in range(3):
-        if (kind == k).any():
-            length[kind == k] = _chunk(span[kind == k], heads, _STEP[k], _LEAST[k], _workgroups(k, span[kind == k], heads, head_dim))
-    chunks = -(-span // length)
+        of = kind == k
+        if of.any():
+            chunks[of], each[of] = _few_chunks(span[of], heads, head_dim) if k == _FEW else \
+                _wide_chunks(span[of], t[of, 5], heads, head_dim, _AT_ONCE[k][head_dim])
     items, slots = [], 0
     base: Dict[tuple, int] = {}
     for k in range(len(t)):
         _, b, i0, i1, r0, n_rows, start, end = (int(x) for x in t[k])
-        c, step = int(chunks[k]), int(length[k])
+        c, step = int(chunks[k]), int(each[k])
         last = lengths[b] - queries[b] if causal else lengths[b] - 1
         if c == 1:  # nothing to join
             items.append((starts[b], start, end - start, firsts[b], r0, n_rows, 0, 0, last, 0, 0, 0))

@@ -136,6 +136,12 @@ def test_rows_that_are_zero_tiny_huge_or_not_finite():
 
 # ----------------------------------------------------------------- attention --
 
+def step(few):
+    """Relative errors of a query's coordinate and of a weight: few rows' queries have 16 bits below the largest coordinate
+    (2^-16 of it: what counts of smaller ones is within the sum's bound) and weights 22; wider tiles round weights to fp16."""
+    return 2.0 ** -15 if few else 2.0 ** -11
+
+
 def check_attention(pool, tables, lens, queries, q, got, dtype, causal=True, window=0, scale=None, layer=0, few=None):
     """Every row against 64 bits, by the bound of what the kernels round (oracle/four_bit.py) plus half a step of the output."""
     d = pool.head_dim
@@ -148,8 +154,7 @@ def check_attention(pool, tables, lens, queries, q, got, dtype, causal=True, win
             mask = ref.seen(n, m, causal, window)
             want, bound = ref.attend(q[row:row + m].cpu(), kl, ks, vl, vs, mask, d ** -0.5 if scale is None else scale)
             narrow = m * (q.shape[1] // pool.num_heads) <= 16 if few is None else few
-            # 22 bits are a step of 2^-22 of what fp16 holds in full; below that 2^-25 of a row's largest (in 2^14 .. 2^15)
-            u = 2.0 ** -21 if narrow else 2.0 ** -11
+            u = step(narrow)
             off = (got[row:row + m].cpu().double() - want).abs()
             lim = bound(u, u) + want.abs() * torch.finfo(dtype).eps / 2 + 2.0 ** -25
             assert (off <= lim).all(), (n, m, float((off - lim).max()))
@@ -257,7 +262,7 @@ def test_scales_and_queries_of_all_sizes(dtype):
             kl, ks = ref.sequence(pool.key_codes[0].cpu(), pool.key_scales[0].cpu(), tables[0], n)
             vl, vs = ref.sequence(pool.value_codes[0].cpu(), pool.value_scales[0].cpu(), tables[0], n)
             want, bound = ref.attend(q.cpu(), kl, ks, vl, vs, ref.seen(n, queries, True, 0), 128 ** -0.5)
-            u = 2.0 ** -21 if queries == 1 else 2.0 ** -11
+            u = step(queries == 1)
             assert ((got.cpu().double() - want).abs() <= bound(u, u) + want.abs() * torch.finfo(T).eps / 2 + 2.0 ** -25).all()
 
 
