@@ -118,8 +118,67 @@ struct AppendArgs {
     float hscale;
 };
 
+// One row encoded in 64 bits by a whole wave, from its input on: lane l coordinates D / 64 l .. .
+template <int DT, int D>
+__device__ __forceinline__ void encode_exactly(const uint8_t* from, const float* angles, int lane, uint32_t* codes, uint16_t* scale) {
+    constexpr int V = D / 64;
+    double x[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        if constexpr (DT == NQ_F16) x[k] = (double)f16_bits_to_f32(reinterpret_cast<const uint16_t*>(from)[V * lane + k]);
+        else x[k] = (double)bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(from)[V * lane + k]);
+    }
+    if (angles) {
+        const int half = V * (lane & 31);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const double other = __shfl_xor(x[k], 32, 64), c = angles[half + k], s = angles[D / 2 + half + k];
+            x[k] = x[k] * c + (lane < 32 ? -other : other) * s;
+        }
+    }
+#pragma unroll
+    for (int len = 1; len < V; len <<= 1)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            if (k & len) continue;
+            const double u = x[k], v = x[k + len];
+            x[k] = u + v;
+            x[k + len] = u - v;
+        }
+    double most = 0.0;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const double other = __shfl_xor(x[k], o, 64);
+            x[k] = (lane & o) ? other - x[k] : x[k] + other;
+        }
+        most = fmax(most, fabs(x[k]));
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) most = fmax(most, __shfl_xor(most, o, 64));
+    const double h = D == 64 ? 0.125 : D == 256 ? 0.0625 : 0.08838834764831844;  // 1 / sqrt(D)
+    const uint32_t s16 = f32_to_f16_bits((float)fmin(most * h / 7.5, 65504.0));  // by way of fp32, as where 32 bits suffice
+    const double inv = s16 ? h / (double)f16_bits_to_f32(s16) : 0.0;
+    uint32_t w = 0;
+#pragma unroll
+    for (int k = 0; k < V; ++k) w |= (uint32_t)fmin(fmax(floor(x[k] * inv + 8.5), 0.0), 15.0) << (4 * ((V * lane + k) & 7));
+#pragma unroll
+    for (int o = 1; o < 8 / V; o <<= 1) w |= (uint32_t)__shfl_xor((int)w, o, 64);
+    if ((V * lane & 7) == 0) codes[V * lane >> 3] = w;
+    if (lane == 0) *scale = (uint16_t)s16;
+}
+
 // A wave takes a token, and its heads sixteen at a time, a quad a head (nq_rowmath.h): keys, then values, then queries.
 // The token's cosines and sines stay in registers.
+//
+// 32 bits decide a level, or the scale, wrongly where it lies next to a border: of 10 K prompt tokens' keys and values of
+// 8 x 128 some 30 coordinates in 21 M were a whole step off, and what is read back was 5.1e-4 from 64 bits where fp16's own
+// rounding is 2.1e-4.  So a row with a coordinate within kNear of a border, or a scale next to one of fp16's, is encoded
+// again in 64 bits from its cosines and sines on, by the whole wave: some 4 rows in 1000, 2.8e-4, 2 us of 60.  Sixteen
+// rows at a time, a quad a row, it took 256 registers and 26 more at head_dim 256 (one wave a SIMD for two).
+constexpr float kNear = 0x1p-17f;
+
 template <int DT, int D>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     constexpr int C = D / 32, HC = C / 2;
@@ -127,18 +186,12 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     const uint32_t wave = blockIdx.x * 4u + (threadIdx.x >> 6), token = wave / a.waves;
     if (token >= a.rows) return;  // whole wave
     float cs[HC][8], sn[HC][8];
+    if (a.angles) {
 #pragma unroll
-    for (int c = 0; c < HC; ++c) {
-        if (a.angles) {
+        for (int c = 0; c < HC; ++c) {
             const float* const t = a.angles + (size_t)token * D + 32 * c + 8 * q;
             load8f(t, cs[c]);
             load8f(t + D / 2, sn[c]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                cs[c][i] = 1.0f;
-                sn[c][i] = 0.0f;
-            }
         }
     }
     const int32_t slot = a.slots[token];
@@ -187,20 +240,36 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
         big = max(big, dpp_u32<kQuadXor2>(big));
         const bool finite = big < 0x7f800000u;
         const float amax = finite ? __builtin_bit_cast(float, big) : 0.0f;
-        const uint32_t s16 = f32_to_f16_bits(__builtin_fminf(amax / 7.5f, 65504.0f));
+        const float s32 = __builtin_fminf(amax / 7.5f, 65504.0f);
+        const uint32_t s16 = f32_to_f16_bits(s32);
         const float s = f16_bits_to_f32(s16);
         const float inv = (s > 0.0f ? 1.0f / s : 0.0f) * quad_sign(q);  // the transform's sign (nq_rowmath.h)
         uint32_t w[C];
+        float far = 0.0f;  // from the nearest level
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             w[c] = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float y = __builtin_fminf(__builtin_fmaxf(v[c][i] * inv + 8.5f, 0.0f), 15.0f);
-                w[c] |= (uint32_t)y << (4 * i);  // (truncates; what is past 15 is level 15)
+                const float y = v[c][i] * inv, level = __builtin_rintf(y);
+                far = __builtin_fmaxf(far, __builtin_fabsf(y - level));
+                w[c] |= (uint32_t)(int)__builtin_fminf(__builtin_fmaxf(level + 8.0f, 0.0f), 15.0f) << (4 * i);
             }
         }
-        if (stored && role < 2 && want == h) {
+        far = __builtin_fmaxf(far, dpp_f32<kQuadXor1>(far));
+        far = __builtin_fmaxf(far, dpp_f32<kQuadXor2>(far));
+        const bool mine = stored && role < 2 && want == h;
+        const bool near = mine && finite && (far > 0.5f - kNear || f32_to_f16_bits(s32 * (1.0f - 0x1p-21f)) != f32_to_f16_bits(s32 * (1.0f + 0x1p-21f)));
+        for (uint64_t todo = __ballot(near && q == 0); todo; todo &= todo - 1) {
+            const int from = __builtin_ctzll(todo);
+            const uint32_t value = (uint32_t)__builtin_amdgcn_readlane((int)role, from), of = (uint32_t)__builtin_amdgcn_readlane((int)head, from);
+            const size_t to = ((size_t)page * a.kv_heads + of) * a.tokens + off;
+            encode_exactly<DT, D>((value ? a.x[1] : a.x[0]) + token * (value ? a.row[1] : a.row[0]) + of * (value ? a.head[1] : a.head[0]),
+                                  value || !a.angles ? nullptr : a.angles + (size_t)token * D, lane,
+                                  reinterpret_cast<uint32_t*>((value ? a.pool.codes[1] : a.pool.codes[0]) + to * (D / 2)),
+                                  (value ? a.pool.scales[1] : a.pool.scales[0]) + to);
+        }
+        if (mine && !near) {
             const size_t to = ((size_t)page * a.kv_heads + head) * a.tokens + off;
             uint32_t* const codes = reinterpret_cast<uint32_t*>((role ? a.pool.codes[1] : a.pool.codes[0]) + to * (D / 2)) + q;
 #pragma unroll
