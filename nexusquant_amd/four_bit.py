@@ -26,7 +26,7 @@ from . import _lib
 from .hadamard import hadamard_constant
 from .ops import PlanTensor, on_device
 from .page_pool import PagePool
-from .rotary import Rotation, aligned, check_out, same_or_apart
+from .rotary import Rotation, aligned, check_out, empty_as, same_or_apart
 
 _HEAD_DIMS = (64, 128, 256)
 _DTYPES = (torch.float16, torch.bfloat16)
@@ -87,6 +87,11 @@ _MANY, _SOME, _FEW = 0, 1, 2
 # tiles of many 78 (they leave half of the CUs idle); 2048 x 4 rows over 32768 of 8 x 128 1340 and 1204 (what is decoded
 # serves twice the rows).
 _MANY_ROWS = 512
+# Up to so many rows of a sequence are tiles of few, 16 rows each, which end to end take less than one of 128 rows with the rest
+# left idle, and round weights to 22 bits.  us as few and as some: 16 sequences of 4096 tokens of 8 x 128, 20 rows 27.8 and 40.7,
+# 32 29.4 and 44.0, 64 43.8 and 55.6, 96 50.9 and 65.6, 128 68.8 and 73.1; one of 32768, 20 rows 21.4 and 29.8, 96 42.8 and 41.4,
+# 128 49.6 and 44.9; 64 of 8192 of 8 x 64, 96 rows 217 and 261, 128 291 and 268.
+_FEW_ROWS = 96
 _FEW_STEP = 128  # tokens that a workgroup takes at a time
 _STAGE, _LEAST = 64, 256  # of wider tiles, and the least of a chunk
 _AT_ONCE = ({64: 256, 128: 256, 256: 256}, {64: 512, 128: 512, 256: 256})  # workgroups of many and of some rows
@@ -164,14 +169,15 @@ def attention_items(pages: Sequence[int], lengths: Sequence[int], queries: Seque
         first_page += pages[b]
         if n == 0 or q == 0:
             continue
-        per = max(1, wide // group)  # query tokens of a tile
+        most = rows[_FEW] if q * group <= _FEW_ROWS else wide
+        per = max(1, most // group)  # query tokens of a tile
         for i0 in range(0, q, per):
             i1 = min(i0 + per, q)
             end = n - q + i1 if causal else n
             start = max(0, n - q + i0 - window + 1) if window else 0
-            kind = _FEW if (i1 - i0) * group <= rows[_FEW] else _MANY if wide > rows[_SOME] else _SOME
-            for r0 in range(i0 * group, i1 * group, wide):  # (more heads than a tile has rows: several, cut alike)
-                tiles.append((kind, b, i0, i1, r0, min(wide, i1 * group - r0), start, end))
+            kind = _FEW if most == rows[_FEW] or (i1 - i0) * group <= rows[_FEW] else _MANY if wide > rows[_SOME] else _SOME
+            for r0 in range(i0 * group, i1 * group, most):  # (more heads than a tile has rows: several, cut alike)
+                tiles.append((kind, b, i0, i1, r0, min(most, i1 * group - r0), start, end))
     if not tiles:
         return (np.zeros(0, np.int32), np.array(joins, np.int32).reshape(-1)), (0, 0, 0, len(joins), 0, 0)
     t = np.array(tiles, dtype=np.int64)
@@ -316,18 +322,21 @@ class FourBitPagePool(PagePool):
         replays then store into the same slots."""
         self._check_plan(plan, SlotPlan, "append", layer)
         dtype, dev, rows, d = key.dtype, self.device, plan.rows, self.head_dim
-        tensors = [("key", key), ("value", value)] + ([] if query is None else [("query", query)])
-        for name, t in tensors:
-            _lib.require_device(t, name)
-            if t.dim() != 3 or t.shape[0] != rows or t.shape[2] != d or (name != "query" and t.shape[1] != self.num_heads):
+        grad = torch.is_grad_enabled()
+        for name, t in (("key", key), ("value", value), ("query", query)):
+            if t is None and name == "query":
+                continue
+            if t.device != dev:
+                _lib.require_device(t, name)
+                raise ValueError(f"{name} is on {t.device}, the pool on {dev}")
+            shape = t.shape
+            if len(shape) != 3 or shape[0] != rows or shape[2] != d or (shape[1] != self.num_heads and name != "query"):
                 heads = "q_heads" if name == "query" else self.num_heads
-                raise ValueError(f"{name} must be ({rows} tokens, {heads}, {d}), got {tuple(t.shape)}")
+                raise ValueError(f"{name} must be ({rows} tokens, {heads}, {d}), got {tuple(shape)}")
             if t.dtype != dtype or dtype not in _DTYPES:
                 raise ValueError(f"key, value and query must share an fp16 or bf16 dtype, got {t.dtype}")
-            if t.device != dev:
-                raise ValueError(f"{name} is on {t.device}, the pool on {dev}")
-        if torch.is_grad_enabled() and any(t.requires_grad for _, t in tensors):
-            raise NotImplementedError("append has no backward pass; call it under torch.no_grad()")
+            if grad and t.requires_grad:
+                raise NotImplementedError("append has no backward pass; call it under torch.no_grad()")
         if rotation is None:
             if query is not None:
                 raise ValueError("append: a query is rotated along with the keys; without a rotation it is not taken")
@@ -349,7 +358,7 @@ class FourBitPagePool(PagePool):
                         raise ValueError(f"append: page {int(plan.pages[refs > 1][0])} is shared and cannot be written")
                 plan.writable_at = self._changes
             if query is not None and out is None:
-                out = torch.empty(query.shape, dtype=dtype, device=dev)
+                out = empty_as(query)
             if rows == 0:
                 return out
             k, v = aligned(key), aligned(value)
@@ -370,7 +379,8 @@ class FourBitPagePool(PagePool):
         bf16 or fp32.  Rows of slot -1 are zero."""
         self._check_plan(plan, SlotPlan, "read", layer)
         code = _lib.dtype_code(dtype)
-        keys, values = (torch.empty(plan.rows, self.num_heads, self.head_dim, dtype=dtype, device=self.device) for _ in range(2))
+        keys = torch.empty(plan.rows, self.num_heads, self.head_dim, dtype=dtype, device=self.device)
+        values = empty_as(keys)
         if plan.rows:
             with on_device(self.device):
                 st = _lib.load().nq_fourbit_read(self.desc, int(layer), plan.slots.address(), plan.rows, code,
@@ -420,9 +430,9 @@ class FourBitPagePool(PagePool):
         from the whole plan: outputs of one row alone and in a batch agree to roundings.
         A captured graph reads the plan's arrays: keep the plan while it is replayed.  Inference only."""
         self._check_plan(plan, FourBitAttentionPlan, "attend", layer)
-        _lib.require_device(query, "query")
         shape, dtype, dev = query.shape, query.dtype, self.device
         if query.device != dev:
+            _lib.require_device(query, "query")
             raise ValueError(f"query is on {query.device}, the pool on {dev}")
         if len(shape) != 3 or shape[0] < plan.rows or shape[2] != self.head_dim:
             raise ValueError(f"query must be ({plan.rows} rows or more, num_heads, {self.head_dim}), got {tuple(shape)}")
@@ -436,7 +446,7 @@ class FourBitPagePool(PagePool):
         hq = shape[1]
         ints, places, counts, nbytes = plan._work.get(hq) or plan.work(hq)
         if out is None:
-            out = torch.empty(shape, dtype=dtype, device=dev)
+            out = empty_as(query)
             if shape[0] > plan.rows:
                 out[plan.rows:].zero_()
         else:

@@ -122,6 +122,11 @@ def plan_rotation(positions, head_dim: int, base: float = 10000.0, rope_scaling:
     return Rotation(angles=angles, rows=rows, head_dim=head_dim)
 
 
+def empty_as(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape and type (1.3 us; torch.empty given those takes 2.3)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def aligned(t: torch.Tensor) -> torch.Tensor:
     """t with contiguous, 16-byte aligned vectors: itself when they are, any strides of rows and heads."""
     row, head, one = t.stride()
@@ -173,17 +178,20 @@ _PACK = struct.Struct("6i5P8q")
 
 
 def _launch(query, key, rotation: Rotation, inverse: bool, q_out, k_out) -> None:
-    q = None if query is None else aligned(query)
-    k = None if key is None else aligned(key)
-    like = q if q is not None else k
-    none = (0, 0)
-    strides = [none if t is None else t.stride()[:2] for t in (q, k, q_out, k_out)]
+    rows = q_at = qo_at = q_heads = k_at = ko_at = k_heads = 0
+    q_strides = qo_strides = k_strides = ko_strides = (0, 0)
+    if query is not None:
+        q = aligned(query)
+        (rows, q_heads, d), q_at, q_strides, qo_at, qo_strides = q.shape, q.data_ptr(), q.stride()[:2], q_out.data_ptr(), q_out.stride()[:2]
+    if key is not None:
+        k = aligned(key)
+        (rows, k_heads, d), k_at, k_strides, ko_at, ko_strides = k.shape, k.data_ptr(), k.stride()[:2], k_out.data_ptr(), k_out.stride()[:2]
+    like = q_out if query is not None else k_out
     dev = like.device
     with on_device(dev):
         st = _lib.load().nq_rotate(_PACK.pack(
-            like.shape[0], 0 if q is None else q.shape[1], 0 if k is None else k.shape[1], like.shape[2],
-            _lib.dtype_code(like.dtype), int(inverse), *(0 if t is None else t.data_ptr() for t in (q, k, q_out, k_out)),
-            rotation.angles.data_ptr(), *(s for pair in strides for s in pair)), _lib.current_stream_handle(dev))
+            rows, q_heads, k_heads, d, _lib.dtype_code(like.dtype), int(inverse), q_at, k_at, qo_at, ko_at,
+            rotation.angles.data_ptr(), *q_strides, *k_strides, *qo_strides, *ko_strides), _lib.current_stream_handle(dev))
     _lib.check(st, "nq_rotate")
 
 
@@ -196,7 +204,7 @@ class _Rotate(torch.autograd.Function):
         ctx.inverse = inverse
         ctx.set_materialize_grads(False)
         rotation = Rotation(angles=angles, rows=angles.shape[0], head_dim=2 * angles.shape[2])
-        outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (query, key)]
+        outs = [None if t is None else empty_as(t) for t in (query, key)]
         _launch(query, key, rotation, inverse, *outs)
         return tuple(outs)
 
@@ -217,24 +225,27 @@ def rotate(query: torch.Tensor, key: Optional[torch.Tensor], rotation: Rotation,
     fp16, bf16 or fp32, computed in fp32 and rounded once; any strides of rows and heads: slices of one fused projection
     are read in place.  inverse: by the opposite angles.  out: where the results go; (query, key) rotates in place.
     Differentiable (without out)."""
-    tensors = [("query", query)] + ([] if key is None else [("key", key)])
-    shape, dtype, dev = query.shape, query.dtype, query.device
-    for name, t in tensors:
-        _lib.require_device(t, name)
-        if t.dim() != 3 or t.shape[0] != rotation.rows or t.shape[2] != rotation.head_dim:
-            raise ValueError(f"{name} must be [{rotation.rows} rows, heads, {rotation.head_dim}], got {tuple(t.shape)}")
-        if t.dtype not in _DTYPES or t.dtype != dtype:
+    dtype, dev, grad = query.dtype, rotation.device, False
+    for name, t in (("query", query), ("key", key)):
+        if t is None and name == "key":
+            continue
+        if t.device != dev:
+            _lib.require_device(t, name)
+            raise ValueError(f"{name} is on {t.device}, the rotation on {dev}")
+        shape = t.shape
+        if len(shape) != 3 or shape[0] != rotation.rows or shape[2] != rotation.head_dim:
+            raise ValueError(f"{name} must be [{rotation.rows} rows, heads, {rotation.head_dim}], got {tuple(shape)}")
+        if t.dtype != dtype or dtype not in _DTYPES:
             raise ValueError(f"query and key must share an fp16, bf16 or fp32 dtype, got {t.dtype}")
-        if t.device != rotation.device or t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, the rotation on {rotation.device}")
+        grad = grad or t.requires_grad
     if rotation.rows >= 1 << 31:
         raise ValueError(f"{rotation.rows} rows: a call takes less than 2^31")
-    grad = torch.is_grad_enabled() and any(t.requires_grad for _, t in tensors)
+    grad = grad and torch.is_grad_enabled()
     if out is None:
         if grad:
             return _Rotate.apply(query, key, rotation.angles, bool(inverse))
-        q_out = torch.empty(shape, dtype=dtype, device=dev)
-        k_out = None if key is None else torch.empty(key.shape, dtype=dtype, device=dev)
+        q_out = empty_as(query)
+        k_out = None if key is None else empty_as(key)
     else:
         q_out, k_out = out
         if grad or any(t is not None and t.requires_grad and torch.is_grad_enabled() for t in (q_out, k_out)):

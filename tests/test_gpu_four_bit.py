@@ -216,6 +216,29 @@ def test_attention(dtype, heads, group, d, tokens, lens, queries, causal, window
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,group,d,tokens,lens,queries,window", [
+    (2, 8, 256, 8, [70, 100, 1025], [1, 12, 13], 0),      # 96 rows of a sequence and 104
+    (1, 24, 128, 16, [300, 130, 3000], [5, 4, 1], 0),     # a token's heads in two tiles, over several chunks
+    (4, 3, 64, 16, [900, 40], [32, 33], 0),
+    (1, 96, 128, 16, [5000, 70], [1, 1], 0),
+    (2, 4, 128, 16, [2000, 900], [24, 25], 300),
+])
+def test_rows_up_to_and_past_several_small_tiles(dtype, heads, group, d, tokens, lens, queries, window):
+    T = TYPES[dtype]
+    pool = FourBitPagePool(sum(-(-n // tokens) for n in lens) + 3, heads, tokens, d)
+    fill(pool, d + heads)
+    tables = sequences(pool, lens, 5)
+    q = torch.randn(sum(queries), heads * group, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(12)).to(T)
+    plan = pool.plan_attention(tables, lens, queries, sliding_window=window or None)
+    check_attention(pool, tables, lens, queries, q, pool.attend(plan, q), T, True, window)
+    for b, (n, m) in enumerate(zip(lens, queries)):  # up to 96 rows weights and queries are not rounded to 11 bits, alone or in a batch
+        if m * group <= 96:
+            alone = pool.plan_attention([tables[b]], [n], [m], sliding_window=window or None)
+            rows = q[sum(queries[:b]):sum(queries[:b + 1])]
+            check_attention(pool, [tables[b]], [n], [m], rows, pool.attend(alone, rows), T, True, window, few=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("queries", [1, 4, 40])
 def test_what_some_queries_do_not_see_may_be_anything(dtype, queries):
     """A NaN or infinite scale at a sequence's last token reaches the last query alone."""
