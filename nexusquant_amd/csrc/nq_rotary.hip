@@ -77,60 +77,95 @@ struct RotateArgs {
     uint8_t* y[2];
     int64_t x_row[2], x_head[2], y_row[2], y_head[2];  // strides, bytes
     const float* angles;    // [rows, 2, d / 2]
-    uint32_t rows, heads[2], parts;
+    uint32_t rows, heads[2], parts;  // waves that share a row's heads
     float sign;             // -1: the inverse
+    uint32_t stream;
 };
 
-template <int DT>
+// STREAM: past the caches (kStreamBytes, nq_rowmath.h).
+template <int DT, bool STREAM>
 __device__ __forceinline__ void store8(uint8_t* p, const float (&x)[8]) {
+    NQ_GLOBAL u32x4* const to = (NQ_GLOBAL u32x4*)(uint64_t)p;
+    auto put = [&](int i, u32x4 v) {
+        if constexpr (STREAM) __builtin_nontemporal_store(v, to + i);
+        else to[i] = v;
+    };
     if constexpr (DT == NQ_F32) {
-        reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-        reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            u32x4 v;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = __builtin_bit_cast(uint32_t, x[4 * i + k]);
+            put(i, v);
+        }
     } else {
         typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
         typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
         typedef float f32x2 __attribute__((ext_vector_type(2)));
-        uint32_t w[4];
+        u32x4 w;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const f32x2 v = {x[2 * k], x[2 * k + 1]};
             if constexpr (DT == NQ_F16) w[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
             else w[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
         }
-        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        put(0, w);
     }
 }
 
-// D / 16 lanes a row, eight pairs a lane: its cosines and sines stay in registers for the heads of the block's part.
+// A wave takes a token's heads h = first, first + step, .., D / 16 lanes a head and eight pairs a lane, 1024 / D heads one after
+// another in memory at a time: the angles stay in registers, and N steps' inputs are read before their outputs are written.
+// 16384 tokens of 32 + 8 heads of 128 (336 MB) with their angles: a wave on eight tokens of one head at a time 83 us, on eight
+// heads of a token 71, with stores past the caches 58, reading ahead 57 (50 and 6.7 for the angles: 6.7 TB/s, the inputs being
+// in the last-level cache still); 8188 tokens in fp32, forward and back (671 MB), 139 to 146, of which it keeps nothing.
+template <int DT, int D, bool STREAM, typename Where>
+__device__ __forceinline__ void rotate_heads(const float* angles, float sign, uint32_t first, uint32_t step, uint32_t heads, int at, Where where) {
+    constexpr int SIZE = DT == NQ_F32 ? 4 : 2, N = DT == NQ_F32 ? 2 : 4;
+    float c[8], s[8];
+    load8f(angles + 8 * at, c);
+    load8f(angles + D / 2 + 8 * at, s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] *= sign;
+    for (uint32_t h = first; h < heads; h += N * step) {
+        float lo[N][8], hi[N][8];
+        uint8_t* to[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const uint8_t* from;
+            where(min(h + n * step, heads - 1u), from, to[n]);
+            load8<DT>(from + 8 * SIZE * at, 0, lo[n]);
+            load8<DT>(from + 8 * SIZE * at, D / 2, hi[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            if (h + n * step >= heads) continue;
+            float u[8], v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                u[i] = __builtin_fmaf(lo[n][i], c[i], -(hi[n][i] * s[i]));
+                v[i] = __builtin_fmaf(hi[n][i], c[i], lo[n][i] * s[i]);
+            }
+            store8<DT, STREAM>(to[n] + 8 * SIZE * at, u);
+            store8<DT, STREAM>(to[n] + (8 * at + D / 2) * SIZE, v);
+        }
+    }
+}
+
 template <int DT, int D>
 __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
-    constexpr int LANES = D / 16, ROWS = 256 / LANES, SIZE = DT == NQ_F32 ? 4 : 2, UNROLL = DT == NQ_F32 ? 2 : 4;
-    const uint32_t row = (blockIdx.x / a.parts) * ROWS + threadIdx.x / LANES, part = blockIdx.x % a.parts, at = threadIdx.x % LANES;
-    if (row >= a.rows) return;
-    float c[8], s[8];
-    const float* const t = a.angles + (size_t)row * D + 8 * at;
-    load8f(t, c);
-    load8f(t + D / 2, s);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] *= a.sign;
-    const uint32_t n = a.heads[0] + a.heads[1];
-#pragma unroll UNROLL
-    for (uint32_t h = part; h < n; h += a.parts) {
+    constexpr int LANES = D / 16, HEADS = 64 / LANES;
+    const uint32_t wave = blockIdx.x * 4u + (threadIdx.x >> 6), row = wave / a.parts, lane = threadIdx.x & 63u;
+    if (row >= a.rows) return;  // whole wave
+    auto where = [&](uint32_t h, const uint8_t*& from, uint8_t*& to) {
         const bool key = h >= a.heads[0];
         const uint32_t head = key ? h - a.heads[0] : h;
-        const uint8_t* const x = a.x[key] + row * a.x_row[key] + head * a.x_head[key] + 8 * SIZE * at;
-        uint8_t* const y = a.y[key] + row * a.y_row[key] + head * a.y_head[key] + 8 * SIZE * at;
-        float lo[8], hi[8], u[8], v[8];
-        load8<DT>(x, 0, lo);
-        load8<DT>(x, D / 2, hi);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            u[i] = __builtin_fmaf(lo[i], c[i], -(hi[i] * s[i]));
-            v[i] = __builtin_fmaf(hi[i], c[i], lo[i] * s[i]);
-        }
-        store8<DT>(y, u);
-        store8<DT>(y + D / 2 * SIZE, v);
-    }
+        from = (key ? a.x[1] : a.x[0]) + row * (key ? a.x_row[1] : a.x_row[0]) + head * (key ? a.x_head[1] : a.x_head[0]);
+        to = (key ? a.y[1] : a.y[0]) + row * (key ? a.y_row[1] : a.y_row[0]) + head * (key ? a.y_head[1] : a.y_head[0]);
+    };
+    const float* const angles = a.angles + (size_t)row * D;
+    const uint32_t first = wave % a.parts * HEADS + lane / LANES, heads = a.heads[0] + a.heads[1];
+    if (a.stream) rotate_heads<DT, D, true>(angles, a.sign, first, a.parts * HEADS, heads, lane % LANES, where);
+    else rotate_heads<DT, D, false>(angles, a.sign, first, a.parts * HEADS, heads, lane % LANES, where);
 }
 
 // ----------------------------------------------------------------- append ----
@@ -144,7 +179,8 @@ struct AppendArgs {
     const int32_t* slots;               // [rows]
     FourBitRows pool;
     uint32_t rows, q_heads, kv_heads;
-    uint32_t batches, waves;            // of 16 heads a token; waves that share a token's
+    uint32_t batches, waves;            // of 16 keys and values of a token; waves that share a token's heads
+    uint32_t stream;
     uint32_t tokens, slot_end;
     FastDiv by_tokens;
     float hscale;
@@ -201,8 +237,7 @@ __device__ __forceinline__ void encode_exactly(const uint8_t* from, const float*
     if (lane == 0) *scale = (uint16_t)s16;
 }
 
-// A wave takes a token, and its heads sixteen at a time, a quad a head (nq_rowmath.h): keys, then values, then queries.
-// The token's cosines and sines stay in registers.
+// A wave takes a token: its keys and values sixteen at a time, a quad a head (nq_rowmath.h), then its queries.
 //
 // 32 bits decide a level, or the scale, wrongly where it lies next to a border: of 10 K prompt tokens' keys and values of
 // 8 x 128 some 30 coordinates in 21 M were a whole step off, and what is read back was 5.1e-4 from 64 bits where fp16's own
@@ -229,18 +264,15 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     const int32_t slot = a.slots[token];
     const bool stored = slot >= 0 && (uint32_t)slot < a.slot_end;
     const uint32_t page = stored ? div((uint32_t)slot, a.by_tokens) : 0u, off = stored ? (uint32_t)slot - page * a.tokens : 0u;
-    const uint32_t total = 2u * a.kv_heads + a.q_heads;
-    for (uint32_t batch = wave % a.waves; batch < a.batches; batch += a.waves) {
-        const uint32_t want = 16u * batch + ((uint32_t)lane >> 2), h = min(want, total - 1u);
-        const uint32_t role = h < a.kv_heads ? 0u : h < 2u * a.kv_heads ? 1u : 2u;
-        const uint32_t head = h - role * a.kv_heads;
-        const int64_t row = role == 0 ? a.row[0] : role == 1 ? a.row[1] : a.row[2], step = role == 0 ? a.head[0] : role == 1 ? a.head[1] : a.head[2];
-        const uint8_t* const base = role == 0 ? a.x[0] : role == 1 ? a.x[1] : a.x[2];
-        const uint8_t* const x = base + token * row + head * step;
+    uint32_t batch = wave % a.waves;
+    for (; batch < a.batches; batch += a.waves) {
+        const uint32_t want = 16u * batch + ((uint32_t)lane >> 2), h = min(want, 2u * a.kv_heads - 1u);
+        const uint32_t role = h < a.kv_heads ? 0u : 1u, head = h - role * a.kv_heads;
+        const uint8_t* const x = (role ? a.x[1] : a.x[0]) + token * (role ? a.row[1] : a.row[0]) + head * (role ? a.head[1] : a.head[0]);
         float v[C][8];
 #pragma unroll
         for (int c = 0; c < C; ++c) load8<DT>(x, 32 * c + 8 * q, v[c]);
-        if (role != 1 && a.angles) {
+        if (role == 0 && a.angles) {
 #pragma unroll
             for (int c = 0; c < HC; ++c)
 #pragma unroll
@@ -250,14 +282,6 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
                     v[c + HC][i] = __builtin_fmaf(hi, cs[c][i], lo * sn[c][i]);
                 }
         }
-        if (role == 2) {
-            if (want == h) {
-                uint8_t* const o = a.out + token * a.out_row + head * a.out_head;
-#pragma unroll
-                for (int c = 0; c < C; ++c) store8<DT>(o + 2 * (32 * c + 8 * q), v[c]);
-            }
-        }
-        if (16u * batch >= 2u * a.kv_heads) continue;  // whole wave: queries alone
         fwht_row<C>(v, q);
         // the largest |t| as an integer: infinities and NaNs are larger than any number
         uint32_t big = 0;
@@ -290,7 +314,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
         }
         far = __builtin_fmaxf(far, dpp_f32<kQuadXor1>(far));
         far = __builtin_fmaxf(far, dpp_f32<kQuadXor2>(far));
-        const bool mine = stored && role < 2 && want == h;
+        const bool mine = stored && want == h;
         const bool near = mine && finite && (far > 0.5f - kNear || f32_to_f16_bits(s32 * (1.0f - 0x1p-21f)) != f32_to_f16_bits(s32 * (1.0f + 0x1p-21f)));
         for (uint64_t todo = __ballot(near && q == 0); todo; todo &= todo - 1) {
             const int from = __builtin_ctzll(todo);
@@ -309,6 +333,16 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
             if (q == 0) (role ? a.pool.scales[1] : a.pool.scales[0])[to] = finite ? (uint16_t)s16 : (uint16_t)0x7e00u;
         }
     }
+    if (a.q_heads == 0) return;
+    constexpr int LANES = D / 16, HEADS = 64 / LANES;
+    auto where = [&](uint32_t head, const uint8_t*& from, uint8_t*& to) {
+        from = a.x[2] + token * a.row[2] + head * a.head[2];
+        to = a.out + token * a.out_row + head * a.out_head;
+    };
+    const float* const angles = a.angles + (size_t)token * D;
+    const uint32_t first = (batch - a.batches) * HEADS + (uint32_t)lane / LANES;
+    if (a.stream) rotate_heads<DT, D, true>(angles, 1.0f, first, a.waves * HEADS, a.q_heads, lane % LANES, where);
+    else rotate_heads<DT, D, false>(angles, 1.0f, first, a.waves * HEADS, a.q_heads, lane % LANES, where);
 }
 
 // ------------------------------------------------------------------- read ----
@@ -317,14 +351,14 @@ struct ReadArgs {
     uint8_t* out[2];        // [rows, kv_heads, d]
     const int32_t* slots;
     FourBitRows pool;
-    uint32_t rows, kv_heads, tokens, slot_end;
+    uint32_t rows, kv_heads, tokens, slot_end, stream;
     FastDiv by_tokens, by_heads;
     float hscale;
 };
 
 // A quad a row and role; sums of n - 8 are whole numbers of at most 2048, so fp16 holds them exactly, and each coordinate is rounded by its scale and by its type.
-template <int DT, int D>
-__global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
+template <int DT, int D, bool STREAM>
+__device__ __forceinline__ void read_rows(const ReadArgs& a) {
     constexpr int C = D / 32, SIZE = DT == NQ_F32 ? 4 : 2;
     const int q = threadIdx.x & 3;
     const uint32_t u = blockIdx.x * 64u + (threadIdx.x >> 2), n = a.rows * a.kv_heads, r = min(u, n - 1u);
@@ -360,9 +394,15 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
                 x[2 * k] = stored ? (float)h[c][k].x * f : 0.0f;
                 x[2 * k + 1] = stored ? (float)h[c][k].y * f : 0.0f;
             }
-            store8<DT>(o + SIZE * (32 * c + 8 * q), x);
+            store8<DT, STREAM>(o + SIZE * (32 * c + 8 * q), x);
         }
     }
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
+    if (a.stream) read_rows<DT, D, true>(a);
+    else read_rows<DT, D, false>(a);
 }
 
 int check_fourbit_pool(const nq_pool* p, int32_t layer, const char* who) {
@@ -464,11 +504,12 @@ extern "C" int nq_rotate(const nq_rotate_desc* d, void* stream) {
     a.heads[0] = (uint32_t)d->q_heads;
     a.heads[1] = (uint32_t)d->k_heads;
     a.sign = d->inverse ? -1.0f : 1.0f;
-    const uint32_t per = 256u / (uint32_t)(d->head_dim / 16);
-    const uint64_t blocks = ((uint64_t)d->rows + per - 1) / per;
-    a.parts = share(blocks, a.heads[0] + a.heads[1]);
-    NQ_CHECK_ARG(blocks * a.parts <= max_blocks(256), "nq_rotate: grid too large");
-    const dim3 grid((uint32_t)(blocks * a.parts));
+    const uint32_t per = 1024u / (uint32_t)d->head_dim;
+    a.parts = share(((uint64_t)d->rows + 3) / 4, (a.heads[0] + a.heads[1] + per - 1) / per);
+    a.stream = (uint64_t)d->rows * (a.heads[0] + (uint64_t)a.heads[1]) * d->head_dim * size >= kStreamBytes;
+    const uint64_t blocks = ((uint64_t)d->rows * a.parts + 3) / 4;
+    NQ_CHECK_ARG(blocks <= max_blocks(256) && (uint64_t)d->rows * a.parts < (1ull << 32), "nq_rotate: grid too large");
+    const dim3 grid((uint32_t)blocks);
     hipStream_t s = (hipStream_t)stream;
     if (d->dtype == NQ_F16) NQ_BY_DIM(rotate_kernel, NQ_F16, d->head_dim, grid, dim3(256), 0, s, a)
     else if (d->dtype == NQ_BF16) NQ_BY_DIM(rotate_kernel, NQ_BF16, d->head_dim, grid, dim3(256), 0, s, a)
@@ -512,8 +553,10 @@ extern "C" int nq_fourbit_append(const nq_fourbit_append_desc* d, void* stream) 
     a.q_heads = (uint32_t)d->q_heads;
     a.kv_heads = (uint32_t)p->heads;
     NQ_CHECK_ARG(2ll * p->heads + d->q_heads < (1ll << 30), "nq_fourbit_append: too many heads");
-    a.batches = (2u * a.kv_heads + a.q_heads + 15u) / 16u;
-    a.waves = share(((uint64_t)d->rows + 3) / 4, a.batches);
+    a.batches = (2u * a.kv_heads + 15u) / 16u;
+    const uint32_t per = 1024u / (uint32_t)dim;  // queries at a time
+    a.waves = share(((uint64_t)d->rows + 3) / 4, a.batches + (a.q_heads + per - 1u) / per);
+    a.stream = (uint64_t)d->rows * a.q_heads * dim * 2 >= kStreamBytes;
     a.tokens = (uint32_t)p->tokens;
     a.slot_end = (uint32_t)p->pages * (uint32_t)p->tokens;
     a.by_tokens = fast_div(a.tokens);
@@ -549,6 +592,7 @@ extern "C" int nq_fourbit_read(const nq_pool* p, int32_t layer, const int32_t* s
     a.by_tokens = fast_div(a.tokens);
     a.by_heads = fast_div(a.kv_heads);
     a.hscale = hadamard_scale;
+    a.stream = 2ull * n * p->heads * p->head_dim * (dtype == NQ_F32 ? 4 : 2) >= kStreamBytes;
     const uint64_t blocks = ((uint64_t)n * p->heads + 63) / 64;
     NQ_CHECK_ARG(blocks <= max_blocks(256), "nq_fourbit_read: grid too large");
     const dim3 grid((uint32_t)blocks);
