@@ -227,10 +227,10 @@ __device__ __forceinline__ void encode_exactly(const uint8_t* from, const float*
     for (int o = 1; o < 64; o <<= 1) most = fmax(most, __shfl_xor(most, o, 64));
     const double h = D == 64 ? 0.125 : D == 256 ? 0.0625 : 0.08838834764831844;  // 1 / sqrt(D)
     const uint32_t s16 = f32_to_f16_bits((float)fmin(most * h / 7.5, 65504.0));  // by way of fp32, as where 32 bits suffice
-    const double inv = s16 ? h / (double)f16_bits_to_f32(s16) : 0.0;
+    const double scale64 = s16 ? (double)f16_bits_to_f32(s16) : 1.0;
     uint32_t w = 0;
 #pragma unroll
-    for (int k = 0; k < V; ++k) w |= (uint32_t)fmin(fmax(floor(x[k] * inv + 8.5), 0.0), 15.0) << (4 * ((V * lane + k) & 7));
+    for (int k = 0; k < V; ++k) w |= (uint32_t)fmin(fmax(floor(x[k] * h / scale64 + 8.5), 0.0), 15.0) << (4 * ((V * lane + k) & 7));
 #pragma unroll
     for (int o = 1; o < 8 / V; o <<= 1) w |= (uint32_t)__shfl_xor((int)w, o, 64);
     if ((V * lane & 7) == 0) codes[V * lane >> 3] = w;

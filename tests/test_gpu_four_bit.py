@@ -105,6 +105,30 @@ def test_append_and_read(dtype, d, heads, hq, tokens, rows, axes):
             assert (y.cpu()[[i for i, p in enumerate(slots) if p < 0]] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_levels_next_to_a_border_are_decided_in_64_bits(dtype, d):
+    """Values (nothing is rotated) are stored as 64 bits have them, bit for bit: sums of few-bit numbers, whose transforms lie
+    on borders at d = 64 and 256, and random rows, whose sums in 32 bits are off by some 2^-24 of them (independent roundings
+    in 6 to 8 stages; six times their spread is 2^-21 of the largest, 2^-18 of a step, and closer than 2^-17 is done again)."""
+    T = TYPES[dtype]
+    pool = FourBitPagePool(70, 2, 16, d)
+    pages = pool.allocate(70)
+    slots = [p * 16 + i for p in pages for i in range(16)]
+    g = torch.Generator().manual_seed(d)
+    x = torch.randn(len(slots), 2, d, generator=g)
+    x[:300] = torch.randint(-2, 3, (300, 2, d), generator=g).float()
+    x[300] = 1.0
+    x[301] = -0.75
+    x[302, :, 1:] = 0.0
+    x = x.to(T)
+    pool.append(pool.plan_slots(slots), torch.zeros_like(x).cuda(), x.cuda())
+    codes, scales = ref.encode(x)
+    at = torch.tensor(slots)
+    assert torch.equal(pool.value_scales[0].cpu()[at // 16, :, at % 16], scales)
+    assert torch.equal(pool.value_codes[0].cpu()[at // 16, :, at % 16], codes)
+
+
 def test_rows_that_are_zero_tiny_huge_or_not_finite():
     d = 128
     pool = FourBitPagePool(2, 1, 16, d)
