@@ -177,7 +177,7 @@ def check_out(out: torch.Tensor, like: torch.Tensor, name: str, align: int = 16)
 _PACK = struct.Struct("6i5P8q")
 
 
-def _launch(query, key, rotation: Rotation, inverse: bool, q_out, k_out) -> None:
+def _launch(query, key, angles: torch.Tensor, inverse: bool, q_out, k_out) -> None:
     rows = q_at = qo_at = q_heads = k_at = ko_at = k_heads = 0
     q_strides = qo_strides = k_strides = ko_strides = (0, 0)
     if query is not None:
@@ -191,8 +191,14 @@ def _launch(query, key, rotation: Rotation, inverse: bool, q_out, k_out) -> None
     with on_device(dev):
         st = _lib.load().nq_rotate(_PACK.pack(
             rows, q_heads, k_heads, d, _lib.dtype_code(like.dtype), int(inverse), q_at, k_at, qo_at, ko_at,
-            rotation.angles.data_ptr(), *q_strides, *k_strides, *qo_strides, *ko_strides), _lib.current_stream_handle(dev))
+            angles.data_ptr(), *q_strides, *k_strides, *qo_strides, *ko_strides), _lib.current_stream_handle(dev))
     _lib.check(st, "nq_rotate")
+
+
+def _rotated(query, key, angles: torch.Tensor, inverse: bool):
+    q_out, k_out = (None if t is None else empty_as(t) for t in (query, key))
+    _launch(query, key, angles, inverse, q_out, k_out)
+    return q_out, k_out
 
 
 class _Rotate(torch.autograd.Function):
@@ -203,17 +209,15 @@ class _Rotate(torch.autograd.Function):
         ctx.save_for_backward(angles)
         ctx.inverse = inverse
         ctx.set_materialize_grads(False)
-        rotation = Rotation(angles=angles, rows=angles.shape[0], head_dim=2 * angles.shape[2])
-        outs = [None if t is None else empty_as(t) for t in (query, key)]
-        _launch(query, key, rotation, inverse, *outs)
-        return tuple(outs)
+        return _rotated(query, key, angles, inverse)
 
     @staticmethod
     def backward(ctx, grad_query, grad_key):
         if grad_query is None and grad_key is None:
             return None, None, None, None
         angles, = ctx.saved_tensors
-        return (*_Rotate.apply(grad_query, grad_key, angles, not ctx.inverse), None, None)
+        again = _Rotate.apply if torch.is_grad_enabled() else _rotated  # (a gradient of the gradient is asked for, or not)
+        return (*again(grad_query, grad_key, angles, not ctx.inverse), None, None)
 
 
 def rotate(query: torch.Tensor, key: Optional[torch.Tensor], rotation: Rotation, inverse: bool = False,
@@ -260,5 +264,5 @@ def rotate(query: torch.Tensor, key: Optional[torch.Tensor], rotation: Rotation,
                 (k_out is not None and q_out.numel() and q_out.data_ptr() == k_out.data_ptr()) or \
                 (key is not None and query.numel() and (q_out.data_ptr() == key.data_ptr() or k_out.data_ptr() == query.data_ptr())):
             raise ValueError("out may be query and key themselves, and must not overlap them or each other otherwise")
-    _launch(query, key, rotation, bool(inverse), q_out, k_out)
+    _launch(query, key, rotation.angles, bool(inverse), q_out, k_out)
     return q_out, k_out
