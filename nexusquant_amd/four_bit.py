@@ -16,6 +16,7 @@ gives up is re-rotation: compact keeps positions.
 
 from __future__ import annotations
 
+import heapq
 import struct
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -93,6 +94,7 @@ _MANY_ROWS = 512
 # 128 49.6 and 44.9; 64 of 8192 of 8 x 64, 96 rows 217 and 261, 128 291 and 268.
 _FEW_ROWS = 96
 _FEW_STEP = 128  # tokens that a workgroup takes at a time
+_ITEM_INTS = 12
 _STAGE, _LEAST = 64, 256  # of wider tiles, and the least of a chunk
 _AT_ONCE = ({64: 256, 128: 256, 256: 256}, {64: 512, 128: 512, 256: 256})  # workgroups of many and of some rows
 _STAGE_US = {64: 1.8, 128: 2.3, 256: 3.7}
@@ -126,25 +128,58 @@ def _few_chunks(spans: np.ndarray, heads: int, head_dim: int):
     return _even(spans, lo * _FEW_STEP, _FEW_STEP)
 
 
+def _last_end(stages: np.ndarray, places: int) -> float:
+    """When the last of these ends, each begun in turn on the place that is free first."""
+    if len(stages) <= places:
+        return float(stages.max())
+    if len(stages) > 16 * places:
+        return float(stages.sum()) / places + float(stages[-1])
+    ends = stages[:places].tolist()
+    heapq.heapify(ends)
+    for n in stages[places:].tolist():
+        heapq.heapreplace(ends, ends[0] + n)
+    return max(ends)
+
+
 def _wide_chunks(spans: np.ndarray, rows: np.ndarray, heads: int, head_dim: int, at_once: int):
-    """Chunks of many or some rows, by what the launch would take: where all workgroups run at once the longest, else their
-    share of the work and half a chunk until the last has ended; and the sums that are joined."""
+    """Chunks of many or some rows: (chunks, tokens of a chunk) of each span, by what the launch and the sums that are joined
+    would take, the longest chunks begun first.
+
+    Either all chunks of a span are alike, or a span is cut at a length that is the CUs' share or somewhat more, and its rest
+    fills a place where a short span has ended.  us, alike and cut so: 4 sequences of 512 query tokens or fewer over up to
+    16384 of 8 x 128, 313 and 278; 6 of 256 over up to 20000, 310 and 264; 5 of 300 over up to 12000 of 4 x 256, 351 and 342.
+    (Expected: 323 and 275, with 5 us and 3.5 TB/s for the join.  A twentieth on top keeps whole what would
+    gain as little: 2048 query tokens of 32768 of 8 x 64 take 851 whole, 904 cut.)"""
+    places = max(1, at_once // heads)  # (a kv head's chunks run beside the other heads')
+    share = float(spans.sum()) / places
     longest = int(spans.max())
-    best = float("inf")
-    for cut in (1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 32, 48, 64, 128):
-        length = max(_LEAST, -(-longest // (cut * _STAGE)) * _STAGE)
-        chunks, each = _even(spans, length, _STAGE)
-        n = heads * int(chunks.sum())
-        stages = heads * float(spans.sum()) / _STAGE + n * _START_STAGES
-        most = float(np.minimum(spans, each).max()) / _STAGE
-        us = _STAGE_US[head_dim] * (most + _START_STAGES if n <= at_once else stages / at_once + most / 2)
+    lengths = {(False, -(-longest // (cut * _STAGE))) for cut in (1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64, 128)}
+    lengths |= {(True, -(-int(share * f) // _STAGE)) for f in (0.52, 0.56, 0.62, 1.0, 1.04, 1.08, 1.12, 1.2)}
+    tries = []
+    for cut_off, stages in lengths:
+        length = max(_LEAST, stages * _STAGE)
+        if cut_off:
+            chunks, each = -(-spans // length), np.minimum(spans, length)
+        else:
+            chunks, each = _even(spans, length, _STAGE)
+        n = int(chunks.sum())
         split = chunks > 1
+        most = float(each.max()) / _STAGE + _START_STAGES
+        total = float(spans.sum()) / _STAGE + n * _START_STAGES
+        join = 0.0
         if split.any():
-            us += 5.0 + heads * head_dim * 8.0 * float((rows * chunks)[split].sum()) / 3.5e6
+            join = 0.05 * _STAGE_US[head_dim] * total / places + 5.0 + heads * head_dim * 8.0 * float((rows * chunks)[split].sum()) / 3.5e6
+        tries.append((_STAGE_US[head_dim] * max(most, total / places) + join, n, join, chunks, each))
+    tries.sort(key=lambda x: x[:2])
+    best = float("inf")
+    for least, n, join, chunks, each in tries:
+        if least >= best:
+            break
+        stages = np.repeat(each, chunks)
+        stages[np.cumsum(chunks) - 1] = spans - (chunks - 1) * each
+        us = _STAGE_US[head_dim] * _last_end(-np.sort(-stages) / _STAGE + _START_STAGES, places) + join
         if us < best:
             best, found = us, (chunks, each)
-        if length == _LEAST:
-            break
     return found
 
 
@@ -209,7 +244,10 @@ def attention_items(pages: Sequence[int], lengths: Sequence[int], queries: Seque
     if slots >= 1 << 31:
         raise ValueError("too many partial sums: split the queries over several plans")
     n_items = [int(chunks[kind == k].sum()) for k in range(3)]
-    return ((np.array(items, np.int32).reshape(-1), np.array(joins, np.int32).reshape(-1)),
+    items = np.array(items, np.int32).reshape(-1, _ITEM_INTS)
+    wide_items = n_items[_MANY] + n_items[_SOME]  # the longest first
+    items[:wide_items] = items[:wide_items][np.argsort(-items[:wide_items, 2], kind="stable")]
+    return ((items.reshape(-1), np.array(joins, np.int32).reshape(-1)),
             (*n_items, len(joins), slots, int(chunks.max())))
 
 
