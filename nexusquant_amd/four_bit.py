@@ -112,12 +112,11 @@ def _even(spans: np.ndarray, most: int, step: int):
 def _few_chunks(spans: np.ndarray, heads: int, head_dim: int):
     """Chunks of few rows, of the least length with which the launch is so many workgroups.
 
-    1024 run at once (at head_dim 256 512).  With more than that a ragged batch ends evenly, with fewer there is less to
-    join, or nothing, where a chunk has all of a sequence.  us with 512, 1024 and 2048: 64 rows up to 8192 tokens of 8 x 128
-    86, 80, 77; one row of 131072 34, 33, 37; 8 rows of 4096 15.3, 17.3, 20.8; 24 rows up to 1500 of 20 x 64 13.0, 16.4,
-    18.2; 32 rows up to 8192 of 4 x 256 33, 38, 39."""
+    1024 run at once (at head_dim 256 512); with fewer there is less to join, or nothing, where a chunk has all of a sequence.
+    us with 512, 1024 and 2048: 64 rows up to 8192 tokens of 8 x 128 86, 71, 70; 16 rows up to 30000 64, 61, 63; one row of
+    131072 34, 34, 39; 24 rows up to 1500 of 20 x 64 13.4, 15.8, 17.9; 32 rows up to 8192 of 4 x 256 32, 37, 39."""
     work = heads * int(spans.sum()) * head_dim // 128
-    workgroups = 2048 if work >= 2048 * 1024 else 1024 if work >= 1024 * 512 and head_dim < 256 else 512
+    workgroups = 1024 if work >= 1024 * 512 and head_dim < 256 else 512
     lo, hi = 1, -(-int(spans.max()) // _FEW_STEP)
     while lo < hi:
         mid = (lo + hi) // 2
@@ -245,8 +244,8 @@ def attention_items(pages: Sequence[int], lengths: Sequence[int], queries: Seque
         raise ValueError("too many partial sums: split the queries over several plans")
     n_items = [int(chunks[kind == k].sum()) for k in range(3)]
     items = np.array(items, np.int32).reshape(-1, _ITEM_INTS)
-    wide_items = n_items[_MANY] + n_items[_SOME]  # the longest first
-    items[:wide_items] = items[:wide_items][np.argsort(-items[:wide_items, 2], kind="stable")]
+    # the longest of a kind first (64 rows up to 8192 tokens 77 to 72 us)
+    items = items[np.lexsort((-items[:, 2], np.repeat(np.arange(3), n_items)))]
     return ((items.reshape(-1), np.array(joins, np.int32).reshape(-1)),
             (*n_items, len(joins), slots, int(chunks.max())))
 
