@@ -755,10 +755,11 @@ int nq_rotate(const nq_rotate_desc* desc, void* stream);
 
 /*
  * A pool whose pages hold 4 bits a coordinate is an nq_pool with reserved 4,
- * codes of head_dim / 2 bytes a row (uint8) and positions NULL.  A row x of d coordinates is held as t = H x, H the orthonormal
- * Walsh-Hadamard matrix: scale s = fp16(max |t| / 7.5) (at most 65504; NaN
- * where t is not finite) and n = clamp(floor(t / s + 8.5), 0, 15), coordinate i
- * in nibble i % 2 of byte i / 2.  It stands for H ((n - 8) s).
+ * codes of head_dim / 2 bytes a row (uint8) and positions NULL.  A row x of d
+ * coordinates is held as t = H x, H the orthonormal Walsh-Hadamard matrix:
+ * scale s = fp16(max |t| / 7.5) (at most 65504; NaN where t is not finite) and
+ * n = clamp(floor(t / s + 8.5), 0, 15), coordinate i in nibble i % 2 of byte
+ * i / 2.  It stands for H ((n - 8) s).
  * nq_pool_copy_pages and nq_pool_compact (renumber 0) take such pools.
  *
  * nq_fourbit_append encodes tokens into their slots of a layer: keys [rows,

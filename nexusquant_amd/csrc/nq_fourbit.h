@@ -1,11 +1,11 @@
 // A cache held in 4 bits: what its kernels share.
 //
 // A token's vector x of one head, d coordinates, is held as its Walsh-Hadamard transform t = H x (H orthonormal) in 16
-// levels: s = fp16(max |t| / 7.5), n = clamp(floor(t / s + 8.5), 0, 15); it stands for H ((n - 8) s).  All 16 levels serve,
-// -8 .. 7, and no coordinate is off by more than s / 2: the largest, 7.5 s, is held as 7 s or -7 s.  Zero is a level (with
-// odd halves for levels a vector whose transform has one coordinate would get the others' halves on top of it).  The 8-bit
-// pages' lattice in 4 bits a coordinate would lower the squared error by 0.65 dB, and cost a coset to be found out for each
-// 8 nibbles.
+// levels: s = fp16(max |t| / 7.5), n = clamp(floor(t / s + 8.5), 0, 15); it stands for H ((n - 8) s).  No coordinate is off by
+// more than s / 2 (and what fp16 takes from s: 2^-11 of the largest, which is 7.5 s and held as 7 s or -7 s; -8 s stands only
+// where fp16 rounded s down).  Zero is a level: with odd halves for levels a vector whose transform has one coordinate would
+// get the others' halves on top of it.  The 8-bit pages' lattice in 4 bits a coordinate would lower the squared error by 0.65
+// dB, and cost a coset to be found out for each 8 nibbles.
 // Coordinate i of a row is nibble i % 2 of byte i / 2.  Keys are transformed after their rotation, so a product with a
 // query needs neither: q . x = s (H q) . (n - 8).
 //

@@ -3,13 +3,14 @@
 //
 // With q~ = H q, a token's codes n and scales s:
 //   logit = scale * s_k sum q~ (n - 8)         out = H sum p s_v (n - 8)
-// so nothing is undone a token: codes go to fp16 (exactly) and into the matrix cores, the transform is applied to a query
-// before and to its output after.
+// so nothing is undone a token: keys' codes go into int8 products with the query's two digits, values' into fp16 products with
+// the weights, both exactly, and the transform is applied to a query before and to its output after.
 //
-// The host cuts each sequence's queries into tiles of rows (a row: a query token and one of the kv head's query heads)
-// and its tokens into chunks.  A workgroup takes a tile, a chunk and a kv head: up to 16 rows few_kernel, more wide_kernel.
-// A partial (maximum, sum, value sum) per row and chunk goes to the workspace; join_kernel joins a row's, transforms and
-// rounds.
+// The host cuts each sequence's queries into tiles of rows (a row: a query token and one of the kv head's query heads) and its
+// tokens into chunks.  A workgroup takes a tile, a chunk and a kv head: up to 16 rows few_kernel, bound by the codes' bytes or,
+// where there are few, by launches; up to 128 or 256 rows wide_kernel, bound by instructions issued.  A chunk with all that a
+// tile's rows see goes to the output as it is; of others a partial (maximum, sum, value sum) a row goes to the workspace, and
+// fourbit_join_kernel joins a row's, transforms and rounds.
 #include <type_traits>
 
 #include "nq_flash.h"
@@ -191,6 +192,9 @@ __device__ __forceinline__ void butterflies(float (&x)[N]) {
 // Where a section's tokens are and their scales stand in LDS, in one of three places: the next section's are written in the
 // middle of this one, behind a barrier there a wave's last unit asks for the next section's first codes, and a wave that is
 // ahead writes the section after that one, which no wave reads yet.
+//
+// Measured (a copy of 2 GiB reads and writes 4.9 TB/s): 64 rows up to 8192 tokens of 8 x 128 (335 MB) 65 us, 5.2 TB/s, and 4.2
+// for the join; one row of 131072 (138 MB) 28 and 5; four rows of 1000 6.2 and 3.3.
 template <int D>
 struct FewShape {
     static constexpr int WAVES = 4, ROWS = 16;
@@ -590,7 +594,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
 
 // The chunks' sums of a (query token, head) weighted and added in a fixed order, then the transform, h and the softmax's sum.
 // A row that saw nothing is zero.  WIDE: a workgroup for it, D / 4 lanes a chunk; else a wave, all lanes a chunk (2900 tokens
-// of 20 heads x 64 in one to three chunks: 59 us with workgroups).
+// of 20 heads x 64 in one to three chunks: 59 us with workgroups, 9 with waves).  985 tokens of 32 x 128 in 2500 slots (41 MB)
+// 15 us; a decode step's 3.3 to 5, a launch and two loads that wait for each other.
 template <int D, int QDT, bool WIDE>
 __global__ __launch_bounds__(256) void fourbit_join_kernel(FourBitArgs a, uint32_t n) {
     constexpr int V = WIDE ? 4 : D / 64, LANES = D / V, NG = (WIDE ? 256 : 64) / LANES;  // chunks at a time
@@ -653,6 +658,12 @@ __global__ __launch_bounds__(256) void fourbit_join_kernel(FourBitArgs a, uint32
 // products of two digits, O^T += V^T P^T as in nq_flash.h (Rows).  Scales go to LDS as fp32: the keys' times the logits, the
 // values' times the weights.  With few rows several waves share them and split a stage's two tiles; the upper tile's sums are
 // then joined to the lower's in LDS.
+//
+// Bound by instructions issued: 2048 query tokens x 4 heads over 32768 tokens of 8 x 128 take 1215 us, 872 TFLOP/s where a
+// library product of 8192^3 reaches 1340; a CU issues in 81 % of its cycles, the matrix cores are busy in 35 (int8 products
+// count half of fp16's), the vector units in 64, LDS in 34.  With head_dim 64 (851 us) half as much is done for a softmax's
+// weight, with 256 (1024 tokens over 16384, 917 us) a wave a SIMD hides less.  Tried: scaled keys and values in fp16 for exact
+// codes (no faster), two halves of a workgroup in opposite order (11 % slower), waves' priorities (0 to 6 % slower).
 constexpr int kWideStage = 64;
 
 template <int D, int NW>

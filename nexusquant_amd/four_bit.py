@@ -223,31 +223,38 @@ def attention_items(pages: Sequence[int], lengths: Sequence[int], queries: Seque
         if of.any():
             chunks[of], each[of] = _few_chunks(span[of], heads, head_dim) if k == _FEW else \
                 _wide_chunks(span[of], t[of, 5], heads, head_dim, _AT_ONCE[k][head_dim])
-    items, slots = [], 0
-    base: Dict[tuple, int] = {}
-    for k in range(len(t)):
-        _, b, i0, i1, r0, n_rows, start, end = (int(x) for x in t[k])
-        c, step = int(chunks[k]), int(each[k])
-        last = lengths[b] - queries[b] if causal else lengths[b] - 1
-        if c == 1:  # nothing to join
-            items.append((starts[b], start, end - start, firsts[b], r0, n_rows, 0, 0, last, 0, 0, 0))
-            continue
-        at = base.get((b, i0))
-        if at is None:
-            at = base[(b, i0)] = slots
-            slots += (i1 - i0) * c
-            joins += [(firsts[b] + i, at + (i - i0) * c, c, 0) for i in range(i0, i1)]
-        for j in range(c):
-            first = start + j * step
-            items.append((starts[b], first, min(step, end - first), firsts[b], r0, n_rows, at - i0 * c + j, c, last, 0, 0, 0))
+    _, b, i0, i1, r0, n_rows, start, end = t.T
+    news = np.asarray(queries, dtype=np.int64)[b]
+    last = np.asarray(lengths, dtype=np.int64)[b] - (news if causal else 1)
+    starts, firsts = np.asarray(starts, dtype=np.int64)[b], np.asarray(firsts, dtype=np.int64)[b]
+    # partial sums: slots for the query tokens of a tile that is split, the same ones for further tiles of their heads (which
+    # follow it); a tile that is not goes to the output
+    split = chunks > 1
+    own = split & (r0 == i0 * group)
+    need = np.where(own, (i1 - i0) * chunks, 0)
+    slots = int(need.sum())
     if slots >= 1 << 31:
         raise ValueError("too many partial sums: split the queries over several plans")
+    at = np.cumsum(need) - need
+    at = at[np.maximum.accumulate(np.where(own | ~split, np.arange(len(t)), 0))]
+    of = np.repeat(np.arange(len(t)), chunks)  # an item's tile
+    j = np.arange(len(of)) - (np.cumsum(chunks) - chunks)[of]
+    first = start[of] + j * each[of]
+    items = np.zeros((len(of), _ITEM_INTS), dtype=np.int32)
+    items[:, 0], items[:, 1], items[:, 2] = starts[of], first, np.minimum(each[of], end[of] - first)
+    items[:, 3], items[:, 4], items[:, 5] = firsts[of], r0[of], n_rows[of]
+    items[:, 6], items[:, 7] = np.where(split, at - i0 * chunks, 0)[of] + np.where(split[of], j, 0), np.where(split, chunks, 0)[of]
+    items[:, 8] = last[of]
+    tokens = np.where(own, i1 - i0, 0)
+    of = np.repeat(np.arange(len(t)), tokens)  # a joined query token's tile
+    i = np.arange(len(of)) - (np.cumsum(tokens) - tokens)[of]
+    joined = np.zeros((len(joins) + len(of), 4), dtype=np.int32)
+    joined[:len(joins)] = np.array(joins, dtype=np.int32).reshape(-1, 4)
+    joined[len(joins):, 0], joined[len(joins):, 1], joined[len(joins):, 2] = (firsts + i0)[of] + i, at[of] + i * chunks[of], chunks[of]
     n_items = [int(chunks[kind == k].sum()) for k in range(3)]
-    items = np.array(items, np.int32).reshape(-1, _ITEM_INTS)
     # the longest of a kind first (64 rows up to 8192 tokens 77 to 72 us)
     items = items[np.lexsort((-items[:, 2], np.repeat(np.arange(3), n_items)))]
-    return ((items.reshape(-1), np.array(joins, np.int32).reshape(-1)),
-            (*n_items, len(joins), slots, int(chunks.max())))
+    return (items.reshape(-1), joined.reshape(-1)), (*n_items, len(joined), slots, int(chunks.max()))
 
 
 # nq_fourbit_append_desc and nq_fourbit_desc, packed in one go and passed as bytes
@@ -262,8 +269,8 @@ class FourBitPagePool(PagePool):
     key_scales, value_scales  fp16 [layers, pages, heads, tokens]
 
     A vector x is held as t = H x (H the orthonormal Walsh-Hadamard matrix): scale = fp16(max |t| / 7.5), nibble
-    n = clamp(floor(t / scale + 8.5), 0, 15), which stands for H ((n - 8) scale): half a scale off at most.  A vector with an infinity or a NaN has a
-    NaN scale; queries that see it get NaN.
+    n = clamp(floor(t / scale + 8.5), 0, 15), which stands for H ((n - 8) scale): half a scale off at most.  A vector with
+    an infinity or a NaN has a NaN scale; queries that see it get NaN.
 
     Page numbers, fork, copy_pages, free: as CompressedPagePool.  compact keeps positions (keys are stored rotated)."""
 
@@ -462,9 +469,9 @@ class FourBitPagePool(PagePool):
         and heads) over the plan's tokens in one layer.  scale: 1 / sqrt(head_dim) by default.
 
         Returns [rows, q_heads, head_dim].  Rows behind the plan's are left as they are in `out`, and are zero without one;
-        `out` may be query.  Codes are exact in the products; queries (transformed) and weights are rounded to twice fp16's
-        11 bits where a kv head has up to 16 rows of a sequence, to 11 where it has more.  How a row's tokens are cut follows
-        from the whole plan: outputs of one row alone and in a batch agree to roundings.
+        `out` may be query.  Codes are exact in the products; a transformed query is rounded to 2^-16 of its largest
+        coordinate, weights to 22 bits where a kv head has up to 96 rows of a sequence and to 11 where it has more.  How a
+        row's tokens are cut follows from the whole plan: outputs of one row alone and in a batch agree to roundings.
         A captured graph reads the plan's arrays: keep the plan while it is replayed.  Inference only."""
         self._check_plan(plan, FourBitAttentionPlan, "attend", layer)
         shape, dtype, dev = query.shape, query.dtype, self.device

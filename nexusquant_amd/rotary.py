@@ -29,7 +29,8 @@ _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 @dataclasses.dataclass(frozen=True)
 class Rotation:
-    """Cosines and sines of some rows' positions: fp32 [rows, 2, head_dim / 2] on the device."""
+    """Cosines and sines of some rows' positions: fp32 [rows, 2, head_dim / 2] on the device.  Made on the current stream;
+    work on other streams waits for it, and keeps it, as for any tensor."""
     angles: torch.Tensor
     rows: int
     head_dim: int
@@ -228,7 +229,8 @@ def rotate(query: torch.Tensor, key: Optional[torch.Tensor], rotation: Rotation,
 
     fp16, bf16 or fp32, computed in fp32 and rounded once; any strides of rows and heads: slices of one fused projection
     are read in place.  inverse: by the opposite angles.  out: where the results go; (query, key) rotates in place.
-    Differentiable (without out)."""
+    Differentiable (without out).  As with any operator, a backward pass is captured into a graph only while no eager
+    graph of the same leaves lives."""
     dtype, dev, grad = query.dtype, rotation.device, False
     for name, t in (("query", query), ("key", key)):
         if t is None and name == "key":
