@@ -660,8 +660,8 @@ __global__ __launch_bounds__(256) void fourbit_join_kernel(FourBitArgs a, uint32
 // then joined to the lower's in LDS.
 //
 // Bound by instructions issued: 2048 query tokens x 4 heads over 32768 tokens of 8 x 128 take 1215 us, 872 TFLOP/s where a
-// library product of 8192^3 reaches 1340; a CU issues in 81 % of its cycles, the matrix cores are busy in 35 (int8 products
-// count half of fp16's), the vector units in 64, LDS in 34.  With head_dim 64 (851 us) half as much is done for a softmax's
+// library product of 8192^3 reaches 1340; a CU issues in 81 % of its cycles, the matrix cores are busy in 40, the vector units
+// in 65, LDS in 34.  With head_dim 64 (851 us) half as much is done for a softmax's
 // weight, with 256 (1024 tokens over 16384, 917 us) a wave a SIMD hides less.  Tried: scaled keys and values in fp16 for exact
 // codes (no faster), two halves of a workgroup in opposite order (11 % slower), waves' priorities (0 to 6 % slower).
 constexpr int kWideStage = 64;
