@@ -137,12 +137,13 @@ def aligned(t: torch.Tensor) -> torch.Tensor:
 
 
 def _extent(t: torch.Tensor) -> Tuple[int, int]:
-    return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+    (n, m, d), (row, head, one), at = t.shape, t.stride(), t.data_ptr()
+    return at, at + t.element_size() * (1 + (n - 1) * row + (m - 1) * head + (d - 1) * one)
 
 
 def same_or_apart(out: torch.Tensor, x: torch.Tensor) -> bool:
     """Whether out [rows, heads, d] is x, element for element, or certainly shares no memory with it."""
-    if out.numel() == 0 or x.numel() == 0:
+    if out is x or out.numel() == 0 or x.numel() == 0:
         return True
     if out.data_ptr() == x.data_ptr() and out.shape == x.shape and out.stride() == x.stride():
         return True
@@ -166,11 +167,11 @@ def vectors_apart(t: torch.Tensor) -> bool:
 
 
 def check_out(out: torch.Tensor, like: torch.Tensor, name: str, align: int = 16) -> None:
-    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
+    if out is not like and (out.shape != like.shape or out.dtype != like.dtype or out.device != like.device):
         raise ValueError(f"{name} must be {tuple(like.shape)} {like.dtype} on {like.device}")
-    size = out.element_size()
-    if (out.shape[2] > 1 and out.stride(2) != 1) or (out.stride(0) * size | out.stride(1) * size | out.data_ptr()) % align \
-            or not vectors_apart(out):
+    size, (row, head, one) = out.element_size(), out.stride()
+    if (one != 1 and out.shape[2] > 1) or (row * size | head * size | out.data_ptr()) % align \
+            or not (out.is_contiguous() or vectors_apart(out)):
         raise ValueError(f"{name} must have {align}-byte aligned head vectors of their own")
 
 
