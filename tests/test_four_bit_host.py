@@ -82,6 +82,14 @@ def test_long_sequences_and_many():
     replay([0], [0], [3], True, 0, 4, 8, 128)
 
 
+def test_ragged_prompts_are_cut_at_the_share():
+    """Long and short sequences of many rows: some are cut, unevenly, others whole."""
+    for lengths, queries, group, heads, d, causal in (([16384, 8371, 11749, 951], [51, 35, 11, 3], 40, 8, 128, True),
+                                                      ([9000, 3000, 5000, 640], [130, 300, 97, 200], 2, 4, 256, False),
+                                                      ([20000, 100], [70, 20], 8, 100, 64, True), ([4000] * 9, [64] * 9, 16, 400, 64, True)):
+        replay([-(-n // 16) for n in lengths], lengths, queries, causal, 0, group, heads, d)
+
+
 def cpu_pool(pages=6, heads=2, tokens=16, d=128, layers=1):
     """A pool without a device, for what is checked before one is needed."""
     pool = four_bit.FourBitPagePool.__new__(four_bit.FourBitPagePool)

@@ -105,6 +105,33 @@ def test_append_and_read(dtype, d, heads, hq, tokens, rows, axes):
             assert (y.cpu()[[i for i, p in enumerate(slots) if p < 0]] == 0).all()
 
 
+@pytest.mark.parametrize("dtype,d,heads,hq,rows", [("fp16", 128, 4, 40, 3400), ("bf16", 64, 16, 16, 3000), ("fp16", 256, 2, 18, 4000)])
+def test_large_steps_are_stored_as_small_ones(dtype, d, heads, hq, rows):
+    """Past 32 MB queries and values read are written in another way; a wave takes a token's heads in several steps."""
+    T = TYPES[dtype]
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    pools = [FourBitPagePool(rows // 16 + 1, heads, 16, d) for _ in range(2)]
+    slots = [p * 16 + i for p in pools[0].allocate(rows // 16 + 1) for i in range(16)][:rows]
+    assert pools[1].allocate(rows // 16 + 1)[0] == slots[0] // 16
+    qkv = torch.randn(rows, hq + 2 * heads, d, device="cuda", generator=g).to(T)
+    q, k, v = qkv[:, :hq], qkv[:, hq:hq + heads], qkv[:, hq + heads:]
+    pos = torch.arange(rows, device="cuda")
+    whole = pools[0].append(pools[0].plan_slots(slots), k, v, rotation=plan_rotation(pos, d), query=q)
+    for a in range(0, rows, 501):
+        part = slice(a, min(a + 501, rows))
+        small = pools[1].append(pools[1].plan_slots(slots[part]), k[part], v[part], rotation=plan_rotation(pos[part], d), query=q[part])
+        assert torch.equal(whole[part], small)
+    for name in ("key_codes", "value_codes", "key_scales", "value_scales"):
+        used = torch.tensor(slots, device="cuda")
+        a, b = (getattr(p, name)[0][used // 16, :, used % 16] for p in pools)
+        assert torch.equal(a, b)
+    for out in (T, torch.float32):
+        whole = pools[0].read(pools[0].plan_slots(slots), dtype=out)
+        for a in range(0, rows, 501):
+            small = pools[0].read(pools[0].plan_slots(slots[a:a + 501]), dtype=out)
+            assert all(torch.equal(x[a:a + 501], y) for x, y in zip(whole, small))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_levels_next_to_a_border_are_decided_in_64_bits(dtype, d):

@@ -153,6 +153,61 @@ def test_a_graph_replays():
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("dtype,rows,hq,hk,d", [("bf16", 5000, 70, 9, 64), ("fp32", 1500, 37, 8, 128), ("fp16", 2100, 33, 1, 256)])
+def test_large_outputs_and_many_heads_are_as_small_ones(dtype, rows, hq, hk, d):
+    """Past 32 MB outputs are stored in another way, and a wave takes a row's heads in several steps."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    qkv = torch.randn(rows, hq + hk, d, device="cuda", generator=g).to(TYPES[dtype])
+    assert qkv.numel() * qkv.element_size() >= 32 << 20
+    pos = torch.arange(rows, device="cuda") * 3
+    got = rotate(qkv[:, :hq], qkv[:, hq:], plan_rotation(pos, d))
+    ang = ref.angles(pos[None], inv_freq(d, 10000.0), frequency_axes(d, None, False))
+    for a in range(0, rows, 613):
+        part = slice(a, min(a + 613, rows))
+        for h in range(0, hq, 8):
+            small, _ = rotate(qkv[part, h:min(h + 8, hq)], None, plan_rotation(pos[part], d))
+            assert torch.equal(got[0][part, h:h + 8], small)
+        small, _ = rotate(qkv[part, hq:], None, plan_rotation(pos[part], d))
+        assert torch.equal(got[1][part], small)
+    x = qkv[-20:].cpu()
+    want = ref.rotate(x, ang[-20:])
+    y = torch.cat([got[0][-20:], got[1][-20:]], dim=1)
+    assert ((y.double().cpu() - want).abs() <= limit(want, x, TYPES[dtype])).all()
+    rotate(qkv[:, :hq], qkv[:, hq:], plan_rotation(pos, d), out=(qkv[:, :hq], qkv[:, hq:]))
+    assert torch.equal(qkv[:, :hq], got[0]) and torch.equal(qkv[:, hq:], got[1])
+
+
+def test_a_captured_gradient_replays():
+    rows, d = 70, 128
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q, k = (torch.randn(rows, h, d, device="cuda", generator=g).bfloat16().requires_grad_() for h in (6, 2))
+    gq, gk = torch.randn_like(q), torch.randn_like(k)
+    r = plan_rotation(torch.arange(rows, device="cuda"), d)
+
+    def step():
+        y = rotate(q, k, r)
+        return [x.detach() for x in y] + list(torch.autograd.grad(y, (q, k), (gq, gk)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        with torch.no_grad():
+            for t in (q, k, gq, gk):
+                t.copy_(torch.randn(t.shape, device="cuda", generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
+        torch.cuda.synchronize()
+
+
 def test_another_stream_and_refusals():
     r = plan_rotation(torch.arange(8, device="cuda"), 64)
     q = torch.randn(8, 2, 64, device="cuda")
