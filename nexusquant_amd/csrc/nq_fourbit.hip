@@ -143,6 +143,19 @@ struct Bytes {  // the levels of a word's nibbles as int8, times 16: coordinates
     __device__ __forceinline__ uint32_t even(uint32_t w) const { return ((w << 4) & mask) ^ sign; }
     __device__ __forceinline__ uint32_t odd(uint32_t w) const { return (w & mask) ^ sign; }
 };
+// Nibbles of two 16-bit numbers as fp16 numbers below its smallest normal one, which the matrix cores take as they are: n 2^-24
+// for nibbles 0 and 2, n 2^-20 for 1 and 3.  Five instructions for four pairs, and no bias but the levels' own 8.
+struct Small {
+    uint32_t even, odd;
+    __device__ __forceinline__ void init() {
+        even = 0x000F000Fu;
+        odd = 0x00F000F0u;
+        asm volatile("" : "+s"(even));
+        asm volatile("" : "+s"(odd));
+    }
+};
+constexpr float kEvenNibble = 0x1p24f, kOddNibble = 0x1p20f;
+
 struct Pairs {  // nibbles j and j + 4 of a word as fp16 values 16 + n (nq_fourbit.h)
     uint32_t mask, sixteen;
     __device__ __forceinline__ void init() {
@@ -186,15 +199,16 @@ __device__ __forceinline__ void butterflies(float (&x)[N]) {
 //   O^T = V^T P^T  16x16x32 fp16 products; S came out as lane (query, kg) with tokens 4 kg + 0..3 of either half, which is
 //                  the B operand as it stands; A: lane (m, kg) the D / 16 nibbles from D / 16 m on of these eight tokens,
 //                  nibble j of all of them the operand of output tile j
-// Values' codes stand in the operand as 16 + n; the 24 too much of each comes off by one more tile of ones, which sums the
+// Values' codes stand in the operand as n (Small); the 8 too much of each comes off by one more tile of ones, which sums the
 // weights.  Weights go in twice, as fp16 and what that rounds off: 22 bits.
 //
 // Where a section's tokens are and their scales stand in LDS, in one of three places: the next section's are written in the
 // middle of this one, behind a barrier there a wave's last unit asks for the next section's first codes, and a wave that is
 // ahead writes the section after that one, which no wave reads yet.
 //
-// Measured (a copy of 2 GiB reads and writes 4.9 TB/s): 64 rows up to 8192 tokens of 8 x 128 (335 MB) 65 us, 5.2 TB/s, and 4.2
-// for the join; one row of 131072 (138 MB) 28 and 5; four rows of 1000 6.2 and 3.3.
+// Measured (a copy of 2 GiB reads and writes 4.9 TB/s): 64 rows up to 8192 tokens of 8 x 128 (335 MB) 64 us, 5.2 TB/s, and 4.2
+// for the join; one row of 131072 (138 MB) 27 and 5; four rows of 1000 6.2 and 3.3.  Eight waves a workgroup were no faster where
+// one takes a whole sequence (24 of up to 1500 tokens) and 5 to 10 % slower in the others.
 template <int D>
 struct FewShape {
     static constexpr int WAVES = 4, ROWS = 16;
@@ -265,7 +279,10 @@ __device__ __forceinline__ void few_queries(const FourBitArgs& a, const Item& it
     }
 }
 
-template <int D, int QDT>
+// FAR: a layer's codes take more than 4 GiB.  Else an offset has 32 bits, and a load one instruction for its address, where three
+// are needed for 64 (ten loads a unit of some 240).  With the nibbles as they are (Small) 2 to 6 % less: one row of 131072 tokens
+// 34.4 to 32.6 us, 32 rows up to 8192 of 8 x 64 27.4 to 26.0, 64 of 8 x 128 71.3 to 70.1.
+template <int D, int QDT, bool FAR>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>::PER_SIMD))) void few_kernel(FourBitArgs a) {
     using F = FewShape<D>;
     constexpr int KW = D / 32, KS = D / 64, TILES = D / 16, NW = F::WAVES, NT = 64 * NW, RB = D / 2;
@@ -285,10 +302,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
         return (uint32_t)it.pages[p];
     };
     auto row_in = [&](uint32_t page, uint32_t off) { return (page * a.kv_heads + kh) * a.tokens + off; };
-    const uint8_t* const kbase = a.pool.codes[0] + 4 * KW * kg;
-    const uint8_t* const vbase = a.pool.codes[1] + (D == 64 ? 4 * (n16 >> 1) : 4 * VW * n16);
+    const uint32_t k_at = 4 * KW * kg, v_at = D == 64 ? 4 * (n16 >> 1) : 4 * VW * n16;
+    auto code_at = [&](const uint8_t* base, uint32_t row, uint32_t at) {
+        if constexpr (FAR) return reinterpret_cast<const uint32_t*>(base + ((size_t)row * RB + at));
+        else return reinterpret_cast<const uint32_t*>(base + (row * RB + at));
+    };
     auto load_keys = [&](int half, uint32_t row) {
-        const uint32_t* const p = reinterpret_cast<const uint32_t*>(kbase + (size_t)row * RB);
+        const uint32_t* const p = code_at(a.pool.codes[0], row, k_at);
         if constexpr (KW == 2) {
             const u32x2 w = *reinterpret_cast<const u32x2*>(p);
             kcode[half][0] = w.x;
@@ -303,8 +323,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
         }
     };
     auto load_values = [&](int i, uint32_t row) {
-        const uint8_t* const p = vbase + (size_t)row * RB;
-        if constexpr (VW == 1) vcode[i][0] = *reinterpret_cast<const uint32_t*>(p);
+        const uint32_t* const p = code_at(a.pool.codes[1], row, v_at);
+        if constexpr (VW == 1) vcode[i][0] = *p;
         else {
             const u32x2 w = *reinterpret_cast<const u32x2*>(p);
             vcode[i][0] = w.x;
@@ -382,9 +402,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
     // [64, 128), so weights (2^kSlack at most) stay below 2^15.  The power of two is in the sum of weights as well.
     float m = kNoMax, l = 0.0f, lift = 31.0f;
     Bytes bytes;
-    Pairs pairs;
+    Small small;
     bytes.init();
-    pairs.init();
+    small.init();
     const uint32_t pick_lo = D == 64 && (n16 & 1) ? 0x07060302u : 0x05040100u;
     const u32x4 ones = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
     auto rescale = [&](float f) {
@@ -477,10 +497,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
                     f32x4& to = o[8 * k + 4 * half + j];
                     to = mfma16(v, rest, mfma16(v, w, to));
                 };
-                tile(0, u32x4{pairs.get<0>(y[0]), pairs.get<0>(y[1]), pairs.get<0>(y[2]), pairs.get<0>(y[3])});
-                tile(1, u32x4{pairs.get<1>(y[0]), pairs.get<1>(y[1]), pairs.get<1>(y[2]), pairs.get<1>(y[3])});
-                tile(2, u32x4{pairs.get<2>(y[0]), pairs.get<2>(y[1]), pairs.get<2>(y[2]), pairs.get<2>(y[3])});
-                tile(3, u32x4{pairs.get<3>(y[0]), pairs.get<3>(y[1]), pairs.get<3>(y[2]), pairs.get<3>(y[3])});
+#pragma unroll
+                for (int j = 0; j < 4; j += 2) {
+                    tile(j, u32x4{y[0] & small.even, y[1] & small.even, y[2] & small.even, y[3] & small.even});
+                    tile(j + 1, u32x4{y[0] & small.odd, y[1] & small.odd, y[2] & small.odd, y[3] & small.odd});
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[i] >>= 8;
+                }
             }
         values_at(next);
         if (last && u + NW < n_units) {  // the next section's scales
@@ -526,7 +549,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
 #pragma unroll
     for (int j = 0; j < TILES; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[j][i] = __builtin_fmaf(-kNibbleBias, wsum[i], o[j][i]);
+        for (int i = 0; i < 4; ++i) o[j][i] = __builtin_fmaf(-8.0f, wsum[i], o[j][i] * (j & 1 ? kOddNibble : kEvenNibble));
 
     // ---- the waves' sums joined: the upper half's into the lower half's, twice ----
     l = four_sum(l);
@@ -1078,13 +1101,14 @@ constexpr int kManyWaves = D == 256 ? 4 : 8;
 constexpr uint32_t kWaveChunks = 16;
 
 template <int D, int QDT>
-static hipError_t launch_fourbit(FourBitArgs a, const uint32_t (&n_items)[3], uint32_t n_joins, uint32_t most_chunks, hipStream_t s) {
+static hipError_t launch_fourbit(FourBitArgs a, const uint32_t (&n_items)[3], uint32_t n_joins, uint32_t most_chunks, bool far, hipStream_t s) {
     for (int k = 0; k < 3; ++k) {
         if (n_items[k] == 0) continue;
         const dim3 grid(n_items[k] * a.kv_heads);
         if (k == 0) hipLaunchKernelGGL((wide_kernel<D, QDT, kManyWaves<D>>), grid, dim3(64 * kManyWaves<D>), 0, s, a);
         else if (k == 1) hipLaunchKernelGGL((wide_kernel<D, QDT, 4>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((few_kernel<D, QDT>), grid, dim3(256), 0, s, a);
+        else if (far) hipLaunchKernelGGL((few_kernel<D, QDT, true>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((few_kernel<D, QDT, false>), grid, dim3(256), 0, s, a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
         a.items += (size_t)kItemInts * n_items[k];
@@ -1098,11 +1122,11 @@ static hipError_t launch_fourbit(FourBitArgs a, const uint32_t (&n_items)[3], ui
 }
 
 template <int QDT>
-static hipError_t fourbit_dims(int32_t d, const FourBitArgs& a, const uint32_t (&n_items)[3], uint32_t n_joins, uint32_t most_chunks, hipStream_t s) {
+static hipError_t fourbit_dims(int32_t d, const FourBitArgs& a, const uint32_t (&n_items)[3], uint32_t n_joins, uint32_t most_chunks, bool far, hipStream_t s) {
     switch (d) {
-        case 64: return launch_fourbit<64, QDT>(a, n_items, n_joins, most_chunks, s);
-        case 128: return launch_fourbit<128, QDT>(a, n_items, n_joins, most_chunks, s);
-        default: return launch_fourbit<256, QDT>(a, n_items, n_joins, most_chunks, s);
+        case 64: return launch_fourbit<64, QDT>(a, n_items, n_joins, most_chunks, far, s);
+        case 128: return launch_fourbit<128, QDT>(a, n_items, n_joins, most_chunks, far, s);
+        default: return launch_fourbit<256, QDT>(a, n_items, n_joins, most_chunks, far, s);
     }
 }
 
@@ -1170,7 +1194,8 @@ extern "C" int nq_fourbit_attention(const nq_fourbit_desc* d, void* stream) {
     a.c = d->scale * 1.44269504088896340736f * d->hadamard_scale;
     hipStream_t s = (hipStream_t)stream;
     const uint32_t n[3] = {(uint32_t)d->n_items[0], (uint32_t)d->n_items[1], (uint32_t)d->n_items[2]};
-    NQ_CHECK_HIP(d->q_dtype == NQ_F16 ? fourbit_dims<NQ_F16>(dim, a, n, (uint32_t)d->n_joins, (uint32_t)d->most_chunks, s)
-                                      : fourbit_dims<NQ_BF16>(dim, a, n, (uint32_t)d->n_joins, (uint32_t)d->most_chunks, s));
+    const bool far = (uint64_t)p->pages * p->heads * p->tokens * (uint64_t)(dim / 2) > 1ull << 32;
+    NQ_CHECK_HIP(d->q_dtype == NQ_F16 ? fourbit_dims<NQ_F16>(dim, a, n, (uint32_t)d->n_joins, (uint32_t)d->most_chunks, far, s)
+                                      : fourbit_dims<NQ_BF16>(dim, a, n, (uint32_t)d->n_joins, (uint32_t)d->most_chunks, far, s));
     return NQ_OK;
 }
