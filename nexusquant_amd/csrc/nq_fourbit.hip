@@ -143,19 +143,6 @@ struct Bytes {  // the levels of a word's nibbles as int8, times 16: coordinates
     __device__ __forceinline__ uint32_t even(uint32_t w) const { return ((w << 4) & mask) ^ sign; }
     __device__ __forceinline__ uint32_t odd(uint32_t w) const { return (w & mask) ^ sign; }
 };
-// Nibbles of two 16-bit numbers as fp16 numbers below its smallest normal one, which the matrix cores take as they are: n 2^-24
-// for nibbles 0 and 2, n 2^-20 for 1 and 3.  Five instructions for four pairs, and no bias but the levels' own 8.
-struct Small {
-    uint32_t even, odd;
-    __device__ __forceinline__ void init() {
-        even = 0x000F000Fu;
-        odd = 0x00F000F0u;
-        asm volatile("" : "+s"(even));
-        asm volatile("" : "+s"(odd));
-    }
-};
-constexpr float kEvenNibble = 0x1p24f, kOddNibble = 0x1p20f;
-
 struct Pairs {  // nibbles j and j + 4 of a word as fp16 values 16 + n (nq_fourbit.h)
     uint32_t mask, sixteen;
     __device__ __forceinline__ void init() {
@@ -199,8 +186,9 @@ __device__ __forceinline__ void butterflies(float (&x)[N]) {
 //   O^T = V^T P^T  16x16x32 fp16 products; S came out as lane (query, kg) with tokens 4 kg + 0..3 of either half, which is
 //                  the B operand as it stands; A: lane (m, kg) the D / 16 nibbles from D / 16 m on of these eight tokens,
 //                  nibble j of all of them the operand of output tile j
-// Values' codes stand in the operand as n (Small); the 8 too much of each comes off by one more tile of ones, which sums the
-// weights.  Weights go in twice, as fp16 and what that rounds off: 22 bits.
+// Values' codes stand in the operand as 16 + n; the 24 too much of each comes off by one more tile of ones, which sums the
+// weights (n alone, as a subnormal number, would need fewer instructions, but the matrix cores then add to some 20 bits: one row
+// of 131072 tokens is 5.4e-4 off for 2.1e-4).  Weights go in twice, as fp16 and what that rounds off: 22 bits.
 //
 // Where a section's tokens are and their scales stand in LDS, in one of three places: the next section's are written in the
 // middle of this one, behind a barrier there a wave's last unit asks for the next section's first codes, and a wave that is
@@ -280,8 +268,8 @@ __device__ __forceinline__ void few_queries(const FourBitArgs& a, const Item& it
 }
 
 // FAR: a layer's codes take more than 4 GiB.  Else an offset has 32 bits, and a load one instruction for its address, where three
-// are needed for 64 (ten loads a unit of some 240).  With the nibbles as they are (Small) 2 to 6 % less: one row of 131072 tokens
-// 34.4 to 32.6 us, 32 rows up to 8192 of 8 x 64 27.4 to 26.0, 64 of 8 x 128 71.3 to 70.1.
+// are needed for 64 (ten loads a unit of some 240): one row of 131072 tokens 35.1 to 33.8 us, 16 sequences of 20 rows over 4096
+// 19.5 to 18.5, 64 rows up to 8192 73.9 to 72.3.
 template <int D, int QDT, bool FAR>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>::PER_SIMD))) void few_kernel(FourBitArgs a) {
     using F = FewShape<D>;
@@ -402,9 +390,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
     // [64, 128), so weights (2^kSlack at most) stay below 2^15.  The power of two is in the sum of weights as well.
     float m = kNoMax, l = 0.0f, lift = 31.0f;
     Bytes bytes;
-    Small small;
+    Pairs pairs;
     bytes.init();
-    small.init();
+    pairs.init();
     const uint32_t pick_lo = D == 64 && (n16 & 1) ? 0x07060302u : 0x05040100u;
     const u32x4 ones = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
     auto rescale = [&](float f) {
@@ -497,13 +485,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
                     f32x4& to = o[8 * k + 4 * half + j];
                     to = mfma16(v, rest, mfma16(v, w, to));
                 };
-#pragma unroll
-                for (int j = 0; j < 4; j += 2) {
-                    tile(j, u32x4{y[0] & small.even, y[1] & small.even, y[2] & small.even, y[3] & small.even});
-                    tile(j + 1, u32x4{y[0] & small.odd, y[1] & small.odd, y[2] & small.odd, y[3] & small.odd});
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) y[i] >>= 8;
-                }
+                tile(0, u32x4{pairs.get<0>(y[0]), pairs.get<0>(y[1]), pairs.get<0>(y[2]), pairs.get<0>(y[3])});
+                tile(1, u32x4{pairs.get<1>(y[0]), pairs.get<1>(y[1]), pairs.get<1>(y[2]), pairs.get<1>(y[3])});
+                tile(2, u32x4{pairs.get<2>(y[0]), pairs.get<2>(y[1]), pairs.get<2>(y[2]), pairs.get<2>(y[3])});
+                tile(3, u32x4{pairs.get<3>(y[0]), pairs.get<3>(y[1]), pairs.get<3>(y[2]), pairs.get<3>(y[3])});
             }
         values_at(next);
         if (last && u + NW < n_units) {  // the next section's scales
@@ -549,7 +534,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
 #pragma unroll
     for (int j = 0; j < TILES; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[j][i] = __builtin_fmaf(-8.0f, wsum[i], o[j][i] * (j & 1 ? kOddNibble : kEvenNibble));
+        for (int i = 0; i < 4; ++i) o[j][i] = __builtin_fmaf(-kNibbleBias, wsum[i], o[j][i]);
 
     // ---- the waves' sums joined: the upper half's into the lower half's, twice ----
     l = four_sum(l);
