@@ -289,6 +289,19 @@ def test_rows_up_to_and_past_several_small_tiles(dtype, heads, group, d, tokens,
             check_attention(pool, [tables[b]], [n], [m], rows, pool.attend(alone, rows), T, True, window, few=True)
 
 
+@pytest.mark.parametrize("d,group,n,queries", [(128, 8, 131072, 1), (64, 2, 50000, 40), (128, 4, 40000, 40)])
+def test_sums_over_long_sequences_keep_their_bits(d, group, n, queries):
+    """Many values whose weighted sum is near zero: what the sums' additions lose counts hundreds of times."""
+    pool = FourBitPagePool(n // 64 + 3, 1, 64, d)
+    fill(pool, 4)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    low, high = (torch.randint(1, 16, pool.value_codes.shape, device="cuda", generator=g, dtype=torch.uint8) for _ in range(2))
+    pool.value_codes.copy_(low | high << 4)  # levels -7 .. 7
+    tables = sequences(pool, [n], 9)
+    q = torch.randn(queries, group, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).half()
+    check_attention(pool, tables, [n], [queries], q, pool.attend(pool.plan_attention(tables, [n], [queries]), q), torch.float16)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("queries", [1, 4, 40])
 def test_what_some_queries_do_not_see_may_be_anything(dtype, queries):
