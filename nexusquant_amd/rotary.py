@@ -105,7 +105,8 @@ def plan_rotation(positions, head_dim: int, base: float = 10000.0, rope_scaling:
     elif device is not None and torch.device(device) != positions.device and torch.device(device) != torch.device("cuda"):
         raise ValueError(f"positions are on {positions.device}, not on {device}")
     sections = None if sections is None else tuple(int(n) for n in sections)
-    axes, _, _, freq, axis_of = _table(head_dim, float(base), rope_scaling, sections, bool(interleaved))
+    table = _table(head_dim, float(base), rope_scaling, sections, bool(interleaved))  # (held until the call has read its arrays)
+    axes, _, _, freq, axis_of = table
     if positions.dim() == 1 and axes == 1:
         positions = positions[None]
     if positions.dim() != 2 or positions.shape[0] != axes:

@@ -67,3 +67,41 @@ def test_entry_points_refuse_bad_arguments():
                dict(rows=(1 << 31) - 1, hq=1 << 20)):
         assert lib.nq_rotate(desc(**kw), None) == -1, kw
     assert lib.nq_rotate(desc(rows=0), None) == lib.nq_rotate(desc(hq=0, hk=0), None) == 0
+
+
+def test_frequencies_live_until_the_call_has_read_them(monkeypatch):
+    """Another thread may empty the tables while a call is on its way to the device."""
+    import contextlib
+    import gc
+    import weakref
+
+    class OnDevice(torch.Tensor):  # a tensor of the host that says it is on a device
+        is_cuda = True
+
+    held, read = [], []
+    table = rotary._table
+
+    def watched(*args):
+        got = table(*args)
+        held.extend(weakref.ref(a) for a in got[1:3])
+        return got
+
+    class Lib:
+        @staticmethod
+        def nq_rotation(positions, wide, axes, stride, rows, half, freq, axis_of, out, stream):
+            rotary._tables.clear()
+            gc.collect()
+            assert all(a() is not None for a in held)
+            read.append(np.ctypeslib.as_array(ctypes.cast(freq, ctypes.POINTER(ctypes.c_float)), (half,)).copy())
+            read.append(np.ctypeslib.as_array(ctypes.cast(axis_of, ctypes.POINTER(ctypes.c_uint8)), (half,)).copy())
+            return 0
+
+    monkeypatch.setattr(rotary, "_table", watched)
+    monkeypatch.setattr(rotary._lib, "load", Lib)
+    monkeypatch.setattr(rotary._lib, "current_stream_handle", lambda dev: None)
+    monkeypatch.setattr(rotary, "on_device", lambda dev: contextlib.nullcontext())
+    positions = torch.zeros(2, 3, dtype=torch.int64).as_subclass(OnDevice)
+    rotary.plan_rotation(positions, 64, base=12345.0, sections=[20, 12])
+    assert len(held) == 2
+    assert np.array_equal(read[0], rotary.inv_freq(64, 12345.0).numpy())
+    assert np.array_equal(read[1], rotary.frequency_axes(64, [20, 12], False))
