@@ -212,7 +212,10 @@ class _Rotate(torch.autograd.Function):
         ctx.save_for_backward(angles)
         ctx.inverse = inverse
         ctx.set_materialize_grads(False)
-        return _rotated(query, key, angles, inverse)
+        out = _rotated(query, key, angles, inverse)
+        # of an input that needs no gradient the output needs none, and backward does not turn one for it
+        ctx.mark_non_differentiable(*(y for y, needs in zip(out, ctx.needs_input_grad) if y is not None and not needs))
+        return out
 
     @staticmethod
     def backward(ctx, grad_query, grad_key):

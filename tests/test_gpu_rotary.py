@@ -10,6 +10,7 @@ from nexusquant_amd import plan_rotation, rotate
 from nexusquant_amd.rope import inv_freq
 from nexusquant_amd.rotary import frequency_axes
 from oracle import four_bit as ref
+from test_rotary_host import check_gradients_of_those_that_need_one
 
 pytestmark = pytest.mark.gpu
 
@@ -236,3 +237,7 @@ def test_another_stream_and_refusals():
         plan_rotation(torch.arange(6, device="cuda").view(2, 3), 64)
     with pytest.raises(TypeError):
         plan_rotation(torch.arange(6, device="cuda").float(), 64)
+
+
+def test_gradients_of_those_that_need_one():
+    check_gradients_of_those_that_need_one(plan_rotation(torch.arange(5, device="cuda"), 64), [])

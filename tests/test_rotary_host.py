@@ -105,3 +105,50 @@ def test_frequencies_live_until_the_call_has_read_them(monkeypatch):
     assert len(held) == 2
     assert np.array_equal(read[0], rotary.inv_freq(64, 12345.0).numpy())
     assert np.array_equal(read[1], rotary.frequency_axes(64, [20, 12], False))
+
+
+def turned(x, angles, inverse):
+    c, s = angles[:, None, 0], angles[:, None, 1] * (-1.0 if inverse else 1.0)
+    a, b = x.chunk(2, dim=-1)
+    return torch.cat([a * c - b * s, b * c + a * s], dim=-1)
+
+
+def host_rotation(monkeypatch, rows=5, d=64):
+    """A rotation of the host, and what is launched: pairs (query or not, key or not), computed in torch's operations."""
+    launched = []
+
+    def launch(query, key, angles, inverse, q_out, k_out):
+        launched.append((query is not None, key is not None))
+        with torch.no_grad():
+            for x, y in ((query, q_out), (key, k_out)):
+                if x is not None:
+                    y.copy_(turned(x, angles, inverse))
+
+    monkeypatch.setattr(rotary, "_launch", launch)
+    angle = torch.rand(rows, d // 2, generator=torch.Generator().manual_seed(1)) * 6
+    return rotary.Rotation(angles=torch.stack([angle.cos(), angle.sin()], dim=1), rows=rows, head_dim=d), launched
+
+
+def check_gradients_of_those_that_need_one(r, launched):
+    """The query alone, the key alone: the other's output needs no gradient, and none is computed.  Both, of which one is used."""
+    dev, (rows, d) = r.device, (r.rows, r.head_dim)
+    g = torch.Generator().manual_seed(2)
+    for of_query, of_key in ((True, False), (False, True)):
+        q, k = (torch.randn(rows, h, d, generator=g).to(dev).requires_grad_(need) for h, need in ((4, of_query), (2, of_key)))
+        w = [torch.randn(x.shape, generator=g).to(dev) for x in (q, k)]
+        y = rotary.rotate(q, k, r)
+        assert (y[0].requires_grad, y[1].requires_grad) == (of_query, of_key)
+        before = len(launched)
+        got, = torch.autograd.grad((y[0] * w[0]).sum() + (y[1] * w[1]).sum(), (q if of_query else k,))
+        assert launched[before:] in ([(of_query, of_key)], [])  # (empty: the kernel itself ran)
+        assert (got - turned(w[0 if of_query else 1], r.angles, True)).abs().max() <= 1e-5
+    q, k = (torch.randn(rows, h, d, generator=g).to(dev).requires_grad_() for h in (4, 2))
+    y = rotary.rotate(q, k, r)
+    assert y[0].requires_grad and y[1].requires_grad
+    w = torch.randn(k.shape, generator=g).to(dev)
+    got = torch.autograd.grad((y[1] * w).sum(), (q, k), allow_unused=True)
+    assert got[0] is None and (got[1] - turned(w, r.angles, True)).abs().max() <= 1e-5
+
+
+def test_gradients_of_those_that_need_one(monkeypatch):
+    check_gradients_of_those_that_need_one(*host_rotation(monkeypatch))
