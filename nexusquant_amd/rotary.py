@@ -18,6 +18,7 @@ from typing import Dict, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import on_device
@@ -204,26 +205,47 @@ def _rotated(query, key, angles: torch.Tensor, inverse: bool):
     return q_out, k_out
 
 
+def has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether forward mode differentiates one of these (outside of its levels 0.06 us; unpack_dual takes 0.4 a tensor)."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 class _Rotate(torch.autograd.Function):
-    """The gradient of a rotation is the rotation by the opposite angle."""
+    """The gradient of a rotation is the rotation by the opposite angle, its derivative along a tangent the tangent's rotation."""
 
     @staticmethod
-    def forward(ctx, query, key, angles, inverse):
+    def forward(ctx, query, key, angles, inverse, tangents):
         ctx.save_for_backward(angles)
+        ctx.save_for_forward(angles)
         ctx.inverse = inverse
         ctx.set_materialize_grads(False)
         out = _rotated(query, key, angles, inverse)
         # of an input that needs no gradient the output needs none, and backward does not turn one for it
-        ctx.mark_non_differentiable(*(y for y, needs in zip(out, ctx.needs_input_grad) if y is not None and not needs))
+        ctx.moves = [t is not None and any(x) for t, *x in zip((query, key), ctx.needs_input_grad, tangents)]
+        ctx.mark_non_differentiable(*(y for y, moves in zip(out, ctx.moves) if y is not None and not moves))
+        ctx.shapes = [None if t is None else t.shape for t in (query, key)]
         return out
 
     @staticmethod
     def backward(ctx, grad_query, grad_key):
         if grad_query is None and grad_key is None:
-            return None, None, None, None
+            return (None,) * 5
         angles, = ctx.saved_tensors
-        again = _Rotate.apply if torch.is_grad_enabled() else _rotated  # (a gradient of the gradient is asked for, or not)
-        return (*again(grad_query, grad_key, angles, not ctx.inverse), None, None)
+        # (derivatives of the gradient are asked for, or not)
+        again = _differentiable if torch.is_grad_enabled() or has_tangent(grad_query, grad_key) else _rotated
+        return (*again(grad_query, grad_key, angles, not ctx.inverse), None, None, None)
+
+    @staticmethod
+    def jvp(ctx, query, key, *_):
+        angles, = ctx.saved_tensors
+        again = _differentiable if torch.is_grad_enabled() else _rotated
+        like = query if query is not None else key
+        return tuple(y if y is not None or not moves else like.new_zeros(shape)
+                     for y, moves, shape in zip(again(query, key, angles, ctx.inverse), ctx.moves, ctx.shapes))
+
+
+def _differentiable(query, key, angles: torch.Tensor, inverse: bool):
+    return _Rotate.apply(query, key, angles, inverse, (has_tangent(query), has_tangent(key)))  # (forward sees no tangents)
 
 
 def rotate(query: torch.Tensor, key: Optional[torch.Tensor], rotation: Rotation, inverse: bool = False,
@@ -234,8 +256,8 @@ def rotate(query: torch.Tensor, key: Optional[torch.Tensor], rotation: Rotation,
 
     fp16, bf16 or fp32, computed in fp32 and rounded once; any strides of rows and heads: slices of one fused projection
     are read in place.  inverse: by the opposite angles.  out: where the results go; (query, key) rotates in place.
-    Differentiable (without out).  As with any operator, a backward pass is captured into a graph only while no eager
-    graph of the same leaves lives."""
+    Differentiable (without out), in reverse and in forward mode.  As with any operator, a backward pass is captured into a
+    graph only while no eager graph of the same leaves lives."""
     dtype, dev, grad = query.dtype, rotation.device, False
     for name, t in (("query", query), ("key", key)):
         if t is None and name == "key":
@@ -251,15 +273,15 @@ def rotate(query: torch.Tensor, key: Optional[torch.Tensor], rotation: Rotation,
         grad = grad or t.requires_grad
     if rotation.rows >= 1 << 31:
         raise ValueError(f"{rotation.rows} rows: a call takes less than 2^31")
-    grad = grad and torch.is_grad_enabled()
+    grad = grad and torch.is_grad_enabled() or has_tangent(query, key)
     if out is None:
         if grad:
-            return _Rotate.apply(query, key, rotation.angles, bool(inverse))
+            return _differentiable(query, key, rotation.angles, bool(inverse))
         q_out = empty_as(query)
         k_out = None if key is None else empty_as(key)
     else:
         q_out, k_out = out
-        if grad or any(t is not None and t.requires_grad and torch.is_grad_enabled() for t in (q_out, k_out)):
+        if grad or has_tangent(q_out, k_out) or any(t is not None and t.requires_grad and torch.is_grad_enabled() for t in (q_out, k_out)):
             raise NotImplementedError("rotate into given tensors has no backward pass; call it under torch.no_grad()")
         if q_out is None or (k_out is None) != (key is None):
             raise ValueError("out must be a pair of tensors for query and key")

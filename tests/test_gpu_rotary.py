@@ -10,7 +10,7 @@ from nexusquant_amd import plan_rotation, rotate
 from nexusquant_amd.rope import inv_freq
 from nexusquant_amd.rotary import frequency_axes
 from oracle import four_bit as ref
-from test_rotary_host import check_gradients_of_those_that_need_one
+from test_rotary_host import check_forward_mode, check_gradients_of_those_that_need_one
 
 pytestmark = pytest.mark.gpu
 
@@ -241,3 +241,7 @@ def test_another_stream_and_refusals():
 
 def test_gradients_of_those_that_need_one():
     check_gradients_of_those_that_need_one(plan_rotation(torch.arange(5, device="cuda"), 64), [])
+
+
+def test_forward_mode():
+    check_forward_mode(plan_rotation(torch.arange(5, device="cuda"), 64))

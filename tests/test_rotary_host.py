@@ -119,10 +119,9 @@ def host_rotation(monkeypatch, rows=5, d=64):
 
     def launch(query, key, angles, inverse, q_out, k_out):
         launched.append((query is not None, key is not None))
-        with torch.no_grad():
-            for x, y in ((query, q_out), (key, k_out)):
-                if x is not None:
-                    y.copy_(turned(x, angles, inverse))
+        for x, y in ((query, q_out), (key, k_out)):
+            if x is not None:  # (by memory alone, as a kernel)
+                y.detach().numpy()[:] = turned(torch.from_numpy(x.detach().numpy()), angles, inverse).numpy()
 
     monkeypatch.setattr(rotary, "_launch", launch)
     angle = torch.rand(rows, d // 2, generator=torch.Generator().manual_seed(1)) * 6
@@ -152,3 +151,51 @@ def check_gradients_of_those_that_need_one(r, launched):
 
 def test_gradients_of_those_that_need_one(monkeypatch):
     check_gradients_of_those_that_need_one(*host_rotation(monkeypatch))
+
+
+def check_forward_mode(r):
+    """Tangents turn as their tensors do; with them gradients, tangents of gradients and gradients of tangents."""
+    from torch.autograd import forward_ad
+    dev, (rows, d) = r.device, (r.rows, r.head_dim)
+    g = torch.Generator().manual_seed(3)
+    q, k, tq, tk, w = (torch.randn(rows, h, d, generator=g).to(dev) for h in (4, 2, 4, 2, 4))
+
+    def close(x, want):
+        assert (x - want).abs().max() <= 1e-5
+
+    for inverse in (False, True):
+        for grads in (False, True):
+            with torch.set_grad_enabled(grads), forward_ad.dual_level():
+                y = rotary.rotate(forward_ad.make_dual(q, tq), forward_ad.make_dual(k, tk), r, inverse=inverse)
+                for out, x, t in ((y[0], q, tq), (y[1], k, tk)):
+                    got = forward_ad.unpack_dual(out)
+                    close(got.primal, turned(x, r.angles, inverse))
+                    close(got.tangent, turned(t, r.angles, inverse))
+                # of one of the two, and of a query alone
+                y = rotary.rotate(q, forward_ad.make_dual(k, tk), r, inverse=inverse)
+                assert forward_ad.unpack_dual(y[0]).tangent is None
+                close(forward_ad.unpack_dual(y[1]).tangent, turned(tk, r.angles, inverse))
+                y = rotary.rotate(forward_ad.make_dual(q, tq), None, r, inverse=inverse)
+                assert y[1] is None
+                close(forward_ad.unpack_dual(y[0]).tangent, turned(tq, r.angles, inverse))
+    with forward_ad.dual_level():
+        # a gradient with respect to the query beside a tangent of the key
+        leaf = q.clone().requires_grad_()
+        y = rotary.rotate(leaf, forward_ad.make_dual(k, tk), r)
+        t = forward_ad.unpack_dual(y[0]).tangent
+        assert t is None or not t.any()
+        close(forward_ad.unpack_dual(y[1]).tangent, turned(tk, r.angles, False))
+        got, = torch.autograd.grad(y[0], leaf, forward_ad.make_dual(w, tq))  # a gradient's tangent
+        close(got, turned(w, r.angles, True))
+        close(forward_ad.unpack_dual(got).tangent, turned(tq, r.angles, True))
+        leaf = tq.clone().requires_grad_()  # a tangent's gradient
+        y = rotary.rotate(forward_ad.make_dual(q, leaf), None, r)[0]
+        got, = torch.autograd.grad(forward_ad.unpack_dual(y).tangent, leaf, w)
+        close(got, turned(w, r.angles, True))
+        for args in ((forward_ad.make_dual(q, tq), None), (q, forward_ad.make_dual(k, tk))):
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                rotary.rotate(*args, r, out=(torch.empty_like(q), None if args[1] is None else torch.empty_like(k)))
+
+
+def test_forward_mode(monkeypatch):
+    check_forward_mode(host_rotation(monkeypatch)[0])
