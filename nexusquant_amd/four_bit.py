@@ -27,7 +27,7 @@ from . import _lib
 from .hadamard import hadamard_constant
 from .ops import PlanTensor, on_device
 from .page_pool import PagePool
-from .rotary import Rotation, aligned, check_out, empty_as, same_or_apart
+from .rotary import Rotation, aligned, check_out, empty_as, has_tangent, same_or_apart
 
 _HEAD_DIMS = (64, 128, 256)
 _DTYPES = (torch.float16, torch.bfloat16)
@@ -381,6 +381,8 @@ class FourBitPagePool(PagePool):
                 raise ValueError(f"key, value and query must share an fp16 or bf16 dtype, got {t.dtype}")
             if grad and t.requires_grad:
                 raise NotImplementedError("append has no backward pass; call it under torch.no_grad()")
+        if has_tangent(key, value, query):
+            raise NotImplementedError("append has no derivative in forward mode; call it on tensors without tangents")
         if rotation is None:
             if query is not None:
                 raise ValueError("append: a query is rotated along with the keys; without a rotation it is not taken")
@@ -484,6 +486,8 @@ class FourBitPagePool(PagePool):
             raise ValueError(f"attend takes fp16 or bf16 queries, got {dtype}")
         if query.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("attend has no backward pass; call it under torch.no_grad()")
+        if has_tangent(query):
+            raise NotImplementedError("attend has no derivative in forward mode; call it on a query without a tangent")
         scale = self.head_dim ** -0.5 if scale is None else float(scale)
         if not 0.0 < scale < 1e30:
             raise ValueError(f"scale must be positive, got {scale}")

@@ -217,3 +217,63 @@ def test_descriptors_match_the_c_compiler(tmp_path):
     import struct
     assert out[0][1] == struct.calcsize("6i5P6q") and out[1][1] == struct.calcsize("P4i6P8q") and out[2][1] == struct.calcsize("P4i6P")
     assert out[3][1] == struct.calcsize("P10i2fi") + (-struct.calcsize("P10i2fi")) % 8 and out[4][1] == struct.calcsize("P10i2fi5P4qP")
+
+
+def no_launch(monkeypatch):
+    """What a pool of the host gets as far as the launch with; calls are counted."""
+    import contextlib
+
+    class Lib:
+        launched = 0
+
+        def __getattr__(self, name):
+            if name.startswith("nq_fourbit_r") or name.endswith("workspace"):
+                return getattr(real, name)
+            return self.launch
+
+        def launch(self, *args):
+            Lib.launched += 1
+            return 0
+
+    class Ints:
+        def __init__(self, values, device):
+            pass
+
+        def address(self):
+            return 4096
+
+    real = _lib.load()
+    monkeypatch.setattr(_lib, "load", Lib)
+    monkeypatch.setattr(_lib, "current_stream_handle", lambda dev: None)
+    monkeypatch.setattr(four_bit, "on_device", lambda dev: contextlib.nullcontext())
+    monkeypatch.setattr(four_bit, "PlanTensor", Ints)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    return Lib
+
+
+def host_step(pool):
+    """Plans of two tokens of a sequence of 20, their rotation, and tensors for them."""
+    from nexusquant_amd.rotary import Rotation
+    t = pool.allocate(2)
+    rotation = Rotation(angles=torch.zeros(2, 2, 64), rows=2, head_dim=128)
+    q, k, v = (torch.randn(2, h, 128).half() for h in (4, 2, 2))
+    return pool.plan_slots(pool.slots(t, 18, 20)), pool.plan_attention([t], [20], [2]), rotation, q, k, v
+
+
+def test_tensors_with_tangents_are_refused(monkeypatch):
+    from torch.autograd import forward_ad
+    lib, pool = no_launch(monkeypatch), cpu_pool()
+    slots, plan, rotation, q, k, v = host_step(pool)
+    for grads in (False, True):
+        with torch.set_grad_enabled(grads), forward_ad.dual_level():
+            pool.append(slots, k, v, rotation=rotation, query=q)
+            pool.attend(plan, q)
+            launched = lib.launched
+            dq, dk, dv = (forward_ad.make_dual(x, torch.ones_like(x)) for x in (q, k, v))
+            for args in ((dk, v, q), (k, dv, q), (k, v, dq)):
+                with pytest.raises(NotImplementedError, match="forward mode"):
+                    pool.append(slots, *args[:2], rotation=rotation, query=args[2])
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                pool.attend(plan, dq)
+            assert lib.launched == launched
+    assert launched == 4
