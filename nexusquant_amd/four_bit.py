@@ -27,7 +27,7 @@ from . import _lib
 from .hadamard import hadamard_constant
 from .ops import PlanTensor, on_device
 from .page_pool import PagePool
-from .rotary import Rotation, aligned, check_out, empty_as, has_tangent, same_or_apart
+from .rotary import Rotation, aligned, check_out, empty_as, has_tangent, same_or_apart, written
 
 _HEAD_DIMS = (64, 128, 256)
 _DTYPES = (torch.float16, torch.bfloat16)
@@ -403,6 +403,7 @@ class FourBitPagePool(PagePool):
                     if refs.max() > 1:
                         raise ValueError(f"append: page {int(plan.pages[refs > 1][0])} is shared and cannot be written")
                 plan.writable_at = self._changes
+            given = out
             if query is not None and out is None:
                 out = empty_as(query)
             if rows == 0:
@@ -418,6 +419,7 @@ class FourBitPagePool(PagePool):
                     *(none if q is None else q.stride()[:2]), *k.stride()[:2], *v.stride()[:2],
                     *(none if q is None else out.stride()[:2]), hadamard_constant(d), 0), _lib.current_stream_handle(dev))
             _lib.check(st, "nq_fourbit_append")
+            written(given)
         return out
 
     def read(self, plan: SlotPlan, layer: int = 0, dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -493,6 +495,7 @@ class FourBitPagePool(PagePool):
             raise ValueError(f"scale must be positive, got {scale}")
         hq = shape[1]
         ints, places, counts, nbytes = plan._work.get(hq) or plan.work(hq)
+        given = out
         if out is None:
             out = empty_as(query)
             if shape[0] > plan.rows:
@@ -513,4 +516,5 @@ class FourBitPagePool(PagePool):
                 base + places[0], base + places[1], base + places[2], *q.stride()[:2], *out.stride()[:2],
                 0 if ws is None else ws.data_ptr(), nbytes), _lib.current_stream_handle(dev))
         _lib.check(st, "nq_fourbit_attention")
+        written(given)
         return out

@@ -177,6 +177,13 @@ def check_out(out: torch.Tensor, like: torch.Tensor, name: str, align: int = 16)
         raise ValueError(f"{name} must have {align}-byte aligned head vectors of their own")
 
 
+def written(*tensors: Optional[torch.Tensor]) -> None:
+    """Tell autograd that a launch wrote into these: a graph that has saved one raises, as it does after torch's own writes."""
+    for t in tensors:
+        if t is not None:
+            torch.autograd.graph.increment_version(t)
+
+
 # nq_rotate_desc, packed in one go and passed as bytes
 _PACK = struct.Struct("6i5P8q")
 
@@ -294,4 +301,6 @@ def rotate(query: torch.Tensor, key: Optional[torch.Tensor], rotation: Rotation,
                 (key is not None and query.numel() and (q_out.data_ptr() == key.data_ptr() or k_out.data_ptr() == query.data_ptr())):
             raise ValueError("out may be query and key themselves, and must not overlap them or each other otherwise")
     _launch(query, key, rotation.angles, bool(inverse), q_out, k_out)
+    if out is not None:
+        written(q_out, k_out)
     return q_out, k_out

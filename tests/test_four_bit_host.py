@@ -9,6 +9,7 @@ import torch
 
 from nexusquant_amd import _lib, four_bit
 from oracle import four_bit as ref
+from test_rotary_host import check_written_tensors_are_seen
 
 
 def replay(pages, lengths, queries, causal, window, group, heads, d):
@@ -277,3 +278,21 @@ def test_tensors_with_tangents_are_refused(monkeypatch):
                 pool.attend(plan, dq)
             assert lib.launched == launched
     assert launched == 4
+
+
+def test_writes_in_place_are_seen_by_autograd(monkeypatch):
+    no_launch(monkeypatch)
+    pool = cpu_pool()
+    slots, plan, rotation, q, k, v = host_step(pool)
+    into = torch.empty_like(q)
+    for out in (q, into):
+        check_written_tensors_are_seen(lambda: pool.append(slots, k, v, rotation=rotation, query=q, out=out), out)
+        check_written_tensors_are_seen(lambda: pool.attend(plan, q, out=out), out)
+    versions = [x._version for x in (q, k, v)]
+    pool.append(slots, k, v, rotation=rotation, query=q)
+    pool.attend(plan, q)
+    assert [x._version for x in (q, k, v)] == versions
+    with torch.inference_mode():
+        q = q.clone()
+        pool.append(slots, k, v, rotation=rotation, query=q, out=q)
+        pool.attend(plan, q, out=q)

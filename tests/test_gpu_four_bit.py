@@ -9,6 +9,7 @@ from nexusquant_amd import FourBitPagePool, plan_rotation, rotate
 from nexusquant_amd.rope import inv_freq
 from nexusquant_amd.rotary import frequency_axes
 from oracle import four_bit as ref
+from test_rotary_host import check_written_tensors_are_seen
 
 pytestmark = pytest.mark.gpu
 
@@ -600,3 +601,12 @@ def test_refusals():
         other.attend(step, q[:1])
     with pytest.raises(NotImplementedError):
         pool.attend(step, q[:1].clone().requires_grad_())
+
+
+def test_writes_in_place_are_seen_by_autograd():
+    pool = FourBitPagePool(4, 2, 16, 128)
+    t = pool.allocate(2)
+    slots, plan, rotation = pool.plan_slots(pool.slots(t, 18, 20)), pool.plan_attention([t], [20], [2]), plan_rotation([18, 19], 128)
+    q, k, v = (torch.randn(2, h, 128, device="cuda").half() for h in (4, 2, 2))
+    check_written_tensors_are_seen(lambda: pool.append(slots, k, v, rotation=rotation, query=q, out=q), q)
+    check_written_tensors_are_seen(lambda: pool.attend(plan, q, out=q), q)

@@ -10,7 +10,7 @@ from nexusquant_amd import plan_rotation, rotate
 from nexusquant_amd.rope import inv_freq
 from nexusquant_amd.rotary import frequency_axes
 from oracle import four_bit as ref
-from test_rotary_host import check_forward_mode, check_gradients_of_those_that_need_one
+from test_rotary_host import check_forward_mode, check_gradients_of_those_that_need_one, check_written_tensors_are_seen
 
 pytestmark = pytest.mark.gpu
 
@@ -245,3 +245,10 @@ def test_gradients_of_those_that_need_one():
 
 def test_forward_mode():
     check_forward_mode(plan_rotation(torch.arange(5, device="cuda"), 64))
+
+
+def test_writes_in_place_are_seen_by_autograd():
+    r = plan_rotation(torch.arange(5, device="cuda"), 64)
+    qkv = torch.randn(5, 8, 64, device="cuda")
+    q, k = qkv[:, :4], qkv[:, 4:6]
+    check_written_tensors_are_seen(lambda: rotate(q, k, r, out=(q, k)), q, k, qkv)

@@ -199,3 +199,35 @@ def check_forward_mode(r):
 
 def test_forward_mode(monkeypatch):
     check_forward_mode(host_rotation(monkeypatch)[0])
+
+
+def saved_by_a_graph(x):
+    """The output of a graph that has saved x."""
+    return (torch.ones_like(x, requires_grad=True) * x).sum()
+
+
+def check_written_tensors_are_seen(write, *outs):
+    """A graph that has saved what `write` writes into raises in its backward pass."""
+    graphs, before = [saved_by_a_graph(x) for x in outs], [x._version for x in outs]
+    write()
+    for y, x, version in zip(graphs, outs, before):
+        assert x._version > version
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+
+
+def test_writes_in_place_are_seen_by_autograd(monkeypatch):
+    r, _ = host_rotation(monkeypatch)
+    qkv = torch.randn(5, 8, 64)
+    q, k = qkv[:, :4], qkv[:, 4:6]
+    into = torch.empty(5, 4, 64), torch.empty(5, 2, 64)
+    check_written_tensors_are_seen(lambda: rotary.rotate(q, k, r, out=(q, k)), q, k, qkv)
+    check_written_tensors_are_seen(lambda: rotary.rotate(q, k, r, out=into), *into)
+    check_written_tensors_are_seen(lambda: rotary.rotate(q, None, r, out=(q, None)), q)
+    version = qkv._version
+    rotary.rotate(q, k, r)
+    assert qkv._version == version
+    with torch.inference_mode():  # such tensors have no versions
+        q, k = torch.randn(5, 4, 64), torch.randn(5, 2, 64)
+        rotary.rotate(q, k, r, out=(q, k))
+    rotary.rotate(q, k, r, out=(q, k))
