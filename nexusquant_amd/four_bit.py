@@ -381,7 +381,9 @@ class FourBitPagePool(PagePool):
                 raise ValueError(f"key, value and query must share an fp16 or bf16 dtype, got {t.dtype}")
             if grad and t.requires_grad:
                 raise NotImplementedError("append has no backward pass; call it under torch.no_grad()")
-        if has_tangent(key, value, query):
+        if out is not None and grad and out.requires_grad:
+            raise NotImplementedError("append into a tensor that requires grad has no backward pass; call it under torch.no_grad()")
+        if has_tangent(key, value, query, out):
             raise NotImplementedError("append has no derivative in forward mode; call it on tensors without tangents")
         if rotation is None:
             if query is not None:
@@ -486,9 +488,9 @@ class FourBitPagePool(PagePool):
             raise ValueError(f"query must be ({plan.rows} rows or more, num_heads, {self.head_dim}), got {tuple(shape)}")
         if dtype not in _DTYPES:
             raise ValueError(f"attend takes fp16 or bf16 queries, got {dtype}")
-        if query.requires_grad and torch.is_grad_enabled():
+        if (query.requires_grad or out is not None and out.requires_grad) and torch.is_grad_enabled():
             raise NotImplementedError("attend has no backward pass; call it under torch.no_grad()")
-        if has_tangent(query):
+        if has_tangent(query, out):
             raise NotImplementedError("attend has no derivative in forward mode; call it on a query without a tangent")
         scale = self.head_dim ** -0.5 if scale is None else float(scale)
         if not 0.0 < scale < 1e30:

@@ -296,3 +296,19 @@ def test_writes_in_place_are_seen_by_autograd(monkeypatch):
         q = q.clone()
         pool.append(slots, k, v, rotation=rotation, query=q, out=q)
         pool.attend(plan, q, out=q)
+
+
+def test_outputs_that_require_grad_or_have_tangents_are_refused(monkeypatch):
+    from torch.autograd import forward_ad
+    lib, pool = no_launch(monkeypatch), cpu_pool()
+    slots, plan, rotation, q, k, v = host_step(pool)
+    with forward_ad.dual_level():
+        for out in (torch.empty_like(q).requires_grad_(), forward_ad.make_dual(torch.empty_like(q), torch.ones_like(q))):
+            with pytest.raises(NotImplementedError):
+                pool.append(slots, k, v, rotation=rotation, query=q, out=out)
+            with pytest.raises(NotImplementedError):
+                pool.attend(plan, q, out=out)
+    assert lib.launched == 0
+    with torch.no_grad():
+        out = torch.empty_like(q).requires_grad_()
+        assert pool.append(slots, k, v, rotation=rotation, query=q, out=out) is out and pool.attend(plan, q, out=out) is out
