@@ -22,6 +22,10 @@ struct FourBitRows {
     uint16_t* scales[2];  // fp16
 };
 
+// A pool of 4 bits a coordinate has no positions; one that has them holds 8 bits, whatever `reserved` (which the entry points
+// of such pools never read) is.
+inline bool four_bit(const nq_pool* p) { return p->reserved == 4 && p->positions == nullptr; }
+
 int check_fourbit_pool(const nq_pool* p, int32_t layer, const char* who);
 FourBitRows fourbit_rows(const nq_pool* p, int32_t layer);
 

@@ -6,7 +6,7 @@
 // [heads, tokens] of keys and values, and int32 positions [tokens] per page for all
 // layers.  Nothing is computed: every operator is bytes read once and written once,
 // so HBM's copy rate bounds the large ones and the launch the small ones.
-#include "nq_common.h"
+#include "nq_fourbit.h"
 
 #include <stdlib.h>
 
@@ -232,7 +232,6 @@ static void launch_copy(dim3 grid, hipStream_t s, const CopyArgs& a, uint32_t la
 }
 
 // A row's bytes of codes: a pool of 4 bits a coordinate has half of them, and no positions.
-static bool four_bit(const nq_pool* p) { return p->reserved == 4; }
 static uint32_t row_bytes(const nq_pool* p) { return (uint32_t)(four_bit(p) ? p->head_dim / 2 : p->head_dim); }
 
 static int check_pool(const nq_pool* p, const char* who) {

@@ -410,7 +410,7 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
 
 int check_fourbit_pool(const nq_pool* p, int32_t layer, const char* who) {
     NQ_CHECK_ARG(p != nullptr, "%s: pool is NULL", who);
-    NQ_CHECK_ARG(p->reserved == 4, "%s: the pool holds 8 bits a coordinate", who);
+    NQ_CHECK_ARG(four_bit(p), "%s: the pool holds 8 bits a coordinate", who);
     NQ_CHECK_ARG(p->head_dim == 64 || p->head_dim == 128 || p->head_dim == 256, "%s: head_dim %d unsupported (64, 128, 256)", who, p->head_dim);
     NQ_CHECK_ARG(p->layers > 0 && p->pages > 0 && p->heads > 0 && p->tokens > 0 && layer >= 0 && layer < p->layers,
                  "%s: bad pool geometry, or layer %d of %d", who, layer, p->layers);

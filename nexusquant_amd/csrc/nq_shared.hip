@@ -24,6 +24,7 @@
 // tokens 34.2, 3.3e-4 and 34.7, 2.6e-4; 128 x 4096 24.8, 3.3e-4 and 26.1, 2.7e-4; 512 x 32768 107, 3.4e-4 and 129,
 // 2.7e-4.  The other half of what is above 2.1e-4 is the keys'.
 #include "nq_flash.h"
+#include "nq_fourbit.h"
 #include "nq_keymfma.h"
 #include "nq_rowmath.h"
 
@@ -846,7 +847,7 @@ extern "C" int nq_shared_attention(const nq_shared_desc* d, void* stream) {
     using namespace nq;
     NQ_CHECK_ARG(d != nullptr && d->pool != nullptr, "nq_shared_attention: desc and pool are required");
     const nq_pool* p = d->pool;
-    NQ_CHECK_ARG(p->reserved == 0, "nq_shared_attention: a pool of 4 bits a coordinate is read by nq_fourbit_attention");
+    NQ_CHECK_ARG(!four_bit(p), "nq_shared_attention: a pool of 4 bits a coordinate is read by nq_fourbit_attention");
     NQ_CHECK_ARG(p->head_dim == 64 || p->head_dim == 128 || p->head_dim == 256,
                  "nq_shared_attention: head_dim %d unsupported (64, 128, 256)", p->head_dim);
     NQ_CHECK_ARG(p->layers > 0 && p->pages > 0 && p->heads > 0 && p->tokens > 0 && d->layer >= 0 && d->layer < p->layers,

@@ -312,3 +312,21 @@ def test_outputs_that_require_grad_or_have_tangents_are_refused(monkeypatch):
     with torch.no_grad():
         out = torch.empty_like(q).requires_grad_()
         assert pool.append(slots, k, v, rotation=rotation, query=q, out=out) is out and pool.attend(plan, q, out=out) is out
+
+
+@pytest.mark.parametrize("reserved", [4, 8, -1, 1 << 20])
+def test_pools_with_positions_are_taken_whatever_their_reserved_field_holds(reserved):
+    """The field was not read before there were pools of 4 bits, which have no positions."""
+    lib, at = _lib.load(), 4096
+    pool = _lib.Pool(layers=2, pages=4, heads=2, tokens=16, head_dim=128, reserved=reserved, key_codes=at, value_codes=at, key_scales=at,
+                     value_scales=at, positions=at)
+    tokens = _lib.Pool(layers=1, pages=1, heads=2, tokens=3, head_dim=128, reserved=reserved, key_codes=at, value_codes=at, key_scales=at,
+                       value_scales=at, positions=at)
+    desc = _lib.SharedDesc(pool=ctypes.pointer(pool), q_heads=4, query=at, out=at, row_slots=at)
+    assert lib.nq_shared_attention(ctypes.byref(desc), None) == 0
+    pages = np.array([0, 1], np.int32)
+    assert lib.nq_pool_copy_pages(pool, pages.ctypes.data, pages.ctypes.data, 0, None) == 0
+    # as without the field: refused by what comes after it
+    assert lib.nq_pool_write(pool, 0, tokens, None, 0, 3, None) == -1 and b"slots are required" in lib.nq_last_error()
+    assert lib.nq_pool_compact(pool, at, 100, 0, 1, 1, None, 8, 1, None) == -1 and b"kept list" in lib.nq_last_error()
+    assert lib.nq_fourbit_read(pool, 0, at, 0, 0, 1.0, at, at, None) == -1 and b"8 bits" in lib.nq_last_error()
