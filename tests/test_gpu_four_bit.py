@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from nexusquant_amd import FourBitPagePool, plan_rotation, rotate
+from nexusquant_amd import FourBitPagePool, _lib, four_bit, plan_rotation, rotate
 from nexusquant_amd.rope import inv_freq
 from nexusquant_amd.rotary import frequency_axes
 from oracle import four_bit as ref
@@ -610,3 +610,39 @@ def test_writes_in_place_are_seen_by_autograd():
     q, k, v = (torch.randn(2, h, 128, device="cuda").half() for h in (4, 2, 2))
     check_written_tensors_are_seen(lambda: pool.append(slots, k, v, rotation=rotation, query=q, out=q), q)
     check_written_tensors_are_seen(lambda: pool.attend(plan, q, out=q), q)
+
+
+def planned(pool, tables, lens, queries, q_heads, causal=True, window=0):
+    """The plan's items [n, 12] and their kinds (0: many, 1: some, 2: few)."""
+    rows = [int(_lib.load().nq_fourbit_rows(pool.head_dim, k)) for k in range(3)]
+    (items, _), counts = four_bit.attention_items([len(t) for t in tables], lens, queries, causal, window, q_heads // pool.num_heads,
+                                                  pool.num_heads, pool.head_dim, rows)
+    return items.reshape(-1, 12), torch.repeat_interleave(torch.arange(3), torch.tensor(counts[:3]))
+
+
+@pytest.mark.parametrize("d,group,n", [(128, 4, 131072), (64, 8, 131072), (256, 2, 131072), (128, 16, 32768)])
+def test_one_workgroup_over_a_long_sequence_keeps_its_bits(d, group, n):
+    """So many rows that a workgroup has all of a sequence (one table here, for all of them): levels -7 .. 7, whose sums are
+    small beside the sums of what the codes stand in the products as."""
+    seqs = 1024 if d < 256 else 512
+    pool = FourBitPagePool(n // 64 + 3, 1, 64, d)
+    fill(pool, 4)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    low, high = (torch.randint(1, 16, pool.value_codes.shape, device="cuda", generator=g, dtype=torch.uint8) for _ in range(2))
+    pool.value_codes.copy_(low | high << 4)
+    tables = sequences(pool, [n], 9) * seqs
+    items, kinds = planned(pool, tables, [n] * seqs, [1] * seqs, group)
+    assert (kinds == 2).all() and (items[:, 2] == n).all()
+    q = torch.randn(seqs, group, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).half()
+    got = pool.attend(pool.plan_attention(tables, [n] * seqs), q)
+    fields = [x[0].cpu() for x in (pool.key_codes, pool.key_scales, pool.value_codes, pool.value_scales)]
+    kl, ks = ref.sequence(fields[0], fields[1], tables[0], n)
+    vl, vs = ref.sequence(fields[2], fields[3], tables[0], n)
+    mask = torch.ones(1, n, dtype=torch.bool)
+    for row in (0, seqs // 2, seqs - 1):
+        want, _ = ref.attend(q[row:row + 1].cpu(), kl, ks, vl, vs, mask, d ** -0.5)
+        rel = float((got[row:row + 1].cpu().double() - want).norm() / want.norm())
+        # An output's rounding is uniform within half a step, 2^-11 of it at most: a norm of 2^-11 / sqrt(3) at most, and of 512
+        # numbers one that is 1 / sqrt(1024) of that off by chance (four times that: 1.125).  Queries' and weights' roundings, one
+        # in 2^16 and 2^22, are some 3e-5, and add in squares.
+        assert rel <= ((2.0 ** -11 / math.sqrt(3) * 1.125) ** 2 + 3e-5 ** 2) ** 0.5, (row, rel)
