@@ -646,3 +646,93 @@ def test_one_workgroup_over_a_long_sequence_keeps_its_bits(d, group, n):
         # numbers one that is 1 / sqrt(1024) of that off by chance (four times that: 1.125).  Queries' and weights' roundings, one
         # in 2^16 and 2^22, are some 3e-5, and add in squares.
         assert rel <= ((2.0 ** -11 / math.sqrt(3) * 1.125) ** 2 + 3e-5 ** 2) ** 0.5, (row, rel)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,group,d,tokens,lens,queries,causal,window", [
+    (1, 4, 64, 16, [3000], [200], True, 0),
+    (1, 4, 64, 16, [3000, 100], [200, 3], True, 700),      # chunks that some rows see none of
+    (2, 2, 64, 32, [1500, 40, 0], [300, 17, 3], False, 0),
+    (1, 4, 128, 16, [2000], [300], False, 0),
+    (2, 4, 128, 16, [1500, 240], [300, 200], True, 0),
+    (1, 8, 128, 24, [901, 130], [130, 77], True, 333),
+])
+def test_tiles_of_many_rows_over_several_chunks(dtype, heads, group, d, tokens, lens, queries, causal, window):
+    """Eight waves a workgroup, whose sums are joined."""
+    T = TYPES[dtype]
+    pool = FourBitPagePool(sum(-(-n // tokens) for n in lens) + 3, heads, tokens, d)
+    fill(pool, d + len(lens))
+    tables = sequences(pool, lens, 5)
+    items, kinds = planned(pool, tables, lens, queries, heads * group, causal, window)
+    assert (items[kinds == 0, 7] > 1).any()
+    q = torch.randn(sum(queries), heads * group, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(13)).to(T)
+    plan = pool.plan_attention(tables, lens, queries, causal=causal, sliding_window=window or None)
+    check_attention(pool, tables, lens, queries, q, pool.attend(plan, q), T, causal, window)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group,d,lens,queries,causal", [(4, 64, [300, 512], [300, 140], True), (4, 128, [256, 40], [256, 200], False)])
+def test_tiles_of_many_rows_over_one_chunk(dtype, group, d, lens, queries, causal):
+    """Outputs written by the tiles themselves: many kv heads, so that nothing is cut."""
+    T, heads = TYPES[dtype], 64
+    pool = FourBitPagePool(sum(-(-n // 16) for n in lens), heads, 16, d)
+    fill(pool, d)
+    tables = sequences(pool, lens, 5)
+    items, kinds = planned(pool, tables, lens, queries, heads * group, causal)
+    assert (kinds == 0).all() and (items[:, 7] == 0).any()
+    q = torch.randn(sum(queries), heads * group, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(13)).to(T)
+    got = pool.attend(pool.plan_attention(tables, lens, queries, causal=causal), q)
+    for head in (0, 41):  # (its kv head alone against 64 bits)
+        one = FourBitPagePool(pool.num_pages, 1, 16, d)
+        for name in ("key_codes", "value_codes", "key_scales", "value_scales"):
+            getattr(one, name).copy_(getattr(pool, name)[:, :, head:head + 1])
+        part = slice(head * group, (head + 1) * group)
+        check_attention(one, tables, lens, queries, q[:, part], got[:, part], T, causal)
+
+
+@pytest.mark.parametrize("d,group,n,queries", [(64, 2, 50000, 40), (128, 4, 9000, 24), (256, 4, 5000, 21)])
+def test_up_to_96_rows_of_long_sequences_keep_their_bits(d, group, n, queries):
+    """Values' sums near zero, with the tolerance of few rows."""
+    pool = FourBitPagePool(n // 64 + 3, 1, 64, d)
+    fill(pool, 4)
+    tables = sequences(pool, [n], 9)
+    assert (planned(pool, tables, [n], [queries], group)[1] == 2).all()
+    q = torch.randn(queries, group, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).half()
+    got = pool.attend(pool.plan_attention(tables, [n], [queries]), q)
+    check_attention(pool, tables, [n], [queries], q, got, torch.float16, few=True)
+
+
+@pytest.mark.parametrize("d,pages", [
+    (256, (1 << 32) // (8 * 16 * 128)),      # 4 GiB to the byte: offsets of 32 bits up to their last
+    (128, (1 << 32) // (8 * 16 * 64)),
+    (64, (1 << 32) // (8 * 16 * 32)),
+    (128, (1 << 32) // (8 * 16 * 64) + 40),  # and one page and more past it: of 64 bits
+    (64, (1 << 32) // (8 * 16 * 32) + 40),
+])
+def test_few_rows_at_the_end_of_fields_of_4_gib(d, pages):
+    heads, tokens = 8, 16
+    shape = (1, pages, heads, tokens)
+    codes = [torch.zeros(shape + (d // 2,), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    scales = [torch.zeros(shape, dtype=torch.float16, device="cuda") for _ in range(2)]
+    pool = FourBitPagePool.from_tensors(*codes, *scales)
+    pool.allocate(pages)
+    half = pages // 2  # on either side of 2 GiB
+    tables, lens = [[pages - 1, 0, half, pages - 2, half - 1], [half + 1, pages - 3]], [70, 23]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for t in tables:
+        for page in t:
+            for c, s in zip(codes, scales):
+                c[0, page] = torch.randint(0, 256, c.shape[2:], device="cuda", generator=g, dtype=torch.uint8)
+                s[0, page] = torch.rand(s.shape[2:], device="cuda", generator=g) * 0.3 + 0.05
+    for new in ([1, 1], [7, 4]):
+        assert (planned(pool, tables, lens, new, heads * 2)[1] == 2).all()
+        q = torch.randn(sum(new), heads * 2, d, device="cuda", generator=g).half()
+        got = pool.attend(pool.plan_attention(tables, lens, new), q)
+        row = 0
+        for t, n, m in zip(tables, lens, new):
+            at = torch.tensor(t, device="cuda")
+            kl, ks, vl, vs = (x for c, s in zip(codes, scales) for x in ref.sequence(c[0][at].cpu(), s[0][at].cpu(), range(len(t)), n))
+            want, bound = ref.attend(q[row:row + m].cpu(), kl, ks, vl, vs, ref.seen(n, m, True, 0), d ** -0.5)
+            off = (got[row:row + m].cpu().double() - want).abs()
+            assert (off <= bound(2.0 ** -15, 2.0 ** -15) + want.abs() * 2.0 ** -11 + 2.0 ** -25).all()
+            row += m

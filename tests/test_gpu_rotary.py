@@ -252,3 +252,29 @@ def test_writes_in_place_are_seen_by_autograd():
     qkv = torch.randn(5, 8, 64, device="cuda")
     q, k = qkv[:, :4], qkv[:, 4:6]
     check_written_tensors_are_seen(lambda: rotate(q, k, r, out=(q, k)), q, k, qkv)
+
+
+def test_rotations_planned_by_several_threads():
+    """Each with bases of its own, more than the tables that are kept."""
+    import threading
+    positions = torch.arange(50, device="cuda")
+    bases = [[1000.0 + 7 * i + 1000 * t for i in range(40)] for t in range(4)]
+    got = [[] for _ in bases]
+
+    def plan(t):
+        torch.cuda.set_device(positions.device)
+        for base in bases[t]:
+            got[t].append(plan_rotation(positions, 128, base=base).angles)
+
+    threads = [threading.Thread(target=plan, args=(t,)) for t in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for t, many in enumerate(bases):
+        assert len(got[t]) == len(many)
+        for base, angles in zip(many, got[t]):
+            ang = ref.angles(positions[None], inv_freq(128, base), frequency_axes(128, None, False))
+            assert (angles[:, 0].double().cpu() - ang.cos()).abs().max() <= 2.0 ** -24
+            assert (angles[:, 1].double().cpu() - ang.sin()).abs().max() <= 2.0 ** -24
