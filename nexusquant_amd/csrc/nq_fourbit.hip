@@ -93,8 +93,23 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// A scale, or 0 for one that is not finite: what those who see it get of it must not change what others get.
-__device__ __forceinline__ float finite_scale(uint16_t bits) { return (bits & 0x7c00u) == 0x7c00u ? 0.0f : f16_bits_to_f32(bits); }
+// Weights go into their products as fp16 numbers, times the values' scales and 2^lift, lift such that the largest scale that a
+// row has seen is in [64, 128) then: with weights of 2^kSlack at most that is below 2^15, and what counts keeps its bits.  It is
+// a row's own.  Scales that all of a workgroup's rows see lower it for all of them at once, as they come to LDS; others in the
+// tiles that hide tokens, for those who see them: a token's scale changes nothing for a row before it.  (With one for all
+// rows, a hidden token's scale 2^24 times the others' left an output 8e-3 from 64 bits, 2^28 times 0.1; 2.1e-4 and 2.6e-4 now.)
+// One that is not finite lowers nothing.
+constexpr float kMostLift = 31.0f;
+__device__ __forceinline__ float scale_size(uint16_t bits) { return (bits & 0x7c00u) == 0x7c00u ? 0.0f : f16_bits_to_f32(bits & 0x7fffu); }
+__device__ __forceinline__ float scale_size(float scale) {
+    const float x = __builtin_fabsf(scale);
+    return x <= 65504.0f ? x : 0.0f;
+}
+__device__ __forceinline__ float lift_of(float big) {
+    int e = -24;
+    if (big > 0.0f) (void)__builtin_frexpf(big, &e);
+    return (float)(7 - e);
+}
 
 // ----------------------------------------------------------------------- queries ----
 
@@ -319,6 +334,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
             vcode[i][VW - 1] = w.y;
         }
     };
+    // What every row sees are the chunk's tokens [whole0, whole1].
+    int whole0, whole1;
+    {
+        int unused;
+        seen_by(a, it, div((uint32_t)it.r0, a.by_group), unused, whole1);
+        seen_by(a, it, div((uint32_t)(it.r0 + it.n_rows - 1), a.by_group), whole0, unused);
+    }
     // A section's places, two a thread: pages, then rows and scales, then LDS, each asked for before it is needed.
     constexpr int PER = F::SECTION / NT;
     uint32_t page[PER], off[PER], row[PER];
@@ -335,7 +357,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
             vs[i] = a.pool.scales[1][row[i]];
         }
     };
-    auto write = [&](int place) {
+    auto write = [&](int section, int place) {
         float big = 0.0f;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
@@ -343,7 +365,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
             lds.row[place][at] = row[i];
             lds.ks[place][at] = f16_bits_to_f32(ks[i]);
             lds.vs[place][at] = f16_bits_to_f32(vs[i]);
-            big = __builtin_fmaxf(big, finite_scale(vs[i]));
+            const int t = F::SECTION * section + at;
+            big = __builtin_fmaxf(big, t >= whole0 && t <= whole1 ? scale_size(vs[i]) : 0.0f);
         }
 #pragma unroll
         for (int o = 32; o >= 1; o >>= 1) big = __builtin_fmaxf(big, __shfl_xor(big, o, 64));
@@ -359,7 +382,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
         for (int t = 0; t < 2; ++t) load_keys(t, row_in(first_page[t], first_off[t]));
     }
     few_queries<D, QDT>(a, it, kh, lds, lane, wave);
-    write(0);
+    write(0, 0);
     look_up(1);
     const RowAt my = row_at(a, (uint32_t)(it.r0 + min(n16, it.n_rows - 1)), kh);
     int lo, hi;
@@ -386,9 +409,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
     f32x4 o[TILES], wsum = {};
 #pragma unroll
     for (int j = 0; j < TILES; ++j) o[j] = f32x4{};
-    // m: c * (lagging) maximum - lift.  The values' scales go with the weights: times 2^lift the largest so far is in
-    // [64, 128), so weights (2^kSlack at most) stay below 2^15.  The power of two is in the sum of weights as well.
-    float m = kNoMax, l = 0.0f, lift = 31.0f;
+    // m: c * (lagging) maximum - lift.  The power of two is in the sum of weights as well.
+    float m = kNoMax, l = 0.0f, lift = kMostLift;
     Bytes bytes;
     Pairs pairs;
     bytes.init();
@@ -401,18 +423,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
 #pragma unroll
         for (int j = 0; j < TILES; ++j) o[j] *= f;
     };
-    auto lower = [&](int place) {  // a section's scales may be larger than those before
-        float big = lds.max[place][0];
-#pragma unroll
-        for (int w = 1; w < NW; ++w) big = __builtin_fmaxf(big, lds.max[place][w]);
-        int e = -24;
-        if (big > 0.0f) (void)__builtin_frexpf(big, &e);
-        const float to = __builtin_fminf(lift, (float)(7 - e));
-        if (to < lift) {
+    auto lower = [&](float big) {  // scales that come may be larger than those before
+        const float to = __builtin_fminf(lift, lift_of(big));
+        if (__any(to < lift)) {
             rescale(__builtin_amdgcn_exp2f(to - lift));
             m += lift - to;
             lift = to;
         }
+    };
+    auto section_max = [&](int place) {
+        float big = lds.max[place][0];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) big = __builtin_fmaxf(big, lds.max[place][w]);
+        return big;
     };
     // The 24 too much of each code, taken off once a section: sums of codes as they stand are up to 24 times the sum of weights,
     // and what their additions round off is of that size, however near to zero the values' sum is.  Taken off at the end
@@ -426,13 +449,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
         wsum = f32x4{};
     };
     int place = 0, next_place = 1;  // of this section and the next
-    lower(0);
+    lower(section_max(0));
     auto unit = [&](int u, auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
         const int in = u % F::UNITS, first = 32 * in;  // within the section; its last unit of this wave is UNITS - NW + wave
         const bool last = in >= F::UNITS - NW;
         const int ahead = u + NW < n_units ? (last ? 32 * wave : first + 32 * NW) : first;
         const uint32_t* const next = lds.row[last && u + NW < n_units ? next_place : place] + ahead;
+        if (MASKED && (32 * u < whole0 || min(32 * u + 31, it.n_tok - 1) > whole1)) {
+            float big = 0.0f;
+#pragma unroll 1
+            for (int t = 0; t < 2; ++t) {
+                const int at = 32 * u + 16 * t + 4 * kg;
+                const f32x4 scale = *reinterpret_cast<const f32x4*>(lds.vs[place] + first + 16 * t + 4 * kg);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) big = __builtin_fmaxf(big, at + i >= lo && at + i <= hi ? scale_size(scale[i]) : 0.0f);
+            }
+            lower(four_max(big));
+            __builtin_amdgcn_sched_barrier(0);
+        }
         // ---- logits of 16 tokens twice ----
         float p[8], mx = -__builtin_inff();
 #pragma unroll
@@ -457,6 +492,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t) load_keys(t, next[16 * t + n16]);
+        if constexpr (FAR) __builtin_amdgcn_sched_barrier(0);  // (registers)
         // ---- weights ----
         mx *= c;
         if (__any(mx > m + lift + kSlack)) {
@@ -506,27 +542,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
             fold();
             place = next_place;
             next_place = next_place == 2 ? 0 : next_place + 1;
-            lower(place);
+            lower(section_max(place));
         }
     };
     // In the middle of a section that another one follows (so that every wave has all its units of it): the next one to LDS.
     auto middle = [&](int u) {
         const int section = u / F::UNITS;
         if (u % F::UNITS / NW != F::UNITS / NW / 2 || section + 1 >= n_sections) return;
-        write(next_place);
+        write(section + 1, next_place);
         load_scales();
         look_up(section + 3);
         __syncthreads();
     };
-    // Units that every row sees whole are [u0, u1).
-    int u0, u1;
-    {
-        int a0, a1, b0, b1;
-        seen_by(a, it, div((uint32_t)it.r0, a.by_group), a0, a1);
-        seen_by(a, it, div((uint32_t)(it.r0 + it.n_rows - 1), a.by_group), b0, b1);
-        u0 = (b0 + 31) / 32;
-        u1 = (a1 + 1) / 32;
-    }
+    const int u0 = (whole0 + 31) / 32, u1 = (whole1 + 1) / 32;  // units that every row sees whole: [u0, u1)
     int u = wave;
 #pragma unroll 1
     for (; u < min(u0, n_units); u += NW) {
@@ -710,7 +738,7 @@ wide_kernel(FourBitArgs a) {
     static_assert(W::LOOKUPS == 1 || W::PER == 2 * W::LOOKUPS, "keys' and values' pieces of a thread are of the same rows");
     __shared__ __align__(16) char s_kv[W::LDS];
     __shared__ __align__(16) float s_k[2][kWideStage], s_v[2][kWideStage];
-    __shared__ int s_exp[2];
+    __shared__ float s_lift[2];
     __shared__ float s_m[NW / 2][32], s_l[NW / 2][32];
 
     const int lane = threadIdx.x & 63, n = lane & 31, g = lane >> 5;
@@ -755,9 +783,6 @@ wide_kernel(FourBitArgs a) {
     Pairs pairs;
     bytes.init();
     pairs.init();
-    // The values' scales times 2^(7 - e), e the exponent of the largest so far: weights (2^kSlack at most) stay below 2^15.
-    // e grows seldom; the sums are then rescaled.
-    int vexp = -40;
     auto store = [&](int buf) {
         char* const kv = s_kv + buf * W::BUF;
 #pragma unroll
@@ -791,17 +816,12 @@ wide_kernel(FourBitArgs a) {
             }
         }
         if (wave == 0) {
-            float big = finite_scale(vs);
+            float big = scale_size(vs);
 #pragma unroll
             for (int o = 32; o >= 1; o >>= 1) big = __builtin_fmaxf(big, __shfl_xor(big, o, 64));
-            if (big > 0.0f) {
-                int e;
-                (void)__builtin_frexpf(big, &e);
-                vexp = max(vexp, e);
-            }
             s_k[buf][lane] = f16_bits_to_f32(ks);
-            s_v[buf][lane] = __builtin_ldexpf(f16_bits_to_f32(vs), 7 - vexp);
-            if (lane == 0) s_exp[buf] = vexp;
+            s_v[buf][lane] = f16_bits_to_f32(vs);
+            if (lane == 0) s_lift[buf] = lift_of(big);
         }
     };
     look_up(0);
@@ -863,7 +883,7 @@ wide_kernel(FourBitArgs a) {
     load();
     look_up(2);
     __syncthreads();
-    int cur = s_exp[0];
+    float lift = kMostLift;  // rows.m: c * (lagging) maximum - lift; the power of two is in the sum of weights as well
 
     auto logits = [&](const char* kbuf, const float* scales) {
         i32x16 sh = {}, sl = {};
@@ -896,11 +916,48 @@ wide_kernel(FourBitArgs a) {
             }
         }
     };
+    auto lower = [&](float most) {
+        const float to = __builtin_fminf(lift, most);
+        if (__any(to < lift)) {
+            const float f = __builtin_amdgcn_exp2f(to - lift);
+            rows.m += lift - to;
+            lift = to;
+            rows.l *= f;
+#pragma unroll
+            for (int b = 0; b < T::DB; ++b) rows.o[b] *= f;
+        }
+    };
+    // Where a stage has scales larger than those before, lift follows for all rows at once, and in a stage that hides tokens
+    // from some by what a row sees of it.
+    float top = kMostLift;  // no row's lift is more
+    auto larger = [&](int buf, float& most) {
+        most = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, s_lift[buf])));
+        return most < top;
+    };
     auto begin = [&](int buf) {
-        const int e = s_exp[buf];
-        if (e != cur) {
-            const float f = __builtin_ldexpf(1.0f, cur - e);
-            cur = e;
+        float most;
+        if (__builtin_expect(larger(buf, most), 0)) {
+            top = most;
+            lower(most);
+        }
+    };
+    auto begin_masked = [&](int buf, int first) {
+        float most, big = 0.0f;
+        if (__builtin_expect(!live || !larger(buf, most), 1)) return;
+#pragma unroll 1
+        for (int i = 32 * tile0 + 4 * g; i < 32 * (tile0 + tiles); i += 8) {
+            const f32x4 f = *reinterpret_cast<const f32x4*>(s_v[buf] + i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) big = __builtin_fmaxf(big, first + i + k >= lo && first + i + k <= hi ? scale_size(f[k]) : 0.0f);
+        }
+        lower(lift_of(both_max(big)));
+    };
+    auto raise = [&](float mx) {
+        mx = both_max(mx) * c;
+        if (__any(mx > rows.m + lift + kSlack)) {
+            const float to = __builtin_fmaxf(rows.m, mx - lift), f = __builtin_amdgcn_exp2f(rows.m - to);
+            rows.m = to;
+            rows.l *= f;
 #pragma unroll
             for (int b = 0; b < T::DB; ++b) rows.o[b] *= f;
         }
@@ -911,7 +968,7 @@ wide_kernel(FourBitArgs a) {
         float mx = s[0];
 #pragma unroll
         for (int j = 1; j < 16; ++j) mx = __builtin_fmaxf(mx, s[j]);
-        rows.template raise<true>(mx, c);
+        raise(mx);
         uint32_t p[8];
         rows.template weights<true>(s, c, p, sv + 32 * t, g);
         add_values(p, kv + W::KEYS + 32 * ROWB * t);
@@ -936,7 +993,7 @@ wide_kernel(FourBitArgs a) {
                 s[j] = key >= from && key <= to ? s[j] : -__builtin_inff();
                 mx = __builtin_fmaxf(mx, s[j]);
             }
-            rows.template raise<true>(mx, c);
+            raise(mx);
             uint32_t p[8];
             float sum = 0.0f;
 #pragma unroll
@@ -977,7 +1034,7 @@ wide_kernel(FourBitArgs a) {
     int at = 0;
 #pragma unroll 1
     for (; at < it0; ++at) {
-        begin(at & 1);
+        begin_masked(at & 1, kWideStage * at);
         masked(at & 1, kWideStage * at);
         end(at);
     }
@@ -1008,7 +1065,7 @@ wide_kernel(FourBitArgs a) {
     }
 #pragma unroll 1
     for (; at < n_stages; ++at) {
-        begin(at & 1);
+        begin_masked(at & 1, kWideStage * at);
         masked(at & 1, kWideStage * at);
         end(at);
     }
@@ -1049,7 +1106,6 @@ wide_kernel(FourBitArgs a) {
                 for (int k = 0; k < 4; ++k) rows.o[b][4 * i + k] = __builtin_fmaf(y[k], fo, rows.o[b][4 * i + k] * f);
             }
     }
-    const float unscale = __builtin_ldexpf(1.0f, cur - 7);
     // lane (n, g), register 4 i + k of block b: coordinate 32 b + 8 i + 4 g + k
     if (it.slots == 0) {  // the row's only chunk: transformed and rounded here
         float y[16 * T::DB];
@@ -1058,7 +1114,7 @@ wide_kernel(FourBitArgs a) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) y[16 * b + j] = rows.o[b][j];
         butterflies(y);
-        const float sign = g2 ? -1.0f : 1.0f, f = l == 0.0f ? 0.0f : a.hscale * unscale / l;
+        const float sign = g2 ? -1.0f : 1.0f, f = l == 0.0f ? 0.0f : a.hscale / l;
 #pragma unroll
         for (int i = 0; i < 16 * T::DB; ++i) {
             const f32x2 h = halves(y[i]);
@@ -1083,8 +1139,8 @@ wide_kernel(FourBitArgs a) {
     for (int b = 0; b < T::DB; ++b)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<f32x4*>(to + 32 * b + 8 * i) = f32x4{rows.o[b][4 * i] * unscale, rows.o[b][4 * i + 1] * unscale,
-                                                                   rows.o[b][4 * i + 2] * unscale, rows.o[b][4 * i + 3] * unscale};
+            *reinterpret_cast<f32x4*>(to + 32 * b + 8 * i) =
+                f32x4{rows.o[b][4 * i], rows.o[b][4 * i + 1], rows.o[b][4 * i + 2], rows.o[b][4 * i + 3]};
 }
 
 // Waves of a workgroup of many rows: at head_dim 256 registers leave one wave a SIMD.

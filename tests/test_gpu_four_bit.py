@@ -736,3 +736,35 @@ def test_few_rows_at_the_end_of_fields_of_4_gib(d, pages):
             off = (got[row:row + m].cpu().double() - want).abs()
             assert (off <= bound(2.0 ** -15, 2.0 ** -15) + want.abs() * 2.0 ** -11 + 2.0 ** -25).all()
             row += m
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("queries,window,at", [(4, 0, 159), (40, 0, 159), (150, 0, 159), (150, 0, 100), (4, 20, 159), (4, 20, 137),
+                                               (40, 20, 159), (40, 20, 101), (150, 20, 159), (150, 20, 60)])
+def test_a_large_scale_takes_no_bits_from_rows_that_do_not_see_it(d, queries, window, at):
+    """fp16's largest scale at one token beside others of some 2^-12: later tokens, and tokens before a window."""
+    n = 160
+    pool = FourBitPagePool(12, 2, 16, d)
+    fill(pool, 2)
+    pool.value_scales.mul_(2.0 ** -10)
+    tables = sequences(pool, [n], 1)
+    q = torch.randn(queries, 8, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).half()
+    pool.value_scales[0, tables[0][at // 16], 1, at % 16] = 65504.0
+    got = pool.attend(pool.plan_attention(tables, [n], [queries], sliding_window=window or None), q).cpu().double()
+    kl, ks = ref.sequence(pool.key_codes[0].cpu(), pool.key_scales[0].cpu(), tables[0], n)
+    vl, vs = ref.sequence(pool.value_codes[0].cpu(), pool.value_scales[0].cpu(), tables[0], n)
+    mask = ref.seen(n, queries, True, window)
+    want, bound = ref.attend(q.cpu(), kl, ks, vl, vs, mask, d ** -0.5)
+    few = 4 * queries <= 96
+    # (rounded to fp16 below its smallest normal number, which values of 2^-12 come near to: 2^-25)
+    lim = bound(step(few), step(few)) + want.abs() * 2.0 ** -11 + 2.0 ** -25
+    # An output of 65504 p |n - 8| sqrt(d) at most: numbers of 65520, half a step past fp16's largest, and more are infinite.
+    finite = want.abs() + lim < 65520.0
+    assert ((got - want).abs() <= lim)[finite].all()
+    infinite = want.abs() - lim >= 65520.0
+    assert (got == torch.sign(want) * math.inf)[infinite].all()
+    rows = ~mask[:, at]
+    assert rows.any() and not rows.all()
+    off, size = (got - want)[rows], want[rows]
+    below = 2.0 ** -25 * off.numel() ** 0.5
+    assert off.norm() <= size.norm() * (2.0 ** -11 + (0.0 if few else 3 * 2.0 ** -11)) + below, float(off.norm() / size.norm())
