@@ -100,8 +100,10 @@ def plan_rotation(positions, head_dim: int, base: float = 10000.0, rope_scaling:
         dev = torch.device("cuda" if device is None else device)
         if dev.type != "cuda":
             raise _lib.NexusQuantError(f"nexusquant_amd runs on MI355X (ROCm) devices only; the rotation is for {dev}")
-        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("positions on the host cannot be copied to the device in a graph: copy them before capturing")
+        if torch.cuda.is_initialized():
+            with on_device(dev):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("positions on the host cannot be copied to the device in a graph: copy them before capturing")
         positions = positions.to(dev)
     elif device is not None and torch.device(device) != positions.device and torch.device(device) != torch.device("cuda"):
         raise ValueError(f"positions are on {positions.device}, not on {device}")

@@ -231,3 +231,21 @@ def test_writes_in_place_are_seen_by_autograd(monkeypatch):
         q, k = torch.randn(5, 4, 64), torch.randn(5, 2, 64)
         rotary.rotate(q, k, r, out=(q, k))
     rotary.rotate(q, k, r, out=(q, k))
+
+
+def test_a_capture_is_looked_for_on_the_rotation_s_device(monkeypatch):
+    """Which need not be the current one."""
+    import contextlib
+    current = [torch.device("cuda", 0)]
+
+    @contextlib.contextmanager
+    def on_device(dev):
+        current.append(dev)
+        yield
+        current.pop()
+
+    monkeypatch.setattr(rotary, "on_device", on_device)
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: current[-1].index == 1)
+    with pytest.raises(RuntimeError, match="before capturing"):
+        rotary.plan_rotation([1, 2], 64, device="cuda:1")
