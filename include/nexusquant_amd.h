@@ -618,7 +618,7 @@ int nq_prompt_attention(const nq_prompt_desc* desc, void* stream);
  */
 typedef struct nq_pool {
     int32_t layers, pages, heads, tokens, head_dim; /* head_dim 64, 128 or 256 */
-    int32_t reserved;     /* 0; 4: a pool of 4 bits a coordinate, see nq_fourbit_append */
+    int32_t reserved;     /* 4, with positions NULL: a pool of 4 bits a coordinate, see nq_fourbit_append; else not read */
     int8_t* key_codes;    /* [layers, pages, heads, tokens, head_dim] */
     int8_t* value_codes;
     void* key_scales;     /* fp16 [layers, pages, heads, tokens] */

@@ -30,11 +30,12 @@ int check_fourbit_pool(const nq_pool* p, int32_t layer, const char* who);
 FourBitRows fourbit_rows(const nq_pool* p, int32_t layer);
 
 // Nibbles of a word in pairs (j, j + 4), j = 0 .. 3, as fp16 values 16 + n: the nibble under the exponent of 16.
+constexpr uint32_t kNibbleMask = 0x03C003C0u, kSixteens = 0x4C004C00u;
 template <int J>
-__device__ __forceinline__ uint32_t nibble_pair(uint32_t w) {
+__device__ __forceinline__ uint32_t nibble_pair(uint32_t w, uint32_t mask = kNibbleMask, uint32_t sixteens = kSixteens) {
     constexpr int at = 6 - 4 * J;  // where the nibble goes, from where it is
     const uint32_t x = at >= 0 ? w << (at >= 0 ? at : 0) : w >> (at < 0 ? -at : 0);
-    return (x & 0x03C003C0u) | 0x4C004C00u;
+    return (x & mask) | sixteens;
 }
 constexpr float kNibbleBias = 24.0f;  // (16 + n) - kNibbleBias = n - 8
 

@@ -44,15 +44,15 @@ struct Item {
     const int32_t* pages;
     int tok0, n_tok, q_row0, r0, n_rows, slot0, slots, last;
 };
-__device__ __forceinline__ Item item_of(const FourBitArgs& a, uint32_t i, int most_rows, int most_tokens) {
+__device__ __forceinline__ Item item_of(const FourBitArgs& a, uint32_t i, int most_rows) {
     const int32_t* const it = a.items + (size_t)kItemInts * i;
     Item x;
     x.pages = a.pages + it[0];
     x.tok0 = it[1];
-    x.n_tok = min(max(it[2], 1), most_tokens);  // what LDS is sized for, whatever a plan from elsewhere holds
+    x.n_tok = max(it[2], 1);
     x.q_row0 = it[3];
     x.r0 = it[4];
-    x.n_rows = min(max(it[5], 1), most_rows);
+    x.n_rows = min(max(it[5], 1), most_rows);  // what registers and LDS are for, whatever a plan from elsewhere holds
     x.slot0 = it[6];
     x.slots = it[7];
     x.last = it[8];
@@ -159,19 +159,15 @@ struct Bytes {  // the levels of a word's nibbles as int8, times 16: coordinates
     __device__ __forceinline__ uint32_t odd(uint32_t w) const { return (w & mask) ^ sign; }
 };
 struct Pairs {  // nibbles j and j + 4 of a word as fp16 values 16 + n (nq_fourbit.h)
-    uint32_t mask, sixteen;
+    uint32_t mask, sixteens;
     __device__ __forceinline__ void init() {
-        mask = 0x03C003C0u;
-        sixteen = 0x4C004C00u;
+        mask = kNibbleMask;
+        sixteens = kSixteens;
         asm volatile("" : "+s"(mask));
-        asm volatile("" : "+v"(sixteen));
+        asm volatile("" : "+v"(sixteens));
     }
     template <int J>
-    __device__ __forceinline__ uint32_t get(uint32_t w) const {
-        constexpr int at = 6 - 4 * J;
-        const uint32_t x = at >= 0 ? w << (at >= 0 ? at : 0) : w >> (at < 0 ? -at : 0);
-        return (x & mask) | sixteen;
-    }
+    __device__ __forceinline__ uint32_t get(uint32_t w) const { return nibble_pair<J>(w, mask, sixteens); }
 };
 
 // What a row's logits are multiplied by: above zero (what is not seen is -infinity, times zero a NaN), or NaN.
@@ -209,8 +205,8 @@ __device__ __forceinline__ void butterflies(float (&x)[N]) {
 // middle of this one, behind a barrier there a wave's last unit asks for the next section's first codes, and a wave that is
 // ahead writes the section after that one, which no wave reads yet.
 //
-// Measured (a copy of 2 GiB reads and writes 4.9 TB/s): 64 rows up to 8192 tokens of 8 x 128 (335 MB) 64 us, 5.2 TB/s, and 4.2
-// for the join; one row of 131072 (138 MB) 27 and 5; four rows of 1000 6.2 and 3.3.  Eight waves a workgroup were no faster where
+// Measured (a copy of 2 GiB reads and writes 4.9 TB/s): 64 rows up to 8192 tokens of 8 x 128 (335 MB) 64 us, 5.2 TB/s, and 4.8
+// for the join; one row of 131072 (138 MB) 28 and 5.4; four rows of 1000 6.2 and 3.8.  Eight waves a workgroup were no faster where
 // one takes a whole sequence (24 of up to 1500 tokens) and 5 to 10 % slower in the others.
 template <int D>
 struct FewShape {
@@ -283,8 +279,7 @@ __device__ __forceinline__ void few_queries(const FourBitArgs& a, const Item& it
 }
 
 // FAR: a layer's codes take more than 4 GiB.  Else an offset has 32 bits, and a load one instruction for its address, where three
-// are needed for 64 (ten loads a unit of some 240): one row of 131072 tokens 35.1 to 33.8 us, 16 sequences of 20 rows over 4096
-// 19.5 to 18.5, 64 rows up to 8192 73.9 to 72.3.
+// are needed for 64 (ten loads a unit of some 240): 2 to 5 % less time (64 rows up to 8192 tokens 73.9 and 72.3 us).
 template <int D, int QDT, bool FAR>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>::PER_SIMD))) void few_kernel(FourBitArgs a) {
     using F = FewShape<D>;
@@ -294,7 +289,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
     const int lane = threadIdx.x & 63, n16 = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t item = div(blockIdx.x, a.by_kv), kh = blockIdx.x - item * a.kv_heads;
-    const Item it = item_of(a, item, F::ROWS, 0x7fffffff);
+    const Item it = item_of(a, item, F::ROWS);
     const int n_units = (it.n_tok + 31) / 32, n_sections = (n_units + F::UNITS - 1) / F::UNITS;
 
     // ---- tokens: places past the chunk repeat its last (no row sees them) ----
@@ -706,9 +701,14 @@ __global__ __launch_bounds__(256) void fourbit_join_kernel(FourBitArgs a, uint32
 //
 // Bound by instructions issued: 2048 query tokens x 4 heads over 32768 tokens of 8 x 128 take 1215 us, 872 TFLOP/s where a
 // library product of 8192^3 reaches 1340; a CU issues in 81 % of its cycles, the matrix cores are busy in 40, the vector units
-// in 65, LDS in 34.  With head_dim 64 (851 us) half as much is done for a softmax's
-// weight, with 256 (1024 tokens over 16384, 917 us) a wave a SIMD hides less.  Tried: scaled keys and values in fp16 for exact
+// in 65, LDS in 34, with nearly a cycle of bank conflicts for each of its instructions (which of them was not counted).  With
+// head_dim 64 (850 us) half as much is done for a softmax's weight, with 256 (1024 tokens over 16384, 902 us) a wave a SIMD
+// hides less.  Tried: scaled keys and values in fp16 for exact
 // codes (no faster), two halves of a workgroup in opposite order (11 % slower), waves' priorities (0 to 6 % slower).
+//
+// Weights, times their values' scales, are rounded to fp16 once: with 11 bits an fp16 output is 2.6e-4 from 64 bits where its
+// own rounding is 2.1e-4, and a bf16 output as near as without (1.7e-3).  A second product for the rest, as few rows have it,
+// would be half as many matrix instructions again in a kernel that is bound by issue.
 constexpr int kWideStage = 64;
 
 template <int D, int NW>
@@ -744,7 +744,7 @@ wide_kernel(FourBitArgs a) {
     const int lane = threadIdx.x & 63, n = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t item = div(blockIdx.x, a.by_kv), kh = blockIdx.x - item * a.kv_heads;
-    const Item it = item_of(a, item, W::ROWS, 0x7fffffff);
+    const Item it = item_of(a, item, W::ROWS);
     const int n_stages = (it.n_tok + kWideStage - 1) / kWideStage;
 
     // ---- tokens: places past the chunk repeat its last (no row sees them) ----

@@ -116,8 +116,9 @@ __device__ __forceinline__ void store8(uint8_t* p, const float (&x)[8]) {
 // A wave takes a token's heads h = first, first + step, .., D / 16 lanes a head and eight pairs a lane, 1024 / D heads one after
 // another in memory at a time: the angles stay in registers, and N steps' inputs are read before their outputs are written.
 // 16384 tokens of 32 + 8 heads of 128 (336 MB) with their angles: a wave on eight tokens of one head at a time 83 us, on eight
-// heads of a token 71, with stores past the caches 58, reading ahead 57 (50 and 6.7 for the angles: 6.7 TB/s, the inputs being
-// in the last-level cache still); 8188 tokens in fp32, forward and back (671 MB), 139 to 146, of which it keeps nothing.
+// heads of a token 71, with stores past the caches 58, reading ahead the same (51 and 6 for the angles: 6.6 TB/s, the inputs
+// being in the last-level cache still from the call before; 67 where they are not); 8188 tokens in fp32, forward and back (671
+// MB), 139 to 146, of which it keeps nothing.
 template <int DT, int D, bool STREAM, typename Where>
 __device__ __forceinline__ void rotate_heads(const float* angles, float sign, uint32_t first, uint32_t step, uint32_t heads, int at, Where where) {
     constexpr int SIZE = DT == NQ_F32 ? 4 : 2, N = DT == NQ_F32 ? 2 : 4;
@@ -358,8 +359,8 @@ struct ReadArgs {
     float hscale;
 };
 
-// A quad a row and role; sums of n - 8 are whole numbers of at most 2048, so fp16 holds them exactly, and each coordinate is rounded by its scale and by its type.
-// A quad a row, its keys and values.  10149 tokens of 8 heads of 128 (11 MB to 42 MB) 11 us, 4.8 TB/s.
+// A quad a row, its keys and then its values; sums of n - 8 are whole numbers of at most 2048, so fp16 holds them exactly, and
+// each coordinate is rounded by its scale and by its type.  10149 tokens of 8 heads of 128 (11 MB to 42 MB) 11 us, 4.8 TB/s.
 template <int DT, int D, bool STREAM>
 __device__ __forceinline__ void read_rows(const ReadArgs& a) {
     constexpr int C = D / 32, SIZE = DT == NQ_F32 ? 4 : 2;
@@ -438,7 +439,7 @@ FourBitRows fourbit_rows(const nq_pool* p, int32_t layer) {
         default: hipLaunchKernelGGL((KERNEL<DT, 256>), __VA_ARGS__); break;               \
     }
 
-// Blocks that share a row's heads: one until the launch has fewer than 1024.
+// Waves that share a row's heads: one until the launch has fewer than 1024 workgroups.
 static uint32_t share(uint64_t blocks, uint32_t most) {
     uint32_t n = 1;
     while (n < most && blocks * n < 1024) n *= 2;

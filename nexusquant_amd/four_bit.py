@@ -88,10 +88,12 @@ _MANY, _SOME, _FEW = 0, 1, 2
 # tiles of many 78 (they leave half of the CUs idle); 2048 x 4 rows over 32768 of 8 x 128 1340 and 1204 (what is decoded
 # serves twice the rows).
 _MANY_ROWS = 512
-# Up to so many rows of a sequence are tiles of few, 16 rows each, which end to end take less than one of 128 rows with the rest
-# left idle, and round weights to 22 bits.  us as few and as some: 16 sequences of 4096 tokens of 8 x 128, 20 rows 27.8 and 40.7,
-# 32 29.4 and 44.0, 64 43.8 and 55.6, 96 50.9 and 65.6, 128 68.8 and 73.1; one of 32768, 20 rows 21.4 and 29.8, 96 42.8 and 41.4,
-# 128 49.6 and 44.9; 64 of 8192 of 8 x 64, 96 rows 217 and 261, 128 291 and 268.
+# Up to so many rows of a sequence are tiles of few, 16 rows each: weights keep 22 bits there, where wider tiles round them to 11.
+# Fewer rows also take less time so than as one tile of 128 rows with the rest left idle, more of them at head_dim 64 and 128 do
+# not.  us as few and as some, with no other kind in the plan: 16 sequences of 4096 tokens of 8 x 128, 20 rows 32 and 44, 32 31
+# and 45, 64 51 and 49, 96 64 and 62, 128 81 and 68; one of 32768, 20 rows 20 and 29, 96 42 and 41, 128 48 and 44; 64 of 8192 of
+# 8 x 64, 32 rows 126 and 181, 64 238 and 184, 96 346 and 248; 24 of 1500 of 20 x 64, 20 rows 26 and 40, 48 39 and 42, 96 70 and
+# 56; 8 of 8192 of 8 x 256, 64 rows 81 and 105, 96 126 and 133, 128 134 and 138.
 _FEW_ROWS = 96
 _FEW_STEP = 128  # tokens that a workgroup takes at a time
 _ITEM_INTS = 12
@@ -113,8 +115,10 @@ def _few_chunks(spans: np.ndarray, heads: int, head_dim: int):
     """Chunks of few rows, of the least length with which the launch is so many workgroups.
 
     1024 run at once (at head_dim 256 512); with fewer there is less to join, or nothing, where a chunk has all of a sequence.
-    us with 512, 1024 and 2048: 64 rows up to 8192 tokens of 8 x 128 86, 71, 70; 16 rows up to 30000 64, 61, 63; one row of
-    131072 34, 34, 39; 24 rows up to 1500 of 20 x 64 13.4, 15.8, 17.9; 32 rows up to 8192 of 4 x 256 32, 37, 39."""
+    us with 512, 1024 and 2048: 64 rows up to 8192 tokens of 8 x 128 84, 62, 63; 16 rows up to 30000 62, 61, 61; one row of
+    131072 34, 35, 36; 24 rows up to 1500 of 20 x 64 12.8, 14.8, 17.2; 32 rows up to 8192 of 4 x 256 33, 37, 40.  Around the
+    work from which on 1024 are taken: 8 rows up to 8192 of 8 x 128 (0.6 of it) 18.3, 18.7, 20.0; 32 up to 8192 of 8 x 64 (1.02)
+    28.1, 25.1, 27.3; 16 up to 8192 of 8 x 128 (1.1) 23.0, 24.2, 24.7."""
     work = heads * int(spans.sum()) * head_dim // 128
     workgroups = 1024 if work >= 1024 * 512 and head_dim < 256 else 512
     lo, hi = 1, -(-int(spans.max()) // _FEW_STEP)
@@ -270,7 +274,7 @@ class FourBitPagePool(PagePool):
 
     A vector x is held as t = H x (H the orthonormal Walsh-Hadamard matrix): scale = fp16(max |t| / 7.5), nibble
     n = clamp(floor(t / scale + 8.5), 0, 15), which stands for H ((n - 8) scale): half a scale off at most.  A vector with
-    an infinity or a NaN has a NaN scale; queries that see it get NaN.
+    an infinity or a NaN, or with sums past fp32, has a NaN scale; queries that see it get NaN.
 
     Page numbers, fork, copy_pages, free: as CompressedPagePool.  compact keeps positions (keys are stored rotated)."""
 
@@ -476,8 +480,11 @@ class FourBitPagePool(PagePool):
 
         Returns [rows, q_heads, head_dim].  Rows behind the plan's are left as they are in `out`, and are zero without one;
         `out` may be query.  Codes are exact in the products; a transformed query is rounded to 2^-16 of its largest
-        coordinate, weights to 22 bits where a kv head has up to 96 rows of a sequence and to 11 where it has more.  How a
-        row's tokens are cut follows from the whole plan: outputs of one row alone and in a batch agree to roundings.
+        coordinate, weights to 22 bits where a kv head has up to 96 rows of a sequence (query tokens x query heads), and to 11
+        where it has more, but for up to 16 rows that are left over behind full tiles.  A weight times its value's scale
+        that is below 2^-30 of the largest scale that the row sees is lost.  An fp16 output is then 2.1e-4 from 64 bits, which
+        is its own rounding, or 2.6e-4.  How a row's tokens are cut follows from the whole plan: outputs of one row alone and
+        in a batch agree to roundings.
         A captured graph reads the plan's arrays: keep the plan while it is replayed.  Inference only."""
         self._check_plan(plan, FourBitAttentionPlan, "attend", layer)
         shape, dtype, dev = query.shape, query.dtype, self.device

@@ -216,7 +216,7 @@ def _rotated(query, key, angles: torch.Tensor, inverse: bool):
 
 def has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether forward mode differentiates one of these (outside of its levels 0.06 us; unpack_dual takes 0.4 a tensor)."""
-    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 class _Rotate(torch.autograd.Function):

@@ -249,3 +249,15 @@ def test_a_capture_is_looked_for_on_the_rotation_s_device(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: current[-1].index == 1)
     with pytest.raises(RuntimeError, match="before capturing"):
         rotary.plan_rotation([1, 2], 64, device="cuda:1")
+
+
+def test_function_transforms_are_refused(monkeypatch):
+    """Not passed by: their tensors have no memory that a kernel could read."""
+    r, _ = host_rotation(monkeypatch)
+    q = torch.randn(5, 4, 64)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: rotary.rotate(x, None, r)[0], (q,), (q,))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda x: rotary.rotate(x, None, r)[0].sum())(q)
+    with pytest.raises((RuntimeError, ValueError)):
+        torch.func.vmap(lambda x: rotary.rotate(x, None, r)[0])(q[None])
