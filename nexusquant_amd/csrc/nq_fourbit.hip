@@ -461,7 +461,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
                 for (int i = 0; i < 4; ++i) big = __builtin_fmaxf(big, at + i >= lo && at + i <= hi ? scale_size(scale[i]) : 0.0f);
             }
             lower(four_max(big));
-            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(0);  // (or the logits' registers are taken beside these)
         }
         // ---- logits of 16 tokens twice ----
         float p[8], mx = -__builtin_inff();
@@ -487,7 +487,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FewShape<D>
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t) load_keys(t, next[16 * t + n16]);
-        if constexpr (FAR) __builtin_amdgcn_sched_barrier(0);  // (registers)
+        if constexpr (FAR) __builtin_amdgcn_sched_barrier(0);  // (20 bytes of scratch at head_dim 128 otherwise)
         // ---- weights ----
         mx *= c;
         if (__any(mx > m + lift + kSlack)) {
@@ -703,8 +703,8 @@ __global__ __launch_bounds__(256) void fourbit_join_kernel(FourBitArgs a, uint32
 // library product of 8192^3 reaches 1340; a CU issues in 81 % of its cycles, the matrix cores are busy in 40, the vector units
 // in 65, LDS in 34, with nearly a cycle of bank conflicts for each of its instructions (which of them was not counted).  With
 // head_dim 64 (850 us) half as much is done for a softmax's weight, with 256 (1024 tokens over 16384, 902 us) a wave a SIMD
-// hides less.  Tried: scaled keys and values in fp16 for exact
-// codes (no faster), two halves of a workgroup in opposite order (11 % slower), waves' priorities (0 to 6 % slower).
+// hides less.  Tried: scaled keys and values in fp16 for exact codes (no faster), two halves of a workgroup in opposite order
+// (11 % slower), waves' priorities (0 to 6 % slower).
 //
 // Weights, times their values' scales, are rounded to fp16 once: with 11 bits an fp16 output is 2.6e-4 from 64 bits where its
 // own rounding is 2.1e-4, and a bf16 output as near as without (1.7e-3).  A second product for the rest, as few rows have it,
